@@ -8,6 +8,7 @@
 #include "../../include/duck_b200.h"
 #include "aux_kernels.cuh"
 #include "bam_kernels.cuh"
+#include "capi.hpp"
 #include "ppo_kernels.cuh"
 
 #include <cstdlib>
@@ -21,17 +22,6 @@
 using namespace duckb200;
 
 namespace {
-thread_local std::string lastError;
-
-struct CudaError : std::runtime_error {
-  using std::runtime_error::runtime_error;
-};
-void check(cudaError_t e, const char *what) {
-  if (e != cudaSuccess) throw CudaError(std::string(what) + ": " + cudaGetErrorString(e));
-}
-void require(bool c, const char *msg) {
-  if (!c) throw std::invalid_argument(msg);
-}
 // Lanes per environment: the smallest power of two (>= 4) holding the largest
 // colour class, unless DUCK_B200_LANES (4, 8, 16 or 32) asks for a wider team.
 int teamSize(int colorMax) {
@@ -174,22 +164,6 @@ template <class R> duck_batch *create(const ParsedModel &parsed, int n, double d
   check(cudaEventCreateWithFlags(&b->ready, cudaEventDisableTiming), "cudaEventCreate");
   check(cudaEventRecord(b->ready, s), "cudaEventRecord");
   return b.release();
-}
-
-template <class F> int guarded(F &&f) {
-  try {
-    f();
-    return DUCK_OK;
-  } catch (const std::invalid_argument &e) {
-    lastError = e.what();
-    return DUCK_EINVAL;
-  } catch (const CudaError &e) {
-    lastError = e.what();
-    return DUCK_ECUDA;
-  } catch (const std::exception &e) {
-    lastError = e.what();
-    return DUCK_EMODEL;
-  }
 }
 
 }  // namespace

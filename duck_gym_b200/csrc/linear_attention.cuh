@@ -1,0 +1,153 @@
+// Linear attention with one decay per head over rollouts with episode ends.
+//
+//   S_t = f_t S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t,
+//   f_t = decay_h, or 0 where an episode begins at t (reset_t)
+//
+// for every environment e and head h, S [Dk, Dv] in float32.  With
+// dS_t = f_{t+1} dS_{t+1} + scale q_t do_t^T the gradients are
+//
+//   dq_t = scale S_t do_t,   dk_t = dS_t v_t,   dv_t = dS_t^T k_t,
+//   dS_initial = f_0 dS_0
+//
+// so each of the three is the same recurrence again, over other operands and
+// for two of them backwards in time (struct Sweep).  A reset replaces the state
+// instead of multiplying it by zero: what an earlier episode left there,
+// infinities and NaN included, does not reach the next one.
+#pragma once
+#include "numeric_types.cuh"
+
+namespace duckb200 {
+
+constexpr int kHeadMax = 128;   // largest Dk and Dv
+
+// Strides of a [T, E, H, D] operand in elements; D is dense.
+struct Rows {
+  int64_t t, e, h;
+};
+
+// X_t = f X_{t-1} + mulA a_t b_t^T  (rows of a's size Di, columns of b's size
+// Dj), y_t = mulC X_t^T c_t.  The state arrays are indexed i * ri + j * rj
+// within their (e, h).
+struct Sweep {
+  const void *a, *b, *c;
+  void *y;                     // [T, E, H, Dj] dense
+  Rows as, bs, cs;
+  const float *init;           // or null: zero
+  float *last;                 // or null
+  const float *decay;          // [H]
+  const uint8_t *resets;       // [T, E] dense, or null
+  int T, E, H, Di, Dj, ri, rj, reverse;
+  float mulA, mulC;
+};
+
+constexpr int kScanSteps = 16;
+
+// One thread per column of the state, its DI rows in registers; the rows'
+// operands of 16 steps at a time in shared memory.
+template <class T, int DI> __global__ void __launch_bounds__(128) attentionScan(Sweep s) {
+  __shared__ __align__(16) float a[kScanSteps][DI], c[kScanSteps][DI];
+  __shared__ uint8_t cut[kScanSteps];
+  const int64_t eh = blockIdx.x;
+  const int e = int(eh / s.H), h = int(eh - int64_t(e) * s.H);
+  const int j = blockIdx.y * blockDim.x + threadIdx.x;
+  const bool live = j < s.Dj;
+  const T *pa = static_cast<const T *>(s.a) + e * s.as.e + h * s.as.h;
+  const T *pb = static_cast<const T *>(s.b) + e * s.bs.e + h * s.bs.h + (live ? j : 0);
+  const T *pc = static_cast<const T *>(s.c) + e * s.cs.e + h * s.cs.h;
+  T *py = static_cast<T *>(s.y) + eh * s.Dj + j;
+  const int64_t yt = int64_t(s.E) * s.H * s.Dj, base = eh * s.Di * s.Dj;
+  const float decay = s.decay[h];
+  float x[DI];
+#pragma unroll
+  for (int i = 0; i < DI; ++i) x[i] = s.init && live && i < s.Di ? s.init[base + int64_t(i) * s.ri + int64_t(j) * s.rj] : 0.f;
+  for (int t0 = 0; t0 < s.T; t0 += kScanSteps) {
+    const int count = min(kScanSteps, s.T - t0);
+    __syncthreads();
+    for (int q = threadIdx.x; q < count * DI; q += blockDim.x) {
+      const int u = q / DI, i = q - u * DI;
+      const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
+      a[u][i] = i < s.Di ? s.mulA * toFloat(pa[t * s.as.t + i]) : 0.f;
+      c[u][i] = i < s.Di ? s.mulC * toFloat(pc[t * s.cs.t + i]) : 0.f;
+    }
+    for (int u = threadIdx.x; u < count; u += blockDim.x) {
+      // The factor between a step and the one before it in the sweep: the
+      // reset of the later of the two in time.
+      const int64_t t = s.reverse ? s.T - (t0 + u) : t0 + u;
+      cut[u] = s.resets && t < s.T ? s.resets[t * s.E + e] : 0;
+    }
+    __syncthreads();
+    for (int u = 0; u < count; ++u) {
+      const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
+      const float b = live ? toFloat(pb[t * s.bs.t]) : 0.f;
+      const float f = s.reverse && t0 + u == 0 ? 1.f : decay;
+      if (cut[u]) {
+#pragma unroll
+        for (int i = 0; i < DI; ++i) x[i] = 0.f;
+      }
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DI; ++i) {
+        x[i] = fmaf(f, x[i], a[u][i] * b);
+        y[i & 3] = fmaf(c[u][i], x[i], y[i & 3]);
+      }
+      if (live && s.y) py[t * yt] = fromFloat<T>((y[0] + y[1]) + (y[2] + y[3]));
+    }
+  }
+  if (s.last && live) {
+    // Backwards, the state before the first step is one more factor away.
+    const bool gone = s.reverse && s.T > 0 && s.resets && s.resets[e];
+    const float f = s.reverse && s.T > 0 ? decay : 1.f;
+#pragma unroll
+    for (int i = 0; i < DI; ++i)
+      if (i < s.Di) s.last[base + int64_t(i) * s.ri + int64_t(j) * s.rj] = gone ? 0.f : f * x[i];
+  }
+}
+
+struct StepOf {
+  const void *q, *k, *v;       // rows of [E, H, D], D dense
+  void *out;                   // [E, H, Dv] dense
+  float *state;                // [E, H, Dk, Dv] dense, updated in place
+  const float *decay;
+  const uint8_t *resets;       // [E] or null
+  int64_t qe, qh, ke, kh, ve, vh;
+  int E, H, Dk, Dv;
+  float scale;
+};
+
+// One step of the recurrence, one block per (e, h): 32 columns by 4 rows of
+// threads walk the state.
+template <class T> __global__ void __launch_bounds__(128) attentionStepAny(StepOf s) {
+  __shared__ float q[kHeadMax], k[kHeadMax], red[4][32];
+  const int64_t eh = blockIdx.x;
+  const int e = int(eh / s.H), h = int(eh - int64_t(e) * s.H);
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  if (int(threadIdx.x) < s.Dk) {
+    q[threadIdx.x] = s.scale * toFloat(static_cast<const T *>(s.q)[e * s.qe + h * s.qh + threadIdx.x]);
+    k[threadIdx.x] = toFloat(static_cast<const T *>(s.k)[e * s.ke + h * s.kh + threadIdx.x]);
+  }
+  const bool cut = s.resets && s.resets[e];
+  const float decay = s.decay[h];
+  __syncthreads();
+  for (int j0 = 0; j0 < s.Dv; j0 += 32) {
+    const int j = j0 + lane;
+    float o = 0.f;
+    if (j < s.Dv) {
+      const float v = toFloat(static_cast<const T *>(s.v)[e * s.ve + h * s.vh + j]);
+      float *state = s.state + eh * s.Dk * s.Dv + j;
+      for (int i = part; i < s.Dk; i += 4) {
+        const float old = cut ? 0.f : state[int64_t(i) * s.Dv];
+        const float x = fmaf(decay, old, k[i] * v);
+        state[int64_t(i) * s.Dv] = x;
+        o = fmaf(q[i], x, o);
+      }
+    }
+    red[part][lane] = o;
+    __syncthreads();
+    if (part == 0 && j < s.Dv)
+      static_cast<T *>(s.out)[eh * s.Dv + j] =
+          fromFloat<T>((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+    __syncthreads();
+  }
+}
+
+}  // namespace duckb200

@@ -74,6 +74,16 @@ def library():
         lib.duck_fp32_peak.argtypes = [I, I, ctypes.POINTER(D), P]
         lib.duck_ppo_loss_scratch.argtypes = [I, I]
         lib.duck_ppo_loss.argtypes = [I, I] + [P] * 10 + [D, D, D] + [P] * 5 + [P]
+        L = ctypes.c_int64
+        lib.duck_layer_norm_forward.argtypes = [P] * 5 + [L, I, L, D, I, P]
+        lib.duck_layer_norm_scratch.argtypes = [L, I]
+        lib.duck_layer_norm_scratch.restype = L
+        lib.duck_layer_norm_backward.argtypes = [P] * 8 + [L, I, L, L, I, P]
+        lib.duck_elu_checkpoint.argtypes = [P] * 4 + [L, I, I, P]
+        lib.duck_elu_restore.argtypes = [P] * 5 + [L, I, I, P]
+        lib.duck_linear_attention_sizes.argtypes = [P, P]
+        for name in ("duck_linear_attention_forward", "duck_linear_attention_backward", "duck_linear_attention_step"):
+            getattr(lib, name).argtypes = [P, P]
         lib.duck_env_obs_dim.argtypes = [P, P]
         lib.duck_env_targets.argtypes = [P, P, D, P, P, P, P, P, P]
         lib.duck_env_reference_targets.argtypes = [P, P, P, D, P, P, P, P, P, P, P, P]
@@ -96,7 +106,9 @@ def library():
                      "duck_env_targets", "duck_env_reference_targets", "duck_env_post_step", "duck_env_observe", "duck_env_reset_buffers",
                      "duck_bam_critic_dim", "duck_bam_step", "duck_bam_begin", "duck_bam_substep", "duck_bam_finish",
                      "duck_bam_servo", "duck_bam_reset_buffers", "duck_bam_observe", "duck_ppo_loss_scratch",
-                     "duck_ppo_loss"):
+                     "duck_ppo_loss", "duck_layer_norm_forward", "duck_layer_norm_backward", "duck_elu_checkpoint",
+                     "duck_elu_restore", "duck_linear_attention_sizes", "duck_linear_attention_forward",
+                     "duck_linear_attention_backward", "duck_linear_attention_step"):
             getattr(lib, name).restype = I
         _lib = lib
     return _lib

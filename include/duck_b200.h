@@ -348,6 +348,77 @@ int duck_ppo_loss(int batch, int actions, const float *mu, const float *std, con
                   double entropy_coef, float *scratch, float *out, float *grad_mu, float *grad_std,
                   float *grad_value, duck_stream stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators of a policy with memory (no reference counterpart; the Python side
+ * is duck_gym_b200/memory.py).  All of them run asynchronously on `stream` of
+ * the current device, take device pointers, allocate nothing and never wait for
+ * the host, so they can be captured in CUDA graphs.  `type` is the element type
+ * of the activations and their gradients (DUCK_FLOAT32 or DUCK_BFLOAT16);
+ * statistics, weights, states and scales are float32.  Strides count elements;
+ * the last axis of every operand is dense.  Results repeat bit for bit. */
+enum { DUCK_FLOAT32 = 0, DUCK_BFLOAT16 = 1 };
+
+/* Layer norm of the rows of x [rows, n] (rows x_stride apart):
+ * y = (x - mean) rstd weight + bias, y dense.  weight and bias [n] may be NULL
+ * (1 and 0).  stats [rows, 2] receives mean and rstd for the backward pass, or
+ * is NULL. */
+int duck_layer_norm_forward(const void *x, const float *weight, const float *bias, void *y, float *stats,
+                            int64_t rows, int n, int64_t x_stride, double eps, int type, duck_stream stream);
+/* Floats of scratch that duck_layer_norm_backward needs; -1 for sizes that it
+ * refuses. */
+int64_t duck_layer_norm_scratch(int64_t rows, int n);
+/* Gradients of duck_layer_norm_forward: dx [rows, n] dense, dweight and dbias
+ * [n].  dx may be NULL, and so may dweight and dbias.  scratch may be NULL where
+ * both of these are. */
+int duck_layer_norm_backward(const void *x, const void *dy, const float *weight, const float *stats, void *dx,
+                             float *dweight, float *dbias, float *scratch, int64_t rows, int n, int64_t x_stride,
+                             int64_t dy_stride, int type, duck_stream stream);
+
+/* ELU with its output kept in 8 bits: y = x > 0 ? x : exp(x) - 1 [rows, n],
+ * codes [rows, n] and one scale per group of 128 values of a row, scales
+ * [rows, ceil(n / 128)]; y is kept as code * scale.  All arrays are dense. */
+int duck_elu_checkpoint(const void *x, void *y, int8_t *codes, float *scales, int64_t rows, int n, int type,
+                        duck_stream stream);
+/* Backward pass from the kept output: y (the kept values, in dy's type) and
+ * dx = dy (y > 0 ? 1 : 1 + y).  y may be NULL. */
+int duck_elu_restore(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows, int n,
+                     int type, duck_stream stream);
+
+/* Linear attention with one decay per head, for E environments and H heads:
+ *   S_t = f_t S_{t-1} + k_t v_t^T,  o_t = scale S_t^T q_t,
+ *   f_t = decay[h], or 0 where resets[t, e] is set (an episode begins at t).
+ * q and k are [T, E, H, Dk], v, out and dout [T, E, H, Dv] with 1 <= Dk, Dv <=
+ * 128; q, k, v and dout have the strides given, {t, e, h}; the outputs are
+ * dense.  States are dense [E, H, Dk, Dv] float32.  decay [H] is in [0, 1]. */
+typedef struct duck_attention {
+  const void *q, *k, *v;
+  void *out;                  /* forward */
+  const float *decay;         /* [H] */
+  const uint8_t *resets;      /* [T, E] dense, or NULL */
+  const float *state_in;      /* S before the first step, or NULL for zero */
+  float *state_out;           /* forward: S after the last step, or NULL */
+  const void *dout;           /* backward: gradient of out */
+  const float *dstate_out;    /* backward: gradient of state_out, or NULL */
+  void *dq, *dk, *dv;         /* backward */
+  float *dstate_in;           /* backward: gradient of state_in, or NULL */
+  void *saved;                /* forward writes, backward reads: duck_linear_attention_sizes; or NULL */
+  float *scratch;             /* duck_linear_attention_sizes */
+  int64_t q_stride[3], k_stride[3], v_stride[3], dout_stride[3];
+  int32_t T, E, H, Dk, Dv, type;
+  float scale;
+} duck_attention;
+
+/* Bytes of workspace for a call of these sizes (only T, E, H, Dk, Dv, type and
+ * which pointers are NULL are looked at): out[0] scratch of the forward call,
+ * out[1] scratch of the backward call, out[2] `saved`, which a forward call that
+ * a backward call will follow has to be given. */
+int duck_linear_attention_sizes(const duck_attention *args, int64_t *out);
+int duck_linear_attention_forward(const duck_attention *args, duck_stream stream);
+int duck_linear_attention_backward(const duck_attention *args, duck_stream stream);
+/* One step (T is not read), q, k and v [E, H, D]: the state in state_out is
+ * updated in place and `out` written.  resets is [E]. */
+int duck_linear_attention_step(const duck_attention *args, duck_stream stream);
+
 /* No reference counterpart.  FP32 fused-multiply-add throughput probe used
  * as the roofline denominator: runs `iterations` dependent FMA chains on
  * every SM and returns achieved TFLOP/s (2 flops per FMA) in *tflops. */
