@@ -1,0 +1,743 @@
+// Linear attention with a decay in chunks of C steps, bfloat16 operands.
+//
+// Within a chunk that starts from the state S (i, j steps of the chunk, L its
+// length, decay l, everything of one environment and head):
+//
+//   o_i  = scale [ l^(i+1) S^T q_i + sum_{j <= i} l^(i-j) (q_i . k_j) v_j ]
+//   S'   = l^L S + sum_j l^(L-1-j) k_j v_j^T
+//
+// which are the products Q K^T, (Q K^T . decays) V, Q S and K^T V.  A warp owns
+// 16 steps of the chunk and a slice of S, which stays in its registers in
+// float32 from chunk to chunk; a bfloat16 copy in shared memory is the operand
+// of the next chunk's Q S.
+//
+// Decays without an exponential per pair: of the 16 steps a warp owns, a pair
+// within the warp's own 16x16 block has one of 31 fixed factors (kept in
+// registers); a pair with an earlier block j has l^(i-i0) l^(i0-j), a factor per
+// row and one per column, both at most 1 whatever l is.
+//
+// Roundings to bfloat16, each of 8 significant bits: the decayed scores, and the
+// copy of S.  The state itself is kept to float32 accuracy: its operand
+// l^(L-1-j) k_j is split into the sum of two bfloat16 numbers (16 bits), a second
+// product each.
+//
+// Episodes: step i sees step j only if no reset lies in (j, i]; S only if none
+// lies at or before i.  Scores and states that are masked are replaced, not
+// multiplied by zero.  A product still multiplies a masked zero with whatever
+// the other operand holds, so an infinity or NaN of an earlier episode (or of a
+// later step in the same tile) would come out as NaN.  So a block that saw
+// anything in its outputs or its state that is not finite says so in a flag, and
+// redoAttention() computes the environments and heads of such blocks once more
+// step by step, where nothing masked is ever touched.  (What is wrong in this way is
+// never finite, the saved states and those of segments included, and whoever reads
+// those sees it too.)
+#pragma once
+#include "linear_attention.cuh"
+#include "tensor_tiles.cuh"
+
+namespace duckb200 {
+
+struct ChunkArgs {
+  const bf16 *q, *k, *v;
+  bf16 *out;                   // [T, E, H, Dv] dense
+  Rows qs, ks, vs;
+  const float *decay;
+  const uint8_t *resets;       // [T, E] or null
+  const float *stateIn;        // [E, H, Dk, Dv] or null
+  float *stateOut;             // or null
+  bf16 *saved;                 // [E, H, chunks, Dk, Dv]: the state before each chunk, or null
+  float *segments;             // [E, H, segmentCount, Dk, Dv] where T is split, else null
+  uint8_t *segmentCut;         // [E, H, segmentCount]
+  uint8_t *flags;              // [E, H, segmentCount, columnTiles]: blocks that saw what is not finite
+  int T, E, H, Dk, Dv;
+  int segmentLength, segmentCount, columnTiles;
+  int vecQ, vecK, vecV;        // rows can be read in 16-byte pieces
+  float scale;
+};
+
+// Bit i: an episode begins at step t0 + i (i < 64, t0 + i < end).
+__device__ __forceinline__ unsigned long long resetMask(const uint8_t *resets, int E, int e, int t0, int end) {
+  if (!resets) return 0;
+  const int lane = threadIdx.x & 31;
+  const bool a = t0 + lane < end && resets[int64_t(t0 + lane) * E + e];
+  const bool b = t0 + 32 + lane < end && resets[int64_t(t0 + 32 + lane) * E + e];
+  const unsigned low = __ballot_sync(0xffffffffu, a), high = __ballot_sync(0xffffffffu, b);
+  return (static_cast<unsigned long long>(high) << 32) | low;
+}
+// Number of resets at steps 0..i: steps of one number are of one episode.
+__device__ __forceinline__ int episodeOf(unsigned long long mask, int i) { return __popcll(mask & (~0ull >> (63 - i))); }
+
+// Rows t0.. (count of them, the rest zero) of an operand, columns c0..c0+D-1
+// (those from `width` on zero), into a tile of C rows.
+template <int C, int D, int THREADS>
+__device__ __forceinline__ void loadTile(bf16 *tile, const bf16 *base, int64_t stride, int t0, int count, int c0,
+                                         int width, bool vec) {
+  constexpr int L = D + 8;
+  if (vec) {
+    constexpr int pieces = D / 8;
+#pragma unroll
+    for (int x = 0; x < C * pieces / THREADS; ++x) {
+      const int id = x * THREADS + threadIdx.x, r = id / pieces, c = (id % pieces) * 8;
+      const bool valid = r < count && c0 + c < width;
+      copyAsync16(tile + r * L + c, valid ? base + int64_t(t0 + r) * stride + c0 + c : base, valid);
+    }
+  } else {
+    for (int id = threadIdx.x; id < C * D; id += THREADS) {
+      const int r = id / D, c = id % D;
+      tile[r * L + c] = r < count && c0 + c < width ? base[int64_t(t0 + r) * stride + c0 + c] : fromFloat<bf16>(0.f);
+    }
+  }
+}
+
+// Shared memory of a block: tiles in `buffers` copies.
+template <int C, int DK, int DV, bool OUT> constexpr int chunkTileElements() {
+  return C * (DK + 8) * (OUT ? 2 : 1) + C * (DV + 8);
+}
+template <int C, int DK, int DV, bool OUT> constexpr int chunkSharedBytes(int buffers) {
+  return buffers * (chunkTileElements<C, DK, DV, OUT>() + (OUT ? DK * (DV + 8) : 0)) * 2 + 4 * 2 * C;
+}
+
+// One block per (environment, head), segment of T and tile of DV columns; C / 16
+// warps.  OUT = false computes the state at the segment's end only.
+template <int C, int DK, int DV, bool OUT>
+__global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionChunks(ChunkArgs p, int buffers) {
+  constexpr int W = C / 16, THREADS = W * 32, LQ = DK + 8, LV = DV + 8;
+  constexpr int RT = DK / 16;                                  // row tiles of the state
+  constexpr int SM = RT >= W ? RT / W : 1;                     // of which a warp has
+  constexpr int SPLIT = RT >= W ? 1 : W / RT;                  // warps that share a row tile
+  constexpr int SN = DV / 8 / SPLIT;                           // tiles of 8 columns of a warp's slice
+  static_assert(SN % 2 == 0, "operands of the state come two column tiles at a time");
+  extern __shared__ __align__(16) unsigned char shared[];
+  bf16 *tiles = reinterpret_cast<bf16 *>(shared);
+  bf16 *copies = tiles + buffers * chunkTileElements<C, DK, DV, OUT>();      // the state in bfloat16
+  float *before = reinterpret_cast<float *>(copies + (OUT ? buffers * DK * LV : 0));   // scale l^(C - x)
+  float *toEnd = before + C;                                                  // l^(L - 1 - j)
+
+  const int64_t eh = blockIdx.x;
+  const int e = int(eh / p.H), h = int(eh - int64_t(e) * p.H);
+  const int seg = blockIdx.y / p.columnTiles, col0 = (blockIdx.y - seg * p.columnTiles) * DV;
+  const int t0 = seg * p.segmentLength, t1 = min(p.T, t0 + p.segmentLength);
+  const int chunks = (t1 - t0 + C - 1) / C;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
+  const bf16 *q = p.q + e * p.qs.e + h * p.qs.h, *k = p.k + e * p.ks.e + h * p.ks.h, *v = p.v + e * p.vs.e + h * p.vs.h;
+  const int64_t stateSize = int64_t(p.Dk) * p.Dv;
+  const float *init = p.segments && OUT ? p.segments + (eh * p.segmentCount + seg) * stateSize
+                      : p.stateIn && !p.segments ? p.stateIn + eh * stateSize : nullptr;
+  float *last = !OUT ? p.segments + (eh * p.segmentCount + seg) * stateSize
+                : p.stateOut && seg == p.segmentCount - 1 ? p.stateOut + eh * stateSize : nullptr;
+
+  auto load = [&](int c, int buffer) {
+    bf16 *tile = tiles + buffer * chunkTileElements<C, DK, DV, OUT>();
+    const int first = t0 + c * C, count = min(C, t1 - first);
+    loadTile<C, DK, THREADS>(tile, k, p.ks.t, first, count, 0, p.Dk, p.vecK);
+    loadTile<C, DV, THREADS>(tile + C * LQ, v, p.vs.t, first, count, col0, p.Dv, p.vecV);
+    if (OUT) loadTile<C, DK, THREADS>(tile + C * (LQ + LV), q, p.qs.t, first, count, 0, p.Dk, p.vecQ);
+    commitCopies();
+  };
+  if (chunks > 0) load(0, 0);
+
+  // Powers of the decay.
+  const float decay = p.decay[h];
+  const float logDecay = fmaxf(log2f(decay), -1e30f);   // finite: no 0 times infinity for a decay of zero
+  // (Of a negative or NaN decay: NaN, which leaves the block to redoAttention().)
+  auto power = [&](int n) { return decay >= 0.f ? exp2f(float(n) * logDecay) : __int_as_float(0x7fc00000); };
+  for (int x = threadIdx.x; x < C; x += THREADS) {
+    before[x] = p.scale * power(C - x);
+    toEnd[x] = power(C - 1 - x);
+  }
+  float inBlock[2][4];   // scale l^(i - j) of the warp's 16x16 block, 0 above its diagonal
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int d = g + (x >> 1) * 8 - (2 * tq + (x & 1) + 8 * n);
+      inBlock[n][x] = d >= 0 ? p.scale * power(d) : 0.f;
+    }
+  const float fromStart = p.scale * power(16 * warp + 1);   // of the warp's first step to S
+  const float row0 = power(g), row1 = power(g + 8);
+  const float fullChunk = power(C);
+
+  // The warp's slice of the state.
+  const int sm0 = RT >= W ? warp * SM : warp / SPLIT, sn0 = RT >= W ? 0 : (warp % SPLIT) * SN;
+  float S[SM][SN][4];
+#pragma unroll
+  for (int m = 0; m < SM; ++m)
+#pragma unroll
+    for (int n = 0; n < SN; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int i = (sm0 + m) * 16 + g + (x >> 1) * 8, j = col0 + (sn0 + n) * 8 + 2 * tq + (x & 1);
+        S[m][n][x] = init && i < p.Dk && j < p.Dv ? init[int64_t(i) * p.Dv + j] : 0.f;
+      }
+  auto copyState = [&](int buffer) {
+    bf16 *copy = copies + buffer * DK * LV;
+#pragma unroll
+    for (int m = 0; m < SM; ++m)
+#pragma unroll
+      for (int n = 0; n < SN; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          *reinterpret_cast<uint32_t *>(copy + ((sm0 + m) * 16 + g + y * 8) * LV + (sn0 + n) * 8 + 2 * tq) =
+              packPair(S[m][n][2 * y], S[m][n][2 * y + 1]);
+  };
+  if (OUT) copyState(0);
+
+  bool bad = false, anyReset = false;
+  for (int c = 0; c < chunks; ++c) {
+    const int buffer = buffers > 1 ? c & 1 : 0, first = t0 + c * C, count = min(C, t1 - first);
+    const unsigned long long mask = resetMask(p.resets, p.E, e, first, min(t1, first + C));
+    anyReset |= mask != 0;
+    waitCopies();
+    __syncthreads();
+    if (c + 1 < chunks) load(c + 1, (c + 1) & 1);
+    const bf16 *K = tiles + buffer * chunkTileElements<C, DK, DV, OUT>(), *V = K + C * LQ, *Q = V + C * LV;
+    if (count < C)
+      for (int x = threadIdx.x; x < C; x += THREADS) toEnd[x] = x < count ? power(count - 1 - x) : 0.f;
+
+    if (OUT) {
+      const bf16 *copy = copies + buffer * DK * LV;
+      const int i0 = 16 * warp;
+      const int part0 = episodeOf(mask, i0 + g), part1 = episodeOf(mask, i0 + g + 8);
+      if (p.saved && seg * (p.segmentLength / C) + c > 0) {
+        bf16 *to = p.saved + (eh * ((p.T + C - 1) / C) + seg * (p.segmentLength / C) + c) * stateSize;
+        for (int x = threadIdx.x; x < p.Dk * DV; x += THREADS) {
+          const int i = x / DV, j = x % DV;
+          if (col0 + j < p.Dv) to[int64_t(i) * p.Dv + col0 + j] = copy[i * LV + j];
+        }
+      }
+      uint32_t a[DK / 16][4];
+#pragma unroll
+      for (int kk = 0; kk < DK / 16; ++kk) operandA<LQ>(a[kk], Q, i0, kk * 16);
+      float o[DV / 8][4];
+#pragma unroll
+      for (int n = 0; n < DV / 8; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[n][x] = 0.f;
+      // Q S
+#pragma unroll
+      for (int kk = 0; kk < DK / 16; ++kk)
+#pragma unroll
+        for (int n = 0; n < DV / 16; ++n) {
+          uint32_t b[4];
+          operandBTransposed<LV>(b, copy, kk * 16, n * 16);
+          multiplyAdd(o[2 * n], a[kk], b[0], b[1]);
+          multiplyAdd(o[2 * n + 1], a[kk], b[2], b[3]);
+        }
+#pragma unroll
+      for (int n = 0; n < DV / 8; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[n][x] = (x < 2 ? part0 : part1) == 0 ? o[n][x] * fromStart : 0.f;
+      // Earlier blocks, then the warp's own.
+      for (int block = 0; block <= warp; ++block) {
+        float s[2][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < DK / 16; ++kk) {
+          uint32_t b[4];
+          operandB<LQ>(b, K, block * 16, kk * 16);
+          multiplyAdd(s[0], a[kk], b[0], b[1]);
+          multiplyAdd(s[1], a[kk], b[2], b[3]);
+        }
+        if (block < warp) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float2 f = *reinterpret_cast<const float2 *>(before + C - i0 + block * 16 + n * 8 + 2 * tq);
+            s[n][0] *= f.x;
+            s[n][1] *= f.y;
+            s[n][2] *= f.x;
+            s[n][3] *= f.y;
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < DV / 8; ++n) {
+            o[n][0] *= row0;
+            o[n][1] *= row0;
+            o[n][2] *= row1;
+            o[n][3] *= row1;
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              s[n][x] = g + (x >> 1) * 8 >= 2 * tq + (x & 1) + 8 * n ? s[n][x] * inBlock[n][x] : 0.f;
+        }
+        if (mask) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (episodeOf(mask, block * 16 + n * 8 + 2 * tq + (x & 1)) != (x < 2 ? part0 : part1)) s[n][x] = 0.f;
+        }
+        const uint32_t w[4] = {packPair(s[0][0], s[0][1]), packPair(s[0][2], s[0][3]), packPair(s[1][0], s[1][1]),
+                               packPair(s[1][2], s[1][3])};
+#pragma unroll
+        for (int n = 0; n < DV / 16; ++n) {
+          uint32_t b[4];
+          operandBTransposed<LV>(b, V, block * 16, n * 16);
+          multiplyAdd(o[2 * n], w, b[0], b[1]);
+          multiplyAdd(o[2 * n + 1], w, b[2], b[3]);
+        }
+      }
+      float finite = 0.f;
+#pragma unroll
+      for (int n = 0; n < DV / 8; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) finite = fmaf(o[n][x], 0.f, finite);
+      bad |= finite != 0.f;   // NaN
+#pragma unroll
+      for (int n = 0; n < DV / 8; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int i = i0 + g + y * 8, j = col0 + n * 8 + 2 * tq;
+          if (i >= count) continue;
+          bf16 *to = p.out + (int64_t(first + i) * p.E * p.H + eh) * p.Dv + j;
+          if (j + 1 < p.Dv && p.Dv % 2 == 0) *reinterpret_cast<uint32_t *>(to) = packPair(o[n][2 * y], o[n][2 * y + 1]);
+          else {
+            if (j < p.Dv) to[0] = fromFloat<bf16>(o[n][2 * y]);
+            if (j + 1 < p.Dv) to[1] = fromFloat<bf16>(o[n][2 * y + 1]);
+          }
+        }
+    }
+
+    // The state at the chunk's end.
+    if (c + 1 < chunks || last) {
+      if (count < C) __syncthreads();   // toEnd
+      const int endPart = episodeOf(mask, 63);
+      const float f = count == C ? fullChunk : power(count);
+#pragma unroll
+      for (int m = 0; m < SM; ++m)
+#pragma unroll
+        for (int n = 0; n < SN; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) S[m][n][x] = endPart == 0 ? S[m][n][x] * f : 0.f;
+#pragma unroll
+      for (int kk = 0; kk < C / 16; ++kk) {
+        float2 f0 = *reinterpret_cast<const float2 *>(toEnd + kk * 16 + 2 * tq);
+        float2 f1 = *reinterpret_cast<const float2 *>(toEnd + kk * 16 + 8 + 2 * tq);
+        bool in[4] = {true, true, true, true};
+        if (mask) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) in[x] = episodeOf(mask, kk * 16 + 2 * tq + (x & 1) + (x >> 1) * 8) == endPart;
+        }
+#pragma unroll
+        for (int m = 0; m < SM; ++m) {
+          uint32_t a[4], high[4], low[4];
+          operandATransposed<LQ>(a, K, (sm0 + m) * 16, kk * 16);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {   // registers 0, 1: steps 2 tq, + 1; registers 2, 3: 8 later
+            const float l = in[(x >> 1) * 2] ? lowOf(a[x]) * (x < 2 ? f0.x : f1.x) : 0.f;
+            const float u = in[(x >> 1) * 2 + 1] ? highOf(a[x]) * (x < 2 ? f0.y : f1.y) : 0.f;
+            high[x] = packPair(l, u);
+            low[x] = packPair(l - lowOf(high[x]), u - highOf(high[x]));
+          }
+#pragma unroll
+          for (int n = 0; n < SN / 2; ++n) {
+            uint32_t b[4];
+            operandBTransposed<LV>(b, V, kk * 16, (sn0 + 2 * n) * 8);
+            multiplyAdd(S[m][2 * n], high, b[0], b[1]);
+            multiplyAdd(S[m][2 * n + 1], high, b[2], b[3]);
+            multiplyAdd(S[m][2 * n], low, b[0], b[1]);
+            multiplyAdd(S[m][2 * n + 1], low, b[2], b[3]);
+          }
+        }
+      }
+      float finite = 0.f;
+#pragma unroll
+      for (int m = 0; m < SM; ++m)
+#pragma unroll
+        for (int n = 0; n < SN; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) finite = fmaf(S[m][n][x], 0.f, finite);
+      bad |= finite != 0.f;
+      if (OUT && c + 1 < chunks) copyState((c + 1) & 1);
+    }
+  }
+  if (!OUT && col0 == 0 && threadIdx.x == 0) p.segmentCut[eh * p.segmentCount + seg] = anyReset;
+  if (OUT) {
+    const bool redo = __syncthreads_or(bad);
+    if (threadIdx.x == 0) p.flags[eh * gridDim.y + blockIdx.y] = redo;
+  }
+  if (last) {
+#pragma unroll
+    for (int m = 0; m < SM; ++m)
+#pragma unroll
+      for (int n = 0; n < SN; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int i = (sm0 + m) * 16 + g + y * 8, j = col0 + (sn0 + n) * 8 + 2 * tq;
+          if (i >= p.Dk) continue;
+          float *to = last + int64_t(i) * p.Dv + j;
+          if (j < p.Dv) to[0] = S[m][n][2 * y];
+          if (j + 1 < p.Dv) to[1] = S[m][n][2 * y + 1];
+        }
+  }
+}
+
+// Operands and arrays of a backward call.
+struct BackwardArgs {
+  const bf16 *q, *k, *v, *dout;
+  bf16 *dq, *dk, *dv;          // dense
+  Rows qs, ks, vs, os;
+  const float *decay;
+  const uint8_t *resets;
+  const float *stateIn, *dstateOut;
+  float *dstateIn;
+  const bf16 *saved;           // the state before each chunk but the first
+  float *segments;             // [E, H, segmentCount, Dk, Dv]: gradient of the state after each segment, or null
+  uint8_t *segmentCut;
+  uint8_t *flags;              // [E, H, segmentCount]
+  int T, E, H, Dk, Dv;
+  int segmentLength, segmentCount;
+  int vecQ, vecK, vecV, vecO;
+  float scale;
+};
+
+template <int C, int D, bool OUT> constexpr int backwardWarps() { return OUT && D == 128 ? C / 8 : C / 16; }
+template <int C, int D, bool OUT> constexpr int backwardSharedBytes() {
+  return (OUT ? (4 * C + 2 * D) : 2 * C) * (D + 8) * 2 + (16 + C + 4) * 4;
+}
+
+// Rows of 16 steps by N tiles of 8 columns of a dense [T, E, H, width] output.
+template <int N>
+__device__ __forceinline__ void storeTile(bf16 *out, const float (&x)[N][4], int64_t stepStride, int first, int count,
+                                          int row0, int col0, int width) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int i = row0 + g + y * 8, j = col0 + n * 8 + 2 * tq;
+      if (i >= count) continue;
+      bf16 *to = out + int64_t(first + i) * stepStride + j;
+      if (j + 1 < width && width % 2 == 0) *reinterpret_cast<uint32_t *>(to) = packPair(x[n][2 * y], x[n][2 * y + 1]);
+      else {
+        if (j < width) to[0] = fromFloat<bf16>(x[n][2 * y]);
+        if (j + 1 < width) to[1] = fromFloat<bf16>(x[n][2 * y + 1]);
+      }
+    }
+}
+
+template <int N> __device__ __forceinline__ bool notFinite(const float (&x)[N][4]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) sum = fmaf(x[n][y], 0.f, sum);
+  return sum != 0.f;
+}
+
+// One block per (environment, head) and segment of T, chunks from the last to the
+// first.  With X the gradient of the state after the chunk and S the state before
+// it, steps i and j, L the chunk's length:
+//
+//   dq_i = scale [ l^(i+1) S do_i + sum_{j <= i} l^(i-j) (do_i . v_j) k_j ]
+//   dk_j = l^(L-1-j) X v_j   + scale sum_{i >= j} l^(i-j) (v_j . do_i) q_i
+//   dv_j = l^(L-1-j) X^T k_j + scale sum_{i >= j} l^(i-j) (k_j . q_i) do_i
+//   X'   = l^L X + scale sum_i l^(i+1) q_i do_i^T
+//
+// S comes from the forward pass in bfloat16, X stays in registers in float32 as
+// S does there, with the same split of its operand.  Each of the three outputs
+// takes its scores from products of its own, in the layout in which they are the
+// next product's operand: six instead of five products of C x C x D, and no score
+// passes through shared memory.  OUT = false: X' of a segment alone.
+template <int C, int D, bool OUT>
+__global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 64 : 256) / C)
+    attentionChunksBackward(BackwardArgs p) {
+  constexpr int W = backwardWarps<C, D, OUT>(), THREADS = W * 32, LD = D + 8;
+  constexpr int PARTS = W / (C / 16);                          // warps that share 16 rows of the outputs
+  constexpr int N = D / 8 / PARTS;                             // tiles of 8 columns of a warp's outputs
+  constexpr int RT = D / 16, SM = RT >= W ? RT / W : 1, SPLIT = RT >= W ? 1 : W / RT, SN = D / 8 / SPLIT;
+  extern __shared__ __align__(16) unsigned char shared[];
+  bf16 *Q = reinterpret_cast<bf16 *>(shared), *O = Q + C * LD, *K = O + C * LD, *V = K + C * LD, *S = V + C * LD,
+       *X = S + D * LD;
+  float *powers = reinterpret_cast<float *>(OUT ? X + D * LD : K);   // scale l^(x - 16), 0 for x < 16; C + 20 of them
+  const int64_t eh = blockIdx.x;
+  const int e = int(eh / p.H), h = int(eh - int64_t(e) * p.H), seg = OUT ? blockIdx.y : blockIdx.y + 1;
+  const int t0 = seg * p.segmentLength, t1 = min(p.T, t0 + p.segmentLength);
+  const int chunks = (t1 - t0 + C - 1) / C, allChunks = (p.T + C - 1) / C;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tq = lane & 3;
+  const int row = (warp / PARTS) * 16, col = (warp % PARTS) * N * 8;
+  const bf16 *q = p.q + e * p.qs.e + h * p.qs.h, *o = p.dout + e * p.os.e + h * p.os.h;
+  const bf16 *k = p.k + e * p.ks.e + h * p.ks.h, *v = p.v + e * p.vs.e + h * p.vs.h;
+  const int64_t stateSize = int64_t(p.Dk) * p.Dv;
+  const float *init = p.segments ? (OUT ? p.segments + (eh * p.segmentCount + seg) * stateSize : nullptr)
+                                 : p.dstateOut ? p.dstateOut + eh * stateSize : nullptr;
+  float *last = !OUT ? p.segments + (eh * p.segmentCount + seg) * stateSize
+                : p.dstateIn && seg == 0 ? p.dstateIn + eh * stateSize : nullptr;
+
+  const float decay = p.decay[h];
+  const float logDecay = fmaxf(log2f(decay), -1e30f);
+  auto power = [&](int n) { return decay >= 0.f ? exp2f(float(n) * logDecay) : __int_as_float(0x7fc00000); };
+  for (int x = threadIdx.x; x < C + 20; x += THREADS) powers[x] = x < 16 ? 0.f : p.scale * power(x - 16);
+  const int sm0 = RT >= W ? warp * SM : warp / SPLIT, sn0 = RT >= W ? 0 : (warp % SPLIT) * SN;
+  float dS[SM][SN][4];
+#pragma unroll
+  for (int m = 0; m < SM; ++m)
+#pragma unroll
+    for (int n = 0; n < SN; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int i = (sm0 + m) * 16 + g + (x >> 1) * 8, j = (sn0 + n) * 8 + 2 * tq + (x & 1);
+        dS[m][n][x] = init && i < p.Dk && j < p.Dv ? init[int64_t(i) * p.Dv + j] : 0.f;
+      }
+
+  bool bad = false, anyReset = false, later = init != nullptr;   // later: X is not zero
+  for (int c = chunks - 1; c >= 0; --c) {
+    const int first = t0 + c * C, count = min(C, t1 - first);
+    loadTile<C, D, THREADS>(Q, q, p.qs.t, first, count, 0, p.Dk, p.vecQ);
+    loadTile<C, D, THREADS>(O, o, p.os.t, first, count, 0, p.Dv, p.vecO);
+    const int chunk = seg * (p.segmentLength / C) + c;
+    const bool earlier = OUT && (chunk > 0 || p.stateIn);          // S is not zero
+    if (OUT) {
+      loadTile<C, D, THREADS>(K, k, p.ks.t, first, count, 0, p.Dk, p.vecK);
+      loadTile<C, D, THREADS>(V, v, p.vs.t, first, count, 0, p.Dv, p.vecV);
+      if (chunk > 0) {
+        loadTile<D, D, THREADS>(S, p.saved + (eh * allChunks + chunk) * stateSize, p.Dv, 0, p.Dk, 0, p.Dv,
+                                p.Dv % 8 == 0);
+      } else if (p.stateIn) {
+        const float *from = p.stateIn + eh * stateSize;
+        for (int x = threadIdx.x; x < D * D / 2; x += THREADS) {
+          const int i = x / (D / 2), j = x % (D / 2) * 2;
+          const float low = i < p.Dk && j < p.Dv ? from[int64_t(i) * p.Dv + j] : 0.f;
+          const float high = i < p.Dk && j + 1 < p.Dv ? from[int64_t(i) * p.Dv + j + 1] : 0.f;
+          *reinterpret_cast<uint32_t *>(S + i * LD + j) = packPair(low, high);
+        }
+      }
+      if (later) {
+#pragma unroll
+        for (int m = 0; m < SM; ++m)
+#pragma unroll
+          for (int n = 0; n < SN; ++n)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              *reinterpret_cast<uint32_t *>(X + ((sm0 + m) * 16 + g + y * 8) * LD + (sn0 + n) * 8 + 2 * tq) =
+                  packPair(dS[m][n][2 * y], dS[m][n][2 * y + 1]);
+      }
+    }
+    commitCopies();
+    const unsigned long long mask = resetMask(p.resets, p.E, e, first, min(t1, first + C));
+    anyReset |= mask != 0;
+    waitCopies();
+    __syncthreads();
+    const int endPart = episodeOf(mask, 63);
+    const int part0 = episodeOf(mask, row + g), part1 = episodeOf(mask, row + g + 8);
+
+    if (OUT) {
+      const int blockRow = row / 16, blocks = (count + 15) / 16;
+      uint32_t a[D / 16][4];
+      float out[N][4];
+      // The scores of the warp's rows with a block of 16 other steps, times their decays; `sign` 1: the rows are
+      // the later steps.
+      auto weights = [&](uint32_t (&w)[4], const bf16 *other, int block, int sign) {
+        float s[2][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t b[4];
+          operandB<LD>(b, other, block * 16, kk * 16);
+          multiplyAdd(s[0], a[kk], b[0], b[1]);
+          multiplyAdd(s[1], a[kk], b[2], b[3]);
+        }
+        const float *f = powers + 16 + sign * (row - block * 16 + g - 2 * tq);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[n][x] *= f[sign * ((x >> 1) * 8 - (x & 1) - n * 8)];
+        if (mask) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (episodeOf(mask, block * 16 + n * 8 + 2 * tq + (x & 1)) != (x < 2 ? part0 : part1)) s[n][x] = 0.f;
+        }
+        w[0] = packPair(s[0][0], s[0][1]);
+        w[1] = packPair(s[0][2], s[0][3]);
+        w[2] = packPair(s[1][0], s[1][1]);
+        w[3] = packPair(s[1][2], s[1][3]);
+      };
+      auto accumulate = [&](const uint32_t (&w)[4], const bf16 *rows, int block) {
+#pragma unroll
+        for (int n = 0; n < N / 2; ++n) {
+          uint32_t b[4];
+          operandBTransposed<LD>(b, rows, block * 16, col + n * 16);
+          multiplyAdd(out[2 * n], w, b[0], b[1]);
+          multiplyAdd(out[2 * n + 1], w, b[2], b[3]);
+        }
+      };
+      auto rowsOfA = [&](const bf16 *x) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) operandA<LD>(a[kk], x, row, kk * 16);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) out[n][x] = 0.f;
+      };
+      auto scaleRows = [&](float f0, float f1) {   // a factor of zero replaces
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) out[n][x] = (x < 2 ? f0 : f1) == 0.f ? 0.f : out[n][x] * (x < 2 ? f0 : f1);
+      };
+      const int64_t stepK = int64_t(p.E) * p.H * p.Dk, stepV = int64_t(p.E) * p.H * p.Dv;
+      if (row < count) {
+        // dq
+        rowsOfA(O);
+        if (earlier) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int n = 0; n < N / 2; ++n) {
+              uint32_t b[4];
+              operandB<LD>(b, S, col + n * 16, kk * 16);
+              multiplyAdd(out[2 * n], a[kk], b[0], b[1]);
+              multiplyAdd(out[2 * n + 1], a[kk], b[2], b[3]);
+            }
+          scaleRows(part0 == 0 ? powers[16 + row + g + 1] : 0.f, part1 == 0 ? powers[16 + row + g + 9] : 0.f);
+        }
+        for (int block = 0; block <= blockRow; ++block) {
+          uint32_t w[4];
+          weights(w, V, block, 1);
+          accumulate(w, K, block);
+        }
+        bad |= notFinite(out);
+        storeTile(p.dq + eh * p.Dk, out, stepK, first, count, row, col, p.Dk);
+        // dv, dk
+        const int end0 = count - 1 - row - g, end1 = end0 - 8;
+        const float f0 = part0 == endPart && end0 >= 0 ? power(end0) : 0.f;
+        const float f1 = part1 == endPart && end1 >= 0 ? power(end1) : 0.f;
+        rowsOfA(K);
+        if (later) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int n = 0; n < N / 2; ++n) {
+              uint32_t b[4];
+              operandBTransposed<LD>(b, X, kk * 16, col + n * 16);
+              multiplyAdd(out[2 * n], a[kk], b[0], b[1]);
+              multiplyAdd(out[2 * n + 1], a[kk], b[2], b[3]);
+            }
+          scaleRows(f0, f1);
+        }
+        for (int block = blockRow; block < blocks; ++block) {
+          uint32_t w[4];
+          weights(w, Q, block, -1);
+          accumulate(w, O, block);
+        }
+        bad |= notFinite(out);
+        storeTile(p.dv + eh * p.Dv, out, stepV, first, count, row, col, p.Dv);
+        rowsOfA(V);
+        if (later) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int n = 0; n < N / 2; ++n) {
+              uint32_t b[4];
+              operandB<LD>(b, X, col + n * 16, kk * 16);
+              multiplyAdd(out[2 * n], a[kk], b[0], b[1]);
+              multiplyAdd(out[2 * n + 1], a[kk], b[2], b[3]);
+            }
+          scaleRows(f0, f1);
+        }
+        for (int block = blockRow; block < blocks; ++block) {
+          uint32_t w[4];
+          weights(w, O, block, -1);
+          accumulate(w, Q, block);
+        }
+        bad |= notFinite(out);
+        storeTile(p.dk + eh * p.Dk, out, stepK, first, count, row, col, p.Dk);
+      }
+    }
+
+    if (c > 0 || last) {
+      const float f = power(count);
+#pragma unroll
+      for (int m = 0; m < SM; ++m)
+#pragma unroll
+        for (int n = 0; n < SN; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) dS[m][n][x] = endPart == 0 ? dS[m][n][x] * f : 0.f;
+      for (int kk = 0; kk < (count + 15) / 16; ++kk) {
+        float w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int i = kk * 16 + 2 * tq + (x & 1) + (x >> 1) * 8;
+          w[x] = episodeOf(mask, i) == 0 ? powers[16 + i + 1] : 0.f;
+        }
+#pragma unroll
+        for (int m = 0; m < SM; ++m) {
+          uint32_t a[4], high[4], low[4];
+          operandATransposed<LD>(a, Q, (sm0 + m) * 16, kk * 16);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float l = lowOf(a[x]) * w[(x >> 1) * 2], u = highOf(a[x]) * w[(x >> 1) * 2 + 1];
+            high[x] = packPair(l, u);
+            low[x] = packPair(l - lowOf(high[x]), u - highOf(high[x]));
+          }
+#pragma unroll
+          for (int n = 0; n < SN / 2; ++n) {
+            uint32_t b[4];
+            operandBTransposed<LD>(b, O, kk * 16, (sn0 + 2 * n) * 8);
+            multiplyAdd(dS[m][2 * n], high, b[0], b[1]);
+            multiplyAdd(dS[m][2 * n + 1], high, b[2], b[3]);
+            multiplyAdd(dS[m][2 * n], low, b[0], b[1]);
+            multiplyAdd(dS[m][2 * n + 1], low, b[2], b[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < SM; ++m) bad |= notFinite(dS[m]);
+      later = true;
+      __syncthreads();   // the tiles and X are free
+    }
+  }
+  if (!OUT && threadIdx.x == 0) p.segmentCut[eh * p.segmentCount + seg] = anyReset;
+  if (OUT) {
+    const bool redo = __syncthreads_or(bad);
+    if (threadIdx.x == 0) p.flags[eh * p.segmentCount + seg] = redo;
+  }
+  if (last) {
+#pragma unroll
+    for (int m = 0; m < SM; ++m)
+#pragma unroll
+      for (int n = 0; n < SN; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int i = (sm0 + m) * 16 + g + (x >> 1) * 8, j = (sn0 + n) * 8 + 2 * tq + (x & 1);
+          if (i < p.Dk && j < p.Dv) last[int64_t(i) * p.Dv + j] = dS[m][n][x];
+        }
+  }
+}
+
+// States at the segments' ends that a sweep enters them by, from what each
+// segment adds, in place: forwards in time from `init`, or backwards.  The
+// last segment of the sweep adds nothing that is needed.
+__global__ void __launch_bounds__(256) joinSegments(float *segments, const uint8_t *cut, const float *init,
+                                                    const float *decay, int H, int T, int segmentCount,
+                                                    int segmentLength, int64_t stateSize, int reverse) {
+  const int64_t eh = blockIdx.x, x = int64_t(blockIdx.y) * blockDim.x + threadIdx.x;
+  if (x >= stateSize) return;
+  const float d = decay[eh % H], logDecay = fmaxf(log2f(d), -1e30f);
+  float S = init ? init[eh * stateSize + x] : 0.f;
+  for (int u = 0; u < segmentCount; ++u) {
+    const int s = reverse ? segmentCount - 1 - u : u;
+    float *at = segments + (eh * segmentCount + s) * stateSize + x;
+    const bool final = u + 1 == segmentCount;
+    const float added = final ? 0.f : *at;
+    *at = S;
+    if (final) break;
+    const int length = min(segmentLength, T - s * segmentLength);
+    const float f = d >= 0.f ? exp2f(float(length) * logDecay) : __int_as_float(0x7fc00000);
+    S = cut[eh * segmentCount + s] ? added : fmaf(f, S, added);
+  }
+}
+
+// Sweeps of a call step by step, for the environments and heads that have one of
+// their `count` flags set.
+template <int DI> __global__ void __launch_bounds__(128) redoAttention(Sweep s, const uint8_t *flags, int count) {
+  const int64_t all = int64_t(s.E) * s.H;
+  for (int64_t eh = blockIdx.x; eh < all; eh += gridDim.x) {
+    bool any = false;
+    for (int x = threadIdx.x; x < count; x += blockDim.x) any |= flags[eh * count + x] != 0;
+    if (__syncthreads_or(any)) scanSteps<bf16, DI>(s, eh, blockIdx.y * blockDim.x + threadIdx.x);
+  }
+}
+
+}  // namespace duckb200

@@ -44,12 +44,10 @@ constexpr int kScanSteps = 16;
 
 // One thread per column of the state, its DI rows in registers; the rows'
 // operands of 16 steps at a time in shared memory.
-template <class T, int DI> __global__ void __launch_bounds__(128) attentionScan(Sweep s) {
+template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int j) {
   __shared__ __align__(16) float a[kScanSteps][DI], c[kScanSteps][DI];
   __shared__ uint8_t cut[kScanSteps];
-  const int64_t eh = blockIdx.x;
   const int e = int(eh / s.H), h = int(eh - int64_t(e) * s.H);
-  const int j = blockIdx.y * blockDim.x + threadIdx.x;
   const bool live = j < s.Dj;
   const T *pa = static_cast<const T *>(s.a) + e * s.as.e + h * s.as.h;
   const T *pb = static_cast<const T *>(s.b) + e * s.bs.e + h * s.bs.h + (live ? j : 0);
@@ -101,6 +99,10 @@ template <class T, int DI> __global__ void __launch_bounds__(128) attentionScan(
     for (int i = 0; i < DI; ++i)
       if (i < s.Di) s.last[base + int64_t(i) * s.ri + int64_t(j) * s.rj] = gone ? 0.f : f * x[i];
   }
+}
+
+template <class T, int DI> __global__ void __launch_bounds__(128) attentionScan(Sweep s) {
+  scanSteps<T, DI>(s, blockIdx.x, blockIdx.y * blockDim.x + threadIdx.x);
 }
 
 struct StepOf {

@@ -1,5 +1,6 @@
 // C entries of the operators of a policy with memory (declared in
 // include/duck_b200.h): argument checks, the choice of a kernel, launches.
+#include "attention_chunks.cuh"
 #include "capi.hpp"
 #include "checkpoint8.cuh"
 #include "layer_norm.cuh"
@@ -52,6 +53,195 @@ template <class T> void launchScan(const Sweep &s, cudaStream_t stream) {
   else if (s.Di <= 64) attentionScan<T, 64><<<grid, threads, 0, stream>>>(s);
   else attentionScan<T, 128><<<grid, threads, 0, stream>>>(s);
   check(cudaGetLastError(), "linear attention launch");
+}
+
+template <int DI> void launchRedo(const Sweep &s, const uint8_t *flags, int count, cudaStream_t stream) {
+  const int threads = std::min(128, int(ceilDiv(s.Dj, 32)) * 32);
+  const dim3 grid(unsigned(std::min<int64_t>(int64_t(s.E) * s.H, 296)), unsigned(ceilDiv(s.Dj, threads)));
+  redoAttention<DI><<<grid, threads, 0, stream>>>(s, flags, count);
+  check(cudaGetLastError(), "linear attention launch");
+}
+void launchRedo(const Sweep &s, const uint8_t *flags, int count, cudaStream_t stream) {
+  if (s.Di <= 32) launchRedo<32>(s, flags, count, stream);
+  else launchRedo<128>(s, flags, count, stream);
+}
+
+Sweep forwardSweep(const duck_attention &a) {
+  return {a.k, a.v, a.q, a.out, rowsOf(a.k_stride), rowsOf(a.v_stride), rowsOf(a.q_stride), a.state_in, a.state_out,
+          a.decay, a.resets, a.T, a.E, a.H, a.Dk, a.Dv, a.Dv, 1, 0, 1.f, a.scale};
+}
+Sweep gradientOfQ(const duck_attention &a) {
+  return {a.v, a.k, a.dout, a.dq, rowsOf(a.v_stride), rowsOf(a.k_stride), rowsOf(a.dout_stride), a.state_in, nullptr,
+          a.decay, a.resets, a.T, a.E, a.H, a.Dv, a.Dk, 1, a.Dv, 0, 1.f, a.scale};
+}
+Sweep gradientOfK(const duck_attention &a) {
+  return {a.dout, a.q, a.v, a.dk, rowsOf(a.dout_stride), rowsOf(a.q_stride), rowsOf(a.v_stride), a.dstate_out, nullptr,
+          a.decay, a.resets, a.T, a.E, a.H, a.Dv, a.Dk, 1, a.Dv, 1, a.scale, 1.f};
+}
+Sweep gradientOfV(const duck_attention &a) {   // and of the state
+  return {a.q, a.dout, a.k, a.dv, rowsOf(a.q_stride), rowsOf(a.dout_stride), rowsOf(a.k_stride), a.dstate_out,
+          a.dstate_in, a.decay, a.resets, a.T, a.E, a.H, a.Dk, a.Dv, a.Dv, 1, 1, a.scale, 1.f};
+}
+
+// How a forward or backward call in bfloat16 is laid out.
+struct ChunkPlan {
+  int C, columnTiles, segmentLength, segmentCount, chunks;
+  int64_t stateSize, segmentBytes, cutBytes, flagBytes;   // of the scratch, in this order
+};
+ChunkPlan planChunks(const duck_attention &a) {
+  ChunkPlan p{};
+  p.C = a.T <= 32 ? 32 : 64;
+  p.columnTiles = int(ceilDiv(a.Dv, 64));
+  p.chunks = int(ceilDiv(a.T, p.C));
+  p.stateSize = int64_t(a.Dk) * a.Dv;
+  const int64_t blocks = int64_t(a.E) * a.H * p.columnTiles;
+  const int64_t want = blocks < 296 ? std::min<int64_t>(ceilDiv(p.chunks, 4), ceilDiv(444, blocks)) : 1;
+  p.segmentLength = int(ceilDiv(p.chunks, std::max<int64_t>(1, want))) * p.C;
+  p.segmentCount = std::max(1, int(ceilDiv(a.T, p.segmentLength ? p.segmentLength : 1)));
+  const int64_t states = int64_t(a.E) * a.H * p.segmentCount;
+  if (p.segmentCount > 1) {
+    p.segmentBytes = states * p.stateSize * 4;
+    p.cutBytes = states;
+  }
+  p.flagBytes = states * p.columnTiles;   // the backward call needs one a segment only
+  return p;
+}
+
+bool dense16(const void *base, const int64_t *strides, int width) {
+  return reinterpret_cast<uintptr_t>(base) % 16 == 0 && strides[0] % 8 == 0 && strides[1] % 8 == 0 &&
+         strides[2] % 8 == 0 && width % 8 == 0;
+}
+
+// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device.
+template <auto kernel> void allowShared(int bytes) {
+  static bool done[64] = {};
+  int device = 0;
+  check(cudaGetDevice(&device), "cudaGetDevice");
+  if (device < 64 && done[device]) return;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  if (device < 64) done[device] = true;
+}
+
+template <int C, int DK, int DV, bool OUT>
+void launchChunks(const ChunkArgs &a, int segments, int buffers, cudaStream_t stream) {
+  const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(segments * a.columnTiles));
+  constexpr auto kernel = attentionChunks<C, DK, DV, OUT>;
+  constexpr int most = chunkSharedBytes<C, DK, DV, OUT>(2);
+  if constexpr (most > 48 * 1024) allowShared<kernel>(most);
+  kernel<<<grid, C * 2, chunkSharedBytes<C, DK, DV, OUT>(buffers), stream>>>(a, buffers);
+  check(cudaGetLastError(), "linear attention launch");
+}
+template <int C, bool OUT> void launchChunks(const ChunkArgs &a, int segments, int buffers, cudaStream_t stream) {
+  const bool narrow = a.Dv <= 32;
+  if (a.Dk <= 32) narrow ? launchChunks<C, 32, 32, OUT>(a, segments, buffers, stream)
+                         : launchChunks<C, 32, 64, OUT>(a, segments, buffers, stream);
+  else if (a.Dk <= 64) narrow ? launchChunks<C, 64, 32, OUT>(a, segments, buffers, stream)
+                              : launchChunks<C, 64, 64, OUT>(a, segments, buffers, stream);
+  else narrow ? launchChunks<C, 128, 32, OUT>(a, segments, buffers, stream)
+              : launchChunks<C, 128, 64, OUT>(a, segments, buffers, stream);
+}
+
+void forwardChunks(const duck_attention &a, cudaStream_t stream) {
+  const ChunkPlan plan = planChunks(a);
+  const bool split = plan.segmentCount > 1;
+  require(a.scratch, "Invalid arguments");
+  ChunkArgs c{};
+  c.q = static_cast<const bf16 *>(a.q);
+  c.k = static_cast<const bf16 *>(a.k);
+  c.v = static_cast<const bf16 *>(a.v);
+  c.out = static_cast<bf16 *>(a.out);
+  c.qs = rowsOf(a.q_stride);
+  c.ks = rowsOf(a.k_stride);
+  c.vs = rowsOf(a.v_stride);
+  c.decay = a.decay;
+  c.resets = a.resets;
+  c.stateIn = a.state_in;
+  c.stateOut = a.state_out;
+  c.saved = static_cast<bf16 *>(a.saved);
+  c.T = a.T, c.E = a.E, c.H = a.H, c.Dk = a.Dk, c.Dv = a.Dv;
+  c.segmentLength = plan.segmentLength;
+  c.segmentCount = plan.segmentCount;
+  c.columnTiles = plan.columnTiles;
+  c.vecQ = dense16(a.q, a.q_stride, a.Dk);
+  c.vecK = dense16(a.k, a.k_stride, a.Dk);
+  c.vecV = dense16(a.v, a.v_stride, a.Dv);
+  c.scale = a.scale;
+  c.flags = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes + plan.cutBytes;
+  const int buffers = std::min(plan.chunks, plan.segmentLength / plan.C) > 1 ? 2 : 1;
+  if (split) {
+    c.segments = a.scratch;
+    c.segmentCut = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes;
+    launchChunks<64, false>(c, plan.segmentCount - 1, buffers, stream);
+    const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(ceilDiv(plan.stateSize, 256)));
+    joinSegments<<<grid, 256, 0, stream>>>(c.segments, c.segmentCut, a.state_in, a.decay, a.H, a.T, plan.segmentCount,
+                                           plan.segmentLength, plan.stateSize, 0);
+    check(cudaGetLastError(), "linear attention launch");
+  }
+  if (plan.C == 32) launchChunks<32, true>(c, plan.segmentCount, buffers, stream);
+  else launchChunks<64, true>(c, plan.segmentCount, buffers, stream);
+  launchRedo(forwardSweep(a), c.flags, plan.segmentCount * plan.columnTiles, stream);
+}
+
+template <int C, int D, bool OUT> void launchBackward(const BackwardArgs &a, int segments, cudaStream_t stream) {
+  const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(segments));
+  constexpr auto kernel = attentionChunksBackward<C, D, OUT>;
+  constexpr int bytes = backwardSharedBytes<C, D, OUT>();
+  if constexpr (bytes > 48 * 1024) allowShared<kernel>(bytes);
+  kernel<<<grid, backwardWarps<C, D, OUT>() * 32, bytes, stream>>>(a);
+  check(cudaGetLastError(), "linear attention backward launch");
+}
+template <int C, bool OUT> void launchBackward(const BackwardArgs &a, int segments, cudaStream_t stream) {
+  const int d = std::max(a.Dk, a.Dv);
+  if (d <= 32) launchBackward<C, 32, OUT>(a, segments, stream);
+  else if (d <= 64) launchBackward<C, 64, OUT>(a, segments, stream);
+  else launchBackward<C, 128, OUT>(a, segments, stream);
+}
+
+void backwardChunks(const duck_attention &a, cudaStream_t stream) {
+  const ChunkPlan plan = planChunks(a);
+  const bool split = plan.segmentCount > 1;
+  require(a.scratch && (plan.chunks <= 1 || a.saved), "Invalid arguments");
+  BackwardArgs c{};
+  c.q = static_cast<const bf16 *>(a.q);
+  c.k = static_cast<const bf16 *>(a.k);
+  c.v = static_cast<const bf16 *>(a.v);
+  c.dout = static_cast<const bf16 *>(a.dout);
+  c.dq = static_cast<bf16 *>(a.dq);
+  c.dk = static_cast<bf16 *>(a.dk);
+  c.dv = static_cast<bf16 *>(a.dv);
+  c.qs = rowsOf(a.q_stride);
+  c.ks = rowsOf(a.k_stride);
+  c.vs = rowsOf(a.v_stride);
+  c.os = rowsOf(a.dout_stride);
+  c.decay = a.decay;
+  c.resets = a.resets;
+  c.stateIn = a.state_in;
+  c.dstateOut = a.dstate_out;
+  c.dstateIn = a.dstate_in;
+  c.saved = static_cast<const bf16 *>(a.saved);
+  c.T = a.T, c.E = a.E, c.H = a.H, c.Dk = a.Dk, c.Dv = a.Dv;
+  c.segmentLength = plan.segmentLength;
+  c.segmentCount = plan.segmentCount;
+  c.vecQ = dense16(a.q, a.q_stride, a.Dk);
+  c.vecK = dense16(a.k, a.k_stride, a.Dk);
+  c.vecV = dense16(a.v, a.v_stride, a.Dv);
+  c.vecO = dense16(a.dout, a.dout_stride, a.Dv);
+  c.scale = a.scale;
+  c.flags = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes + plan.cutBytes;
+  if (split) {
+    c.segments = a.scratch;
+    c.segmentCut = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes;
+    launchBackward<64, false>(c, plan.segmentCount - 1, stream);
+    const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(ceilDiv(plan.stateSize, 256)));
+    joinSegments<<<grid, 256, 0, stream>>>(c.segments, c.segmentCut, a.dstate_out, a.decay, a.H, a.T,
+                                           plan.segmentCount, plan.segmentLength, plan.stateSize, 1);
+    check(cudaGetLastError(), "linear attention backward launch");
+  }
+  if (plan.C == 32) launchBackward<32, true>(c, plan.segmentCount, stream);
+  else launchBackward<64, true>(c, plan.segmentCount, stream);
+  launchRedo(gradientOfQ(a), c.flags, plan.segmentCount, stream);
+  launchRedo(gradientOfK(a), c.flags, plan.segmentCount, stream);
+  launchRedo(gradientOfV(a), c.flags, plan.segmentCount, stream);
 }
 
 }  // namespace
@@ -149,8 +339,11 @@ int duck_elu_restore(const void *dy, const int8_t *codes, const float *scales, v
 int duck_linear_attention_sizes(const duck_attention *args, int64_t *out) {
   return guarded([&] {
     require(out != nullptr, "Invalid arguments");
-    attentionChecked(args);
     out[0] = out[1] = out[2] = 0;
+    if (!attentionChecked(args) || args->type != DUCK_BFLOAT16 || args->T == 0) return;
+    const ChunkPlan plan = planChunks(*args);
+    out[0] = out[1] = plan.segmentBytes + plan.cutBytes + plan.flagBytes;
+    out[2] = plan.chunks > 1 ? int64_t(args->E) * args->H * plan.chunks * plan.stateSize * 2 : 0;
   });
 }
 
@@ -159,8 +352,11 @@ int duck_linear_attention_forward(const duck_attention *args, duck_stream stream
     if (!attentionChecked(args)) return;
     const duck_attention &a = *args;
     require(a.decay && (a.T == 0 || (a.q && a.k && a.v && a.out)), "Invalid arguments");
-    Sweep s{a.k, a.v, a.q, a.out, rowsOf(a.k_stride), rowsOf(a.v_stride), rowsOf(a.q_stride), a.state_in, a.state_out,
-            a.decay, a.resets, a.T, a.E, a.H, a.Dk, a.Dv, a.Dv, 1, 0, 1.f, a.scale};
+    if (a.type == DUCK_BFLOAT16 && a.T > 0) {
+      forwardChunks(a, reinterpret_cast<cudaStream_t>(stream));
+      return;
+    }
+    const Sweep s = forwardSweep(a);
     withType(a.type, [&](auto zero) { launchScan<decltype(zero)>(s, reinterpret_cast<cudaStream_t>(stream)); });
   });
 }
@@ -170,18 +366,15 @@ int duck_linear_attention_backward(const duck_attention *args, duck_stream strea
     if (!attentionChecked(args)) return;
     const duck_attention &a = *args;
     require(a.decay && (a.T == 0 || (a.q && a.k && a.v && a.dout && a.dq && a.dk && a.dv)), "Invalid arguments");
-    const Rows q = rowsOf(a.q_stride), k = rowsOf(a.k_stride), v = rowsOf(a.v_stride), o = rowsOf(a.dout_stride);
-    const Sweep dq{a.v, a.k, a.dout, a.dq, v, k, o, a.state_in, nullptr, a.decay, a.resets,
-                   a.T, a.E, a.H, a.Dv, a.Dk, 1, a.Dv, 0, 1.f, a.scale};
-    const Sweep dk{a.dout, a.q, a.v, a.dk, o, q, v, a.dstate_out, nullptr, a.decay, a.resets,
-                   a.T, a.E, a.H, a.Dv, a.Dk, 1, a.Dv, 1, a.scale, 1.f};
-    const Sweep dv{a.q, a.dout, a.k, a.dv, q, o, k, a.dstate_out, a.dstate_in, a.decay, a.resets,
-                   a.T, a.E, a.H, a.Dk, a.Dv, a.Dv, 1, 1, a.scale, 1.f};
+    if (a.type == DUCK_BFLOAT16 && a.T > 0) {
+      backwardChunks(a, reinterpret_cast<cudaStream_t>(stream));
+      return;
+    }
     withType(a.type, [&](auto zero) {
       using T = decltype(zero);
-      launchScan<T>(dq, reinterpret_cast<cudaStream_t>(stream));
-      launchScan<T>(dk, reinterpret_cast<cudaStream_t>(stream));
-      launchScan<T>(dv, reinterpret_cast<cudaStream_t>(stream));
+      launchScan<T>(gradientOfQ(a), reinterpret_cast<cudaStream_t>(stream));
+      launchScan<T>(gradientOfK(a), reinterpret_cast<cudaStream_t>(stream));
+      launchScan<T>(gradientOfV(a), reinterpret_cast<cudaStream_t>(stream));
     });
   });
 }

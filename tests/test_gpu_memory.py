@@ -240,6 +240,24 @@ def test_attention_strides(D, dtype):
     assert ref.error(grad, want[3].sum(2, keepdim=True)) <= ref.bound(dtype, 1000, 6)
 
 
+def test_attention_of_many_heads_that_are_not_finite():
+    T, E, H, D = 40, 250, 2, 16
+    q, k, v, decay, S, _, do, _ = attention_case(37, T, E, H, D, D, torch.bfloat16, state=False)
+    r = torch.zeros(T, E, dtype=torch.bool)
+    r[20] = True
+    want = ref.attention(q, k, v, decay, None, r, D ** -0.5, do)
+    v = v.clone()
+    v[3] = float("inf")
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    o, last = memory.linear_attention(*leaves, decay.cuda(), None, r.cuda())
+    grads = torch.autograd.grad(o, leaves, do.cuda())
+    tol = ref.bound(torch.bfloat16, 1000, 4)
+    assert ref.error(o[:3], want[0][:3]) <= tol and ref.error(o[20:], want[0][20:]) <= tol
+    assert ref.error(last, want[1]) <= STATE
+    for got, exact in zip(grads, want[2:5]):
+        assert ref.error(got[20:], exact[20:]) <= tol
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T", [24, 150, 900])
 def test_attention_keeps_episodes_and_the_future_apart(T, dtype):
