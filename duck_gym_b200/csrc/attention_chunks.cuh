@@ -35,6 +35,8 @@
 #include "linear_attention.cuh"
 #include "tensor_tiles.cuh"
 
+#include <type_traits>
+
 namespace duckb200 {
 
 struct ChunkArgs {
@@ -52,6 +54,7 @@ struct ChunkArgs {
   int T, E, H, Dk, Dv;
   int segmentLength, segmentCount, columnTiles;
   int vecQ, vecK, vecV;        // rows can be read in 16-byte pieces
+  int precise;                 // the state is an output: its operand is split in two
   float scale;
 };
 
@@ -64,8 +67,16 @@ __device__ __forceinline__ unsigned long long resetMask(const uint8_t *resets, i
   const unsigned low = __ballot_sync(0xffffffffu, a), high = __ballot_sync(0xffffffffu, b);
   return (static_cast<unsigned long long>(high) << 32) | low;
 }
-// Number of resets at steps 0..i: steps of one number are of one episode.
-__device__ __forceinline__ int episodeOf(unsigned long long mask, int i) { return __popcll(mask & (~0ull >> (63 - i))); }
+// Last step of a chunk up to i at which an episode begins, or -1: step i sees the
+// steps from there on, and the state before the chunk if there is none.
+__device__ __forceinline__ int episodeStart(unsigned long long mask, int i) {
+  return 63 - __clzll(static_cast<long long>(mask & (~0ull >> (63 - i))));
+}
+// First step after j at which an episode begins: the steps before it see step j.
+__device__ __forceinline__ int episodeEnd(unsigned long long mask, int j) {
+  const unsigned long long after = mask & ~(~0ull >> (63 - j));
+  return after ? __ffsll(static_cast<long long>(after)) - 1 : 1 << 30;
+}
 
 // Rows t0.. (count of them, the rest zero) of an operand, columns c0..c0+D-1
 // (those from `width` on zero), into a tile of C rows.
@@ -74,12 +85,15 @@ __device__ __forceinline__ void loadTile(bf16 *tile, const bf16 *base, int64_t s
                                          int width, bool vec) {
   constexpr int L = D + 8;
   if (vec) {
-    constexpr int pieces = D / 8;
+    constexpr int pieces = D / 8, rows = THREADS / pieces;   // rows that the block's threads copy at once
+    const int r0 = threadIdx.x / pieces, c = (threadIdx.x % pieces) * 8;
+    const bool inside = c0 + c < width;
+    const bf16 *from = base + int64_t(t0 + r0) * stride + c0 + c;
 #pragma unroll
-    for (int x = 0; x < C * pieces / THREADS; ++x) {
-      const int id = x * THREADS + threadIdx.x, r = id / pieces, c = (id % pieces) * 8;
-      const bool valid = r < count && c0 + c < width;
-      copyAsync16(tile + r * L + c, valid ? base + int64_t(t0 + r) * stride + c0 + c : base, valid);
+    for (int x = 0; x < C / rows; ++x) {
+      const bool valid = inside && r0 + x * rows < count;
+      copyAsync16(tile + (r0 + x * rows) * L + c, valid ? from : base, valid);
+      from += rows * stride;
     }
   } else {
     for (int id = threadIdx.x; id < C * D; id += THREADS) {
@@ -87,6 +101,144 @@ __device__ __forceinline__ void loadTile(bf16 *tile, const bf16 *base, int64_t s
       tile[r * L + c] = r < count && c0 + c < width ? base[int64_t(t0 + r) * stride + c0 + c] : fromFloat<bf16>(0.f);
     }
   }
+}
+
+// Rows of 16 steps by N tiles of 8 columns of a dense [T, E, H, width] output,
+// as the products leave them: lane 4 g + q has columns 2 q and 2 q + 1 of row g
+// (and g + 8) of each tile.  Where rows are whole 16-byte pieces, the four lanes
+// of a row exchange their pairs of four tiles (a 4 x 4 transpose, two rounds),
+// so that each stores all of one tile: 64 bytes of a row at a time.
+template <int N>
+__device__ __forceinline__ void storeTile(bf16 *out, const float (&x)[N][4], int64_t stepStride, int first, int count,
+                                          int row0, int col0, int width) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  if (N % 4 == 0 && width % 8 == 0) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int i = row0 + g + y * 8;
+      bf16 *to = out + int64_t(first + i) * stepStride + col0 + tq * 8;
+#pragma unroll
+      for (int n = 0; n < N / 4 * 4; n += 4) {
+        uint32_t p[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) p[m] = packPair(x[n + m][2 * y], x[n + m][2 * y + 1]);
+        const bool odd = tq & 1, upper = tq & 2;
+        const uint32_t a = __shfl_xor_sync(0xffffffffu, odd ? p[0] : p[1], 1);
+        const uint32_t b = __shfl_xor_sync(0xffffffffu, odd ? p[2] : p[3], 1);
+        // Of tiles (0, 2) + odd: columns of the lower and the upper lane of the pair.
+        const uint32_t l0 = odd ? a : p[0], u0 = odd ? p[1] : a, l2 = odd ? b : p[2], u2 = odd ? p[3] : b;
+        const uint32_t c = __shfl_xor_sync(0xffffffffu, upper ? l0 : l2, 2);
+        const uint32_t d = __shfl_xor_sync(0xffffffffu, upper ? u0 : u2, 2);
+        const uint4 whole = upper ? make_uint4(c, d, l2, u2) : make_uint4(l0, u0, c, d);
+        if (i < count && col0 + (n + tq) * 8 < width) *reinterpret_cast<uint4 *>(to + n * 8) = whole;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int i = row0 + g + y * 8, j = col0 + n * 8 + 2 * tq;
+      if (i >= count) continue;
+      bf16 *to = out + int64_t(first + i) * stepStride + j;
+      if (j + 1 < width && width % 2 == 0) *reinterpret_cast<uint32_t *>(to) = packPair(x[n][2 * y], x[n][2 * y + 1]);
+      else {
+        if (j < width) to[0] = fromFloat<bf16>(x[n][2 * y]);
+        if (j + 1 < width) to[1] = fromFloat<bf16>(x[n][2 * y + 1]);
+      }
+    }
+}
+
+template <int N> __device__ __forceinline__ bool notFinite(const float (&x)[N][4]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) sum = fmaf(x[n][y], 0.f, sum);
+  return sum != 0.f;
+}
+
+// A float32 state [rows, width] (from column c0 on, D columns) as a bfloat16 tile.
+template <int DK, int D, int THREADS>
+__device__ __forceinline__ void loadState(bf16 *tile, const float *from, int rows, int c0, int width) {
+  constexpr int L = D + 8, quads = D / 4;
+  if (width % 4 == 0) {
+#pragma unroll 4
+    for (int id = threadIdx.x; id < DK * quads; id += THREADS) {
+      const int i = id / quads, j = (id % quads) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (from && i < rows && c0 + j < width) v = *reinterpret_cast<const float4 *>(from + int64_t(i) * width + c0 + j);
+      *reinterpret_cast<uint2 *>(tile + i * L + j) = make_uint2(packPair(v.x, v.y), packPair(v.z, v.w));
+    }
+  } else {
+    for (int id = threadIdx.x; id < DK * D; id += THREADS) {
+      const int i = id / D, j = id % D;
+      tile[i * L + j] = fromFloat<bf16>(from && i < rows && c0 + j < width ? from[int64_t(i) * width + c0 + j] : 0.f);
+    }
+  }
+}
+
+// The warp's slice of a float32 state: row tiles of 16 from m0 on by column tiles
+// of 8 from n0 on (of those from column c0 of the state on).
+template <int SM, int SN>
+__device__ __forceinline__ void readSlice(float (&S)[SM][SN][4], const float *from, int m0, int n0, int c0, int rows,
+                                          int width) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int m = 0; m < SM; ++m)
+#pragma unroll
+    for (int n = 0; n < SN; ++n)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int i = (m0 + m) * 16 + g + y * 8, j = c0 + (n0 + n) * 8 + 2 * tq;
+        float2 v = make_float2(0.f, 0.f);
+        if (from && i < rows) {
+          const float *at = from + int64_t(i) * width + j;
+          if (width % 2 == 0) {
+            if (j < width) v = *reinterpret_cast<const float2 *>(at);
+          } else {
+            if (j < width) v.x = at[0];
+            if (j + 1 < width) v.y = at[1];
+          }
+        }
+        S[m][n][2 * y] = v.x;
+        S[m][n][2 * y + 1] = v.y;
+      }
+}
+template <int SM, int SN>
+__device__ __forceinline__ void writeSlice(float *to, const float (&S)[SM][SN][4], int m0, int n0, int c0, int rows,
+                                           int width) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int m = 0; m < SM; ++m)
+#pragma unroll
+    for (int n = 0; n < SN; ++n)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int i = (m0 + m) * 16 + g + y * 8, j = c0 + (n0 + n) * 8 + 2 * tq;
+        if (i >= rows) continue;
+        float *at = to + int64_t(i) * width + j;
+        if (width % 2 == 0) {
+          if (j < width) *reinterpret_cast<float2 *>(at) = make_float2(S[m][n][2 * y], S[m][n][2 * y + 1]);
+        } else {
+          if (j < width) at[0] = S[m][n][2 * y];
+          if (j + 1 < width) at[1] = S[m][n][2 * y + 1];
+        }
+      }
+}
+// ... and its bfloat16 copy in a tile with rows of L.
+template <int L, int SM, int SN>
+__device__ __forceinline__ void copySlice(bf16 *tile, const float (&S)[SM][SN][4], int m0, int n0) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int m = 0; m < SM; ++m)
+#pragma unroll
+    for (int n = 0; n < SN; ++n)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        *reinterpret_cast<uint32_t *>(tile + ((m0 + m) * 16 + g + y * 8) * L + (n0 + n) * 8 + 2 * tq) =
+            packPair(S[m][n][2 * y], S[m][n][2 * y + 1]);
 }
 
 // Shared memory of a block: tiles in `buffers` copies.
@@ -98,9 +250,11 @@ template <int C, int DK, int DV, bool OUT> constexpr int chunkSharedBytes(int bu
 }
 
 // One block per (environment, head), segment of T and tile of DV columns; C / 16
-// warps.  OUT = false computes the state at the segment's end only.
-template <int C, int DK, int DV, bool OUT>
-__global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionChunks(ChunkArgs p, int buffers) {
+// warps.  OUT = false computes the state at the segment's end only; STATE = false
+// is for one chunk whose last state nobody wants.
+template <int C, int DK, int DV, bool OUT, bool STATE>
+__global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) / C)
+    attentionChunks(ChunkArgs p, int buffers) {
   constexpr int W = C / 16, THREADS = W * 32, LQ = DK + 8, LV = DV + 8;
   constexpr int RT = DK / 16;                                  // row tiles of the state
   constexpr int SM = RT >= W ? RT / W : 1;                     // of which a warp has
@@ -134,7 +288,17 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionC
     if (OUT) loadTile<C, DK, THREADS>(tile + C * (LQ + LV), q, p.qs.t, first, count, 0, p.Dk, p.vecQ);
     commitCopies();
   };
-  if (chunks > 0) load(0, 0);
+  load(0, 0);
+
+  // The warp's slice of the state, and its copy.
+  const int sm0 = RT >= W ? warp * SM : warp / SPLIT, sn0 = RT >= W ? 0 : (warp % SPLIT) * SN;
+  float S[SM][SN][4];
+  if (STATE) {
+    readSlice(S, init, sm0, sn0, col0, p.Dk, p.Dv);
+    if (OUT) copySlice<LV>(copies, S, sm0, sn0);
+  } else if (init) {
+    loadState<DK, DV, THREADS>(copies, init, p.Dk, col0, p.Dv);
+  }
 
   // Powers of the decay.
   const float decay = p.decay[h];
@@ -153,36 +317,13 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionC
       const int d = g + (x >> 1) * 8 - (2 * tq + (x & 1) + 8 * n);
       inBlock[n][x] = d >= 0 ? p.scale * power(d) : 0.f;
     }
-  const float fromStart = p.scale * power(16 * warp + 1);   // of the warp's first step to S
+  const int i0 = 16 * warp;
+  const float fromStart = p.scale * power(i0 + 1);   // of the warp's first step to S
   const float row0 = power(g), row1 = power(g + 8);
   const float fullChunk = power(C);
 
-  // The warp's slice of the state.
-  const int sm0 = RT >= W ? warp * SM : warp / SPLIT, sn0 = RT >= W ? 0 : (warp % SPLIT) * SN;
-  float S[SM][SN][4];
-#pragma unroll
-  for (int m = 0; m < SM; ++m)
-#pragma unroll
-    for (int n = 0; n < SN; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int i = (sm0 + m) * 16 + g + (x >> 1) * 8, j = col0 + (sn0 + n) * 8 + 2 * tq + (x & 1);
-        S[m][n][x] = init && i < p.Dk && j < p.Dv ? init[int64_t(i) * p.Dv + j] : 0.f;
-      }
-  auto copyState = [&](int buffer) {
-    bf16 *copy = copies + buffer * DK * LV;
-#pragma unroll
-    for (int m = 0; m < SM; ++m)
-#pragma unroll
-      for (int n = 0; n < SN; ++n)
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-          *reinterpret_cast<uint32_t *>(copy + ((sm0 + m) * 16 + g + y * 8) * LV + (sn0 + n) * 8 + 2 * tq) =
-              packPair(S[m][n][2 * y], S[m][n][2 * y + 1]);
-  };
-  if (OUT) copyState(0);
-
-  bool bad = false, anyReset = false;
+  float finite = 0.f;
+  bool anyReset = false, later = init != nullptr;   // later: S is not zero
   for (int c = 0; c < chunks; ++c) {
     const int buffer = buffers > 1 ? c & 1 : 0, first = t0 + c * C, count = min(C, t1 - first);
     const unsigned long long mask = resetMask(p.resets, p.E, e, first, min(t1, first + C));
@@ -191,18 +332,25 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionC
     __syncthreads();
     if (c + 1 < chunks) load(c + 1, (c + 1) & 1);
     const bf16 *K = tiles + buffer * chunkTileElements<C, DK, DV, OUT>(), *V = K + C * LQ, *Q = V + C * LV;
-    if (count < C)
+    if (STATE && count < C)
       for (int x = threadIdx.x; x < C; x += THREADS) toEnd[x] = x < count ? power(count - 1 - x) : 0.f;
 
     if (OUT) {
       const bf16 *copy = copies + buffer * DK * LV;
-      const int i0 = 16 * warp;
-      const int part0 = episodeOf(mask, i0 + g), part1 = episodeOf(mask, i0 + g + 8);
-      if (p.saved && seg * (p.segmentLength / C) + c > 0) {
-        bf16 *to = p.saved + (eh * ((p.T + C - 1) / C) + seg * (p.segmentLength / C) + c) * stateSize;
-        for (int x = threadIdx.x; x < p.Dk * DV; x += THREADS) {
-          const int i = x / DV, j = x % DV;
-          if (col0 + j < p.Dv) to[int64_t(i) * p.Dv + col0 + j] = copy[i * LV + j];
+      const int start0 = episodeStart(mask, i0 + g), start1 = episodeStart(mask, i0 + g + 8);
+      const int chunk = seg * (p.segmentLength / C) + c;
+      if (STATE && p.saved && chunk > 0) {
+        bf16 *to = p.saved + (eh * ((p.T + C - 1) / C) + chunk) * stateSize + col0;
+        if (p.Dv % 8 == 0) {
+#pragma unroll
+          for (int x = threadIdx.x; x < DK * DV / 8; x += THREADS) {
+            const int i = x / (DV / 8), j = x % (DV / 8) * 8;
+            if (i < p.Dk && col0 + j < p.Dv)
+              *reinterpret_cast<uint4 *>(to + i * p.Dv + j) = *reinterpret_cast<const uint4 *>(copy + i * LV + j);
+          }
+        } else {
+          for (int x = threadIdx.x; x < p.Dk * DV; x += THREADS)
+            if (col0 + x % DV < p.Dv) to[x / DV * p.Dv + x % DV] = copy[x / DV * LV + x % DV];
         }
       }
       uint32_t a[DK / 16][4];
@@ -213,20 +361,21 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionC
       for (int n = 0; n < DV / 8; ++n)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[n][x] = 0.f;
-      // Q S
+      if (later) {   // Q S
 #pragma unroll
-      for (int kk = 0; kk < DK / 16; ++kk)
+        for (int kk = 0; kk < DK / 16; ++kk)
 #pragma unroll
-        for (int n = 0; n < DV / 16; ++n) {
-          uint32_t b[4];
-          operandBTransposed<LV>(b, copy, kk * 16, n * 16);
-          multiplyAdd(o[2 * n], a[kk], b[0], b[1]);
-          multiplyAdd(o[2 * n + 1], a[kk], b[2], b[3]);
-        }
+          for (int n = 0; n < DV / 16; ++n) {
+            uint32_t b[4];
+            operandBTransposed<LV>(b, copy, kk * 16, n * 16);
+            multiplyAdd(o[2 * n], a[kk], b[0], b[1]);
+            multiplyAdd(o[2 * n + 1], a[kk], b[2], b[3]);
+          }
 #pragma unroll
-      for (int n = 0; n < DV / 8; ++n)
+        for (int n = 0; n < DV / 8; ++n)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[n][x] = (x < 2 ? part0 : part1) == 0 ? o[n][x] * fromStart : 0.f;
+          for (int x = 0; x < 4; ++x) o[n][x] = (x < 2 ? start0 : start1) < 0 ? o[n][x] * fromStart : 0.f;
+      }
       // Earlier blocks, then the warp's own.
       for (int block = 0; block <= warp; ++block) {
         float s[2][4] = {};
@@ -237,14 +386,14 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionC
           multiplyAdd(s[0], a[kk], b[0], b[1]);
           multiplyAdd(s[1], a[kk], b[2], b[3]);
         }
+        const int j0 = block * 16 + 2 * tq;
         if (block < warp) {
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const float2 f = *reinterpret_cast<const float2 *>(before + C - i0 + block * 16 + n * 8 + 2 * tq);
-            s[n][0] *= f.x;
-            s[n][1] *= f.y;
-            s[n][2] *= f.x;
-            s[n][3] *= f.y;
+            const float2 f = *reinterpret_cast<const float2 *>(before + C - i0 + j0 + n * 8);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              s[n][x] = j0 + n * 8 + (x & 1) >= (x < 2 ? start0 : start1) ? s[n][x] * (x & 1 ? f.y : f.x) : 0.f;
           }
         } else {
 #pragma unroll
@@ -258,14 +407,9 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionC
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              s[n][x] = g + (x >> 1) * 8 >= 2 * tq + (x & 1) + 8 * n ? s[n][x] * inBlock[n][x] : 0.f;
-        }
-        if (mask) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (episodeOf(mask, block * 16 + n * 8 + 2 * tq + (x & 1)) != (x < 2 ? part0 : part1)) s[n][x] = 0.f;
+              s[n][x] = g + (x >> 1) * 8 >= 2 * tq + (x & 1) + 8 * n &&
+                                j0 + n * 8 + (x & 1) >= (x < 2 ? start0 : start1)
+                            ? s[n][x] * inBlock[n][x] : 0.f;
         }
         const uint32_t w[4] = {packPair(s[0][0], s[0][1]), packPair(s[0][2], s[0][3]), packPair(s[1][0], s[1][1]),
                                packPair(s[1][2], s[1][3])};
@@ -277,55 +421,39 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionC
           multiplyAdd(o[2 * n + 1], w, b[2], b[3]);
         }
       }
-      float finite = 0.f;
 #pragma unroll
       for (int n = 0; n < DV / 8; ++n)
 #pragma unroll
         for (int x = 0; x < 4; ++x) finite = fmaf(o[n][x], 0.f, finite);
-      bad |= finite != 0.f;   // NaN
-#pragma unroll
-      for (int n = 0; n < DV / 8; ++n)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int i = i0 + g + y * 8, j = col0 + n * 8 + 2 * tq;
-          if (i >= count) continue;
-          bf16 *to = p.out + (int64_t(first + i) * p.E * p.H + eh) * p.Dv + j;
-          if (j + 1 < p.Dv && p.Dv % 2 == 0) *reinterpret_cast<uint32_t *>(to) = packPair(o[n][2 * y], o[n][2 * y + 1]);
-          else {
-            if (j < p.Dv) to[0] = fromFloat<bf16>(o[n][2 * y]);
-            if (j + 1 < p.Dv) to[1] = fromFloat<bf16>(o[n][2 * y + 1]);
-          }
-        }
+      storeTile(p.out + eh * p.Dv, o, int64_t(p.E) * p.H * p.Dv, first, count, i0, col0, p.Dv);
     }
 
     // The state at the chunk's end.
-    if (c + 1 < chunks || last) {
+    if (STATE && (c + 1 < chunks || last)) {
       if (count < C) __syncthreads();   // toEnd
-      const int endPart = episodeOf(mask, 63);
+      const int start = episodeStart(mask, 63);
       const float f = count == C ? fullChunk : power(count);
 #pragma unroll
       for (int m = 0; m < SM; ++m)
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) S[m][n][x] = endPart == 0 ? S[m][n][x] * f : 0.f;
+          for (int x = 0; x < 4; ++x) S[m][n][x] = start < 0 ? S[m][n][x] * f : 0.f;
 #pragma unroll
       for (int kk = 0; kk < C / 16; ++kk) {
-        float2 f0 = *reinterpret_cast<const float2 *>(toEnd + kk * 16 + 2 * tq);
-        float2 f1 = *reinterpret_cast<const float2 *>(toEnd + kk * 16 + 8 + 2 * tq);
-        bool in[4] = {true, true, true, true};
-        if (mask) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) in[x] = episodeOf(mask, kk * 16 + 2 * tq + (x & 1) + (x >> 1) * 8) == endPart;
-        }
+        const int j = kk * 16 + 2 * tq;
+        float2 f0 = *reinterpret_cast<const float2 *>(toEnd + j), f1 = *reinterpret_cast<const float2 *>(toEnd + j + 8);
+        f0.x = j >= start ? f0.x : 0.f;
+        f0.y = j + 1 >= start ? f0.y : 0.f;
+        f1.x = j + 8 >= start ? f1.x : 0.f;
+        f1.y = j + 9 >= start ? f1.y : 0.f;
 #pragma unroll
         for (int m = 0; m < SM; ++m) {
           uint32_t a[4], high[4], low[4];
           operandATransposed<LQ>(a, K, (sm0 + m) * 16, kk * 16);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {   // registers 0, 1: steps 2 tq, + 1; registers 2, 3: 8 later
-            const float l = in[(x >> 1) * 2] ? lowOf(a[x]) * (x < 2 ? f0.x : f1.x) : 0.f;
-            const float u = in[(x >> 1) * 2 + 1] ? highOf(a[x]) * (x < 2 ? f0.y : f1.y) : 0.f;
+            const float l = lowOf(a[x]) * (x < 2 ? f0.x : f1.x), u = highOf(a[x]) * (x < 2 ? f0.y : f1.y);
             high[x] = packPair(l, u);
             low[x] = packPair(l - lowOf(high[x]), u - highOf(high[x]));
           }
@@ -335,42 +463,32 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : 256) / C) attentionC
             operandBTransposed<LV>(b, V, kk * 16, (sn0 + 2 * n) * 8);
             multiplyAdd(S[m][2 * n], high, b[0], b[1]);
             multiplyAdd(S[m][2 * n + 1], high, b[2], b[3]);
-            multiplyAdd(S[m][2 * n], low, b[0], b[1]);
-            multiplyAdd(S[m][2 * n + 1], low, b[2], b[3]);
+            if (p.precise) {
+              multiplyAdd(S[m][2 * n], low, b[0], b[1]);
+              multiplyAdd(S[m][2 * n + 1], low, b[2], b[3]);
+            }
           }
         }
       }
-      float finite = 0.f;
-#pragma unroll
-      for (int m = 0; m < SM; ++m)
-#pragma unroll
-        for (int n = 0; n < SN; ++n)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) finite = fmaf(S[m][n][x], 0.f, finite);
-      bad |= finite != 0.f;
-      if (OUT && c + 1 < chunks) copyState((c + 1) & 1);
+      later = true;
+      if (OUT && c + 1 < chunks) copySlice<LV>(copies + ((c + 1) & 1) * DK * LV, S, sm0, sn0);
     }
+  }
+  bool bad = finite != 0.f;   // NaN
+  if (STATE && last) {
+    writeSlice(last, S, sm0, sn0, col0, p.Dk, p.Dv);
+#pragma unroll
+    for (int m = 0; m < SM; ++m) bad |= notFinite(S[m]);
   }
   if (!OUT && col0 == 0 && threadIdx.x == 0) p.segmentCut[eh * p.segmentCount + seg] = anyReset;
   if (OUT) {
     const bool redo = __syncthreads_or(bad);
     if (threadIdx.x == 0) p.flags[eh * gridDim.y + blockIdx.y] = redo;
   }
-  if (last) {
-#pragma unroll
-    for (int m = 0; m < SM; ++m)
-#pragma unroll
-      for (int n = 0; n < SN; ++n)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int i = (sm0 + m) * 16 + g + y * 8, j = col0 + (sn0 + n) * 8 + 2 * tq;
-          if (i >= p.Dk) continue;
-          float *to = last + int64_t(i) * p.Dv + j;
-          if (j < p.Dv) to[0] = S[m][n][2 * y];
-          if (j + 1 < p.Dv) to[1] = S[m][n][2 * y + 1];
-        }
-  }
 }
+
+using Forwards = std::integral_constant<int, 1>;
+using Backwards = std::integral_constant<int, -1>;
 
 // Operands and arrays of a backward call.
 struct BackwardArgs {
@@ -388,41 +506,13 @@ struct BackwardArgs {
   int T, E, H, Dk, Dv;
   int segmentLength, segmentCount;
   int vecQ, vecK, vecV, vecO;
+  int precise;                 // the gradient of the state is an output
   float scale;
 };
 
 template <int C, int D, bool OUT> constexpr int backwardWarps() { return OUT && D == 128 ? C / 8 : C / 16; }
 template <int C, int D, bool OUT> constexpr int backwardSharedBytes() {
   return (OUT ? (4 * C + 2 * D) : 2 * C) * (D + 8) * 2 + (16 + C + 4) * 4;
-}
-
-// Rows of 16 steps by N tiles of 8 columns of a dense [T, E, H, width] output.
-template <int N>
-__device__ __forceinline__ void storeTile(bf16 *out, const float (&x)[N][4], int64_t stepStride, int first, int count,
-                                          int row0, int col0, int width) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const int i = row0 + g + y * 8, j = col0 + n * 8 + 2 * tq;
-      if (i >= count) continue;
-      bf16 *to = out + int64_t(first + i) * stepStride + j;
-      if (j + 1 < width && width % 2 == 0) *reinterpret_cast<uint32_t *>(to) = packPair(x[n][2 * y], x[n][2 * y + 1]);
-      else {
-        if (j < width) to[0] = fromFloat<bf16>(x[n][2 * y]);
-        if (j + 1 < width) to[1] = fromFloat<bf16>(x[n][2 * y + 1]);
-      }
-    }
-}
-
-template <int N> __device__ __forceinline__ bool notFinite(const float (&x)[N][4]) {
-  float sum = 0.f;
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int y = 0; y < 4; ++y) sum = fmaf(x[n][y], 0.f, sum);
-  return sum != 0.f;
 }
 
 // One block per (environment, head) and segment of T, chunks from the last to the
@@ -439,8 +529,9 @@ template <int N> __device__ __forceinline__ bool notFinite(const float (&x)[N][4
 // takes its scores from products of its own, in the layout in which they are the
 // next product's operand: six instead of five products of C x C x D, and no score
 // passes through shared memory.  OUT = false: X' of a segment alone.
-template <int C, int D, bool OUT>
-__global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 64 : 256) / C)
+// STATE = false is for one chunk whose first state's gradient nobody wants.
+template <int C, int D, bool OUT, bool STATE>
+__global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 64 : STATE ? 192 : 256) / C)
     attentionChunksBackward(BackwardArgs p) {
   constexpr int W = backwardWarps<C, D, OUT>(), THREADS = W * 32, LD = D + 8;
   constexpr int PARTS = W / (C / 16);                          // warps that share 16 rows of the outputs
@@ -470,17 +561,10 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
   for (int x = threadIdx.x; x < C + 20; x += THREADS) powers[x] = x < 16 ? 0.f : p.scale * power(x - 16);
   const int sm0 = RT >= W ? warp * SM : warp / SPLIT, sn0 = RT >= W ? 0 : (warp % SPLIT) * SN;
   float dS[SM][SN][4];
-#pragma unroll
-  for (int m = 0; m < SM; ++m)
-#pragma unroll
-    for (int n = 0; n < SN; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int i = (sm0 + m) * 16 + g + (x >> 1) * 8, j = (sn0 + n) * 8 + 2 * tq + (x & 1);
-        dS[m][n][x] = init && i < p.Dk && j < p.Dv ? init[int64_t(i) * p.Dv + j] : 0.f;
-      }
+  if (STATE) readSlice(dS, init, sm0, sn0, 0, p.Dk, p.Dv);
 
-  bool bad = false, anyReset = false, later = init != nullptr;   // later: X is not zero
+  float finite = 0.f;
+  bool anyReset = false, later = init != nullptr;   // later: X is not zero
   for (int c = chunks - 1; c >= 0; --c) {
     const int first = t0 + c * C, count = min(C, t1 - first);
     loadTile<C, D, THREADS>(Q, q, p.qs.t, first, count, 0, p.Dk, p.vecQ);
@@ -494,23 +578,12 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
         loadTile<D, D, THREADS>(S, p.saved + (eh * allChunks + chunk) * stateSize, p.Dv, 0, p.Dk, 0, p.Dv,
                                 p.Dv % 8 == 0);
       } else if (p.stateIn) {
-        const float *from = p.stateIn + eh * stateSize;
-        for (int x = threadIdx.x; x < D * D / 2; x += THREADS) {
-          const int i = x / (D / 2), j = x % (D / 2) * 2;
-          const float low = i < p.Dk && j < p.Dv ? from[int64_t(i) * p.Dv + j] : 0.f;
-          const float high = i < p.Dk && j + 1 < p.Dv ? from[int64_t(i) * p.Dv + j + 1] : 0.f;
-          *reinterpret_cast<uint32_t *>(S + i * LD + j) = packPair(low, high);
-        }
+        loadState<D, D, THREADS>(S, p.stateIn + eh * stateSize, p.Dk, 0, p.Dv);
       }
-      if (later) {
-#pragma unroll
-        for (int m = 0; m < SM; ++m)
-#pragma unroll
-          for (int n = 0; n < SN; ++n)
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-              *reinterpret_cast<uint32_t *>(X + ((sm0 + m) * 16 + g + y * 8) * LD + (sn0 + n) * 8 + 2 * tq) =
-                  packPair(dS[m][n][2 * y], dS[m][n][2 * y + 1]);
+      if (STATE) {
+        if (later) copySlice<LD>(X, dS, sm0, sn0);
+      } else if (init) {
+        loadState<D, D, THREADS>(X, init, p.Dk, 0, p.Dv);
       }
     }
     commitCopies();
@@ -518,8 +591,7 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
     anyReset |= mask != 0;
     waitCopies();
     __syncthreads();
-    const int endPart = episodeOf(mask, 63);
-    const int part0 = episodeOf(mask, row + g), part1 = episodeOf(mask, row + g + 8);
+    const int endStart = episodeStart(mask, 63);   // the state after the chunk sees the steps from there on
 
     if (OUT) {
       const int blockRow = row / 16, blocks = (count + 15) / 16;
@@ -527,7 +599,10 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
       float out[N][4];
       // The scores of the warp's rows with a block of 16 other steps, times their decays; `sign` 1: the rows are
       // the later steps.
-      auto weights = [&](uint32_t (&w)[4], const bf16 *other, int block, int sign) {
+      const int start0 = episodeStart(mask, row + g), start1 = episodeStart(mask, row + g + 8);
+      const int end0 = episodeEnd(mask, row + g), end1 = episodeEnd(mask, row + g + 8);
+      auto weights = [&](uint32_t (&w)[4], const bf16 *other, int block, auto sign_) {
+        constexpr int sign = decltype(sign_)::value;
         float s[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -540,14 +615,11 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[n][x] *= f[sign * ((x >> 1) * 8 - (x & 1) - n * 8)];
-        if (mask) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (episodeOf(mask, block * 16 + n * 8 + 2 * tq + (x & 1)) != (x < 2 ? part0 : part1)) s[n][x] = 0.f;
-        }
+          for (int x = 0; x < 4; ++x) {
+            const int at = block * 16 + n * 8 + 2 * tq + (x & 1);
+            const bool sees = sign > 0 ? at >= (x < 2 ? start0 : start1) : at < (x < 2 ? end0 : end1);
+            s[n][x] = sees ? s[n][x] * f[sign * ((x >> 1) * 8 - (x & 1) - n * 8)] : 0.f;
+          }
         w[0] = packPair(s[0][0], s[0][1]);
         w[1] = packPair(s[0][2], s[0][3]);
         w[2] = packPair(s[1][0], s[1][1]);
@@ -576,6 +648,12 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
 #pragma unroll
           for (int x = 0; x < 4; ++x) out[n][x] = (x < 2 ? f0 : f1) == 0.f ? 0.f : out[n][x] * (x < 2 ? f0 : f1);
       };
+      auto check = [&]() {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) finite = fmaf(out[n][x], 0.f, finite);
+      };
       const int64_t stepK = int64_t(p.E) * p.H * p.Dk, stepV = int64_t(p.E) * p.H * p.Dv;
       if (row < count) {
         // dq
@@ -590,19 +668,19 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
               multiplyAdd(out[2 * n], a[kk], b[0], b[1]);
               multiplyAdd(out[2 * n + 1], a[kk], b[2], b[3]);
             }
-          scaleRows(part0 == 0 ? powers[16 + row + g + 1] : 0.f, part1 == 0 ? powers[16 + row + g + 9] : 0.f);
+          scaleRows(start0 < 0 ? powers[16 + row + g + 1] : 0.f, start1 < 0 ? powers[16 + row + g + 9] : 0.f);
         }
         for (int block = 0; block <= blockRow; ++block) {
           uint32_t w[4];
-          weights(w, V, block, 1);
+          weights(w, V, block, Forwards());
           accumulate(w, K, block);
         }
-        bad |= notFinite(out);
+        check();
         storeTile(p.dq + eh * p.Dk, out, stepK, first, count, row, col, p.Dk);
         // dv, dk
-        const int end0 = count - 1 - row - g, end1 = end0 - 8;
-        const float f0 = part0 == endPart && end0 >= 0 ? power(end0) : 0.f;
-        const float f1 = part1 == endPart && end1 >= 0 ? power(end1) : 0.f;
+        const int left0 = count - 1 - row - g, left1 = left0 - 8;
+        const float f0 = row + g >= endStart && left0 >= 0 ? power(left0) : 0.f;
+        const float f1 = row + g + 8 >= endStart && left1 >= 0 ? power(left1) : 0.f;
         rowsOfA(K);
         if (later) {
 #pragma unroll
@@ -618,10 +696,10 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
         }
         for (int block = blockRow; block < blocks; ++block) {
           uint32_t w[4];
-          weights(w, Q, block, -1);
+          weights(w, Q, block, Backwards());
           accumulate(w, O, block);
         }
-        bad |= notFinite(out);
+        check();
         storeTile(p.dv + eh * p.Dv, out, stepV, first, count, row, col, p.Dv);
         rowsOfA(V);
         if (later) {
@@ -638,28 +716,29 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
         }
         for (int block = blockRow; block < blocks; ++block) {
           uint32_t w[4];
-          weights(w, O, block, -1);
+          weights(w, O, block, Backwards());
           accumulate(w, Q, block);
         }
-        bad |= notFinite(out);
+        check();
         storeTile(p.dk + eh * p.Dk, out, stepK, first, count, row, col, p.Dk);
       }
     }
 
-    if (c > 0 || last) {
+    if (STATE && (c > 0 || last)) {
+      const int firstReset = episodeEnd(mask, 0);   // of the steps after 0
       const float f = power(count);
 #pragma unroll
       for (int m = 0; m < SM; ++m)
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) dS[m][n][x] = endPart == 0 ? dS[m][n][x] * f : 0.f;
+          for (int x = 0; x < 4; ++x) dS[m][n][x] = endStart < 0 ? dS[m][n][x] * f : 0.f;
       for (int kk = 0; kk < (count + 15) / 16; ++kk) {
         float w[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int i = kk * 16 + 2 * tq + (x & 1) + (x >> 1) * 8;
-          w[x] = episodeOf(mask, i) == 0 ? powers[16 + i + 1] : 0.f;
+          w[x] = !(mask & 1) && i < firstReset ? powers[16 + i + 1] : 0.f;
         }
 #pragma unroll
         for (int m = 0; m < SM; ++m) {
@@ -677,32 +756,27 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
             operandBTransposed<LD>(b, O, kk * 16, (sn0 + 2 * n) * 8);
             multiplyAdd(dS[m][2 * n], high, b[0], b[1]);
             multiplyAdd(dS[m][2 * n + 1], high, b[2], b[3]);
-            multiplyAdd(dS[m][2 * n], low, b[0], b[1]);
-            multiplyAdd(dS[m][2 * n + 1], low, b[2], b[3]);
+            if (p.precise) {
+              multiplyAdd(dS[m][2 * n], low, b[0], b[1]);
+              multiplyAdd(dS[m][2 * n + 1], low, b[2], b[3]);
+            }
           }
         }
       }
-#pragma unroll
-      for (int m = 0; m < SM; ++m) bad |= notFinite(dS[m]);
       later = true;
       __syncthreads();   // the tiles and X are free
     }
+  }
+  bool bad = finite != 0.f;   // NaN
+  if (STATE && last) {
+    writeSlice(last, dS, sm0, sn0, 0, p.Dk, p.Dv);
+#pragma unroll
+    for (int m = 0; m < SM; ++m) bad |= notFinite(dS[m]);
   }
   if (!OUT && threadIdx.x == 0) p.segmentCut[eh * p.segmentCount + seg] = anyReset;
   if (OUT) {
     const bool redo = __syncthreads_or(bad);
     if (threadIdx.x == 0) p.flags[eh * p.segmentCount + seg] = redo;
-  }
-  if (last) {
-#pragma unroll
-    for (int m = 0; m < SM; ++m)
-#pragma unroll
-      for (int n = 0; n < SN; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int i = (sm0 + m) * 16 + g + (x >> 1) * 8, j = (sn0 + n) * 8 + 2 * tq + (x & 1);
-          if (i < p.Dk && j < p.Dv) last[int64_t(i) * p.Dv + j] = dS[m][n][x];
-        }
   }
 }
 
@@ -730,14 +804,28 @@ __global__ void __launch_bounds__(256) joinSegments(float *segments, const uint8
 }
 
 // Sweeps of a call step by step, for the environments and heads that have one of
-// their `count` flags set.
-template <int DI> __global__ void __launch_bounds__(128) redoAttention(Sweep s, const uint8_t *flags, int count) {
-  const int64_t all = int64_t(s.E) * s.H;
-  for (int64_t eh = blockIdx.x; eh < all; eh += gridDim.x) {
-    bool any = false;
+// their `count` flags set; usually none has.  A block has a run of them and looks
+// at all its flags at once first.  blockIdx.z says which sweep.
+template <int DI> __device__ __forceinline__ void redoFlagged(const Sweep &s, const uint8_t *flags, int count) {
+  const int64_t all = int64_t(s.E) * s.H, run = (all + gridDim.x - 1) / gridDim.x;
+  const int64_t first = blockIdx.x * run, end = min(all, first + run);
+  bool any = false;
+  for (int64_t x = first * count + threadIdx.x; x < end * count; x += blockDim.x) any |= flags[x] != 0;
+  if (!__syncthreads_or(any)) return;
+  for (int64_t eh = first; eh < end; ++eh) {
+    any = false;
     for (int x = threadIdx.x; x < count; x += blockDim.x) any |= flags[eh * count + x] != 0;
     if (__syncthreads_or(any)) scanSteps<bf16, DI>(s, eh, blockIdx.y * blockDim.x + threadIdx.x);
   }
+}
+template <int DI> __global__ void __launch_bounds__(128) redoAttention(Sweep s, const uint8_t *flags, int count) {
+  redoFlagged<DI>(s, flags, count);
+}
+template <int DI>
+__global__ void __launch_bounds__(128) redoBackward(Sweep q, Sweep k, Sweep v, const uint8_t *flags, int count) {
+  if (blockIdx.z == 0) redoFlagged<DI>(q, flags, count);
+  else if (blockIdx.z == 1) redoFlagged<DI>(k, flags, count);
+  else redoFlagged<DI>(v, flags, count);
 }
 
 }  // namespace duckb200

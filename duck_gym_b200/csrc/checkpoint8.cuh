@@ -11,6 +11,12 @@
 // reciprocals.  A group whose scale would be zero or denormal keeps zeros; one
 // that holds an infinity or NaN keeps NaN throughout (its scale is not finite),
 // so a diverged activation is not hidden by its checkpoint.
+//
+// Bound by memory where the arithmetic stays small: forward 2 values and a byte
+// an element, backward 3 values and a byte.  Rows of whole 16-byte pieces: 16
+// lanes (bfloat16; 32 in float32) hold a group in registers, the next group's
+// loads issued before.  The largest magnitude is taken on the bits, where NaN
+// is above infinity and that above all numbers, two bfloat16 at a time.
 #pragma once
 #include "numeric_types.cuh"
 
@@ -92,6 +98,184 @@ template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluRest
       if (p.y) static_cast<T *>(p.y)[at + c] = fromFloat<T>(y);
       static_cast<T *>(p.dx)[at + c] = fromFloat<T>(dy * (y > 0.f ? 1.f : y + 1.f));
     }
+  }
+}
+
+// exp(x) - 1 for x <= 0 to a few 1e-7 of itself, for results that are rounded to
+// bfloat16 next: its series where 1 would cancel (the sixth term is below
+// 0.25^5 / 720 = 1.4e-6 of the sum), else the hardware's power of two.
+__device__ __forceinline__ float eluRounded(float x) {
+  const float series = x * fmaf(x, fmaf(x, fmaf(x, fmaf(x, 1.f / 120.f, 1.f / 24.f), 1.f / 6.f), 0.5f), 1.f);
+  const float power = __expf(x) - 1.f;
+  const float below = x > -0.25f ? series : power;
+  return x > 0.f ? x : below;
+}
+
+// Eight or four values as the 16 bytes that they are moved in.
+template <class T> struct Piece;
+template <> struct Piece<bf16> {
+  static constexpr int values = 8, lanes = 16;
+  // elu of the values, in place; the bits of the largest magnitude as float bits.
+  static __device__ __forceinline__ uint32_t elu(uint4 &piece) {
+    uint32_t *w = reinterpret_cast<uint32_t *>(&piece), largest = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float low = __uint_as_float(w[i] << 16), high = __uint_as_float(w[i] & 0xffff0000u);
+      const __nv_bfloat162 y = __floats2bfloat162_rn(eluRounded(low), eluRounded(high));
+      w[i] = *reinterpret_cast<const uint32_t *>(&y);
+      largest = __vmaxu2(largest, w[i] & 0x7fff7fffu);
+    }
+    return max(largest << 16, largest & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void floats(float (&x)[8], const uint4 &piece) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&piece);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 round(const float (&x)[8]) {
+    uint4 piece;
+    uint32_t *w = reinterpret_cast<uint32_t *>(&piece);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 y = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&y);
+    }
+    return piece;
+  }
+};
+template <> struct Piece<float> {
+  static constexpr int values = 4, lanes = 32;
+  static __device__ __forceinline__ uint32_t elu(uint4 &piece) {
+    uint32_t *w = reinterpret_cast<uint32_t *>(&piece), largest = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __float_as_uint(duckb200::elu(__uint_as_float(w[i])));
+      largest = max(largest, w[i] & 0x7fffffffu);
+    }
+    return largest;
+  }
+  static __device__ __forceinline__ void floats(float (&x)[4], const uint4 &piece) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&piece);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+  }
+  static __device__ __forceinline__ uint4 round(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+};
+
+// Group `at` of the next ones of a team, without a division in the loop.
+struct GroupWalk {
+  int64_t row, rowStep;
+  int group, groupStep, groups;
+  __device__ __forceinline__ GroupWalk(int64_t first, int64_t step, int groups_)
+      : row(first / groups_), rowStep(step / groups_), group(int(first % groups_)), groupStep(int(step % groups_)),
+        groups(groups_) {}
+  __device__ __forceinline__ void advance() {
+    row += rowStep;
+    group += groupStep;
+    if (group >= groups) {
+      group -= groups;
+      ++row;
+    }
+  }
+};
+
+template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluCheckpointPieces(CheckpointArgs p) {
+  constexpr int V = Piece<T>::values, LANES = Piece<T>::lanes;
+  const int lane = threadIdx.x % LANES;
+  const int64_t teams = int64_t(gridDim.x) * (kCheckpointThreads / LANES);
+  GroupWalk now(int64_t(blockIdx.x) * (kCheckpointThreads / LANES) + threadIdx.x / LANES, teams, p.groups), next = now;
+  const T *x = static_cast<const T *>(p.in);
+  uint4 ahead;
+  auto load = [&](const GroupWalk &at) {
+    const int c = at.group * kGroup + lane * V;
+    ahead = at.row < p.rows && c < p.n ? __ldcs(reinterpret_cast<const uint4 *>(x + at.row * p.n + c))
+                                       : make_uint4(0, 0, 0, 0);
+  };
+  load(next);
+  // A warp's teams go round together: the exchange is among whole warps.
+  while (__any_sync(0xffffffffu, now.row < p.rows)) {
+    uint4 piece = ahead;
+    next.advance();
+    load(next);
+    uint32_t bits = Piece<T>::elu(piece);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    const GroupScale s = groupScale(__uint_as_float(bits));
+    const uint32_t keep = bits < 0x7f800000u ? 0xffffffffu : 0u;   // not finite: code 0 throughout
+    float y[V];
+    Piece<T>::floats(y, piece);
+    uint32_t codes[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      // Adding 1.5 2^23 rounds to a whole number, ties to even, and leaves it in the low bits.
+      uint32_t t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = __float_as_uint(__fadd_rn(__fmul_rn(y[4 * i + j], s.inverse), 12582912.f));
+      codes[i] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410) & keep;
+    }
+    const int c = now.group * kGroup + lane * V;
+    if (now.row < p.rows && c < p.n) {
+      const int64_t at = now.row * p.n + c;
+      *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + at) = piece;
+      if (V == 8) *reinterpret_cast<uint2 *>(p.codes + at) = make_uint2(codes[0], codes[V / 4 - 1]);
+      else *reinterpret_cast<uint32_t *>(p.codes + at) = codes[0];
+      if (lane == 0) p.scales[now.row * p.groups + now.group] = s.scale;
+    }
+    now = next;
+  }
+}
+
+template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluRestorePieces(CheckpointArgs p) {
+  constexpr int V = Piece<T>::values, LANES = Piece<T>::lanes;
+  const int lane = threadIdx.x % LANES;
+  const int64_t teams = int64_t(gridDim.x) * (kCheckpointThreads / LANES);
+  GroupWalk now(int64_t(blockIdx.x) * (kCheckpointThreads / LANES) + threadIdx.x / LANES, teams, p.groups), next = now;
+  uint4 aheadDy;
+  uint32_t aheadCodes[V / 4];
+  float aheadScale;
+  auto load = [&](const GroupWalk &at) {
+    const int c = at.group * kGroup + lane * V;
+    if (at.row >= p.rows || c >= p.n) return;
+    const int64_t from = at.row * p.n + c;
+    aheadDy = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.in) + from));
+    if (V == 8) {
+      const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(p.codes + from));
+      aheadCodes[0] = w.x;
+      aheadCodes[V / 4 - 1] = w.y;
+    } else {
+      aheadCodes[0] = __ldcs(reinterpret_cast<const uint32_t *>(p.codes + from));
+    }
+    aheadScale = p.scales[at.row * p.groups + at.group];
+  };
+  load(next);
+  for (; now.row < p.rows; now = next) {
+    const uint4 piece = aheadDy;
+    uint32_t codes[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) codes[i] = aheadCodes[i];
+    const float scale = aheadScale;
+    next.advance();
+    load(next);
+    const int c = now.group * kGroup + lane * V;
+    if (c >= p.n) continue;
+    float dy[V], y[V];
+    Piece<T>::floats(dy, piece);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      // code + 128 in the low byte of 2^23 is the number 2^23 + code + 128.
+      const uint32_t biased = codes[i / 4] ^ 0x80808080u;
+      const float code = __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7440 + i % 4)) - 8388736.f;
+      y[i] = code * scale;
+      dy[i] *= y[i] > 0.f ? 1.f : y[i] + 1.f;
+    }
+    const int64_t at = now.row * p.n + c;
+    *reinterpret_cast<uint4 *>(static_cast<T *>(p.dx) + at) = Piece<T>::round(dy);
+    if (p.y) *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + at) = Piece<T>::round(y);
   }
 }
 

@@ -11,6 +11,14 @@
 // rounded before it is used (no fused product), so that it is the same number in
 // its mean and in the difference from it: the gradient of a row of one value,
 // or of a g that is the same throughout, is zero and not a rounding times rstd.
+//
+// Bound by memory: forward 2 values moved per element, backward 3.  A row is held
+// in the registers of a team of 8, 16 or 32 lanes, or of a block of 128 to 512
+// threads (up to 16 values a lane, so rows of up to 8192), and read once; the next row's
+// loads are issued before the current one is reduced.  In the backward pass a lane
+// keeps the same columns for all of its rows, so the sums for the weight and the
+// bias stay in its registers and leave the block as one partial row.  Wider rows
+// take the kernels that read a row several times (norm...Any).
 #pragma once
 #include "numeric_types.cuh"
 
@@ -104,20 +112,235 @@ template <class T> __global__ void __launch_bounds__(256) normColumnsAny(NormArg
   }
 }
 
-__global__ void __launch_bounds__(256) normColumnsFinish(NormArgs p, int splits) {
-  __shared__ float red[8][32];
+// Rows in registers: LANES lanes of a team, VEC consecutive values a load, P values a lane.
+template <class T, int LANES, int VEC, int P> struct NormRow {
+  static constexpr int loads = P / VEC;
+  using Raw = typename PieceOf<T, VEC>::type;
+  Raw raw[loads];
+
+  __device__ __forceinline__ void load(const T *row, int lane, int n) {
+#pragma unroll
+    for (int i = 0; i < loads; ++i) {
+      const int c = (lane + LANES * i) * VEC;
+      raw[i] = c < n ? *reinterpret_cast<const Raw *>(row + c) : Raw();
+    }
+  }
+  __device__ __forceinline__ void values(float (&x)[P]) const {
+#pragma unroll
+    for (int i = 0; i < loads; ++i) {
+      T v[VEC];
+      *reinterpret_cast<Raw *>(v) = raw[i];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[i * VEC + j] = toFloat(v[j]);
+    }
+  }
+  static __device__ __forceinline__ void store(T *row, const float (&x)[P], int lane, int n) {
+#pragma unroll
+    for (int i = 0; i < loads; ++i) {
+      const int c = (lane + LANES * i) * VEC;
+      Raw out;
+      T *v = reinterpret_cast<T *>(&out);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = fromFloat<T>(x[i * VEC + j]);
+      if (c < n) *reinterpret_cast<Raw *>(row + c) = out;
+    }
+  }
+};
+
+// Values of the weight or the bias for a lane's columns.
+template <int LANES, int VEC, int P>
+__device__ __forceinline__ void normColumns(float (&w)[P], const float *from, float otherwise, int lane, int n) {
+#pragma unroll
+  for (int i = 0; i < P / VEC; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int c = (lane + LANES * i) * VEC + j;
+      w[i * VEC + j] = from && c < n ? from[c] : otherwise;
+    }
+}
+
+// Sums of a team, the same bits in each of its lanes.  A team of more than a warp
+// is the block, and `red` has two rows of its warps, used in turn.
+template <int LANES> __device__ __forceinline__ float2 teamSum(float2 x, float2 *red) {
+#pragma unroll
+  for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) {
+    x.x += __shfl_xor_sync(0xffffffffu, x.x, o);
+    x.y += __shfl_xor_sync(0xffffffffu, x.y, o);
+  }
+  if (LANES > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = red[0];
+#pragma unroll
+    for (int k = 1; k < LANES / 32; ++k) {
+      x.x += red[k].x;
+      x.y += red[k].y;
+    }
+  }
+  return x;
+}
+
+__host__ __device__ constexpr int normBlock(int lanes) { return lanes > 32 ? lanes : 128; }
+
+template <class T, int LANES, int VEC, int P>
+__global__ void __launch_bounds__(normBlock(LANES)) normForwardRows(NormArgs p) {
+  constexpr int THREADS = normBlock(LANES), TEAMS = THREADS / LANES;
+  __shared__ float2 red[2][16];
+  const int lane = threadIdx.x % LANES;
+  const int64_t step = int64_t(gridDim.x) * TEAMS;
+  int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / LANES;
+  const T *x = static_cast<const T *>(p.x);
+  T *y = static_cast<T *>(p.y);
+  float w[P], b[P];
+  normColumns<LANES, VEC, P>(w, p.weight, 1.f, lane, p.n);
+  normColumns<LANES, VEC, P>(b, p.bias, 0.f, lane, p.n);
+  const float inverse = 1.f / float(p.n);
+  NormRow<T, LANES, VEC, P> now, next;
+  // All teams of a warp go round as often as its first: the sums are over whole warps.
+  int64_t lead = LANES < 32 ? row - (threadIdx.x & 31) / LANES : row;
+  if (row < p.rows) next.load(x + row * p.xStride, lane, p.n);
+  for (; lead < p.rows; lead += step, row += step) {
+    now = next;
+    const bool live = row < p.rows;
+    if (row + step < p.rows) next.load(x + (row + step) * p.xStride, lane, p.n);
+    float v[P];
+    now.values(v);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) sum += v[i];
+    const float mean = teamSum<LANES>(make_float2(sum, 0.f), red[0]).x / float(p.n);
+    float square = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = (lane + LANES * (i / VEC)) * VEC + i % VEC;
+      v[i] -= mean;
+      if (c < p.n) square = fmaf(v[i], v[i], square);
+    }
+    const float rstd = rsqrtf(teamSum<LANES>(make_float2(square, 0.f), red[1]).x * inverse + p.eps);
+#pragma unroll
+    for (int i = 0; i < P; ++i) v[i] = fmaf(v[i] * rstd, w[i], b[i]);
+    if (live) {
+      NormRow<T, LANES, VEC, P>::store(y + row * p.n, v, lane, p.n);
+      if (p.stats && lane == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
+    }
+  }
+}
+
+// COLUMNS: the sums for the weight's and the bias' gradients too; DX: that of x.
+template <class T, int LANES, int VEC, int P, bool DX, bool COLUMNS>
+__global__ void __launch_bounds__(normBlock(LANES)) normBackwardRows(NormArgs p) {
+  constexpr int THREADS = normBlock(LANES), TEAMS = THREADS / LANES;
+  extern __shared__ float sums[];   // [warps, 2, n] where a team is a warp or less
+  __shared__ float2 red[2][16];
+  const int lane = threadIdx.x % LANES;
+  const int64_t step = int64_t(gridDim.x) * TEAMS;
+  int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / LANES;
+  const T *x = static_cast<const T *>(p.x), *dy = static_cast<const T *>(p.dy);
+  T *dx = static_cast<T *>(p.dx);
+  const float2 *stats = reinterpret_cast<const float2 *>(p.stats);
+  float w[P], dw[P], db[P];
+  if (DX) normColumns<LANES, VEC, P>(w, p.weight, 1.f, lane, p.n);
+#pragma unroll
+  for (int i = 0; i < P; ++i) dw[i] = db[i] = 0.f;
+  const float count = float(p.n);
+  NormRow<T, LANES, VEC, P> nowX, nowY, nextX, nextY;
+  float2 nextStats = make_float2(0.f, 0.f);
+  auto load = [&](int64_t r) {
+    nextX.load(x + r * p.xStride, lane, p.n);
+    nextY.load(dy + r * p.dyStride, lane, p.n);
+    nextStats = stats[r];
+  };
+  int64_t lead = LANES < 32 ? row - (threadIdx.x & 31) / LANES : row;
+  if (row < p.rows) load(row);
+  int turn = 0;
+  for (; lead < p.rows; lead += step, row += step) {
+    nowX = nextX;
+    nowY = nextY;
+    const float mean = nextStats.x, rstd = nextStats.y;
+    const bool live = row < p.rows;
+    if (row + step < p.rows) load(row + step);
+    float u[P], d[P];
+    nowX.values(u);
+    nowY.values(d);
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = (lane + LANES * (i / VEC)) * VEC + i % VEC;
+      u[i] = (u[i] - mean) * rstd;
+      if (COLUMNS && live && c < p.n) {
+        dw[i] = fmaf(d[i], u[i], dw[i]);
+        db[i] += d[i];
+      }
+      if (DX) {
+        d[i] = c < p.n ? __fmul_rn(d[i], w[i]) : 0.f;
+        s.x += d[i];
+        if (c < p.n) s.y = fmaf(d[i], u[i], s.y);
+      }
+    }
+    if (DX) {
+      s = teamSum<LANES>(s, red[turn]);
+      turn ^= 1;
+      s.x /= count;
+      s.y /= count;
+#pragma unroll
+      for (int i = 0; i < P; ++i) d[i] = rstd * (d[i] - s.x - u[i] * s.y);
+      if (live) NormRow<T, LANES, VEC, P>::store(dx + row * p.n, d, lane, p.n);
+    }
+  }
+  if (!COLUMNS) return;
+  float *out = p.partials + int64_t(blockIdx.x) * 2 * p.n;
+  if (LANES > 32) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = (lane + LANES * (i / VEC)) * VEC + i % VEC;
+      if (c < p.n) {
+        out[c] = dw[i];
+        out[p.n + c] = db[i];
+      }
+    }
+    return;
+  }
+  float *mine = sums + (threadIdx.x >> 5) * 2 * p.n;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+#pragma unroll
+    for (int o = 16; o >= LANES; o >>= 1) {
+      dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
+      db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+    }
+    const int c = (lane + LANES * (i / VEC)) * VEC + i % VEC;
+    if (c < p.n && (threadIdx.x & 31) < LANES) {
+      mine[c] = dw[i];
+      mine[p.n + c] = db[i];
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * p.n; c += THREADS) {
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < THREADS / 32; ++k) total += sums[k * 2 * p.n + c];
+    out[c] = total;
+  }
+}
+
+// The gradients from the blocks' partial rows: 32 of the 2 n sums a block, its
+// warps every 32nd partial each, in a fixed order.
+__global__ void __launch_bounds__(1024) normPartials(NormArgs p, int splits) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;   // of the 2 n sums
+  const int c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < 2 * p.n)
-    for (int k = part; k < splits; k += 8) s += p.partials[int64_t(k) * 2 * p.n + c];
+  if (c < 2 * p.n) {
+#pragma unroll 4
+    for (int k = part; k < splits; k += 32) s += p.partials[int64_t(k) * 2 * p.n + c];
+  }
   red[part][lane] = s;
   __syncthreads();
-  if (part == 0 && c < 2 * p.n) {
-    float total = 0.f;
-    for (int k = 0; k < 8; ++k) total += red[k][lane];
-    float *out = c < p.n ? p.dweight : p.dbias;
-    if (out) out[c < p.n ? c : c - p.n] = total;
+  const float total = warpSum(red[lane][part]);
+  const int column = blockIdx.x * 32 + part;
+  if (lane == 0 && column < 2 * p.n) {
+    float *out = column < p.n ? p.dweight : p.dbias;
+    if (out) out[column < p.n ? column : column - p.n] = total;
   }
 }
 

@@ -152,4 +152,65 @@ template <class T> __global__ void __launch_bounds__(128) attentionStepAny(StepO
   }
 }
 
+// The same with four columns a thread: bound by the state's way through memory,
+// 8 bytes an element, so the loads of eight rows are in flight before the first
+// is used, and a state that a reset clears is not read.
+template <class T> __global__ void __launch_bounds__(128) attentionStepQuads(StepOf s) {
+  constexpr int AHEAD = 8;
+  __shared__ float q[kHeadMax], k[kHeadMax];
+  __shared__ float4 red[128];
+  const int64_t eh = blockIdx.x;
+  const int e = int(eh / s.H), h = int(eh - int64_t(e) * s.H);
+  const int columns = s.Dv / 4, rows = 128 / columns;   // of threads
+  const int part = threadIdx.x / columns, j = threadIdx.x - part * columns;
+  const bool live = part < rows;
+  const bool cut = s.resets && s.resets[e];
+  float4 *state = reinterpret_cast<float4 *>(s.state + eh * s.Dk * s.Dv) + j;
+  float4 old[AHEAD];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i = i0 + part + u * rows;
+      old[u] = live && !cut && i < s.Dk ? __ldcs(state + i * columns) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  load(0);
+  if (int(threadIdx.x) < s.Dk) {
+    q[threadIdx.x] = s.scale * toFloat(static_cast<const T *>(s.q)[e * s.qe + h * s.qh + threadIdx.x]);
+    k[threadIdx.x] = toFloat(static_cast<const T *>(s.k)[e * s.ke + h * s.kh + threadIdx.x]);
+  }
+  const float decay = s.decay[h];
+  float v[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) v[x] = live ? toFloat(static_cast<const T *>(s.v)[e * s.ve + h * s.vh + 4 * j + x]) : 0.f;
+  __syncthreads();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < s.Dk; i0 += AHEAD * rows) {
+    if (i0 > 0) load(i0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i = i0 + part + u * rows;
+      if (!live || i >= s.Dk) continue;
+      float4 x = old[u];
+      x.x = fmaf(decay, x.x, k[i] * v[0]);
+      x.y = fmaf(decay, x.y, k[i] * v[1]);
+      x.z = fmaf(decay, x.z, k[i] * v[2]);
+      x.w = fmaf(decay, x.w, k[i] * v[3]);
+      __stcs(state + i * columns, x);
+      o.x = fmaf(q[i], x.x, o.x);
+      o.y = fmaf(q[i], x.y, o.y);
+      o.z = fmaf(q[i], x.z, o.z);
+      o.w = fmaf(q[i], x.w, o.w);
+    }
+  }
+  red[threadIdx.x] = o;
+  __syncthreads();
+  if (int(threadIdx.x) < s.Dv) {
+    const float *sums = reinterpret_cast<const float *>(red) + threadIdx.x;
+    float total = 0.f;
+    for (int r = 0; r < rows; ++r) total += sums[r * s.Dv];
+    static_cast<T *>(s.out)[eh * s.Dv + threadIdx.x] = fromFloat<T>(total);
+  }
+}
+
 }  // namespace duckb200

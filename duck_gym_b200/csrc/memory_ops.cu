@@ -8,6 +8,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <type_traits>
 
 using namespace duckb200;
 
@@ -29,10 +31,66 @@ void requireType(int type) { require(type == DUCK_FLOAT32 || type == DUCK_BFLOAT
 
 int64_t ceilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Row groups that the sums of the weight's gradient are split into.
-int normSplits(int64_t rows, int n) {
+// Whether rows at these addresses and distances (in elements) are made of whole
+// 16-byte pieces; a null pointer is.
+bool pieces16(std::initializer_list<const void *> pointers, std::initializer_list<int64_t> strides, int type) {
+  const int64_t piece = type == DUCK_FLOAT32 ? 4 : 8;
+  for (const void *p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (int64_t s : strides)
+    if (s % piece) return false;
+  return true;
+}
+
+// Layer norm kernels that hold a row in registers: 16-byte pieces where rows are
+// made of them, else single values; up to 8192 values.  Calls f with a kernel's
+// lanes, values a load and values a lane.
+constexpr int kNormWidest = 8192;
+template <int N> using Constant = std::integral_constant<int, N>;
+template <class T, class F> void withNormRows(int n, bool pieces, F &&f) {
+  constexpr int V = 16 / sizeof(T);
+  auto wide = [&](auto vec) {
+    if (n <= 256) f(Constant<32>(), vec, Constant<8>());
+    else if (n <= 512) f(Constant<32>(), vec, Constant<16>());
+    else if (n <= 1024) f(Constant<128>(), vec, Constant<8>());
+    else if (n <= 2048) f(Constant<256>(), vec, Constant<8>());
+    else if (n <= 4096) f(Constant<256>(), vec, Constant<16>());
+    else f(Constant<512>(), vec, Constant<16>());
+  };
+  if (pieces && n <= 64) f(Constant<8>(), Constant<V>(), Constant<8>());
+  else if (pieces && n <= 128) f(Constant<16>(), Constant<V>(), Constant<8>());
+  else if (pieces) wide(Constant<V>());
+  else if (n <= 64) f(Constant<32>(), Constant<1>(), Constant<2>());
+  else wide(Constant<1>());
+}
+// Blocks of a pass over the rows.
+int64_t normBlocks(int64_t rows, int n, bool pieces, int perSm) {
+  int teams = 1;
+  withNormRows<float>(n, pieces, [&](auto lanes, auto, auto) { teams = normBlock(lanes.value) / lanes.value; });
+  return std::max<int64_t>(1, std::min<int64_t>(ceilDiv(rows, teams), int64_t(148) * perSm));
+}
+
+// Partial rows that the sums of the weight's and bias' gradients come in.
+int64_t normSplits(int64_t rows, int n) {
+  if (n <= kNormWidest) return std::max(normBlocks(rows, n, true, 4), normBlocks(rows, n, false, 4));
   const int64_t columns = ceilDiv(n, 32);
-  return int(std::max<int64_t>(1, std::min<int64_t>(ceilDiv(rows, 64), ceilDiv(148 * 8, columns))));
+  return std::max<int64_t>(1, std::min<int64_t>(ceilDiv(rows, 64), ceilDiv(148 * 8, columns)));
+}
+
+// Codes are moved 8 or 4 at a time beside pieces of 16 bytes of values; their array
+// has to be aligned for that.
+void launchGroups(const CheckpointArgs &a, int type, bool pieces, duck_stream stream, bool restore) {
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  pieces = pieces && reinterpret_cast<uintptr_t>(a.codes) % 8 == 0;
+  withType(type, [&](auto zero) {
+    using T = decltype(zero);
+    const int lanes = pieces ? Piece<T>::lanes : 32;
+    const unsigned blocks = unsigned(std::min<int64_t>(ceilDiv(a.rows * a.groups, kCheckpointThreads / lanes), 148 * 8));
+    if (pieces && restore) eluRestorePieces<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
+    else if (pieces) eluCheckpointPieces<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
+    else if (restore) eluRestoreAny<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
+    else eluCheckpointAny<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
+  });
 }
 
 bool attentionChecked(const duck_attention *a) {
@@ -44,6 +102,10 @@ bool attentionChecked(const duck_attention *a) {
   return a->E > 0 && a->H > 0;
 }
 Rows rowsOf(const int64_t *s) { return {s[0], s[1], s[2]}; }
+void requireAligned(std::initializer_list<const void *> pointers) {
+  for (const void *p : pointers)
+    require(reinterpret_cast<uintptr_t>(p) % 16 == 0, "States, outputs and workspaces have to be 16-byte aligned");
+}
 
 template <class T> void launchScan(const Sweep &s, cudaStream_t stream) {
   const int threads = std::min(128, int(ceilDiv(s.Dj, 32)) * 32);
@@ -55,15 +117,19 @@ template <class T> void launchScan(const Sweep &s, cudaStream_t stream) {
   check(cudaGetLastError(), "linear attention launch");
 }
 
-template <int DI> void launchRedo(const Sweep &s, const uint8_t *flags, int count, cudaStream_t stream) {
+void launchRedo(const Sweep &s, const uint8_t *flags, int count, cudaStream_t stream) {
   const int threads = std::min(128, int(ceilDiv(s.Dj, 32)) * 32);
-  const dim3 grid(unsigned(std::min<int64_t>(int64_t(s.E) * s.H, 296)), unsigned(ceilDiv(s.Dj, threads)));
-  redoAttention<DI><<<grid, threads, 0, stream>>>(s, flags, count);
+  const dim3 grid(unsigned(std::min<int64_t>(int64_t(s.E) * s.H, 148)), unsigned(ceilDiv(s.Dj, threads)));
+  if (s.Di <= 32) redoAttention<32><<<grid, threads, 0, stream>>>(s, flags, count);
+  else redoAttention<128><<<grid, threads, 0, stream>>>(s, flags, count);
   check(cudaGetLastError(), "linear attention launch");
 }
-void launchRedo(const Sweep &s, const uint8_t *flags, int count, cudaStream_t stream) {
-  if (s.Di <= 32) launchRedo<32>(s, flags, count, stream);
-  else launchRedo<128>(s, flags, count, stream);
+void launchRedo(const Sweep &q, const Sweep &k, const Sweep &v, const uint8_t *flags, int count, cudaStream_t stream) {
+  const int most = std::max(q.Di, q.Dj), threads = std::min(128, int(ceilDiv(most, 32)) * 32);
+  const dim3 grid(unsigned(std::min<int64_t>(int64_t(q.E) * q.H, 148)), unsigned(ceilDiv(most, threads)), 3);
+  if (most <= 32) redoBackward<32><<<grid, threads, 0, stream>>>(q, k, v, flags, count);
+  else redoBackward<128><<<grid, threads, 0, stream>>>(q, k, v, flags, count);
+  check(cudaGetLastError(), "linear attention backward launch");
 }
 
 Sweep forwardSweep(const duck_attention &a) {
@@ -122,23 +188,24 @@ template <auto kernel> void allowShared(int bytes) {
   if (device < 64) done[device] = true;
 }
 
-template <int C, int DK, int DV, bool OUT>
+template <int C, int DK, int DV, bool OUT, bool STATE>
 void launchChunks(const ChunkArgs &a, int segments, int buffers, cudaStream_t stream) {
   const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(segments * a.columnTiles));
-  constexpr auto kernel = attentionChunks<C, DK, DV, OUT>;
-  constexpr int most = chunkSharedBytes<C, DK, DV, OUT>(2);
+  constexpr auto kernel = attentionChunks<C, DK, DV, OUT, STATE>;
+  constexpr int most = chunkSharedBytes<C, DK, DV, OUT>(STATE ? 2 : 1);
   if constexpr (most > 48 * 1024) allowShared<kernel>(most);
   kernel<<<grid, C * 2, chunkSharedBytes<C, DK, DV, OUT>(buffers), stream>>>(a, buffers);
   check(cudaGetLastError(), "linear attention launch");
 }
-template <int C, bool OUT> void launchChunks(const ChunkArgs &a, int segments, int buffers, cudaStream_t stream) {
+template <int C, bool OUT, bool STATE>
+void launchChunks(const ChunkArgs &a, int segments, int buffers, cudaStream_t stream) {
   const bool narrow = a.Dv <= 32;
-  if (a.Dk <= 32) narrow ? launchChunks<C, 32, 32, OUT>(a, segments, buffers, stream)
-                         : launchChunks<C, 32, 64, OUT>(a, segments, buffers, stream);
-  else if (a.Dk <= 64) narrow ? launchChunks<C, 64, 32, OUT>(a, segments, buffers, stream)
-                              : launchChunks<C, 64, 64, OUT>(a, segments, buffers, stream);
-  else narrow ? launchChunks<C, 128, 32, OUT>(a, segments, buffers, stream)
-              : launchChunks<C, 128, 64, OUT>(a, segments, buffers, stream);
+  if (a.Dk <= 32) narrow ? launchChunks<C, 32, 32, OUT, STATE>(a, segments, buffers, stream)
+                         : launchChunks<C, 32, 64, OUT, STATE>(a, segments, buffers, stream);
+  else if (a.Dk <= 64) narrow ? launchChunks<C, 64, 32, OUT, STATE>(a, segments, buffers, stream)
+                              : launchChunks<C, 64, 64, OUT, STATE>(a, segments, buffers, stream);
+  else narrow ? launchChunks<C, 128, 32, OUT, STATE>(a, segments, buffers, stream)
+              : launchChunks<C, 128, 64, OUT, STATE>(a, segments, buffers, stream);
 }
 
 void forwardChunks(const duck_attention &a, cudaStream_t stream) {
@@ -166,35 +233,40 @@ void forwardChunks(const duck_attention &a, cudaStream_t stream) {
   c.vecK = dense16(a.k, a.k_stride, a.Dk);
   c.vecV = dense16(a.v, a.v_stride, a.Dv);
   c.scale = a.scale;
+  c.precise = a.state_out || split;
   c.flags = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes + plan.cutBytes;
   const int buffers = std::min(plan.chunks, plan.segmentLength / plan.C) > 1 ? 2 : 1;
   if (split) {
     c.segments = a.scratch;
     c.segmentCut = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes;
-    launchChunks<64, false>(c, plan.segmentCount - 1, buffers, stream);
+    launchChunks<64, false, true>(c, plan.segmentCount - 1, buffers, stream);
     const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(ceilDiv(plan.stateSize, 256)));
     joinSegments<<<grid, 256, 0, stream>>>(c.segments, c.segmentCut, a.state_in, a.decay, a.H, a.T, plan.segmentCount,
                                            plan.segmentLength, plan.stateSize, 0);
     check(cudaGetLastError(), "linear attention launch");
   }
-  if (plan.C == 32) launchChunks<32, true>(c, plan.segmentCount, buffers, stream);
-  else launchChunks<64, true>(c, plan.segmentCount, buffers, stream);
+  const bool advance = plan.chunks > 1 || a.state_out;
+  if (plan.C == 32) advance ? launchChunks<32, true, true>(c, 1, 1, stream) : launchChunks<32, true, false>(c, 1, 1, stream);
+  else advance ? launchChunks<64, true, true>(c, plan.segmentCount, buffers, stream)
+               : launchChunks<64, true, false>(c, 1, 1, stream);
   launchRedo(forwardSweep(a), c.flags, plan.segmentCount * plan.columnTiles, stream);
 }
 
-template <int C, int D, bool OUT> void launchBackward(const BackwardArgs &a, int segments, cudaStream_t stream) {
+template <int C, int D, bool OUT, bool STATE>
+void launchBackward(const BackwardArgs &a, int segments, cudaStream_t stream) {
   const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(segments));
-  constexpr auto kernel = attentionChunksBackward<C, D, OUT>;
+  constexpr auto kernel = attentionChunksBackward<C, D, OUT, STATE>;
   constexpr int bytes = backwardSharedBytes<C, D, OUT>();
   if constexpr (bytes > 48 * 1024) allowShared<kernel>(bytes);
   kernel<<<grid, backwardWarps<C, D, OUT>() * 32, bytes, stream>>>(a);
   check(cudaGetLastError(), "linear attention backward launch");
 }
-template <int C, bool OUT> void launchBackward(const BackwardArgs &a, int segments, cudaStream_t stream) {
+template <int C, bool OUT, bool STATE>
+void launchBackward(const BackwardArgs &a, int segments, cudaStream_t stream) {
   const int d = std::max(a.Dk, a.Dv);
-  if (d <= 32) launchBackward<C, 32, OUT>(a, segments, stream);
-  else if (d <= 64) launchBackward<C, 64, OUT>(a, segments, stream);
-  else launchBackward<C, 128, OUT>(a, segments, stream);
+  if (d <= 32) launchBackward<C, 32, OUT, STATE>(a, segments, stream);
+  else if (d <= 64) launchBackward<C, 64, OUT, STATE>(a, segments, stream);
+  else launchBackward<C, 128, OUT, STATE>(a, segments, stream);
 }
 
 void backwardChunks(const duck_attention &a, cudaStream_t stream) {
@@ -227,21 +299,22 @@ void backwardChunks(const duck_attention &a, cudaStream_t stream) {
   c.vecV = dense16(a.v, a.v_stride, a.Dv);
   c.vecO = dense16(a.dout, a.dout_stride, a.Dv);
   c.scale = a.scale;
+  c.precise = a.dstate_in || split;
   c.flags = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes + plan.cutBytes;
   if (split) {
     c.segments = a.scratch;
     c.segmentCut = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes;
-    launchBackward<64, false>(c, plan.segmentCount - 1, stream);
+    launchBackward<64, false, true>(c, plan.segmentCount - 1, stream);
     const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(ceilDiv(plan.stateSize, 256)));
     joinSegments<<<grid, 256, 0, stream>>>(c.segments, c.segmentCut, a.dstate_out, a.decay, a.H, a.T,
                                            plan.segmentCount, plan.segmentLength, plan.stateSize, 1);
     check(cudaGetLastError(), "linear attention backward launch");
   }
-  if (plan.C == 32) launchBackward<32, true>(c, plan.segmentCount, stream);
-  else launchBackward<64, true>(c, plan.segmentCount, stream);
-  launchRedo(gradientOfQ(a), c.flags, plan.segmentCount, stream);
-  launchRedo(gradientOfK(a), c.flags, plan.segmentCount, stream);
-  launchRedo(gradientOfV(a), c.flags, plan.segmentCount, stream);
+  const bool advance = plan.chunks > 1 || a.dstate_in;
+  if (plan.C == 32) advance ? launchBackward<32, true, true>(c, 1, stream) : launchBackward<32, true, false>(c, 1, stream);
+  else advance ? launchBackward<64, true, true>(c, plan.segmentCount, stream)
+               : launchBackward<64, true, false>(c, 1, stream);
+  launchRedo(gradientOfQ(a), gradientOfK(a), gradientOfV(a), c.flags, plan.segmentCount, stream);
 }
 
 }  // namespace
@@ -259,9 +332,20 @@ int duck_layer_norm_forward(const void *x, const float *weight, const float *bia
     NormArgs a{};
     a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.stats = stats;
     a.rows = rows; a.n = n; a.xStride = x_stride; a.eps = float(eps);
-    const int64_t blocks = std::min<int64_t>(ceilDiv(rows, kNormThreads / 32), int64_t(multiprocessors()) * 16);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const bool pieces = pieces16({x, y}, {x_stride, int64_t(n)}, type);
     withType(type, [&](auto zero) {
-      normForwardAny<decltype(zero)><<<unsigned(blocks), kNormThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+      using T = decltype(zero);
+      if (n > kNormWidest) {
+        const int64_t blocks = std::min<int64_t>(ceilDiv(rows, kNormThreads / 32), int64_t(148) * 16);
+        normForwardAny<T><<<unsigned(blocks), kNormThreads, 0, s>>>(a);
+        return;
+      }
+      withNormRows<T>(n, pieces, [&](auto lanes, auto vec, auto values) {
+        constexpr int L = lanes.value;
+        normForwardRows<T, L, vec.value, values.value>
+            <<<unsigned(normBlocks(rows, n, pieces, L > 32 ? 8 : 16)), normBlock(L), 0, s>>>(a);
+      });
     });
     check(cudaGetLastError(), "layer norm launch");
   });
@@ -269,7 +353,7 @@ int duck_layer_norm_forward(const void *x, const float *weight, const float *bia
 
 int64_t duck_layer_norm_scratch(int64_t rows, int n) {
   if (rows < 0 || n <= 0) return -1;
-  return int64_t(normSplits(rows, n)) * 2 * n;
+  return normSplits(rows, n) * 2 * n;
 }
 
 int duck_layer_norm_backward(const void *x, const void *dy, const float *weight, const float *stats, void *dx,
@@ -279,22 +363,37 @@ int duck_layer_norm_backward(const void *x, const void *dy, const float *weight,
     requireType(type);
     require(rows >= 0 && n > 0 && x_stride >= 0 && dy_stride >= 0, "Invalid layer norm sizes");
     const bool columns = dweight || dbias;
+    if (!columns && !dx) return;
     require(!columns || scratch, "Invalid arguments");
     require(rows == 0 || (x && dy && stats), "Invalid arguments");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     NormArgs a{};
     a.x = x; a.dy = dy; a.weight = weight; a.dx = dx; a.stats = const_cast<float *>(stats); a.partials = scratch;
     a.dweight = dweight; a.dbias = dbias; a.rows = rows; a.n = n; a.xStride = x_stride; a.dyStride = dy_stride;
-    const int splits = normSplits(rows, n);
+    const bool pieces = pieces16({x, dy, dx}, {x_stride, dy_stride, int64_t(n)}, type);
+    int splits = 0;
     withType(type, [&](auto zero) {
       using T = decltype(zero);
-      if (dx && rows > 0) {
-        const int64_t blocks = std::min<int64_t>(ceilDiv(rows, kNormThreads / 32), int64_t(multiprocessors()) * 16);
-        normBackwardAny<T><<<unsigned(blocks), kNormThreads, 0, s>>>(a);
+      if (n > kNormWidest) {
+        if (dx && rows > 0) {
+          const int64_t blocks = std::min<int64_t>(ceilDiv(rows, kNormThreads / 32), int64_t(148) * 16);
+          normBackwardAny<T><<<unsigned(blocks), kNormThreads, 0, s>>>(a);
+        }
+        splits = int(normSplits(rows, n));
+        if (columns) normColumnsAny<T><<<dim3(unsigned(ceilDiv(n, 32)), unsigned(splits)), 256, 0, s>>>(a);
+        return;
       }
-      if (columns) normColumnsAny<T><<<dim3(unsigned(ceilDiv(n, 32)), unsigned(splits)), 256, 0, s>>>(a);
+      withNormRows<T>(n, pieces, [&](auto lanes, auto vec, auto values) {
+        constexpr int L = lanes.value, V = vec.value, P = values.value;
+        const int64_t blocks = normBlocks(rows, n, pieces, 4);
+        const int shared = L > 32 ? 0 : normBlock(L) / 32 * 2 * n * int(sizeof(float));
+        splits = int(blocks);
+        if (dx && columns) normBackwardRows<T, L, V, P, true, true><<<unsigned(blocks), normBlock(L), shared, s>>>(a);
+        else if (dx) normBackwardRows<T, L, V, P, true, false><<<unsigned(blocks), normBlock(L), 0, s>>>(a);
+        else normBackwardRows<T, L, V, P, false, true><<<unsigned(blocks), normBlock(L), shared, s>>>(a);
+      });
     });
-    if (columns) normColumnsFinish<<<unsigned(ceilDiv(int64_t(2) * n, 32)), 256, 0, s>>>(a, splits);
+    if (columns) normPartials<<<unsigned(ceilDiv(int64_t(2) * n, 32)), 1024, 0, s>>>(a, splits);
     check(cudaGetLastError(), "layer norm backward launch");
   });
 }
@@ -307,12 +406,7 @@ int duck_elu_checkpoint(const void *x, void *y, int8_t *codes, float *scales, in
     if (rows == 0) return;
     require(x && y && codes && scales, "Invalid arguments");
     CheckpointArgs a{x, y, nullptr, codes, scales, rows, n, int(ceilDiv(n, kGroup))};
-    const int64_t blocks = std::min<int64_t>(ceilDiv(rows * a.groups, kCheckpointThreads / 32),
-                                             int64_t(multiprocessors()) * 32);
-    withType(type, [&](auto zero) {
-      eluCheckpointAny<decltype(zero)>
-          <<<unsigned(blocks), kCheckpointThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-    });
+    launchGroups(a, type, pieces16({x, y}, {int64_t(n)}, type), stream, false);
     check(cudaGetLastError(), "checkpoint launch");
   });
 }
@@ -326,12 +420,7 @@ int duck_elu_restore(const void *dy, const int8_t *codes, const float *scales, v
     require(dy && codes && scales && dx, "Invalid arguments");
     CheckpointArgs a{dy, y, dx, const_cast<int8_t *>(codes), const_cast<float *>(scales), rows, n,
                      int(ceilDiv(n, kGroup))};
-    const int64_t blocks = std::min<int64_t>(ceilDiv(rows * a.groups, kCheckpointThreads / 32),
-                                             int64_t(multiprocessors()) * 32);
-    withType(type, [&](auto zero) {
-      eluRestoreAny<decltype(zero)>
-          <<<unsigned(blocks), kCheckpointThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-    });
+    launchGroups(a, type, pieces16({dy, y, dx}, {int64_t(n)}, type), stream, true);
     check(cudaGetLastError(), "checkpoint launch");
   });
 }
@@ -352,6 +441,7 @@ int duck_linear_attention_forward(const duck_attention *args, duck_stream stream
     if (!attentionChecked(args)) return;
     const duck_attention &a = *args;
     require(a.decay && (a.T == 0 || (a.q && a.k && a.v && a.out)), "Invalid arguments");
+    requireAligned({a.out, a.state_in, a.state_out, a.saved, a.scratch});
     if (a.type == DUCK_BFLOAT16 && a.T > 0) {
       forwardChunks(a, reinterpret_cast<cudaStream_t>(stream));
       return;
@@ -366,6 +456,7 @@ int duck_linear_attention_backward(const duck_attention *args, duck_stream strea
     if (!attentionChecked(args)) return;
     const duck_attention &a = *args;
     require(a.decay && (a.T == 0 || (a.q && a.k && a.v && a.dout && a.dq && a.dk && a.dv)), "Invalid arguments");
+    requireAligned({a.state_in, a.dstate_out, a.dq, a.dk, a.dv, a.dstate_in, a.saved, a.scratch});
     if (a.type == DUCK_BFLOAT16 && a.T > 0) {
       backwardChunks(a, reinterpret_cast<cudaStream_t>(stream));
       return;
@@ -386,9 +477,14 @@ int duck_linear_attention_step(const duck_attention *args, duck_stream stream) {
     require(a.q && a.k && a.v && a.out && a.decay && a.state_out, "Invalid arguments");
     StepOf s{a.q, a.k, a.v, a.out, a.state_out, a.decay, a.resets, a.q_stride[1], a.q_stride[2], a.k_stride[1],
              a.k_stride[2], a.v_stride[1], a.v_stride[2], a.E, a.H, a.Dk, a.Dv, a.scale};
+    // Four columns a thread where rows of the state are whole 16-byte pieces.
+    const bool quads = a.Dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.state_out) % 16 == 0;
     withType(a.type, [&](auto zero) {
-      attentionStepAny<decltype(zero)>
-          <<<unsigned(int64_t(a.E) * a.H), 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(s);
+      using T = decltype(zero);
+      const unsigned blocks = unsigned(int64_t(a.E) * a.H);
+      cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+      if (quads) attentionStepQuads<T><<<blocks, 128, 0, st>>>(s);
+      else attentionStepAny<T><<<blocks, 128, 0, st>>>(s);
     });
     check(cudaGetLastError(), "linear attention step launch");
   });

@@ -14,6 +14,14 @@ template <class T> __device__ __forceinline__ T fromFloat(float x);
 template <> __device__ __forceinline__ float fromFloat<float>(float x) { return x; }
 template <> __device__ __forceinline__ bf16 fromFloat<bf16>(float x) { return __float2bfloat16_rn(x); }
 
+// The register type that VEC elements are moved as: 16 bytes, or one element.
+template <class T, int VEC> struct PieceOf {
+  using type = uint4;
+};
+template <class T> struct PieceOf<T, 1> {
+  using type = T;
+};
+
 // Sum over the lanes of a warp, the same bits in every lane.
 __device__ __forceinline__ float warpSum(float x) {
 #pragma unroll

@@ -166,6 +166,12 @@ def _dense_last(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+def _aligned(state):
+    """Dense and on a 16-byte boundary."""
+    state = state.contiguous()
+    return state if state.data_ptr() % 16 == 0 else state.clone()
+
+
 def _sizes(packed):
     out = (ctypes.c_int64 * 3)()
     _raise(library().duck_linear_attention_sizes(packed, out))
@@ -209,7 +215,7 @@ class _LinearAttention(torch.autograd.Function):
         T, E, H, Dk = q.shape
         Dv = v.shape[3]
         dout = q.new_zeros((T, E, H, Dv)) if dout is None else _dense_last(dout)
-        dlast = None if dlast is None else dlast.contiguous()
+        dlast = None if dlast is None else _aligned(dlast)
         dq, dk = (torch.empty((T, E, H, Dk), dtype=q.dtype, device=q.device) for _ in range(2))
         dv = torch.empty((T, E, H, Dv), dtype=q.dtype, device=q.device)
         dstate = torch.empty_like(state) if ctx.needs_input_grad[4] else None
@@ -290,8 +296,8 @@ def linear_attention(q, k, v, decay, state=None, resets=None, scale=None, final_
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     if decay.dtype != torch.float32 or not decay.is_contiguous():
         decay = decay.float().contiguous()
-    if state is not None and not state.is_contiguous():
-        state = state.contiguous()
+    if state is not None:
+        state = _aligned(state)
     if _grad_needed(q, k, v, state):
         return _LinearAttention.apply(q, k, v, decay, state, resets, scale, final_state)
     return _attention_forward(q, k, v, decay, state, resets, scale, final_state, False)[:2]

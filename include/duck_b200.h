@@ -389,7 +389,9 @@ int duck_elu_restore(const void *dy, const int8_t *codes, const float *scales, v
  *   f_t = decay[h], or 0 where resets[t, e] is set (an episode begins at t).
  * q and k are [T, E, H, Dk], v, out and dout [T, E, H, Dv] with 1 <= Dk, Dv <=
  * 128; q, k, v and dout have the strides given, {t, e, h}; the outputs are
- * dense.  States are dense [E, H, Dk, Dv] float32.  decay [H] is in [0, 1]. */
+ * dense.  States are dense [E, H, Dk, Dv] float32.  decay [H] is in [0, 1].
+ * Outputs, workspaces and the states of whole rollouts lie on 16-byte
+ * boundaries. */
 typedef struct duck_attention {
   const void *q, *k, *v;
   void *out;                  /* forward */
