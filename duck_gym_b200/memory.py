@@ -23,6 +23,7 @@ synchronise and can be captured in CUDA graphs.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from typing import NamedTuple
 
@@ -37,22 +38,37 @@ HEAD_MAX = 128   # largest head size of the linear attention
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
-class _Device:
-    """Makes the device of a launch current where it is not, and gives the
-    stream that torch uses there."""
+# The stream and device that torch has current, without the objects around them:
+# the public calls cost more than a launch.
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
-    def __init__(self, device):
-        self.index = device.index
-        self.previous = torch.cuda.current_device()
 
-    def __enter__(self):
-        if self.previous != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+def _launch(entry, device, *args):
+    """Calls a C entry on torch's current stream of `device`."""
+    index = device.index
+    if index == _current_device():
+        status = entry(*args, _stream_of(index))
+    else:
+        with torch.cuda.device(device):
+            status = entry(*args, _stream_of(index))
+    if status:
+        _raise(status)
 
-    def __exit__(self, *unused):
-        if self.previous != self.index:
-            torch.cuda.set_device(self.previous)
+
+def _once(backward):
+    """A backward pass without a second one.  torch's once_differentiable does
+    the bookkeeping for create_graph; it is left out where no graph is made."""
+    twice = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (twice if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
+def _pointer(t):
+    return None if t is None else t.data_ptr()
 
 
 def _require(condition, message):
@@ -79,46 +95,44 @@ def _rows_of(x):
     return x if x.stride(1) == 1 or n == 1 else x.contiguous()
 
 
+def _dense_like(x):
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _norm_forward(x, weight, bias, eps, keep):
-    rows, n = x.shape
-    y = torch.empty((rows, n), dtype=x.dtype, device=x.device)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if keep else None
-    with _Device(x.device) as stream:
-        _raise(library().duck_layer_norm_forward(
-            x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
-            y.data_ptr(), stats.data_ptr() if keep else None, rows, n, x.stride(0), eps, _TYPES[x.dtype], stream))
-    return y, stats
+    rows = _rows_of(x)
+    y = _dense_like(x)
+    stats = torch.empty((rows.shape[0], 2), dtype=torch.float32, device=x.device) if keep else None
+    _launch(library().duck_layer_norm_forward, x.device, rows.data_ptr(), _pointer(weight), _pointer(bias),
+            y.data_ptr(), _pointer(stats), rows.shape[0], rows.shape[1], rows.stride(0), eps, _TYPES[x.dtype])
+    return y, rows, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        rows = _rows_of(x)
-        y, stats = _norm_forward(rows, weight, bias, eps, True)
-        ctx.save_for_backward(rows, weight, stats)
-        ctx.bias = bias is not None
-        return y.view(x.shape)
+        y, rows, stats = _norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(rows, weight, bias, stats)
+        return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        shape, dy = dy.shape, _rows_of(dy)
+        x, weight, bias, stats = ctx.saved_tensors
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         rows, n = x.shape
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(dy.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(bias) if need_b else None
         lib = library()
-        dx = torch.empty((rows, n), dtype=x.dtype, device=x.device) if need_x else None
-        # The weight's and the bias' gradients and the partial sums in one buffer.
-        sums = need_w or need_b
-        floats = torch.empty(2 * n + lib.duck_layer_norm_scratch(rows, n), device=x.device) if sums else None
-        at = floats.data_ptr() if sums else 0
-        with _Device(x.device) as stream:
-            _raise(lib.duck_layer_norm_backward(
-                x.data_ptr(), dy.data_ptr(), None if weight is None else weight.data_ptr(), stats.data_ptr(),
-                dx.data_ptr() if need_x else None, at if need_w else None, at + 4 * n if need_b else None,
-                at + 8 * n if sums else None, rows, n, x.stride(0), dy.stride(0), _TYPES[x.dtype], stream))
-        return (dx.view(shape) if need_x else None, floats[:n] if need_w else None,
-                floats[n:2 * n] if need_b else None, None)
+        scratch = None
+        if need_w or need_b:
+            scratch = torch.empty(lib.duck_layer_norm_scratch(rows, n), dtype=torch.float32, device=x.device)
+        dy = _rows_of(dy)
+        _launch(lib.duck_layer_norm_backward, x.device, x.data_ptr(), dy.data_ptr(), _pointer(weight),
+                stats.data_ptr(), _pointer(dx), _pointer(dw), _pointer(db), _pointer(scratch), rows, n, x.stride(0),
+                dy.stride(0), _TYPES[x.dtype])
+        return dx, dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -140,12 +154,16 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         bias = bias.float().contiguous()
     if _grad_needed(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
-    return _norm_forward(_rows_of(x), weight, bias, eps, False)[0].view(x.shape)
+    return _norm_forward(x, weight, bias, eps, False)[0]
 
 
 # ------------------------------------------------------------ linear attention
 # struct duck_attention of include/duck_b200.h.
 _ATTENTION = struct.Struct("@16P12q6if4x")
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _pack(q, k, v, decay, resets, scale, out=0, state_in=0, state_out=0, dout=None, dstate_out=0, dq=0, dk=0, dv=0,
@@ -158,10 +176,6 @@ def _pack(q, k, v, decay, resets, scale, out=0, state_in=0, state_out=0, dout=No
         T, E, H, Dk, v.shape[3], _TYPES[q.dtype], scale)
 
 
-def _pointer(t):
-    return 0 if t is None else t.data_ptr()
-
-
 def _dense_last(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
@@ -172,10 +186,14 @@ def _aligned(state):
     return state if state.data_ptr() % 16 == 0 else state.clone()
 
 
-def _sizes(packed):
+@functools.lru_cache(maxsize=1024)
+def _workspace(T, E, H, Dk, Dv, kind):
+    """Bytes of scratch of a forward and of a backward call, and of what the
+    first keeps for the second."""
     out = (ctypes.c_int64 * 3)()
-    _raise(library().duck_linear_attention_sizes(packed, out))
-    return out
+    _raise(library().duck_linear_attention_sizes(
+        _ATTENTION.pack(*(0,) * 16, *(0,) * 12, T, E, H, Dk, Dv, kind, 1.0), out))
+    return tuple(out)
 
 
 def _buffer(bytes_, device):
@@ -187,13 +205,12 @@ def _attention_forward(q, k, v, decay, state, resets, scale, final_state, keep):
     Dv = v.shape[3]
     out = torch.empty((T, E, H, Dv), dtype=q.dtype, device=q.device)
     last = torch.empty((E, H, Dk, Dv), dtype=torch.float32, device=q.device) if final_state else None
-    args = dict(out=out.data_ptr(), state_in=_pointer(state), state_out=_pointer(last))
-    sizes = _sizes(_pack(q, k, v, decay, resets, scale, **args))
+    args = dict(out=out.data_ptr(), state_in=_address(state), state_out=_address(last))
+    sizes = _workspace(T, E, H, Dk, Dv, _TYPES[q.dtype])
     scratch = _buffer(sizes[0], q.device)
     saved = _buffer(sizes[2], q.device) if keep else None
-    with _Device(q.device) as stream:
-        _raise(library().duck_linear_attention_forward(
-            _pack(q, k, v, decay, resets, scale, scratch=_pointer(scratch), saved=_pointer(saved), **args), stream))
+    _launch(library().duck_linear_attention_forward, q.device,
+            _pack(q, k, v, decay, resets, scale, scratch=_address(scratch), saved=_address(saved), **args))
     return out, last, saved
 
 
@@ -207,7 +224,7 @@ class _LinearAttention(torch.autograd.Function):
         return out, last
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout, dlast):
         q, k, v, decay, state, resets, saved = ctx.saved_tensors
         if dout is None and dlast is None:
@@ -219,12 +236,11 @@ class _LinearAttention(torch.autograd.Function):
         dq, dk = (torch.empty((T, E, H, Dk), dtype=q.dtype, device=q.device) for _ in range(2))
         dv = torch.empty((T, E, H, Dv), dtype=q.dtype, device=q.device)
         dstate = torch.empty_like(state) if ctx.needs_input_grad[4] else None
-        args = dict(state_in=_pointer(state), dout=dout, dstate_out=_pointer(dlast), dq=dq.data_ptr(),
-                    dk=dk.data_ptr(), dv=dv.data_ptr(), dstate_in=_pointer(dstate), saved=_pointer(saved))
-        scratch = _buffer(_sizes(_pack(q, k, v, decay, resets, ctx.scale, **args))[1], q.device)
-        with _Device(q.device) as stream:
-            _raise(library().duck_linear_attention_backward(
-                _pack(q, k, v, decay, resets, ctx.scale, scratch=_pointer(scratch), **args), stream))
+        args = dict(state_in=_address(state), dout=dout, dstate_out=_address(dlast), dq=dq.data_ptr(),
+                    dk=dk.data_ptr(), dv=dv.data_ptr(), dstate_in=_address(dstate), saved=_address(saved))
+        scratch = _buffer(_workspace(T, E, H, Dk, Dv, _TYPES[q.dtype])[1], q.device)
+        _launch(library().duck_linear_attention_backward, q.device,
+                _pack(q, k, v, decay, resets, ctx.scale, scratch=_address(scratch), **args))
         return dq, dk, dv, None, dstate, None, None, None
 
 
@@ -326,12 +342,11 @@ def linear_attention_step(q, k, v, decay, state, reset=None, scale=None):
         decay = decay.float().contiguous()
     E, H, Dk = q.shape
     out = torch.empty((E, H, v.shape[2]), dtype=q.dtype, device=q.device)
-    with _Device(q.device) as stream:
-        _raise(library().duck_linear_attention_step(
+    _launch(library().duck_linear_attention_step, q.device,
             _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr(),
-                            _pointer(reset), 0, state.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0,
+                            _address(reset), 0, state.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0,
                             0, *q.stride()[:2], 0, *k.stride()[:2], 0, *v.stride()[:2], 0, 0, 0,
-                            1, E, H, Dk, v.shape[2], _TYPES[q.dtype], scale), stream))
+                            1, E, H, Dk, v.shape[2], _TYPES[q.dtype], scale))
     return out
 
 
@@ -376,9 +391,8 @@ def elu_checkpoint(x):
     y = torch.empty_like(x)
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scales = torch.empty((*x.shape[:-1], -(-n // GROUP)), dtype=torch.float32, device=x.device)
-    with _Device(x.device) as stream:
-        _raise(library().duck_elu_checkpoint(x.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-                                             x.numel() // n, n, _TYPES[x.dtype], stream))
+    _launch(library().duck_elu_checkpoint, x.device, x.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+            x.numel() // n, n, _TYPES[x.dtype])
     return y, Checkpoint8(codes, scales)
 
 
@@ -401,9 +415,8 @@ def elu_restore(dy, kept, restore=True):
     n = dy.shape[-1]
     dx = torch.empty_like(dy)
     y = torch.empty_like(dy) if restore else None
-    with _Device(dy.device) as stream:
-        _raise(library().duck_elu_restore(dy.data_ptr(), codes.data_ptr(), scales.data_ptr(), _pointer(y),
-                                          dx.data_ptr(), dy.numel() // n, n, _TYPES[dy.dtype], stream))
+    _launch(library().duck_elu_restore, dy.device, dy.data_ptr(), codes.data_ptr(), scales.data_ptr(), _pointer(y),
+            dx.data_ptr(), dy.numel() // n, n, _TYPES[dy.dtype])
     return dx, y
 
 
@@ -422,7 +435,7 @@ class _CheckpointedMLP(torch.autograd.Function):
         return x
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dz):
         saved, n = ctx.saved_tensors, ctx.layers
         weights = saved[2 * n - 1:]

@@ -410,8 +410,8 @@ typedef struct duck_attention {
   float scale;
 } duck_attention;
 
-/* Bytes of workspace for a call of these sizes (only T, E, H, Dk, Dv, type and
- * which pointers are NULL are looked at): out[0] scratch of the forward call,
+/* Bytes of workspace for calls of these sizes (only T, E, H, Dk, Dv and type are
+ * looked at): out[0] scratch of the forward call,
  * out[1] scratch of the backward call, out[2] `saved`, which a forward call that
  * a backward call will follow has to be given. */
 int duck_linear_attention_sizes(const duck_attention *args, int64_t *out);
