@@ -790,16 +790,25 @@ __global__ void __launch_bounds__(256) joinSegments(float *segments, const uint8
   if (x >= stateSize) return;
   const float d = decay[eh % H], logDecay = fmaxf(log2f(d), -1e30f);
   float S = init ? init[eh * stateSize + x] : 0.f;
-  for (int u = 0; u < segmentCount; ++u) {
-    const int s = reverse ? segmentCount - 1 - u : u;
-    float *at = segments + (eh * segmentCount + s) * stateSize + x;
-    const bool final = u + 1 == segmentCount;
-    const float added = final ? 0.f : *at;
-    *at = S;
-    if (final) break;
-    const int length = min(segmentLength, T - s * segmentLength);
-    const float f = d >= 0.f ? exp2f(float(length) * logDecay) : __int_as_float(0x7fc00000);
-    S = cut[eh * segmentCount + s] ? added : fmaf(f, S, added);
+  float *states = segments + eh * segmentCount * stateSize + x;
+  constexpr int AHEAD = 8;   // loads in flight: the chain itself is a multiplication a segment
+  for (int u0 = 0; u0 < segmentCount; u0 += AHEAD) {
+    float added[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int u = u0 + k, s = reverse ? segmentCount - 1 - u : u;
+      added[k] = u + 1 < segmentCount ? states[s * stateSize] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int u = u0 + k, s = reverse ? segmentCount - 1 - u : u;
+      if (u >= segmentCount) break;
+      states[s * stateSize] = S;
+      if (u + 1 == segmentCount) break;
+      const int length = min(segmentLength, T - s * segmentLength);
+      const float f = d >= 0.f ? exp2f(float(length) * logDecay) : __int_as_float(0x7fc00000);
+      S = cut[eh * segmentCount + s] ? added[k] : fmaf(f, S, added[k]);
+    }
   }
 }
 
@@ -815,14 +824,14 @@ template <int DI> __device__ __forceinline__ void redoFlagged(const Sweep &s, co
   for (int64_t eh = first; eh < end; ++eh) {
     any = false;
     for (int x = threadIdx.x; x < count; x += blockDim.x) any |= flags[eh * count + x] != 0;
-    if (__syncthreads_or(any)) scanSteps<bf16, DI>(s, eh, blockIdx.y * blockDim.x + threadIdx.x);
+    if (__syncthreads_or(any)) scanSteps<bf16, DI>(s, eh, blockIdx.y);
   }
 }
-template <int DI> __global__ void __launch_bounds__(128) redoAttention(Sweep s, const uint8_t *flags, int count) {
+template <int DI> __global__ void __launch_bounds__(scanThreads(DI)) redoAttention(Sweep s, const uint8_t *flags, int count) {
   redoFlagged<DI>(s, flags, count);
 }
 template <int DI>
-__global__ void __launch_bounds__(128) redoBackward(Sweep q, Sweep k, Sweep v, const uint8_t *flags, int count) {
+__global__ void __launch_bounds__(scanThreads(DI)) redoBackward(Sweep q, Sweep k, Sweep v, const uint8_t *flags, int count) {
   if (blockIdx.z == 0) redoFlagged<DI>(q, flags, count);
   else if (blockIdx.z == 1) redoFlagged<DI>(k, flags, count);
   else redoFlagged<DI>(v, flags, count);

@@ -40,55 +40,103 @@ struct Sweep {
   float mulA, mulC;
 };
 
-constexpr int kScanSteps = 16;
+// The recurrence step by step: float32 operands, and what redoAttention() finds.
+//
+// A block has 32 columns of the state of one (e, h); a column's DI rows are split
+// over scanLanes() neighbouring lanes, at most 16 rows each, so that a step is a
+// short chain: three operations a row and a reduction over those lanes.  The
+// operands of 16 steps lie in shared memory while those of the next 16 are on
+// their way in registers; outputs leave 16 steps at a time.  Bound by instructions,
+// 3 a row and column and step, and not by memory.
+constexpr int kScanSteps = 16, kScanColumns = 32;
+__host__ __device__ constexpr int scanLanes(int rows) { return rows > 64 ? 8 : 4; }
+__host__ __device__ constexpr int scanThreads(int rows) { return kScanColumns * scanLanes(rows); }
 
-// One thread per column of the state, its DI rows in registers; the rows'
-// operands of 16 steps at a time in shared memory.
-template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int j) {
+template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile) {
+  constexpr int LANES = scanLanes(DI), R = DI / LANES, THREADS = scanThreads(DI);
+  constexpr int AC = kScanSteps * DI / THREADS, B = kScanSteps * kScanColumns / THREADS;   // values a thread fetches
   __shared__ __align__(16) float a[kScanSteps][DI], c[kScanSteps][DI];
+  __shared__ float b[kScanSteps][kScanColumns], y[kScanSteps][kScanColumns];
   __shared__ uint8_t cut[kScanSteps];
   const int e = int(eh / s.H), h = int(eh - int64_t(e) * s.H);
+  const int lane = threadIdx.x % LANES, column = threadIdx.x / LANES, first = tile * kScanColumns;
+  const int j = first + column, i0 = lane * R;
   const bool live = j < s.Dj;
   const T *pa = static_cast<const T *>(s.a) + e * s.as.e + h * s.as.h;
-  const T *pb = static_cast<const T *>(s.b) + e * s.bs.e + h * s.bs.h + (live ? j : 0);
+  const T *pb = static_cast<const T *>(s.b) + e * s.bs.e + h * s.bs.h + first;
   const T *pc = static_cast<const T *>(s.c) + e * s.cs.e + h * s.cs.h;
-  T *py = static_cast<T *>(s.y) + eh * s.Dj + j;
+  T *py = static_cast<T *>(s.y) + eh * s.Dj + first;
   const int64_t yt = int64_t(s.E) * s.H * s.Dj, base = eh * s.Di * s.Dj;
   const float decay = s.decay[h];
-  float x[DI];
+  float x[R];
 #pragma unroll
-  for (int i = 0; i < DI; ++i) x[i] = s.init && live && i < s.Di ? s.init[base + int64_t(i) * s.ri + int64_t(j) * s.rj] : 0.f;
+  for (int r = 0; r < R; ++r)
+    x[r] = s.init && live && i0 + r < s.Di ? s.init[base + int64_t(i0 + r) * s.ri + int64_t(j) * s.rj] : 0.f;
+  float nextA[AC], nextC[AC], nextB[B];
+  bool nextCut = false;
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int n = 0; n < AC; ++n) {
+      const int q = n * THREADS + threadIdx.x, u = q / DI, i = q % DI;
+      const bool in = t0 + u < s.T && i < s.Di;
+      const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
+      nextA[n] = in ? s.mulA * toFloat(pa[t * s.as.t + i]) : 0.f;
+      nextC[n] = in ? s.mulC * toFloat(pc[t * s.cs.t + i]) : 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < B; ++n) {
+      const int q = n * THREADS + threadIdx.x, u = q / kScanColumns, k = q % kScanColumns;
+      const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
+      nextB[n] = t0 + u < s.T && first + k < s.Dj ? toFloat(pb[t * s.bs.t + k]) : 0.f;
+    }
+    // The factor between a step and the one before it in the sweep: the reset of
+    // the later of the two in time.
+    const int u = threadIdx.x;
+    const int64_t t = s.reverse ? s.T - (t0 + u) : t0 + u;
+    nextCut = u < kScanSteps && t0 + u < s.T && s.resets && t < s.T && s.resets[t * s.E + e];
+  };
+  if (s.T > 0) fetch(0);
   for (int t0 = 0; t0 < s.T; t0 += kScanSteps) {
     const int count = min(kScanSteps, s.T - t0);
     __syncthreads();
-    for (int q = threadIdx.x; q < count * DI; q += blockDim.x) {
-      const int u = q / DI, i = q - u * DI;
-      const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
-      a[u][i] = i < s.Di ? s.mulA * toFloat(pa[t * s.as.t + i]) : 0.f;
-      c[u][i] = i < s.Di ? s.mulC * toFloat(pc[t * s.cs.t + i]) : 0.f;
+#pragma unroll
+    for (int n = 0; n < AC; ++n) {
+      const int q = n * THREADS + threadIdx.x;
+      (&a[0][0])[q] = nextA[n];
+      (&c[0][0])[q] = nextC[n];
     }
-    for (int u = threadIdx.x; u < count; u += blockDim.x) {
-      // The factor between a step and the one before it in the sweep: the
-      // reset of the later of the two in time.
-      const int64_t t = s.reverse ? s.T - (t0 + u) : t0 + u;
-      cut[u] = s.resets && t < s.T ? s.resets[t * s.E + e] : 0;
-    }
+#pragma unroll
+    for (int n = 0; n < B; ++n) (&b[0][0])[n * THREADS + threadIdx.x] = nextB[n];
+    if (threadIdx.x < kScanSteps) cut[threadIdx.x] = nextCut;
     __syncthreads();
+    if (t0 + kScanSteps < s.T) fetch(t0 + kScanSteps);
+#pragma unroll 4
     for (int u = 0; u < count; ++u) {
-      const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
-      const float b = live ? toFloat(pb[t * s.bs.t]) : 0.f;
+      const float value = b[u][column];
       const float f = s.reverse && t0 + u == 0 ? 1.f : decay;
       if (cut[u]) {
 #pragma unroll
-        for (int i = 0; i < DI; ++i) x[i] = 0.f;
+        for (int r = 0; r < R; ++r) x[r] = 0.f;
       }
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < DI; ++i) {
-        x[i] = fmaf(f, x[i], a[u][i] * b);
-        y[i & 3] = fmaf(c[u][i], x[i], y[i & 3]);
+      for (int r = 0; r < R; ++r) {
+        x[r] = fmaf(f, x[r], a[u][i0 + r] * value);
+        sum[r & 1] = fmaf(c[u][i0 + r], x[r], sum[r & 1]);
       }
-      if (live && s.y) py[t * yt] = fromFloat<T>((y[0] + y[1]) + (y[2] + y[3]));
+      float total = sum[0] + sum[1];
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      if (lane == 0) y[u][column] = total;
+    }
+    __syncthreads();
+    if (s.y) {
+#pragma unroll
+      for (int n = 0; n < B; ++n) {
+        const int q = n * THREADS + threadIdx.x, u = q / kScanColumns, k = q % kScanColumns;
+        const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
+        if (u < count && first + k < s.Dj) py[t * yt + k] = fromFloat<T>(y[u][k]);
+      }
     }
   }
   if (s.last && live) {
@@ -96,13 +144,13 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
     const bool gone = s.reverse && s.T > 0 && s.resets && s.resets[e];
     const float f = s.reverse && s.T > 0 ? decay : 1.f;
 #pragma unroll
-    for (int i = 0; i < DI; ++i)
-      if (i < s.Di) s.last[base + int64_t(i) * s.ri + int64_t(j) * s.rj] = gone ? 0.f : f * x[i];
+    for (int r = 0; r < R; ++r)
+      if (i0 + r < s.Di) s.last[base + int64_t(i0 + r) * s.ri + int64_t(j) * s.rj] = gone ? 0.f : f * x[r];
   }
 }
 
-template <class T, int DI> __global__ void __launch_bounds__(128) attentionScan(Sweep s) {
-  scanSteps<T, DI>(s, blockIdx.x, blockIdx.y * blockDim.x + threadIdx.x);
+template <class T, int DI> __global__ void __launch_bounds__(scanThreads(DI)) attentionScan(Sweep s) {
+  scanSteps<T, DI>(s, blockIdx.x, blockIdx.y);
 }
 
 struct StepOf {

@@ -15,13 +15,6 @@ using namespace duckb200;
 
 namespace {
 
-int multiprocessors() {
-  int device = 0, n = 0;
-  check(cudaGetDevice(&device), "cudaGetDevice");
-  check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device), "cudaDeviceGetAttribute");
-  return n;
-}
-
 // Calls f with a value of the element type.
 template <class F> void withType(int type, F &&f) {
   if (type == DUCK_FLOAT32) f(0.f);
@@ -107,28 +100,29 @@ void requireAligned(std::initializer_list<const void *> pointers) {
     require(reinterpret_cast<uintptr_t>(p) % 16 == 0, "States, outputs and workspaces have to be 16-byte aligned");
 }
 
+template <class T, int DI> void launchScan(const Sweep &s, cudaStream_t stream) {
+  const dim3 grid(unsigned(int64_t(s.E) * s.H), unsigned(ceilDiv(s.Dj, kScanColumns)));
+  attentionScan<T, DI><<<grid, scanThreads(DI), 0, stream>>>(s);
+}
 template <class T> void launchScan(const Sweep &s, cudaStream_t stream) {
-  const int threads = std::min(128, int(ceilDiv(s.Dj, 32)) * 32);
-  const dim3 grid(unsigned(int64_t(s.E) * s.H), unsigned(ceilDiv(s.Dj, threads)));
-  if (s.Di <= 16) attentionScan<T, 16><<<grid, threads, 0, stream>>>(s);
-  else if (s.Di <= 32) attentionScan<T, 32><<<grid, threads, 0, stream>>>(s);
-  else if (s.Di <= 64) attentionScan<T, 64><<<grid, threads, 0, stream>>>(s);
-  else attentionScan<T, 128><<<grid, threads, 0, stream>>>(s);
+  if (s.Di <= 16) launchScan<T, 16>(s, stream);
+  else if (s.Di <= 32) launchScan<T, 32>(s, stream);
+  else if (s.Di <= 64) launchScan<T, 64>(s, stream);
+  else launchScan<T, 128>(s, stream);
   check(cudaGetLastError(), "linear attention launch");
 }
 
 void launchRedo(const Sweep &s, const uint8_t *flags, int count, cudaStream_t stream) {
-  const int threads = std::min(128, int(ceilDiv(s.Dj, 32)) * 32);
-  const dim3 grid(unsigned(std::min<int64_t>(int64_t(s.E) * s.H, 148)), unsigned(ceilDiv(s.Dj, threads)));
-  if (s.Di <= 32) redoAttention<32><<<grid, threads, 0, stream>>>(s, flags, count);
-  else redoAttention<128><<<grid, threads, 0, stream>>>(s, flags, count);
+  const dim3 grid(unsigned(std::min<int64_t>(int64_t(s.E) * s.H, 148)), unsigned(ceilDiv(s.Dj, kScanColumns)));
+  if (s.Di <= 32) redoAttention<32><<<grid, scanThreads(32), 0, stream>>>(s, flags, count);
+  else redoAttention<128><<<grid, scanThreads(128), 0, stream>>>(s, flags, count);
   check(cudaGetLastError(), "linear attention launch");
 }
 void launchRedo(const Sweep &q, const Sweep &k, const Sweep &v, const uint8_t *flags, int count, cudaStream_t stream) {
-  const int most = std::max(q.Di, q.Dj), threads = std::min(128, int(ceilDiv(most, 32)) * 32);
-  const dim3 grid(unsigned(std::min<int64_t>(int64_t(q.E) * q.H, 148)), unsigned(ceilDiv(most, threads)), 3);
-  if (most <= 32) redoBackward<32><<<grid, threads, 0, stream>>>(q, k, v, flags, count);
-  else redoBackward<128><<<grid, threads, 0, stream>>>(q, k, v, flags, count);
+  const int most = std::max(q.Di, q.Dj);
+  const dim3 grid(unsigned(std::min<int64_t>(int64_t(q.E) * q.H, 148)), unsigned(ceilDiv(most, kScanColumns)), 3);
+  if (most <= 32) redoBackward<32><<<grid, scanThreads(32), 0, stream>>>(q, k, v, flags, count);
+  else redoBackward<128><<<grid, scanThreads(128), 0, stream>>>(q, k, v, flags, count);
   check(cudaGetLastError(), "linear attention backward launch");
 }
 
@@ -154,22 +148,26 @@ struct ChunkPlan {
   int C, columnTiles, segmentLength, segmentCount, chunks;
   int64_t stateSize, segmentBytes, cutBytes, flagBytes;   // of the scratch, in this order
 };
-ChunkPlan planChunks(const duck_attention &a) {
+// With fewer blocks than half of what fits on the GPU at once, T is split so that
+// the segments' blocks fill it once: a second, partly filled round costs as much as a
+// full one (a replay of 16384 steps, 8 heads of 128: 187 us in 26 segments).
+ChunkPlan planChunks(const duck_attention &a, bool backward) {
   ChunkPlan p{};
   p.C = a.T <= 32 ? 32 : 64;
-  p.columnTiles = int(ceilDiv(a.Dv, 64));
+  p.columnTiles = backward ? 1 : int(ceilDiv(a.Dv, 64));
   p.chunks = int(ceilDiv(a.T, p.C));
   p.stateSize = int64_t(a.Dk) * a.Dv;
   const int64_t blocks = int64_t(a.E) * a.H * p.columnTiles;
-  const int64_t want = blocks < 296 ? std::min<int64_t>(ceilDiv(p.chunks, 4), ceilDiv(444, blocks)) : 1;
-  p.segmentLength = int(ceilDiv(p.chunks, std::max<int64_t>(1, want))) * p.C;
-  p.segmentCount = std::max(1, int(ceilDiv(a.T, p.segmentLength ? p.segmentLength : 1)));
+  const int64_t fit = std::max(a.Dk, a.Dv) <= 64 ? 3 * 148 : backward ? 148 : 2 * 148;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(p.chunks / 4, fit / blocks));
+  p.segmentLength = int(ceilDiv(std::max(1, p.chunks), want)) * p.C;
+  p.segmentCount = std::max(1, int(ceilDiv(a.T, p.segmentLength)));
   const int64_t states = int64_t(a.E) * a.H * p.segmentCount;
   if (p.segmentCount > 1) {
     p.segmentBytes = states * p.stateSize * 4;
     p.cutBytes = states;
   }
-  p.flagBytes = states * p.columnTiles;   // the backward call needs one a segment only
+  p.flagBytes = states * p.columnTiles;
   return p;
 }
 
@@ -209,7 +207,7 @@ void launchChunks(const ChunkArgs &a, int segments, int buffers, cudaStream_t st
 }
 
 void forwardChunks(const duck_attention &a, cudaStream_t stream) {
-  const ChunkPlan plan = planChunks(a);
+  const ChunkPlan plan = planChunks(a, false);
   const bool split = plan.segmentCount > 1;
   require(a.scratch, "Invalid arguments");
   ChunkArgs c{};
@@ -270,7 +268,7 @@ void launchBackward(const BackwardArgs &a, int segments, cudaStream_t stream) {
 }
 
 void backwardChunks(const duck_attention &a, cudaStream_t stream) {
-  const ChunkPlan plan = planChunks(a);
+  const ChunkPlan plan = planChunks(a, true);
   const bool split = plan.segmentCount > 1;
   require(a.scratch && (plan.chunks <= 1 || a.saved), "Invalid arguments");
   BackwardArgs c{};
@@ -430,8 +428,9 @@ int duck_linear_attention_sizes(const duck_attention *args, int64_t *out) {
     require(out != nullptr, "Invalid arguments");
     out[0] = out[1] = out[2] = 0;
     if (!attentionChecked(args) || args->type != DUCK_BFLOAT16 || args->T == 0) return;
-    const ChunkPlan plan = planChunks(*args);
-    out[0] = out[1] = plan.segmentBytes + plan.cutBytes + plan.flagBytes;
+    const ChunkPlan plan = planChunks(*args, false), back = planChunks(*args, true);
+    out[0] = plan.segmentBytes + plan.cutBytes + plan.flagBytes;
+    out[1] = back.segmentBytes + back.cutBytes + back.flagBytes;
     out[2] = plan.chunks > 1 ? int64_t(args->E) * args->H * plan.chunks * plan.stateSize * 2 : 0;
   });
 }
