@@ -814,8 +814,11 @@ __global__ void __launch_bounds__(256) joinSegments(float *segments, const uint8
 
 // Sweeps of a call step by step, for the environments and heads that have one of
 // their `count` flags set; usually none has.  A block has a run of them and looks
-// at all its flags at once first.  blockIdx.z says which sweep.
-template <int DI> __device__ __forceinline__ void redoFlagged(const Sweep &s, const uint8_t *flags, int count) {
+// at all its flags at once first.
+template <int DI>
+__global__ void __launch_bounds__(scanThreads(DI))
+    redoAttention(const __grid_constant__ Sweeps p, const uint8_t *flags, int count) {
+  const Sweep &s = p.s[blockIdx.z];
   const int64_t all = int64_t(s.E) * s.H, run = (all + gridDim.x - 1) / gridDim.x;
   const int64_t first = blockIdx.x * run, end = min(all, first + run);
   bool any = false;
@@ -826,15 +829,6 @@ template <int DI> __device__ __forceinline__ void redoFlagged(const Sweep &s, co
     for (int x = threadIdx.x; x < count; x += blockDim.x) any |= flags[eh * count + x] != 0;
     if (__syncthreads_or(any)) scanSteps<bf16, DI>(s, eh, blockIdx.y);
   }
-}
-template <int DI> __global__ void __launch_bounds__(scanThreads(DI)) redoAttention(Sweep s, const uint8_t *flags, int count) {
-  redoFlagged<DI>(s, flags, count);
-}
-template <int DI>
-__global__ void __launch_bounds__(scanThreads(DI)) redoBackward(Sweep q, Sweep k, Sweep v, const uint8_t *flags, int count) {
-  if (blockIdx.z == 0) redoFlagged<DI>(q, flags, count);
-  else if (blockIdx.z == 1) redoFlagged<DI>(k, flags, count);
-  else redoFlagged<DI>(v, flags, count);
 }
 
 }  // namespace duckb200

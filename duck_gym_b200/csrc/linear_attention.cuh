@@ -61,6 +61,7 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
   const int e = int(eh / s.H), h = int(eh - int64_t(e) * s.H);
   const int lane = threadIdx.x % LANES, column = threadIdx.x / LANES, first = tile * kScanColumns;
   const int j = first + column, i0 = lane * R;
+  if (first >= s.Dj) return;   // the sweeps of a call may differ in their columns
   const bool live = j < s.Dj;
   const T *pa = static_cast<const T *>(s.a) + e * s.as.e + h * s.as.h;
   const T *pb = static_cast<const T *>(s.b) + e * s.bs.e + h * s.bs.h + first;
@@ -149,8 +150,13 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
   }
 }
 
-template <class T, int DI> __global__ void __launch_bounds__(scanThreads(DI)) attentionScan(Sweep s) {
-  scanSteps<T, DI>(s, blockIdx.x, blockIdx.y);
+// Up to three sweeps of one call, the blocks' third index.
+struct Sweeps {
+  Sweep s[3];
+};
+template <class T, int DI>
+__global__ void __launch_bounds__(scanThreads(DI)) attentionScan(const __grid_constant__ Sweeps p) {
+  scanSteps<T, DI>(p.s[blockIdx.z], blockIdx.x, blockIdx.y);
 }
 
 struct StepOf {

@@ -100,30 +100,35 @@ void requireAligned(std::initializer_list<const void *> pointers) {
     require(reinterpret_cast<uintptr_t>(p) % 16 == 0, "States, outputs and workspaces have to be 16-byte aligned");
 }
 
-template <class T, int DI> void launchScan(const Sweep &s, cudaStream_t stream) {
-  const dim3 grid(unsigned(int64_t(s.E) * s.H), unsigned(ceilDiv(s.Dj, kScanColumns)));
-  attentionScan<T, DI><<<grid, scanThreads(DI), 0, stream>>>(s);
+// The most rows and columns of some sweeps' states.
+int mostRows(const Sweeps &p, int count) {
+  int n = 0;
+  for (int i = 0; i < count; ++i) n = std::max(n, p.s[i].Di);
+  return n;
 }
-template <class T> void launchScan(const Sweep &s, cudaStream_t stream) {
-  if (s.Di <= 16) launchScan<T, 16>(s, stream);
-  else if (s.Di <= 32) launchScan<T, 32>(s, stream);
-  else if (s.Di <= 64) launchScan<T, 64>(s, stream);
-  else launchScan<T, 128>(s, stream);
+int mostColumns(const Sweeps &p, int count) {
+  int n = 0;
+  for (int i = 0; i < count; ++i) n = std::max(n, p.s[i].Dj);
+  return n;
+}
+template <class T> void launchScan(const Sweeps &p, int count, cudaStream_t stream) {
+  const int rows = mostRows(p, count);
+  const dim3 grid(unsigned(int64_t(p.s[0].E) * p.s[0].H), unsigned(ceilDiv(mostColumns(p, count), kScanColumns)),
+                  unsigned(count));
+  if (rows <= 16) attentionScan<T, 16><<<grid, scanThreads(16), 0, stream>>>(p);
+  else if (rows <= 32) attentionScan<T, 32><<<grid, scanThreads(32), 0, stream>>>(p);
+  else if (rows <= 64) attentionScan<T, 64><<<grid, scanThreads(64), 0, stream>>>(p);
+  else attentionScan<T, 128><<<grid, scanThreads(128), 0, stream>>>(p);
   check(cudaGetLastError(), "linear attention launch");
 }
-
-void launchRedo(const Sweep &s, const uint8_t *flags, int count, cudaStream_t stream) {
-  const dim3 grid(unsigned(std::min<int64_t>(int64_t(s.E) * s.H, 148)), unsigned(ceilDiv(s.Dj, kScanColumns)));
-  if (s.Di <= 32) redoAttention<32><<<grid, scanThreads(32), 0, stream>>>(s, flags, count);
-  else redoAttention<128><<<grid, scanThreads(128), 0, stream>>>(s, flags, count);
+// One round of blocks: there is usually nothing to do but to look at the flags.
+void launchRedo(const Sweeps &p, int count, const uint8_t *flags, int flagCount, cudaStream_t stream) {
+  const int64_t tiles = ceilDiv(mostColumns(p, count), kScanColumns);
+  const int64_t blocks = std::min<int64_t>(int64_t(p.s[0].E) * p.s[0].H, 148 / (tiles * count));
+  const dim3 grid{unsigned(blocks), unsigned(tiles), unsigned(count)};
+  if (mostRows(p, count) <= 32) redoAttention<32><<<grid, scanThreads(32), 0, stream>>>(p, flags, flagCount);
+  else redoAttention<128><<<grid, scanThreads(128), 0, stream>>>(p, flags, flagCount);
   check(cudaGetLastError(), "linear attention launch");
-}
-void launchRedo(const Sweep &q, const Sweep &k, const Sweep &v, const uint8_t *flags, int count, cudaStream_t stream) {
-  const int most = std::max(q.Di, q.Dj);
-  const dim3 grid(unsigned(std::min<int64_t>(int64_t(q.E) * q.H, 148)), unsigned(ceilDiv(most, kScanColumns)), 3);
-  if (most <= 32) redoBackward<32><<<grid, scanThreads(32), 0, stream>>>(q, k, v, flags, count);
-  else redoBackward<128><<<grid, scanThreads(128), 0, stream>>>(q, k, v, flags, count);
-  check(cudaGetLastError(), "linear attention backward launch");
 }
 
 Sweep forwardSweep(const duck_attention &a) {
@@ -247,7 +252,7 @@ void forwardChunks(const duck_attention &a, cudaStream_t stream) {
   if (plan.C == 32) advance ? launchChunks<32, true, true>(c, 1, 1, stream) : launchChunks<32, true, false>(c, 1, 1, stream);
   else advance ? launchChunks<64, true, true>(c, plan.segmentCount, buffers, stream)
                : launchChunks<64, true, false>(c, 1, 1, stream);
-  launchRedo(forwardSweep(a), c.flags, plan.segmentCount * plan.columnTiles, stream);
+  launchRedo({{forwardSweep(a)}}, 1, c.flags, plan.segmentCount * plan.columnTiles, stream);
 }
 
 template <int C, int D, bool OUT, bool STATE>
@@ -312,7 +317,7 @@ void backwardChunks(const duck_attention &a, cudaStream_t stream) {
   if (plan.C == 32) advance ? launchBackward<32, true, true>(c, 1, stream) : launchBackward<32, true, false>(c, 1, stream);
   else advance ? launchBackward<64, true, true>(c, plan.segmentCount, stream)
                : launchBackward<64, true, false>(c, 1, stream);
-  launchRedo(gradientOfQ(a), gradientOfK(a), gradientOfV(a), c.flags, plan.segmentCount, stream);
+  launchRedo({{gradientOfQ(a), gradientOfK(a), gradientOfV(a)}}, 3, c.flags, plan.segmentCount, stream);
 }
 
 }  // namespace
@@ -445,8 +450,8 @@ int duck_linear_attention_forward(const duck_attention *args, duck_stream stream
       forwardChunks(a, reinterpret_cast<cudaStream_t>(stream));
       return;
     }
-    const Sweep s = forwardSweep(a);
-    withType(a.type, [&](auto zero) { launchScan<decltype(zero)>(s, reinterpret_cast<cudaStream_t>(stream)); });
+    const Sweeps p{{forwardSweep(a)}};
+    withType(a.type, [&](auto zero) { launchScan<decltype(zero)>(p, 1, reinterpret_cast<cudaStream_t>(stream)); });
   });
 }
 
@@ -460,12 +465,8 @@ int duck_linear_attention_backward(const duck_attention *args, duck_stream strea
       backwardChunks(a, reinterpret_cast<cudaStream_t>(stream));
       return;
     }
-    withType(a.type, [&](auto zero) {
-      using T = decltype(zero);
-      launchScan<T>(gradientOfQ(a), reinterpret_cast<cudaStream_t>(stream));
-      launchScan<T>(gradientOfK(a), reinterpret_cast<cudaStream_t>(stream));
-      launchScan<T>(gradientOfV(a), reinterpret_cast<cudaStream_t>(stream));
-    });
+    const Sweeps p{{gradientOfQ(a), gradientOfK(a), gradientOfV(a)}};
+    withType(a.type, [&](auto zero) { launchScan<decltype(zero)>(p, 3, reinterpret_cast<cudaStream_t>(stream)); });
   });
 }
 
