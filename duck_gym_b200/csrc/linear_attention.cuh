@@ -42,54 +42,95 @@ struct Sweep {
 
 // The recurrence step by step: float32 operands, and what redoAttention() finds.
 //
-// A block has 32 columns of the state of one (e, h); a column's DI rows are split
-// over scanLanes() neighbouring lanes, at most 16 rows each, so that a step is a
-// short chain: three operations a row and a reduction over those lanes.  The
-// operands of 16 steps lie in shared memory while those of the next 16 are on
-// their way in registers; outputs leave 16 steps at a time.  Bound by instructions,
-// 3 a row and column and step, and not by memory.
+// A block has 32 columns of the state of one (e, h).  A thread has two of them and
+// at most 16 of their rows, the others lie with its neighbouring lanes, so that a
+// step is a short chain: three operations a row, two rows in one instruction
+// (float32 pairs), and a reduction over scanLanes() lanes.  The operands of 16
+// steps lie in shared memory while those of the next 16 are on their way in
+// registers; outputs leave 16 steps at a time.  Bound by instructions and shared
+// memory: each operand is moved from memory once.
 constexpr int kScanSteps = 16, kScanColumns = 32;
-__host__ __device__ constexpr int scanLanes(int rows) { return rows > 64 ? 8 : 4; }
-__host__ __device__ constexpr int scanThreads(int rows) { return kScanColumns * scanLanes(rows); }
+__host__ __device__ constexpr int scanLanes(int rows) { return rows > 64 ? 8 : rows > 16 ? 4 : 2; }
+__host__ __device__ constexpr int scanThreads(int rows) { return kScanColumns / 2 * scanLanes(rows); }
+
+// Two float32 numbers in one register pair, and operations on both.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pairOf(float low, float high) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(low), "f"(high));
+  return p;
+}
+__device__ __forceinline__ float2 parts(Pair p) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile) {
   constexpr int LANES = scanLanes(DI), R = DI / LANES, THREADS = scanThreads(DI);
   constexpr int AC = kScanSteps * DI / THREADS, B = kScanSteps * kScanColumns / THREADS;   // values a thread fetches
   __shared__ __align__(16) float a[kScanSteps][DI], c[kScanSteps][DI];
-  __shared__ float b[kScanSteps][kScanColumns], y[kScanSteps][kScanColumns];
+  __shared__ __align__(16) float b[kScanSteps][kScanColumns], y[kScanSteps][kScanColumns];
+  __shared__ float factor[kScanSteps];
   __shared__ uint8_t cut[kScanSteps];
   const int e = int(eh / s.H), h = int(eh - int64_t(e) * s.H);
-  const int lane = threadIdx.x % LANES, column = threadIdx.x / LANES, first = tile * kScanColumns;
+  const int lane = threadIdx.x % LANES, column = threadIdx.x / LANES * 2, first = tile * kScanColumns;
   const int j = first + column, i0 = lane * R;
   if (first >= s.Dj) return;   // the sweeps of a call may differ in their columns
-  const bool live = j < s.Dj;
   const T *pa = static_cast<const T *>(s.a) + e * s.as.e + h * s.as.h;
   const T *pb = static_cast<const T *>(s.b) + e * s.bs.e + h * s.bs.h + first;
   const T *pc = static_cast<const T *>(s.c) + e * s.cs.e + h * s.cs.h;
   T *py = static_cast<T *>(s.y) + eh * s.Dj + first;
   const int64_t yt = int64_t(s.E) * s.H * s.Dj, base = eh * s.Di * s.Dj;
   const float decay = s.decay[h];
-  float x[R];
+  Pair x[2][R / 2];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    x[r] = s.init && live && i0 + r < s.Di ? s.init[base + int64_t(i0 + r) * s.ri + int64_t(j) * s.rj] : 0.f;
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int r = 0; r < R / 2; ++r) {
+      float v[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int i = i0 + 2 * r + n;
+        v[n] = s.init && j + k < s.Dj && i < s.Di ? s.init[base + int64_t(i) * s.ri + int64_t(j + k) * s.rj] : 0.f;
+      }
+      x[k][r] = pairOf(v[0], v[1]);
+    }
+  // A thread fetches one row's value of every RP-th step and one column's of every
+  // BP-th, along pointers that go from tile to tile.
+  constexpr int RP = THREADS / DI, BP = THREADS / kScanColumns;
+  const int uA = threadIdx.x / DI, iA = threadIdx.x % DI, uB = threadIdx.x / kScanColumns, kB = threadIdx.x % kScanColumns;
+  const int64_t dir = s.reverse ? -1 : 1, begin = s.reverse ? s.T - 1 : 0;
+  const T *fromA = pa + (begin + dir * uA) * s.as.t + iA, *fromC = pc + (begin + dir * uA) * s.cs.t + iA;
+  const T *fromB = pb + (begin + dir * uB) * s.bs.t + kB;
+  T *toY = py + (begin + dir * uB) * yt + kB;
+  const int64_t stepA = dir * RP * s.as.t, stepC = dir * RP * s.cs.t, stepB = dir * BP * s.bs.t, stepY = dir * BP * yt;
+  const bool rowIn = iA < s.Di, columnIn = first + kB < s.Dj;
   float nextA[AC], nextC[AC], nextB[B];
   bool nextCut = false;
   auto fetch = [&](int t0) {
+    const int left = s.T - t0;
 #pragma unroll
     for (int n = 0; n < AC; ++n) {
-      const int q = n * THREADS + threadIdx.x, u = q / DI, i = q % DI;
-      const bool in = t0 + u < s.T && i < s.Di;
-      const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
-      nextA[n] = in ? s.mulA * toFloat(pa[t * s.as.t + i]) : 0.f;
-      nextC[n] = in ? s.mulC * toFloat(pc[t * s.cs.t + i]) : 0.f;
+      const bool in = rowIn && n * RP + uA < left;
+      nextA[n] = in ? s.mulA * toFloat(fromA[n * stepA]) : 0.f;
+      nextC[n] = in ? s.mulC * toFloat(fromC[n * stepC]) : 0.f;
     }
 #pragma unroll
-    for (int n = 0; n < B; ++n) {
-      const int q = n * THREADS + threadIdx.x, u = q / kScanColumns, k = q % kScanColumns;
-      const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
-      nextB[n] = t0 + u < s.T && first + k < s.Dj ? toFloat(pb[t * s.bs.t + k]) : 0.f;
-    }
+    for (int n = 0; n < B; ++n) nextB[n] = columnIn && n * BP + uB < left ? toFloat(fromB[n * stepB]) : 0.f;
+    fromA += AC * stepA;
+    fromC += AC * stepC;
+    fromB += B * stepB;
     // The factor between a step and the one before it in the sweep: the reset of
     // the later of the two in time.
     const int u = threadIdx.x;
@@ -108,45 +149,73 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
     }
 #pragma unroll
     for (int n = 0; n < B; ++n) (&b[0][0])[n * THREADS + threadIdx.x] = nextB[n];
-    if (threadIdx.x < kScanSteps) cut[threadIdx.x] = nextCut;
-    __syncthreads();
+    if (threadIdx.x < kScanSteps) {
+      cut[threadIdx.x] = nextCut;
+      factor[threadIdx.x] = s.reverse && t0 + int(threadIdx.x) == 0 ? 1.f : decay;
+    }
+    const bool anyCut = __syncthreads_or(nextCut);
     if (t0 + kScanSteps < s.T) fetch(t0 + kScanSteps);
+    auto step = [&](int u) {
+      const float2 value = *reinterpret_cast<const float2 *>(&b[u][column]);
+      const Pair f2 = pairOf(factor[u], factor[u]), v2[2] = {pairOf(value.x, value.x), pairOf(value.y, value.y)};
+      Pair sum[2] = {0, 0};
+#pragma unroll
+      for (int r = 0; r < R / 2; r += 2) {
+        const ulonglong2 pairsA = *reinterpret_cast<const ulonglong2 *>(&a[u][i0 + 2 * r]);
+        const ulonglong2 pairsC = *reinterpret_cast<const ulonglong2 *>(&c[u][i0 + 2 * r]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          x[k][r] = fma2(f2, x[k][r], mul2(pairsA.x, v2[k]));
+          x[k][r + 1] = fma2(f2, x[k][r + 1], mul2(pairsA.y, v2[k]));
+          sum[k] = fma2(pairsC.x, x[k][r], sum[k]);
+          sum[k] = fma2(pairsC.y, x[k][r + 1], sum[k]);
+        }
+      }
+      float2 p0 = parts(sum[0]), p1 = parts(sum[1]);
+      float2 total = make_float2(p0.x + p0.y, p1.x + p1.y);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) {
+        total.x += __shfl_xor_sync(0xffffffffu, total.x, o);
+        total.y += __shfl_xor_sync(0xffffffffu, total.y, o);
+      }
+      if (lane == 0) *reinterpret_cast<float2 *>(&y[u][column]) = total;
+    };
+    if (!anyCut && count == kScanSteps) {   // nothing in the way of overlapping one step with the next
 #pragma unroll 4
-    for (int u = 0; u < count; ++u) {
-      const float value = b[u][column];
-      const float f = s.reverse && t0 + u == 0 ? 1.f : decay;
-      if (cut[u]) {
+      for (int u = 0; u < kScanSteps; ++u) step(u);
+    } else {
+      for (int u = 0; u < count; ++u) {
+        if (cut[u]) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) x[r] = 0.f;
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int r = 0; r < R / 2; ++r) x[k][r] = 0;
+        }
+        step(u);
       }
-      float sum[2] = {0.f, 0.f};
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        x[r] = fmaf(f, x[r], a[u][i0 + r] * value);
-        sum[r & 1] = fmaf(c[u][i0 + r], x[r], sum[r & 1]);
-      }
-      float total = sum[0] + sum[1];
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      if (lane == 0) y[u][column] = total;
     }
     __syncthreads();
-    if (s.y) {
+    if (s.y && columnIn) {
 #pragma unroll
-      for (int n = 0; n < B; ++n) {
-        const int q = n * THREADS + threadIdx.x, u = q / kScanColumns, k = q % kScanColumns;
-        const int64_t t = s.reverse ? s.T - 1 - (t0 + u) : t0 + u;
-        if (u < count && first + k < s.Dj) py[t * yt + k] = fromFloat<T>(y[u][k]);
-      }
+      for (int n = 0; n < B; ++n)
+        if (n * BP + uB < count) toY[n * stepY] = fromFloat<T>(y[n * BP + uB][kB]);
     }
+    toY += B * stepY;
   }
-  if (s.last && live) {
+  if (s.last) {
     // Backwards, the state before the first step is one more factor away.
     const bool gone = s.reverse && s.T > 0 && s.resets && s.resets[e];
     const float f = s.reverse && s.T > 0 ? decay : 1.f;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (i0 + r < s.Di) s.last[base + int64_t(i0 + r) * s.ri + int64_t(j) * s.rj] = gone ? 0.f : f * x[r];
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < R / 2; ++r) {
+        const float2 v = parts(x[k][r]);
+        const int i = i0 + 2 * r;
+        float *to = s.last + base + int64_t(i) * s.ri + int64_t(j + k) * s.rj;
+        if (j + k < s.Dj && i < s.Di) to[0] = gone ? 0.f : f * v.x;
+        if (j + k < s.Dj && i + 1 < s.Di) to[s.ri] = gone ? 0.f : f * v.y;
+      }
   }
 }
 
