@@ -11,10 +11,9 @@
 // float32 from chunk to chunk; a bfloat16 copy in shared memory is the operand
 // of the next chunk's Q S.
 //
-// Decays without an exponential per pair: of the 16 steps a warp owns, a pair
-// within the warp's own 16x16 block has one of 31 fixed factors (kept in
-// registers); a pair with an earlier block j has l^(i-i0) l^(i0-j), a factor per
-// row and one per column, both at most 1 whatever l is.
+// Decays without an exponential per pair: a table of l^n in shared memory, read at
+// i - j (the lanes of a tile read 14 neighbouring words).  The table is zero below
+// n = 0, which is the causal mask.
 //
 // Roundings to bfloat16, each of 8 significant bits: the decayed scores, and the
 // copy of S.  The state itself is kept to float32 accuracy: its operand
@@ -89,11 +88,16 @@ __device__ __forceinline__ void loadTile(bf16 *tile, const bf16 *base, int64_t s
     const int r0 = threadIdx.x / pieces, c = (threadIdx.x % pieces) * 8;
     const bool inside = c0 + c < width;
     const bf16 *from = base + int64_t(t0 + r0) * stride + c0 + c;
+    bf16 *to = tile + r0 * L + c;
+    if (count == C && width >= c0 + D) {
+#pragma unroll
+      for (int x = 0; x < C / rows; ++x) copyAsync16(to + x * rows * L, from + x * (rows * stride));
+      return;
+    }
 #pragma unroll
     for (int x = 0; x < C / rows; ++x) {
       const bool valid = inside && r0 + x * rows < count;
-      copyAsync16(tile + (r0 + x * rows) * L + c, valid ? from : base, valid);
-      from += rows * stride;
+      copyAsync16(to + x * rows * L, valid ? from + x * (rows * stride) : base, valid);
     }
   } else {
     for (int id = threadIdx.x; id < C * D; id += THREADS) {
@@ -105,12 +109,13 @@ __device__ __forceinline__ void loadTile(bf16 *tile, const bf16 *base, int64_t s
 
 // Rows of 16 steps by N tiles of 8 columns of a dense [T, E, H, width] output,
 // as the products leave them: lane 4 g + q has columns 2 q and 2 q + 1 of row g
-// (and g + 8) of each tile.  Where rows are whole 16-byte pieces, the four lanes
-// of a row exchange their pairs of four tiles (a 4 x 4 transpose, two rounds),
-// so that each stores all of one tile: 64 bytes of a row at a time.
+// (and g + 8) of each tile.  `finite` becomes NaN if one of them is not finite.
+// Where rows are whole 16-byte pieces, the four lanes of a row exchange their
+// pairs of four tiles (a 4 x 4 transpose, two rounds), so that each stores all of
+// one tile: 64 bytes of a row at a time.
 template <int N>
 __device__ __forceinline__ void storeTile(bf16 *out, const float (&x)[N][4], int64_t stepStride, int first, int count,
-                                          int row0, int col0, int width) {
+                                          int row0, int col0, int width, uint32_t &finite) {
   const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   if (N % 4 == 0 && width % 8 == 0) {
 #pragma unroll
@@ -121,7 +126,10 @@ __device__ __forceinline__ void storeTile(bf16 *out, const float (&x)[N][4], int
       for (int n = 0; n < N / 4 * 4; n += 4) {
         uint32_t p[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) p[m] = packPair(x[n + m][2 * y], x[n + m][2 * y + 1]);
+        for (int m = 0; m < 4; ++m) {
+          p[m] = packPair(x[n + m][2 * y], x[n + m][2 * y + 1]);
+          finite = addZeroTimes(p[m], finite);
+        }
         const bool odd = tq & 1, upper = tq & 2;
         const uint32_t a = __shfl_xor_sync(0xffffffffu, odd ? p[0] : p[1], 1);
         const uint32_t b = __shfl_xor_sync(0xffffffffu, odd ? p[2] : p[3], 1);
@@ -139,15 +147,46 @@ __device__ __forceinline__ void storeTile(bf16 *out, const float (&x)[N][4], int
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
+      const uint32_t p = packPair(x[n][2 * y], x[n][2 * y + 1]);
+      finite = addZeroTimes(p, finite);
       const int i = row0 + g + y * 8, j = col0 + n * 8 + 2 * tq;
       if (i >= count) continue;
       bf16 *to = out + int64_t(first + i) * stepStride + j;
-      if (j + 1 < width && width % 2 == 0) *reinterpret_cast<uint32_t *>(to) = packPair(x[n][2 * y], x[n][2 * y + 1]);
+      if (j + 1 < width && width % 2 == 0) *reinterpret_cast<uint32_t *>(to) = p;
       else {
         if (j < width) to[0] = fromFloat<bf16>(x[n][2 * y]);
         if (j + 1 < width) to[1] = fromFloat<bf16>(x[n][2 * y + 1]);
       }
     }
+}
+// The same through 16 rows of shared memory (D of them wide at least) that only
+// this warp uses.
+template <int D, int N>
+__device__ __forceinline__ void storeTileStaged(bf16 *out, bf16 *stage, const float (&x)[N][4], int64_t stepStride,
+                                                int first, int count, int row0, int col0, int width,
+                                                uint32_t &finite) {
+  constexpr int L = D + 8, pieces = N, rows = 32 / pieces;   // lanes of a row, rows of an instruction
+  if (width % 8 != 0) {
+    storeTile(out, x, stepStride, first, count, row0, col0, width, finite);
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < N; n += 2) {
+    const uint32_t p[4] = {packPair(x[n][0], x[n][1]), packPair(x[n][2], x[n][3]), packPair(x[n + 1][0], x[n + 1][1]),
+                           packPair(x[n + 1][2], x[n + 1][3])};
+#pragma unroll
+    for (int m = 0; m < 4; ++m) finite = addZeroTimes(p[m], finite);
+    storeMatrices<L>(stage, 0, n * 8, p);
+  }
+  __syncwarp();
+  const int lane = threadIdx.x & 31, r0 = lane / pieces, c = (lane % pieces) * 8;
+  bf16 *to = out + int64_t(first + row0 + r0) * stepStride + col0 + c;
+  const bool inside = col0 + c < width;
+#pragma unroll
+  for (int r = 0; r < 16 / rows; ++r)
+    if (inside && row0 + r0 + r * rows < count)
+      *reinterpret_cast<uint4 *>(to + r * (rows * stepStride)) =
+          *reinterpret_cast<const uint4 *>(stage + (r0 + r * rows) * L + c);
 }
 
 template <int N> __device__ __forceinline__ bool notFinite(const float (&x)[N][4]) {
@@ -230,15 +269,14 @@ __device__ __forceinline__ void writeSlice(float *to, const float (&S)[SM][SN][4
 // ... and its bfloat16 copy in a tile with rows of L.
 template <int L, int SM, int SN>
 __device__ __forceinline__ void copySlice(bf16 *tile, const float (&S)[SM][SN][4], int m0, int n0) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
 #pragma unroll
   for (int m = 0; m < SM; ++m)
 #pragma unroll
-    for (int n = 0; n < SN; ++n)
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-        *reinterpret_cast<uint32_t *>(tile + ((m0 + m) * 16 + g + y * 8) * L + (n0 + n) * 8 + 2 * tq) =
-            packPair(S[m][n][2 * y], S[m][n][2 * y + 1]);
+    for (int n = 0; n < SN; n += 2) {
+      const uint32_t p[4] = {packPair(S[m][n][0], S[m][n][1]), packPair(S[m][n][2], S[m][n][3]),
+                             packPair(S[m][n + 1][0], S[m][n + 1][1]), packPair(S[m][n + 1][2], S[m][n + 1][3])};
+      storeMatrices<L>(tile, (m0 + m) * 16, (n0 + n) * 8, p);
+    }
 }
 
 // Shared memory of a block: tiles in `buffers` copies.
@@ -246,7 +284,7 @@ template <int C, int DK, int DV, bool OUT> constexpr int chunkTileElements() {
   return C * (DK + 8) * (OUT ? 2 : 1) + C * (DV + 8);
 }
 template <int C, int DK, int DV, bool OUT> constexpr int chunkSharedBytes(int buffers) {
-  return buffers * (chunkTileElements<C, DK, DV, OUT>() + (OUT ? DK * (DV + 8) : 0)) * 2 + 4 * 2 * C;
+  return buffers * (chunkTileElements<C, DK, DV, OUT>() + (OUT ? DK * (DV + 8) : 0)) * 2 + 4 * (2 * C + 20);
 }
 
 // One block per (environment, head), segment of T and tile of DV columns; C / 16
@@ -264,8 +302,8 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
   extern __shared__ __align__(16) unsigned char shared[];
   bf16 *tiles = reinterpret_cast<bf16 *>(shared);
   bf16 *copies = tiles + buffers * chunkTileElements<C, DK, DV, OUT>();      // the state in bfloat16
-  float *before = reinterpret_cast<float *>(copies + (OUT ? buffers * DK * LV : 0));   // scale l^(C - x)
-  float *toEnd = before + C;                                                  // l^(L - 1 - j)
+  float *toEnd = reinterpret_cast<float *>(copies + (OUT ? buffers * DK * LV : 0));   // l^(L - 1 - j)
+  float *powers = toEnd + C;                                                  // scale l^(x - 16), 0 for x < 16
 
   const int64_t eh = blockIdx.x;
   const int e = int(eh / p.H), h = int(eh - int64_t(e) * p.H);
@@ -305,24 +343,12 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
   const float logDecay = fmaxf(log2f(decay), -1e30f);   // finite: no 0 times infinity for a decay of zero
   // (Of a negative or NaN decay: NaN, which leaves the block to redoAttention().)
   auto power = [&](int n) { return decay >= 0.f ? exp2f(float(n) * logDecay) : __int_as_float(0x7fc00000); };
-  for (int x = threadIdx.x; x < C; x += THREADS) {
-    before[x] = p.scale * power(C - x);
-    toEnd[x] = power(C - 1 - x);
-  }
-  float inBlock[2][4];   // scale l^(i - j) of the warp's 16x16 block, 0 above its diagonal
-#pragma unroll
-  for (int n = 0; n < 2; ++n)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int d = g + (x >> 1) * 8 - (2 * tq + (x & 1) + 8 * n);
-      inBlock[n][x] = d >= 0 ? p.scale * power(d) : 0.f;
-    }
+  for (int x = threadIdx.x; x < C; x += THREADS) toEnd[x] = power(C - 1 - x);
+  for (int x = threadIdx.x; x < C + 20; x += THREADS) powers[x] = x < 16 ? 0.f : p.scale * power(x - 16);
   const int i0 = 16 * warp;
-  const float fromStart = p.scale * power(i0 + 1);   // of the warp's first step to S
-  const float row0 = power(g), row1 = power(g + 8);
   const float fullChunk = power(C);
 
-  float finite = 0.f;
+  uint32_t finite = 0;
   bool anyReset = false, later = init != nullptr;   // later: S is not zero
   for (int c = 0; c < chunks; ++c) {
     const int buffer = buffers > 1 ? c & 1 : 0, first = t0 + c * C, count = min(C, t1 - first);
@@ -371,12 +397,18 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
             multiplyAdd(o[2 * n], a[kk], b[0], b[1]);
             multiplyAdd(o[2 * n + 1], a[kk], b[2], b[3]);
           }
+        const float f0 = powers[16 + i0 + g + 1], f1 = powers[16 + i0 + g + 9];
 #pragma unroll
         for (int n = 0; n < DV / 8; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[n][x] = (x < 2 ? start0 : start1) < 0 ? o[n][x] * fromStart : 0.f;
+          for (int x = 0; x < 4; ++x) o[n][x] *= x < 2 ? f0 : f1;
+        if (mask) {
+#pragma unroll
+          for (int n = 0; n < DV / 8; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[n][x] = (x < 2 ? start0 : start1) < 0 ? o[n][x] : 0.f;
+        }
       }
-      // Earlier blocks, then the warp's own.
       for (int block = 0; block <= warp; ++block) {
         float s[2][4] = {};
 #pragma unroll
@@ -386,30 +418,17 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
           multiplyAdd(s[0], a[kk], b[0], b[1]);
           multiplyAdd(s[1], a[kk], b[2], b[3]);
         }
-        const int j0 = block * 16 + 2 * tq;
-        if (block < warp) {
+        const float *f = powers + 16 + i0 - block * 16 + g - 2 * tq;   // of the distance i - j, 0 below zero
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const float2 f = *reinterpret_cast<const float2 *>(before + C - i0 + j0 + n * 8);
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              s[n][x] = j0 + n * 8 + (x & 1) >= (x < 2 ? start0 : start1) ? s[n][x] * (x & 1 ? f.y : f.x) : 0.f;
-          }
-        } else {
-#pragma unroll
-          for (int n = 0; n < DV / 8; ++n) {
-            o[n][0] *= row0;
-            o[n][1] *= row0;
-            o[n][2] *= row1;
-            o[n][3] *= row1;
-          }
+          for (int x = 0; x < 4; ++x) s[n][x] *= f[(x >> 1) * 8 - (x & 1) - n * 8];
+        if (mask) {
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              s[n][x] = g + (x >> 1) * 8 >= 2 * tq + (x & 1) + 8 * n &&
-                                j0 + n * 8 + (x & 1) >= (x < 2 ? start0 : start1)
-                            ? s[n][x] * inBlock[n][x] : 0.f;
+              if (block * 16 + 2 * tq + n * 8 + (x & 1) < (x < 2 ? start0 : start1)) s[n][x] = 0.f;
         }
         const uint32_t w[4] = {packPair(s[0][0], s[0][1]), packPair(s[0][2], s[0][3]), packPair(s[1][0], s[1][1]),
                                packPair(s[1][2], s[1][3])};
@@ -421,11 +440,12 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
           multiplyAdd(o[2 * n + 1], w, b[2], b[3]);
         }
       }
-#pragma unroll
-      for (int n = 0; n < DV / 8; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) finite = fmaf(o[n][x], 0.f, finite);
-      storeTile(p.out + eh * p.Dv, o, int64_t(p.E) * p.H * p.Dv, first, count, i0, col0, p.Dv);
+      // The warp's rows of Q are its own and done with.
+      bf16 *out = p.out + eh * p.Dv;
+      const int64_t stepStride = int64_t(p.E) * p.H * p.Dv;
+      if constexpr (DV <= DK)
+        storeTileStaged<DK>(out, const_cast<bf16 *>(Q) + i0 * LQ, o, stepStride, first, count, i0, col0, p.Dv, finite);
+      else storeTile(out, o, stepStride, first, count, i0, col0, p.Dv, finite);
     }
 
     // The state at the chunk's end.
@@ -438,15 +458,25 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) S[m][n][x] = start < 0 ? S[m][n][x] * f : 0.f;
+          for (int x = 0; x < 4; ++x) S[m][n][x] *= f;
+      if (start >= 0) {
+#pragma unroll
+        for (int m = 0; m < SM; ++m)
+#pragma unroll
+          for (int n = 0; n < SN; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) S[m][n][x] = 0.f;
+      }
 #pragma unroll
       for (int kk = 0; kk < C / 16; ++kk) {
         const int j = kk * 16 + 2 * tq;
         float2 f0 = *reinterpret_cast<const float2 *>(toEnd + j), f1 = *reinterpret_cast<const float2 *>(toEnd + j + 8);
-        f0.x = j >= start ? f0.x : 0.f;
-        f0.y = j + 1 >= start ? f0.y : 0.f;
-        f1.x = j + 8 >= start ? f1.x : 0.f;
-        f1.y = j + 9 >= start ? f1.y : 0.f;
+        if (mask) {
+          f0.x = j >= start ? f0.x : 0.f;
+          f0.y = j + 1 >= start ? f0.y : 0.f;
+          f1.x = j + 8 >= start ? f1.x : 0.f;
+          f1.y = j + 9 >= start ? f1.y : 0.f;
+        }
 #pragma unroll
         for (int m = 0; m < SM; ++m) {
           uint32_t a[4], high[4], low[4];
@@ -474,7 +504,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
       if (OUT && c + 1 < chunks) copySlice<LV>(copies + ((c + 1) & 1) * DK * LV, S, sm0, sn0);
     }
   }
-  bool bad = finite != 0.f;   // NaN
+  bool bad = (finite & 0x7fff7fffu) != 0;   // NaN
   if (STATE && last) {
     writeSlice(last, S, sm0, sn0, col0, p.Dk, p.Dv);
 #pragma unroll
@@ -511,8 +541,9 @@ struct BackwardArgs {
 };
 
 template <int C, int D, bool OUT> constexpr int backwardWarps() { return OUT && D == 128 ? C / 8 : C / 16; }
-template <int C, int D, bool OUT> constexpr int backwardSharedBytes() {
-  return (OUT ? (4 * C + 2 * D) : 2 * C) * (D + 8) * 2 + (16 + C + 4) * 4;
+// Where `later` states' gradients never exist, no room for X.
+template <int C, int D, bool OUT> constexpr int backwardSharedBytes(bool later) {
+  return (OUT ? 4 * C + (later ? 2 : 1) * D : 2 * C) * (D + 8) * 2 + (16 + C + 4) * 4;
 }
 
 // One block per (environment, head) and segment of T, chunks from the last to the
@@ -538,9 +569,9 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
   constexpr int N = D / 8 / PARTS;                             // tiles of 8 columns of a warp's outputs
   constexpr int RT = D / 16, SM = RT >= W ? RT / W : 1, SPLIT = RT >= W ? 1 : W / RT, SN = D / 8 / SPLIT;
   extern __shared__ __align__(16) unsigned char shared[];
-  bf16 *Q = reinterpret_cast<bf16 *>(shared), *O = Q + C * LD, *K = O + C * LD, *V = K + C * LD, *S = V + C * LD,
+  float *powers = reinterpret_cast<float *>(shared);   // scale l^(x - 16), 0 for x < 16; C + 20 of them
+  bf16 *Q = reinterpret_cast<bf16 *>(powers + C + 20), *O = Q + C * LD, *K = O + C * LD, *V = K + C * LD, *S = V + C * LD,
        *X = S + D * LD;
-  float *powers = reinterpret_cast<float *>(OUT ? X + D * LD : K);   // scale l^(x - 16), 0 for x < 16; C + 20 of them
   const int64_t eh = blockIdx.x;
   const int e = int(eh / p.H), h = int(eh - int64_t(e) * p.H), seg = OUT ? blockIdx.y : blockIdx.y + 1;
   const int t0 = seg * p.segmentLength, t1 = min(p.T, t0 + p.segmentLength);
@@ -563,7 +594,7 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
   float dS[SM][SN][4];
   if (STATE) readSlice(dS, init, sm0, sn0, 0, p.Dk, p.Dv);
 
-  float finite = 0.f;
+  uint32_t finite = 0;
   bool anyReset = false, later = init != nullptr;   // later: X is not zero
   for (int c = chunks - 1; c >= 0; --c) {
     const int first = t0 + c * C, count = min(C, t1 - first);
@@ -615,11 +646,16 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int at = block * 16 + n * 8 + 2 * tq + (x & 1);
-            const bool sees = sign > 0 ? at >= (x < 2 ? start0 : start1) : at < (x < 2 ? end0 : end1);
-            s[n][x] = sees ? s[n][x] * f[sign * ((x >> 1) * 8 - (x & 1) - n * 8)] : 0.f;
-          }
+          for (int x = 0; x < 4; ++x) s[n][x] *= f[sign * ((x >> 1) * 8 - (x & 1) - n * 8)];
+        if (mask) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int at = block * 16 + n * 8 + 2 * tq + (x & 1);
+              if (sign > 0 ? at < (x < 2 ? start0 : start1) : at >= (x < 2 ? end0 : end1)) s[n][x] = 0.f;
+            }
+        }
         w[0] = packPair(s[0][0], s[0][1]);
         w[1] = packPair(s[0][2], s[0][3]);
         w[2] = packPair(s[1][0], s[1][1]);
@@ -646,13 +682,13 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) out[n][x] = (x < 2 ? f0 : f1) == 0.f ? 0.f : out[n][x] * (x < 2 ? f0 : f1);
-      };
-      auto check = [&]() {
+          for (int x = 0; x < 4; ++x) out[n][x] *= x < 2 ? f0 : f1;
+        if (mask || count < C) {
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) finite = fmaf(out[n][x], 0.f, finite);
+            for (int x = 0; x < 4; ++x) out[n][x] = (x < 2 ? f0 : f1) == 0.f ? 0.f : out[n][x];
+        }
       };
       const int64_t stepK = int64_t(p.E) * p.H * p.Dk, stepV = int64_t(p.E) * p.H * p.Dv;
       if (row < count) {
@@ -675,8 +711,7 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
           weights(w, V, block, Forwards());
           accumulate(w, K, block);
         }
-        check();
-        storeTile(p.dq + eh * p.Dk, out, stepK, first, count, row, col, p.Dk);
+        storeTile(p.dq + eh * p.Dk, out, stepK, first, count, row, col, p.Dk, finite);
         // dv, dk
         const int left0 = count - 1 - row - g, left1 = left0 - 8;
         const float f0 = row + g >= endStart && left0 >= 0 ? power(left0) : 0.f;
@@ -699,8 +734,7 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
           weights(w, Q, block, Backwards());
           accumulate(w, O, block);
         }
-        check();
-        storeTile(p.dv + eh * p.Dv, out, stepV, first, count, row, col, p.Dv);
+        storeTile(p.dv + eh * p.Dv, out, stepV, first, count, row, col, p.Dv, finite);
         rowsOfA(V);
         if (later) {
 #pragma unroll
@@ -719,8 +753,7 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
           weights(w, O, block, Backwards());
           accumulate(w, Q, block);
         }
-        check();
-        storeTile(p.dk + eh * p.Dk, out, stepK, first, count, row, col, p.Dk);
+        storeTile(p.dk + eh * p.Dk, out, stepK, first, count, row, col, p.Dk, finite);
       }
     }
 
@@ -732,7 +765,15 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
 #pragma unroll
         for (int n = 0; n < SN; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) dS[m][n][x] = endStart < 0 ? dS[m][n][x] * f : 0.f;
+          for (int x = 0; x < 4; ++x) dS[m][n][x] *= f;
+      if (endStart >= 0) {
+#pragma unroll
+        for (int m = 0; m < SM; ++m)
+#pragma unroll
+          for (int n = 0; n < SN; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) dS[m][n][x] = 0.f;
+      }
       for (int kk = 0; kk < (count + 15) / 16; ++kk) {
         float w[4];
 #pragma unroll
@@ -767,7 +808,7 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
       __syncthreads();   // the tiles and X are free
     }
   }
-  bool bad = finite != 0.f;   // NaN
+  bool bad = (finite & 0x7fff7fffu) != 0;   // NaN
   if (STATE && last) {
     writeSlice(last, dS, sm0, sn0, 0, p.Dk, p.Dv);
 #pragma unroll

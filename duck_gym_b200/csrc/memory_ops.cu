@@ -259,9 +259,10 @@ template <int C, int D, bool OUT, bool STATE>
 void launchBackward(const BackwardArgs &a, int segments, cudaStream_t stream) {
   const dim3 grid(unsigned(int64_t(a.E) * a.H), unsigned(segments));
   constexpr auto kernel = attentionChunksBackward<C, D, OUT, STATE>;
-  constexpr int bytes = backwardSharedBytes<C, D, OUT>();
-  if constexpr (bytes > 48 * 1024) allowShared<kernel>(bytes);
-  kernel<<<grid, backwardWarps<C, D, OUT>() * 32, bytes, stream>>>(a);
+  constexpr int most = backwardSharedBytes<C, D, OUT>(true);
+  if constexpr (most > 48 * 1024) allowShared<kernel>(most);
+  const bool later = STATE || a.dstateOut;
+  kernel<<<grid, backwardWarps<C, D, OUT>() * 32, backwardSharedBytes<C, D, OUT>(later), stream>>>(a);
   check(cudaGetLastError(), "linear attention backward launch");
 }
 template <int C, bool OUT, bool STATE>

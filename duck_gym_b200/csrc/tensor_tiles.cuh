@@ -59,12 +59,32 @@ __device__ __forceinline__ uint32_t packPair(float low, float high) {
 __device__ __forceinline__ float lowOf(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float highOf(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 
+// Results of products, packed in pairs, into a tile: rows row0.. by columns col0.. (16 x 16): p[0] rows 0-7 and p[1]
+// rows 8-15 of the first 8 columns, p[2] and p[3] of the second.
+template <int stride>
+__device__ __forceinline__ void storeMatrices(bf16 *x, int row0, int col0, const uint32_t (&p)[4]) {
+  const int lane = threadIdx.x & 31;
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
+                   sharedAddress(x + (row0 + (lane & 15)) * stride + col0 + (lane >> 4) * 8)),
+               "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3])
+               : "memory");
+}
+// NaN in the sum if either number of the pair is not finite.
+__device__ __forceinline__ uint32_t addZeroTimes(uint32_t pair, uint32_t sum) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(pair), "r"(0u), "r"(sum));
+  return d;
+}
+
 // 16 bytes from global to shared memory without a register; zeros where !valid
 // (the address is then not read).
 __device__ __forceinline__ void copyAsync16(bf16 *to, const bf16 *from, bool valid) {
   const int bytes = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sharedAddress(to)), "l"(from), "r"(bytes)
                : "memory");
+}
+__device__ __forceinline__ void copyAsync16(bf16 *to, const bf16 *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sharedAddress(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void commitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void waitCopies() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
