@@ -57,15 +57,24 @@ struct ChunkArgs {
   float scale;
 };
 
-// Bit i: an episode begins at step t0 + i (i < 64, t0 + i < end).
-__device__ __forceinline__ unsigned long long resetMask(const uint8_t *resets, int E, int e, int t0, int end) {
-  if (!resets) return 0;
-  const int lane = threadIdx.x & 31;
-  const bool a = t0 + lane < end && resets[int64_t(t0 + lane) * E + e];
-  const bool b = t0 + 32 + lane < end && resets[int64_t(t0 + 32 + lane) * E + e];
-  const unsigned low = __ballot_sync(0xffffffffu, a), high = __ballot_sync(0xffffffffu, b);
-  return (static_cast<unsigned long long>(high) << 32) | low;
-}
+// Where episodes begin in steps t0 .. t0 + 63 before `end`: a lane looks at two of
+// them; read a chunk ahead.
+struct Resets {
+  uint32_t a = 0, b = 0;   // the bytes as they are: looked at only when they are needed
+  __device__ __forceinline__ void read(const uint8_t *resets, int E, int e, int t0, int end) {
+    if (!resets) return;
+    const int t = t0 + (threadIdx.x & 31);
+    const uint8_t *at = resets + int64_t(t) * E + e;
+    a = b = 0;
+    if (t < end) a = at[0];
+    if (t + 32 < end) b = at[int64_t(32) * E];
+  }
+  // Bit i: at step t0 + i.
+  __device__ __forceinline__ unsigned long long mask() const {
+    const unsigned low = __ballot_sync(0xffffffffu, a != 0), high = __ballot_sync(0xffffffffu, b != 0);
+    return (static_cast<unsigned long long>(high) << 32) | low;
+  }
+};
 // Last step of a chunk up to i at which an episode begins, or -1: step i sees the
 // steps from there on, and the state before the chunk if there is none.
 __device__ __forceinline__ int episodeStart(unsigned long long mask, int i) {
@@ -203,17 +212,25 @@ template <int DK, int D, int THREADS>
 __device__ __forceinline__ void loadState(bf16 *tile, const float *from, int rows, int c0, int width) {
   constexpr int L = D + 8, quads = D / 4;
   if (width % 4 == 0) {
-#pragma unroll 4
-    for (int id = threadIdx.x; id < DK * quads; id += THREADS) {
-      const int i = id / quads, j = (id % quads) * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (from && i < rows && c0 + j < width) v = *reinterpret_cast<const float4 *>(from + int64_t(i) * width + c0 + j);
-      *reinterpret_cast<uint2 *>(tile + i * L + j) = make_uint2(packPair(v.x, v.y), packPair(v.z, v.w));
+    constexpr int each = DK * quads / THREADS, AHEAD = each < 16 ? each : 16;   // loads in flight
+    for (int n0 = 0; n0 < each; n0 += AHEAD) {
+      float4 v[AHEAD];
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        const int id = (n0 + n) * THREADS + threadIdx.x, i = id / quads, j = (id % quads) * 4;
+        v[n] = i < rows && c0 + j < width ? *reinterpret_cast<const float4 *>(from + i * width + c0 + j)
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        const int id = (n0 + n) * THREADS + threadIdx.x, i = id / quads, j = (id % quads) * 4;
+        *reinterpret_cast<uint2 *>(tile + i * L + j) = make_uint2(packPair(v[n].x, v[n].y), packPair(v[n].z, v[n].w));
+      }
     }
   } else {
     for (int id = threadIdx.x; id < DK * D; id += THREADS) {
       const int i = id / D, j = id % D;
-      tile[i * L + j] = fromFloat<bf16>(from && i < rows && c0 + j < width ? from[int64_t(i) * width + c0 + j] : 0.f);
+      tile[i * L + j] = fromFloat<bf16>(i < rows && c0 + j < width ? from[i * width + c0 + j] : 0.f);
     }
   }
 }
@@ -288,11 +305,14 @@ template <int C, int DK, int DV, bool OUT> constexpr int chunkSharedBytes(int bu
 }
 
 // One block per (environment, head), segment of T and tile of DV columns; C / 16
-// warps.  OUT = false computes the state at the segment's end only; STATE = false
+// warps.  (Two warps for each 16 steps, with half of the columns each, doubled the
+// warps on a multiprocessor and cost 14 %: the scores twice, and shared memory is
+// what such a kernel waits for.)  OUT = false computes the state at the segment's end only; STATE = false
 // is for one chunk whose last state nobody wants.
 template <int C, int DK, int DV, bool OUT, bool STATE>
 __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) / C)
     attentionChunks(ChunkArgs p, int buffers) {
+  constexpr int N = DV / 8;                                    // column tiles of the outputs
   constexpr int W = C / 16, THREADS = W * 32, LQ = DK + 8, LV = DV + 8;
   constexpr int RT = DK / 16;                                  // row tiles of the state
   constexpr int SM = RT >= W ? RT / W : 1;                     // of which a warp has
@@ -327,6 +347,8 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
     commitCopies();
   };
   load(0, 0);
+  Resets resets;
+  resets.read(p.resets, p.E, e, t0, min(t1, t0 + C));
 
   // The warp's slice of the state, and its copy.
   const int sm0 = RT >= W ? warp * SM : warp / SPLIT, sn0 = RT >= W ? 0 : (warp % SPLIT) * SN;
@@ -345,53 +367,60 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
   auto power = [&](int n) { return decay >= 0.f ? exp2f(float(n) * logDecay) : __int_as_float(0x7fc00000); };
   for (int x = threadIdx.x; x < C; x += THREADS) toEnd[x] = power(C - 1 - x);
   for (int x = threadIdx.x; x < C + 20; x += THREADS) powers[x] = x < 16 ? 0.f : p.scale * power(x - 16);
-  const int i0 = 16 * warp;
+  const int i0 = 16 * warp;   // the warp's steps
   const float fullChunk = power(C);
 
   uint32_t finite = 0;
   bool anyReset = false, later = init != nullptr;   // later: S is not zero
   for (int c = 0; c < chunks; ++c) {
     const int buffer = buffers > 1 ? c & 1 : 0, first = t0 + c * C, count = min(C, t1 - first);
-    const unsigned long long mask = resetMask(p.resets, p.E, e, first, min(t1, first + C));
+    const unsigned long long mask = resets.mask();
     anyReset |= mask != 0;
     waitCopies();
     __syncthreads();
-    if (c + 1 < chunks) load(c + 1, (c + 1) & 1);
+    if (c + 1 < chunks) {
+      load(c + 1, (c + 1) & 1);
+      resets.read(p.resets, p.E, e, first + C, min(t1, first + 2 * C));
+    }
     const bf16 *K = tiles + buffer * chunkTileElements<C, DK, DV, OUT>(), *V = K + C * LQ, *Q = V + C * LV;
     if (STATE && count < C)
       for (int x = threadIdx.x; x < C; x += THREADS) toEnd[x] = x < count ? power(count - 1 - x) : 0.f;
 
-    if (OUT) {
-      const bf16 *copy = copies + buffer * DK * LV;
-      const int start0 = episodeStart(mask, i0 + g), start1 = episodeStart(mask, i0 + g + 8);
+    const bool advance = STATE && (c + 1 < chunks || last);
+    const bf16 *copy = copies + buffer * DK * LV;
+    if (OUT && STATE && p.saved) {
       const int chunk = seg * (p.segmentLength / C) + c;
-      if (STATE && p.saved && chunk > 0) {
-        bf16 *to = p.saved + (eh * ((p.T + C - 1) / C) + chunk) * stateSize + col0;
-        if (p.Dv % 8 == 0) {
+      bf16 *to = p.saved + (eh * ((p.T + C - 1) / C) + chunk) * stateSize + col0;
+      if (chunk == 0) {
+        // the caller has it
+      } else if (p.Dv % 8 == 0) {
 #pragma unroll
-          for (int x = threadIdx.x; x < DK * DV / 8; x += THREADS) {
-            const int i = x / (DV / 8), j = x % (DV / 8) * 8;
-            if (i < p.Dk && col0 + j < p.Dv)
-              *reinterpret_cast<uint4 *>(to + i * p.Dv + j) = *reinterpret_cast<const uint4 *>(copy + i * LV + j);
-          }
-        } else {
-          for (int x = threadIdx.x; x < p.Dk * DV; x += THREADS)
-            if (col0 + x % DV < p.Dv) to[x / DV * p.Dv + x % DV] = copy[x / DV * LV + x % DV];
+        for (int x = threadIdx.x; x < DK * DV / 8; x += THREADS) {
+          const int i = x / (DV / 8), j = x % (DV / 8) * 8;
+          if (i < p.Dk && col0 + j < p.Dv)
+            *reinterpret_cast<uint4 *>(to + i * p.Dv + j) = *reinterpret_cast<const uint4 *>(copy + i * LV + j);
         }
+      } else {
+        for (int x = threadIdx.x; x < p.Dk * DV; x += THREADS)
+          if (col0 + x % DV < p.Dv) to[x / DV * p.Dv + x % DV] = copy[x / DV * LV + x % DV];
       }
-      uint32_t a[DK / 16][4];
+    }
+    const int start0 = episodeStart(mask, i0 + g), start1 = episodeStart(mask, i0 + g + 8);
+    const int start = episodeStart(mask, 63);   // the state after the chunk sees the steps from there on
+    uint32_t a[DK / 16][4];
+    float o[N][4];
+    if (OUT) {
 #pragma unroll
       for (int kk = 0; kk < DK / 16; ++kk) operandA<LQ>(a[kk], Q, i0, kk * 16);
-      float o[DV / 8][4];
 #pragma unroll
-      for (int n = 0; n < DV / 8; ++n)
+      for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[n][x] = 0.f;
       if (later) {   // Q S
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk)
 #pragma unroll
-          for (int n = 0; n < DV / 16; ++n) {
+          for (int n = 0; n < N / 2; ++n) {
             uint32_t b[4];
             operandBTransposed<LV>(b, copy, kk * 16, n * 16);
             multiplyAdd(o[2 * n], a[kk], b[0], b[1]);
@@ -399,17 +428,21 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
           }
         const float f0 = powers[16 + i0 + g + 1], f1 = powers[16 + i0 + g + 9];
 #pragma unroll
-        for (int n = 0; n < DV / 8; ++n)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
           for (int x = 0; x < 4; ++x) o[n][x] *= x < 2 ? f0 : f1;
         if (mask) {
 #pragma unroll
-          for (int n = 0; n < DV / 8; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[n][x] = (x < 2 ? start0 : start1) < 0 ? o[n][x] : 0.f;
         }
       }
-      for (int block = 0; block <= warp; ++block) {
+    }
+    if (OUT) {
+#pragma unroll
+      for (int block = 0; block < C / 16; ++block) {   // of 16 steps
+        if (block > warp) break;
         float s[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
@@ -433,14 +466,14 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
         const uint32_t w[4] = {packPair(s[0][0], s[0][1]), packPair(s[0][2], s[0][3]), packPair(s[1][0], s[1][1]),
                                packPair(s[1][2], s[1][3])};
 #pragma unroll
-        for (int n = 0; n < DV / 16; ++n) {
+        for (int n = 0; n < N / 2; ++n) {
           uint32_t b[4];
           operandBTransposed<LV>(b, V, block * 16, n * 16);
           multiplyAdd(o[2 * n], w, b[0], b[1]);
           multiplyAdd(o[2 * n + 1], w, b[2], b[3]);
         }
       }
-      // The warp's rows of Q are its own and done with.
+      // The warp has its rows of Q for itself and is done with them.
       bf16 *out = p.out + eh * p.Dv;
       const int64_t stepStride = int64_t(p.E) * p.H * p.Dv;
       if constexpr (DV <= DK)
@@ -449,9 +482,8 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
     }
 
     // The state at the chunk's end.
-    if (STATE && (c + 1 < chunks || last)) {
+    if (advance) {
       if (count < C) __syncthreads();   // toEnd
-      const int start = episodeStart(mask, 63);
       const float f = count == C ? fullChunk : power(count);
 #pragma unroll
       for (int m = 0; m < SM; ++m)
@@ -468,8 +500,8 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
             for (int x = 0; x < 4; ++x) S[m][n][x] = 0.f;
       }
 #pragma unroll
-      for (int kk = 0; kk < C / 16; ++kk) {
-        const int j = kk * 16 + 2 * tq;
+      for (int block = 0; block < C / 16; ++block) {
+        const int j = block * 16 + 2 * tq;
         float2 f0 = *reinterpret_cast<const float2 *>(toEnd + j), f1 = *reinterpret_cast<const float2 *>(toEnd + j + 8);
         if (mask) {
           f0.x = j >= start ? f0.x : 0.f;
@@ -479,18 +511,18 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
         }
 #pragma unroll
         for (int m = 0; m < SM; ++m) {
-          uint32_t a[4], high[4], low[4];
-          operandATransposed<LQ>(a, K, (sm0 + m) * 16, kk * 16);
+          uint32_t kt[4], high[4], low[4];
+          operandATransposed<LQ>(kt, K, (sm0 + m) * 16, block * 16);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {   // registers 0, 1: steps 2 tq, + 1; registers 2, 3: 8 later
-            const float l = lowOf(a[x]) * (x < 2 ? f0.x : f1.x), u = highOf(a[x]) * (x < 2 ? f0.y : f1.y);
+            const float l = lowOf(kt[x]) * (x < 2 ? f0.x : f1.x), u = highOf(kt[x]) * (x < 2 ? f0.y : f1.y);
             high[x] = packPair(l, u);
             low[x] = packPair(l - lowOf(high[x]), u - highOf(high[x]));
           }
 #pragma unroll
           for (int n = 0; n < SN / 2; ++n) {
             uint32_t b[4];
-            operandBTransposed<LV>(b, V, kk * 16, (sn0 + 2 * n) * 8);
+            operandBTransposed<LV>(b, V, block * 16, (sn0 + 2 * n) * 8);
             multiplyAdd(S[m][2 * n], high, b[0], b[1]);
             multiplyAdd(S[m][2 * n + 1], high, b[2], b[3]);
             if (p.precise) {
@@ -618,7 +650,9 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
       }
     }
     commitCopies();
-    const unsigned long long mask = resetMask(p.resets, p.E, e, first, min(t1, first + C));
+    Resets resets;
+    resets.read(p.resets, p.E, e, first, min(t1, first + C));
+    const unsigned long long mask = resets.mask();
     anyReset |= mask != 0;
     waitCopies();
     __syncthreads();
