@@ -376,10 +376,15 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
     const int buffer = buffers > 1 ? c & 1 : 0, first = t0 + c * C, count = min(C, t1 - first);
     const unsigned long long mask = resets.mask();
     anyReset |= mask != 0;
+    if (STATE && buffers == 1 && c > 0) {
+      __syncthreads();   // the tiles and the copy of the state are free
+      if (OUT) copySlice<LV>(copies, S, sm0, sn0);
+      load(c, 0);
+    }
     waitCopies();
     __syncthreads();
     if (c + 1 < chunks) {
-      load(c + 1, (c + 1) & 1);
+      if (buffers > 1) load(c + 1, (c + 1) & 1);
       resets.read(p.resets, p.E, e, first + C, min(t1, first + 2 * C));
     }
     const bf16 *K = tiles + buffer * chunkTileElements<C, DK, DV, OUT>(), *V = K + C * LQ, *Q = V + C * LV;
@@ -533,7 +538,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
         }
       }
       later = true;
-      if (OUT && c + 1 < chunks) copySlice<LV>(copies + ((c + 1) & 1) * DK * LV, S, sm0, sn0);
+      if (OUT && buffers > 1 && c + 1 < chunks) copySlice<LV>(copies + ((c + 1) & 1) * DK * LV, S, sm0, sn0);
     }
   }
   bool bad = (finite & 0x7fff7fffu) != 0;   // NaN
@@ -594,7 +599,7 @@ template <int C, int D, bool OUT> constexpr int backwardSharedBytes(bool later) 
 // passes through shared memory.  OUT = false: X' of a segment alone.
 // STATE = false is for one chunk whose first state's gradient nobody wants.
 template <int C, int D, bool OUT, bool STATE>
-__global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 64 : STATE ? 192 : 256) / C)
+__global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 64 : 256) / C)
     attentionChunksBackward(BackwardArgs p) {
   constexpr int W = backwardWarps<C, D, OUT>(), THREADS = W * 32, LD = D + 8;
   constexpr int PARTS = W / (C / 16);                          // warps that share 16 rows of the outputs

@@ -261,28 +261,31 @@ def _attention_plain(q, k, v, decay, state, resets, scale):
     return out.to(dtype), S
 
 
+# The type of states and scores beside a type of activations.
+_WIDE = {torch.float32: torch.float32, torch.bfloat16: torch.float32, torch.float16: torch.float32,
+         torch.float64: torch.float64}
+
+
 def _check_heads(q, k, v, decay, dims, what):
-    _require(q.dim() == k.dim() == v.dim() == dims and q.shape == k.shape and q.shape[:-1] == v.shape[:-1],
-             f"{what}: q and k have one shape, and v theirs but for its last axis")
-    _require(q.dtype == k.dtype == v.dtype and q.device == k.device == v.device,
-             f"{what}: q, k and v have one type and device")
-    _require(1 <= q.shape[-1] <= HEAD_MAX and 1 <= v.shape[-1] <= HEAD_MAX,
-             f"{what}: head sizes are 1 to {HEAD_MAX}")
+    qs, vs, dtype, device = q.shape, v.shape, q.dtype, q.device
+    _require(len(qs) == len(vs) == dims and qs == k.shape and qs[:-1] == vs[:-1],
+             "q and k have one shape, and v theirs but for its last axis")
+    _require(dtype == k.dtype == v.dtype and device == k.device == v.device and dtype in _WIDE,
+             "q, k and v have one floating type and device")
+    _require(1 <= qs[-1] <= HEAD_MAX and 1 <= vs[-1] <= HEAD_MAX, "head sizes are 1 to 128")
     _check_type(q, what)
-    _require(decay.shape == (q.shape[-2],) and decay.device == q.device, f"{what}: decay is [heads] on q's device")
-    _require(not decay.requires_grad, f"{what}: the decay is a constant of the layer, it has no gradient")
+    _require(decay.shape == qs[-2:-1] and decay.device == device, "decay is [heads] on q's device")
+    _require(not decay.requires_grad, "the decay is a constant of the layer, it has no gradient")
 
 
-def _check_state(state, q, v, what):
-    wide = torch.promote_types(q.dtype, torch.float32)
-    shape = (*q.shape[-3:], v.shape[-1])
-    _require(state.shape == shape and state.dtype == wide and state.device == q.device,
-             f"{what}: the state is {wide} [environments, heads, Dk, Dv] on q's device")
+def _check_state(state, q, v):
+    _require(state.shape == q.shape[-3:] + v.shape[-1:] and state.dtype == _WIDE[q.dtype] and state.device == q.device,
+             "the state is float32 [environments, heads, Dk, Dv] on q's device")
 
 
-def _mask(resets, shape, device, what):
+def _mask(resets, shape, device):
     _require(resets.shape == shape and resets.device == device and resets.dtype in (torch.bool, torch.uint8),
-             f"{what}: resets are bool or uint8 {list(shape)} on q's device")
+             "resets are bool or uint8 [steps, environments] on q's device")
     return resets if resets.is_contiguous() else resets.contiguous()
 
 
@@ -299,12 +302,11 @@ def linear_attention(q, k, v, decay, state=None, resets=None, scale=None, final_
     ``scale`` is Dk ** -0.5 by default.  The state after the last step is
     returned where ``final_state`` is set, else None.  Gradients flow to q, k,
     v and the state."""
-    what = "linear_attention"
-    _check_heads(q, k, v, decay, 4, what)
+    _check_heads(q, k, v, decay, 4, "linear_attention")
     if state is not None:
-        _check_state(state, q, v, what)
+        _check_state(state, q, v)
     if resets is not None:
-        resets = _mask(resets, q.shape[:2], q.device, what)
+        resets = _mask(resets, q.shape[:2], q.device)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if not q.is_cuda:
         out, last = _attention_plain(q, k, v, decay, state, resets, scale)
@@ -319,34 +321,35 @@ def linear_attention(q, k, v, decay, state=None, resets=None, scale=None, final_
     return _attention_forward(q, k, v, decay, state, resets, scale, final_state, False)[:2]
 
 
-@torch.no_grad()
 def linear_attention_step(q, k, v, decay, state, reset=None, scale=None):
     """One control step of ``linear_attention`` for every environment, without
     gradients: ``q`` and ``k`` [E, H, Dk], ``v`` [E, H, Dv], ``reset`` [E].
     ``state`` [E, H, Dk, Dv] float32 is updated in place; returns out
     [E, H, Dv]."""
-    what = "linear_attention_step"
-    _check_heads(q, k, v, decay, 3, what)
-    _check_state(state, q, v, what)
+    _check_heads(q, k, v, decay, 3, "linear_attention_step")
+    _check_state(state, q, v)
     if reset is not None:
-        reset = _mask(reset, q.shape[:1], q.device, what)
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+        reset = _mask(reset, q.shape[:1], q.device)
+    E, H, Dk = q.shape
+    scale = Dk ** -0.5 if scale is None else float(scale)
     if not q.is_cuda:
-        out, last = _attention_plain(q[None], k[None], v[None], decay, state, None if reset is None else reset[None],
-                                     scale)
-        state.copy_(last)
+        with torch.no_grad():
+            out, last = _attention_plain(q[None], k[None], v[None], decay, state,
+                                         None if reset is None else reset[None], scale)
+            state.copy_(last)
         return out[0]
-    _require(state.is_contiguous(), f"{what}: the state is updated in place and has to be contiguous")
+    _require(state.is_contiguous(), "the state is updated in place and has to be contiguous")
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     if decay.dtype != torch.float32 or not decay.is_contiguous():
         decay = decay.float().contiguous()
-    E, H, Dk = q.shape
-    out = torch.empty((E, H, v.shape[2]), dtype=q.dtype, device=q.device)
+    qe, qh, _ = q.stride()
+    ke, kh, _ = k.stride()
+    ve, vh, Dv = *v.stride()[:2], v.shape[2]
+    out = torch.empty((E, H, Dv), dtype=q.dtype, device=q.device)
     _launch(library().duck_linear_attention_step, q.device,
             _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr(),
                             _address(reset), 0, state.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0,
-                            0, *q.stride()[:2], 0, *k.stride()[:2], 0, *v.stride()[:2], 0, 0, 0,
-                            1, E, H, Dk, v.shape[2], _TYPES[q.dtype], scale))
+                            0, qe, qh, 0, ke, kh, 0, ve, vh, 0, 0, 0, 1, E, H, Dk, Dv, _TYPES[q.dtype], scale))
     return out
 
 
@@ -389,8 +392,8 @@ def elu_checkpoint(x):
     x = x.contiguous()
     n = x.shape[-1]
     y = torch.empty_like(x)
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], -(-n // GROUP)), dtype=torch.float32, device=x.device)
+    codes = torch.empty_like(x, dtype=torch.int8)
+    scales = torch.empty(x.shape[:-1] + (-(-n // GROUP),), dtype=torch.float32, device=x.device)
     _launch(library().duck_elu_checkpoint, x.device, x.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(),
             x.numel() // n, n, _TYPES[x.dtype])
     return y, Checkpoint8(codes, scales)
@@ -401,8 +404,8 @@ def elu_restore(dy, kept, restore=True):
     dx = dy (y > 0 ? 1 : 1 + y) and the kept output y in dy's type (None where
     ``restore`` is not set)."""
     codes, scales = kept
-    shape = (*codes.shape[:-1], -(-codes.shape[-1] // GROUP))
-    _require(dy.shape == codes.shape and scales.shape == shape and codes.dtype == torch.int8
+    shape = codes.shape
+    _require(dy.shape == shape and len(shape) and scales.shape == shape[:-1] + (-(-shape[-1] // GROUP),) and codes.dtype == torch.int8
              and scales.dtype == torch.float32 and dy.device == codes.device == scales.device,
              "elu_restore: the gradient and the checkpoint do not belong together")
     dy = dy.detach()
