@@ -101,13 +101,12 @@ template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluRest
   }
 }
 
-// exp(x) - 1 for x <= 0 to a few 1e-7 of itself, for results that are rounded to
-// bfloat16 next: its series where 1 would cancel (the sixth term is below
-// 0.25^5 / 720 = 1.4e-6 of the sum), else the hardware's power of two.
+// exp(x) - 1 for x <= 0 to some 4e-6 of itself, for results that are rounded to
+// bfloat16 (2^-8) next: its series where 1 would cancel (three terms; the fourth
+// is below 2^-15 / 24 = 1.3e-6 of the sum), else the hardware's power of two.
 __device__ __forceinline__ float eluRounded(float x) {
-  const float series = x * fmaf(x, fmaf(x, fmaf(x, fmaf(x, 1.f / 120.f, 1.f / 24.f), 1.f / 6.f), 0.5f), 1.f);
-  const float power = __expf(x) - 1.f;
-  const float below = x > -0.25f ? series : power;
+  const float series = x * fmaf(x, fmaf(x, 1.f / 6.f, 0.5f), 1.f), power = __expf(x) - 1.f;
+  const float below = x > -0.03125f ? series : power;
   return x > 0.f ? x : below;
 }
 

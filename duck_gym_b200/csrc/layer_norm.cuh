@@ -181,55 +181,73 @@ template <int LANES> __device__ __forceinline__ float2 teamSum(float2 x, float2 
 }
 
 __host__ __device__ constexpr int normBlock(int lanes) { return lanes > 32 ? lanes : 128; }
+// Blocks that are to fit on a multiprocessor at once, and that are launched for
+// it: a second, smaller round of blocks would cost as much as a full one
+// (backward, 393216 x 512: 313 us with 3 of 4 launched blocks resident).
+__host__ __device__ constexpr int normResident(int lanes, int values, bool backward) {
+  const int warps = backward ? (values <= 8 ? 20 : 16) : (values <= 8 ? 28 : 16);
+  return lanes > 128 ? (warps * 32 / lanes > 0 ? warps * 32 / lanes : 1) : warps / 4;
+}
+// Rows a team has in flight: some 32 KB a multiprocessor keep the memory busy, and
+// these are the fewest that give it at that many warps.
+__host__ __device__ constexpr int normAhead(int words, bool backward) {
+  return words <= 4 ? (backward ? 2 : 4) : words <= 8 && !backward ? 2 : 1;
+}
 
 template <class T, int LANES, int VEC, int P>
-__global__ void __launch_bounds__(normBlock(LANES)) normForwardRows(NormArgs p) {
+__global__ void __launch_bounds__(normBlock(LANES), normResident(LANES, P, false)) normForwardRows(NormArgs p) {
   constexpr int THREADS = normBlock(LANES), TEAMS = THREADS / LANES;
+  constexpr int AHEAD = normAhead(VEC == 1 ? P : P * int(sizeof(T)) / 4, false);
   __shared__ float2 red[2][16];
   const int lane = threadIdx.x % LANES;
   const int64_t step = int64_t(gridDim.x) * TEAMS;
   int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / LANES;
   const T *x = static_cast<const T *>(p.x);
   T *y = static_cast<T *>(p.y);
+  NormRow<T, LANES, VEC, P> next[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (row + k * step < p.rows) next[k].load(x + (row + k * step) * p.xStride, lane, p.n);
   float w[P], b[P];
   normColumns<LANES, VEC, P>(w, p.weight, 1.f, lane, p.n);
   normColumns<LANES, VEC, P>(b, p.bias, 0.f, lane, p.n);
-  const float inverse = 1.f / float(p.n);
-  NormRow<T, LANES, VEC, P> now, next;
   // All teams of a warp go round as often as its first: the sums are over whole warps.
   int64_t lead = LANES < 32 ? row - (threadIdx.x & 31) / LANES : row;
-  if (row < p.rows) next.load(x + row * p.xStride, lane, p.n);
-  for (; lead < p.rows; lead += step, row += step) {
-    now = next;
-    const bool live = row < p.rows;
-    if (row + step < p.rows) next.load(x + (row + step) * p.xStride, lane, p.n);
-    float v[P];
-    now.values(v);
-    float sum = 0.f;
+  for (; lead < p.rows; lead += AHEAD * step) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) sum += v[i];
-    const float mean = teamSum<LANES>(make_float2(sum, 0.f), red[0]).x / float(p.n);
-    float square = 0.f;
+    for (int k = 0; k < AHEAD; ++k, row += step) {
+      if (k > 0 && lead + k * step >= p.rows) break;
+      const bool live = row < p.rows;
+      float v[P];
+      next[k].values(v);
+      if (row + AHEAD * step < p.rows) next[k].load(x + (row + AHEAD * step) * p.xStride, lane, p.n);
+      float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int c = (lane + LANES * (i / VEC)) * VEC + i % VEC;
-      v[i] -= mean;
-      if (c < p.n) square = fmaf(v[i], v[i], square);
-    }
-    const float rstd = rsqrtf(teamSum<LANES>(make_float2(square, 0.f), red[1]).x * inverse + p.eps);
+      for (int i = 0; i < P; ++i) sum += v[i];
+      const float mean = teamSum<LANES>(make_float2(sum, 0.f), red[0]).x / float(p.n);
+      float square = 0.f;
 #pragma unroll
-    for (int i = 0; i < P; ++i) v[i] = fmaf(v[i] * rstd, w[i], b[i]);
-    if (live) {
-      NormRow<T, LANES, VEC, P>::store(y + row * p.n, v, lane, p.n);
-      if (p.stats && lane == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
+      for (int i = 0; i < P; ++i) {
+        const int c = (lane + LANES * (i / VEC)) * VEC + i % VEC;
+        v[i] -= mean;
+        if (c < p.n) square = fmaf(v[i], v[i], square);
+      }
+      const float rstd = rsqrtf(teamSum<LANES>(make_float2(square, 0.f), red[1]).x / float(p.n) + p.eps);
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[i] = fmaf(v[i] * rstd, w[i], b[i]);
+      if (live) {
+        NormRow<T, LANES, VEC, P>::store(y + row * p.n, v, lane, p.n);
+        if (p.stats && lane == 0) *reinterpret_cast<float2 *>(p.stats + 2 * row) = make_float2(mean, rstd);
+      }
     }
   }
 }
 
 // COLUMNS: the sums for the weight's and the bias' gradients too; DX: that of x.
 template <class T, int LANES, int VEC, int P, bool DX, bool COLUMNS>
-__global__ void __launch_bounds__(normBlock(LANES)) normBackwardRows(NormArgs p) {
+__global__ void __launch_bounds__(normBlock(LANES), normResident(LANES, P, true)) normBackwardRows(NormArgs p) {
   constexpr int THREADS = normBlock(LANES), TEAMS = THREADS / LANES;
+  constexpr int AHEAD = normAhead(VEC == 1 ? P : P * int(sizeof(T)) / 4, true);
   extern __shared__ float sums[];   // [warps, 2, n] where a team is a warp or less
   __shared__ float2 red[2][16];
   const int lane = threadIdx.x % LANES;
@@ -238,30 +256,32 @@ __global__ void __launch_bounds__(normBlock(LANES)) normBackwardRows(NormArgs p)
   const T *x = static_cast<const T *>(p.x), *dy = static_cast<const T *>(p.dy);
   T *dx = static_cast<T *>(p.dx);
   const float2 *stats = reinterpret_cast<const float2 *>(p.stats);
+  NormRow<T, LANES, VEC, P> nextX[AHEAD], nextY[AHEAD];
+  float2 nextStats[AHEAD];
+  auto load = [&](int k, int64_t r) {
+    nextX[k].load(x + r * p.xStride, lane, p.n);
+    nextY[k].load(dy + r * p.dyStride, lane, p.n);
+    nextStats[k] = stats[r];
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    nextStats[k] = make_float2(0.f, 0.f);
+    if (row + k * step < p.rows) load(k, row + k * step);
+  }
   float w[P], dw[P], db[P];
   if (DX) normColumns<LANES, VEC, P>(w, p.weight, 1.f, lane, p.n);
 #pragma unroll
   for (int i = 0; i < P; ++i) dw[i] = db[i] = 0.f;
   const float count = float(p.n);
-  NormRow<T, LANES, VEC, P> nowX, nowY, nextX, nextY;
-  float2 nextStats = make_float2(0.f, 0.f);
-  auto load = [&](int64_t r) {
-    nextX.load(x + r * p.xStride, lane, p.n);
-    nextY.load(dy + r * p.dyStride, lane, p.n);
-    nextStats = stats[r];
-  };
   int64_t lead = LANES < 32 ? row - (threadIdx.x & 31) / LANES : row;
-  if (row < p.rows) load(row);
   int turn = 0;
-  for (; lead < p.rows; lead += step, row += step) {
-    nowX = nextX;
-    nowY = nextY;
-    const float mean = nextStats.x, rstd = nextStats.y;
+  auto one = [&](int k) {
+    const float mean = nextStats[k].x, rstd = nextStats[k].y;
     const bool live = row < p.rows;
-    if (row + step < p.rows) load(row + step);
     float u[P], d[P];
-    nowX.values(u);
-    nowY.values(d);
+    nextX[k].values(u);
+    nextY[k].values(d);
+    if (row + AHEAD * step < p.rows) load(k, row + AHEAD * step);
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -285,6 +305,13 @@ __global__ void __launch_bounds__(normBlock(LANES)) normBackwardRows(NormArgs p)
 #pragma unroll
       for (int i = 0; i < P; ++i) d[i] = rstd * (d[i] - s.x - u[i] * s.y);
       if (live) NormRow<T, LANES, VEC, P>::store(dx + row * p.n, d, lane, p.n);
+    }
+  };
+  for (; lead < p.rows; lead += AHEAD * step) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k, row += step) {
+      if (k > 0 && lead + k * step >= p.rows) break;
+      one(k);
     }
   }
   if (!COLUMNS) return;

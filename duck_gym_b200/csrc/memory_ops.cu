@@ -57,15 +57,19 @@ template <class T, class F> void withNormRows(int n, bool pieces, F &&f) {
   else wide(Constant<1>());
 }
 // Blocks of a pass over the rows.
-int64_t normBlocks(int64_t rows, int n, bool pieces, int perSm) {
-  int teams = 1;
-  withNormRows<float>(n, pieces, [&](auto lanes, auto, auto) { teams = normBlock(lanes.value) / lanes.value; });
-  return std::max<int64_t>(1, std::min<int64_t>(ceilDiv(rows, teams), int64_t(148) * perSm));
+int64_t normBlocks(int64_t rows, int n, bool pieces, bool backward) {
+  int64_t blocks = 1;
+  withNormRows<float>(n, pieces, [&](auto lanes, auto, auto values) {
+    constexpr int L = lanes.value;
+    blocks = std::min<int64_t>(ceilDiv(rows, normBlock(L) / L),
+                               148 * (backward ? normResident(L, values.value, true) : normResident(L, values.value, false)));
+  });
+  return std::max<int64_t>(1, blocks);
 }
 
 // Partial rows that the sums of the weight's and bias' gradients come in.
 int64_t normSplits(int64_t rows, int n) {
-  if (n <= kNormWidest) return std::max(normBlocks(rows, n, true, 4), normBlocks(rows, n, false, 4));
+  if (n <= kNormWidest) return std::max(normBlocks(rows, n, true, true), normBlocks(rows, n, false, true));
   const int64_t columns = ceilDiv(n, 32);
   return std::max<int64_t>(1, std::min<int64_t>(ceilDiv(rows, 64), ceilDiv(148 * 8, columns)));
 }
@@ -351,7 +355,7 @@ int duck_layer_norm_forward(const void *x, const float *weight, const float *bia
       withNormRows<T>(n, pieces, [&](auto lanes, auto vec, auto values) {
         constexpr int L = lanes.value;
         normForwardRows<T, L, vec.value, values.value>
-            <<<unsigned(normBlocks(rows, n, pieces, L > 32 ? 8 : 16)), normBlock(L), 0, s>>>(a);
+            <<<unsigned(normBlocks(rows, n, pieces, false)), normBlock(L), 0, s>>>(a);
       });
     });
     check(cudaGetLastError(), "layer norm launch");
@@ -392,7 +396,7 @@ int duck_layer_norm_backward(const void *x, const void *dy, const float *weight,
       }
       withNormRows<T>(n, pieces, [&](auto lanes, auto vec, auto values) {
         constexpr int L = lanes.value, V = vec.value, P = values.value;
-        const int64_t blocks = normBlocks(rows, n, pieces, 4);
+        const int64_t blocks = normBlocks(rows, n, pieces, true);
         const int shared = L > 32 ? 0 : normBlock(L) / 32 * 2 * n * int(sizeof(float));
         splits = int(blocks);
         if (dx && columns) normBackwardRows<T, L, V, P, true, true><<<unsigned(blocks), normBlock(L), shared, s>>>(a);
