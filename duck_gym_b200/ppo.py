@@ -276,8 +276,7 @@ class PPO:
         torch.manual_seed(seed)
         obs = self._split(env.get_observations())
         self.obs, self.critic_obs = obs
-        self.policy = ActorCritic(self.obs.shape[1], self.critic_obs.shape[1], env.num_actions, self.cfg).to(
-            self.device)
+        self.policy = self._make_policy(env).to(self.device)
         self.world = dist.get_world_size() if dist.is_available() and dist.is_initialized() else 1
         if self.world > 1:
             for p in self.policy.parameters():   # every rank starts from rank 0's weights
@@ -298,6 +297,22 @@ class PPO:
         self._updates, self._ugraphs, self._flat_grad = 0, None, None
         self.storage = Storage(self.cfg.steps_per_env, env.num_envs, self.obs.shape[1], self.critic_obs.shape[1],
                                env.num_actions, self.device)
+
+    # What a policy with memory does differently (memory_policy.MemoryPPO).
+    def _make_policy(self, env):
+        return ActorCritic(self.obs.shape[1], self.critic_obs.shape[1], env.num_actions, self.cfg)
+
+    def _begin_rollout(self):
+        pass
+
+    def _before_step(self, t):
+        pass
+
+    def _after_step(self, done):
+        pass
+
+    def _last_values(self):
+        return self.policy.value(self.critic_obs)
 
     def _split(self, out):
         obs = out[0] if isinstance(out, tuple) else out
@@ -340,7 +355,9 @@ class PPO:
     def rollout(self):
         s, cfg = self.storage, self.cfg
         act = self._act_graphed if self.device.type == "cuda" and cfg.graph_rollout else self._act
+        self._begin_rollout()
         for t in range(cfg.steps_per_env):
+            self._before_step(t)
             actions, log_prob, mu, sigma, values = act(self.obs, self.critic_obs)
             s.obs[t], s.critic_obs[t] = self.obs, self.critic_obs
             s.actions[t] = actions
@@ -353,8 +370,9 @@ class PPO:
                 reward = reward + cfg.gamma * s.values[t] * info["time_outs"].to(self.device).float()
             s.rewards[t] = reward
             s.dones[t] = done.to(self.device).float()
+            self._after_step(s.dones[t])
             self.obs, self.critic_obs = self._split(obs)
-        last = self.policy.value(self.critic_obs)
+        last = self._last_values()
         returns, advantages = gae(s.rewards, s.dones, s.values, last, cfg.gamma, cfg.lam)
         s.returns.copy_(returns)   # in place: a captured update reads these buffers
         s.advantages.copy_((advantages - advantages.mean()) / (advantages.std() + 1e-8))
@@ -387,11 +405,14 @@ class PPO:
                 loss.backward()
                 self.reducer.finish()
                 nn.utils.clip_grad_norm_(self.policy.parameters(), cfg.max_grad_norm)
-                with warnings.catch_warnings():   # capturable Adam stepped outside a graph
-                    warnings.simplefilter("ignore", UserWarning)
-                    self.optimizer.step()
+                self._optimizer_step()
                 stats.append(info)
         return {k: torch.stack([x[k] for x in stats]).mean().item() for k in stats[0]}
+
+    def _optimizer_step(self):
+        with warnings.catch_warnings():   # capturable Adam stepped outside a graph
+            warnings.simplefilter("ignore", UserWarning)
+            self.optimizer.step()
 
     def _step_loss(self):
         """Forward and backward of one minibatch (the rows self._idx of the
