@@ -612,7 +612,7 @@ template <int C, int D, bool OUT> constexpr int backwardSharedBytes(bool later) 
 // passes through shared memory.  OUT = false: X' of a segment alone.
 // STATE = false is for one chunk whose first state's gradient nobody wants.
 template <int C, int D, bool OUT, bool STATE>
-__global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 64 : 256) / C)
+__global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 64 : STATE && C == 32 ? 192 : 256) / C)
     attentionChunksBackward(BackwardArgs p) {
   constexpr int W = backwardWarps<C, D, OUT>(), THREADS = W * 32, LD = D + 8;
   constexpr int PARTS = W / (C / 16);                          // warps that share 16 rows of the outputs
@@ -929,7 +929,7 @@ __global__ void __launch_bounds__(scanThreads(DI))
   for (int64_t eh = first; eh < end; ++eh) {
     any = false;
     for (int x = threadIdx.x; x < count; x += blockDim.x) any |= flags[eh * count + x] != 0;
-    if (__syncthreads_or(any)) scanSteps<bf16, DI>(s, eh, blockIdx.y);
+    if (__syncthreads_or(any)) scanSteps<bf16, DI, true>(s, eh, blockIdx.y, 0);
   }
 }
 

@@ -38,6 +38,12 @@ struct Sweep {
   const uint8_t *resets;       // [T, E] dense, or null
   int T, E, H, Di, Dj, ri, rj, reverse;
   float mulA, mulC;
+  // Where the steps are split (of few environments and heads): segments of the
+  // sweep, the states that they begin with [E, H, segments, ...] and whether an
+  // episode begins inside [E, H, segments].
+  int segmentLength, segments;
+  float *starts;
+  uint8_t *cuts;
 };
 
 // The recurrence step by step: float32 operands, and what redoAttention() finds.
@@ -76,7 +82,9 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
   return d;
 }
 
-template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile) {
+// OUT = false: what a segment adds to the state, in the place of the next one's start.
+template <class T, int DI, bool OUT>
+__device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile, int segment) {
   constexpr int LANES = scanLanes(DI), R = DI / LANES, THREADS = scanThreads(DI);
   constexpr int AC = kScanSteps * DI / THREADS, B = kScanSteps * kScanColumns / THREADS;   // values a thread fetches
   __shared__ __align__(16) float a[kScanSteps][DI], c[kScanSteps][DI];
@@ -85,7 +93,9 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
   __shared__ uint8_t cut[kScanSteps];
   const int e = int(eh / s.H), h = int(eh - int64_t(e) * s.H);
   const int lane = threadIdx.x % LANES, column = threadIdx.x / LANES * 2, first = tile * kScanColumns;
-  const int j = first + column, i0 = lane * R;
+  const int j = first + column;
+  // A lane's rows come in fours, those of neighbouring lanes side by side: 16-byte reads without bank conflicts.
+  auto rowOf = [&](int r) { return 4 * (lane + LANES * (r / 4)) + r % 4; };
   if (first >= s.Dj) return;   // the sweeps of a call may differ in their columns
   const T *pa = static_cast<const T *>(s.a) + e * s.as.e + h * s.as.h;
   const T *pb = static_cast<const T *>(s.b) + e * s.bs.e + h * s.bs.h + first;
@@ -93,6 +103,10 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
   T *py = static_cast<T *>(s.y) + eh * s.Dj + first;
   const int64_t yt = int64_t(s.E) * s.H * s.Dj, base = eh * s.Di * s.Dj;
   const float decay = s.decay[h];
+  const bool split = s.segments > 1;
+  const int start = segment * s.segmentLength, end = split ? min(s.T, start + s.segmentLength) : s.T;
+  const int64_t mine = split ? (eh * s.segments + segment) * s.Di * s.Dj : base;
+  const float *init = !split ? s.init : OUT ? s.starts : nullptr;
   Pair x[2][R / 2];
 #pragma unroll
   for (int k = 0; k < 2; ++k)
@@ -101,8 +115,8 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
       float v[2];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const int i = i0 + 2 * r + n;
-        v[n] = s.init && j + k < s.Dj && i < s.Di ? s.init[base + int64_t(i) * s.ri + int64_t(j + k) * s.rj] : 0.f;
+        const int i = rowOf(2 * r + n);
+        v[n] = init && j + k < s.Dj && i < s.Di ? init[mine + int64_t(i) * s.ri + int64_t(j + k) * s.rj] : 0.f;
       }
       x[k][r] = pairOf(v[0], v[1]);
     }
@@ -110,7 +124,7 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
   // BP-th, along pointers that go from tile to tile.
   constexpr int RP = THREADS / DI, BP = THREADS / kScanColumns;
   const int uA = threadIdx.x / DI, iA = threadIdx.x % DI, uB = threadIdx.x / kScanColumns, kB = threadIdx.x % kScanColumns;
-  const int64_t dir = s.reverse ? -1 : 1, begin = s.reverse ? s.T - 1 : 0;
+  const int64_t dir = s.reverse ? -1 : 1, begin = s.reverse ? s.T - 1 - start : start;
   const T *fromA = pa + (begin + dir * uA) * s.as.t + iA, *fromC = pc + (begin + dir * uA) * s.cs.t + iA;
   const T *fromB = pb + (begin + dir * uB) * s.bs.t + kB;
   T *toY = py + (begin + dir * uB) * yt + kB;
@@ -119,12 +133,12 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
   float nextA[AC], nextC[AC], nextB[B];
   bool nextCut = false;
   auto fetch = [&](int t0) {
-    const int left = s.T - t0;
+    const int left = end - t0;
 #pragma unroll
     for (int n = 0; n < AC; ++n) {
       const bool in = rowIn && n * RP + uA < left;
       nextA[n] = in ? s.mulA * toFloat(fromA[n * stepA]) : 0.f;
-      nextC[n] = in ? s.mulC * toFloat(fromC[n * stepC]) : 0.f;
+      nextC[n] = OUT && in ? s.mulC * toFloat(fromC[n * stepC]) : 0.f;
     }
 #pragma unroll
     for (int n = 0; n < B; ++n) nextB[n] = columnIn && n * BP + uB < left ? toFloat(fromB[n * stepB]) : 0.f;
@@ -135,11 +149,12 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
     // the later of the two in time.
     const int u = threadIdx.x;
     const int64_t t = s.reverse ? s.T - (t0 + u) : t0 + u;
-    nextCut = u < kScanSteps && t0 + u < s.T && s.resets && t < s.T && s.resets[t * s.E + e];
+    nextCut = u < kScanSteps && t0 + u < end && s.resets && t < s.T && s.resets[t * s.E + e];
   };
-  if (s.T > 0) fetch(0);
-  for (int t0 = 0; t0 < s.T; t0 += kScanSteps) {
-    const int count = min(kScanSteps, s.T - t0);
+  bool cutInside = false;
+  if (start < end) fetch(start);
+  for (int t0 = start; t0 < end; t0 += kScanSteps) {
+    const int count = min(kScanSteps, end - t0);
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < AC; ++n) {
@@ -154,23 +169,27 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
       factor[threadIdx.x] = s.reverse && t0 + int(threadIdx.x) == 0 ? 1.f : decay;
     }
     const bool anyCut = __syncthreads_or(nextCut);
-    if (t0 + kScanSteps < s.T) fetch(t0 + kScanSteps);
+    cutInside |= anyCut;
+    if (t0 + kScanSteps < end) fetch(t0 + kScanSteps);
     auto step = [&](int u) {
       const float2 value = *reinterpret_cast<const float2 *>(&b[u][column]);
       const Pair f2 = pairOf(factor[u], factor[u]), v2[2] = {pairOf(value.x, value.x), pairOf(value.y, value.y)};
       Pair sum[2] = {0, 0};
 #pragma unroll
       for (int r = 0; r < R / 2; r += 2) {
-        const ulonglong2 pairsA = *reinterpret_cast<const ulonglong2 *>(&a[u][i0 + 2 * r]);
-        const ulonglong2 pairsC = *reinterpret_cast<const ulonglong2 *>(&c[u][i0 + 2 * r]);
+        const ulonglong2 pairsA = *reinterpret_cast<const ulonglong2 *>(&a[u][rowOf(2 * r)]);
+        const ulonglong2 pairsC = *reinterpret_cast<const ulonglong2 *>(&c[u][rowOf(2 * r)]);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           x[k][r] = fma2(f2, x[k][r], mul2(pairsA.x, v2[k]));
           x[k][r + 1] = fma2(f2, x[k][r + 1], mul2(pairsA.y, v2[k]));
-          sum[k] = fma2(pairsC.x, x[k][r], sum[k]);
-          sum[k] = fma2(pairsC.y, x[k][r + 1], sum[k]);
+          if (OUT) {
+            sum[k] = fma2(pairsC.x, x[k][r], sum[k]);
+            sum[k] = fma2(pairsC.y, x[k][r + 1], sum[k]);
+          }
         }
       }
+      if (!OUT) return;
       float2 p0 = parts(sum[0]), p1 = parts(sum[1]);
       float2 total = make_float2(p0.x + p0.y, p1.x + p1.y);
 #pragma unroll
@@ -195,24 +214,26 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
       }
     }
     __syncthreads();
-    if (s.y && columnIn) {
+    if (OUT && s.y && columnIn) {
 #pragma unroll
       for (int n = 0; n < B; ++n)
         if (n * BP + uB < count) toY[n * stepY] = fromFloat<T>(y[n * BP + uB][kB]);
     }
     toY += B * stepY;
   }
-  if (s.last) {
+  if (!OUT && tile == 0 && threadIdx.x == 0) s.cuts[eh * s.segments + segment] = cutInside;
+  float *last = !OUT ? s.starts + mine : segment + 1 == s.segments && s.last ? s.last + base : nullptr;
+  if (last) {
     // Backwards, the state before the first step is one more factor away.
-    const bool gone = s.reverse && s.T > 0 && s.resets && s.resets[e];
-    const float f = s.reverse && s.T > 0 ? decay : 1.f;
+    const bool gone = OUT && s.reverse && s.T > 0 && s.resets && s.resets[e];
+    const float f = OUT && s.reverse && s.T > 0 ? decay : 1.f;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int r = 0; r < R / 2; ++r) {
         const float2 v = parts(x[k][r]);
-        const int i = i0 + 2 * r;
-        float *to = s.last + base + int64_t(i) * s.ri + int64_t(j + k) * s.rj;
+        const int i = rowOf(2 * r);
+        float *to = last + int64_t(i) * s.ri + int64_t(j + k) * s.rj;
         if (j + k < s.Dj && i < s.Di) to[0] = gone ? 0.f : f * v.x;
         if (j + k < s.Dj && i + 1 < s.Di) to[s.ri] = gone ? 0.f : f * v.y;
       }
@@ -223,9 +244,33 @@ template <class T, int DI> __device__ __forceinline__ void scanSteps(const Sweep
 struct Sweeps {
   Sweep s[3];
 };
-template <class T, int DI>
-__global__ void __launch_bounds__(scanThreads(DI)) attentionScan(const __grid_constant__ Sweeps p) {
-  scanSteps<T, DI>(p.s[blockIdx.z], blockIdx.x, blockIdx.y);
+template <class T, int DI, bool OUT>
+__global__ void __launch_bounds__(scanThreads(DI)) attentionScan(const __grid_constant__ Sweeps p, int tiles) {
+  scanSteps<T, DI, OUT>(p.s[blockIdx.z], blockIdx.x, blockIdx.y % tiles, blockIdx.y / tiles);
+}
+// The states that the segments of a sweep begin with, from what each adds, in place.
+__global__ void __launch_bounds__(256) joinSweeps(const __grid_constant__ Sweeps p) {
+  const Sweep &s = p.s[blockIdx.z];
+  const int64_t eh = blockIdx.x, size = int64_t(s.Di) * s.Dj, at = int64_t(blockIdx.y) * blockDim.x + threadIdx.x;
+  if (at >= size) return;
+  const float decay = s.decay[eh % s.H];
+  float x = s.init ? s.init[eh * size + at] : 0.f;
+  float *states = s.starts + eh * s.segments * size + at;
+  constexpr int AHEAD = 8;
+  for (int g0 = 0; g0 < s.segments; g0 += AHEAD) {
+    float added[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) added[k] = g0 + k + 1 < s.segments ? states[(g0 + k) * size] : 0.f;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int g = g0 + k;
+      if (g >= s.segments) break;
+      states[g * size] = x;
+      // A step backwards from the end has no factor before it.
+      const float f = powf(decay, float(s.segmentLength - (s.reverse && g == 0)));
+      x = s.cuts[eh * s.segments + g] ? added[k] : fmaf(f, x, added[k]);
+    }
+  }
 }
 
 struct StepOf {

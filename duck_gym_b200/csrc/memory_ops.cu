@@ -115,15 +115,59 @@ int mostColumns(const Sweeps &p, int count) {
   for (int i = 0; i < count; ++i) n = std::max(n, p.s[i].Dj);
   return n;
 }
-template <class T> void launchScan(const Sweeps &p, int count, cudaStream_t stream) {
-  const int rows = mostRows(p, count);
-  const dim3 grid(unsigned(int64_t(p.s[0].E) * p.s[0].H), unsigned(ceilDiv(mostColumns(p, count), kScanColumns)),
-                  unsigned(count));
-  if (rows <= 16) attentionScan<T, 16><<<grid, scanThreads(16), 0, stream>>>(p);
-  else if (rows <= 32) attentionScan<T, 32><<<grid, scanThreads(32), 0, stream>>>(p);
-  else if (rows <= 64) attentionScan<T, 64><<<grid, scanThreads(64), 0, stream>>>(p);
-  else attentionScan<T, 128><<<grid, scanThreads(128), 0, stream>>>(p);
+template <class T, bool OUT> void launchScan(const Sweeps &p, int count, int segments, cudaStream_t stream) {
+  const int rows = mostRows(p, count), tiles = int(ceilDiv(mostColumns(p, count), kScanColumns));
+  const dim3 grid{unsigned(int64_t(p.s[0].E) * p.s[0].H), unsigned(tiles * segments), unsigned(count)};
+  if (rows <= 16) attentionScan<T, 16, OUT><<<grid, scanThreads(16), 0, stream>>>(p, tiles);
+  else if (rows <= 32) attentionScan<T, 32, OUT><<<grid, scanThreads(32), 0, stream>>>(p, tiles);
+  else if (rows <= 64) attentionScan<T, 64, OUT><<<grid, scanThreads(64), 0, stream>>>(p, tiles);
+  else attentionScan<T, 128, OUT><<<grid, scanThreads(128), 0, stream>>>(p, tiles);
   check(cudaGetLastError(), "linear attention launch");
+}
+
+// How a call's steps are split where it has fewer blocks than four a multiprocessor: segments of 64 steps at least.
+struct ScanPlan {
+  int segmentLength, segments;
+  int64_t stateBytes, cutBytes;   // of one sweep
+};
+ScanPlan planScan(const duck_attention &a) {
+  const int64_t blocks = int64_t(a.E) * a.H * ceilDiv(std::max(a.Dk, a.Dv), kScanColumns);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(a.T / 64, 4 * 148 / blocks));
+  ScanPlan p{};
+  p.segmentLength = int(ceilDiv(ceilDiv(std::max(1, a.T), want), kScanSteps) * kScanSteps);
+  p.segments = std::max(1, int(ceilDiv(a.T, p.segmentLength)));
+  if (p.segments > 1) {
+    p.cutBytes = ceilDiv(int64_t(a.E) * a.H * p.segments, 16) * 16;
+    p.stateBytes = ceilDiv(int64_t(a.E) * a.H * p.segments * a.Dk * a.Dv, 4) * 16;
+  }
+  return p;
+}
+// `own`: which sweeps find their segments' starts; the others share another's.
+template <class T>
+void runScan(const duck_attention &a, Sweeps p, int count, std::initializer_list<int> own, cudaStream_t stream) {
+  const ScanPlan plan = planScan(a);
+  for (int i = 0; i < count; ++i) {
+    p.s[i].segmentLength = plan.segmentLength;
+    p.s[i].segments = plan.segments;
+  }
+  if (plan.segments > 1) {
+    require(a.scratch, "Invalid arguments");
+    Sweeps first{};
+    int n = 0;
+    for (int i : own) {
+      unsigned char *at = reinterpret_cast<unsigned char *>(a.scratch) + n * (plan.stateBytes + plan.cutBytes);
+      p.s[i].starts = reinterpret_cast<float *>(at);
+      p.s[i].cuts = at + plan.stateBytes;
+      first.s[n++] = p.s[i];
+    }
+    for (int i = 0; i < count; ++i)   // (the gradient of k goes along that of v, its state turned)
+      if (!p.s[i].starts) p.s[i].starts = first.s[n - 1].starts, p.s[i].cuts = first.s[n - 1].cuts;
+    launchScan<T, false>(first, n, plan.segments - 1, stream);
+    const dim3 grid{unsigned(int64_t(a.E) * a.H), unsigned(ceilDiv(int64_t(a.Dk) * a.Dv, 256)), unsigned(n)};
+    joinSweeps<<<grid, 256, 0, stream>>>(first);
+    check(cudaGetLastError(), "linear attention launch");
+  }
+  launchScan<T, true>(p, count, plan.segments, stream);
 }
 // One round of blocks: there is usually nothing to do but to look at the flags.
 void launchRedo(const Sweeps &p, int count, const uint8_t *flags, int flagCount, cudaStream_t stream) {
@@ -137,19 +181,19 @@ void launchRedo(const Sweeps &p, int count, const uint8_t *flags, int flagCount,
 
 Sweep forwardSweep(const duck_attention &a) {
   return {a.k, a.v, a.q, a.out, rowsOf(a.k_stride), rowsOf(a.v_stride), rowsOf(a.q_stride), a.state_in, a.state_out,
-          a.decay, a.resets, a.T, a.E, a.H, a.Dk, a.Dv, a.Dv, 1, 0, 1.f, a.scale};
+          a.decay, a.resets, a.T, a.E, a.H, a.Dk, a.Dv, a.Dv, 1, 0, 1.f, a.scale, a.T, 1, nullptr, nullptr};
 }
 Sweep gradientOfQ(const duck_attention &a) {
   return {a.v, a.k, a.dout, a.dq, rowsOf(a.v_stride), rowsOf(a.k_stride), rowsOf(a.dout_stride), a.state_in, nullptr,
-          a.decay, a.resets, a.T, a.E, a.H, a.Dv, a.Dk, 1, a.Dv, 0, 1.f, a.scale};
+          a.decay, a.resets, a.T, a.E, a.H, a.Dv, a.Dk, 1, a.Dv, 0, 1.f, a.scale, a.T, 1, nullptr, nullptr};
 }
 Sweep gradientOfK(const duck_attention &a) {
   return {a.dout, a.q, a.v, a.dk, rowsOf(a.dout_stride), rowsOf(a.q_stride), rowsOf(a.v_stride), a.dstate_out, nullptr,
-          a.decay, a.resets, a.T, a.E, a.H, a.Dv, a.Dk, 1, a.Dv, 1, a.scale, 1.f};
+          a.decay, a.resets, a.T, a.E, a.H, a.Dv, a.Dk, 1, a.Dv, 1, a.scale, 1.f, a.T, 1, nullptr, nullptr};
 }
 Sweep gradientOfV(const duck_attention &a) {   // and of the state
   return {a.q, a.dout, a.k, a.dv, rowsOf(a.q_stride), rowsOf(a.dout_stride), rowsOf(a.k_stride), a.dstate_out,
-          a.dstate_in, a.decay, a.resets, a.T, a.E, a.H, a.Dk, a.Dv, a.Dv, 1, 1, a.scale, 1.f};
+          a.dstate_in, a.decay, a.resets, a.T, a.E, a.H, a.Dk, a.Dv, a.Dv, 1, 1, a.scale, 1.f, a.T, 1, nullptr, nullptr};
 }
 
 // How a forward or backward call in bfloat16 is laid out.
@@ -440,7 +484,13 @@ int duck_linear_attention_sizes(const duck_attention *args, int64_t *out) {
   return guarded([&] {
     require(out != nullptr, "Invalid arguments");
     out[0] = out[1] = out[2] = 0;
-    if (!attentionChecked(args) || args->type != DUCK_BFLOAT16 || args->T == 0) return;
+    if (!attentionChecked(args) || args->T == 0) return;
+    if (args->type != DUCK_BFLOAT16) {
+      const ScanPlan plan = planScan(*args);
+      out[0] = plan.stateBytes + plan.cutBytes;
+      out[1] = 2 * out[0];
+      return;
+    }
     const ChunkPlan plan = planChunks(*args, false), back = planChunks(*args, true);
     out[0] = plan.segmentBytes + plan.cutBytes + plan.flagBytes;
     out[1] = back.segmentBytes + back.cutBytes + back.flagBytes;
@@ -459,7 +509,7 @@ int duck_linear_attention_forward(const duck_attention *args, duck_stream stream
       return;
     }
     const Sweeps p{{forwardSweep(a)}};
-    withType(a.type, [&](auto zero) { launchScan<decltype(zero)>(p, 1, reinterpret_cast<cudaStream_t>(stream)); });
+    withType(a.type, [&](auto zero) { runScan<decltype(zero)>(a, p, 1, {0}, reinterpret_cast<cudaStream_t>(stream)); });
   });
 }
 
@@ -474,7 +524,7 @@ int duck_linear_attention_backward(const duck_attention *args, duck_stream strea
       return;
     }
     const Sweeps p{{gradientOfQ(a), gradientOfK(a), gradientOfV(a)}};
-    withType(a.type, [&](auto zero) { launchScan<decltype(zero)>(p, 3, reinterpret_cast<cudaStream_t>(stream)); });
+    withType(a.type, [&](auto zero) { runScan<decltype(zero)>(a, p, 3, {0, 2}, reinterpret_cast<cudaStream_t>(stream)); });
   });
 }
 

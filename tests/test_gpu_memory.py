@@ -216,7 +216,7 @@ def test_attention_decays(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("T,E,H,D", [(3000, 1, 2, 64), (1500, 2, 1, 128), (2500, 1, 1, 24)])
+@pytest.mark.parametrize("T,E,H,D", [(3000, 1, 2, 64), (1500, 2, 1, 128), (2500, 1, 1, 24), (129, 1, 1, 16), (700, 3, 5, 33)])
 def test_attention_long(T, E, H, D, dtype):
     check_attention(attention_case(T, T, E, H, D, D, dtype, resets=0.005), dtype)
     check_attention(attention_case(T, T, E, H, D, D, dtype, state=False, resets=None), dtype, False)
