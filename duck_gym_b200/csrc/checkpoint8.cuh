@@ -34,9 +34,6 @@ struct CheckpointArgs {
   int n, groups;
 };
 
-// Largest magnitude of two; NaN if either is.
-__device__ __forceinline__ float maxOrNan(float a, float b) { return (a >= b || a != a) ? a : b; }
-
 struct GroupScale {
   float scale, inverse;
 };
@@ -50,57 +47,6 @@ __device__ __forceinline__ GroupScale groupScale(float largest) {
 __device__ __forceinline__ int encode(float y, float inverse) { return __float2int_rn(y * inverse); }
 
 __device__ __forceinline__ float elu(float x) { return x > 0.f ? x : expm1f(x); }
-
-// One warp per group, any width.
-template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluCheckpointAny(CheckpointArgs p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t total = p.rows * p.groups, warps = int64_t(gridDim.x) * (kCheckpointThreads / 32);
-  for (int64_t g = int64_t(blockIdx.x) * (kCheckpointThreads / 32) + threadIdx.x / 32; g < total; g += warps) {
-    const int64_t row = g / p.groups;
-    const int first = int(g - row * p.groups) * kGroup;
-    const int64_t at = row * p.n + first;
-    float y[kGroup / 32], largest = 0.f;
-#pragma unroll
-    for (int i = 0; i < kGroup / 32; ++i) {
-      const int c = lane + 32 * i;
-      y[i] = 0.f;
-      if (first + c < p.n) {
-        const T rounded = fromFloat<T>(elu(toFloat(static_cast<const T *>(p.in)[at + c])));
-        static_cast<T *>(p.y)[at + c] = rounded;
-        y[i] = toFloat(rounded);
-      }
-      largest = maxOrNan(fabsf(y[i]), largest);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) largest = maxOrNan(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    const GroupScale s = groupScale(largest);
-#pragma unroll
-    for (int i = 0; i < kGroup / 32; ++i)
-      if (first + lane + 32 * i < p.n) p.codes[at + lane + 32 * i] = int8_t(encode(y[i], s.inverse));
-    if (lane == 0) p.scales[g] = s.scale;
-  }
-}
-
-template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluRestoreAny(CheckpointArgs p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t total = p.rows * p.groups, warps = int64_t(gridDim.x) * (kCheckpointThreads / 32);
-  for (int64_t g = int64_t(blockIdx.x) * (kCheckpointThreads / 32) + threadIdx.x / 32; g < total; g += warps) {
-    const int64_t row = g / p.groups;
-    const int first = int(g - row * p.groups) * kGroup;
-    const int64_t at = row * p.n + first;
-    const float scale = p.scales[g];
-#pragma unroll
-    for (int i = 0; i < kGroup / 32; ++i) {
-      const int c = lane + 32 * i;
-      if (first + c >= p.n) continue;
-      const float y = float(p.codes[at + c]) * scale;
-      const float dy = toFloat(static_cast<const T *>(p.in)[at + c]);
-      if (p.y) static_cast<T *>(p.y)[at + c] = fromFloat<T>(y);
-      static_cast<T *>(p.dx)[at + c] = fromFloat<T>(dy * (y > 0.f ? 1.f : y + 1.f));
-    }
-  }
-}
-
 // exp(x) - 1 for x <= 0 to some 4e-6 of itself, for results that are rounded to
 // bfloat16 (2^-8) next: its series where 1 would cancel (three terms; the fourth
 // is below 2^-15 / 24 = 1.3e-6 of the sum), else the hardware's power of two.
@@ -108,6 +54,113 @@ __device__ __forceinline__ float eluRounded(float x) {
   const float series = x * fmaf(x, fmaf(x, 1.f / 6.f, 0.5f), 1.f), power = __expf(x) - 1.f;
   const float below = x > -0.03125f ? series : power;
   return x > 0.f ? x : below;
+}
+
+template <class T> __device__ __forceinline__ float eluFor(float x);
+template <> __device__ __forceinline__ float eluFor<float>(float x) { return elu(x); }
+template <> __device__ __forceinline__ float eluFor<bf16>(float x) { return eluRounded(x); }
+
+// Group `at` of the next ones of a team, without a division in the loop.
+struct GroupWalk {
+  int64_t row, rowStep;
+  int group, groupStep, groups;
+  __device__ __forceinline__ GroupWalk(int64_t first, int64_t step, int groups_)
+      : row(first / groups_), rowStep(step / groups_), group(int(first % groups_)), groupStep(int(step % groups_)),
+        groups(groups_) {}
+  __device__ __forceinline__ void next() {
+    if (++group == groups) {
+      group = 0;
+      ++row;
+    }
+  }
+  __device__ __forceinline__ void advance() {
+    row += rowStep;
+    group += groupStep;
+    if (group >= groups) {
+      group -= groups;
+      ++row;
+    }
+  }
+};
+
+// Rows of any width and place: a warp has four groups at a time, one value of each
+// quarter of a group a lane.
+constexpr int kGroupsAtOnce = 4;
+template <class T> __global__ void __launch_bounds__(kCheckpointThreads, 4) eluCheckpointAny(CheckpointArgs p) {
+  constexpr int U = kGroupsAtOnce, V = kGroup / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = int64_t(gridDim.x) * (kCheckpointThreads / 32);
+  const int64_t warp = int64_t(blockIdx.x) * (kCheckpointThreads / 32) + threadIdx.x / 32;
+  const T *x = static_cast<const T *>(p.in);
+  for (GroupWalk first(warp * U, warps * U, p.groups); first.row < p.rows; first.advance()) {
+    float y[U][V];
+    int64_t at[U];
+    int left[U];   // values of the group
+    GroupWalk now = first;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      at[u] = now.row * p.n + now.group * kGroup;
+      left[u] = now.row < p.rows ? min(kGroup, p.n - now.group * kGroup) : 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[u][i] = lane + 32 * i < left[u] ? toFloat(x[at[u] + lane + 32 * i]) : 0.f;
+      now.next();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t largest = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const T rounded = fromFloat<T>(eluFor<T>(y[u][i]));
+        if (lane + 32 * i < left[u]) static_cast<T *>(p.y)[at[u] + lane + 32 * i] = rounded;
+        y[u][i] = toFloat(rounded);
+        largest = max(largest, __float_as_uint(y[u][i]) & 0x7fffffffu);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      const GroupScale s = groupScale(__uint_as_float(largest));
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane + 32 * i < left[u]) p.codes[at[u] + lane + 32 * i] = int8_t(encode(y[u][i], s.inverse));
+      if (lane == 0 && left[u] > 0) p.scales[first.row * p.groups + first.group + u] = s.scale;
+    }
+  }
+}
+
+template <class T> __global__ void __launch_bounds__(kCheckpointThreads, 4) eluRestoreAny(CheckpointArgs p) {
+  constexpr int U = kGroupsAtOnce, V = kGroup / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = int64_t(gridDim.x) * (kCheckpointThreads / 32);
+  const int64_t warp = int64_t(blockIdx.x) * (kCheckpointThreads / 32) + threadIdx.x / 32;
+  const T *in = static_cast<const T *>(p.in);
+  for (GroupWalk first(warp * U, warps * U, p.groups); first.row < p.rows; first.advance()) {
+    float dy[U][V], scale[U];
+    int8_t code[U][V];
+    int64_t at[U];
+    int left[U];
+    GroupWalk now = first;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      at[u] = now.row * p.n + now.group * kGroup;
+      left[u] = now.row < p.rows ? min(kGroup, p.n - now.group * kGroup) : 0;
+      scale[u] = left[u] > 0 ? p.scales[first.row * p.groups + first.group + u] : 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool in_ = lane + 32 * i < left[u];
+        code[u][i] = in_ ? p.codes[at[u] + lane + 32 * i] : int8_t(0);
+        dy[u][i] = in_ ? toFloat(in[at[u] + lane + 32 * i]) : 0.f;
+      }
+      now.next();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (lane + 32 * i >= left[u]) continue;
+        const float y = float(code[u][i]) * scale[u];
+        if (p.y) static_cast<T *>(p.y)[at[u] + lane + 32 * i] = fromFloat<T>(y);
+        static_cast<T *>(p.dx)[at[u] + lane + 32 * i] = fromFloat<T>(dy[u][i] * (y > 0.f ? 1.f : y + 1.f));
+      }
+  }
 }
 
 // Eight or four values as the 16 bytes that they are moved in.
@@ -163,23 +216,6 @@ template <> struct Piece<float> {
   }
   static __device__ __forceinline__ uint4 round(const float (&x)[4]) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-  }
-};
-
-// Group `at` of the next ones of a team, without a division in the loop.
-struct GroupWalk {
-  int64_t row, rowStep;
-  int group, groupStep, groups;
-  __device__ __forceinline__ GroupWalk(int64_t first, int64_t step, int groups_)
-      : row(first / groups_), rowStep(step / groups_), group(int(first % groups_)), groupStep(int(step % groups_)),
-        groups(groups_) {}
-  __device__ __forceinline__ void advance() {
-    row += rowStep;
-    group += groupStep;
-    if (group >= groups) {
-      group -= groups;
-      ++row;
-    }
   }
 };
 

@@ -81,8 +81,8 @@ void launchGroups(const CheckpointArgs &a, int type, bool pieces, duck_stream st
   pieces = pieces && reinterpret_cast<uintptr_t>(a.codes) % 8 == 0;
   withType(type, [&](auto zero) {
     using T = decltype(zero);
-    const int lanes = pieces ? Piece<T>::lanes : 32;
-    const unsigned blocks = unsigned(std::min<int64_t>(ceilDiv(a.rows * a.groups, kCheckpointThreads / lanes), 148 * 8));
+    const int groups = pieces ? kCheckpointThreads / Piece<T>::lanes : kCheckpointThreads / 32 * kGroupsAtOnce;
+    const unsigned blocks = unsigned(std::min<int64_t>(ceilDiv(a.rows * a.groups, groups), 148 * 8));
     if (pieces && restore) eluRestorePieces<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
     else if (pieces) eluCheckpointPieces<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
     else if (restore) eluRestoreAny<T><<<blocks, kCheckpointThreads, 0, s>>>(a);

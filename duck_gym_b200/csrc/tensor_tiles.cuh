@@ -76,6 +76,16 @@ __device__ __forceinline__ uint32_t addZeroTimes(uint32_t pair, uint32_t sum) {
   return d;
 }
 
+// Two numbers as the sum of N pairs of bfloat16 numbers, each the rounding of what the ones before leave.
+template <int N> __device__ __forceinline__ void splitPair(uint32_t (&part)[N][4], int at, float low, float high) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    part[n][at] = packPair(low, high);
+    low -= lowOf(part[n][at]);
+    high -= highOf(part[n][at]);
+  }
+}
+
 // 16 bytes from global to shared memory without a register; zeros where !valid
 // (the address is then not read).
 __device__ __forceinline__ void copyAsync16(bf16 *to, const bf16 *from, bool valid) {

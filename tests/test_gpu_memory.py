@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.bfloat16]
 # States held in float32 from bfloat16 operands: an operand that carries a decay is kept as the sum of two
-# bfloat16 numbers (2^-16 relative at most), and sums are float32.
+# bfloat16 numbers at least (2^-16 relative at most), and sums are float32.
 STATE = 1e-5
 
 
