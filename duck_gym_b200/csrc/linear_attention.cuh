@@ -54,7 +54,11 @@ struct Sweep {
 // (float32 pairs), and a reduction over scanLanes() lanes.  The operands of 16
 // steps lie in shared memory while those of the next 16 are on their way in
 // registers; outputs leave 16 steps at a time.  Bound by instructions and shared
-// memory: each operand is moved from memory once.
+// memory: each operand is moved from memory once a sweep.  Measured on a B200,
+// float32, 101 steps, 301 environments, 3 heads of 20 x 28: forward and the three
+// backward sweeps 125 us, eight times their bytes' time; one row of eight in a lane
+// and one column instead of two: 156 us.  Few environments: 8192 steps, one head of 64,
+// forward and backward 187 us a call, split over the steps.
 constexpr int kScanSteps = 16, kScanColumns = 32;
 __host__ __device__ constexpr int scanLanes(int rows) { return rows > 64 ? 8 : rows > 16 ? 4 : 2; }
 __host__ __device__ constexpr int scanThreads(int rows) { return kScanColumns / 2 * scanLanes(rows); }
@@ -322,7 +326,8 @@ template <class T> __global__ void __launch_bounds__(128) attentionStepAny(StepO
 
 // The same with four columns a thread: bound by the state's way through memory,
 // 8 bytes an element, so the loads of eight rows are in flight before the first
-// is used, and a state that a reset clears is not read.
+// is used, and a state that a reset clears is not read.  4096 environments, 4 heads
+// of 64 x 64 on a B200: 83 us, 6.5 TB/s.
 template <class T> __global__ void __launch_bounds__(128) attentionStepQuads(StepOf s) {
   constexpr int AHEAD = 8;
   __shared__ float q[kHeadMax], k[kHeadMax];

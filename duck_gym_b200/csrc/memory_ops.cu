@@ -61,6 +61,8 @@ int64_t normBlocks(int64_t rows, int n, bool pieces, bool backward) {
   int64_t blocks = 1;
   withNormRows<float>(n, pieces, [&](auto lanes, auto, auto values) {
     constexpr int L = lanes.value;
+    // Up to 16 rows a team, one block: its sums need no second kernel, which costs as much as the rows do.
+    if (backward && rows <= 16 * (normBlock(L) / L)) return;
     blocks = std::min<int64_t>(ceilDiv(rows, normBlock(L) / L),
                                148 * (backward ? normResident(L, values.value, true) : normResident(L, values.value, false)));
   });
@@ -448,7 +450,7 @@ int duck_layer_norm_backward(const void *x, const void *dy, const float *weight,
         else normBackwardRows<T, L, V, P, false, true><<<unsigned(blocks), normBlock(L), shared, s>>>(a);
       });
     });
-    if (columns) normPartials<<<unsigned(ceilDiv(int64_t(2) * n, 32)), 1024, 0, s>>>(a, splits);
+    if (columns && (splits > 1 || n > kNormWidest)) normPartials<<<unsigned(ceilDiv(int64_t(2) * n, 32)), 1024, 0, s>>>(a, splits);
     check(cudaGetLastError(), "layer norm backward launch");
   });
 }

@@ -108,6 +108,11 @@ def _norm_forward(x, weight, bias, eps, keep):
     return y, rows, stats
 
 
+@functools.lru_cache(maxsize=1024)
+def _norm_scratch(rows, n):
+    return library().duck_layer_norm_scratch(rows, n)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -121,15 +126,12 @@ class _LayerNorm(torch.autograd.Function):
         x, weight, bias, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         rows, n = x.shape
-        dx = torch.empty(dy.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dx = _dense_like(dy) if need_x else None
         dw = torch.empty_like(weight) if need_w else None
         db = torch.empty_like(bias) if need_b else None
-        lib = library()
-        scratch = None
-        if need_w or need_b:
-            scratch = torch.empty(lib.duck_layer_norm_scratch(rows, n), dtype=torch.float32, device=x.device)
+        scratch = stats.new_empty(_norm_scratch(rows, n)) if need_w or need_b else None
         dy = _rows_of(dy)
-        _launch(lib.duck_layer_norm_backward, x.device, x.data_ptr(), dy.data_ptr(), _pointer(weight),
+        _launch(library().duck_layer_norm_backward, x.device, x.data_ptr(), dy.data_ptr(), _pointer(weight),
                 stats.data_ptr(), _pointer(dx), _pointer(dw), _pointer(db), _pointer(scratch), rows, n, x.stride(0),
                 dy.stride(0), _TYPES[x.dtype])
         return dx, dw, db, None
@@ -203,7 +205,7 @@ def _buffer(bytes_, device):
 def _attention_forward(q, k, v, decay, state, resets, scale, final_state, keep):
     T, E, H, Dk = q.shape
     Dv = v.shape[3]
-    out = torch.empty((T, E, H, Dv), dtype=q.dtype, device=q.device)
+    out = _dense_like(v)
     last = torch.empty((E, H, Dk, Dv), dtype=torch.float32, device=q.device) if final_state else None
     args = dict(out=out.data_ptr(), state_in=_address(state), state_out=_address(last))
     sizes = _workspace(T, E, H, Dk, Dv, _TYPES[q.dtype])
@@ -233,8 +235,7 @@ class _LinearAttention(torch.autograd.Function):
         Dv = v.shape[3]
         dout = q.new_zeros((T, E, H, Dv)) if dout is None else _dense_last(dout)
         dlast = None if dlast is None else _aligned(dlast)
-        dq, dk = (torch.empty((T, E, H, Dk), dtype=q.dtype, device=q.device) for _ in range(2))
-        dv = torch.empty((T, E, H, Dv), dtype=q.dtype, device=q.device)
+        dq, dk, dv = _dense_like(q), _dense_like(k), _dense_like(v)
         dstate = torch.empty_like(state) if ctx.needs_input_grad[4] else None
         args = dict(state_in=_address(state), dout=dout, dstate_out=_address(dlast), dq=dq.data_ptr(),
                     dk=dk.data_ptr(), dv=dv.data_ptr(), dstate_in=_address(dstate), saved=_address(saved))
@@ -345,7 +346,7 @@ def linear_attention_step(q, k, v, decay, state, reset=None, scale=None):
     qe, qh, _ = q.stride()
     ke, kh, _ = k.stride()
     ve, vh, Dv = *v.stride()[:2], v.shape[2]
-    out = torch.empty((E, H, Dv), dtype=q.dtype, device=q.device)
+    out = _dense_like(v)
     _launch(library().duck_linear_attention_step, q.device,
             _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr(),
                             _address(reset), 0, state.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0,

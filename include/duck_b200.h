@@ -360,8 +360,8 @@ enum { DUCK_FLOAT32 = 0, DUCK_BFLOAT16 = 1 };
 
 /* Layer norm of the rows of x [rows, n] (rows x_stride apart):
  * y = (x - mean) rstd weight + bias, y dense.  weight and bias [n] may be NULL
- * (1 and 0).  stats [rows, 2] receives mean and rstd for the backward pass, or
- * is NULL. */
+ * (1 and 0).  stats [rows, 2], on an 8-byte boundary, receives mean and rstd for
+ * the backward pass, or is NULL. */
 int duck_layer_norm_forward(const void *x, const float *weight, const float *bias, void *y, float *stats,
                             int64_t rows, int n, int64_t x_stride, double eps, int type, duck_stream stream);
 /* Floats of scratch that duck_layer_norm_backward needs; -1 for sizes that it
@@ -391,7 +391,8 @@ int duck_elu_restore(const void *dy, const int8_t *codes, const float *scales, v
  * 128; q, k, v and dout have the strides given, {t, e, h}; the outputs are
  * dense.  States are dense [E, H, Dk, Dv] float32.  decay [H] is in [0, 1].
  * Outputs, workspaces and the states of whole rollouts lie on 16-byte
- * boundaries. */
+ * boundaries, and no output overlaps an input (state_out is another array than
+ * state_in; the single step updates state_out alone, on any boundary). */
 typedef struct duck_attention {
   const void *q, *k, *v;
   void *out;                  /* forward */
