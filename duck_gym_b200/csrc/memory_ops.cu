@@ -286,7 +286,7 @@ void forwardChunks(const duck_attention &a, cudaStream_t stream) {
   c.vecK = dense16(a.k, a.k_stride, a.Dk);
   c.vecV = dense16(a.v, a.v_stride, a.Dv);
   c.scale = a.scale;
-  c.precise = a.state_out || split;
+  c.precise = a.state_out != nullptr;
   c.flags = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes + plan.cutBytes;
 // Two sets of tiles, except where they are so large (128 rows of state) that two blocks on a multiprocessor hide
   // a chunk's loads better than one block's own next set: 107 -> 90 us for the replay of 16384 steps.
@@ -356,7 +356,7 @@ void backwardChunks(const duck_attention &a, cudaStream_t stream) {
   c.vecV = dense16(a.v, a.v_stride, a.Dv);
   c.vecO = dense16(a.dout, a.dout_stride, a.Dv);
   c.scale = a.scale;
-  c.precise = a.dstate_in || split;
+  c.precise = a.dstate_in != nullptr;
   c.flags = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes + plan.cutBytes;
   if (split) {
     c.segments = a.scratch;

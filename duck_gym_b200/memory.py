@@ -245,6 +245,7 @@ class _LinearAttention(torch.autograd.Function):
         return dq, dk, dv, None, dstate, None, None, None
 
 
+@torch.autocast("cpu", enabled=False)
 def _attention_plain(q, k, v, decay, state, resets, scale):
     """The recurrence step by step, in float32 or wider."""
     dtype = q.dtype
@@ -463,4 +464,5 @@ def checkpointed_mlp(x, weights, biases):
     derivative of ELU and the next layer's weight gradient come from there."""
     _require(x.dim() == 2 and len(weights) == len(biases) > 0, "checkpointed_mlp: rows, weights and biases")
     _require(all(t.dtype == x.dtype for t in (*weights, *biases)), "checkpointed_mlp: one type for x and parameters")
-    return _CheckpointedMLP.apply(x, len(weights), *weights, *biases)
+    with torch.autocast(x.device.type, enabled=False):   # the backward pass multiplies in the same type
+        return _CheckpointedMLP.apply(x, len(weights), *weights, *biases)

@@ -292,6 +292,48 @@ def test_attention_keeps_episodes_and_the_future_apart(T, dtype):
     assert ref.error(o[:, 1, 1], want[0][:, 1, 1]) <= tol
 
 
+@pytest.mark.parametrize("Dk,Dv", [(16, 16), (64, 64), (128, 128), (40, 64), (128, 24), (7, 100)])
+def test_attention_keeps_apart_at_every_head_size(Dk, Dv):
+    for T in (20, 70, 300):
+        q, k, v, decay, S, _, do, dlast = attention_case(Dk + T, T, 3, 2, Dk, Dv, torch.bfloat16)
+        cut = T // 2
+        r = torch.zeros(T, 3, dtype=torch.bool)
+        r[cut] = True
+        want = ref.attention(q, k, v, decay, S, r, Dk ** -0.5, do, dlast)
+        for name in range(4):   # in v, k, q, the gradient of the output, of environment 1 alone
+            dirty = [t.clone() for t in (v, k, q, do)]
+            dirty[name][cut - 2, 1] = float("nan")
+            leaves = [t.cuda().requires_grad_() for t in (dirty[2], dirty[1], dirty[0])]
+            state = S.cuda().requires_grad_()
+            o, last = memory.linear_attention(*leaves, decay.cuda(), state, r.cuda())
+            grads = torch.autograd.grad([o, last], [*leaves, state], [dirty[3].cuda(), dlast.cuda()])
+            tol = ref.bound(torch.bfloat16, 1, 4)
+            assert ref.error(last, want[1]) <= STATE
+            for got, exact in zip((o, *grads[:3]), (want[0], *want[2:5])):
+                assert ref.error(got[cut:], exact[cut:]) <= tol
+                assert ref.error(got[:, ::2], exact[:, ::2]) <= tol
+            assert ref.error(o[:cut - 2], want[0][:cut - 2]) <= tol
+            assert ref.error(grads[0][:cut - 2], want[2][:cut - 2]) <= tol
+            assert ref.error(grads[1][cut - 1:], want[3][cut - 1:]) <= tol
+            assert ref.error(grads[3][::2], want[5][::2]) <= STATE
+
+
+def test_attention_of_a_state_at_an_odd_place():
+    T, E, H, D = 40, 2, 2, 32
+    q, k, v, decay, S, r, do, _ = attention_case(3, T, E, H, D, D, torch.bfloat16)
+    flat = torch.empty(S.numel() + 1, device="cuda")
+    state = flat[1:].view(S.shape).copy_(S)
+    want = ref.attention(q, k, v, decay, S, r, D ** -0.5)
+    o, last = memory.linear_attention(q.cuda(), k.cuda(), v.cuda(), decay.cuda(), state, r.cuda())
+    assert ref.error(o, want[0]) <= ref.bound(torch.bfloat16, 1, 4) and ref.error(last, want[1]) <= STATE
+    first = ref.attention(q[:1], k[:1], v[:1], decay, S, r[:1], D ** -0.5)
+    o = memory.linear_attention_step(q[0].cuda(), k[0].cuda(), v[0].cuda(), decay.cuda(), state, r[0].cuda())
+    assert ref.error(o, first[0][0]) <= ref.bound(torch.bfloat16, 1) and ref.error(state, first[1]) <= 1e-6
+    odd = torch.empty(q.numel() + 1, device="cuda", dtype=torch.bfloat16)[1:].view(q.shape).copy_(q)
+    o2, _ = memory.linear_attention(odd, k.cuda(), v.cuda(), decay.cuda(), S.cuda(), r.cuda())
+    assert ref.error(o2, want[0]) <= ref.bound(torch.bfloat16, 1, 4)
+
+
 def test_attention_empty_and_far():
     decay = torch.tensor([0.9], device="cuda")
     S = torch.randn(2, 1, 8, 8, device="cuda", requires_grad=True)
@@ -301,6 +343,8 @@ def test_attention_empty_and_far():
     dS, = torch.autograd.grad(last.sum(), S)
     assert torch.equal(dS, torch.ones_like(S))
     assert torch.equal(memory.linear_attention(q.detach(), q.detach(), q.detach(), decay)[1], torch.zeros_like(S))
+    q16 = q.detach().bfloat16()
+    assert torch.equal(memory.linear_attention(q16, q16, q16, decay, S.detach())[1], S)
     none = torch.zeros(4, 0, 1, 8, device="cuda")
     assert memory.linear_attention(none, none, none, decay)[0].shape == (4, 0, 1, 8)
     # Offsets past 2^31 elements between steps.

@@ -107,6 +107,18 @@ def test_checkpointed_mlp_gradients():
         assert ref.error(a, c) <= 0.02
 
 
+def test_checkpointed_mlp_under_autocast_and_its_second_derivative():
+    g = gen(7)
+    w, b = [torch.randn(6, 5, generator=g, requires_grad=True)], [torch.zeros(6, requires_grad=True)]
+    x = torch.randn(4, 5, generator=g, requires_grad=True)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        y = memory.checkpointed_mlp(x, w, b)
+    assert y.dtype == torch.float32
+    dx, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):   # there is no second one
+        torch.autograd.grad(dx.sum(), w)
+
+
 def test_refusals():
     x, decay = torch.zeros(4, 2, 1, 8), torch.ones(1)
     state = torch.zeros(2, 1, 8, 8)
