@@ -43,8 +43,9 @@
 // pipe 35 % active, shared memory 53 %, memory 45 % busy), backward 332 us; 24 steps,
 // 1024 environments: 29 and 44 us (3.9 and 3.5 TB/s); 16384 steps, one environment, 8
 // heads of 128, in 18 segments: 44 us for what each adds, 6 for the join, 94 us.
-// Tried and slower: two warps for the same 16 steps (235 us), rows of V read once for
-// scores and state (258 us), the backward blocks unrolled (357 us).
+// Tried and slower: two warps for the same 16 steps (235 us), 32 steps a warp (241 us
+// with a third fewer reads of shared memory), rows of V read once for scores and state
+// (258 us), the backward blocks unrolled (357 us).
 #pragma once
 #include "linear_attention.cuh"
 #include "tensor_tiles.cuh"

@@ -117,13 +117,13 @@ int mostColumns(const Sweeps &p, int count) {
   for (int i = 0; i < count; ++i) n = std::max(n, p.s[i].Dj);
   return n;
 }
-template <class T, bool OUT> void launchScan(const Sweeps &p, int count, int segments, cudaStream_t stream) {
+template <bool OUT> void launchScan(const Sweeps &p, int count, int segments, cudaStream_t stream) {
   const int rows = mostRows(p, count), tiles = int(ceilDiv(mostColumns(p, count), kScanColumns));
   const dim3 grid{unsigned(int64_t(p.s[0].E) * p.s[0].H), unsigned(tiles * segments), unsigned(count)};
-  if (rows <= 16) attentionScan<T, 16, OUT><<<grid, scanThreads(16), 0, stream>>>(p, tiles);
-  else if (rows <= 32) attentionScan<T, 32, OUT><<<grid, scanThreads(32), 0, stream>>>(p, tiles);
-  else if (rows <= 64) attentionScan<T, 64, OUT><<<grid, scanThreads(64), 0, stream>>>(p, tiles);
-  else attentionScan<T, 128, OUT><<<grid, scanThreads(128), 0, stream>>>(p, tiles);
+  if (rows <= 16) attentionScan<float, 16, OUT><<<grid, scanThreads(16), 0, stream>>>(p, tiles);
+  else if (rows <= 32) attentionScan<float, 32, OUT><<<grid, scanThreads(32), 0, stream>>>(p, tiles);
+  else if (rows <= 64) attentionScan<float, 64, OUT><<<grid, scanThreads(64), 0, stream>>>(p, tiles);
+  else attentionScan<float, 128, OUT><<<grid, scanThreads(128), 0, stream>>>(p, tiles);
   check(cudaGetLastError(), "linear attention launch");
 }
 
@@ -144,8 +144,7 @@ ScanPlan planScan(const duck_attention &a) {
   }
   return p;
 }
-// `own`: which sweeps find their segments' starts; the others share another's.
-template <class T>
+// float32 operands.  `own`: which sweeps find their segments' starts; the others share another's.
 void runScan(const duck_attention &a, Sweeps p, int count, std::initializer_list<int> own, cudaStream_t stream) {
   const ScanPlan plan = planScan(a);
   for (int i = 0; i < count; ++i) {
@@ -164,12 +163,12 @@ void runScan(const duck_attention &a, Sweeps p, int count, std::initializer_list
     }
     for (int i = 0; i < count; ++i)   // (the gradient of k goes along that of v, its state turned)
       if (!p.s[i].starts) p.s[i].starts = first.s[n - 1].starts, p.s[i].cuts = first.s[n - 1].cuts;
-    launchScan<T, false>(first, n, plan.segments - 1, stream);
+    launchScan<false>(first, n, plan.segments - 1, stream);
     const dim3 grid{unsigned(int64_t(a.E) * a.H), unsigned(ceilDiv(int64_t(a.Dk) * a.Dv, 256)), unsigned(n)};
     joinSweeps<<<grid, 256, 0, stream>>>(first);
     check(cudaGetLastError(), "linear attention launch");
   }
-  launchScan<T, true>(p, count, plan.segments, stream);
+  launchScan<true>(p, count, plan.segments, stream);
 }
 // One round of blocks: there is usually nothing to do but to look at the flags.
 void launchRedo(const Sweeps &p, int count, const uint8_t *flags, int flagCount, cudaStream_t stream) {
@@ -179,6 +178,14 @@ void launchRedo(const Sweeps &p, int count, const uint8_t *flags, int flagCount,
   if (mostRows(p, count) <= 32) redoAttention<32><<<grid, scanThreads(32), 0, stream>>>(p, flags, flagCount);
   else redoAttention<128><<<grid, scanThreads(128), 0, stream>>>(p, flags, flagCount);
   check(cudaGetLastError(), "linear attention launch");
+}
+
+// No steps: the state before them is the one after them.
+void copyState(const duck_attention &a, const float *from, float *to, cudaStream_t stream) {
+  if (!to) return;
+  const size_t bytes = size_t(a.E) * a.H * a.Dk * a.Dv * sizeof(float);
+  check(from ? cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, stream) : cudaMemsetAsync(to, 0, bytes, stream),
+        "linear attention state");
 }
 
 Sweep forwardSweep(const duck_attention &a) {
@@ -506,12 +513,10 @@ int duck_linear_attention_forward(const duck_attention *args, duck_stream stream
     const duck_attention &a = *args;
     require(a.decay && (a.T == 0 || (a.q && a.k && a.v && a.out)), "Invalid arguments");
     requireAligned({a.out, a.state_in, a.state_out, a.saved, a.scratch});
-    if (a.type == DUCK_BFLOAT16 && a.T > 0) {
-      forwardChunks(a, reinterpret_cast<cudaStream_t>(stream));
-      return;
-    }
-    const Sweeps p{{forwardSweep(a)}};
-    withType(a.type, [&](auto zero) { runScan<decltype(zero)>(a, p, 1, {0}, reinterpret_cast<cudaStream_t>(stream)); });
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (a.T == 0) copyState(a, a.state_in, a.state_out, s);
+    else if (a.type == DUCK_BFLOAT16) forwardChunks(a, s);
+    else runScan(a, {{forwardSweep(a)}}, 1, {0}, s);
   });
 }
 
@@ -521,12 +526,10 @@ int duck_linear_attention_backward(const duck_attention *args, duck_stream strea
     const duck_attention &a = *args;
     require(a.decay && (a.T == 0 || (a.q && a.k && a.v && a.dout && a.dq && a.dk && a.dv)), "Invalid arguments");
     requireAligned({a.state_in, a.dstate_out, a.dq, a.dk, a.dv, a.dstate_in, a.saved, a.scratch});
-    if (a.type == DUCK_BFLOAT16 && a.T > 0) {
-      backwardChunks(a, reinterpret_cast<cudaStream_t>(stream));
-      return;
-    }
-    const Sweeps p{{gradientOfQ(a), gradientOfK(a), gradientOfV(a)}};
-    withType(a.type, [&](auto zero) { runScan<decltype(zero)>(a, p, 3, {0, 2}, reinterpret_cast<cudaStream_t>(stream)); });
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (a.T == 0) copyState(a, a.dstate_out, a.dstate_in, s);
+    else if (a.type == DUCK_BFLOAT16) backwardChunks(a, s);
+    else runScan(a, {{gradientOfQ(a), gradientOfK(a), gradientOfV(a)}}, 3, {0, 2}, s);
   });
 }
 

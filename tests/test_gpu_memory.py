@@ -577,5 +577,14 @@ def test_c_entries_refuse():
     assert lib.duck_layer_norm_scratch(4, 0) == -1
     assert lib.duck_elu_checkpoint(p, p, None, p, 4, 8, 0, None) != 0
     assert lib.duck_elu_restore(p, p, p, None, p, -1, 8, 0, None) != 0
+    q, decay = torch.zeros(4, 2, 1, 8, device="cuda"), torch.ones(1, device="cuda")
+    state = torch.zeros(2, 1, 8, 8, device="cuda")
+    for wrong in (dict(out=0), dict(out=p, state_in=state.data_ptr() + 4)):
+        assert lib.duck_linear_attention_forward(memory._pack(q, q, q, decay, None, 1.0, **wrong), None) != 0
+    assert lib.duck_linear_attention_backward(memory._pack(q, q, q, decay, None, 1.0, out=p), None) != 0
+    wide = torch.zeros(1, 1, 1, 129, device="cuda")
+    assert lib.duck_linear_attention_step(memory._pack(wide, wide, wide, decay, None, 1.0, out=p), None) != 0
+    half = torch.zeros(4, 2, 1, 8, device="cuda", dtype=torch.bfloat16)
+    assert lib.duck_linear_attention_forward(memory._pack(half, half, half, decay, None, 1.0, out=p), None) != 0   # scratch
     assert lib.duck_linear_attention_forward(None, None) != 0
     assert b"Invalid" in lib.duck_last_error()
