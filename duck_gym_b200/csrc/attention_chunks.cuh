@@ -39,8 +39,8 @@
 // times 64, 24 steps a rollout) and half of a score matrix is masked; a warp's 16
 // steps are a natural piece of both.  What bounds them on a B200 is the operands' way from
 // shared memory and the latency of short chains of products, with 12 to 16 warps a
-// multiprocessor: 1000 steps, 256 environments, 4 heads of 64, forward 213 us (tensor
-// pipe 35 % active, shared memory 53 %, memory 45 % busy), backward 332 us; 24 steps,
+// multiprocessor: 1000 steps, 256 environments, 4 heads of 64, forward 204 us (tensor
+// pipe 35 % active, shared memory 53 %, memory 45 % busy), backward 328 us; 24 steps,
 // 1024 environments: 29 and 44 us (3.9 and 3.5 TB/s); 16384 steps, one environment, 8
 // heads of 128, in 18 segments: 44 us for what each adds, 6 for the join, 94 us.
 // Tried and slower: two warps for the same 16 steps (235 us), 32 steps a warp (241 us
@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
       }
     }
     const int start0 = episodeStart(mask, i0 + g), start1 = episodeStart(mask, i0 + g + 8);
+    const int lowest = episodeStart(mask, i0), highest = episodeStart(mask, i0 + 15);   // of the warp's steps
     const int start = episodeStart(mask, 63);   // the state after the chunk sees the steps from there on
     uint32_t a[DK / 16][4];
     float o[N][4];
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[n][x] = 0.f;
-      if (later) {   // Q S
+      if (later && lowest < 0) {   // Q S
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk)
 #pragma unroll
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
         for (int n = 0; n < N; ++n)
 #pragma unroll
           for (int x = 0; x < 4; ++x) o[n][x] *= x < 2 ? f0 : f1;
-        if (mask) {
+        if (highest >= 0) {
 #pragma unroll
           for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int x = 0; x < 4; ++x) s[n][x] *= f[(x >> 1) * 8 - (x & 1) - n * 8];
-        if (mask) {
+        if (block * 16 < highest) {
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
