@@ -327,9 +327,12 @@ def linear_attention_step(q, k, v, decay, state, reset=None, scale=None):
     """One control step of ``linear_attention`` for every environment, without
     gradients: ``q`` and ``k`` [E, H, Dk], ``v`` [E, H, Dv], ``reset`` [E].
     ``state`` [E, H, Dk, Dv] float32 is updated in place; returns out
-    [E, H, Dv]."""
+    [E, H, Dv].  A backward pass that still needs the state as it was raises, as
+    after any operation in place (a replay of a CUDA graph is not seen)."""
     _check_heads(q, k, v, decay, 3, "linear_attention_step")
     _check_state(state, q, v)
+    _require(not (state.requires_grad and torch.is_grad_enabled()),
+             "the state is updated in place without gradients, it must not require one")
     if reset is not None:
         reset = _mask(reset, q.shape[:1], q.device)
     E, H, Dk = q.shape
@@ -352,6 +355,7 @@ def linear_attention_step(q, k, v, decay, state, reset=None, scale=None):
             _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr(),
                             _address(reset), 0, state.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0,
                             0, qe, qh, 0, ke, kh, 0, ve, vh, 0, 0, 0, 1, E, H, Dk, Dv, _TYPES[q.dtype], scale))
+    torch.autograd.graph.increment_version(state)   # autograd does not see a kernel's writes
     return out
 
 

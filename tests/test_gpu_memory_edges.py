@@ -1,0 +1,51 @@
+"""GPU: the memory operators' kernels where autograd, states in place and values
+that are not finite meet, and the precision of states and outputs."""
+
+import pytest
+import torch
+
+import memory_math as ref
+from duck_gym_b200 import memory
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16]
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def normal(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [24, 150])
+def test_a_step_on_the_first_state_is_seen_by_the_backward_pass(T, dtype):
+    g = gen(T)
+    E, H, D = 2, 2, 32
+    q, k, v, do = (normal(g, T, E, H, D, dtype=dtype) for _ in range(4))
+    S, decay = normal(g, E, H, D, D), torch.tensor([0.9, 0.95])
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    step = [t[0].detach() for t in leaves]
+    state = S.cuda()
+    o, _ = memory.linear_attention(*leaves, decay.cuda(), state)
+    memory.linear_attention_step(*step, decay.cuda(), state)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(o, leaves, do.cuda())
+    # On a copy of the state, and before a rollout, a step is in nobody's way.
+    state = S.cuda()
+    o, _ = memory.linear_attention(*leaves, decay.cuda(), state)
+    memory.linear_attention_step(*step, decay.cuda(), state.clone())
+    grads = torch.autograd.grad(o, leaves, do.cuda())
+    want = ref.attention(q, k, v, decay, S, None, D ** -0.5, do)
+    for got, exact in zip(grads, want[2:5]):
+        assert ref.error(got, exact) <= ref.bound(dtype, (T + 8) * 2 * D, 4)
+    memory.linear_attention_step(*step, decay.cuda(), state)
+    o, _ = memory.linear_attention(*leaves, decay.cuda(), state)
+    torch.autograd.grad(o, leaves, do.cuda())
+    with torch.inference_mode():
+        memory.linear_attention_step(*step, decay.cuda(), torch.zeros_like(state))
