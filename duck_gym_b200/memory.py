@@ -29,6 +29,7 @@ from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .cuda_batch import _raise, library
@@ -82,7 +83,9 @@ def _check_type(x, what):
 
 
 def _grad_needed(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call goes through its autograd function: also wherever forward-mode
+    derivatives are on, since that refuses an input with a tangent."""
+    return forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 # ------------------------------------------------------------------ layer norm

@@ -49,3 +49,26 @@ def test_a_step_on_the_first_state_is_seen_by_the_backward_pass(T, dtype):
     torch.autograd.grad(o, leaves, do.cuda())
     with torch.inference_mode():
         memory.linear_attention_step(*step, decay.cuda(), torch.zeros_like(state))
+
+
+def test_forward_mode_derivatives_are_refused():
+    from torch.autograd import forward_ad
+
+    decay = torch.tensor([0.9, 0.95], device="cuda")
+    x = torch.randn(4, 3, 2, 8, device="cuda")
+    weight, state = torch.ones(8, device="cuda"), torch.randn(3, 2, 8, 8, device="cuda")
+    calls = [(memory.layer_norm, x), (lambda w: memory.layer_norm(x, w), weight),
+             (lambda q: memory.linear_attention(q, x, x, decay)[0], x),
+             (lambda v: memory.linear_attention(x, x, v, decay)[1], x),
+             (lambda S: memory.linear_attention(x, x, x, decay, S)[0], state)]
+    for f, at in calls:
+        want = f(at)
+        with forward_ad.dual_level():
+            assert torch.equal(f(at), want)   # no tangent, nothing to refuse
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    f(forward_ad.make_dual(at, torch.ones_like(at)))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (at,), (torch.ones_like(at),))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(at)
