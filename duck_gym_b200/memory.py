@@ -449,6 +449,11 @@ class _CheckpointedMLP(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dz):
+        with torch.autocast(dz.device.type, enabled=False):   # as in the forward pass
+            return _CheckpointedMLP._gradients(ctx, dz)
+
+    @staticmethod
+    def _gradients(ctx, dz):
         saved, n = ctx.saved_tensors, ctx.layers
         weights = saved[2 * n - 1:]
         dw, db, dx = [None] * n, [None] * n, None
@@ -471,5 +476,5 @@ def checkpointed_mlp(x, weights, biases):
     derivative of ELU and the next layer's weight gradient come from there."""
     _require(x.dim() == 2 and len(weights) == len(biases) > 0, "checkpointed_mlp: rows, weights and biases")
     _require(all(t.dtype == x.dtype for t in (*weights, *biases)), "checkpointed_mlp: one type for x and parameters")
-    with torch.autocast(x.device.type, enabled=False):   # the backward pass multiplies in the same type
+    with torch.autocast(x.device.type, enabled=False):   # products in x's type, in the backward pass too
         return _CheckpointedMLP.apply(x, len(weights), *weights, *biases)

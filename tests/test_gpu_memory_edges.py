@@ -72,3 +72,17 @@ def test_forward_mode_derivatives_are_refused():
             torch.func.jvp(f, (at,), (torch.ones_like(at),))
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda t: f(t).sum())(at)
+
+
+def test_checkpointed_mlp_backward_inside_autocast():
+    g = gen(2)
+    sizes = (61, 200, 96, 14)
+    w = [(normal(g, o, i) / i ** 0.5).cuda().requires_grad_() for i, o in zip(sizes, sizes[1:])]
+    b = [(0.1 * normal(g, o)).cuda().requires_grad_() for o in sizes[1:]]
+    x, dy = normal(g, 300, 61).cuda().requires_grad_(), normal(g, 300, 14).cuda()
+    want = torch.autograd.grad(memory.checkpointed_mlp(x, w, b), [x, *w, *b], dy)
+    y = memory.checkpointed_mlp(x, w, b)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = torch.autograd.grad(y, [x, *w, *b], dy)
+    for a, c in zip(got, want):
+        assert a.dtype == torch.float32 and ref.error(a, c) <= ref.bound(torch.float32, 300)

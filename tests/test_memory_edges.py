@@ -26,3 +26,19 @@ def test_step_refuses_a_state_that_requires_a_gradient():
         memory.linear_attention_step(q, k, v, decay, state)
     with torch.no_grad():
         memory.linear_attention_step(q, k, v, decay, state)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_checkpointed_mlp_backward_inside_autocast(dtype):
+    g = gen(1)
+    sizes = (7, 40, 30, 3)
+    w = [(torch.randn(o, i, generator=g) / i ** 0.5).to(dtype) for i, o in zip(sizes, sizes[1:])]
+    b = [(0.1 * torch.randn(o, generator=g)).to(dtype) for o in sizes[1:]]
+    leaves = [t.requires_grad_() for t in (torch.randn(50, 7, generator=g).to(dtype), *w, *b)]
+    dy = torch.randn(50, 3, generator=g).to(dtype)
+    run = lambda: memory.checkpointed_mlp(leaves[0], leaves[1:4], leaves[4:])
+    want = torch.autograd.grad(run(), leaves, dy)
+    y = run()
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))   # the very products of the pass outside
