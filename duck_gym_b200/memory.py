@@ -250,7 +250,9 @@ class _LinearAttention(torch.autograd.Function):
 
 @torch.autocast("cpu", enabled=False)
 def _attention_plain(q, k, v, decay, state, resets, scale):
-    """The recurrence step by step, in float32 or wider."""
+    """The recurrence step by step, in float32 or wider.  Element by element: the
+    gradient of a matrix product would be rounded to fewer bits by a backward
+    pass inside an autocast region."""
     dtype = q.dtype
     wide = torch.promote_types(dtype, torch.float32)
     T, E, H, Dk = q.shape
@@ -261,7 +263,7 @@ def _attention_plain(q, k, v, decay, state, resets, scale):
         if resets is not None:
             S = torch.where(resets[t, :, None, None, None] != 0, torch.zeros_like(S), S)
         S = decay * S + k[t][..., :, None] * v[t][..., None, :]
-        out.append((q[t][..., None, :] @ S)[..., 0, :])
+        out.append((q[t][..., :, None] * S).sum(-2))
     out = torch.stack(out) if T else q.new_zeros(0, E, H, v.shape[3])
     return out.to(dtype), S
 

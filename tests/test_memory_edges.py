@@ -42,3 +42,15 @@ def test_checkpointed_mlp_backward_inside_autocast(dtype):
     with torch.autocast("cpu", dtype=torch.bfloat16):
         got = torch.autograd.grad(y, leaves, dy)
     assert all(torch.equal(a, c) for a, c in zip(got, want))   # the very products of the pass outside
+
+
+def test_attention_backward_inside_autocast():
+    g = gen(2)
+    leaves = [t.requires_grad_() for t in (*heads(g, 9, 2, 2, 8), torch.randn(2, 2, 8, 8, generator=g))]
+    decay, do = torch.tensor([0.5, 0.9]), torch.randn(9, 2, 2, 8, generator=g)
+    run = lambda: memory.linear_attention(*leaves[:3], decay, leaves[3])[0]
+    want = torch.autograd.grad(run(), leaves, do)
+    out = run()
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = torch.autograd.grad(out, leaves, do)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
