@@ -257,7 +257,7 @@ def _attention_plain(q, k, v, decay, state, resets, scale):
     wide = torch.promote_types(dtype, torch.float32)
     T, E, H, Dk = q.shape
     q, k, v, decay = q.to(wide) * scale, k.to(wide), v.to(wide), decay.to(wide)[None, :, None, None]
-    S = q.new_zeros(E, H, Dk, v.shape[3]) if state is None else state
+    S = q.new_zeros(E, H, Dk, v.shape[3]) if state is None else state if T else state.clone()
     out = []
     for t in range(T):
         if resets is not None:

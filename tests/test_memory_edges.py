@@ -54,3 +54,12 @@ def test_attention_backward_inside_autocast():
     with torch.autocast("cpu", dtype=torch.bfloat16):
         got = torch.autograd.grad(out, leaves, do)
     assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_no_steps_give_a_state_of_its_own():
+    S = torch.randn(2, 1, 4, 4, generator=gen(3))
+    q = torch.zeros(0, 2, 1, 4)
+    _, last = memory.linear_attention(q, q, q, torch.tensor([0.9]), S)
+    assert torch.equal(last, S)
+    last.zero_()   # as a control step would
+    assert bool(S.abs().sum() > 0)
