@@ -6,6 +6,10 @@
 //   backward: dx = dy (kept > 0 ? 1 : 1 + kept), and the kept y itself for the
 //   weight gradient of the layer that consumed it.
 //
+// A kept value is off by half a step at most, so that a saturated unit's may lie
+// below -1, beside a largest value of 12 at -1.039.  The bounded backward pass takes
+// it as -1 in the derivative, which is then in [0, 1] as that of ELU is.
+//
 // The codes are those of the rounded y, the values that the next layer saw.
 // The division by 127 and by the scale are products with their float32
 // reciprocals.  A group whose scale would be zero or denormal keeps zeros; one
@@ -35,6 +39,7 @@ struct CheckpointArgs {
   float *scales;        // [rows, groups]
   int64_t rows;
   int n, groups;
+  float lowest;         // backward: kept values below it count as it in the derivative
 };
 
 struct GroupScale {
@@ -57,6 +62,11 @@ __device__ __forceinline__ float eluRounded(float x) {
   const float series = x * fmaf(x, fmaf(x, 1.f / 6.f, 0.5f), 1.f), power = __expf(x) - 1.f;
   const float below = x > -0.03125f ? series : power;
   return x > 0.f ? x : below;
+}
+
+// ELU's derivative from its kept output; NaN stays.
+__device__ __forceinline__ float eluSlope(float y, float lowest) {
+  return y > 0.f ? 1.f : (y < lowest ? lowest : y) + 1.f;
 }
 
 template <class T> __device__ __forceinline__ float eluFor(float x);
@@ -161,7 +171,7 @@ template <class T> __global__ void __launch_bounds__(kCheckpointThreads, 4) eluR
         if (lane + 32 * i >= left[u]) continue;
         const float y = float(code[u][i]) * scale[u];
         if (p.y) static_cast<T *>(p.y)[at[u] + lane + 32 * i] = fromFloat<T>(y);
-        static_cast<T *>(p.dx)[at[u] + lane + 32 * i] = fromFloat<T>(dy[u][i] * (y > 0.f ? 1.f : y + 1.f));
+        static_cast<T *>(p.dx)[at[u] + lane + 32 * i] = fromFloat<T>(dy[u][i] * eluSlope(y, p.lowest));
       }
   }
 }
@@ -309,7 +319,7 @@ template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluRest
       const uint32_t biased = codes[i / 4] ^ 0x80808080u;
       const float code = __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7440 + i % 4)) - 8388736.f;
       y[i] = code * scale;
-      dy[i] *= y[i] > 0.f ? 1.f : y[i] + 1.f;
+      dy[i] *= eluSlope(y[i], p.lowest);
     }
     const int64_t at = now.row * p.n + c;
     *reinterpret_cast<uint4 *>(static_cast<T *>(p.dx) + at) = Piece<T>::round(dy);

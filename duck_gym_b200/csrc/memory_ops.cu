@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <limits>
 #include <type_traits>
 
 using namespace duckb200;
@@ -89,6 +90,20 @@ void launchGroups(const CheckpointArgs &a, int type, bool pieces, duck_stream st
     else if (pieces) eluCheckpointPieces<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
     else if (restore) eluRestoreAny<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
     else eluCheckpointAny<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
+  });
+}
+
+int restoreElu(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows, int n, int type,
+               float lowest, duck_stream stream) {
+  return guarded([&] {
+    requireType(type);
+    require(rows >= 0 && n > 0, "Invalid checkpoint sizes");
+    if (rows == 0) return;
+    require(dy && codes && scales && dx, "Invalid arguments");
+    CheckpointArgs a{dy, y, dx, const_cast<int8_t *>(codes), const_cast<float *>(scales), rows, n,
+                     int(ceilDiv(n, kGroup)), lowest};
+    launchGroups(a, type, pieces16({dy, y, dx}, {int64_t(n)}, type), stream, true);
+    check(cudaGetLastError(), "checkpoint launch");
   });
 }
 
@@ -469,7 +484,7 @@ int duck_elu_checkpoint(const void *x, void *y, int8_t *codes, float *scales, in
     require(rows >= 0 && n > 0, "Invalid checkpoint sizes");
     if (rows == 0) return;
     require(x && y && codes && scales, "Invalid arguments");
-    CheckpointArgs a{x, y, nullptr, codes, scales, rows, n, int(ceilDiv(n, kGroup))};
+    CheckpointArgs a{x, y, nullptr, codes, scales, rows, n, int(ceilDiv(n, kGroup)), 0.f};
     launchGroups(a, type, pieces16({x, y}, {int64_t(n)}, type), stream, false);
     check(cudaGetLastError(), "checkpoint launch");
   });
@@ -477,16 +492,12 @@ int duck_elu_checkpoint(const void *x, void *y, int8_t *codes, float *scales, in
 
 int duck_elu_restore(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows, int n,
                      int type, duck_stream stream) {
-  return guarded([&] {
-    requireType(type);
-    require(rows >= 0 && n > 0, "Invalid checkpoint sizes");
-    if (rows == 0) return;
-    require(dy && codes && scales && dx, "Invalid arguments");
-    CheckpointArgs a{dy, y, dx, const_cast<int8_t *>(codes), const_cast<float *>(scales), rows, n,
-                     int(ceilDiv(n, kGroup))};
-    launchGroups(a, type, pieces16({dy, y, dx}, {int64_t(n)}, type), stream, true);
-    check(cudaGetLastError(), "checkpoint launch");
-  });
+  return restoreElu(dy, codes, scales, y, dx, rows, n, type, -std::numeric_limits<float>::infinity(), stream);
+}
+
+int duck_elu_restore_bounded(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows,
+                             int n, int type, duck_stream stream) {
+  return restoreElu(dy, codes, scales, y, dx, rows, n, type, -1.f, stream);
 }
 
 int duck_linear_attention_sizes(const duck_attention *args, int64_t *out) {

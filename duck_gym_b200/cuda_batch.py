@@ -80,7 +80,7 @@ def library():
         lib.duck_layer_norm_scratch.restype = L
         lib.duck_layer_norm_backward.argtypes = [P] * 8 + [L, I, L, L, I, P]
         lib.duck_elu_checkpoint.argtypes = [P] * 4 + [L, I, I, P]
-        lib.duck_elu_restore.argtypes = [P] * 5 + [L, I, I, P]
+        lib.duck_elu_restore.argtypes = lib.duck_elu_restore_bounded.argtypes = [P] * 5 + [L, I, I, P]
         lib.duck_linear_attention_sizes.argtypes = [P, P]
         for name in ("duck_linear_attention_forward", "duck_linear_attention_backward", "duck_linear_attention_step"):
             getattr(lib, name).argtypes = [P, P]
@@ -107,7 +107,7 @@ def library():
                      "duck_bam_critic_dim", "duck_bam_step", "duck_bam_begin", "duck_bam_substep", "duck_bam_finish",
                      "duck_bam_servo", "duck_bam_reset_buffers", "duck_bam_observe", "duck_ppo_loss_scratch",
                      "duck_ppo_loss", "duck_layer_norm_forward", "duck_layer_norm_backward", "duck_elu_checkpoint",
-                     "duck_elu_restore", "duck_linear_attention_sizes", "duck_linear_attention_forward",
+                     "duck_elu_restore", "duck_elu_restore_bounded", "duck_linear_attention_sizes", "duck_linear_attention_forward",
                      "duck_linear_attention_backward", "duck_linear_attention_step"):
             getattr(lib, name).restype = I
         _lib = lib

@@ -410,10 +410,12 @@ def elu_checkpoint(x):
     return y, Checkpoint8(codes, scales)
 
 
-def elu_restore(dy, kept, restore=True):
+def elu_restore(dy, kept, restore=True, bounded=False):
     """``(dx, y)`` from the gradient of elu's output and its checkpoint:
     dx = dy (y > 0 ? 1 : 1 + y) and the kept output y in dy's type (None where
-    ``restore`` is not set)."""
+    ``restore`` is not set).  A saturated unit's kept output may lie below -1, by
+    half a step of its group at most; with ``bounded`` it counts as -1 in dx, so that
+    the derivative is in [0, 1] as that of elu is."""
     codes, scales = kept
     shape = codes.shape
     _require(dy.shape == shape and len(shape) and scales.shape == shape[:-1] + (-(-shape[-1] // GROUP),) and codes.dtype == torch.int8
@@ -422,14 +424,16 @@ def elu_restore(dy, kept, restore=True):
     dy = dy.detach()
     if not dy.is_cuda:
         y = _kept_plain(kept)
-        dx = (dy.float() * torch.where(y > 0, torch.ones_like(y), y + 1.0)).to(dy.dtype)
+        below = torch.where(y < -1.0, -torch.ones_like(y), y) if bounded else y
+        dx = (dy.float() * torch.where(y > 0, torch.ones_like(y), below + 1.0)).to(dy.dtype)
         return dx, y.to(dy.dtype) if restore else None
     _check_type(dy, "elu_restore")
     dy, codes, scales = dy.contiguous(), codes.contiguous(), scales.contiguous()
     n = dy.shape[-1]
     dx = torch.empty_like(dy)
     y = torch.empty_like(dy) if restore else None
-    _launch(library().duck_elu_restore, dy.device, dy.data_ptr(), codes.data_ptr(), scales.data_ptr(), _pointer(y),
+    entry = library().duck_elu_restore_bounded if bounded else library().duck_elu_restore
+    _launch(entry, dy.device, dy.data_ptr(), codes.data_ptr(), scales.data_ptr(), _pointer(y),
             dx.data_ptr(), dy.numel() // n, n, _TYPES[dy.dtype])
     return dx, y
 
@@ -465,7 +469,7 @@ class _CheckpointedMLP(torch.autograd.Function):
                 y = saved[0]
                 dx = dz @ weights[0] if ctx.needs_input_grad[0] else None
             else:
-                dnext, y = elu_restore(dz @ weights[i], Checkpoint8(*saved[2 * i - 1:2 * i + 1]))
+                dnext, y = elu_restore(dz @ weights[i], Checkpoint8(*saved[2 * i - 1:2 * i + 1]), bounded=True)
             dw[i] = dz.t() @ y
             if i:
                 dz = dnext

@@ -383,6 +383,11 @@ int duck_elu_checkpoint(const void *x, void *y, int8_t *codes, float *scales, in
  * dx = dy (y > 0 ? 1 : 1 + y).  y may be NULL. */
 int duck_elu_restore(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows, int n,
                      int type, duck_stream stream);
+/* The same, but for kept values below -1 (of saturated units: a value is kept to
+ * half a step of its group), which count as -1 in dx, so that the derivative is in
+ * [0, 1] as that of ELU is. */
+int duck_elu_restore_bounded(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows,
+                             int n, int type, duck_stream stream);
 
 /* Linear attention with one decay per head, for E environments and H heads:
  *   S_t = f_t S_{t-1} + k_t v_t^T,  o_t = scale S_t^T q_t,

@@ -86,3 +86,26 @@ def test_checkpointed_mlp_backward_inside_autocast():
         got = torch.autograd.grad(y, [x, *w, *b], dy)
     for a, c in zip(got, want):
         assert a.dtype == torch.float32 and ref.error(a, c) <= ref.bound(torch.float32, 300)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [304, 300, 7])   # rows of whole 16-byte pieces and others
+def test_the_bounded_derivative_is_that_of_an_elu(n, dtype):
+    g = gen(n)
+    x = normal(g, 50, n) * 3 - 4
+    x[:, ::60] = 4 + 9 * torch.rand(50, 1, generator=g)
+    x[:, 1::7] = -30.0
+    x[0, 1], x[1, 1] = float("nan"), float("inf")
+    x = x.to(dtype).cuda()
+    y, kept = memory.elu_checkpoint(x)
+    dy = normal(g, 50, n, dtype=dtype).cuda()
+    plain, back = memory.elu_restore(dy, kept)
+    dx, same = memory.elu_restore(dy, kept, bounded=True)
+    stood = kept.codes.float() * kept.scales.repeat_interleave(128, 1)[:, :n]
+    assert bool((stood < -1).any()) and torch.equal(back[2:], same[2:])
+    slope = torch.where(stood > 0, 1.0, stood.clamp_min(-1) + 1)
+    assert torch.equal(dx[2:], (dy.float() * slope)[2:].to(dtype))
+    assert torch.equal(dx[stood >= -1], plain[stood >= -1]) and float((dx[2:] * dy[2:]).min()) >= 0.0
+    assert bool(dx[:2, :min(n, 128)].isnan().all())   # what is not finite stays visible
+    only, nothing = memory.elu_restore(dy, kept, restore=False, bounded=True)
+    assert nothing is None and torch.equal(only[2:], dx[2:])

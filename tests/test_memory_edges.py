@@ -63,3 +63,48 @@ def test_no_steps_give_a_state_of_its_own():
     assert torch.equal(last, S)
     last.zero_()   # as a control step would
     assert bool(S.abs().sum() > 0)
+
+
+def saturated(g):
+    """Rows whose groups have a largest value of 12, 5 or 40 and many units that are saturated, or nearly."""
+    x = torch.randn(3, 300, generator=g) * 3 - 4
+    x[:, ::60] = torch.tensor([12.0, 5.0, 40.0])[:, None]
+    x[:, 1::7] = -30.0
+    return x
+
+
+def test_the_bounded_derivative_is_that_of_an_elu():
+    x = saturated(gen(4))
+    y, kept = memory.elu_checkpoint(x)
+    ones = torch.ones_like(x)
+    plain, back = memory.elu_restore(ones, kept)
+    dx, same = memory.elu_restore(ones, kept, bounded=True)
+    assert bool((back < -1).any()) and torch.equal(back, same)
+    assert float(dx.min()) >= 0.0 and float(dx.max()) <= 1.0
+    assert torch.equal(dx, plain.clamp_min(0))
+    exact = torch.where(x > 0, 1.0, x.double().exp())
+    step = kept.scales.double().repeat_interleave(128, 1)[:, :300]
+    # Half a step, and a step where the kept value of a small positive one is zero or the other way round.
+    assert bool(((dx - exact).abs() <= 0.501 * step).all())
+    # What is not finite stays visible.
+    y, kept = memory.elu_checkpoint(torch.full((1, 4), float("nan")))
+    assert bool(memory.elu_restore(torch.ones(1, 4), kept, bounded=True)[0].isnan().all())
+
+
+def test_checkpointed_mlp_sends_nothing_back_through_saturated_units_that_are_kept_below():
+    g = gen(5)
+    bias = torch.full((64,), -20.0)
+    bias[0] = 12.0
+    first, second = 0.1 * torch.randn(64, 6, generator=g), torch.randn(3, 64, generator=g)
+    leaves = [t.requires_grad_() for t in (torch.randn(40, 6, generator=g), first, second, bias, torch.zeros(3))]
+    dz = torch.randn(40, 3, generator=g)
+    grads = torch.autograd.grad(memory.checkpointed_mlp(leaves[0], leaves[1:3], leaves[3:]), leaves, dz)
+    x, w, v, b, _ = (t.detach().double() for t in leaves)
+    _, kept = memory.elu_checkpoint(torch.addmm(leaves[3], leaves[0], first.t()))
+    stood = kept.codes.double() * kept.scales.double()
+    assert bool((stood < -1).any())
+    slope = torch.where(stood > 0, 1.0, (stood + 1).clamp_min(0))
+    dy = (dz.double() @ v) * slope
+    # float32 sums of 40 and of 64 terms.
+    for got, want in zip((grads[0], grads[1], grads[3]), (dy @ w, dy.t() @ x, dy.sum(0))):
+        assert float((got.double() - want).norm() / want.norm()) <= 4 * (64 ** 0.5 + 8) * 2.0 ** -24
