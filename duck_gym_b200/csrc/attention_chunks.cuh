@@ -934,7 +934,7 @@ __global__ void __launch_bounds__(scanThreads(DI))
   for (int64_t eh = first; eh < end; ++eh) {
     any = false;
     for (int x = threadIdx.x; x < count; x += blockDim.x) any |= flags[eh * count + x] != 0;
-    if (__syncthreads_or(any)) scanSteps<bf16, DI, true>(s, eh, blockIdx.y, 0);
+    if (__syncthreads_or(any)) scanSteps<bf16, DI, true, true>(s, eh, blockIdx.y, 0);
   }
 }
 

@@ -16,6 +16,8 @@
 #pragma once
 #include "numeric_types.cuh"
 
+#include <type_traits>
+
 namespace duckb200 {
 
 constexpr int kHeadMax = 128;   // largest Dk and Dv
@@ -80,14 +82,23 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
+// The first `count` of a pair, zeros in the place of the others.
+__device__ __forceinline__ Pair firstOf(Pair p, int count) {
+  const float2 v = parts(p);
+  return pairOf(count > 0 ? v.x : 0.f, count > 1 ? v.y : 0.f);
+}
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
   Pair d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 
-// OUT = false: what a segment adds to the state, in the place of the next one's start.
-template <class T, int DI, bool OUT>
+// OUT = false: what a segment adds to the state, in the segment's own slot of the
+// starts, which joinSweeps() turns into its start.
+// PADDED: some sweep of the call has fewer than DI rows.  The rows beyond are zero,
+// but beside a b that is not finite they would become NaN and reach the outputs, so
+// that tiles with such a b go step by step and clear them.
+template <class T, int DI, bool OUT, bool PADDED>
 __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile, int segment) {
   constexpr int LANES = scanLanes(DI), R = DI / LANES, THREADS = scanThreads(DI);
   constexpr int AC = kScanSteps * DI / THREADS, B = kScanSteps * kScanColumns / THREADS;   // values a thread fetches
@@ -168,14 +179,22 @@ __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile, 
     }
 #pragma unroll
     for (int n = 0; n < B; ++n) (&b[0][0])[n * THREADS + threadIdx.x] = nextB[n];
+    bool special = nextCut;
+    if (PADDED) {
+      float zero = 0.f;
+#pragma unroll
+      for (int n = 0; n < B; ++n) zero = fmaf(nextB[n], 0.f, zero);
+      special |= zero != 0.f;
+    }
     if (threadIdx.x < kScanSteps) {
       cut[threadIdx.x] = nextCut;
       factor[threadIdx.x] = s.reverse && t0 + int(threadIdx.x) == 0 ? 1.f : decay;
     }
-    const bool anyCut = __syncthreads_or(nextCut);
-    cutInside |= anyCut;
+    special = __syncthreads_or(special);
+    if (!OUT) cutInside |= special;
     if (t0 + kScanSteps < end) fetch(t0 + kScanSteps);
-    auto step = [&](int u) {
+    auto step = [&](int u, auto clear_) {
+      constexpr bool CLEAR = decltype(clear_)::value;
       const float2 value = *reinterpret_cast<const float2 *>(&b[u][column]);
       const Pair f2 = pairOf(factor[u], factor[u]), v2[2] = {pairOf(value.x, value.x), pairOf(value.y, value.y)};
       Pair sum[2] = {0, 0};
@@ -187,7 +206,24 @@ __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile, 
         for (int k = 0; k < 2; ++k) {
           x[k][r] = fma2(f2, x[k][r], mul2(pairsA.x, v2[k]));
           x[k][r + 1] = fma2(f2, x[k][r + 1], mul2(pairsA.y, v2[k]));
-          if (OUT) {
+          if (OUT && !CLEAR) {
+            sum[k] = fma2(pairsC.x, x[k][r], sum[k]);
+            sum[k] = fma2(pairsC.y, x[k][r + 1], sum[k]);
+          }
+        }
+      }
+      if (CLEAR) {
+        if (!(fmaf(value.x, 0.f, value.y * 0.f) == 0.f)) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int r = 0; r < R / 2; ++r) x[k][r] = firstOf(x[k][r], s.Di - rowOf(2 * r));
+        }
+#pragma unroll
+        for (int r = 0; r < R / 2; r += 2) {
+          const ulonglong2 pairsC = *reinterpret_cast<const ulonglong2 *>(&c[u][rowOf(2 * r)]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
             sum[k] = fma2(pairsC.x, x[k][r], sum[k]);
             sum[k] = fma2(pairsC.y, x[k][r + 1], sum[k]);
           }
@@ -203,9 +239,9 @@ __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile, 
       }
       if (lane == 0) *reinterpret_cast<float2 *>(&y[u][column]) = total;
     };
-    if (!anyCut && count == kScanSteps) {   // nothing in the way of overlapping one step with the next
+    if (!special && count == kScanSteps) {   // nothing in the way of overlapping one step with the next
 #pragma unroll 4
-      for (int u = 0; u < kScanSteps; ++u) step(u);
+      for (int u = 0; u < kScanSteps; ++u) step(u, std::false_type());
     } else {
       for (int u = 0; u < count; ++u) {
         if (cut[u]) {
@@ -214,7 +250,7 @@ __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile, 
 #pragma unroll
             for (int r = 0; r < R / 2; ++r) x[k][r] = 0;
         }
-        step(u);
+        step(u, std::bool_constant<PADDED>());
       }
     }
     __syncthreads();
@@ -248,9 +284,9 @@ __device__ __forceinline__ void scanSteps(const Sweep &s, int64_t eh, int tile, 
 struct Sweeps {
   Sweep s[3];
 };
-template <class T, int DI, bool OUT>
+template <class T, int DI, bool OUT, bool PADDED>
 __global__ void __launch_bounds__(scanThreads(DI)) attentionScan(const __grid_constant__ Sweeps p, int tiles) {
-  scanSteps<T, DI, OUT>(p.s[blockIdx.z], blockIdx.x, blockIdx.y % tiles, blockIdx.y / tiles);
+  scanSteps<T, DI, OUT, PADDED>(p.s[blockIdx.z], blockIdx.x, blockIdx.y % tiles, blockIdx.y / tiles);
 }
 // The states that the segments of a sweep begin with, from what each adds, in place.
 __global__ void __launch_bounds__(256) joinSweeps(const __grid_constant__ Sweeps p) {

@@ -132,14 +132,21 @@ int mostColumns(const Sweeps &p, int count) {
   for (int i = 0; i < count; ++i) n = std::max(n, p.s[i].Dj);
   return n;
 }
-template <bool OUT> void launchScan(const Sweeps &p, int count, int segments, cudaStream_t stream) {
-  const int rows = mostRows(p, count), tiles = int(ceilDiv(mostColumns(p, count), kScanColumns));
+template <int DI, bool OUT> void launchScan(const Sweeps &p, int count, int segments, cudaStream_t stream) {
+  const int tiles = int(ceilDiv(mostColumns(p, count), kScanColumns));
   const dim3 grid{unsigned(int64_t(p.s[0].E) * p.s[0].H), unsigned(tiles * segments), unsigned(count)};
-  if (rows <= 16) attentionScan<float, 16, OUT><<<grid, scanThreads(16), 0, stream>>>(p, tiles);
-  else if (rows <= 32) attentionScan<float, 32, OUT><<<grid, scanThreads(32), 0, stream>>>(p, tiles);
-  else if (rows <= 64) attentionScan<float, 64, OUT><<<grid, scanThreads(64), 0, stream>>>(p, tiles);
-  else attentionScan<float, 128, OUT><<<grid, scanThreads(128), 0, stream>>>(p, tiles);
+  bool padded = false;
+  for (int i = 0; i < count; ++i) padded |= p.s[i].Di < DI;
+  if (OUT && padded) attentionScan<float, DI, OUT, OUT><<<grid, scanThreads(DI), 0, stream>>>(p, tiles);
+  else attentionScan<float, DI, OUT, false><<<grid, scanThreads(DI), 0, stream>>>(p, tiles);
   check(cudaGetLastError(), "linear attention launch");
+}
+template <bool OUT> void launchScan(const Sweeps &p, int count, int segments, cudaStream_t stream) {
+  const int rows = mostRows(p, count);
+  if (rows <= 16) launchScan<16, OUT>(p, count, segments, stream);
+  else if (rows <= 32) launchScan<32, OUT>(p, count, segments, stream);
+  else if (rows <= 64) launchScan<64, OUT>(p, count, segments, stream);
+  else launchScan<128, OUT>(p, count, segments, stream);
 }
 
 // How a call's steps are split where it has fewer blocks than four a multiprocessor: segments of 64 steps at least.

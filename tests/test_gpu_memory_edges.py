@@ -109,3 +109,29 @@ def test_the_bounded_derivative_is_that_of_an_elu(n, dtype):
     assert bool(dx[:2, :min(n, 128)].isnan().all())   # what is not finite stays visible
     only, nothing = memory.elu_restore(dy, kept, restore=False, bounded=True)
     assert nothing is None and torch.equal(only[2:], dx[2:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Dk,Dv", [(1, 1), (20, 28), (32, 32), (40, 9), (100, 128), (128, 66)])
+def test_infinity_beside_head_sizes_that_are_padded(Dk, Dv, dtype):
+    """Of operands without a negative number an infinity makes infinities, and no NaN."""
+    T, E, H = 45, 2, 2
+    g = gen(Dk * 131 + Dv)
+    q, k, v, do = (normal(g, T, E, H, D, dtype=dtype).abs() + 0.1 for D in (Dk, Dk, Dv, Dv))
+    S, decay = normal(g, E, H, Dk, Dv).abs(), torch.tensor([0.5, 0.9])
+    r = torch.zeros(T, E, dtype=torch.bool)
+    r[30] = True
+    v[7, 0, 0, Dv // 2] = do[20, 1, 0, 0] = float("inf")
+    q[21, 0, 1, Dk - 1] = k[40, 1, 1, 0] = float("inf")
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v, S)]
+    o, last = memory.linear_attention(*leaves[:3], decay.cuda(), leaves[3], r.cuda())
+    dlast = torch.ones_like(last)
+    grads = torch.autograd.grad([o, last], leaves, [do.cuda(), dlast])
+    want = ref.attention(q, k, v, decay, S, r, Dk ** -0.5, do, dlast.cpu())
+    for i, (got, exact) in enumerate(zip((o, last, *grads), want)):
+        got = got.cpu().double()
+        assert not bool(exact.isnan().any()) and bool(exact.isinf().any())
+        assert torch.equal(got.isinf(), exact.isinf()) and not bool(got.isnan().any()), i
+        fine = exact.isfinite()
+        terms = (T + 8) * (Dk + Dv)
+        assert ref.error(got[fine], exact[fine]) <= (ref.bound(dtype, terms, 4) if i not in (1, 5) else 1e-5)
