@@ -39,7 +39,6 @@ struct CheckpointArgs {
   float *scales;        // [rows, groups]
   int64_t rows;
   int n, groups;
-  float lowest;         // backward: kept values below it count as it in the derivative
 };
 
 struct GroupScale {
@@ -65,8 +64,8 @@ __device__ __forceinline__ float eluRounded(float x) {
 }
 
 // ELU's derivative from its kept output; NaN stays.
-__device__ __forceinline__ float eluSlope(float y, float lowest) {
-  return y > 0.f ? 1.f : (y < lowest ? lowest : y) + 1.f;
+template <bool BOUNDED> __device__ __forceinline__ float eluSlope(float y) {
+  return y > 0.f ? 1.f : BOUNDED && y < -1.f ? 0.f : y + 1.f;
 }
 
 template <class T> __device__ __forceinline__ float eluFor(float x);
@@ -139,7 +138,8 @@ template <class T> __global__ void __launch_bounds__(kCheckpointThreads, 4) eluC
   }
 }
 
-template <class T> __global__ void __launch_bounds__(kCheckpointThreads, 4) eluRestoreAny(CheckpointArgs p) {
+template <class T, bool BOUNDED>
+__global__ void __launch_bounds__(kCheckpointThreads, 4) eluRestoreAny(CheckpointArgs p) {
   constexpr int U = kGroupsAtOnce, V = kGroup / 32;
   const int lane = threadIdx.x & 31;
   const int64_t warps = int64_t(gridDim.x) * (kCheckpointThreads / 32);
@@ -171,7 +171,7 @@ template <class T> __global__ void __launch_bounds__(kCheckpointThreads, 4) eluR
         if (lane + 32 * i >= left[u]) continue;
         const float y = float(code[u][i]) * scale[u];
         if (p.y) static_cast<T *>(p.y)[at[u] + lane + 32 * i] = fromFloat<T>(y);
-        static_cast<T *>(p.dx)[at[u] + lane + 32 * i] = fromFloat<T>(dy[u][i] * eluSlope(y, p.lowest));
+        static_cast<T *>(p.dx)[at[u] + lane + 32 * i] = fromFloat<T>(dy[u][i] * eluSlope<BOUNDED>(y));
       }
   }
 }
@@ -278,7 +278,8 @@ template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluChec
   }
 }
 
-template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluRestorePieces(CheckpointArgs p) {
+template <class T, bool BOUNDED>
+__global__ void __launch_bounds__(kCheckpointThreads) eluRestorePieces(CheckpointArgs p) {
   constexpr int V = Piece<T>::values, LANES = Piece<T>::lanes;
   const int lane = threadIdx.x % LANES;
   const int64_t teams = int64_t(gridDim.x) * (kCheckpointThreads / LANES);
@@ -319,7 +320,7 @@ template <class T> __global__ void __launch_bounds__(kCheckpointThreads) eluRest
       const uint32_t biased = codes[i / 4] ^ 0x80808080u;
       const float code = __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7440 + i % 4)) - 8388736.f;
       y[i] = code * scale;
-      dy[i] *= eluSlope(y[i], p.lowest);
+      dy[i] *= eluSlope<BOUNDED>(y[i]);
     }
     const int64_t at = now.row * p.n + c;
     *reinterpret_cast<uint4 *>(static_cast<T *>(p.dx) + at) = Piece<T>::round(dy);

@@ -9,7 +9,6 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
-#include <limits>
 #include <type_traits>
 
 using namespace duckb200;
@@ -79,30 +78,31 @@ int64_t normSplits(int64_t rows, int n) {
 
 // Codes are moved 8 or 4 at a time beside pieces of 16 bytes of values; their array
 // has to be aligned for that.
-void launchGroups(const CheckpointArgs &a, int type, bool pieces, duck_stream stream, bool restore) {
+enum class Groups { keep, restore, restoreBounded };
+void launchGroups(const CheckpointArgs &a, int type, bool pieces, duck_stream stream, Groups what) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   pieces = pieces && reinterpret_cast<uintptr_t>(a.codes) % 8 == 0;
   withType(type, [&](auto zero) {
     using T = decltype(zero);
     const int groups = pieces ? kCheckpointThreads / Piece<T>::lanes : kCheckpointThreads / 32 * kGroupsAtOnce;
     const unsigned blocks = unsigned(std::min<int64_t>(ceilDiv(a.rows * a.groups, groups), 148 * 8));
-    if (pieces && restore) eluRestorePieces<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
-    else if (pieces) eluCheckpointPieces<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
-    else if (restore) eluRestoreAny<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
-    else eluCheckpointAny<T><<<blocks, kCheckpointThreads, 0, s>>>(a);
+    auto kernel = what == Groups::keep      ? (pieces ? eluCheckpointPieces<T> : eluCheckpointAny<T>)
+                  : what == Groups::restore ? (pieces ? eluRestorePieces<T, false> : eluRestoreAny<T, false>)
+                                            : (pieces ? eluRestorePieces<T, true> : eluRestoreAny<T, true>);
+    kernel<<<blocks, kCheckpointThreads, 0, s>>>(a);
   });
 }
 
 int restoreElu(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows, int n, int type,
-               float lowest, duck_stream stream) {
+               Groups what, duck_stream stream) {
   return guarded([&] {
     requireType(type);
     require(rows >= 0 && n > 0, "Invalid checkpoint sizes");
     if (rows == 0) return;
     require(dy && codes && scales && dx, "Invalid arguments");
     CheckpointArgs a{dy, y, dx, const_cast<int8_t *>(codes), const_cast<float *>(scales), rows, n,
-                     int(ceilDiv(n, kGroup)), lowest};
-    launchGroups(a, type, pieces16({dy, y, dx}, {int64_t(n)}, type), stream, true);
+                     int(ceilDiv(n, kGroup))};
+    launchGroups(a, type, pieces16({dy, y, dx}, {int64_t(n)}, type), stream, what);
     check(cudaGetLastError(), "checkpoint launch");
   });
 }
@@ -491,20 +491,20 @@ int duck_elu_checkpoint(const void *x, void *y, int8_t *codes, float *scales, in
     require(rows >= 0 && n > 0, "Invalid checkpoint sizes");
     if (rows == 0) return;
     require(x && y && codes && scales, "Invalid arguments");
-    CheckpointArgs a{x, y, nullptr, codes, scales, rows, n, int(ceilDiv(n, kGroup)), 0.f};
-    launchGroups(a, type, pieces16({x, y}, {int64_t(n)}, type), stream, false);
+    CheckpointArgs a{x, y, nullptr, codes, scales, rows, n, int(ceilDiv(n, kGroup))};
+    launchGroups(a, type, pieces16({x, y}, {int64_t(n)}, type), stream, Groups::keep);
     check(cudaGetLastError(), "checkpoint launch");
   });
 }
 
 int duck_elu_restore(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows, int n,
                      int type, duck_stream stream) {
-  return restoreElu(dy, codes, scales, y, dx, rows, n, type, -std::numeric_limits<float>::infinity(), stream);
+  return restoreElu(dy, codes, scales, y, dx, rows, n, type, Groups::restore, stream);
 }
 
 int duck_elu_restore_bounded(const void *dy, const int8_t *codes, const float *scales, void *y, void *dx, int64_t rows,
                              int n, int type, duck_stream stream) {
-  return restoreElu(dy, codes, scales, y, dx, rows, n, type, -1.f, stream);
+  return restoreElu(dy, codes, scales, y, dx, rows, n, type, Groups::restoreBounded, stream);
 }
 
 int duck_linear_attention_sizes(const duck_attention *args, int64_t *out) {
