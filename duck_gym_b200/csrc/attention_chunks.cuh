@@ -18,11 +18,11 @@
 // Roundings to bfloat16, each of 8 significant bits: the decayed scores, and the
 // copy of S.  The state's own operand l^(L-1-j) k_j is not rounded to 8 bits: it is
 // split into the sum of two bfloat16 numbers (16 bits), a product each, so that an
-// output has two roundings on its way besides its own at most; and of three (24
-// bits) where the state is an output and still remembers the chunk: what has faded
-// to 1/64 by the last step does not need the third there.  (Measured against 64
-// bits: outputs and gradients 2.3e-3 in the 2-norm, where one rounding is 1.7e-3;
-// states 2e-7 to 7e-7.)
+// output has one rounding on its way besides its own; and of three (24 bits) where
+// the state is an output, in every chunk: the steps after a chunk may add nothing, so
+// that what has faded is all there is.  (Measured against 64 bits: outputs and
+// gradients 2.3e-3 in the 2-norm, where one rounding is 1.7e-3; states 1.5e-7 to
+// 1.0e-6, the more the longer they remember.)
 //
 // Episodes: step i sees step j only if no reset lies in (j, i]; S only if none
 // lies at or before i.  Scores and states that are masked are replaced, not
@@ -73,7 +73,13 @@ struct ChunkArgs {
   float scale;
 };
 
-constexpr float kFaded = 1.f / 64.f;
+// A power of a decay to a few units in the last place, however far it has faded (2 to
+// the n times a float32 logarithm would be off by 2^-24 of the exponent: 2e-6 of what
+// 500 steps at 0.9 leave).  Of a negative or NaN decay: NaN, which leaves a block to
+// redoAttention().
+__device__ __forceinline__ float powerOf(float decay, int n) {
+  return decay >= 0.f ? powf(decay, float(n)) : __int_as_float(0x7fc00000);
+}
 
 // Where episodes begin in steps t0 .. t0 + 63 before `end`: a lane looks at two of
 // them; read a chunk ahead.
@@ -319,7 +325,7 @@ template <int C, int DK, int DV, bool OUT> constexpr int chunkTileElements() {
   return C * (DK + 8) * (OUT ? 2 : 1) + C * (DV + 8);
 }
 template <int C, int DK, int DV, bool OUT> constexpr int chunkSharedBytes(int buffers) {
-  return buffers * (chunkTileElements<C, DK, DV, OUT>() + (OUT ? DK * (DV + 8) : 0)) * 2 + 4 * (2 * C + 20);
+  return buffers * (chunkTileElements<C, DK, DV, OUT>() + (OUT ? DK * (DV + 8) : 0)) * 2 + 4 * (3 * C + 21);
 }
 
 // One block per (environment, head), segment of T and tile of DV columns; C / 16
@@ -340,6 +346,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
   bf16 *copies = tiles + buffers * chunkTileElements<C, DK, DV, OUT>();      // the state in bfloat16
   float *toEnd = reinterpret_cast<float *>(copies + (OUT ? buffers * DK * LV : 0));   // l^(L - 1 - j)
   float *powers = toEnd + C;                                                  // scale l^(x - 16), 0 for x < 16
+  float *decays = powers + C + 20;                                            // l^x, x up to C
 
   const int64_t eh = blockIdx.x;
   const int e = int(eh / p.H), h = int(eh - int64_t(e) * p.H);
@@ -378,13 +385,15 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
 
   // Powers of the decay.
   const float decay = p.decay[h];
-  const float logDecay = fmaxf(log2f(decay), -1e30f);   // finite: no 0 times infinity for a decay of zero
-  // (Of a negative or NaN decay: NaN, which leaves the block to redoAttention().)
-  auto power = [&](int n) { return decay >= 0.f ? exp2f(float(n) * logDecay) : __int_as_float(0x7fc00000); };
-  for (int x = threadIdx.x; x < C; x += THREADS) toEnd[x] = power(C - 1 - x);
-  for (int x = threadIdx.x; x < C + 20; x += THREADS) powers[x] = x < 16 ? 0.f : p.scale * power(x - 16);
+  for (int x = threadIdx.x; x < C + 20; x += THREADS) {
+    const int n = x - 16;
+    const float f = powerOf(decay, n < 0 ? 0 : n);
+    powers[x] = n < 0 ? 0.f : p.scale * f;
+    if (n >= 0 && n <= C) decays[n] = f;
+    if (n >= 0 && n < C) toEnd[C - 1 - n] = f;
+  }
   const int i0 = 16 * warp;   // the warp's steps
-  const float fullChunk = power(C);
+  const bool precise = p.precise && (!OUT || last);   // what this block adds reaches the last state
 
   uint32_t finite = 0;
   bool anyReset = false, later = init != nullptr;   // later: S is not zero
@@ -405,7 +414,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
     }
     const bf16 *K = tiles + buffer * chunkTileElements<C, DK, DV, OUT>(), *V = K + C * LQ, *Q = V + C * LV;
     if (STATE && count < C)
-      for (int x = threadIdx.x; x < C; x += THREADS) toEnd[x] = x < count ? power(count - 1 - x) : 0.f;
+      for (int x = threadIdx.x; x < C; x += THREADS) toEnd[x] = x < count ? decays[count - 1 - x] : 0.f;
 
     const bool advance = STATE && (c + 1 < chunks || last);
     const bf16 *copy = copies + buffer * DK * LV;
@@ -506,8 +515,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
     // The state at the chunk's end.
     if (advance) {
       if (count < C) __syncthreads();   // toEnd
-      const float f = count == C ? fullChunk : power(count);
-      const bool precise = p.precise && power(p.T - first - count) > kFaded;
+      const float f = decays[count];
 #pragma unroll
       for (int m = 0; m < SM; ++m)
 #pragma unroll
@@ -602,7 +610,7 @@ struct BackwardArgs {
 template <int C, int D, bool OUT> constexpr int backwardWarps() { return OUT && D == 128 ? C / 8 : C / 16; }
 // Where `later` states' gradients never exist, no room for X.
 template <int C, int D, bool OUT> constexpr int backwardSharedBytes(bool later) {
-  return (OUT ? 4 * C + (later ? 2 : 1) * D : 2 * C) * (D + 8) * 2 + (16 + C + 4) * 4;
+  return (OUT ? 4 * C + (later ? 2 : 1) * D : 2 * C) * (D + 8) * 2 + (2 * C + 24) * 4;
 }
 
 // One block per (environment, head) and segment of T, chunks from the last to the
@@ -629,7 +637,8 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
   constexpr int RT = D / 16, SM = RT >= W ? RT / W : 1, SPLIT = RT >= W ? 1 : W / RT, SN = D / 8 / SPLIT;
   extern __shared__ __align__(16) unsigned char shared[];
   float *powers = reinterpret_cast<float *>(shared);   // scale l^(x - 16), 0 for x < 16; C + 20 of them
-  bf16 *Q = reinterpret_cast<bf16 *>(powers + C + 20), *O = Q + C * LD, *K = O + C * LD, *V = K + C * LD, *S = V + C * LD,
+  float *decays = powers + C + 20;                     // l^x, x up to C; C + 4 of them, for the tiles' alignment
+  bf16 *Q = reinterpret_cast<bf16 *>(decays + C + 4), *O = Q + C * LD, *K = O + C * LD, *V = K + C * LD, *S = V + C * LD,
        *X = S + D * LD;
   const int64_t eh = blockIdx.x;
   const int e = int(eh / p.H), h = int(eh - int64_t(e) * p.H), seg = OUT ? blockIdx.y : blockIdx.y + 1;
@@ -646,9 +655,13 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
                 : p.dstateIn && seg == 0 ? p.dstateIn + eh * stateSize : nullptr;
 
   const float decay = p.decay[h];
-  const float logDecay = fmaxf(log2f(decay), -1e30f);
-  auto power = [&](int n) { return decay >= 0.f ? exp2f(float(n) * logDecay) : __int_as_float(0x7fc00000); };
-  for (int x = threadIdx.x; x < C + 20; x += THREADS) powers[x] = x < 16 ? 0.f : p.scale * power(x - 16);
+  for (int x = threadIdx.x; x < C + 20; x += THREADS) {
+    const int n = x - 16;
+    const float f = powerOf(decay, n < 0 ? 0 : n);
+    powers[x] = n < 0 ? 0.f : p.scale * f;
+    if (n >= 0) decays[n] = f;
+  }
+  const bool precise = p.precise && (!OUT || last);   // what this block adds reaches the first state's gradient
   const int sm0 = RT >= W ? warp * SM : warp / SPLIT, sn0 = RT >= W ? 0 : (warp % SPLIT) * SN;
   float dS[SM][SN][4];
   if (STATE) readSlice(dS, init, sm0, sn0, 0, p.Dk, p.Dv);
@@ -775,8 +788,8 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
         storeTile(p.dq + eh * p.Dk, out, stepK, first, count, row, col, p.Dk, finite);
         // dv, dk
         const int left0 = count - 1 - row - g, left1 = left0 - 8;
-        const float f0 = row + g >= endStart && left0 >= 0 ? power(left0) : 0.f;
-        const float f1 = row + g + 8 >= endStart && left1 >= 0 ? power(left1) : 0.f;
+        const float f0 = row + g >= endStart && left0 >= 0 ? decays[left0] : 0.f;
+        const float f1 = row + g + 8 >= endStart && left1 >= 0 ? decays[left1] : 0.f;
         rowsOfA(K);
         if (later) {
 #pragma unroll
@@ -820,8 +833,7 @@ __global__ void __launch_bounds__(backwardWarps<C, D, OUT>() * 32, (D == 128 ? 6
 
     if (STATE && (c > 0 || last)) {
       const int firstReset = episodeEnd(mask, 0);   // of the steps after 0
-      const float f = power(count);
-      const bool precise = p.precise && power(first) > kFaded;
+      const float f = decays[count];
 #pragma unroll
       for (int m = 0; m < SM; ++m)
 #pragma unroll
@@ -895,7 +907,7 @@ __global__ void __launch_bounds__(256) joinSegments(float *segments, const uint8
                                                     int segmentLength, int64_t stateSize, int reverse) {
   const int64_t eh = blockIdx.x, x = int64_t(blockIdx.y) * blockDim.x + threadIdx.x;
   if (x >= stateSize) return;
-  const float d = decay[eh % H], logDecay = fmaxf(log2f(d), -1e30f);
+  const float d = decay[eh % H], whole = powerOf(d, segmentLength);
   float S = init ? init[eh * stateSize + x] : 0.f;
   float *states = segments + eh * segmentCount * stateSize + x;
   constexpr int AHEAD = 8;   // loads in flight: the chain itself is a multiplication a segment
@@ -913,7 +925,7 @@ __global__ void __launch_bounds__(256) joinSegments(float *segments, const uint8
       states[s * stateSize] = S;
       if (u + 1 == segmentCount) break;
       const int length = min(segmentLength, T - s * segmentLength);
-      const float f = d >= 0.f ? exp2f(float(length) * logDecay) : __int_as_float(0x7fc00000);
+      const float f = length == segmentLength ? whole : powerOf(d, length);
       S = cut[eh * segmentCount + s] ? added[k] : fmaf(f, S, added[k]);
     }
   }

@@ -135,3 +135,29 @@ def test_infinity_beside_head_sizes_that_are_padded(Dk, Dv, dtype):
         fine = exact.isfinite()
         terms = (T + 8) * (Dk + Dv)
         assert ref.error(got[fine], exact[fine]) <= (ref.bound(dtype, terms, 4) if i not in (1, 5) else 1e-5)
+
+
+# A state from bfloat16 operands: each operand with its decay is the sum of three bfloat16 numbers (2^-24 of it is
+# left), sums are float32 (2^-24 of the state for each product that it still remembers, at random: some 60 of 16 steps
+# at 1000 steps), and a power of the decay is as exact as the logarithm in its exponent (2^-24 ln(1 / fading)).  All
+# of it stays below 1.5e-6; two numbers an operand leave 2^-17 of it in the mean, 2.1e-6 to 2.4e-6 in the state.
+WHOLE_STATE = 1.5e-6
+
+
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("T,quiet", [(104, 40), (192, 128), (1000, 300), (2000, 500), (24, 0), (1000, 0)])
+@pytest.mark.parametrize("decay", [0.9, 0.97, 0.99])
+def test_states_are_whole_where_later_steps_add_nothing(D, T, quiet, decay):
+    """The last steps of the rollout for its last state, the first ones for the gradient of its first state."""
+    g = gen(T + quiet + D)
+    E = 1 if T > 1000 else 2   # the long ones are split over the steps
+    q, k, v, do = (normal(g, T, E, 1, D, dtype=torch.bfloat16) for _ in range(4))
+    k[T - quiet:], q[:quiet] = 0.0, 0.0
+    decay = torch.tensor([decay])
+    leaves = [t.cuda() for t in (q, k, v)]
+    S = torch.zeros(E, 1, D, D, device="cuda", requires_grad=True)
+    o, last = memory.linear_attention(*leaves, decay.cuda(), S)
+    dS, = torch.autograd.grad(o, S, do.cuda())
+    want = ref.attention(q, k, v, decay, torch.zeros(E, 1, D, D), None, D ** -0.5, do)
+    assert ref.error(last, want[1]) <= WHOLE_STATE
+    assert ref.error(dS, want[5]) <= WHOLE_STATE
