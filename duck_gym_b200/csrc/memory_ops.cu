@@ -107,12 +107,15 @@ int restoreElu(const void *dy, const int8_t *codes, const float *scales, void *y
   });
 }
 
+constexpr int kStepsMax = INT32_MAX - (1 << 24);
 bool attentionChecked(const duck_attention *a) {
   require(a != nullptr, "Invalid arguments");
   requireType(a->type);
   require(a->T >= 0 && a->E >= 0 && a->H >= 0, "Invalid attention sizes");
   require(a->Dk > 0 && a->Dk <= kHeadMax && a->Dv > 0 && a->Dv <= kHeadMax, "Head sizes have to be 1 to 128");
   require(int64_t(a->E) * a->H < (int64_t(1) << 31), "Too many environments and heads");
+  // Steps are counted in 32 bits, up to a chunk for each of some hundred segments past the last one.
+  require(a->T <= kStepsMax, "Too many steps");
   return a->E > 0 && a->H > 0;
 }
 Rows rowsOf(const int64_t *s) { return {s[0], s[1], s[2]}; }

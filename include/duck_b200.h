@@ -393,7 +393,7 @@ int duck_elu_restore_bounded(const void *dy, const int8_t *codes, const float *s
  *   S_t = f_t S_{t-1} + k_t v_t^T,  o_t = scale S_t^T q_t,
  *   f_t = decay[h], or 0 where resets[t, e] is set (an episode begins at t).
  * q and k are [T, E, H, Dk], v, out and dout [T, E, H, Dv] with 1 <= Dk, Dv <=
- * 128; q, k, v and dout have the strides given, {t, e, h}; the outputs are
+ * 128 and T <= 2^31 - 2^24 - 1; q, k, v and dout have the strides given, {t, e, h}; the outputs are
  * dense.  States are dense [E, H, Dk, Dv] float32.  decay [H] is in [0, 1].
  * Outputs, workspaces and the states of whole rollouts lie on 16-byte
  * boundaries, and no output overlaps an input (state_out is another array than

@@ -108,3 +108,12 @@ def test_checkpointed_mlp_sends_nothing_back_through_saturated_units_that_are_ke
     # float32 sums of 40 and of 64 terms.
     for got, want in zip((grads[0], grads[1], grads[3]), (dy @ w, dy.t() @ x, dy.sum(0))):
         assert float((got.double() - want).norm() / want.norm()) <= 4 * (64 ** 0.5 + 8) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+def test_more_steps_than_are_counted_in_32_bits_are_refused(kind):
+    """Their segments end past 2^31, where the count of steps would turn negative."""
+    for T in (2 ** 31 - 1, 2 ** 31 - 2 ** 24):
+        with pytest.raises(RuntimeError, match="steps"):
+            memory._workspace(T, 1, 1, 1, 1, kind)
+    assert memory._workspace(2 ** 31 - 2 ** 24 - 1, 1, 1, 1, 1, kind)[0] > 0
