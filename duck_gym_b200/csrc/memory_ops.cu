@@ -35,6 +35,11 @@ bool pieces16(std::initializer_list<const void *> pointers, std::initializer_lis
   return true;
 }
 
+// Mean and rstd are moved together.
+void requireStats(const float *stats) {
+  require(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "Statistics have to be 8-byte aligned");
+}
+
 // Layer norm kernels that hold a row in registers: 16-byte pieces where rows are
 // made of them, else single values; up to 8192 values.  Calls f with a kernel's
 // lanes, values a load and values a lane.
@@ -418,6 +423,7 @@ int duck_layer_norm_forward(const void *x, const float *weight, const float *bia
     require(eps >= 0 && std::isfinite(eps), "Invalid layer norm eps");
     if (rows == 0) return;
     require(x && y, "Invalid arguments");
+    requireStats(stats);
     NormArgs a{};
     a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.stats = stats;
     a.rows = rows; a.n = n; a.xStride = x_stride; a.eps = float(eps);
@@ -455,6 +461,7 @@ int duck_layer_norm_backward(const void *x, const void *dy, const float *weight,
     if (!columns && !dx) return;
     require(!columns || scratch, "Invalid arguments");
     require(rows == 0 || (x && dy && stats), "Invalid arguments");
+    requireStats(stats);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     NormArgs a{};
     a.x = x; a.dy = dy; a.weight = weight; a.dx = dx; a.stats = const_cast<float *>(stats); a.partials = scratch;

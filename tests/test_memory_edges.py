@@ -117,3 +117,15 @@ def test_more_steps_than_are_counted_in_32_bits_are_refused(kind):
         with pytest.raises(RuntimeError, match="steps"):
             memory._workspace(T, 1, 1, 1, 1, kind)
     assert memory._workspace(2 ** 31 - 2 ** 24 - 1, 1, 1, 1, 1, kind)[0] > 0
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="calls with host addresses, which only a refusal keeps from a GPU")
+def test_statistics_at_an_odd_place_are_refused():
+    from duck_gym_b200.cuda_batch import library
+
+    lib = library()
+    p = torch.zeros(64).data_ptr()
+    assert lib.duck_layer_norm_forward(p, None, None, p, p + 4, 4, 8, 8, 1e-5, 0, None) == 1   # DUCK_EINVAL
+    assert b"aligned" in lib.duck_last_error()
+    assert lib.duck_layer_norm_backward(p, p, None, p + 4, p, None, None, None, 4, 8, 8, 8, 0, None) == 1
+    assert b"aligned" in lib.duck_last_error()
