@@ -7,6 +7,7 @@
 #include "linear_attention.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
 #include <type_traits>
@@ -268,9 +269,10 @@ bool dense16(const void *base, const int64_t *strides, int width) {
          strides[2] % 8 == 0 && width % 8 == 0;
 }
 
-// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device.
+// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device
+// (by whichever thread comes first: autograd calls from its own).
 template <auto kernel> void allowShared(int bytes) {
-  static bool done[64] = {};
+  static std::atomic<bool> done[64] = {};
   int device = 0;
   check(cudaGetDevice(&device), "cudaGetDevice");
   if (device < 64 && done[device]) return;
