@@ -161,3 +161,22 @@ def test_states_are_whole_where_later_steps_add_nothing(D, T, quiet, decay):
     want = ref.attention(q, k, v, decay, torch.zeros(E, 1, D, D), None, D ** -0.5, do)
     assert ref.error(last, want[1]) <= WHOLE_STATE
     assert ref.error(dS, want[5]) <= WHOLE_STATE
+
+
+@pytest.mark.parametrize("T,D,decay", [(48, 64, 0.97), (1000, 64, 0.996), (1000, 128, 0.99), (2000, 32, 0.996)])
+def test_outputs_have_two_roundings(T, D, decay):
+    """An output or gradient in bfloat16 is rounded once itself, and on its way each term once: a decayed score, or the
+    state's copy.  A rounding to 8 bits of a normal value is 1.66e-3 in the mean square (2^-7 / sqrt(12) over values
+    between 1 and 2 and their multiples), two are 2.35e-3; a third, an operand of the state rounded too, would make
+    2.87e-3 where the state carries most of it."""
+    g = gen(T + D)
+    q, k, v, do = (normal(g, T, 4, 1, D, dtype=torch.bfloat16) for _ in range(4))
+    S, dlast, decay = 3 * normal(g, 4, 1, D, D), 3 * normal(g, 4, 1, D, D), torch.tensor([decay])
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    for final in (False, True):
+        o, last = memory.linear_attention(*leaves, decay.cuda(), S.cuda(), None, None, final)
+        grads = torch.autograd.grad([o, last] if final else [o], leaves,
+                                    [do.cuda(), dlast.cuda()] if final else [do.cuda()])
+        want = ref.attention(q, k, v, decay, S, None, D ** -0.5, do, dlast if final else None)
+        for got, exact in zip((o, *grads), (want[0], *want[2:5])):
+            assert ref.error(got, exact) <= 2.6e-3
