@@ -23,6 +23,7 @@ trains one on the synthetic biped's velocity task.
 
 from __future__ import annotations
 
+import warnings
 from dataclasses import dataclass
 
 import torch
@@ -42,6 +43,7 @@ class MemoryPPOConfig(PPOConfig):
     hidden: int = 512        # of a block's MLP
     shortest: float = 4.0    # steps that the fastest and the slowest head remember
     longest: float = 256.0
+    graph_update: bool = False   # minibatches run eagerly, whatever is set here
 
 
 class LayerNorm(nn.Module):
@@ -136,10 +138,13 @@ class _Computed:
 
 
 class MemoryPPO(PPO):
-    """PPO whose minibatches are environments, with all of their steps."""
+    """PPO whose minibatches are environments, with all of their steps.  Rollout
+    steps replay a CUDA graph (``graph_rollout``), updates run eagerly."""
 
     def __init__(self, env, cfg: MemoryPPOConfig | None = None, device=None, seed=0):
         super().__init__(env, cfg or MemoryPPOConfig(), device, seed)
+        if self.cfg.graph_update:
+            warnings.warn("MemoryPPO's updates run eagerly: graph_update is not used")
         E = env.num_envs
         if E < self.cfg.mini_batches:
             raise ValueError("fewer environments than minibatches")

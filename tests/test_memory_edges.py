@@ -129,3 +129,18 @@ def test_statistics_at_an_odd_place_are_refused():
     assert b"aligned" in lib.duck_last_error()
     assert lib.duck_layer_norm_backward(p, p, None, p + 4, p, None, None, None, 4, 8, 8, 8, 0, None) == 1
     assert b"aligned" in lib.duck_last_error()
+
+
+def test_memory_ppo_says_that_its_update_is_not_captured():
+    import warnings
+
+    from duck_gym_b200.memory_policy import MemoryPPO, MemoryPPOConfig
+    from test_memory_policy import RecallEnv
+
+    small = dict(bf16=False, width=16, heads=2, head_size=8, hidden=24, steps_per_env=4)
+    assert not MemoryPPOConfig().graph_update
+    with pytest.warns(UserWarning, match="graph_update"):
+        MemoryPPO(RecallEnv(8), MemoryPPOConfig(**small, graph_update=True), device="cpu")
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        MemoryPPO(RecallEnv(8), MemoryPPOConfig(**small), device="cpu")
