@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
     if (n >= 0 && n < C) toEnd[C - 1 - n] = f;
   }
   const int i0 = 16 * warp;   // the warp's steps
-  const bool precise = p.precise && (!OUT || last);   // what this block adds reaches the last state
+  const float fullChunk = powerOf(decay, C);
 
   uint32_t finite = 0;
   bool anyReset = false, later = init != nullptr;   // later: S is not zero
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
     // The state at the chunk's end.
     if (advance) {
       if (count < C) __syncthreads();   // toEnd
-      const float f = decays[count];
+      const float f = count == C ? fullChunk : decays[count];
 #pragma unroll
       for (int m = 0; m < SM; ++m)
 #pragma unroll
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(C * 2, (DK == 128 ? 128 : STATE ? 192 : 256) /
         }
       }
       };
-      if (precise) add(std::integral_constant<int, 3>());
+      if (p.precise && (!OUT || last)) add(std::integral_constant<int, 3>());   // it reaches the last state
       else add(std::integral_constant<int, 2>());
       later = true;
       if (OUT && buffers > 1 && c + 1 < chunks) copySlice<LV>(copies + ((c + 1) & 1) * DK * LV, S, sm0, sn0);
