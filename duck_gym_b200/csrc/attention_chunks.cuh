@@ -21,8 +21,9 @@
 // output has one rounding on its way besides its own; and of three (24 bits) where
 // the state is an output, in every chunk: the steps after a chunk may add nothing, so
 // that what has faded is all there is.  (Measured against 64 bits: outputs and
-// gradients 2.3e-3 in the 2-norm, where one rounding is 1.7e-3; states 1.5e-7 to
-// 1.0e-6, the more the longer they remember.)
+// gradients 2.3e-3 in the 2-norm, where one rounding is 1.7e-3; states and their
+// gradients 1.4e-7 to 1.04e-6, the more the longer they remember.  With three parts
+// throughout, 1000 x 256 takes 224 us forward and 353 backward.)
 //
 // Episodes: step i sees step j only if no reset lies in (j, i]; S only if none
 // lies at or before i.  Scores and states that are masked are replaced, not
@@ -39,10 +40,11 @@
 // times 64, 24 steps a rollout) and half of a score matrix is masked; a warp's 16
 // steps are a natural piece of both.  What bounds them on a B200 is the operands' way from
 // shared memory and the latency of short chains of products, with 12 to 16 warps a
-// multiprocessor: 1000 steps, 256 environments, 4 heads of 64, forward 204 us (tensor
-// pipe 35 % active, shared memory 53 %, memory 45 % busy), backward 328 us; 24 steps,
-// 1024 environments: 29 and 44 us (3.9 and 3.5 TB/s); 16384 steps, one environment, 8
-// heads of 128, in 18 segments: 44 us for what each adds, 6 for the join, 94 us.
+// multiprocessor: 1000 steps, 256 environments, 4 heads of 64, forward 202 us (tensor
+// pipe 34 % active, shared memory's data pipe 40 %, issue slots 36 %, DRAM 36 %),
+// backward 320 to 344 us by the run (42 %, 53 %, 42 %, 35 %); 24 steps, 1024
+// environments: 29 and 44 us (3.9 and 3.5 TB/s); 16384 steps, one environment, 8 heads
+// of 128, in 18 segments: 49 us for what each adds, 8 for the join, 88 us.
 // Tried and slower: two warps for the same 16 steps (235 us), 32 steps a warp (241 us
 // with a third fewer reads of shared memory), rows of V read once for scores and state
 // (258 us), the backward blocks unrolled (357 us).
@@ -932,8 +934,10 @@ __global__ void __launch_bounds__(256) joinSegments(float *segments, const uint8
 }
 
 // Sweeps of a call step by step, for the environments and heads that have one of
-// their `count` flags set; usually none has.  A block has a run of them and looks
-// at all its flags at once first.
+// their `count` flags set; usually none has (2.4 us).  A block has a run of them and
+// looks at all its flags at once first.  Where many are set this is slow, one head
+// after the other: 24 steps of 4096 environments, 4 heads of 64, forward and backward,
+// 149 us a call with none, 343 us with one environment, 11.2 ms with all.
 template <int DI>
 __global__ void __launch_bounds__(scanThreads(DI))
     redoAttention(const __grid_constant__ Sweeps p, const uint8_t *flags, int count) {

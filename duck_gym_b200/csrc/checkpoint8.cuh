@@ -21,8 +21,8 @@
 // lanes (bfloat16; 32 in float32) hold a group in registers, the next group's
 // loads issued before; other rows take four groups a warp, one value at a time.
 // Measured cold on a B200, bfloat16, 24576 x 512: forward 16.8 us (3.8 TB/s; some
-// 20 operations an element keep it from more), backward 15.4 us (5.7 TB/s);
-// float32, 4999 x 129: 6.3 and 5.0 us.  The largest magnitude is taken on the bits, where NaN
+// 20 operations an element keep it from more: issue slots 60 %), backward 15.5 us (5.7 TB/s);
+// float32, 4999 x 129: 6.4 and 5.0 us.  The largest magnitude is taken on the bits, where NaN
 // is above infinity and that above all numbers, two bfloat16 at a time.
 #pragma once
 #include "numeric_types.cuh"

@@ -19,8 +19,8 @@
 // keeps the same columns for all of its rows, so the sums for the weight and the
 // bias stay in its registers and leave the block as one partial row.  Wider rows
 // take the kernels that read a row several times (norm...Any).  Measured cold on a
-// B200, bfloat16, 393216 x 512: forward 156 us (5.2 TB/s), backward 220 us
-// (5.5 TB/s) and 4 us for the partial rows; 24576 x 256: 11, 11.5 and 4.5 us, of
+// B200, bfloat16, 393216 x 512: forward 156 us (5.2 TB/s), backward 216 us
+// (5.6 TB/s) and 4 us for the partial rows; 24576 x 256: 11, 11.5 and 4.5 us, of
 // which some 7 are a launch's own and the first loads'.
 #pragma once
 #include "numeric_types.cuh"

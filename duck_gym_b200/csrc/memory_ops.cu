@@ -243,7 +243,8 @@ struct ChunkPlan {
 };
 // With fewer blocks than half of what fits on the GPU at once, T is split so that
 // the segments' blocks fill it once: a second, partly filled round costs as much as a
-// full one (a replay of 16384 steps, 8 heads of 128: 187 us in 26 segments).
+// full one (a replay of 16384 steps, 8 heads of 128: 187 us in 26 segments).  Of the
+// backward pass at head sizes up to 64 a fourth block would fit.
 ChunkPlan planChunks(const duck_attention &a, bool backward) {
   ChunkPlan p{};
   p.C = a.T <= 32 ? 32 : 64;
@@ -327,7 +328,7 @@ void forwardChunks(const duck_attention &a, cudaStream_t stream) {
   c.scale = a.scale;
   c.precise = a.state_out != nullptr;
   c.flags = reinterpret_cast<uint8_t *>(a.scratch) + plan.segmentBytes + plan.cutBytes;
-// Two sets of tiles, except where they are so large (128 rows of state) that two blocks on a multiprocessor hide
+  // Two sets of tiles, except where they are so large (128 rows of state) that two blocks on a multiprocessor hide
   // a chunk's loads better than one block's own next set: 107 -> 90 us for the replay of 16384 steps.
   const bool more = std::min(plan.chunks, plan.segmentLength / plan.C) > 1;
   const int buffers = more && a.Dk <= 64 ? 2 : 1;

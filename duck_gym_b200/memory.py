@@ -308,7 +308,12 @@ def linear_attention(q, k, v, decay, state=None, resets=None, scale=None, final_
     layer; ``state`` [E, H, Dk, Dv] float32 before the first step (None: zero);
     ``scale`` is Dk ** -0.5 by default.  The state after the last step is
     returned where ``final_state`` is set, else None.  Gradients flow to q, k,
-    v and the state."""
+    v and the state.
+
+    bfloat16 operands on the GPU: each term of an output or gradient is rounded to
+    8 bits once on its way (a decayed score, or the state it is read from), and
+    the result once more; the states themselves are float32.  Float32 operands
+    are not rounded."""
     _check_heads(q, k, v, decay, 4, "linear_attention")
     if state is not None:
         _check_state(state, q, v)
