@@ -88,6 +88,13 @@ def _grad_needed(*tensors):
     return forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _refuse_tangents(*tensors):
+    """For the calls without an autograd function: a tangent would be dropped."""
+    if forward_ad._current_level >= 0:
+        _require(all(forward_ad.unpack_dual(t).tangent is None for t in tensors),
+                 "there are no forward-mode derivatives of this call")
+
+
 # ------------------------------------------------------------------ layer norm
 def _rows_of(x):
     """x as rows of its last axis, with a stride between them: a view where the
@@ -353,6 +360,7 @@ def linear_attention_step(q, k, v, decay, state, reset=None, scale=None):
                                          None if reset is None else reset[None], scale)
             state.copy_(last)
         return out[0]
+    _refuse_tangents(q, k, v, state)
     _require(state.is_contiguous(), "the state is updated in place and has to be contiguous")
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     if decay.dtype != torch.float32 or not decay.is_contiguous():
@@ -400,6 +408,7 @@ def elu_checkpoint(x):
     pass (``elu_restore``).  Not differentiable by itself; ``checkpointed_mlp``
     is the differentiable use."""
     _require(x.dim() > 0 and x.shape[-1] > 0, "elu_checkpoint: the last axis is empty")
+    _refuse_tangents(x)
     x = x.detach()
     if not x.is_cuda:
         y = F.elu(x)
@@ -426,6 +435,7 @@ def elu_restore(dy, kept, restore=True, bounded=False):
     _require(dy.shape == shape and len(shape) and scales.shape == shape[:-1] + (-(-shape[-1] // GROUP),) and codes.dtype == torch.int8
              and scales.dtype == torch.float32 and dy.device == codes.device == scales.device,
              "elu_restore: the gradient and the checkpoint do not belong together")
+    _refuse_tangents(dy, scales)
     dy = dy.detach()
     if not dy.is_cuda:
         y = _kept_plain(kept)

@@ -180,3 +180,23 @@ def test_outputs_have_two_roundings(T, D, decay):
         want = ref.attention(q, k, v, decay, S, None, D ** -0.5, do, dlast if final else None)
         for got, exact in zip((o, *grads), (want[0], *want[2:5])):
             assert ref.error(got, exact) <= 2.6e-3
+
+
+def test_tangents_are_refused_by_calls_without_gradients():
+    from torch.autograd import forward_ad
+
+    decay, x = torch.tensor([0.9, 0.95], device="cuda"), torch.randn(3, 2, 8, device="cuda")
+    state = torch.randn(3, 2, 8, 8, device="cuda")
+    y, kept = memory.elu_checkpoint(x)
+    calls = [(lambda q: memory.linear_attention_step(q, x, x, decay, state.clone()), x),
+             (lambda S: memory.linear_attention_step(x, x, x, decay, S.clone()), state),
+             (lambda t: memory.elu_checkpoint(t)[0], x), (lambda t: memory.elu_restore(t, kept)[0], y),
+             (lambda s: memory.elu_restore(y, memory.Checkpoint8(kept.codes, s))[0], kept.scales)]
+    for f, at in calls:
+        want = f(at)
+        with forward_ad.dual_level():
+            assert torch.equal(f(at), want)
+            with pytest.raises(RuntimeError):
+                f(forward_ad.make_dual(at, torch.ones_like(at)))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (at,), (torch.ones_like(at),))
