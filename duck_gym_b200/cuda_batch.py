@@ -84,6 +84,9 @@ def library():
         lib.duck_linear_attention_sizes.argtypes = [P, P]
         for name in ("duck_linear_attention_forward", "duck_linear_attention_backward", "duck_linear_attention_step"):
             getattr(lib, name).argtypes = [P, P]
+        for name in ("duck_gated_recurrence_sizes", "duck_gated_recurrence_forward", "duck_gated_recurrence_backward",
+                     "duck_gated_recurrence_step"):
+            getattr(lib, name).argtypes = [P, P]
         lib.duck_env_obs_dim.argtypes = [P, P]
         lib.duck_env_targets.argtypes = [P, P, D, P, P, P, P, P, P]
         lib.duck_env_reference_targets.argtypes = [P, P, P, D, P, P, P, P, P, P, P, P]
@@ -108,7 +111,8 @@ def library():
                      "duck_bam_servo", "duck_bam_reset_buffers", "duck_bam_observe", "duck_ppo_loss_scratch",
                      "duck_ppo_loss", "duck_layer_norm_forward", "duck_layer_norm_backward", "duck_elu_checkpoint",
                      "duck_elu_restore", "duck_elu_restore_bounded", "duck_linear_attention_sizes", "duck_linear_attention_forward",
-                     "duck_linear_attention_backward", "duck_linear_attention_step"):
+                     "duck_linear_attention_backward", "duck_linear_attention_step", "duck_gated_recurrence_sizes",
+                     "duck_gated_recurrence_forward", "duck_gated_recurrence_backward", "duck_gated_recurrence_step"):
             getattr(lib, name).restype = I
         _lib = lib
     return _lib

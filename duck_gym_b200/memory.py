@@ -1,9 +1,12 @@
 """Operators of a policy with memory: layer norm, linear attention with one
-decay per head, and activations kept in 8 bits for the backward pass.
+decay per head, a gated linear recurrence, and activations kept in 8 bits for the
+backward pass.
 
     layer_norm(x, weight, bias, eps)                           -> y
     linear_attention(q, k, v, decay, state, resets, ...)       -> out, state
     linear_attention_step(q, k, v, decay, state, reset, ...)   -> out
+    gated_recurrence(gates, values, state, resets, ...)        -> out, state
+    gated_recurrence_step(gates, values, state, reset)         -> out
     elu_checkpoint(x)                                          -> y, Checkpoint8
     elu_restore(dy, kept)                                      -> dx, y
     checkpointed_mlp(x, weights, biases)                       -> y
@@ -373,6 +376,148 @@ def linear_attention_step(q, k, v, decay, state, reset=None, scale=None):
             _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr(),
                             _address(reset), 0, state.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0,
                             0, qe, qh, 0, ke, kh, 0, ve, vh, 0, 0, 0, 1, E, H, Dk, Dv, _TYPES[q.dtype], scale))
+    torch.autograd.graph.increment_version(state)   # autograd does not see a kernel's writes
+    return out
+
+
+# ------------------------------------------------------------ gated recurrence
+# struct duck_recurrence of include/duck_b200.h.
+_RECURRENCE = struct.Struct("@13P6q4i")
+
+
+@functools.lru_cache(maxsize=1024)
+def _recurrence_workspace(T, E, N, kind):
+    """Bytes of scratch of a call, and of what a forward call keeps for the
+    backward one."""
+    out = (ctypes.c_int64 * 2)()
+    _raise(library().duck_gated_recurrence_sizes(_RECURRENCE.pack(*(0,) * 13, *(0,) * 6, T, E, N, kind), out))
+    return tuple(out)
+
+
+def _recurrence_forward(gates, values, state, resets, final_state, keep):
+    T, E, N = gates.shape
+    kind = _TYPES[gates.dtype]
+    out = _dense_like(gates)
+    last = torch.empty((E, N), dtype=torch.float32, device=gates.device) if final_state else None
+    sizes = _recurrence_workspace(T, E, N, kind)
+    scratch = _buffer(sizes[0], gates.device)
+    saved = _buffer(sizes[1], gates.device) if keep else None
+    _launch(library().duck_gated_recurrence_forward, gates.device,
+            _RECURRENCE.pack(gates.data_ptr(), values.data_ptr(), out.data_ptr(), _address(resets), _address(state),
+                             _address(last), 0, 0, 0, 0, 0, _address(saved), _address(scratch),
+                             *gates.stride()[:2], *values.stride()[:2], 0, 0, T, E, N, kind))
+    return out, last, saved
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gates, values, state, resets, final_state):
+        out, last, saved = _recurrence_forward(gates, values, state, resets, final_state, True)
+        ctx.save_for_backward(gates, values, state, resets, saved)
+        ctx.set_materialize_grads(False)
+        return out, last
+
+    @staticmethod
+    @_once
+    def backward(ctx, dout, dlast):
+        gates, values, state, resets, saved = ctx.saved_tensors
+        if dout is None and dlast is None:
+            return (None,) * 5
+        T, E, N = gates.shape
+        kind = _TYPES[gates.dtype]
+        dout = gates.new_zeros((T, E, N)) if dout is None else _dense_last(dout)
+        dlast = None if dlast is None else _aligned(dlast)
+        dgates, dvalues = _dense_like(gates), _dense_like(values)
+        dstate = torch.empty_like(state) if ctx.needs_input_grad[2] else None
+        scratch = _buffer(_recurrence_workspace(T, E, N, kind)[0], gates.device)
+        _launch(library().duck_gated_recurrence_backward, gates.device,
+                _RECURRENCE.pack(gates.data_ptr(), values.data_ptr(), 0, _address(resets), _address(state), 0,
+                                 dout.data_ptr(), _address(dlast), dgates.data_ptr(), dvalues.data_ptr(),
+                                 _address(dstate), _address(saved), _address(scratch),
+                                 *gates.stride()[:2], *values.stride()[:2], *dout.stride()[:2], T, E, N, kind))
+        return dgates, dvalues, dstate, None, None
+
+
+def _recurrence_plain(gates, values, state, resets):
+    """The recurrence step by step, in float32 or wider."""
+    dtype = gates.dtype
+    wide = torch.promote_types(dtype, torch.float32)
+    T, E, N = gates.shape
+    gates, values = gates.to(wide), values.to(wide)
+    h = gates.new_zeros(E, N) if state is None else state if T else state.clone()
+    out = []
+    for t in range(T):
+        if resets is not None:
+            h = torch.where(resets[t, :, None] != 0, torch.zeros_like(h), h)
+        h = torch.sigmoid(gates[t]) * h + torch.sigmoid(-gates[t]) * values[t]
+        out.append(h)
+    out = torch.stack(out) if T else gates.new_zeros(0, E, N)
+    return out.to(dtype), h
+
+
+def _check_channels(gates, values, state, dims, what):
+    _require(gates.dim() == dims and gates.shape == values.shape and gates.dtype == values.dtype
+             and gates.device == values.device and gates.dtype in _WIDE,
+             f"{what}: gates and values have one shape, floating type and device")
+    _check_type(gates, what)
+    _require(state is None or (state.shape == gates.shape[-2:] and state.dtype == _WIDE[gates.dtype]
+                               and state.device == gates.device),
+             f"{what}: the state is float32 [environments, channels] on the gates' device")
+
+
+def gated_recurrence(gates, values, state=None, resets=None, final_state=True):
+    """A gated linear recurrence over a rollout, channel by channel: ``(out, state)``
+    with
+
+        out_t = f_t out_{t-1} + (1 - f_t) values_t,   f_t = sigmoid(gates_t),
+
+    out_{t-1} being zero where ``resets[t, e]`` says that an episode begins.
+
+    ``gates`` and ``values`` [T, E, N] (T steps, E environments, N channels),
+    ``state`` [E, N] float32 before the first step (None: zero).  The state after
+    the last step is returned where ``final_state`` is set, else None.  Gradients
+    flow to gates, values and the state.  States are float32; out has the gates'
+    type, rounded once, and so have the gradients."""
+    _check_channels(gates, values, state, 3, "gated_recurrence")
+    if resets is not None:
+        resets = _mask(resets, gates.shape[:2], gates.device)
+    if not gates.is_cuda:
+        out, last = _recurrence_plain(gates, values, state, resets)
+        return out, last if final_state else None
+    gates, values = _dense_last(gates), _dense_last(values)
+    if state is not None:
+        state = _aligned(state)
+    if _grad_needed(gates, values, state):
+        return _GatedRecurrence.apply(gates, values, state, resets, final_state)
+    return _recurrence_forward(gates, values, state, resets, final_state, False)[:2]
+
+
+def gated_recurrence_step(gates, values, state, reset=None):
+    """One control step of ``gated_recurrence`` for every environment, without
+    gradients: ``gates`` and ``values`` [E, N], ``reset`` [E].  ``state`` [E, N]
+    float32 is updated in place; returns out [E, N].  A backward pass that still
+    needs the state as it was raises, as after any operation in place (a replay of
+    a CUDA graph is not seen)."""
+    _require(state is not None, "gated_recurrence_step: there is no state")
+    _check_channels(gates, values, state, 2, "gated_recurrence_step")
+    _require(not (state.requires_grad and torch.is_grad_enabled()),
+             "the state is updated in place without gradients, it must not require one")
+    if reset is not None:
+        reset = _mask(reset, gates.shape[:1], gates.device)
+    if not gates.is_cuda:
+        with torch.no_grad():
+            out, last = _recurrence_plain(gates[None], values[None], state, None if reset is None else reset[None])
+            state.copy_(last)
+        return out[0]
+    _refuse_tangents(gates, values, state)
+    _require(state.is_contiguous(), "the state is updated in place and has to be contiguous")
+    gates, values = _dense_last(gates), _dense_last(values)
+    E, N = gates.shape
+    out = _dense_like(gates)
+    _launch(library().duck_gated_recurrence_step, gates.device,
+            _RECURRENCE.pack(gates.data_ptr(), values.data_ptr(), out.data_ptr(), _address(reset), 0, state.data_ptr(),
+                             0, 0, 0, 0, 0, 0, 0, 0, gates.stride(0), 0, values.stride(0), 0, 0, 1, E, N,
+                             _TYPES[gates.dtype]))
     torch.autograd.graph.increment_version(state)   # autograd does not see a kernel's writes
     return out
 

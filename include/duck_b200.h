@@ -427,6 +427,41 @@ int duck_linear_attention_backward(const duck_attention *args, duck_stream strea
  * updated in place and `out` written.  resets is [E]. */
 int duck_linear_attention_step(const duck_attention *args, duck_stream stream);
 
+/* Gated linear recurrence for E environments of N channels:
+ *   h_t = f_t h_{t-1} + (1 - f_t) c_t,  f_t = sigmoid(gate_t),
+ * h_{t-1} being zero where resets[t, e] is set (an episode begins at t).  gates,
+ * values (c), out (h) and their gradients are [T, E, N]; gates, values and dout
+ * have the strides given, {t, e}; the outputs are dense.  States are dense [E, N]
+ * float32.  Outputs, workspaces and the states of whole rollouts lie on 16-byte
+ * boundaries, and no output overlaps an input.  T <= 2^31 - 2^24 - 1 and
+ * E N < 2^31. */
+typedef struct duck_recurrence {
+  const void *gates, *values;
+  void *out;                  /* forward */
+  const uint8_t *resets;      /* [T, E] dense, or NULL */
+  const float *state_in;      /* h before the first step, or NULL for zero */
+  float *state_out;           /* forward: h after the last step, or NULL */
+  const void *dout;           /* backward: gradient of out */
+  const float *dstate_out;    /* backward: gradient of state_out, or NULL */
+  void *dgates, *dvalues;     /* backward */
+  float *dstate_in;           /* backward: gradient of state_in, or NULL */
+  float *saved;               /* forward writes, backward reads: duck_gated_recurrence_sizes; or NULL */
+  float *scratch;             /* duck_gated_recurrence_sizes */
+  int64_t gates_stride[2], values_stride[2], dout_stride[2];
+  int32_t T, E, N, type;
+} duck_recurrence;
+
+/* Bytes of workspace for calls of these sizes (only T, E, N and type are looked
+ * at): out[0] scratch of a forward or backward call, out[1] `saved`, which a
+ * forward call that a backward call will follow has to be given. */
+int duck_gated_recurrence_sizes(const duck_recurrence *args, int64_t *out);
+int duck_gated_recurrence_forward(const duck_recurrence *args, duck_stream stream);
+int duck_gated_recurrence_backward(const duck_recurrence *args, duck_stream stream);
+/* One step (T and the strides over it are not read), gates, values and out
+ * [E, N]: the state in state_out, on a 4-byte boundary, is updated in place.
+ * resets is [E]. */
+int duck_gated_recurrence_step(const duck_recurrence *args, duck_stream stream);
+
 /* No reference counterpart.  FP32 fused-multiply-add throughput probe used
  * as the roofline denominator: runs `iterations` dependent FMA chains on
  * every SM and returns achieved TFLOP/s (2 flops per FMA) in *tflops. */
