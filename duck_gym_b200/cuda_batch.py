@@ -87,6 +87,9 @@ def library():
         for name in ("duck_gated_recurrence_sizes", "duck_gated_recurrence_forward", "duck_gated_recurrence_backward",
                      "duck_gated_recurrence_step"):
             getattr(lib, name).argtypes = [P, P]
+        lib.duck_gradient_squares.argtypes = [P, I, I, P, P, P]
+        lib.duck_adamw_step.argtypes = [P, I, P, P]
+        lib.duck_moment_values.argtypes = [P, I, P]
         lib.duck_env_obs_dim.argtypes = [P, P]
         lib.duck_env_targets.argtypes = [P, P, D, P, P, P, P, P, P]
         lib.duck_env_reference_targets.argtypes = [P, P, P, D, P, P, P, P, P, P, P, P]
@@ -112,7 +115,8 @@ def library():
                      "duck_ppo_loss", "duck_layer_norm_forward", "duck_layer_norm_backward", "duck_elu_checkpoint",
                      "duck_elu_restore", "duck_elu_restore_bounded", "duck_linear_attention_sizes", "duck_linear_attention_forward",
                      "duck_linear_attention_backward", "duck_linear_attention_step", "duck_gated_recurrence_sizes",
-                     "duck_gated_recurrence_forward", "duck_gated_recurrence_backward", "duck_gated_recurrence_step"):
+                     "duck_gated_recurrence_forward", "duck_gated_recurrence_backward", "duck_gated_recurrence_step",
+                     "duck_gradient_squares", "duck_adamw_step", "duck_moment_values"):
             getattr(lib, name).restype = I
         _lib = lib
     return _lib

@@ -1,0 +1,374 @@
+"""AdamW over all tensors of a model in one launch, with moments in 32 bits or in
+8, and gradients clipped by their common norm on the way.
+
+    adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, ...)
+    state8_zeros(like, signed)                                   -> State8
+    state8_values(states)                                        -> tensors
+    AdamW(params, lr, ..., bits=8, max_grad_norm=1.0)            torch.optim.Optimizer
+
+The reference trains with torch's Adam (scripts/train_bam_native.py:14-140), whose
+formula this is; see ``ppo.PPOConfig.optimizer``.
+
+CUDA tensors run the library's kernels on the current stream (float32 or bfloat16
+parameters, no other type; there is no fallback), CPU tensors a plain torch
+restatement of the same arithmetic.  Wrong devices, types or shapes raise
+``RuntimeError``.  The calls allocate only with torch, never synchronise and can be
+captured in CUDA graphs: the count of steps is a tensor on the device, and so can
+the learning rate be.
+"""
+
+from __future__ import annotations
+
+import bisect
+import ctypes
+import math
+import struct
+from typing import NamedTuple
+
+import torch
+
+from .cuda_batch import library
+from .memory import _launch
+
+GROUP = 128          # values that share one exponent of a moment in 8 bits
+SUMS = 592           # DUCK_GRADIENT_SUMS
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_TENSOR = struct.Struct("@6Pq2i")       # struct duck_adamw_tensor of include/duck_b200.h
+_OPTIONS = struct.Struct("@3P6d2i")     # struct duck_adamw
+
+
+class State8(NamedTuple):
+    """A moment in 8 bits: ``codes`` of its tensor's shape, int8 for a first moment
+    and uint8 for a second one, and ``exponents`` uint8, one per group of 128 values.
+    A value's float32 has the leading 12 bits |code| + max(0, 8 exponent + 8 - most),
+    most = 127 and 255; code 0 is zero, and exponent 255 makes a group's values NaN."""
+
+    codes: torch.Tensor
+    exponents: torch.Tensor
+
+
+def _require(condition, message):
+    if not condition:
+        raise RuntimeError(message)
+
+
+def _groups(t):
+    return -(-t.numel() // GROUP)
+
+
+def state8_zeros(like, signed):
+    """The first (``signed``) or second moment of a tensor before any step."""
+    return State8(torch.zeros(like.shape, dtype=torch.int8 if signed else torch.uint8, device=like.device),
+                  torch.zeros(_groups(like), dtype=torch.uint8, device=like.device))
+
+
+def _check_state8(state, shape, device, dtypes, what):
+    codes, exponents = state
+    _require(codes.dtype in dtypes and exponents.dtype == torch.uint8 and codes.shape == shape
+             and exponents.shape == (_groups(codes),) and codes.device == exponents.device == device
+             and codes.is_contiguous() and exponents.is_contiguous(),
+             f"{what}: a moment in 8 bits is dense codes of its tensor's shape and one exponent for 128 of them")
+
+
+# ------------------------------------------------------------ plain restatement
+def _mix(x):
+    """The 32-bit finaliser of MurmurHash3, on int64."""
+    x = (x ^ (x >> 16)) * 0x85EBCA6B & 0xFFFFFFFF
+    x = (x ^ (x >> 13)) * 0xC2B2AE35 & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def _spread(per_group, n):
+    return per_group.repeat_interleave(GROUP)[:n]
+
+
+def _decode(codes, exponents):
+    most, n = 127 if codes.dtype == torch.int8 else 255, codes.numel()
+    c, e = codes.reshape(-1).int(), exponents.int()
+    bits = torch.where(c == 0, 0, c.abs() + _spread((8 * e + (8 - most)).clamp_min(0), n)) << 20
+    value = torch.where(_spread(e, n) == 255, math.nan, bits.view(torch.float32))
+    return torch.where(c < 0, -value, value).view(codes.shape)
+
+
+def _encode(x, state, noise):
+    """Writes x to `state`, its low 20 bits rounded by `noise` in [0, 2^20)."""
+    codes, exponents = state
+    most, n = 127 if codes.dtype == torch.int8 else 255, x.numel()
+    if n == 0:
+        return
+    bits = x.reshape(-1).view(torch.int32) & 0x7FFFFFFF
+    padded = torch.nn.functional.pad(bits, (0, exponents.numel() * GROUP - n)).view(-1, GROUP)
+    e = padded.amax(1) >> 23
+    place = ((bits.clamp_max(0x7F800000) + noise.int()) >> 20).clamp_max(2039)
+    place = place - _spread((8 * e + (8 - most)).clamp_min(0), n)
+    place = place.clamp(0, 127) if most == 127 else torch.where(bits == 0, 0, place.clamp(1, 255))
+    if most == 127:
+        place = torch.where(x.reshape(-1).signbit(), -place, place)
+    codes.copy_(place.view(codes.shape))
+    exponents.copy_(e)
+
+
+def _plain_tensor(place, p, g, m, v, count, clip, beta1, beta2, ahead, widen, shrink, eps):
+    eight = not torch.is_tensor(m)
+    m32, v32 = (_decode(*m), _decode(*v)) if eight else (m, v)
+    g = g.float() if clip is None else g.float() * clip
+    m32 = m32 * beta1 + g * (1.0 - beta1)
+    v32 = v32 * beta2 + g * g * (1.0 - beta2)
+    new = p.float() * shrink - ahead * (m32 / (v32.sqrt() * widen + eps))
+    if eight or p.dtype == torch.bfloat16:
+        key = _mix(torch.tensor((count + 0x9E3779B9 * (place + 1)) & 0xFFFFFFFF))
+        noise = _mix(key ^ (torch.arange(p.numel()) & 0xFFFFFFFF))
+    if p.dtype == torch.bfloat16:
+        bits = new.reshape(-1).view(torch.int32)
+        up = torch.where(new.reshape(-1).isfinite(), bits + (noise & 0xFFFF).int(), bits)
+        new = torch.where(new.isfinite(), (up & -65536).view(torch.float32).view(p.shape), new)
+    p.copy_(new)
+    if eight:
+        _encode(m32, m, (noise >> 20 << 8) + 128)
+        _encode(v32, v, noise & 0xFFFFF)
+    else:
+        m.copy_(m32)
+        v.copy_(v32)
+
+
+def _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm, total):
+    step += 1
+    count, rate = int(step), float(lr)
+    clip = None
+    if max_norm is not None:
+        clip = (max_norm / (total.sqrt() + 1e-6)).clamp_max(1.0).float()
+    scalars = (torch.tensor(x, dtype=torch.float64).float() for x in (
+        rate / (1.0 - betas[0] ** count), (1.0 - betas[1] ** count) ** -0.5, 1.0 - rate * weight_decay))
+    ahead, widen, shrink = scalars
+    for place, each in enumerate(zip(params, grads, ms, vs)):
+        _plain_tensor(place, *each, count, clip, *betas, ahead, widen, shrink, eps)
+
+
+# ----------------------------------------------------------------- entry points
+def _check_apart(written, read, what):
+    """Spans (first byte, end) of arrays: none that is written overlaps another one."""
+    written.sort()
+    starts = [a for a, _ in written]
+    for (_, end), b in zip(written, starts[1:]):
+        _require(end <= b, f"{what}: a tensor is there twice, or two of them overlap")
+    for a, end in read:
+        i = bisect.bisect_left(starts, end)   # the spans that begin before its end
+        _require(i == 0 or written[i - 1][1] <= a, f"{what}: a gradient overlaps what is written")
+
+
+def _checked(params, grads, exp_avgs, exp_avg_sqs):
+    """Whether the moments have 8 bits, the tensors' device and dense gradients."""
+    _require(len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) > 0,
+             "adamw_step: one gradient and two moments for each of one or more parameters")
+    device = params[0].device
+    eight = not torch.is_tensor(exp_avgs[0])
+    dense, spans = [], []
+    span = lambda t: (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
+        _require(p.dtype in _TYPES and p.device == device and p.is_contiguous(),
+                 "adamw_step: parameters are dense float32 or bfloat16 tensors of one device")
+        _require(g.shape == p.shape and g.dtype == p.dtype and g.device == device and not g.is_sparse,
+                 "adamw_step: a gradient has its parameter's shape, type and device")
+        _require(torch.is_tensor(m) != eight and torch.is_tensor(v) != eight,
+                 "adamw_step: all moments have 32 bits, or all have 8")
+        spans.append(span(p))
+        if eight:
+            _check_state8(m, p.shape, device, (torch.int8,), "adamw_step")
+            _check_state8(v, p.shape, device, (torch.uint8,), "adamw_step")
+            spans += [span(t) for t in (*m, *v)]
+        else:
+            for t in (m, v):
+                _require(t.dtype == torch.float32 and t.shape == p.shape and t.device == device and t.is_contiguous(),
+                         "adamw_step: moments are dense float32 tensors of their parameters' shapes")
+                spans.append(span(t))
+        dense.append(g if g.is_contiguous() else g.contiguous())
+    _check_apart([s for s in spans if s[1] > s[0]], [s for s in map(span, dense) if s[1] > s[0]], "adamw_step")
+    return eight, device, dense
+
+
+def _table(rows):
+    return b"".join(_TENSOR.pack(*row) for row in rows)
+
+
+def _rows(params, grads, ms, vs, eight):
+    if eight:
+        return [(p.data_ptr(), g.data_ptr(), m[0].data_ptr(), v[0].data_ptr(), m[1].data_ptr(), v[1].data_ptr(), p.numel(),
+                 _TYPES[p.dtype], i) for i, (p, g, m, v) in enumerate(zip(params, grads, ms, vs))]
+    return [(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, p.numel(), _TYPES[p.dtype], i)
+            for i, (p, g, m, v) in enumerate(zip(params, grads, ms, vs))]
+
+
+class _Norm:
+    """The squares of gradients, summed over several lists of them."""
+
+    def __init__(self, device):
+        self.count = 0
+        self.sums = (torch.empty(SUMS, dtype=torch.float64, device=device) if device.type == "cuda"
+                     else torch.zeros((), dtype=torch.float64))
+
+    def add(self, grads):
+        if self.sums.dim() == 0:
+            for g in grads:
+                self.sums += g.double().square().sum()
+            return
+        rows = [(0, g.data_ptr(), 0, 0, 0, 0, g.numel(), _TYPES[g.dtype], 0) for g in grads]
+        count = ctypes.c_int()
+        _launch(library().duck_gradient_squares, self.sums.device, _table(rows), len(rows), self.count,
+                self.sums.data_ptr(), ctypes.byref(count))
+        self.count = count.value
+        if self.count == 0:   # only empty gradients: a norm of zero
+            self.sums[:1].zero_()
+            self.count = 1
+
+
+def _step(params, grads, ms, vs, eight, device, step, lr, betas, eps, weight_decay, max_norm, norm):
+    if device.type != "cuda":
+        return _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm,
+                      None if norm is None else norm.sums)
+    on_device = torch.is_tensor(lr) and lr.is_cuda
+    if on_device and lr.dtype != torch.float32:
+        lr = lr.float()
+    rows = _rows(params, grads, ms, vs, eight)
+    options = _OPTIONS.pack(step.data_ptr(), lr.data_ptr() if on_device else 0, norm.sums.data_ptr() if norm else 0,
+                            0.0 if on_device else float(lr), *betas, eps, weight_decay, 0.0 if norm is None else max_norm,
+                            norm.count if norm else 0, 8 if eight else 32)
+    _launch(library().duck_adamw_step, device, _table(rows), len(rows), options)
+    written = [*params, step]
+    for m, v in zip(ms, vs):
+        written += [*m, *v] if eight else [m, v]
+    torch.autograd.graph.increment_version(written)   # autograd does not see a kernel's writes
+
+
+def _check_options(step, lr, betas, eps, weight_decay, max_norm, device):
+    _require(torch.is_tensor(step) and step.dtype == torch.int64 and step.numel() == 1 and step.device == device,
+             "adamw_step: the count of steps is an int64 tensor of one value on the parameters' device")
+    if torch.is_tensor(lr):
+        _require(lr.numel() == 1 and lr.is_floating_point() and lr.device in (device, torch.device("cpu")),
+                 "adamw_step: the learning rate is a number, or a floating tensor of one value")
+    _require(len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas) and 0.0 <= eps < math.inf
+             and 0.0 <= weight_decay < math.inf, "adamw_step: betas in [0, 1), eps and weight decay of 0 or more")
+    _require(max_norm is None or max_norm >= 0.0, "adamw_step: a norm of 0 or more")
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
+               max_norm=None):
+    """One AdamW step over lists of tensors, in place:
+
+        m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+
+    ``exp_avgs`` (m) and ``exp_avg_sqs`` (v) are float32 tensors, or all of them
+    ``State8``; ``step`` is an int64 tensor, the steps done before (t - 1), and is
+    counted up (not to be read on another stream meanwhile).  ``lr`` is a number or a
+    tensor.  With ``max_norm`` g is the gradient times min(1, max_norm / (norm + 1e-6)),
+    norm that of all gradients together; the gradients themselves stay as they are.
+
+    bfloat16 parameters and codes are rounded up or down at random, by a hash of t, the
+    tensor's place in the list and the value's place in the tensor: what a step adds is
+    mostly less than half a place of theirs, and would be lost."""
+    eight, device, grads = _checked(params, grads, exp_avgs, exp_avg_sqs)
+    _check_options(step, lr, betas, eps, weight_decay, max_norm, device)
+    norm = None
+    if max_norm is not None:
+        norm = _Norm(device)
+        norm.add(grads)
+    _step(params, grads, exp_avgs, exp_avg_sqs, eight, device, step, lr, betas, eps, weight_decay, max_norm, norm)
+
+
+@torch.no_grad()
+def state8_values(states):
+    """The float32 tensors that moments in 8 bits stand for."""
+    states = [State8(*s) for s in states]
+    if not states:
+        return []
+    device = states[0].codes.device
+    for s in states:
+        _check_state8(s, s.codes.shape, device, (torch.int8, torch.uint8), "state8_values")
+    if device.type != "cuda":
+        return [_decode(*s) for s in states]
+    values = [torch.empty(s.codes.shape, dtype=torch.float32, device=device) for s in states]
+    rows = []
+    for value, (codes, exponents) in zip(values, states):
+        signed = codes.dtype == torch.int8
+        m, me, v, ve = (codes.data_ptr(), exponents.data_ptr(), 0, 0) if signed else (0, 0, codes.data_ptr(), exponents.data_ptr())
+        rows.append((value.data_ptr(), 0, m, v, me, ve, codes.numel(), 0, 0))
+    _launch(library().duck_moment_values, device, _table(rows), len(rows))
+    return values
+
+
+class AdamW(torch.optim.Optimizer):
+    """``adamw_step`` as a torch optimizer.
+
+    ``bits`` (32 or 8) of the moments; with ``max_grad_norm`` gradients are clipped by
+    the norm of those of all groups, in the step itself (``.grad`` stays as it is).
+    ``lr`` may be a tensor on the device that a schedule writes to.  A group has one
+    count of steps; a parameter without a gradient is left as it is, as torch's is, but
+    its steps are counted."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits=32, max_grad_norm=None):
+        if bits not in (8, 32):
+            raise ValueError("moments have 8 or 32 bits")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError("invalid max_grad_norm")
+        self.max_grad_norm = max_grad_norm
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits))
+
+    def _moments(self, p, bits):
+        state = self.state[p]
+        if not state:
+            if bits == 8:
+                m, v = state8_zeros(p, True), state8_zeros(p, False)
+                state.update(exp_avg=m.codes, exp_avg_exponents=m.exponents, exp_avg_sq=v.codes,
+                             exp_avg_sq_exponents=v.exponents)
+            else:
+                state["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                state["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        if bits == 8:
+            return (State8(state["exp_avg"], state["exp_avg_exponents"]),
+                    State8(state["exp_avg_sq"], state["exp_avg_sq_exponents"]))
+        return state["exp_avg"], state["exp_avg_sq"]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work, norms = [], {}
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            if "step" not in group:
+                group["step"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
+            moments = [self._moments(p, group["bits"]) for p in params]
+            ms, vs = [m for m, _ in moments], [v for _, v in moments]
+            eight, device, grads = _checked(params, [p.grad for p in params], ms, vs)
+            _check_options(group["step"], group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                           self.max_grad_norm, device)
+            if self.max_grad_norm is not None:
+                _require(not norms or device in norms, "AdamW: one device where gradients are clipped")
+                norms.setdefault(device, None)
+                norms[device] = norms[device] or _Norm(device)
+                norms[device].add(grads)
+            work.append((params, grads, ms, vs, eight, device, group))
+        for params, grads, ms, vs, eight, device, group in work:
+            _step(params, grads, ms, vs, eight, device, group["step"], group["lr"], group["betas"], group["eps"],
+                  group["weight_decay"], self.max_grad_norm, norms.get(device))
+        return loss
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """As torch's, but moments keep their types (torch would convert them to the
+        parameters')."""
+        super().load_state_dict(state_dict)
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        mine = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(saved, mine):
+            for name, value in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(value):
+                    self.state[p][name] = value.to(p.device, copy=True).contiguous()
+        for group in self.param_groups:
+            if torch.is_tensor(group.get("step")):
+                group["step"] = group["step"].to(group["params"][0].device, copy=True)

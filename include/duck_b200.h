@@ -462,6 +462,42 @@ int duck_gated_recurrence_backward(const duck_recurrence *args, duck_stream stre
  * resets is [E]. */
 int duck_gated_recurrence_step(const duck_recurrence *args, duck_stream stream);
 
+/* AdamW over many tensors (the Python side is duck_gym_b200/optim.py).  A tensor
+ * has n dense values of `type`; its gradient has the same.  Moments are float32
+ * [n], or (bits = 8) codes [n], int8 for exp_avg and uint8 for exp_avg_sq, with one
+ * exponent byte per 128 values: a value's float32 has the leading 12 bits
+ * |code| + max(0, 8 exponent + 8 - most), most = 127 and 255; code 0 is 0, and
+ * exponent 255 makes its values NaN.  `place` is the tensor's place in the caller's
+ * list, which random roundings (of codes and of bfloat16 parameters) depend on. */
+typedef struct duck_adamw_tensor {
+  void *param;
+  const void *grad;
+  void *exp_avg, *exp_avg_sq;
+  uint8_t *exp_avg_exponents, *exp_avg_sq_exponents;
+  int64_t n;
+  int32_t type, place;
+} duck_adamw_tensor;
+typedef struct duck_adamw {
+  int64_t *step;              /* device: steps done, counted up by the call; its high half is used meanwhile */
+  const float *rate;          /* device: learning rate, or NULL for rate_value */
+  const double *sums;         /* of the gradients' squares (duck_gradient_squares), sum_count of them */
+  double rate_value, beta1, beta2, eps, weight_decay, max_norm;
+  int32_t sum_count;          /* 0: gradients are taken as they are */
+  int32_t bits;               /* of the moments, 8 or 32 */
+} duck_adamw;
+
+/* Sums of the gradients' squares in device memory, at most DUCK_GRADIENT_SUMS,
+ * added to the first `before` that are there already; *sum_count says how many there
+ * are then.  Only grad, n and type of a tensor are looked at. */
+enum { DUCK_GRADIENT_SUMS = 592 };
+int duck_gradient_squares(const duck_adamw_tensor *tensors, int count, int before, double *sums, int *sum_count,
+                          duck_stream stream);
+/* One step.  The arrays of the tensors are read on the host during the call. */
+int duck_adamw_step(const duck_adamw_tensor *tensors, int count, const duck_adamw *options, duck_stream stream);
+/* Values of moments in 8 bits, as float32 [n] in param: of exp_avg or of
+ * exp_avg_sq, the other being NULL. */
+int duck_moment_values(const duck_adamw_tensor *tensors, int count, duck_stream stream);
+
 /* No reference counterpart.  FP32 fused-multiply-add throughput probe used
  * as the roofline denominator: runs `iterations` dependent FMA chains on
  * every SM and returns achieved TFLOP/s (2 flops per FMA) in *tflops. */

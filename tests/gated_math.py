@@ -28,3 +28,34 @@ def recurrence(gates, values, state, resets, dout=None, dlast=None):
         dg[t] = dh * (before[t] - c[t]) * f[t] * rest[t]
         x = torch.where(cut[t][:, None], torch.zeros_like(x), dh * f[t])
     return out, h, dg, dc, x
+
+
+def adamw(p, g, m, v, t, lr, betas, eps, weight_decay, clip=1.0):
+    """New (p, m, v) of one tensor after step number t."""
+    p, g, m, v = (x.double() for x in (p, g, m, v))
+    g = g * clip
+    m, v = betas[0] * m + (1 - betas[0]) * g, betas[1] * v + (1 - betas[1]) * g * g
+    step = m / (1 - betas[0] ** t) / ((v / (1 - betas[1] ** t)).sqrt() + eps)
+    return p - lr * weight_decay * p - lr * step, m, v
+
+
+def hashed(t, place, n):
+    """The random bits of the first n values of the place-th tensor at step t."""
+    def mix(x):
+        x = (x ^ x >> 16) * 0x85EBCA6B % 2**32
+        x = (x ^ x >> 13) * 0xC2B2AE35 % 2**32
+        return x ^ x >> 16
+    key = mix((t + 0x9E3779B9 * (place + 1)) % 2**32)
+    return [mix(key ^ i) for i in range(n)]
+
+
+def code_values(codes, exponents):
+    """What a moment in 8 bits stands for, value by value: an octave and eighths."""
+    most, flat = 127 if codes.dtype == torch.int8 else 255, codes.reshape(-1).tolist()
+    out = []
+    for i, c in enumerate(flat):
+        e = int(exponents[i // 128])
+        octave, eighths = divmod(abs(c) + max(0, 8 * e + 8 - most), 8)
+        value = 2.0 ** (octave - 127) * (1 + eighths / 8) if octave else eighths * 2.0 ** -129
+        out.append(float("nan") if e == 255 else 0.0 if c == 0 else value if c > 0 else -value)
+    return torch.tensor(out, dtype=torch.float64).view(codes.shape)
