@@ -1,0 +1,667 @@
+// Gated linear layer: two projections of the same rows, one of them through an
+// activation, multiplied.
+//
+//   a = x Wg^T + bg,  u = x Wu^T + bu,  h = act(a) u
+//   da = dh u act'(a),  du = dh act(a)
+//   dx = da Wg + du Wu,  dWg = da^T x,  dWu = du^T x,  dbg = sum of da,  dbu = sum of du
+//
+// bfloat16 (gatedTiles): products on the tensor cores, operands by the TMA into a
+// ring of shared memory tiles, accumulators in tensor memory.  Both projections of
+// a tile are one product, the rows of Wg and of Wu side by side as its columns, and
+// leave tensor memory together, so that a and u are never in memory.  The backward
+// pass computes them again (a third more products than from stored ones), in
+// float32, and rounds da and du once: a and u as bfloat16 would add two roundings to
+// each, and their two arrays cost as much memory as the layer's output twice.  So
+// forward passes keep x only.
+//
+// One block a multiprocessor goes through tiles of 128 rows: one thread issues the
+// copies, one the products, eight warps take finished accumulators out, while the
+// products of the next tile go to the other half of tensor memory.
+//
+// float32 (gatedProducts): FMA in pairs; a and u are kept, since they are exact and
+// their products are what the time goes to.
+#pragma once
+#include "numeric_types.cuh"
+#include "umma.cuh"
+
+#include <type_traits>
+
+namespace duckb200 {
+
+enum Activation { kSilu = 0, kGelu = 1, kSigmoid = 2 };
+
+struct Activated {
+  float y, slope;
+};
+// act(a) and its derivative.  FAST: the exponential and the quotient of the
+// hardware (2^-21), for results that are rounded to bfloat16.
+template <int ACT, bool FAST> __device__ __forceinline__ Activated activate(float a) {
+  if constexpr (ACT == kGelu) {
+    const float below = 0.5f * (1.f + erff(a * 0.70710678f));
+    const float density = 0.39894228f * (FAST ? __expf(-0.5f * a * a) : expf(-0.5f * a * a));
+    return {a * below, below + a * density};
+  } else {
+    const float s = FAST ? __fdividef(1.f, 1.f + __expf(-a)) : 1.f / (1.f + expf(-a));
+    const float rest = FAST ? 1.f - s : 1.f / (1.f + expf(a));
+    if constexpr (ACT == kSilu) return {a * s, s + a * s * rest};
+    else return {s, s * rest};
+  }
+}
+template <class F> __device__ __forceinline__ void withActivation(int kind, F &&f) {
+  if (kind == kSilu) f(std::integral_constant<int, kSilu>());
+  else if (kind == kGelu) f(std::integral_constant<int, kGelu>());
+  else f(std::integral_constant<int, kSigmoid>());
+}
+
+// ------------------------------------------------------------------- bfloat16
+// What a pass of gatedTiles computes.
+enum class Pass {
+  forward,     // h
+  gradients,   // da and du, from x, the weights and dh
+  input,       // dx
+  weights      // dWg and dWu, or parts of them
+};
+
+struct TileArgs {
+  const bf16 *bGate, *bUp;   // or null
+  bf16 *h;                   // forward
+  const bf16 *dh;            // gradients
+  bf16 *both;                // [rows, 2, stride]: da and du
+  float *biasParts;          // [128-row tiles x 4, 2, F]: sums over 32 rows, or null
+  bf16 *dx;                  // input
+  bf16 *dwGate, *dwUp;       // weights, where they are not split
+  float *parts;              // [splits, 2, F, D]
+  int64_t rows, dhStride;
+  int D, F, stride, activation;
+  int tiles, columnTiles, rowTiles, splits, steps;   // steps of 64 of a tile's product
+  bool wholeH, wholeDh;      // rows of 16-byte pieces
+};
+struct TileMaps {
+  CUtensorMap a0, a1, b0, b1;
+};
+
+constexpr int kTileThreads = 384, kTileRows = 128, kTileSteps = 64, kTileWarps = 8;
+template <int BN> struct TileShared {
+  static constexpr int stages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int a = kTileRows * kTileSteps * 2, b = BN * kTileSteps * 2;
+  static constexpr int staging = 32 * 64, bias = 2 * 32 * 4;   // of a warp
+  static constexpr int bytes = 1024 + stages * (a + b) + kTileWarps * (staging + bias) + 256;
+};
+
+// A warp's 32 rows of 64 bytes: pieces of 16 bytes, so placed that neither rows of
+// pieces nor columns of them meet in a bank.
+__device__ __forceinline__ uint4 *stagedPiece(uint4 *staging, int row, int piece) {
+  return staging + row * 4 + (piece ^ (row >> 1 & 3));
+}
+
+// Column sums over the 32 lanes: lane i is left with column i's.
+__device__ __forceinline__ float columnSum(float (&x)[32], int lane) {
+#pragma unroll
+  for (int half = 16; half > 0; half /= 2) {
+    const bool upper = lane & half;
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float send = upper ? x[i] : x[i + half], keep = upper ? x[i + half] : x[i];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, half);
+    }
+  }
+  return x[0];
+}
+
+// A warp's rows of 32 bfloat16 columns, one row a lane, to memory: `columns` of them
+// exist; whole pieces where rows are made of them.
+__device__ __forceinline__ void storeRows(uint4 *staging, const float (&x)[32], bf16 *to, int64_t rowStride, int64_t rowsLeft,
+                                          int columns, bool pieces, int lane) {
+#pragma unroll
+  for (int piece = 0; piece < 4; ++piece) {
+    uint4 v;
+    uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 two = __floats2bfloat162_rn(x[piece * 8 + 2 * i], x[piece * 8 + 2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&two);
+    }
+    *stagedPiece(staging, lane, piece) = v;
+  }
+  __syncwarp();
+  const int piece = lane % 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = lane / 4 + 8 * i;
+    if (row >= rowsLeft || piece * 8 >= columns) continue;
+    const uint4 v = *stagedPiece(staging, row, piece);
+    bf16 *at = to + row * rowStride + piece * 8;
+    if (pieces && piece * 8 + 8 <= columns) {
+      *reinterpret_cast<uint4 *>(at) = v;
+    } else {
+      const bf16 *e = reinterpret_cast<const bf16 *>(&v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (piece * 8 + j < columns) at[j] = e[j];
+    }
+  }
+  __syncwarp();
+}
+
+template <Pass PASS, int BN> __global__ void __launch_bounds__(kTileThreads, 1)
+gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
+  using S = TileShared<BN>;
+  constexpr bool kDual = PASS == Pass::forward || PASS == Pass::gradients;
+  constexpr bool kAlongA = PASS != Pass::weights, kAlongB = kDual;
+  constexpr int kColumns = kDual ? BN / 2 : BN;   // of the output that a tile has
+  extern __shared__ uint8_t raw[];
+  uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *tileA = base, *tileB = base + S::stages * S::a;
+  uint8_t *staging = tileB + S::stages * S::b;
+  float *biases = reinterpret_cast<float *>(staging + kTileWarps * S::staging);
+  uint64_t *full = reinterpret_cast<uint64_t *>(biases + kTileWarps * S::bias / 4);
+  uint64_t *empty = full + S::stages, *done = empty + S::stages, *taken = done + 2;
+  uint32_t *tensor = reinterpret_cast<uint32_t *>(taken + 2);
+  volatile int *broken = reinterpret_cast<volatile int *>(tensor + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    *broken = 0;
+    for (int i = 0; i < S::stages; ++i) barrierInit(full + i, 1), barrierInit(empty + i, 1);
+    for (int i = 0; i < 2; ++i) barrierInit(done + i, 1), barrierInit(taken + i, kTileWarps);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 2) tensorAllocate(tensor, 2 * BN);
+  tensorFenceBefore();
+  __syncthreads();
+  tensorFenceAfter();
+  const uint32_t accumulators = *tensor;
+
+  // Where a tile lies.
+  struct Tile {
+    int row, column, split, half;   // first output row (of Wg or Wu: half 1) and column
+  };
+  auto tileAt = [&](int t) {
+    Tile at{};
+    const int column = t % p.columnTiles, rest = t / p.columnTiles;
+    at.column = column * kColumns;
+    if constexpr (PASS == Pass::weights) {
+      const int row = rest % (2 * p.rowTiles);
+      at.split = rest / (2 * p.rowTiles);
+      at.half = row >= p.rowTiles;
+      at.row = (row - at.half * p.rowTiles) * kTileRows;
+    } else {
+      at.row = rest * kTileRows;
+    }
+    return at;
+  };
+  auto stepsOf = [&](const Tile &at, int &first) {
+    if constexpr (PASS == Pass::weights) {
+      const int each = (p.steps + p.splits - 1) / p.splits;
+      first = at.split * each;
+      return max(0, min(p.steps, first + each) - first);
+    } else if constexpr (PASS == Pass::input) {
+      first = 0;
+      return 2 * p.steps;
+    } else {
+      first = 0;
+      return p.steps;
+    }
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetchMap(&maps.a0);
+      prefetchMap(&maps.b0);
+      int stage = 0, issued = 0;
+      uint32_t parity = 0;
+      bool fine = true;
+      for (int t = blockIdx.x; t < p.tiles && fine; t += gridDim.x) {
+        const Tile at = tileAt(t);
+        int first;
+        const int steps = stepsOf(at, first);
+        for (int k = 0; k < steps; ++k) {
+          fine = barrierWait(empty + stage, parity ^ 1, broken);
+          if (!fine) break;
+          uint64_t *bar = full + stage;
+          uint8_t *a = tileA + stage * S::a, *b = tileB + stage * S::b;
+          barrierExpect(bar, S::a + S::b);
+          if constexpr (kDual) {
+            const int x = k * kTileSteps;
+            copyBox(a, &maps.a0, x, at.row, bar);
+            copyBox(b, &maps.b0, x, at.column, bar);
+            copyBox(b + S::b / 2, &maps.b1, x, at.column, bar);
+          } else if constexpr (PASS == Pass::input) {
+            const bool up = k >= p.steps;
+            const int x = (up ? k - p.steps : k) * kTileSteps;
+            copyBox(a, up ? &maps.a1 : &maps.a0, x, at.row, bar);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) copyBox(b + j * 8192, up ? &maps.b1 : &maps.b0, at.column + 64 * j, x, bar);
+          } else {
+            const int y = (first + k) * kTileSteps;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) copyBox(a + j * 8192, at.half ? &maps.a1 : &maps.a0, at.row + 64 * j, y, bar);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) copyBox(b + j * 8192, &maps.b0, at.column + 64 * j, y, bar);
+          }
+          issued = min(issued + 1, S::stages);
+          if (++stage == S::stages) stage = 0, parity ^= 1;
+        }
+      }
+      // Given up: the copies in flight come to their end before the block does.
+      for (int i = 0; !fine && i < issued; ++i) {
+        if (--stage < 0) stage = S::stages - 1, parity ^= 1;
+        int none = 0;
+        barrierWait(full + stage, parity, &none);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, n = 0;
+      uint32_t parity = 0;
+      bool fine = true;
+      constexpr uint32_t shape = productShape(BN, kAlongA, kAlongB);
+      for (int t = blockIdx.x; t < p.tiles && fine; t += gridDim.x, ++n) {
+        const Tile at = tileAt(t);
+        int first;
+        const int steps = stepsOf(at, first), buffer = n & 1;
+        fine = barrierWait(taken + buffer, (n >> 1 & 1) ^ 1, broken);
+        tensorFenceAfter();
+        for (int k = 0; k < steps && fine; ++k) {
+          fine = barrierWait(full + stage, parity, broken);
+          if (!fine) break;
+          tensorFenceAfter();
+          const uint64_t a = operandDescriptor<kAlongA>(sharedAddress(tileA + stage * S::a));
+          const uint64_t b = operandDescriptor<kAlongB>(sharedAddress(tileB + stage * S::b));
+#pragma unroll
+          for (int i = 0; i < kTileSteps / 16; ++i)
+            tensorProduct(accumulators + buffer * BN, a + i * kDescriptorStep<kAlongA>, b + i * kDescriptorStep<kAlongB>, shape,
+                          k > 0 || i > 0);
+          tensorCommit(empty + stage);
+          if (++stage == S::stages) stage = 0, parity ^= 1;
+        }
+        if (fine) tensorCommit(done + buffer);
+      }
+    }
+  } else if (warp >= 4) {
+    const int quarter = warp % 4, half = (warp - 4) / 4;   // of the tile's rows, and of its columns
+    uint4 *stage = reinterpret_cast<uint4 *>(staging + (warp - 4) * S::staging);
+    float *bias = biases + (warp - 4) * S::bias / 4;
+    int n = 0;
+    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++n) {
+      const Tile at = tileAt(t);
+      const int buffer = n & 1;
+      int first;
+      const int steps = stepsOf(at, first);
+      const bool fine = __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken));
+      tensorFenceAfter();
+      const uint32_t tensorRow = accumulators + buffer * BN + (uint32_t(quarter * 32) << 16);
+      const int64_t row = at.row + quarter * 32;
+      const int64_t rowsLeft = (PASS == Pass::weights ? int64_t(p.F) : p.rows) - row;
+      constexpr int kChunk = kColumns / 2 < 32 ? kColumns / 2 : 32;
+      // 32 columns of the accumulators from `column` on (16 of them beyond kChunk's are not read); zero where a tile has no steps.
+      auto take = [&](float (&x)[32], int column) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = fine ? 0.f : __int_as_float(0x7fffffff);
+        if (fine && steps > 0) {
+          tensorLoad16(x, tensorRow + column);
+          if (kChunk > 16) tensorLoad16(x + 16, tensorRow + column + 16);
+        }
+      };
+      for (int c = half * (kColumns / 2); c < (half + 1) * (kColumns / 2); c += kChunk) {
+        const int column = at.column + c;
+        if constexpr (kDual) {
+          const int columns = min(kChunk, p.F - column);
+          if (columns <= 0) break;
+          float a[32], u[32];
+          take(a, c);
+          take(u, BN / 2 + c);
+          uint4 dh[4];
+          const bool mine = lane < rowsLeft;
+          if constexpr (PASS == Pass::gradients) {
+            const bf16 *from = p.dh + (row + lane) * p.dhStride + column;
+            if (p.wholeDh && columns == kChunk) {
+#pragma unroll
+              for (int i = 0; i < kChunk / 8; ++i) dh[i] = mine ? reinterpret_cast<const uint4 *>(from)[i] : make_uint4(0, 0, 0, 0);
+            } else {
+              bf16 *e = reinterpret_cast<bf16 *>(dh);
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i) e[i] = mine && i < columns ? from[i] : __ushort_as_bfloat16(0);
+            }
+          }
+          if (p.bGate) {
+            const bool in = lane < columns;
+            bias[lane] = in ? toFloat(p.bGate[column + lane]) : 0.f;
+            bias[32 + lane] = in ? toFloat(p.bUp[column + lane]) : 0.f;
+            __syncwarp();
+          }
+          tensorLoadWait();
+          tensorLoaded(a);
+          tensorLoaded(u);
+          if (p.bGate) {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) a[i] += bias[i], u[i] += bias[32 + i];
+            __syncwarp();
+          }
+          withActivation(p.activation, [&](auto kind) {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+              const Activated f = activate<kind.value, true>(a[i]);
+              if constexpr (PASS == Pass::forward) {
+                a[i] = f.y * u[i];
+              } else {
+                const float d = toFloat(reinterpret_cast<const bf16 *>(dh)[i]);
+                a[i] = d * u[i] * f.slope;
+                u[i] = d * f.y;
+              }
+            }
+          });
+          if constexpr (PASS == Pass::forward) {
+            storeRows(stage, a, p.h + row * p.F + column, p.F, rowsLeft, columns, p.wholeH, lane);
+          } else {
+            bf16 *to = p.both + row * 2 * p.stride + column;
+            storeRows(stage, a, to, 2 * int64_t(p.stride), rowsLeft, columns, true, lane);
+            storeRows(stage, u, to + p.stride, 2 * int64_t(p.stride), rowsLeft, columns, true, lane);
+            if (p.biasParts) {
+              if (!mine) {   // (a row that is not there may have become NaN beside an infinite bias)
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) a[i] = u[i] = 0.f;
+              }
+              if (kChunk < 32) {
+#pragma unroll
+                for (int i = kChunk; i < 32; ++i) a[i] = u[i] = 0.f;
+              }
+              const float sumA = columnSum(a, lane), sumU = columnSum(u, lane);
+              float *parts = p.biasParts + (int64_t(at.row / kTileRows) * 4 + quarter) * 2 * p.F + column;
+              if (lane < columns) parts[lane] = sumA, parts[p.F + lane] = sumU;
+            }
+          }
+        } else {
+          const int columns = min(kChunk, p.D - column);
+          if (columns <= 0) break;
+          float x[32];
+          take(x, c);
+          tensorLoadWait();
+          tensorLoaded(x);
+          if constexpr (PASS == Pass::input) {
+            storeRows(stage, x, p.dx + row * p.D + column, p.D, rowsLeft, columns, true, lane);
+          } else if (p.splits == 1) {
+            storeRows(stage, x, (at.half ? p.dwUp : p.dwGate) + row * p.D + column, p.D, rowsLeft, columns, true, lane);
+          } else {
+            float *to = p.parts + ((int64_t(at.split) * 2 + at.half) * p.F + row) * p.D + column;
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {   // 16 columns, 64 bytes of a row
+#pragma unroll
+              for (int piece = 0; piece < 4; ++piece) {
+                const float *v = x + part * 16 + piece * 4;
+                *reinterpret_cast<float4 *>(stagedPiece(stage, lane, piece)) = make_float4(v[0], v[1], v[2], v[3]);
+              }
+              __syncwarp();
+              const int piece = lane % 4;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = lane / 4 + 8 * i, at4 = part * 16 + piece * 4;   // (D is a multiple of 8)
+                if (r < rowsLeft && at4 < columns)
+                  *reinterpret_cast<float4 *>(to + int64_t(r) * p.D + at4) = *reinterpret_cast<float4 *>(stagedPiece(stage, r, piece));
+              }
+              __syncwarp();
+            }
+          }
+        }
+      }
+      tensorFenceBefore();
+      __syncwarp();
+      if (lane == 0) barrierArrive(taken + buffer);
+    }
+  }
+  tensorFenceBefore();
+  __syncthreads();
+  tensorFenceAfter();
+  if (warp == 2) tensorFree(accumulators, 2 * BN);
+}
+
+// -------------------------------------------------------------------- float32
+// Tiles of 128 rows and 128 columns, 16 steps at a time, 8 by 8 values a thread as
+// pairs; the operands of the next steps are on their way in registers.  The forward
+// pass's columns are 64 of Wg and the same 64 of Wu: a thread has both of a value.
+struct ProductArgs {
+  const float *x, *wGate, *wUp, *bGate, *bUp;
+  float *h, *kept;             // forward: h, and a and u [2, rows, F] or null
+  const float *both;           // [2, rows, F]: da and du
+  float *dx, *parts;           // [splits, 2, F, D]
+  int64_t rows, xStride;
+  int D, F, activation, splits;
+  bool wholeX, wholeD, wholeF;   // rows of x, of D and of F values are 16-byte pieces
+};
+constexpr int kProductThreads = 256, kProductTile = 128, kProductSteps = 16, kProductPitch = kProductTile + 4;
+
+// The first `count` of four values.
+__device__ __forceinline__ float4 fetchFour(const float *p, int64_t count, bool whole) {
+  if (count >= 4 && whole) return *reinterpret_cast<const float4 *>(p);
+  return make_float4(count > 0 ? p[0] : 0.f, count > 1 ? p[1] : 0.f, count > 2 ? p[2] : 0.f, count > 3 ? p[3] : 0.f);
+}
+using Two = unsigned long long;
+__device__ __forceinline__ Two twoOf(float a, float b) {
+  Two p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ float2 partsOf(Two p) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void addProduct(Two &d, Two a, Two b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
+}
+
+template <Pass PASS> __global__ void __launch_bounds__(kProductThreads, 2) gatedProducts(ProductArgs p) {
+  static_assert(PASS != Pass::gradients, "gatedGradients");
+  constexpr int T = kProductTile, K = kProductSteps, P = kProductPitch;
+  constexpr bool kAlongA = PASS != Pass::weights, kAlongB = PASS == Pass::forward;   // steps are contiguous
+  __shared__ __align__(16) float as[2][K][P], bs[2][K][P];
+  const int tid = threadIdx.x;
+  const int64_t row0 = int64_t(blockIdx.y) * T;   // weights: of Wg's and then Wu's tiles
+  const int rowTiles = (p.F + T - 1) / T;
+  const int half = PASS == Pass::weights && int(blockIdx.y) >= rowTiles;
+  const int64_t m0 = PASS == Pass::weights ? row0 - int64_t(half) * rowTiles * T : row0;
+  const int n0 = blockIdx.x * (PASS == Pass::forward ? T / 2 : T);
+  const int64_t plane = p.rows * p.F;
+  const int halfSteps = (p.F + K - 1) / K;   // input: steps of the first product, then those of the second
+  const int64_t allSteps = PASS == Pass::forward ? (p.D + K - 1) / K : PASS == Pass::input ? 2 * halfSteps : (p.rows + K - 1) / K;
+  const int64_t each = (allSteps + p.splits - 1) / p.splits;
+  const int64_t first = PASS == Pass::weights ? blockIdx.z * each : 0;
+  const int64_t last = PASS == Pass::weights ? min(allSteps, first + each) : allSteps;
+
+  auto fetchA = [&](int64_t step, int i) {
+    const int at = tid + i * kProductThreads;
+    if constexpr (PASS == Pass::forward) {
+      const int64_t m = m0 + at / 4, k = step * K + at % 4 * 4;
+      return fetchFour(p.x + m * p.xStride + k, m < p.rows ? p.D - k : 0, p.wholeX);
+    } else if constexpr (PASS == Pass::input) {
+      const bool up = step >= halfSteps;
+      const int64_t m = m0 + at / 4, k = (step - (up ? halfSteps : 0)) * K + at % 4 * 4;
+      return fetchFour(p.both + (up ? plane : 0) + m * p.F + k, m < p.rows ? p.F - k : 0, p.wholeF);
+    } else {
+      const int64_t k = step * K + at / 32, m = m0 + at % 32 * 4;
+      return fetchFour(p.both + (half ? plane : 0) + k * p.F + m, k < p.rows ? p.F - m : 0, p.wholeF);
+    }
+  };
+  auto fetchB = [&](int64_t step, int i) {
+    const int at = tid + i * kProductThreads;
+    if constexpr (PASS == Pass::forward) {
+      const int row = at / 4, f = n0 + row % (T / 2);
+      const int64_t k = step * K + at % 4 * 4;
+      return fetchFour((row < T / 2 ? p.wGate : p.wUp) + int64_t(f) * p.D + k, f < p.F ? p.D - k : 0, p.wholeD);
+    } else if constexpr (PASS == Pass::input) {
+      const bool up = step >= halfSteps;
+      const int64_t k = (step - (up ? halfSteps : 0)) * K + at / 32, n = n0 + at % 32 * 4;
+      return fetchFour((up ? p.wUp : p.wGate) + k * p.D + n, k < p.F ? p.D - n : 0, p.wholeD);
+    } else {
+      const int64_t k = step * K + at / 32, n = n0 + at % 32 * 4;
+      return fetchFour(p.x + k * p.xStride + n, k < p.rows ? p.D - n : 0, p.wholeX);
+    }
+  };
+  auto put = [&](float (&tile)[K][P], bool along, int i, float4 v) {
+    const int at = tid + i * kProductThreads;
+    if (along) {
+      const int row = at / 4, k = at % 4 * 4;
+      tile[k][row] = v.x, tile[k + 1][row] = v.y, tile[k + 2][row] = v.z, tile[k + 3][row] = v.w;
+    } else {
+      *reinterpret_cast<float4 *>(&tile[at / 32][at % 32 * 4]) = v;
+    }
+  };
+
+  const int ty = tid / 16, tx = tid % 16;
+  Two sum[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[i][j] = 0;
+  float4 a[2], b[2];
+  if (first < last) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) put(as[0], kAlongA, i, fetchA(first, i)), put(bs[0], kAlongB, i, fetchB(first, i));
+  }
+  __syncthreads();
+  for (int64_t step = first; step < last; ++step) {
+    const int now = int(step - first) & 1;
+    if (step + 1 < last) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) a[i] = fetchA(step + 1, i), b[i] = fetchB(step + 1, i);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float4 a0 = *reinterpret_cast<const float4 *>(&as[now][k][ty * 4]);
+      const float4 a1 = *reinterpret_cast<const float4 *>(&as[now][k][64 + ty * 4]);
+      const ulonglong2 b0 = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][tx * 4]);
+      const ulonglong2 b1 = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][64 + tx * 4]);
+      const float rows[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const Two r = twoOf(rows[i], rows[i]);
+        addProduct(sum[i][0], r, b0.x);
+        addProduct(sum[i][1], r, b0.y);
+        addProduct(sum[i][2], r, b1.x);
+        addProduct(sum[i][3], r, b1.y);
+      }
+    }
+    if (step + 1 < last) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) put(as[now ^ 1], kAlongA, i, a[i]), put(bs[now ^ 1], kAlongB, i, b[i]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t m = m0 + (i / 4) * 64 + ty * 4 + i % 4;
+    if (m >= (PASS == Pass::weights ? int64_t(p.F) : p.rows)) continue;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 two = partsOf(sum[i][j]);
+      v[2 * j] = two.x, v[2 * j + 1] = two.y;
+    }
+    if constexpr (PASS == Pass::forward) {
+      const int f = n0 + tx * 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (f + j >= p.F) break;
+        float gate = v[j], up = v[4 + j];
+        if (p.bGate) gate += p.bGate[f + j], up += p.bUp[f + j];
+        const int64_t at = m * p.F + f + j;
+        if (p.kept) p.kept[at] = gate, p.kept[plane + at] = up;
+        withActivation(p.activation, [&](auto kind) { p.h[at] = activate<kind.value, false>(gate).y * up; });
+      }
+    } else {
+      float *to = PASS == Pass::input ? p.dx + m * p.D : p.parts + ((int64_t(blockIdx.z) * 2 + half) * p.F + m) * p.D;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int n = n0 + (j / 4) * 64 + tx * 4 + j % 4;
+        if (n < p.D) to[n] = v[j];
+      }
+    }
+  }
+}
+
+// da and du from what the forward pass kept, and sums over kGradientRows rows for
+// the biases' gradients.  A warp has 32 columns of every eighth row.
+struct GradientArgs {
+  const float *kept, *dh;
+  float *both, *biasParts;   // [row blocks, 2, F] or null
+  int64_t rows, dhStride;
+  int F, activation;
+};
+constexpr int kGradientRows = 64;
+__global__ void __launch_bounds__(256) gatedGradients(GradientArgs p) {
+  __shared__ float sums[8][2][32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, f = blockIdx.x * 32 + lane;
+  const int64_t row0 = int64_t(blockIdx.y) * kGradientRows, plane = p.rows * p.F;
+  float sumA = 0.f, sumU = 0.f;
+  if (f < p.F)
+    withActivation(p.activation, [&](auto kind) {
+#pragma unroll 4
+      for (int r = warp; r < kGradientRows; r += 8) {
+        const int64_t row = row0 + r, at = row * p.F + f;
+        if (row >= p.rows) break;
+        const float d = p.dh[row * p.dhStride + f], u = p.kept[plane + at];
+        const Activated y = activate<kind.value, false>(p.kept[at]);
+        const float da = d * u * y.slope, du = d * y.y;
+        p.both[at] = da, p.both[plane + at] = du;
+        sumA += da, sumU += du;
+      }
+    });
+  if (!p.biasParts) return;
+  sums[warp][0][lane] = sumA, sums[warp][1][lane] = sumU;
+  __syncthreads();
+  if (warp >= 2 || f >= p.F) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += sums[w][warp][lane];
+  p.biasParts[(int64_t(blockIdx.y) * 2 + warp) * p.F + f] = sum;
+}
+
+// -------------------------------------------------------------- sums of parts
+// out[i] = sum over n of parts[n, i], in float32, to the layer's type; the first
+// `count` values to one array, the next to another.  Bias sums likewise.
+template <class T> struct SumArgs {
+  const float *parts, *biasParts;
+  T *dwGate, *dwUp, *dbGate, *dbUp;
+  int64_t weights;   // F * D
+  int F, splits, biasCount, weightBlocks;
+};
+constexpr int kSumThreads = 256;
+template <class T> __global__ void __launch_bounds__(kSumThreads) sumParts(SumArgs<T> p) {
+  if (int(blockIdx.x) < p.weightBlocks) {
+    const int64_t i = (int64_t(blockIdx.x) * kSumThreads + threadIdx.x) * 4;
+    if (i >= 2 * p.weights) return;
+    if (p.weights % 4 == 0) {
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int n = 0; n < p.splits; ++n) {
+        const float4 v = *reinterpret_cast<const float4 *>(p.parts + n * 2 * p.weights + i);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      T *to = i < p.weights ? p.dwGate + i : p.dwUp + (i - p.weights);
+      to[0] = fromFloat<T>(sum.x), to[1] = fromFloat<T>(sum.y), to[2] = fromFloat<T>(sum.z), to[3] = fromFloat<T>(sum.w);
+    } else {
+      for (int64_t j = i; j < i + 4 && j < 2 * p.weights; ++j) {
+        float sum = 0.f;
+        for (int n = 0; n < p.splits; ++n) sum += p.parts[n * 2 * p.weights + j];
+        (j < p.weights ? p.dwGate[j] : p.dwUp[j - p.weights]) = fromFloat<T>(sum);
+      }
+    }
+    return;
+  }
+  // Biases: a warp has 32 columns, the block's eight warps share the parts.
+  __shared__ float sums[kSumThreads / 32][32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, column = (int(blockIdx.x) - p.weightBlocks) * 32 + lane;
+  float sum = 0.f;
+  if (column < 2 * p.F)
+#pragma unroll 8
+    for (int n = warp; n < p.biasCount; n += kSumThreads / 32) sum += p.biasParts[int64_t(n) * 2 * p.F + column];
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (warp > 0 || column >= 2 * p.F) return;
+#pragma unroll
+  for (int w = 1; w < kSumThreads / 32; ++w) sum += sums[w][lane];
+  (column < p.F ? p.dbGate[column] : p.dbUp[column - p.F]) = fromFloat<T>(sum);
+}
+
+}  // namespace duckb200

@@ -1,9 +1,11 @@
-// C entries of the gated recurrence (declared in include/duck_b200.h): argument
-// checks, the choice of a kernel, launches.
+// C entries of the gated recurrence and of the gated linear layer (declared in
+// include/duck_b200.h): argument checks, the choice of a kernel, launches.
 #include "capi.hpp"
+#include "gated_linear.cuh"
 #include "gated_recurrence.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 
 using namespace duckb200;
@@ -94,9 +96,306 @@ template <class T, int V> void launchBackward(const RecurrenceArgs &r, cudaStrea
   recurrenceBackward<T, V><<<recurrenceGrid(channels, V, r.segmentCount), kRecurrenceThreads, 0, stream>>>(r);
 }
 
+// ---------------------------------------------------------------- gated linear
+bool gatedChecked(const duck_gated *a) {
+  require(a != nullptr, "Invalid arguments");
+  requireType(a->type);
+  require(a->rows >= 0 && a->D > 0 && a->F > 0, "Invalid layer sizes");
+  require(a->rows < (int64_t(1) << 31) - 4096 && a->D <= (1 << 24) && a->F <= (1 << 24), "Too many rows or columns");
+  require(a->activation >= DUCK_SILU && a->activation <= DUCK_SIGMOID, "Invalid activation");
+  require(a->type == DUCK_FLOAT32 || a->D % 8 == 0, "bfloat16 rows have to be whole 16-byte pieces");
+  return a->rows > 0;
+}
+
+// How a backward call's workspace is laid out.
+struct GatedPlan {
+  int stride;                // bfloat16: of da and du
+  int weightColumns;         // of a tile of the weights' gradients
+  int splits;                // of the rows, for the weights' gradients
+  int64_t biasCount;
+  int64_t bothBytes, biasBytes, partBytes, keptBytes;
+};
+int64_t padded(int64_t bytes) { return ceilDiv(bytes, 256) * 256; }
+// As wide a tile as there are columns for.
+int tileColumns(int64_t columns) { return columns > 128 ? 256 : columns > 64 ? 128 : 64; }
+GatedPlan planGated(const duck_gated &a) {
+  GatedPlan p{};
+  const bool weights = a.dw_gate != nullptr, biases = a.db_gate != nullptr;
+  const int64_t rows = a.rows;
+  if (a.type == DUCK_BFLOAT16) {
+    p.stride = int(ceilDiv(a.F, 8) * 8);
+    p.bothBytes = padded(rows * 2 * p.stride * 2);
+    p.biasCount = ceilDiv(rows, kTileRows) * 4;
+    p.weightColumns = tileColumns(a.D);
+    // Rows are split so that the tiles fill the GPU once, into parts of 512 rows at least: a part's sums are written and read once more.
+    const int64_t tiles = 2 * ceilDiv(a.F, kTileRows) * ceilDiv(a.D, p.weightColumns), steps = ceilDiv(rows, kTileSteps);
+    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(148 / tiles, steps / 8)));
+    p.splits = int(std::max<int64_t>(1, ceilDiv(steps, std::max<int64_t>(1, ceilDiv(steps, p.splits)))));
+  } else {
+    p.bothBytes = padded(rows * 2 * a.F * 4);
+    p.keptBytes = rows * 2 * a.F * 4;
+    p.biasCount = ceilDiv(rows, kGradientRows);
+    const int64_t tiles = 2 * ceilDiv(a.F, kProductTile) * ceilDiv(a.D, kProductTile), steps = ceilDiv(rows, kProductSteps);
+    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(2 * 148 / tiles, steps / 16)));
+    p.splits = int(std::max<int64_t>(1, ceilDiv(steps, std::max<int64_t>(1, ceilDiv(steps, p.splits)))));
+  }
+  if (biases) p.biasBytes = padded(p.biasCount * 2 * a.F * 4);
+  if (weights && (a.type == DUCK_FLOAT32 || p.splits > 1)) p.partBytes = padded(int64_t(p.splits) * 2 * a.F * a.D * 4);
+  return p;
+}
+
+// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device
+// (by whichever thread comes first: autograd calls from its own).
+template <auto kernel> void allowShared(int bytes) {
+  static std::atomic<bool> done[64] = {};
+  int device = 0;
+  check(cudaGetDevice(&device), "cudaGetDevice");
+  if (device < 64 && done[device]) return;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  if (device < 64) done[device] = true;
+}
+
+// A map over bfloat16 rows for boxes of 64 values by boxRows rows.
+CUtensorMap mapOf(const void *base, int64_t columns, int64_t rows, int64_t stride, int boxRows) {
+  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void *entry = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    check(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &found),
+          "cuTensorMapEncodeTiled");
+    if (found != cudaDriverEntryPointSuccess || !entry) throw CudaError("cuTensorMapEncodeTiled: not in the driver");
+    return reinterpret_cast<Encode>(entry);
+  }();
+  CUtensorMap map;
+  const cuuint64_t sizes[2] = {cuuint64_t(columns), cuuint64_t(rows)}, strides[1] = {cuuint64_t(stride) * 2};
+  const cuuint32_t box[2] = {64, cuuint32_t(boxRows)}, steps[2] = {1, 1};
+  auto fill = [&] {
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), sizes, strides, box, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult status = fill();
+  if (status == CUDA_ERROR_INVALID_CONTEXT || status == CUDA_ERROR_NOT_INITIALIZED) {
+    // A thread's first call, before any that made its device's context current (autograd has threads of its own).
+    int device = 0;
+    check(cudaGetDevice(&device), "cudaGetDevice");
+    check(cudaSetDevice(device), "cudaSetDevice");
+    status = fill();
+  }
+  require(status != CUDA_ERROR_INVALID_VALUE, "Rows have to be whole 16-byte pieces on 16-byte boundaries");
+  if (status != CUDA_SUCCESS) throw CudaError("cuTensorMapEncodeTiled: error " + std::to_string(int(status)));
+  return map;
+}
+
+template <Pass PASS, int BN> void launchTiles(const TileMaps &maps, const TileArgs &t, cudaStream_t stream) {
+  constexpr auto kernel = gatedTiles<PASS, BN>;
+  allowShared<kernel>(TileShared<BN>::bytes);
+  kernel<<<std::min(t.tiles, 148), kTileThreads, TileShared<BN>::bytes, stream>>>(maps, t);
+  check(cudaGetLastError(), "gated linear launch");
+}
+
+// Both projections' tiles: as wide as leaves one for every multiprocessor.
+template <Pass PASS> void launchProjections(const duck_gated &a, TileArgs t, cudaStream_t stream) {
+  const int64_t rowTiles = ceilDiv(a.rows, kTileRows);
+  auto run = [&](auto columns) {
+    constexpr int BN = columns.value;
+    TileMaps maps;
+    maps.a0 = maps.a1 = mapOf(a.x, a.D, a.rows, a.x_stride, kTileRows);
+    maps.b0 = mapOf(a.w_gate, a.D, a.F, a.D, BN / 2);
+    maps.b1 = mapOf(a.w_up, a.D, a.F, a.D, BN / 2);
+    t.steps = int(ceilDiv(a.D, kTileSteps));
+    t.columnTiles = int(ceilDiv(a.F, BN / 2));
+    const int64_t tiles = rowTiles * t.columnTiles;
+    require(tiles < (int64_t(1) << 31), "Too many rows and columns");
+    t.tiles = int(tiles);
+    launchTiles<PASS, BN>(maps, t, stream);
+  };
+  if (rowTiles * ceilDiv(a.F, 128) >= 148) run(std::integral_constant<int, 256>());
+  else if (rowTiles * ceilDiv(a.F, 64) >= 148) run(std::integral_constant<int, 128>());
+  else run(std::integral_constant<int, 64>());
+}
+template <class F> void withColumns(int columns, F &&f) {
+  if (columns == 256) f(std::integral_constant<int, 256>());
+  else if (columns == 128) f(std::integral_constant<int, 128>());
+  else f(std::integral_constant<int, 64>());
+}
+
+TileArgs tileArgs(const duck_gated &a) {
+  TileArgs t{};
+  t.bGate = static_cast<const bf16 *>(a.b_gate);
+  t.bUp = static_cast<const bf16 *>(a.b_up);
+  t.rows = a.rows, t.D = a.D, t.F = a.F, t.activation = a.activation;
+  t.splits = 1;
+  return t;
+}
+ProductArgs productArgs(const duck_gated &a) {
+  ProductArgs g{};
+  g.x = static_cast<const float *>(a.x);
+  g.wGate = static_cast<const float *>(a.w_gate);
+  g.wUp = static_cast<const float *>(a.w_up);
+  g.bGate = static_cast<const float *>(a.b_gate);
+  g.bUp = static_cast<const float *>(a.b_up);
+  g.rows = a.rows, g.xStride = a.x_stride, g.D = a.D, g.F = a.F, g.activation = a.activation, g.splits = 1;
+  g.wholeX = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 4 == 0;
+  g.wholeD = a.D % 4 == 0 && reinterpret_cast<uintptr_t>(a.w_gate) % 16 == 0 && reinterpret_cast<uintptr_t>(a.w_up) % 16 == 0;
+  g.wholeF = a.F % 4 == 0;
+  return g;
+}
+template <class T>
+void launchSums(const duck_gated &a, const GatedPlan &plan, const float *parts, const float *biasParts, cudaStream_t stream) {
+  SumArgs<T> s{parts, biasParts, static_cast<T *>(a.dw_gate), static_cast<T *>(a.dw_up), static_cast<T *>(a.db_gate),
+               static_cast<T *>(a.db_up), int64_t(a.F) * a.D, a.F, plan.splits, int(plan.biasCount), 0};
+  if (parts) s.weightBlocks = int(ceilDiv(2 * s.weights, kSumThreads * 4));
+  const int64_t blocks = s.weightBlocks + (biasParts ? ceilDiv(2 * int64_t(a.F), 32) : 0);
+  if (blocks == 0) return;
+  sumParts<T><<<unsigned(blocks), kSumThreads, 0, stream>>>(s);
+  check(cudaGetLastError(), "gated linear sums launch");
+}
+
+void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t stream) {
+  TileArgs t = tileArgs(a);
+  unsigned char *scratch = static_cast<unsigned char *>(a.scratch);
+  t.both = reinterpret_cast<bf16 *>(scratch);
+  t.stride = plan.stride;
+  float *biasParts = a.db_gate ? reinterpret_cast<float *>(scratch + plan.bothBytes) : nullptr;
+  float *parts = plan.partBytes ? reinterpret_cast<float *>(scratch + plan.bothBytes + plan.biasBytes) : nullptr;
+  t.dh = static_cast<const bf16 *>(a.dh);
+  t.dhStride = a.dh_stride;
+  t.wholeDh = reinterpret_cast<uintptr_t>(a.dh) % 16 == 0 && a.dh_stride % 8 == 0;
+  t.biasParts = biasParts;
+  launchProjections<Pass::gradients>(a, t, stream);
+  const int64_t rowTiles = ceilDiv(a.rows, kTileRows);
+  if (a.dx) {
+    t.dx = static_cast<bf16 *>(a.dx);
+    t.steps = int(ceilDiv(a.F, kTileSteps));
+    int columns = tileColumns(a.D);
+    while (columns > 64 && rowTiles * ceilDiv(a.D, columns) < 148) columns /= 2;
+    withColumns(columns, [&](auto n) {
+      TileMaps maps;
+      maps.a0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
+      maps.a1 = mapOf(t.both + plan.stride, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
+      maps.b0 = mapOf(a.w_gate, a.D, a.F, a.D, 64);
+      maps.b1 = mapOf(a.w_up, a.D, a.F, a.D, 64);
+      t.columnTiles = int(ceilDiv(a.D, n.value));
+      require(rowTiles * t.columnTiles < (int64_t(1) << 31), "Too many rows and columns");
+      t.tiles = int(rowTiles * t.columnTiles);
+      launchTiles<Pass::input, n.value>(maps, t, stream);
+    });
+  }
+  if (a.dw_gate) {
+    t.dwGate = static_cast<bf16 *>(a.dw_gate);
+    t.dwUp = static_cast<bf16 *>(a.dw_up);
+    t.parts = parts;
+    t.splits = plan.splits;
+    t.steps = int(ceilDiv(a.rows, kTileSteps));
+    t.rowTiles = int(ceilDiv(a.F, kTileRows));
+    withColumns(plan.weightColumns, [&](auto n) {
+      TileMaps maps;
+      maps.a0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(plan.stride), 64);
+      maps.a1 = mapOf(t.both + plan.stride, a.F, a.rows, 2 * int64_t(plan.stride), 64);
+      maps.b0 = maps.b1 = mapOf(a.x, a.D, a.rows, a.x_stride, 64);
+      t.columnTiles = int(ceilDiv(a.D, n.value));
+      const int64_t tiles = int64_t(t.columnTiles) * 2 * t.rowTiles * t.splits;
+      require(tiles < (int64_t(1) << 31), "Too many rows and columns");
+      t.tiles = int(tiles);
+      launchTiles<Pass::weights, n.value>(maps, t, stream);
+    });
+  }
+  launchSums<bf16>(a, plan, a.dw_gate ? parts : nullptr, biasParts, stream);
+}
+
+void gatedBackward32(const duck_gated &a, const GatedPlan &plan, cudaStream_t stream) {
+  ProductArgs g = productArgs(a);
+  unsigned char *scratch = static_cast<unsigned char *>(a.scratch);
+  float *both = reinterpret_cast<float *>(scratch);
+  float *biasParts = a.db_gate ? reinterpret_cast<float *>(scratch + plan.bothBytes) : nullptr;
+  float *parts = a.dw_gate ? reinterpret_cast<float *>(scratch + plan.bothBytes + plan.biasBytes) : nullptr;
+  const int64_t rowBlocks = ceilDiv(a.rows, kGradientRows);
+  require(rowBlocks < 65536 && ceilDiv(a.rows, kProductTile) < 65536 && 2 * ceilDiv(a.F, kProductTile) < 65536,
+          "Too many rows or columns");
+  const GradientArgs e{static_cast<const float *>(a.kept), static_cast<const float *>(a.dh), both, biasParts, a.rows, a.dh_stride,
+                       a.F, a.activation};
+  gatedGradients<<<dim3(unsigned(ceilDiv(a.F, 32)), unsigned(rowBlocks)), 256, 0, stream>>>(e);
+  check(cudaGetLastError(), "gated linear launch");
+  g.both = both;
+  if (a.dx) {
+    g.dx = static_cast<float *>(a.dx);
+    const dim3 grid(unsigned(ceilDiv(a.D, kProductTile)), unsigned(ceilDiv(a.rows, kProductTile)));
+    gatedProducts<Pass::input><<<grid, kProductThreads, 0, stream>>>(g);
+    check(cudaGetLastError(), "gated linear launch");
+  }
+  if (a.dw_gate) {
+    g.parts = parts;
+    g.splits = plan.splits;
+    const dim3 grid(unsigned(ceilDiv(a.D, kProductTile)), unsigned(2 * ceilDiv(a.F, kProductTile)), unsigned(plan.splits));
+    gatedProducts<Pass::weights><<<grid, kProductThreads, 0, stream>>>(g);
+    check(cudaGetLastError(), "gated linear launch");
+  }
+  launchSums<float>(a, plan, parts, biasParts, stream);
+}
+
 }  // namespace
 
 extern "C" {
+
+int duck_gated_linear_sizes(const duck_gated *args, int64_t *out) {
+  return guarded([&] {
+    require(out != nullptr, "Invalid arguments");
+    out[0] = out[1] = 0;
+    if (!gatedChecked(args)) return;
+    const GatedPlan plan = planGated(*args);
+    out[0] = plan.bothBytes + plan.biasBytes + plan.partBytes;
+    out[1] = plan.keptBytes;
+  });
+}
+
+int duck_gated_linear_forward(const duck_gated *args, duck_stream stream) {
+  return guarded([&] {
+    if (!gatedChecked(args)) return;
+    const duck_gated &a = *args;
+    require(a.x && a.w_gate && a.w_up && a.h && !a.b_gate == !a.b_up, "Invalid arguments");
+    requireAligned({a.h, a.kept});
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (a.type == DUCK_BFLOAT16) {
+      TileArgs t = tileArgs(a);
+      t.h = static_cast<bf16 *>(a.h);
+      t.wholeH = a.F % 8 == 0;
+      return launchProjections<Pass::forward>(a, t, s);
+    }
+    ProductArgs g = productArgs(a);
+    g.h = static_cast<float *>(a.h);
+    g.kept = static_cast<float *>(a.kept);
+    require(ceilDiv(a.rows, kProductTile) < 65536, "Too many rows or columns");
+    const dim3 grid(unsigned(ceilDiv(a.F, kProductTile / 2)), unsigned(ceilDiv(a.rows, kProductTile)));
+    gatedProducts<Pass::forward><<<grid, kProductThreads, 0, s>>>(g);
+    check(cudaGetLastError(), "gated linear launch");
+  });
+}
+
+int duck_gated_linear_backward(const duck_gated *args, duck_stream stream) {
+  return guarded([&] {
+    const bool some = gatedChecked(args);
+    const duck_gated &a = *args;
+    require(!a.dw_gate == !a.dw_up && !a.db_gate == !a.db_up && !a.b_gate == !a.b_up, "Invalid arguments");
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (!some) {   // no rows: no sums
+      const size_t size = a.type == DUCK_FLOAT32 ? 4 : 2;
+      for (void *p : {a.dw_gate, a.dw_up})
+        if (p) check(cudaMemsetAsync(p, 0, size_t(a.F) * a.D * size, s), "gated linear gradients");
+      for (void *p : {a.db_gate, a.db_up})
+        if (p) check(cudaMemsetAsync(p, 0, size_t(a.F) * size, s), "gated linear gradients");
+      return;
+    }
+    if (!a.dx && !a.dw_gate && !a.db_gate) return;
+    require(a.x && a.w_gate && a.w_up && a.dh && a.scratch && (a.type == DUCK_BFLOAT16 || a.kept), "Invalid arguments");
+    requireAligned({a.dx, a.dw_gate, a.dw_up, a.kept, a.scratch});
+    const GatedPlan plan = planGated(a);
+    if (a.type == DUCK_BFLOAT16) gatedBackward16(a, plan, s);
+    else gatedBackward32(a, plan, s);
+  });
+}
 
 int duck_gated_recurrence_sizes(const duck_recurrence *args, int64_t *out) {
   return guarded([&] {

@@ -1,12 +1,13 @@
 """Operators of a policy with memory: layer norm, linear attention with one
-decay per head, a gated linear recurrence, and activations kept in 8 bits for the
-backward pass.
+decay per head, a gated linear recurrence, a gated linear layer, and activations
+kept in 8 bits for the backward pass.
 
     layer_norm(x, weight, bias, eps)                           -> y
     linear_attention(q, k, v, decay, state, resets, ...)       -> out, state
     linear_attention_step(q, k, v, decay, state, reset, ...)   -> out
     gated_recurrence(gates, values, state, resets, ...)        -> out, state
     gated_recurrence_step(gates, values, state, reset)         -> out
+    gated_linear(x, w_gate, w_up, b_gate, b_up, activation)    -> h
     elu_checkpoint(x)                                          -> y, Checkpoint8
     elu_restore(dy, kept)                                      -> dx, y
     checkpointed_mlp(x, weights, biases)                       -> y
@@ -520,6 +521,122 @@ def gated_recurrence_step(gates, values, state, reset=None):
                              _TYPES[gates.dtype]))
     torch.autograd.graph.increment_version(state)   # autograd does not see a kernel's writes
     return out
+
+
+# ---------------------------------------------------------------- gated linear
+# struct duck_gated of include/duck_b200.h.
+_GATED = struct.Struct("@14P3q4i")
+ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
+
+
+@functools.lru_cache(maxsize=1024)
+def _gated_workspace(rows, D, F, kind, weights, biases):
+    """Bytes of scratch of a backward call with or without those gradients, and of
+    what a forward call keeps for it."""
+    out = (ctypes.c_int64 * 2)()
+    pointers = [0] * 14
+    pointers[8] = pointers[9] = int(weights)
+    pointers[10] = pointers[11] = int(biases)
+    _raise(library().duck_gated_linear_sizes(_GATED.pack(*pointers, rows, 0, 0, D, F, 0, kind), out))
+    return tuple(out)
+
+
+def _gated_operand(t, strided):
+    """Rows as the kernels take them: dense (`strided`: up to the distance of the
+    rows), for bfloat16 of whole 16-byte pieces on their boundaries."""
+    t = _rows_of(t) if strided else t.contiguous()
+    if t.dtype == torch.bfloat16 and (t.data_ptr() % 16 or t.stride(0) % 8):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _gated_forward(x, w_gate, w_up, b_gate, b_up, activation, keep):
+    rows, D = x.shape
+    F_ = w_gate.shape[0]
+    kind = _TYPES[x.dtype]
+    h = torch.empty((rows, F_), dtype=x.dtype, device=x.device)
+    kept = _buffer(_gated_workspace(rows, D, F_, kind, False, False)[1], x.device) if keep else None
+    _launch(library().duck_gated_linear_forward, x.device,
+            _GATED.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate), _address(b_up), h.data_ptr(),
+                        0, 0, 0, 0, 0, 0, _address(kept), 0, rows, x.stride(0), 0, D, F_, activation, kind))
+    return h, kept
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, activation):
+        ctx.shape = x.shape
+        x, w_gate, w_up = _gated_operand(x, True), _gated_operand(w_gate, False), _gated_operand(w_up, False)
+        h, kept = _gated_forward(x, w_gate, w_up, b_gate, b_up, activation, True)
+        ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up, kept)
+        ctx.activation = activation
+        return h.view(ctx.shape[:-1] + (h.shape[1],))
+
+    @staticmethod
+    @_once
+    def backward(ctx, dh):
+        x, w_gate, w_up, b_gate, b_up, kept = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        weights, biases = needs[1] or needs[2], needs[3] or needs[4]
+        rows, D = x.shape
+        F_ = w_gate.shape[0]
+        kind = _TYPES[x.dtype]
+        dh = _rows_of(dh)
+        empty = functools.partial(torch.empty, dtype=x.dtype, device=x.device)
+        dx = empty((rows, D)) if needs[0] else None
+        dw = (empty((F_, D)), empty((F_, D))) if weights else (None, None)
+        db = (empty(F_), empty(F_)) if biases else (None, None)
+        scratch = _buffer(_gated_workspace(rows, D, F_, kind, weights, biases)[0], x.device)
+        _launch(library().duck_gated_linear_backward, x.device,
+                _GATED.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate), _address(b_up), 0,
+                            dh.data_ptr(), _address(dx), _address(dw[0]), _address(dw[1]), _address(db[0]), _address(db[1]),
+                            _address(kept), _address(scratch), rows, x.stride(0), dh.stride(0), D, F_, ctx.activation, kind))
+        return dx.view(ctx.shape) if needs[0] else None, *dw, *db, None
+
+
+@torch.autocast("cpu", enabled=False)
+def _gated_plain(x, w_gate, w_up, b_gate, b_up, activation):
+    """In float32 or wider, rounded once."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    to = lambda t: None if t is None else t.to(wide)
+    a, u = F.linear(to(x), to(w_gate), to(b_gate)), F.linear(to(x), to(w_up), to(b_up))
+    act = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid}[activation]
+    return (act(a) * u).to(x.dtype)
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
+    """Two projections of the same rows, multiplied, one of them through an
+    activation:
+
+        act(x w_gate^T + b_gate) * (x w_up^T + b_up),   act: "silu", "gelu" (of erf) or "sigmoid"
+
+    ``x`` [..., D], weights [F, D], biases [F] or none, all of one type; returns
+    [..., F].  Gradients flow to all of them.  Sums are float32, and so are the two
+    projections; the result is rounded once.  bfloat16 on the GPU: for the backward
+    pass only x is kept; gradients of the projections are rounded to 8 bits on
+    their way to those of x and the weights."""
+    _require(activation in ACTIVATIONS, f"gated_linear: the activation is one of {', '.join(ACTIVATIONS)}")
+    _require(x.dim() > 0 and w_gate.dim() == 2 and w_gate.shape == w_up.shape and w_gate.shape[1] == x.shape[-1]
+             and w_gate.numel() > 0, "gated_linear: weights are [F, D] for x [..., D]")
+    _require((b_gate is None) == (b_up is None) and all(b is None or b.shape == w_gate.shape[:1] for b in (b_gate, b_up)),
+             "gated_linear: biases are [F], both or neither")
+    given = [t for t in (x, w_gate, w_up, b_gate, b_up) if t is not None]
+    _require(all(t.dtype == x.dtype and t.device == x.device for t in given) and x.dtype in _WIDE,
+             "gated_linear: one floating type and device for x, weights and biases")
+    if not x.is_cuda:
+        return _gated_plain(x, w_gate, w_up, b_gate, b_up, activation)
+    _check_type(x, "gated_linear")
+    odd = -x.shape[-1] % 8
+    if odd and x.dtype == torch.bfloat16:   # rows of whole 16-byte pieces
+        x, w_gate, w_up = (F.pad(t, (0, odd)) for t in (x, w_gate, w_up))
+    if b_gate is not None:
+        b_gate, b_up = b_gate.contiguous(), b_up.contiguous()
+    if _grad_needed(x, w_gate, w_up, b_gate, b_up):
+        return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[activation])
+    shape = x.shape
+    x, w_gate, w_up = _gated_operand(x, True), _gated_operand(w_gate, False), _gated_operand(w_up, False)
+    h, _ = _gated_forward(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[activation], False)
+    return h.view(shape[:-1] + (h.shape[1],))
 
 
 # ----------------------------------------------------------- 8-bit checkpoints

@@ -462,6 +462,37 @@ int duck_gated_recurrence_backward(const duck_recurrence *args, duck_stream stre
  * resets is [E]. */
 int duck_gated_recurrence_step(const duck_recurrence *args, duck_stream stream);
 
+/* Gated linear layer on rows x [rows, D]:
+ *   h = act(x w_gate^T + b_gate) (x w_up^T + b_up),  weights [F, D], biases [F]
+ * and its gradients.  Element types are those of `type` throughout; h, the
+ * weights, their gradients and dx are dense, rows of x and dh have the strides
+ * given.  For DUCK_BFLOAT16 the rows of x, the weights and their gradients are
+ * whole 16-byte pieces on 16-byte boundaries (D a multiple of 8).  `kept` is what a
+ * forward call leaves for the backward one (DUCK_FLOAT32 only, else NULL).
+ * Outputs and workspaces lie on 16-byte boundaries, and no output overlaps an
+ * input. */
+enum { DUCK_SILU = 0, DUCK_GELU = 1, DUCK_SIGMOID = 2 };
+typedef struct duck_gated {
+  const void *x, *w_gate, *w_up;
+  const void *b_gate, *b_up;       /* both or neither */
+  void *h;                         /* forward */
+  const void *dh;                  /* backward */
+  void *dx;                        /* backward: [rows, D], or NULL */
+  void *dw_gate, *dw_up;           /* backward: both, or NULL */
+  void *db_gate, *db_up;           /* backward: both, or NULL */
+  void *kept;                      /* forward writes, backward reads: duck_gated_linear_sizes; or NULL */
+  void *scratch;                   /* backward: duck_gated_linear_sizes */
+  int64_t rows, x_stride, dh_stride;
+  int32_t D, F, activation, type;
+} duck_gated;
+
+/* Bytes of workspace for calls of these sizes (only rows, D, F, type and which of
+ * the backward pass's outputs are given is looked at): out[0] scratch of a
+ * backward call, out[1] `kept`. */
+int duck_gated_linear_sizes(const duck_gated *args, int64_t *out);
+int duck_gated_linear_forward(const duck_gated *args, duck_stream stream);
+int duck_gated_linear_backward(const duck_gated *args, duck_stream stream);
+
 /* AdamW over many tensors (the Python side is duck_gym_b200/optim.py).  A tensor
  * has n dense values of `type`; its gradient has the same.  Moments are float32
  * [n], or (bits = 8) codes [n], int8 for exp_avg and uint8 for exp_avg_sq, with one

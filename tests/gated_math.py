@@ -59,3 +59,17 @@ def code_values(codes, exponents):
         value = 2.0 ** (octave - 127) * (1 + eighths / 8) if octave else eighths * 2.0 ** -129
         out.append(float("nan") if e == 255 else 0.0 if c == 0 else value if c > 0 else -value)
     return torch.tensor(out, dtype=torch.float64).view(codes.shape)
+
+
+def linear(x, w_gate, w_up, b_gate, b_up, activation, dh=None):
+    """h and, with dh, (h, dx, dw_gate, dw_up, db_gate, db_up) for rows x."""
+    x, w_gate, w_up = x.double(), w_gate.double(), w_up.double()
+    a = x @ w_gate.t() + (0.0 if b_gate is None else b_gate.double())
+    u = x @ w_up.t() + (0.0 if b_up is None else b_up.double())
+    s = torch.special.ndtr(a) if activation == "gelu" else 1 / (1 + torch.exp(-a))
+    ds = torch.exp(-a * a / 2) / (2 * torch.pi) ** 0.5 if activation == "gelu" else s * (1 - s)
+    y, slope = (s, ds) if activation == "sigmoid" else (a * s, s + a * ds)
+    if dh is None:
+        return y * u
+    da, du = dh.double() * u * slope, dh.double() * y
+    return y * u, da @ w_gate + du @ w_up, da.t() @ x, du.t() @ x, da.sum(0), du.sum(0)

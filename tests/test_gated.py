@@ -100,3 +100,57 @@ def test_packed_recurrence_has_the_size_of_the_c_struct(tmp_path):
     got = offsets(tmp_path, "duck_recurrence", ("gates", "resets", "state_out", "dgates", "scratch", "gates_stride",
                                                 "dout_stride", "T", "type"))
     assert got == [0, 24, 40, 64, 96, 104, 136, 152, 164, memory._RECURRENCE.size]
+
+
+# ---------------------------------------------------------------- gated linear
+def layer(seed, rows, D, F, dtype=torch.float32, bias=True):
+    g = gen(seed)
+    x, wg, wu = (torch.randn(s, generator=g) for s in ((rows, D), (F, D), (F, D)))
+    bg, bu, dh = (torch.randn(s, generator=g) for s in ((F,), (F,), (rows, F)))
+    x, wg, wu, bg, bu, dh = (t.to(dtype) for t in (x, wg / D ** 0.5, wu / D ** 0.5, 0.3 * bg, 0.3 * bu, dh))
+    return x, wg, wu, bg if bias else None, bu if bias else None, dh
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_linear_matches_restatement(activation, bias):
+    case = layer(1, 20, 7, 11, bias=bias)
+    leaves = [t.requires_grad_() for t in case[:5] if t is not None]
+    h = memory.gated_linear(*case[:5], activation=activation)
+    got = (h, *torch.autograd.grad(h, leaves, case[5]))
+    want = gated_math.linear(*[None if t is None else t.detach() for t in case[:5]], activation, case[5])
+    for a, b in zip(got, want):
+        assert ref.error(a, b) <= ref.bound(torch.float32, 40)
+    assert torch.autograd.gradcheck(lambda *t: memory.gated_linear(*t[:3], *(t[3:] or (None, None)), activation=activation),
+                                    [t.detach()[:4].double().requires_grad_() if i == 0 else t.detach().double().requires_grad_()
+                                     for i, t in enumerate(leaves)])
+
+
+def test_linear_shapes_and_autocast():
+    x, wg, wu, bg, bu, _ = layer(2, 24, 5, 6)
+    h = memory.gated_linear(x, wg, wu, bg, bu)
+    assert torch.equal(memory.gated_linear(x.view(2, 3, 4, 5), wg, wu, bg, bu).view(24, 6), h)
+    assert memory.gated_linear(x[0], wg, wu).shape == (6,) and memory.gated_linear(x[:0], wg, wu).shape == (0, 6)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        assert torch.equal(memory.gated_linear(x, wg, wu, bg, bu), h)
+
+
+def test_linear_refusals():
+    x, wg, wu, bg, bu, _ = layer(3, 4, 5, 6)
+    bad = [
+        lambda: memory.gated_linear(x, wg, wu[:5]), lambda: memory.gated_linear(x[:, :4], wg, wu),
+        lambda: memory.gated_linear(x, wg, wu, bg), lambda: memory.gated_linear(x, wg, wu, bg, bu[:5]),
+        lambda: memory.gated_linear(x, wg, wu.double()), lambda: memory.gated_linear(x, wg, wu, bg.double(), bu),
+        lambda: memory.gated_linear(x, wg, wu, activation="relu"), lambda: memory.gated_linear(x, wg[:0], wu[:0]),
+        lambda: memory.gated_linear(x[:, :0], wg[:, :0], wu[:, :0]), lambda: memory.gated_linear(x.long(), wg.long(), wu.long()),
+        lambda: memory.gated_linear(torch.tensor(1.0), wg, wu), lambda: memory.gated_linear(x, wg[0], wu[0]),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"case {i} was accepted")
+
+
+def test_packed_layer_has_the_size_of_the_c_struct(tmp_path):
+    got = offsets(tmp_path, "duck_gated", ("x", "h", "dw_gate", "db_gate", "kept", "scratch", "rows", "D", "F", "type"))
+    assert got == [0, 40, 64, 80, 96, 104, 112, 136, 140, 148, memory._GATED.size]

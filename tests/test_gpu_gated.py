@@ -286,3 +286,254 @@ def test_recurrence_refusals_on_the_gpu():
     for entry in (lib.duck_gated_recurrence_forward, lib.duck_gated_recurrence_backward, lib.duck_gated_recurrence_step):
         assert entry(None, None) != 0
     assert b"Invalid" in lib.duck_last_error()
+
+
+# ---------------------------------------------------------------- gated linear
+# bfloat16: h and the biases' gradients have one rounding (2^-8 at most); dx and the weights' gradients are sums of
+# products with da or du, rounded once, and are rounded themselves: two, which add in the mean square (memory_math.bound).
+# The hardware's exponential and quotient leave 2^-20.
+def layer(seed, rows, D, F, dtype, bias=True):
+    g = gen(seed)
+    x, wg, wu = normal(g, rows, D), normal(g, F, D) / D ** 0.5, normal(g, F, D) / D ** 0.5
+    bg, bu, dh = 0.3 * normal(g, F), 0.3 * normal(g, F), normal(g, rows, F)
+    x, wg, wu, bg, bu, dh = (t.to(dtype) for t in (x, wg, wu, bg, bu, dh))
+    return [x, wg, wu, bg if bias else None, bu if bias else None, dh]
+
+
+def check_layer(case, activation, devices=None, dh=None):
+    x, wg, wu, bg, bu, _ = case
+    dev = [None if t is None else t.cuda() for t in case[:5]] if devices is None else devices
+    leaves = [t.requires_grad_() for t in dev if t is not None]
+    h = memory.gated_linear(*dev, activation=activation)
+    dtype, (rows, D), F = x.dtype, x.shape, wg.shape[0]
+    assert h.dtype == dtype and h.shape == (rows, F) and h.is_contiguous()
+    grads = torch.autograd.grad(h, leaves, case[5].cuda() if dh is None else dh)
+    want = gated_math.linear(*case[:5], activation, case[5])
+    terms = (D, 2 * F + D, rows + D, rows + D, rows + D, rows + D)
+    for i, (got, exact) in enumerate(zip((h, *grads), want)):
+        assert got.dtype == dtype and got.shape == exact.shape
+        two = 2 if i in (1, 2, 3) else 1
+        assert ref.error(got, exact) <= ref.bound(dtype, terms[i], two) + ref.bound(torch.float32, terms[i]), i
+    return [h, *grads]
+
+
+# Tiles of 128 rows, 64 steps, 32 to 128 features; widths off every boundary; rows that are split for the weights.
+LAYERS = [(1, 1, 1), (1, 64, 64), (2, 8, 5), (16, 256, 512), (127, 61, 33), (128, 64, 128), (129, 72, 130), (300, 61, 301),
+          (513, 200, 96), (2000, 96, 264), (2501, 130, 40), (4096, 256, 512), (19000, 128, 128), (1025, 520, 1030), (64, 1024, 2048)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,D,F", LAYERS)
+def test_linear(rows, D, F, dtype):
+    case = layer(rows + D + F, rows, D, F, dtype)
+    activation = ["silu", "gelu", "sigmoid"][rows % 3]
+    first, again = check_layer(case, activation), check_layer(case, activation)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))   # bit for bit
+    with torch.no_grad():
+        assert torch.equal(memory.gated_linear(*[t.cuda() for t in case[:5]], activation=activation), first[0])
+    check_layer(layer(rows + 1, rows, D, F, dtype, bias=False), "silu")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid"])
+def test_linear_partial_gradients(activation, dtype):
+    case = layer(5, 200, 64, 72, dtype)
+    want = check_layer(case, activation)
+    for which in ((0,), (1,), (2,), (3,), (4,), (0, 3), (1, 2)):
+        dev = [t.cuda().requires_grad_(i in which) for i, t in enumerate(case[:5])]
+        h = memory.gated_linear(*dev, activation=activation)
+        grads = torch.autograd.grad(h, [dev[i] for i in which], case[5].cuda())
+        for i, got in zip(which, grads):
+            assert torch.equal(got, want[1 + i])
+    frozen = [t.cuda() for t in case[:5]]
+    assert not memory.gated_linear(*frozen, activation=activation).requires_grad
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,F", [(64, 96), (61, 35)])
+def test_linear_strides(D, F, dtype):
+    case = layer(D, 150, D, F, dtype)
+    dev = lambda: [t.cuda() for t in case[:5]]
+    x, wg, wu, bg, bu, dh = case
+    wide = torch.empty(150, D + 11, dtype=dtype, device="cuda")
+    wide[:, 3:3 + D] = x.cuda()
+    check_layer(case, "silu", [wide[:, 3:3 + D].detach(), *dev()[1:]])
+    apart = torch.empty(300, D + (-D % 8), dtype=dtype, device="cuda")[::2, :D]
+    apart.copy_(x)
+    check_layer(case, "silu", [apart.detach(), *dev()[1:]])
+    check_layer(case, "silu", [x.t().contiguous().cuda().t().detach(), *dev()[1:]])
+    both = torch.cat((wg, wu)).cuda()   # of one parameter
+    check_layer(case, "silu", [dev()[0], both[:F].detach(), both[F:].detach(), *dev()[3:]])
+    turned = [w.t().contiguous().cuda().t().detach() for w in (wg, wu)]
+    check_layer(case, "silu", [dev()[0], *turned, *dev()[3:]])
+    odd = [torch.empty(t.numel() + 1, dtype=dtype, device="cuda")[1:].view(t.shape) for t in case[:5]]
+    for a, b in zip(odd, case):
+        a.copy_(b)
+    check_layer(case, "silu", [t.detach() for t in odd])
+    same = case[:]
+    same[0], same[5] = x[:1].expand(150, D), dh[:1].expand(150, F)   # rows and their gradients with strides of zero
+    check_layer(same, "gelu", [x[:1].cuda().expand(150, D).detach(), *dev()[1:]], dh[:1].cuda().expand(150, F))
+    loose = torch.empty(150, F + 3, dtype=dtype, device="cuda")[:, 1:1 + F]
+    loose.copy_(dh)
+    check_layer(case, "silu", None, loose)
+    ones = case[:5] + [torch.ones(150, F, dtype=dtype)]
+    check_layer(ones, "silu", None, torch.ones((), dtype=dtype, device="cuda").expand(150, F))
+
+
+def test_linear_shapes():
+    x, wg, wu, bg, bu, dh = [t.cuda() for t in layer(6, 24, 16, 40, torch.bfloat16)]
+    h = memory.gated_linear(x, wg, wu, bg, bu)
+    leaf = x.view(2, 3, 4, 16).detach().requires_grad_()
+    out = memory.gated_linear(leaf, wg, wu, bg, bu)
+    assert out.shape == (2, 3, 4, 40) and torch.equal(out.view(24, 40), h)
+    d, = torch.autograd.grad(out, leaf, dh.view(2, 3, 4, 40))
+    flat = x.detach().requires_grad_()
+    assert torch.equal(d.view(24, 16), torch.autograd.grad(memory.gated_linear(flat, wg, wu, bg, bu), flat, dh)[0])
+    assert memory.gated_linear(x[0], wg, wu).shape == (40,)
+    for dtype in TYPES:
+        leaves = [t.to(dtype).detach().requires_grad_() for t in (x[:0], wg, wu, bg, bu)]
+        out = memory.gated_linear(*leaves)
+        grads = torch.autograd.grad(out, leaves, torch.zeros_like(out))
+        assert out.shape == (0, 40) and grads[0].shape == (0, 16) and all(float(g.abs().sum()) == 0.0 for g in grads)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert memory.gated_linear(x.float(), wg.float(), wu.float()).dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_values_that_are_not_finite(dtype):
+    """They stay in their row of h and dx, and in their feature's gradients."""
+    case = layer(7, 200, 64, 96, dtype)
+    x, wg, wu, bg, bu, dh = case
+    x[3, 5], x[150, 0], dh[40, 7] = float("nan"), float("inf"), float("inf")
+    leaves = [t.cuda().requires_grad_() for t in case[:5]]
+    h = memory.gated_linear(*leaves)
+    assert sorted(h.isfinite().logical_not().any(1).nonzero().flatten().tolist()) == [3, 150]
+    dx, dwg, _, dbg, _ = torch.autograd.grad(h, leaves, dh.cuda())
+    assert sorted(dx.isfinite().logical_not().any(1).nonzero().flatten().tolist()) == [3, 40, 150]
+    wide = torch.zeros(200, 96, dtype=dtype, device="cuda")
+    bias = bg.cuda()
+    bias[95] = float("inf")   # rows and features behind the last ones stay apart
+    case = layer(8, 130, 64, 96, dtype)
+    leaves = [t.cuda().requires_grad_() for t in case[:3]] + [bias.requires_grad_(), bu.cuda().requires_grad_()]
+    h = memory.gated_linear(*leaves)
+    assert bool(h[:, :95].isfinite().all()) and not bool(h[:, 95].isfinite().any())
+    grads = torch.autograd.grad(h, leaves, wide[:130])
+    assert bool(grads[1][:95].isfinite().all()) and bool(grads[3][:95].isfinite().all())
+
+
+def test_linear_large_projections():
+    """Activations far from zero: exponentials that overflow leave no NaN."""
+    for activation in ("silu", "gelu", "sigmoid"):
+        for dtype in TYPES:
+            case = layer(9, 64, 32, 16, dtype)
+            case[1] = (case[1].float() * 300).to(dtype)
+            check_layer(case, activation)
+
+
+def test_linear_of_many_values():
+    """Offsets beyond 2^31 elements, of h and of x."""
+    rows, D, F = (1 << 21) + 70, 64, 1032
+    x = torch.empty(rows, D, dtype=torch.bfloat16, device="cuda").normal_()
+    case = layer(10, 8, D, F, torch.bfloat16)
+    weights = [t.cuda() for t in case[1:5]]
+    with torch.no_grad():
+        h = memory.gated_linear(x, *weights)
+    want = gated_math.linear(x[-70:].cpu(), *case[1:5], "silu")
+    assert ref.error(h[-70:], want) <= ref.bound(torch.bfloat16, D) + ref.bound(torch.float32, D)
+    del h
+    leaf = x[:, :8].contiguous().requires_grad_()
+    small = [t[:, :8].contiguous() for t in weights[:2]]
+    dh = torch.empty(rows, F, dtype=torch.bfloat16, device="cuda").normal_()
+    dx, = torch.autograd.grad(memory.gated_linear(leaf, *small), leaf, dh)
+    want = gated_math.linear(leaf[-70:].detach().cpu(), *[t.cpu() for t in small], None, None, "silu", dh[-70:].cpu())
+    assert ref.error(dx[-70:], want[1]) <= ref.bound(torch.bfloat16, 2 * F, 2) + ref.bound(torch.float32, 2 * F)
+
+
+def test_linear_refuses_second_and_forward_mode_derivatives():
+    from torch.autograd import forward_ad
+
+    x, wg, wu, *_ = [t.cuda() for t in layer(11, 8, 16, 24, torch.float32)]
+    leaf = x.clone().requires_grad_()
+    d, = torch.autograd.grad(memory.gated_linear(leaf, wg, wu).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), leaf)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(wg, torch.ones_like(wg))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                memory.gated_linear(x, dual, wu)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [16, 3000])
+def test_linear_on_another_stream_and_in_a_graph(rows, dtype):
+    case = [t.cuda() for t in layer(12, rows, 64, 128, dtype)]
+
+    def everything():
+        leaves = [t.detach().requires_grad_() for t in case[:5]]
+        h = memory.gated_linear(*leaves)
+        return [h, *torch.autograd.grad(h, leaves, case[5])]
+
+    want = everything()
+    side, third = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (side, third):   # at the same time
+        s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = everything()
+    with torch.cuda.stream(third):
+        another = everything()
+    for s in (side, third):
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, other, another))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = everything()
+    for t in captured:
+        t.detach().zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, captured))
+
+
+def test_linear_as_the_first_call_of_a_thread():
+    """No other call has made the device's context that thread's before."""
+    import threading
+
+    x, wg, wu, *_ = [t.cuda() for t in layer(14, 40, 64, 64, torch.bfloat16)]
+    with torch.no_grad():
+        want, got = memory.gated_linear(x, wg, wu), []
+
+        def run():
+            with torch.no_grad():
+                try:
+                    got.append(memory.gated_linear(x, wg, wu))
+                except RuntimeError as e:
+                    got.append(e)
+
+        thread = threading.Thread(target=run)
+        thread.start()
+        thread.join()
+    assert torch.is_tensor(got[0]), got[0]
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want)
+
+
+def test_linear_refusals_on_the_gpu():
+    from duck_gym_b200.cuda_batch import library
+
+    x, wg, wu, bg, bu, dh = [t.cuda() for t in layer(13, 16, 16, 24, torch.float32)]
+    for call in (lambda: memory.gated_linear(x.half(), wg.half(), wu.half()), lambda: memory.gated_linear(x, wg.cpu(), wu),
+                 lambda: memory.gated_linear(x.double(), wg.double(), wu.double()), lambda: memory.gated_linear(x, wg, wu, bg.cpu(), bu)):
+        with pytest.raises(RuntimeError):
+            call()
+    lib, p = library(), x.data_ptr()
+    fine = dict(x=p, w_gate=p, w_up=p, b_gate=0, b_up=0, h=p, dh=p, dx=p, dw_gate=p, dw_up=p, db_gate=p, db_up=p, kept=p,
+                scratch=p, rows=16, x_stride=16, dh_stride=24, D=16, F=24, activation=0, type=0)
+    pack = lambda **change: memory._GATED.pack(*{**fine, **change}.values())
+    for change in (dict(x=0), dict(w_gate=0), dict(h=0), dict(b_gate=p), dict(D=0), dict(F=-1), dict(rows=-1), dict(rows=1 << 31),
+                   dict(activation=3), dict(type=2), dict(type=1, D=12), dict(h=p + 4), dict(type=1, x=p + 2), dict(type=1, x_stride=15)):
+        assert lib.duck_gated_linear_forward(pack(**change), None) != 0, change
+    for change in (dict(dh=0), dict(scratch=0), dict(kept=0), dict(dw_up=0), dict(db_gate=0), dict(dx=p + 4), dict(type=1, w_up=p + 2)):
+        assert lib.duck_gated_linear_backward(pack(**change), None) != 0, change
+    assert lib.duck_gated_linear_forward(None, None) != 0 and lib.duck_gated_linear_backward(None, None) != 0
+    assert b"Invalid" in lib.duck_last_error()
