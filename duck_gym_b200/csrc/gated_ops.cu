@@ -30,7 +30,9 @@ void requireAligned(std::initializer_list<const void *> pointers) {
     require(reinterpret_cast<uintptr_t>(p) % 16 == 0, "States, outputs and workspaces have to be 16-byte aligned");
 }
 
-// How the steps are split where two channels a thread leave fewer than eight warps on a multiprocessor.
+// How the steps are split where two channels a thread leave fewer than four warps on a multiprocessor: into segments of 64
+// steps at least that give it eight.  They are read twice, so that where threads are enough one pass is faster (1000 steps,
+// 256 x 256 channels: 261 us forward and backward, 396 in two segments); a replay of 16384 steps of 1024 channels takes 63 us.
 struct RecurrencePlan {
   int segmentLength, segments;
   int64_t scratchBytes, keptBytes;
@@ -38,7 +40,7 @@ struct RecurrencePlan {
 RecurrencePlan planRecurrence(const duck_recurrence &a) {
   RecurrencePlan p{};
   const int64_t channels = int64_t(a.E) * a.N, threads = ceilDiv(channels, 2);
-  const int64_t want = threads >= 148 * 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>(a.T / 64, 148 * 512 / threads));
+  const int64_t want = threads >= 148 * 128 ? 1 : std::max<int64_t>(1, std::min<int64_t>(a.T / 64, 148 * 256 / threads));
   p.segmentLength = int(ceilDiv(ceilDiv(std::max(1, a.T), want), kKeep) * kKeep);
   p.segments = std::max(1, int(ceilDiv(a.T, p.segmentLength)));
   if (p.segments > 1) p.scratchBytes = int64_t(p.segments) * 2 * channels * 4;
@@ -79,21 +81,56 @@ void copyState(const duck_recurrence &a, const float *from, float *to, cudaStrea
         "gated recurrence state");
 }
 
+// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device
+// (by whichever thread comes first: autograd calls from its own).
+template <auto kernel> void allowShared(int bytes) {
+  static std::atomic<bool> done[64] = {};
+  int device = 0;
+  check(cudaGetDevice(&device), "cudaGetDevice");
+  if (device < 64 && done[device]) return;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  if (device < 64) done[device] = true;
+}
+
 dim3 recurrenceGrid(int64_t channels, int V, int segments) {
   return dim3(unsigned(ceilDiv(channels, int64_t(kRecurrenceThreads) * V)), unsigned(segments));
 }
 
-template <class T, int V> void launchForward(const RecurrenceArgs &r, cudaStream_t stream) {
+template <class T, int V, int SLOTS> void launchForward(const RecurrenceArgs &r, cudaStream_t stream) {
   const int64_t channels = int64_t(r.E) * r.N;
-  if (r.segmentCount > 1)
-    recurrenceForward<T, V, false><<<recurrenceGrid(channels, V, r.segmentCount - 1), kRecurrenceThreads, 0, stream>>>(r);
-  recurrenceForward<T, V, true><<<recurrenceGrid(channels, V, r.segmentCount), kRecurrenceThreads, 0, stream>>>(r);
+  constexpr int bytes = Ring<T, V, 2, SLOTS>::bytes;
+  constexpr auto find = recurrenceForward<T, V, SLOTS, false>, run = recurrenceForward<T, V, SLOTS, true>;
+  if constexpr (bytes > 48 * 1024) allowShared<find>(bytes), allowShared<run>(bytes);
+  if (r.segmentCount > 1) find<<<recurrenceGrid(channels, V, r.segmentCount - 1), kRecurrenceThreads, bytes, stream>>>(r);
+  run<<<recurrenceGrid(channels, V, r.segmentCount), kRecurrenceThreads, bytes, stream>>>(r);
 }
-template <class T, int V> void launchBackward(const RecurrenceArgs &r, cudaStream_t stream) {
+template <class T, int V, int SLOTS> void launchBackward(const RecurrenceArgs &r, cudaStream_t stream) {
   const int64_t channels = int64_t(r.E) * r.N;
-  if (r.segmentCount > 1)
-    recurrenceBackwardSegments<T, V><<<recurrenceGrid(channels, V, r.segmentCount - 1), kRecurrenceThreads, 0, stream>>>(r);
-  recurrenceBackward<T, V><<<recurrenceGrid(channels, V, r.segmentCount), kRecurrenceThreads, 0, stream>>>(r);
+  constexpr int findBytes = Ring<T, V, 2, SLOTS>::bytes, bytes = Ring<T, V, 3, SLOTS>::bytes;
+  constexpr auto find = recurrenceBackwardSegments<T, V, SLOTS>;
+  constexpr auto run = recurrenceBackward<T, V, SLOTS>;
+  if constexpr (findBytes > 48 * 1024) allowShared<find>(findBytes);
+  if constexpr (bytes > 48 * 1024) allowShared<run>(bytes);
+  if (r.segmentCount > 1) find<<<recurrenceGrid(channels, V, r.segmentCount - 1), kRecurrenceThreads, findBytes, stream>>>(r);
+  run<<<recurrenceGrid(channels, V, r.segmentCount), kRecurrenceThreads, bytes, stream>>>(r);
+}
+// Two channels a thread where they can be moved at once (four take twice the registers: a second, partly filled round of
+// blocks).  Four slots where the blocks are less than four a multiprocessor (1000 steps, 256 x 256 channels: forward 108 us,
+// backward 153; eight slots the same), two where there are more and their copies fill the memory's queue.
+constexpr int kFewBlocks = 148 * 4, kFewSlots = 4;
+template <class T, class F> void withSlots(const RecurrenceArgs &r, bool two, F &&f) {
+  const int64_t blocks = ceilDiv(int64_t(r.E) * r.N, int64_t(kRecurrenceThreads) * (two ? 2 : 1)) * r.segmentCount;
+  const bool few = blocks < kFewBlocks;
+  auto slots = [&](auto v) {
+    if (few) f(v, std::integral_constant<int, kFewSlots>());
+    else f(v, std::integral_constant<int, 2>());
+  };
+  if (two) slots(std::integral_constant<int, 2>());
+  else slots(std::integral_constant<int, 1>());
+}
+template <class F> void withLots(const duck_recurrence &a, const RecurrenceArgs &r, bool two, F &&f) {
+  if (a.type == DUCK_FLOAT32) withSlots<float>(r, two, [&](auto v, auto slots) { f(0.f, v, slots); });
+  else withSlots<bf16>(r, two, [&](auto v, auto slots) { f(bf16(), v, slots); });
 }
 
 // ---------------------------------------------------------------- gated linear
@@ -142,17 +179,6 @@ GatedPlan planGated(const duck_gated &a) {
   if (biases) p.biasBytes = padded(p.biasCount * 2 * a.F * 4);
   if (weights && (a.type == DUCK_FLOAT32 || p.splits > 1)) p.partBytes = padded(int64_t(p.splits) * 2 * a.F * a.D * 4);
   return p;
-}
-
-// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device
-// (by whichever thread comes first: autograd calls from its own).
-template <auto kernel> void allowShared(int bytes) {
-  static std::atomic<bool> done[64] = {};
-  int device = 0;
-  check(cudaGetDevice(&device), "cudaGetDevice");
-  if (device < 64 && done[device]) return;
-  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
-  if (device < 64) done[device] = true;
 }
 
 // A map over bfloat16 rows for boxes of 64 values by boxRows rows.
@@ -419,15 +445,9 @@ int duck_gated_recurrence_forward(const duck_recurrence *args, duck_stream strea
     const RecurrencePlan plan = planRecurrence(a);
     require(plan.segments == 1 || a.scratch, "Invalid arguments");
     const RecurrenceArgs r = argsOf(a, plan);
-    auto lots = [&](int V) {
-      return lotsOf(V, a.N, a.type, {a.gates, a.values, a.out},
-                    {a.gates_stride[0], a.gates_stride[1], a.values_stride[0], a.values_stride[1]});
-    };
-    const bool four = int64_t(a.E) * a.N >= int64_t(148) * 2048 && lots(4), two = lots(2);
-    if (a.type == DUCK_FLOAT32)
-      four ? launchForward<float, 4>(r, s) : two ? launchForward<float, 2>(r, s) : launchForward<float, 1>(r, s);
-    else
-      four ? launchForward<bf16, 4>(r, s) : two ? launchForward<bf16, 2>(r, s) : launchForward<bf16, 1>(r, s);
+    const bool two = lotsOf(2, a.N, a.type, {a.gates, a.values, a.out},
+                            {a.gates_stride[0], a.gates_stride[1], a.values_stride[0], a.values_stride[1]});
+    withLots(a, r, two, [&](auto zero, auto v, auto slots) { launchForward<decltype(zero), v.value, slots.value>(r, s); });
     check(cudaGetLastError(), "gated recurrence launch");
   });
 }
@@ -446,8 +466,7 @@ int duck_gated_recurrence_backward(const duck_recurrence *args, duck_stream stre
     const bool two = lotsOf(2, a.N, a.type, {a.gates, a.values, a.dout, a.dgates, a.dvalues},
                             {a.gates_stride[0], a.gates_stride[1], a.values_stride[0], a.values_stride[1],
                              a.dout_stride[0], a.dout_stride[1]});
-    if (a.type == DUCK_FLOAT32) two ? launchBackward<float, 2>(r, s) : launchBackward<float, 1>(r, s);
-    else two ? launchBackward<bf16, 2>(r, s) : launchBackward<bf16, 1>(r, s);
+    withLots(a, r, two, [&](auto zero, auto v, auto slots) { launchBackward<decltype(zero), v.value, slots.value>(r, s); });
     check(cudaGetLastError(), "gated recurrence backward launch");
   });
 }
