@@ -34,9 +34,9 @@
 namespace duckb200 {
 
 constexpr int kMomentGroup = 128;
-constexpr int kAdamThreads = 256, kAdamAtOnce = 2;
-constexpr int kAdamChunk = kAdamThreads / 32 * kAdamAtOnce * kMomentGroup;   // values of a block's round
-constexpr int kNormChunk = 4 * kAdamChunk;
+constexpr int kAdamThreads = 256, kAdamRound = kAdamThreads / 32 * kMomentGroup;   // one group for each warp
+constexpr int kAdamRoundsMost = 16;
+constexpr int kNormChunk = 8 * kAdamRound, kValuesChunk = 2 * kAdamRound;
 constexpr int kNormBlocks = 148 * 4;   // and sums, at most
 
 struct AdamTensor {
@@ -60,7 +60,7 @@ struct AdamArgs {
   const double *sums;         // of squares, sumCount of them
   double rateHost, beta1, beta2, weightDecay, maxNorm;
   float eps;
-  int sumCount, count, chunks, finish;
+  int sumCount, count, chunks, rounds, finish;   // rounds of a chunk
 };
 
 __device__ __forceinline__ uint32_t mixBits(uint32_t x) {   // the finaliser of MurmurHash3
@@ -72,18 +72,20 @@ __device__ __forceinline__ uint32_t mixBits(uint32_t x) {   // the finaliser of 
 template <int MOST> __device__ __forceinline__ int lowestCode(uint32_t exponent) {
   return max(0, int(8 * exponent) + 8 - MOST);
 }
-__device__ __forceinline__ float momentValue(int magnitude, int low, uint32_t exponent) {
-  const uint32_t bits = magnitude ? uint32_t(magnitude + low) << 20 : 0u;
-  return exponent == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(bits);
+__device__ __forceinline__ float momentValue(int magnitude, int low) {
+  return __uint_as_float(magnitude ? uint32_t(magnitude + low) << 20 : 0u);
 }
-// `bits` of a value's magnitude, finite or not; what a group with an infinity or a NaN gets is not read.
-__device__ __forceinline__ int momentCode(uint32_t bits, uint32_t noise, int low) {
-  return int(min((min(bits, 0x7f800000u) + noise) >> 20, 2039u)) - low;
+// `bits` of a value's magnitude; LEAST for a value that is not zero.  No code stands
+// for an infinity (top); what a group with one, or with a NaN, gets is not read.
+template <int MOST, int LEAST> __device__ __forceinline__ int momentCode(uint32_t bits, uint32_t noise, int low) {
+  const int top = min(MOST, 2039 - low);
+  return max(LEAST, min(top, (int(bits) + int(noise) - (low << 20)) >> 20));
 }
 
-// The chunk's tensor: the last one whose first chunk is not beyond it.
-template <int MOST> __device__ __forceinline__ int tensorOf(const AdamTable<MOST> &table, int count, int chunk) {
-  int low = 0, high = count;
+// The chunk's tensor, the last one whose first chunk is not beyond it; `from` that of an earlier chunk.
+template <int MOST> __device__ __forceinline__ int tensorOf(const AdamTable<MOST> &table, int count, int chunk, int from) {
+  if (from + 1 == count || table.t[from + 1].first > chunk) return from;
+  int low = from + 1, high = count;
   while (high - low > 1) {
     const int middle = (low + high) / 2;
     if (table.t[middle].first <= chunk) low = middle;
@@ -132,8 +134,9 @@ template <class T, int MOST>
 __global__ void __launch_bounds__(kAdamThreads) gradientSquares(const __grid_constant__ AdamTable<MOST> table, int count,
                                                                 int chunks, int before, double *sums) {
   double sum = 0.0;
-  for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    const AdamTensor &t = table.t[tensorOf(table, count, chunk)];
+  for (int chunk = blockIdx.x, index = 0; chunk < chunks; chunk += gridDim.x) {
+    index = tensorOf(table, count, chunk, index);
+    const AdamTensor &t = table.t[index];
     const T *g = static_cast<const T *>(t.grad);
     const int64_t begin = int64_t(chunk - t.first) * kNormChunk, end = min(t.n, begin + kNormChunk);
     constexpr int R = kNormChunk / (4 * kAdamThreads);
@@ -199,11 +202,13 @@ __device__ __forceinline__ void finishStep(const AdamArgs &p, uint32_t count) {
   }
 }
 
-// The approximations leave 2^-21 of the step's size, which is a small part of the parameter's.
+// The approximations leave 2^-21 of the step's size, which is a small part of the
+// parameter's.  (The root of the smallest float is a normal one, and so is eps.)
 __device__ __forceinline__ float adamParameter(float p, float m, float v, const AdamScalars &s, float eps) {
-  float root;
+  float root, inverse;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
-  return p * s.shrink - s.ahead * __fdividef(m, root * s.widen + eps);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(root, s.widen, eps)));
+  return fmaf(p, s.shrink, -s.ahead * (m * inverse));
 }
 template <class T> __device__ __forceinline__ T adamRounded(float p, uint32_t noise);
 template <> __device__ __forceinline__ float adamRounded<float>(float p, uint32_t) { return p; }
@@ -213,138 +218,195 @@ template <> __device__ __forceinline__ bf16 adamRounded<bf16>(float p, uint32_t 
   return finite ? __ushort_as_bfloat16(uint16_t((bits + (noise & 0xffffu)) >> 16)) : __float2bfloat16_rn(p);
 }
 
-template <class T, bool EIGHT, int MOST>
-__global__ void __launch_bounds__(kAdamThreads) adamStep(const __grid_constant__ AdamTable<MOST> table, AdamArgs p) {
-  constexpr int U = kAdamAtOnce;
-  const AdamScalars s = adamScalars(p);
-  const int lane = threadIdx.x % 32;
-  const float beta1 = float(p.beta1), rest1 = float(1.0 - p.beta1), beta2 = float(p.beta2), rest2 = float(1.0 - p.beta2);
-  for (int chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
-    const AdamTensor &t = table.t[tensorOf(table, p.count, chunk)];
-    const int64_t firstGroup = int64_t(chunk - t.first) * (kAdamChunk / kMomentGroup) + threadIdx.x / 32 * U;
-    const uint32_t key = mixBits(s.count + 0x9e3779b9u * (uint32_t(t.place) + 1));
-    T *param = static_cast<T *>(t.param);
-    const T *grad = static_cast<const T *>(t.grad);
-    float x[U][4], g[U][4], m[U][4], v[U][4];
-    // A lane's values: four neighbours where the group is whole and aligned, else every 32nd.
-    bool whole[U];
-    int left[U];
+// A lane's operands on their way: slots in shared memory, of four values of each
+// array, which only this thread writes and reads.
+template <class T, bool EIGHT> struct AdamRing {
+  static constexpr int slots = 4, value = 4 * int(sizeof(T)), moment = EIGHT ? 4 : 16;
+  static constexpr int bytes = slots * 2 * (value + moment) * kAdamThreads;
+  uint8_t *at;   // of slot 0: x, g, m and v of all threads, one after the other
+  __device__ __forceinline__ explicit AdamRing(void *shared) : at(static_cast<uint8_t *>(shared)) {}
+  template <int BYTES> __device__ __forceinline__ void copy(int offset, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(uint32_t(__cvta_generic_to_shared(at + offset))), "l"(from),
+                 "n"(BYTES)
+                 : "memory");
+  }
+  __device__ __forceinline__ int place(int slot) const { return slot * 2 * (value + moment) * kAdamThreads; }
+  __device__ __forceinline__ void ask(int slot, const AdamTensor &t, int64_t here) {
+    const int o = place(slot), tid = threadIdx.x;
+    copy<value>(o + value * tid, static_cast<const T *>(t.param) + here);
+    copy<value>(o + value * (kAdamThreads + tid), static_cast<const T *>(t.grad) + here);
+    const int64_t byte = here * (EIGHT ? 1 : 4);
+    copy<moment>(o + 2 * value * kAdamThreads + moment * tid, static_cast<const uint8_t *>(t.m) + byte);
+    copy<moment>(o + 2 * value * kAdamThreads + moment * (kAdamThreads + tid), static_cast<const uint8_t *>(t.v) + byte);
+  }
+};
+
+// One lane's four values of a group.  WHOLE: neighbours in memory, `at` the first
+// lane's; else every 32nd, `left` of the group.
+template <class T, bool EIGHT> struct AdamLane {
+  float x[4], g[4], m[4], v[4];
+  uint32_t cm[4], cv[4];   // codes; of a whole group all four in the first, until step()
+  uint32_t me, ve;
+  __device__ __forceinline__ void load(const AdamRing<T, EIGHT> &ring, int slot) {
+    using R = AdamRing<T, EIGHT>;
+    const int o = ring.place(slot), tid = threadIdx.x;
+    loadFour(x, reinterpret_cast<const T *>(ring.at + o + R::value * tid));
+    loadFour(g, reinterpret_cast<const T *>(ring.at + o + R::value * (kAdamThreads + tid)));
+    const uint8_t *moments = ring.at + o + 2 * R::value * kAdamThreads;
+    if constexpr (EIGHT) {
+      cm[0] = reinterpret_cast<const uint32_t *>(moments)[tid];
+      cv[0] = reinterpret_cast<const uint32_t *>(moments)[kAdamThreads + tid];
+    } else {
+      loadFour(m, reinterpret_cast<const float *>(moments) + 4 * tid);
+      loadFour(v, reinterpret_cast<const float *>(moments) + 4 * (kAdamThreads + tid));
+    }
+  }
+  __device__ __forceinline__ void load(const AdamTensor &t, int64_t at, int left, int lane) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = (firstGroup + u) * kMomentGroup;
-      left[u] = int(max(int64_t(0), min(int64_t(kMomentGroup), t.n - at)));
-      whole[u] = t.pieces && left[u] == kMomentGroup;
-      uint32_t me = 0, ve = 0;
-      int lowM = 0, lowV = 0;
-      if (EIGHT && left[u] > 0) {
-        me = t.me[firstGroup + u], ve = t.ve[firstGroup + u];
-        lowM = lowestCode<127>(me), lowV = lowestCode<255>(ve);
-      }
-      auto decode = [&](int i, int8_t cm, uint8_t cv) {
-        const float magnitude = momentValue(abs(int(cm)), lowM, me);
-        m[u][i] = cm < 0 ? -magnitude : magnitude;
-        v[u][i] = momentValue(cv, lowV, ve);
-      };
-      if (whole[u]) {
-        const int64_t here = at + 4 * lane;
-        loadFour(x[u], param + here);
-        loadFour(g[u], grad + here);
-        if constexpr (EIGHT) {
-          const char4 cm = *reinterpret_cast<const char4 *>(static_cast<const int8_t *>(t.m) + here);
-          const uchar4 cv = *reinterpret_cast<const uchar4 *>(static_cast<const uint8_t *>(t.v) + here);
-          decode(0, cm.x, cv.x);
-          decode(1, cm.y, cv.y);
-          decode(2, cm.z, cv.z);
-          decode(3, cm.w, cv.w);
-        } else {
-          loadFour(m[u], static_cast<const float *>(t.m) + here);
-          loadFour(v[u], static_cast<const float *>(t.v) + here);
-        }
+    for (int i = 0; i < 4; ++i) {
+      const int64_t here = at + lane + 32 * i;
+      const bool in = lane + 32 * i < left;
+      x[i] = in ? toFloat(static_cast<const T *>(t.param)[here]) : 0.f;
+      g[i] = in ? toFloat(static_cast<const T *>(t.grad)[here]) : 0.f;
+      if constexpr (EIGHT) {
+        cm[i] = in ? uint32_t(int(static_cast<const int8_t *>(t.m)[here])) : 0u;
+        cv[i] = in ? uint32_t(static_cast<const uint8_t *>(t.v)[here]) : 0u;
       } else {
+        m[i] = in ? static_cast<const float *>(t.m)[here] : 0.f;
+        v[i] = in ? static_cast<const float *>(t.v)[here] : 0.f;
+      }
+    }
+  }
+  template <bool WHOLE> __device__ __forceinline__ void step(const AdamTensor &t, const AdamArgs &p, const AdamScalars &s,
+                                                             uint32_t key, int64_t at, int left, int lane) {
+    const float beta1 = float(p.beta1), rest1 = float(1.0 - p.beta1), beta2 = float(p.beta2), rest2 = float(1.0 - p.beta2);
+    if constexpr (EIGHT) {   // values of the codes
+      const int lowM = lowestCode<127>(me), lowV = lowestCode<255>(ve);
+      const uint32_t packedM = cm[0], packedV = cv[0];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = WHOLE ? int(int8_t(packedM >> 8 * i)) : int(cm[i]);
+        m[i] = __uint_as_float(__float_as_uint(momentValue(abs(c), lowM)) | (uint32_t(c) & 0x80000000u));
+        v[i] = momentValue(WHOLE ? int(packedV >> 8 * i & 0xff) : int(cv[i]), lowV);
+      }
+      if (me == 255 || ve == 255) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool in = lane + 32 * i < left[u];
-          const int64_t here = at + lane + 32 * i;
-          x[u][i] = in ? toFloat(param[here]) : 0.f;
-          g[u][i] = in ? toFloat(grad[here]) : 0.f;
-          if constexpr (EIGHT) {
-            decode(i, in ? static_cast<const int8_t *>(t.m)[here] : int8_t(0),
-                   in ? static_cast<const uint8_t *>(t.v)[here] : uint8_t(0));
-            if (!in) m[u][i] = v[u][i] = 0.f;   // (in a group of NaN)
-          } else {
-            m[u][i] = in ? static_cast<const float *>(t.m)[here] : 0.f;
-            v[u][i] = in ? static_cast<const float *>(t.v)[here] : 0.f;
-          }
+          const bool in = WHOLE || lane + 32 * i < left;
+          if (me == 255 && in) m[i] = __int_as_float(0x7fffffff);
+          if (ve == 255 && in) v[i] = __int_as_float(0x7fffffff);
         }
       }
     }
+    uint32_t largestM = 0, largestV = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = (firstGroup + u) * kMomentGroup;
-      uint32_t largestM = 0, largestV = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float gi = p.sumCount ? __fmul_rn(g[u][i], s.clip) : g[u][i];
-        m[u][i] = __fadd_rn(__fmul_rn(m[u][i], beta1), __fmul_rn(gi, rest1));
-        v[u][i] = __fadd_rn(__fmul_rn(v[u][i], beta2), __fmul_rn(__fmul_rn(gi, gi), rest2));
-        const bool in = whole[u] || lane + 32 * i < left[u];
-        if (EIGHT && in) {
-          largestM = max(largestM, __float_as_uint(m[u][i]) & 0x7fffffffu);
-          largestV = max(largestV, __float_as_uint(v[u][i]) & 0x7fffffffu);
-        }
+    for (int i = 0; i < 4; ++i) {
+      const float gi = p.sumCount ? __fmul_rn(g[i], s.clip) : g[i];
+      m[i] = __fadd_rn(__fmul_rn(m[i], beta1), __fmul_rn(gi, rest1));
+      v[i] = __fadd_rn(__fmul_rn(v[i], beta2), __fmul_rn(__fmul_rn(gi, gi), rest2));
+      if (EIGHT && (WHOLE || lane + 32 * i < left)) {
+        largestM = max(largestM, __float_as_uint(m[i]) & 0x7fffffffu);
+        largestV = max(largestV, __float_as_uint(v[i]) & 0x7fffffffu);
       }
-      uint32_t me = 0, ve = 0;
-      int lowM = 0, lowV = 0;
+    }
+    int lowM = 0, lowV = 0;
+    if constexpr (EIGHT) {
+      me = __reduce_max_sync(0xffffffffu, largestM) >> 23;
+      ve = __reduce_max_sync(0xffffffffu, largestV) >> 23;
+      lowM = lowestCode<127>(me), lowV = lowestCode<255>(ve);
+    }
+    T out[4];
+    const uint32_t mixed = key ^ uint32_t(at + (WHOLE ? 4 * lane : 0));   // (at is a multiple of 128)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t noise = 0;
+      if (EIGHT || sizeof(T) == 2) noise = mixBits(WHOLE ? mixed ^ uint32_t(i) : mixed ^ uint32_t(lane + 32 * i));
+      out[i] = adamRounded<T>(adamParameter(x[i], m[i], v[i], s, p.eps), noise);
       if constexpr (EIGHT) {
-        me = __reduce_max_sync(0xffffffffu, largestM) >> 23;
-        ve = __reduce_max_sync(0xffffffffu, largestV) >> 23;
-        lowM = lowestCode<127>(me), lowV = lowestCode<255>(ve);
+        const uint32_t bits = __float_as_uint(m[i]), square = __float_as_uint(v[i]) & 0x7fffffffu;
+        const int magnitude = momentCode<127, 0>(bits & 0x7fffffffu, (noise >> 20 << 8) + 128, lowM), sign = int(bits) >> 31;
+        cm[i] = uint32_t((magnitude ^ sign) - sign);
+        cv[i] = square == 0 ? 0u : uint32_t(momentCode<255, 1>(square, noise & 0xfffffu, lowV));
       }
-      T out[4];
-      int8_t cm[4];
-      uint8_t cv[4];
+    }
+    if constexpr (WHOLE) {
+      const int64_t here = at + 4 * lane;
+      storeFour(static_cast<T *>(t.param) + here, out);
+      if constexpr (EIGHT) {
+        auto packed = [](const uint32_t (&c)[4]) {
+          return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        };
+        *reinterpret_cast<uint32_t *>(static_cast<int8_t *>(t.m) + here) = packed(cm);
+        *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(t.v) + here) = packed(cv);
+      } else {
+        storeFour(static_cast<float *>(t.m) + here, m);
+        storeFour(static_cast<float *>(t.v) + here, v);
+      }
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t noise = 0;
-        if (EIGHT || sizeof(T) == 2)
-          noise = mixBits(key ^ uint32_t(at + (whole[u] ? 4 * lane + i : lane + 32 * i)));
-        out[i] = adamRounded<T>(adamParameter(x[u][i], m[u][i], v[u][i], s, p.eps), noise);
+        if (lane + 32 * i >= left) continue;
+        const int64_t here = at + lane + 32 * i;
+        static_cast<T *>(t.param)[here] = out[i];
         if constexpr (EIGHT) {
-          const uint32_t bits = __float_as_uint(m[u][i]), vbits = __float_as_uint(v[u][i]);
-          const int magnitude = max(0, min(127, momentCode(bits & 0x7fffffffu, (noise >> 20 << 8) + 128, lowM)));
-          cm[i] = int8_t(bits >> 31 ? -magnitude : magnitude);
-          cv[i] = vbits == 0 ? uint8_t(0) : uint8_t(max(1, min(255, momentCode(vbits & 0x7fffffffu, noise & 0xfffffu, lowV))));
-        }
-      }
-      if (whole[u]) {
-        const int64_t here = at + 4 * lane;
-        storeFour(param + here, out);
-        if constexpr (EIGHT) {
-          *reinterpret_cast<char4 *>(static_cast<int8_t *>(t.m) + here) = make_char4(cm[0], cm[1], cm[2], cm[3]);
-          *reinterpret_cast<uchar4 *>(static_cast<uint8_t *>(t.v) + here) = make_uchar4(cv[0], cv[1], cv[2], cv[3]);
+          static_cast<int8_t *>(t.m)[here] = int8_t(cm[i]);
+          static_cast<uint8_t *>(t.v)[here] = uint8_t(cv[i]);
         } else {
-          storeFour(static_cast<float *>(t.m) + here, m[u]);
-          storeFour(static_cast<float *>(t.v) + here, v[u]);
+          static_cast<float *>(t.m)[here] = m[i];
+          static_cast<float *>(t.v)[here] = v[i];
         }
-      } else {
+      }
+    }
+  }
+};
+
+// A block's chunk is p.rounds groups for each of its warps, its groups in turn.
+template <class T, bool EIGHT, int MOST>
+__global__ void __launch_bounds__(kAdamThreads, 4) adamStep(const __grid_constant__ AdamTable<MOST> table, AdamArgs p) {
+  extern __shared__ __align__(16) uint8_t shared[];
+  using Ring = AdamRing<T, EIGHT>;
+  Ring ring(shared);
+  const AdamScalars s = adamScalars(p);
+  constexpr int kWarps = kAdamThreads / 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  for (int chunk = blockIdx.x, index = 0; chunk < p.chunks; chunk += gridDim.x) {
+    index = tensorOf(table, p.count, chunk, index);
+    const AdamTensor &t = table.t[index];
+    const uint32_t key = mixBits(s.count + 0x9e3779b9u * (uint32_t(t.place) + 1));
+    const int64_t begin = int64_t(chunk - t.first) * p.rounds * kWarps * kMomentGroup;
+    const int groups = int(min(int64_t(p.rounds) * kWarps, (t.n - begin + kMomentGroup - 1) / kMomentGroup));
+    const int whole = t.pieces ? int(min(int64_t(groups), (t.n - begin) / kMomentGroup)) : 0;
+    AdamLane<T, EIGHT> values;
+    if (warp < whole) {
+      const int count = (whole - warp + kWarps - 1) / kWarps;   // at most 32
+      const int64_t first = begin + warp * kMomentGroup, mine = first / kMomentGroup + lane * kWarps;
+      // The exponents of the warp's groups: lane i has the i-th one's.
+      uint32_t me = 0, ve = 0;
+      if (EIGHT && lane < count) me = t.me[mine], ve = t.ve[mine];
+      auto ask = [&](int i) {
+        if (i < count) ring.ask(i % Ring::slots, t, first + int64_t(i) * kWarps * kMomentGroup + 4 * lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (lane + 32 * i >= left[u]) continue;
-          const int64_t here = at + lane + 32 * i;
-          param[here] = out[i];
-          if constexpr (EIGHT) {
-            static_cast<int8_t *>(t.m)[here] = cm[i];
-            static_cast<uint8_t *>(t.v)[here] = cv[i];
-          } else {
-            static_cast<float *>(t.m)[here] = m[u][i];
-            static_cast<float *>(t.v)[here] = v[u][i];
-          }
-        }
+      for (int i = 0; i < Ring::slots - 1; ++i) ask(i);
+      for (int i = 0; i < count; ++i) {
+        ask(i + Ring::slots - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(Ring::slots - 1) : "memory");
+        values.load(ring, i % Ring::slots);
+        if constexpr (EIGHT) values.me = __shfl_sync(0xffffffffu, me, i), values.ve = __shfl_sync(0xffffffffu, ve, i);
+        values.template step<true>(t, p, s, key, first + int64_t(i) * kWarps * kMomentGroup, kMomentGroup, lane);
+        if (EIGHT && lane == i) me = values.me, ve = values.ve;
       }
-      if (EIGHT && lane == 0 && left[u] > 0) {
-        t.me[firstGroup + u] = uint8_t(me);
-        t.ve[firstGroup + u] = uint8_t(ve);
-      }
+      if (EIGHT && lane < count) t.me[mine] = uint8_t(me), t.ve[mine] = uint8_t(ve);
+    }
+    for (int group = whole + warp; group < groups; group += kWarps) {
+      const int64_t at = begin + int64_t(group) * kMomentGroup;
+      const int left = int(min(int64_t(kMomentGroup), t.n - at));
+      if constexpr (EIGHT) values.me = t.me[at / kMomentGroup], values.ve = t.ve[at / kMomentGroup];
+      values.load(t, at, left, lane);
+      __syncwarp();   // every lane has read the exponents
+      values.template step<false>(t, p, s, key, at, left, lane);
+      if (EIGHT && lane == 0) t.me[at / kMomentGroup] = uint8_t(values.me), t.ve[at / kMomentGroup] = uint8_t(values.ve);
     }
   }
   finishStep(p, s.count);
@@ -354,24 +416,25 @@ __global__ void __launch_bounds__(kAdamThreads) adamStep(const __grid_constant__
 // or, where m is null, of v.
 template <int MOST>
 __global__ void __launch_bounds__(kAdamThreads) momentValues(const __grid_constant__ AdamTable<MOST> table, int count, int chunks) {
-  constexpr int U = kAdamAtOnce;
+  constexpr int U = kValuesChunk / kAdamRound;
   const int lane = threadIdx.x % 32;
-  for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    const AdamTensor &t = table.t[tensorOf(table, count, chunk)];
-    const int64_t firstGroup = int64_t(chunk - t.first) * (kAdamChunk / kMomentGroup) + threadIdx.x / 32 * U;
+  for (int chunk = blockIdx.x, index = 0; chunk < chunks; chunk += gridDim.x) {
+    index = tensorOf(table, count, chunk, index);
+    const AdamTensor &t = table.t[index];
+    const int64_t first = int64_t(chunk - t.first) * kValuesChunk + threadIdx.x / 32 * U * kMomentGroup;
     float *out = static_cast<float *>(t.param);
     const bool sign = t.m != nullptr;
     const uint8_t *codes = static_cast<const uint8_t *>(sign ? t.m : t.v), *exponents = sign ? t.me : t.ve;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = (firstGroup + u) * kMomentGroup;
-      const int left = int(max(int64_t(0), min(int64_t(kMomentGroup), t.n - at)));
-      if (left == 0) continue;
-      const uint32_t e = exponents[firstGroup + u];
+      const int64_t at = first + u * kMomentGroup;
+      if (at >= t.n) continue;
+      const int left = int(min(int64_t(kMomentGroup), t.n - at));
+      const uint32_t e = exponents[at / kMomentGroup];
       const int low = sign ? lowestCode<127>(e) : lowestCode<255>(e);
       auto value = [&](uint8_t code) {
         const int c = sign ? int(int8_t(code)) : int(code);
-        const float magnitude = momentValue(abs(c), low, e);
+        const float magnitude = e == 255 ? __int_as_float(0x7fffffff) : momentValue(abs(c), low);
         return c < 0 ? -magnitude : magnitude;
       };
       if (t.pieces && left == kMomentGroup) {

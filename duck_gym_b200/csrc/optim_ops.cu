@@ -4,6 +4,8 @@
 #include "capi.hpp"
 
 #include <algorithm>
+#include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <vector>
 
@@ -63,10 +65,24 @@ void tensorsChecked(const duck_adamw_tensor *tensors, int count) {
   }
 }
 
+// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device
+// (by whichever thread comes first).
+template <auto kernel> void allowShared(int bytes) {
+  static std::atomic<bool> done[64] = {};
+  int device = 0;
+  check(cudaGetDevice(&device), "cudaGetDevice");
+  if (device < 64 && done[device]) return;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute");
+  if (device < 64) done[device] = true;
+}
+
 template <class T, bool EIGHT, int MOST>
 void launchStep(const AdamTable<MOST> &table, const AdamArgs &args, cudaStream_t stream) {
   const int blocks = std::max(1, std::min(args.chunks, 148 * 4));
-  adamStep<T, EIGHT, MOST><<<blocks, kAdamThreads, 0, stream>>>(table, args);
+  constexpr auto kernel = adamStep<T, EIGHT, MOST>;
+  constexpr int bytes = AdamRing<T, EIGHT>::bytes;
+  if constexpr (bytes + 1024 > 48 * 1024) allowShared<kernel>(bytes);   // (there is some beside it)
+  kernel<<<blocks, kAdamThreads, bytes, stream>>>(table, args);
 }
 
 }  // namespace
@@ -104,7 +120,7 @@ int duck_adamw_step(const duck_adamw_tensor *tensors, int count, const duck_adam
     require(o.step && on(o.step, 8), "The step count is an int64 on an 8-byte boundary");
     require(o.bits == 8 || o.bits == 32, "Moments have 8 or 32 bits");
     require(o.beta1 >= 0 && o.beta1 < 1 && o.beta2 >= 0 && o.beta2 < 1, "Invalid betas");
-    require(o.eps >= 0 && std::isfinite(o.eps) && o.weight_decay >= 0 && std::isfinite(o.weight_decay),
+    require((o.eps == 0 || o.eps >= FLT_MIN) && std::isfinite(float(o.eps)) && o.weight_decay >= 0 && std::isfinite(o.weight_decay),
             "Invalid eps or weight decay");
     require(o.rate || std::isfinite(o.rate_value), "Invalid learning rate");
     require(o.sum_count >= 0 && o.sum_count <= kNormBlocks && (o.sum_count == 0 || (o.sums && o.max_norm >= 0)),
@@ -115,12 +131,16 @@ int duck_adamw_step(const duck_adamw_tensor *tensors, int count, const duck_adam
       require(t.n == 0 || o.bits == 32 || (t.exp_avg_exponents && t.exp_avg_sq_exponents), "Invalid arguments");
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    std::vector<Launch> launches = launchesOf(tensors, count, kAdamChunk, o.bits == 8);
+    // As many rounds a chunk as leave every block one: a chunk finds its tensor and fills its ring anew.
+    int64_t values = 0;
+    for (int i = 0; i < count; ++i) values += tensors[i].n;
+    const int rounds = int(std::max<int64_t>(1, std::min<int64_t>(kAdamRoundsMost, values / (int64_t(148) * 4 * kAdamRound))));
+    std::vector<Launch> launches = launchesOf(tensors, count, rounds * kAdamRound, o.bits == 8);
     if (launches.empty()) launches.push_back({DUCK_FLOAT32, {}, 0});   // the step is counted all the same
     for (size_t i = 0; i < launches.size(); ++i) {
       const Launch &l = launches[i];
       const AdamArgs args{o.step, o.rate, o.sums, o.rate_value, o.beta1, o.beta2, o.weight_decay, o.max_norm, float(o.eps),
-                          o.sum_count, int(l.tensors.size()), l.chunks, i + 1 == launches.size()};
+                          o.sum_count, int(l.tensors.size()), l.chunks, rounds, i + 1 == launches.size()};
       withTable(l, [&](const auto &table) {
         if (l.type == DUCK_FLOAT32) o.bits == 8 ? launchStep<float, true>(table, args, s) : launchStep<float, false>(table, args, s);
         else o.bits == 8 ? launchStep<bf16, true>(table, args, s) : launchStep<bf16, false>(table, args, s);
@@ -140,7 +160,7 @@ int duck_moment_values(const duck_adamw_tensor *tensors, int count, duck_stream 
               "Invalid arguments");
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    for (const Launch &l : launchesOf(tensors, count, kAdamChunk, true)) {
+    for (const Launch &l : launchesOf(tensors, count, kValuesChunk, true)) {
       withTable(l, [&](const auto &table) {
         constexpr int M = sizeof(table.t) / sizeof(AdamTensor);
         momentValues<M><<<std::min(l.chunks, 148 * 8), kAdamThreads, 0, s>>>(table, int(l.tensors.size()), l.chunks);

@@ -62,11 +62,11 @@ def state8_zeros(like, signed):
                   torch.zeros(_groups(like), dtype=torch.uint8, device=like.device))
 
 
-def _check_state8(state, shape, device, dtypes, what):
+def _check_state8(state, like, dtypes, what):
     codes, exponents = state
-    _require(codes.dtype in dtypes and exponents.dtype == torch.uint8 and codes.shape == shape
-             and exponents.shape == (_groups(codes),) and codes.device == exponents.device == device
-             and codes.is_contiguous() and exponents.is_contiguous(),
+    _require(codes.dtype in dtypes and exponents.dtype is torch.uint8 and codes.is_same_size(like) and exponents.dim() == 1
+             and exponents.numel() == (codes.numel() + GROUP - 1) // GROUP and codes.is_contiguous()
+             and exponents.is_contiguous() and codes.get_device() == exponents.get_device() == like.get_device(),
              f"{what}: a moment in 8 bits is dense codes of its tensor's shape and one exponent for 128 of them")
 
 
@@ -157,45 +157,52 @@ def _check_apart(written, read, what):
 
 
 def _checked(params, grads, exp_avgs, exp_avg_sqs):
-    """Whether the moments have 8 bits, the tensors' device and dense gradients."""
+    """Whether the moments have 8 bits, the tensors' device, and their rows of a
+    table, with dense gradients in the places of others (they are returned too, so
+    that they live until the launch)."""
     _require(len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) > 0,
              "adamw_step: one gradient and two moments for each of one or more parameters")
-    device = params[0].device
+    # This runs before every step: what says the same of a tensor in fewer calls is taken.
+    index = params[0].get_device()
     eight = not torch.is_tensor(exp_avgs[0])
-    dense, spans = [], []
-    span = lambda t: (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
-        _require(p.dtype in _TYPES and p.device == device and p.is_contiguous(),
+    dense, rows, written, read = [], [], [], []
+    for place, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        dtype = p.dtype
+        kind = _TYPES.get(dtype)
+        _require(kind is not None and p.get_device() == index and p.is_contiguous(),
                  "adamw_step: parameters are dense float32 or bfloat16 tensors of one device")
-        _require(g.shape == p.shape and g.dtype == p.dtype and g.device == device and not g.is_sparse,
+        _require(g.dtype is dtype and g.is_same_size(p) and g.get_device() == index and g.layout is torch.strided,
                  "adamw_step: a gradient has its parameter's shape, type and device")
         _require(torch.is_tensor(m) != eight and torch.is_tensor(v) != eight,
                  "adamw_step: all moments have 32 bits, or all have 8")
-        spans.append(span(p))
+        if not g.is_contiguous():
+            g = g.contiguous()
+        n = p.numel()
+        size = n << (2 - kind)
+        at, gat = p.data_ptr(), g.data_ptr()
         if eight:
-            _check_state8(m, p.shape, device, (torch.int8,), "adamw_step")
-            _check_state8(v, p.shape, device, (torch.uint8,), "adamw_step")
-            spans += [span(t) for t in (*m, *v)]
+            _check_state8(m, p, (torch.int8,), "adamw_step")
+            _check_state8(v, p, (torch.uint8,), "adamw_step")
+            mat, vat, meat, veat = m[0].data_ptr(), v[0].data_ptr(), m[1].data_ptr(), v[1].data_ptr()
+            groups = (n + GROUP - 1) // GROUP
+            spans = ((at, at + size), (mat, mat + n), (vat, vat + n), (meat, meat + groups), (veat, veat + groups))
         else:
-            for t in (m, v):
-                _require(t.dtype == torch.float32 and t.shape == p.shape and t.device == device and t.is_contiguous(),
-                         "adamw_step: moments are dense float32 tensors of their parameters' shapes")
-                spans.append(span(t))
-        dense.append(g if g.is_contiguous() else g.contiguous())
-    _check_apart([s for s in spans if s[1] > s[0]], [s for s in map(span, dense) if s[1] > s[0]], "adamw_step")
-    return eight, device, dense
+            _require(m.dtype is torch.float32 and v.dtype is torch.float32 and m.is_same_size(p) and v.is_same_size(p)
+                     and m.get_device() == index and v.get_device() == index and m.is_contiguous() and v.is_contiguous(),
+                     "adamw_step: moments are dense float32 tensors of their parameters' shapes")
+            mat, vat, meat, veat = m.data_ptr(), v.data_ptr(), 0, 0
+            spans = ((at, at + size), (mat, mat + 4 * n), (vat, vat + 4 * n))
+        if n:
+            written += spans
+            read.append((gat, gat + size))
+        dense.append(g)
+        rows.append((at, gat, mat, vat, meat, veat, n, kind, place))
+    _check_apart(written, read, "adamw_step")
+    return eight, params[0].device, rows, dense
 
 
 def _table(rows):
     return b"".join(_TENSOR.pack(*row) for row in rows)
-
-
-def _rows(params, grads, ms, vs, eight):
-    if eight:
-        return [(p.data_ptr(), g.data_ptr(), m[0].data_ptr(), v[0].data_ptr(), m[1].data_ptr(), v[1].data_ptr(), p.numel(),
-                 _TYPES[p.dtype], i) for i, (p, g, m, v) in enumerate(zip(params, grads, ms, vs))]
-    return [(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, p.numel(), _TYPES[p.dtype], i)
-            for i, (p, g, m, v) in enumerate(zip(params, grads, ms, vs))]
 
 
 class _Norm:
@@ -206,12 +213,11 @@ class _Norm:
         self.sums = (torch.empty(SUMS, dtype=torch.float64, device=device) if device.type == "cuda"
                      else torch.zeros((), dtype=torch.float64))
 
-    def add(self, grads):
+    def add(self, rows, grads):
         if self.sums.dim() == 0:
             for g in grads:
                 self.sums += g.double().square().sum()
             return
-        rows = [(0, g.data_ptr(), 0, 0, 0, 0, g.numel(), _TYPES[g.dtype], 0) for g in grads]
         count = ctypes.c_int()
         _launch(library().duck_gradient_squares, self.sums.device, _table(rows), len(rows), self.count,
                 self.sums.data_ptr(), ctypes.byref(count))
@@ -221,14 +227,13 @@ class _Norm:
             self.count = 1
 
 
-def _step(params, grads, ms, vs, eight, device, step, lr, betas, eps, weight_decay, max_norm, norm):
+def _step(params, grads, ms, vs, eight, device, rows, step, lr, betas, eps, weight_decay, max_norm, norm):
     if device.type != "cuda":
         return _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm,
                       None if norm is None else norm.sums)
     on_device = torch.is_tensor(lr) and lr.is_cuda
     if on_device and lr.dtype != torch.float32:
         lr = lr.float()
-    rows = _rows(params, grads, ms, vs, eight)
     options = _OPTIONS.pack(step.data_ptr(), lr.data_ptr() if on_device else 0, norm.sums.data_ptr() if norm else 0,
                             0.0 if on_device else float(lr), *betas, eps, weight_decay, 0.0 if norm is None else max_norm,
                             norm.count if norm else 0, 8 if eight else 32)
@@ -245,8 +250,9 @@ def _check_options(step, lr, betas, eps, weight_decay, max_norm, device):
     if torch.is_tensor(lr):
         _require(lr.numel() == 1 and lr.is_floating_point() and lr.device in (device, torch.device("cpu")),
                  "adamw_step: the learning rate is a number, or a floating tensor of one value")
-    _require(len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas) and 0.0 <= eps < math.inf
-             and 0.0 <= weight_decay < math.inf, "adamw_step: betas in [0, 1), eps and weight decay of 0 or more")
+    _require(len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas) and (eps == 0.0 or 2.0 ** -126 <= eps < 2.0 ** 127)
+             and 0.0 <= weight_decay < math.inf,
+             "adamw_step: betas in [0, 1), eps 0 or a normal float32 number, weight decay of 0 or more")
     _require(max_norm is None or max_norm >= 0.0, "adamw_step: a norm of 0 or more")
 
 
@@ -267,30 +273,35 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999
     bfloat16 parameters and codes are rounded up or down at random, by a hash of t, the
     tensor's place in the list and the value's place in the tensor: what a step adds is
     mostly less than half a place of theirs, and would be lost."""
-    eight, device, grads = _checked(params, grads, exp_avgs, exp_avg_sqs)
+    eight, device, rows, grads = _checked(params, grads, exp_avgs, exp_avg_sqs)
     _check_options(step, lr, betas, eps, weight_decay, max_norm, device)
     norm = None
     if max_norm is not None:
         norm = _Norm(device)
-        norm.add(grads)
-    _step(params, grads, exp_avgs, exp_avg_sqs, eight, device, step, lr, betas, eps, weight_decay, max_norm, norm)
+        norm.add(rows, grads)
+    _step(params, grads, exp_avgs, exp_avg_sqs, eight, device, rows, step, lr, betas, eps, weight_decay, max_norm, norm)
 
 
 @torch.no_grad()
 def state8_values(states):
-    """The float32 tensors that moments in 8 bits stand for."""
-    states = [State8(*s) for s in states]
+    """The float32 tensors that moments in 8 bits stand for (on the GPU, parts of one
+    buffer)."""
+    states = list(states)
     if not states:
         return []
-    device = states[0].codes.device
     for s in states:
-        _check_state8(s, s.codes.shape, device, (torch.int8, torch.uint8), "state8_values")
+        _check_state8(s, s[0], (torch.int8, torch.uint8), "state8_values")
+        _require(s[0].get_device() == states[0][0].get_device(), "state8_values: states of one device")
+    device = states[0][0].device
     if device.type != "cuda":
         return [_decode(*s) for s in states]
-    values = [torch.empty(s.codes.shape, dtype=torch.float32, device=device) for s in states]
+    # One allocation, each tensor on a 16-byte boundary.
+    sizes = [(codes.numel(), -codes.numel() % 4) for codes, _ in states]
+    flat = torch.empty(sum(map(sum, sizes)), dtype=torch.float32, device=device).split([n for pair in sizes for n in pair])[::2]
+    values = [v if s[0].dim() == 1 else v.view(s[0].shape) for v, s in zip(flat, states)]
     rows = []
-    for value, (codes, exponents) in zip(values, states):
-        signed = codes.dtype == torch.int8
+    for value, (codes, exponents) in zip(flat, states):
+        signed = codes.dtype is torch.int8
         m, me, v, ve = (codes.data_ptr(), exponents.data_ptr(), 0, 0) if signed else (0, 0, codes.data_ptr(), exponents.data_ptr())
         rows.append((value.data_ptr(), 0, m, v, me, ve, codes.numel(), 0, 0))
     _launch(library().duck_moment_values, device, _table(rows), len(rows))
@@ -344,17 +355,17 @@ class AdamW(torch.optim.Optimizer):
                 group["step"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
             moments = [self._moments(p, group["bits"]) for p in params]
             ms, vs = [m for m, _ in moments], [v for _, v in moments]
-            eight, device, grads = _checked(params, [p.grad for p in params], ms, vs)
+            eight, device, rows, grads = _checked(params, [p.grad for p in params], ms, vs)
             _check_options(group["step"], group["lr"], group["betas"], group["eps"], group["weight_decay"],
                            self.max_grad_norm, device)
             if self.max_grad_norm is not None:
                 _require(not norms or device in norms, "AdamW: one device where gradients are clipped")
                 norms.setdefault(device, None)
                 norms[device] = norms[device] or _Norm(device)
-                norms[device].add(grads)
-            work.append((params, grads, ms, vs, eight, device, group))
-        for params, grads, ms, vs, eight, device, group in work:
-            _step(params, grads, ms, vs, eight, device, group["step"], group["lr"], group["betas"], group["eps"],
+                norms[device].add(rows, grads)
+            work.append((params, grads, ms, vs, eight, device, rows, group))
+        for params, grads, ms, vs, eight, device, rows, group in work:
+            _step(params, grads, ms, vs, eight, device, rows, group["step"], group["lr"], group["betas"], group["eps"],
                   group["weight_decay"], self.max_grad_norm, norms.get(device))
         return loss
 
