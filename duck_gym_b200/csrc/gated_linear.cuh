@@ -15,7 +15,7 @@
 // forward passes keep x only.
 //
 // One block a multiprocessor goes through tiles of 128 rows: one thread issues the
-// copies, one the products, eight warps take finished accumulators out, while the
+// copies, one the products, sixteen warps take finished accumulators out, while the
 // products of the next tile go to the other half of tensor memory.
 //
 // float32 (gatedProducts): FMA in pairs; a and u are kept, since they are exact and
@@ -41,8 +41,16 @@ template <int ACT, bool FAST> __device__ __forceinline__ Activated activate(floa
     const float density = 0.39894228f * (FAST ? __expf(-0.5f * a * a) : expf(-0.5f * a * a));
     return {a * below, below + a * density};
   } else {
-    const float s = FAST ? __fdividef(1.f, 1.f + __expf(-a)) : 1.f / (1.f + expf(-a));
-    const float rest = FAST ? 1.f - s : 1.f / (1.f + expf(a));
+    float s, rest;
+    if constexpr (FAST) {   // (exp(-a) is held below 2^126; a NaN stays one)
+      float t;
+      asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(t) : "f"(a * -1.4426950408889634f));
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + t));
+      rest = t * s;
+    } else {
+      s = 1.f / (1.f + expf(-a)), rest = 1.f / (1.f + expf(a));
+    }
     if constexpr (ACT == kSilu) return {a * s, s + a * s * rest};
     else return {s, s * rest};
   }
@@ -80,24 +88,24 @@ struct TileMaps {
   CUtensorMap a0, a1, b0, b1;
 };
 
-constexpr int kTileThreads = 384, kTileRows = 128, kTileSteps = 64, kTileWarps = 8;
+constexpr int kTileWarps = 16, kTileThreads = 128 + 32 * kTileWarps, kTileRows = 128, kTileSteps = 64, kTileChunk = 16;
 template <int BN> struct TileShared {
   static constexpr int stages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
   static constexpr int a = kTileRows * kTileSteps * 2, b = BN * kTileSteps * 2;
-  static constexpr int staging = 32 * 64, bias = 2 * 32 * 4;   // of a warp
+  static constexpr int staging = 32 * 32, bias = 2 * kTileChunk * 4;   // of a warp
   static constexpr int bytes = 1024 + stages * (a + b) + kTileWarps * (staging + bias) + 256;
 };
 
-// A warp's 32 rows of 64 bytes: pieces of 16 bytes, so placed that neither rows of
-// pieces nor columns of them meet in a bank.
+// A warp's 32 rows of 32 bytes: two pieces of 16 bytes, so placed that neither rows
+// of pieces nor columns of them meet in a bank.
 __device__ __forceinline__ uint4 *stagedPiece(uint4 *staging, int row, int piece) {
-  return staging + row * 4 + (piece ^ (row >> 1 & 3));
+  return staging + row * 2 + (piece ^ (row >> 2 & 1));
 }
 
-// Column sums over the 32 lanes: lane i is left with column i's.
-__device__ __forceinline__ float columnSum(float (&x)[32], int lane) {
+// Column sums over the 32 lanes: lane i is left with column i % 16's.
+__device__ __forceinline__ float columnSum(float (&x)[kTileChunk], int lane) {
 #pragma unroll
-  for (int half = 16; half > 0; half /= 2) {
+  for (int half = kTileChunk / 2; half > 0; half /= 2) {
     const bool upper = lane & half;
 #pragma unroll
     for (int i = 0; i < half; ++i) {
@@ -105,42 +113,49 @@ __device__ __forceinline__ float columnSum(float (&x)[32], int lane) {
       x[i] = keep + __shfl_xor_sync(0xffffffffu, send, half);
     }
   }
-  return x[0];
+  return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 16);
 }
 
-// A warp's rows of 32 bfloat16 columns, one row a lane, to memory: `columns` of them
-// exist; whole pieces where rows are made of them.
-__device__ __forceinline__ void storeRows(uint4 *staging, const float (&x)[32], bf16 *to, int64_t rowStride, int64_t rowsLeft,
-                                          int columns, bool pieces, int lane) {
-#pragma unroll
-  for (int piece = 0; piece < 4; ++piece) {
-    uint4 v;
-    uint32_t *w = reinterpret_cast<uint32_t *>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 two = __floats2bfloat162_rn(x[piece * 8 + 2 * i], x[piece * 8 + 2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t *>(&two);
-    }
-    *stagedPiece(staging, lane, piece) = v;
-  }
+// A warp's rows of 32 bytes, one row a lane as two pieces, to memory, a row's pieces
+// by neighbouring lanes: `values` of E a row exist; whole pieces where rows are made
+// of them.
+template <class E> __device__ __forceinline__ void storeRows(uint4 *staging, uint4 first, uint4 second, E *to, int64_t rowStride,
+                                                             int64_t rowsLeft, int values, bool pieces, int lane) {
+  constexpr int V = 16 / sizeof(E);
+  *stagedPiece(staging, lane, 0) = first;
+  *stagedPiece(staging, lane, 1) = second;
   __syncwarp();
-  const int piece = lane % 4;
+  const int piece = lane % 2;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = lane / 4 + 8 * i;
-    if (row >= rowsLeft || piece * 8 >= columns) continue;
+  for (int i = 0; i < 2; ++i) {
+    const int row = lane / 2 + 16 * i;
+    if (row >= rowsLeft || piece * V >= values) continue;
     const uint4 v = *stagedPiece(staging, row, piece);
-    bf16 *at = to + row * rowStride + piece * 8;
-    if (pieces && piece * 8 + 8 <= columns) {
+    E *at = to + row * rowStride + piece * V;
+    if (pieces && piece * V + V <= values) {
       *reinterpret_cast<uint4 *>(at) = v;
     } else {
-      const bf16 *e = reinterpret_cast<const bf16 *>(&v);
+      const E *e = reinterpret_cast<const E *>(&v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (piece * 8 + j < columns) at[j] = e[j];
+      for (int j = 0; j < V; ++j)
+        if (piece * V + j < values) at[j] = e[j];
     }
   }
   __syncwarp();
+}
+// Eight floats, rounded.
+__device__ __forceinline__ uint4 eightOf(const float *x) {
+  uint4 v;
+  uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t *>(&two);
+  }
+  return v;
+}
+__device__ __forceinline__ uint4 fourOf(const float *x) {
+  return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
 }
 
 template <Pass PASS, int BN> __global__ void __launch_bounds__(kTileThreads, 1)
@@ -280,7 +295,9 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
       }
     }
   } else if (warp >= 4) {
-    const int quarter = warp % 4, half = (warp - 4) / 4;   // of the tile's rows, and of its columns
+    // A warp has a quarter of the tile's rows (that of tensor memory which it reaches) and of its columns.
+    constexpr int kChunk = kTileChunk, kPart = kColumns / 4 < kChunk ? kChunk : kColumns / 4;
+    const int quarter = warp % 4, part = (warp - 4) / 4;
     uint4 *stage = reinterpret_cast<uint4 *>(staging + (warp - 4) * S::staging);
     float *bias = biases + (warp - 4) * S::bias / 4;
     int n = 0;
@@ -289,46 +306,59 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
       const int buffer = n & 1;
       int first;
       const int steps = stepsOf(at, first);
-      const bool fine = __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken));
-      tensorFenceAfter();
-      const uint32_t tensorRow = accumulators + buffer * BN + (uint32_t(quarter * 32) << 16);
       const int64_t row = at.row + quarter * 32;
       const int64_t rowsLeft = (PASS == Pass::weights ? int64_t(p.F) : p.rows) - row;
-      constexpr int kChunk = kColumns / 2 < 32 ? kColumns / 2 : 32;
-      // 32 columns of the accumulators from `column` on (16 of them beyond kChunk's are not read); zero where a tile has no steps.
-      auto take = [&](float (&x)[32], int column) {
+      const bool mine = lane < rowsLeft;
+      // What the tile needs of memory is asked for before its products are waited for.
+      constexpr int kChunks = kPart / kChunk;
+      uint4 gradients[PASS == Pass::gradients ? kChunks : 1][2];
+      float biasOf[kDual ? kChunks : 1];
+      if constexpr (kDual) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = fine ? 0.f : __int_as_float(0x7fffffff);
-        if (fine && steps > 0) {
-          tensorLoad16(x, tensorRow + column);
-          if (kChunk > 16) tensorLoad16(x + 16, tensorRow + column + 16);
-        }
-      };
-      for (int c = half * (kColumns / 2); c < (half + 1) * (kColumns / 2); c += kChunk) {
-        const int column = at.column + c;
-        if constexpr (kDual) {
-          const int columns = min(kChunk, p.F - column);
-          if (columns <= 0) break;
-          float a[32], u[32];
-          take(a, c);
-          take(u, BN / 2 + c);
-          uint4 dh[4];
-          const bool mine = lane < rowsLeft;
+        for (int k = 0; k < kChunks; ++k) {
+          const int c = part * kPart + k * kChunk, column = at.column + c, columns = c < kColumns ? min(kChunk, p.F - column) : 0;
           if constexpr (PASS == Pass::gradients) {
             const bf16 *from = p.dh + (row + lane) * p.dhStride + column;
             if (p.wholeDh && columns == kChunk) {
 #pragma unroll
-              for (int i = 0; i < kChunk / 8; ++i) dh[i] = mine ? reinterpret_cast<const uint4 *>(from)[i] : make_uint4(0, 0, 0, 0);
+              for (int i = 0; i < 2; ++i)
+                gradients[k][i] = mine ? reinterpret_cast<const uint4 *>(from)[i] : make_uint4(0, 0, 0, 0);
             } else {
-              bf16 *e = reinterpret_cast<bf16 *>(dh);
+              bf16 *e = reinterpret_cast<bf16 *>(gradients[k]);
 #pragma unroll
               for (int i = 0; i < kChunk; ++i) e[i] = mine && i < columns ? from[i] : __ushort_as_bfloat16(0);
             }
           }
           if (p.bGate) {
-            const bool in = lane < columns;
-            bias[lane] = in ? toFloat(p.bGate[column + lane]) : 0.f;
-            bias[32 + lane] = in ? toFloat(p.bUp[column + lane]) : 0.f;
+            const int i = lane % kChunk;
+            biasOf[k] = i < columns ? toFloat((lane < kChunk ? p.bGate : p.bUp)[column + i]) : 0.f;
+          }
+        }
+      }
+      const bool fine = __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken));
+      tensorFenceAfter();
+      const uint32_t tensorRow = accumulators + buffer * BN + (uint32_t(quarter * 32) << 16);
+      // Columns of the accumulators from `column` on; zero where a tile has no steps.
+      auto take = [&](float (&x)[kChunk], int column) {
+        if (fine && steps > 0) {
+          tensorLoad16(x, tensorRow + column);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) x[i] = fine ? 0.f : __int_as_float(0x7fffffff);
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const int c = part * kPart + k * kChunk;
+        const int column = at.column + c, columns = c < kColumns ? min(kChunk, (kDual ? p.F : p.D) - column) : 0;
+        if (columns <= 0) break;
+        __syncwarp();   // loads from tensor memory are the whole warp's
+        if constexpr (kDual) {
+          float a[kChunk], u[kChunk];
+          take(a, c);
+          take(u, BN / 2 + c);
+          if (p.bGate) {
+            bias[lane] = biasOf[k];
             __syncwarp();
           }
           tensorLoadWait();
@@ -336,7 +366,11 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
           tensorLoaded(u);
           if (p.bGate) {
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) a[i] += bias[i], u[i] += bias[32 + i];
+            for (int i = 0; i < kChunk; i += 4) {
+              const float4 g = *reinterpret_cast<const float4 *>(bias + i), b = *reinterpret_cast<const float4 *>(bias + kChunk + i);
+              a[i] += g.x, a[i + 1] += g.y, a[i + 2] += g.z, a[i + 3] += g.w;
+              u[i] += b.x, u[i + 1] += b.y, u[i + 2] += b.z, u[i + 3] += b.w;
+            }
             __syncwarp();
           }
           withActivation(p.activation, [&](auto kind) {
@@ -346,26 +380,24 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
               if constexpr (PASS == Pass::forward) {
                 a[i] = f.y * u[i];
               } else {
-                const float d = toFloat(reinterpret_cast<const bf16 *>(dh)[i]);
+                const uint32_t two = reinterpret_cast<const uint32_t *>(gradients[k])[i / 2];
+                const float d = __uint_as_float(i % 2 ? two & 0xffff0000u : two << 16);
                 a[i] = d * u[i] * f.slope;
                 u[i] = d * f.y;
               }
             }
           });
           if constexpr (PASS == Pass::forward) {
-            storeRows(stage, a, p.h + row * p.F + column, p.F, rowsLeft, columns, p.wholeH, lane);
+            storeRows(stage, eightOf(a), eightOf(a + 8), p.h + row * p.F + column, p.F, rowsLeft, columns, p.wholeH, lane);
           } else {
             bf16 *to = p.both + row * 2 * p.stride + column;
-            storeRows(stage, a, to, 2 * int64_t(p.stride), rowsLeft, columns, true, lane);
-            storeRows(stage, u, to + p.stride, 2 * int64_t(p.stride), rowsLeft, columns, true, lane);
+            const int64_t stride = 2 * int64_t(p.stride);
+            storeRows(stage, eightOf(a), eightOf(a + 8), to, stride, rowsLeft, columns, true, lane);
+            storeRows(stage, eightOf(u), eightOf(u + 8), to + p.stride, stride, rowsLeft, columns, true, lane);
             if (p.biasParts) {
               if (!mine) {   // (a row that is not there may have become NaN beside an infinite bias)
 #pragma unroll
                 for (int i = 0; i < kChunk; ++i) a[i] = u[i] = 0.f;
-              }
-              if (kChunk < 32) {
-#pragma unroll
-                for (int i = kChunk; i < 32; ++i) a[i] = u[i] = 0.f;
               }
               const float sumA = columnSum(a, lane), sumU = columnSum(u, lane);
               float *parts = p.biasParts + (int64_t(at.row / kTileRows) * 4 + quarter) * 2 * p.F + column;
@@ -373,35 +405,19 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
             }
           }
         } else {
-          const int columns = min(kChunk, p.D - column);
-          if (columns <= 0) break;
-          float x[32];
+          float x[kChunk];
           take(x, c);
           tensorLoadWait();
           tensorLoaded(x);
           if constexpr (PASS == Pass::input) {
-            storeRows(stage, x, p.dx + row * p.D + column, p.D, rowsLeft, columns, true, lane);
+            storeRows(stage, eightOf(x), eightOf(x + 8), p.dx + row * p.D + column, p.D, rowsLeft, columns, true, lane);
           } else if (p.splits == 1) {
-            storeRows(stage, x, (at.half ? p.dwUp : p.dwGate) + row * p.D + column, p.D, rowsLeft, columns, true, lane);
+            storeRows(stage, eightOf(x), eightOf(x + 8), (at.half ? p.dwUp : p.dwGate) + row * p.D + column, p.D, rowsLeft, columns,
+                      true, lane);
           } else {
             float *to = p.parts + ((int64_t(at.split) * 2 + at.half) * p.F + row) * p.D + column;
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {   // 16 columns, 64 bytes of a row
-#pragma unroll
-              for (int piece = 0; piece < 4; ++piece) {
-                const float *v = x + part * 16 + piece * 4;
-                *reinterpret_cast<float4 *>(stagedPiece(stage, lane, piece)) = make_float4(v[0], v[1], v[2], v[3]);
-              }
-              __syncwarp();
-              const int piece = lane % 4;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int r = lane / 4 + 8 * i, at4 = part * 16 + piece * 4;   // (D is a multiple of 8)
-                if (r < rowsLeft && at4 < columns)
-                  *reinterpret_cast<float4 *>(to + int64_t(r) * p.D + at4) = *reinterpret_cast<float4 *>(stagedPiece(stage, r, piece));
-              }
-              __syncwarp();
-            }
+            storeRows(stage, fourOf(x), fourOf(x + 4), to, p.D, rowsLeft, columns, true, lane);
+            if (columns > 8) storeRows(stage, fourOf(x + 8), fourOf(x + 12), to + 8, p.D, rowsLeft, columns - 8, true, lane);
           }
         }
       }
@@ -626,7 +642,7 @@ template <class T> struct SumArgs {
   int64_t weights;   // F * D
   int F, splits, biasCount, weightBlocks;
 };
-constexpr int kSumThreads = 256;
+constexpr int kSumThreads = 256, kSumColumns = 8;
 template <class T> __global__ void __launch_bounds__(kSumThreads) sumParts(SumArgs<T> p) {
   if (int(blockIdx.x) < p.weightBlocks) {
     const int64_t i = (int64_t(blockIdx.x) * kSumThreads + threadIdx.x) * 4;
@@ -649,18 +665,21 @@ template <class T> __global__ void __launch_bounds__(kSumThreads) sumParts(SumAr
     }
     return;
   }
-  // Biases: a warp has 32 columns, the block's eight warps share the parts.
-  __shared__ float sums[kSumThreads / 32][32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, column = (int(blockIdx.x) - p.weightBlocks) * 32 + lane;
+  // Biases: a block has eight columns, a sector of each part, and as many parts at once as that leaves threads for.
+  constexpr int kAtOnce = kSumThreads / kSumColumns;
+  __shared__ float sums[kAtOnce][kSumColumns];
+  const int own = threadIdx.x % kSumColumns, from = threadIdx.x / kSumColumns;
+  const int column = (int(blockIdx.x) - p.weightBlocks) * kSumColumns + own;
   float sum = 0.f;
-  if (column < 2 * p.F)
+  if (column < 2 * p.F) {
 #pragma unroll 8
-    for (int n = warp; n < p.biasCount; n += kSumThreads / 32) sum += p.biasParts[int64_t(n) * 2 * p.F + column];
-  sums[warp][lane] = sum;
+    for (int n = from; n < p.biasCount; n += kAtOnce) sum += p.biasParts[int64_t(n) * 2 * p.F + column];
+  }
+  sums[from][own] = sum;
   __syncthreads();
-  if (warp > 0 || column >= 2 * p.F) return;
+  if (from > 0 || column >= 2 * p.F) return;
 #pragma unroll
-  for (int w = 1; w < kSumThreads / 32; ++w) sum += sums[w][lane];
+  for (int k = 1; k < kAtOnce; ++k) sum += sums[k][own];
   (column < p.F ? p.dbGate[column] : p.dbUp[column - p.F]) = fromFloat<T>(sum);
 }
 

@@ -153,8 +153,19 @@ struct GatedPlan {
   int64_t bothBytes, biasBytes, partBytes, keptBytes;
 };
 int64_t padded(int64_t bytes) { return ceilDiv(bytes, 256) * 256; }
-// As wide a tile as there are columns for.
-int tileColumns(int64_t columns) { return columns > 128 ? 256 : columns > 64 ? 128 : 64; }
+// Columns of a tile, of which a row of tiles has `columns`: rounds of tiles over the multiprocessors, times a tile's time.  A
+// product of 128 columns takes 0.77 of the time of one of 256: its operands' way out of shared memory bounds it (16384 x 4096
+// by 1024 twice: 291 us in tiles of 128 columns, 216 in those of 256).
+int tileColumns(int64_t rowTiles, int64_t columns) {
+  int best = 0;
+  int64_t least = 0;
+  for (int n : {256, 128, 64}) {
+    if (n > 64 && n / 2 >= columns) continue;
+    const int64_t cost = ceilDiv(rowTiles * ceilDiv(columns, n), 148) * (n == 256 ? 100 : n == 128 ? 77 : 65);
+    if (best == 0 || cost < least) best = n, least = cost;
+  }
+  return best;
+}
 GatedPlan planGated(const duck_gated &a) {
   GatedPlan p{};
   const bool weights = a.dw_gate != nullptr, biases = a.db_gate != nullptr;
@@ -163,8 +174,9 @@ GatedPlan planGated(const duck_gated &a) {
     p.stride = int(ceilDiv(a.F, 8) * 8);
     p.bothBytes = padded(rows * 2 * p.stride * 2);
     p.biasCount = ceilDiv(rows, kTileRows) * 4;
-    p.weightColumns = tileColumns(a.D);
-    // Rows are split so that the tiles fill the GPU once, into parts of 512 rows at least: a part's sums are written and read once more.
+    // Rows are split so that the tiles fill the GPU once, into parts of 512 rows at least: a part's sums are written and read
+    // once more (24576 rows, 256 x 512: 17 us in 18 parts of 256 columns, 20 in 9 of 128).
+    p.weightColumns = a.D > 128 ? 256 : a.D > 64 ? 128 : 64;
     const int64_t tiles = 2 * ceilDiv(a.F, kTileRows) * ceilDiv(a.D, p.weightColumns), steps = ceilDiv(rows, kTileSteps);
     p.splits = int(std::max<int64_t>(1, std::min<int64_t>(148 / tiles, steps / 8)));
     p.splits = int(std::max<int64_t>(1, ceilDiv(steps, std::max<int64_t>(1, ceilDiv(steps, p.splits)))));
@@ -222,7 +234,13 @@ template <Pass PASS, int BN> void launchTiles(const TileMaps &maps, const TileAr
   check(cudaGetLastError(), "gated linear launch");
 }
 
-// Both projections' tiles: as wide as leaves one for every multiprocessor.
+template <class F> void withColumns(int columns, F &&f) {
+  if (columns == 256) f(std::integral_constant<int, 256>());
+  else if (columns == 128) f(std::integral_constant<int, 128>());
+  else f(std::integral_constant<int, 64>());
+}
+
+// Both projections, side by side.
 template <Pass PASS> void launchProjections(const duck_gated &a, TileArgs t, cudaStream_t stream) {
   const int64_t rowTiles = ceilDiv(a.rows, kTileRows);
   auto run = [&](auto columns) {
@@ -238,16 +256,8 @@ template <Pass PASS> void launchProjections(const duck_gated &a, TileArgs t, cud
     t.tiles = int(tiles);
     launchTiles<PASS, BN>(maps, t, stream);
   };
-  if (rowTiles * ceilDiv(a.F, 128) >= 148) run(std::integral_constant<int, 256>());
-  else if (rowTiles * ceilDiv(a.F, 64) >= 148) run(std::integral_constant<int, 128>());
-  else run(std::integral_constant<int, 64>());
+  withColumns(tileColumns(rowTiles, 2 * int64_t(a.F)), run);
 }
-template <class F> void withColumns(int columns, F &&f) {
-  if (columns == 256) f(std::integral_constant<int, 256>());
-  else if (columns == 128) f(std::integral_constant<int, 128>());
-  else f(std::integral_constant<int, 64>());
-}
-
 TileArgs tileArgs(const duck_gated &a) {
   TileArgs t{};
   t.bGate = static_cast<const bf16 *>(a.b_gate);
@@ -274,7 +284,7 @@ void launchSums(const duck_gated &a, const GatedPlan &plan, const float *parts, 
   SumArgs<T> s{parts, biasParts, static_cast<T *>(a.dw_gate), static_cast<T *>(a.dw_up), static_cast<T *>(a.db_gate),
                static_cast<T *>(a.db_up), int64_t(a.F) * a.D, a.F, plan.splits, int(plan.biasCount), 0};
   if (parts) s.weightBlocks = int(ceilDiv(2 * s.weights, kSumThreads * 4));
-  const int64_t blocks = s.weightBlocks + (biasParts ? ceilDiv(2 * int64_t(a.F), 32) : 0);
+  const int64_t blocks = s.weightBlocks + (biasParts ? ceilDiv(2 * int64_t(a.F), kSumColumns) : 0);
   if (blocks == 0) return;
   sumParts<T><<<unsigned(blocks), kSumThreads, 0, stream>>>(s);
   check(cudaGetLastError(), "gated linear sums launch");
@@ -296,9 +306,7 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
   if (a.dx) {
     t.dx = static_cast<bf16 *>(a.dx);
     t.steps = int(ceilDiv(a.F, kTileSteps));
-    int columns = tileColumns(a.D);
-    while (columns > 64 && rowTiles * ceilDiv(a.D, columns) < 148) columns /= 2;
-    withColumns(columns, [&](auto n) {
+    withColumns(tileColumns(rowTiles, a.D), [&](auto n) {
       TileMaps maps;
       maps.a0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
       maps.a1 = mapOf(t.both + plan.stride, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
