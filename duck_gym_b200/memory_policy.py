@@ -12,11 +12,15 @@ actor and critic each are
 
 with layer norms, linear attention with one decay per head (memories of 4 to 256
 steps; its state is the memory of an environment) and an ELU layer whose output is
-kept in 8 bits for the backward pass.  A rollout advances the states by single
+kept in 8 bits for the backward pass.  ``memory="recurrence"`` has a gated linear
+recurrence in the attention's place, of as many channels, whose state is a number for
+each of them and whose gates decide how long to remember; ``mlp="gated"`` a gated
+linear layer in that of the ELU.  A rollout advances the states by single
 steps; the update runs whole rollouts, from the states that they began with, with
 episode ends inside them (gradients stay within a rollout, as rsl-rl's do).
 
     python -m duck_gym_b200.memory_policy [--envs N] [--iterations N]
+        [--memory attention|recurrence] [--mlp elu|gated] [--optimizer adam|adamw|adamw8]
 
 trains one on the synthetic biped's velocity task.
 """
@@ -43,7 +47,18 @@ class MemoryPPOConfig(PPOConfig):
     hidden: int = 512        # of a block's MLP
     shortest: float = 4.0    # steps that the fastest and the slowest head remember
     longest: float = 256.0
+    memory: str = "attention"    # or "recurrence"
+    mlp: str = "elu"             # or "gated"
     graph_update: bool = False   # minibatches run eagerly, whatever is set here
+
+    def __post_init__(self):
+        if self.memory not in ("attention", "recurrence") or self.mlp not in ("elu", "gated"):
+            raise ValueError("memory is attention or recurrence, mlp is elu or gated")
+
+    @property
+    def state_shape(self):
+        """Of one environment's state in one block."""
+        return (self.heads, self.head_size, self.head_size) if self.memory == "attention" else (self.heads * self.head_size,)
 
 
 class LayerNorm(nn.Module):
@@ -59,30 +74,59 @@ class MemoryBlock(nn.Module):
     def __init__(self, cfg: MemoryPPOConfig):
         super().__init__()
         inner = cfg.heads * cfg.head_size
-        self.shape = (3, cfg.heads, cfg.head_size)
-        self.norm, self.qkv, self.out = LayerNorm(cfg.width), nn.Linear(cfg.width, 3 * inner), nn.Linear(inner, cfg.width)
+        self.attention, self.gated = cfg.memory == "attention", cfg.mlp == "gated"
+        self.norm = LayerNorm(cfg.width)
+        if self.attention:
+            self.shape = (3, cfg.heads, cfg.head_size)
+            self.qkv = nn.Linear(cfg.width, 3 * inner)
+            # An evenly spaced ladder of memories, in their logarithm: decay = 1 - 1 / steps.
+            steps = torch.logspace(0, 1, cfg.heads, base=cfg.longest / cfg.shortest) * cfg.shortest
+            self.register_buffer("decay", 1.0 - 1.0 / steps)
+        else:
+            # The same ladder where the gates begin: sigmoid(log(steps - 1)) = 1 - 1 / steps.
+            self.gate_value = nn.Linear(cfg.width, 2 * inner)
+            steps = torch.logspace(0, 1, inner, base=cfg.longest / cfg.shortest) * cfg.shortest
+            with torch.no_grad():
+                self.gate_value.bias[:inner] = torch.log(steps - 1.0)
+        self.out = nn.Linear(inner, cfg.width)
         self.mlp_norm = LayerNorm(cfg.width)
+        if self.gated:
+            self.gate = nn.Linear(cfg.width, cfg.hidden)
         self.up, self.down = nn.Linear(cfg.width, cfg.hidden), nn.Linear(cfg.hidden, cfg.width)
-        # An evenly spaced ladder of memories, in their logarithm: decay = 1 - 1 / steps.
-        steps = torch.logspace(0, 1, cfg.heads, base=cfg.longest / cfg.shortest) * cfg.shortest
-        self.register_buffer("decay", 1.0 - 1.0 / steps)
 
     def forward(self, x, state, resets):
         """x [T, E, width] or, for one step without gradients, [E, width] with
         the state advanced in place."""
-        qkv = self.qkv(self.norm(x)).unflatten(-1, self.shape)
-        q, k, v = qkv.unbind(-3)
-        if x.dim() == 2:
-            o = memory.linear_attention_step(q, k, v, self.decay, state, resets)
+        x = x + self.out(self._remember(self.norm(x), state, resets))
+        return x + self._mlp(self.mlp_norm(x))
+
+    def _remember(self, x, state, resets):
+        step = x.dim() == 2
+        if self.attention:
+            q, k, v = self.qkv(x).unflatten(-1, self.shape).unbind(-3)
+            if step:
+                o = memory.linear_attention_step(q, k, v, self.decay, state, resets)
+            else:
+                o, _ = memory.linear_attention(q, k, v, self.decay, state, resets, final_state=False)
+            # The size of a sum over steps says little: each head's output is normed by itself.
+            return memory.layer_norm(o).flatten(-2)
+        gates, values = self.gate_value(x).chunk(2, -1)
+        if step:
+            return memory.gated_recurrence_step(gates, values, state, resets)
+        return memory.gated_recurrence(gates, values, state, resets, final_state=False)[0]
+
+    def _mlp(self, h):
+        # The type that a linear layer computes in: the autocast region's, or the parameters'.
+        kind = h.device.type
+        dtype = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else self.up.weight.dtype
+        rows, cast = h.reshape(-1, h.shape[-1]).to(dtype), lambda layer: (layer.weight.to(dtype), layer.bias.to(dtype))
+        (up, up_bias), (down, down_bias) = cast(self.up), cast(self.down)
+        if self.gated:
+            gate, gate_bias = cast(self.gate)
+            y = torch.addmm(down_bias, memory.gated_linear(rows, gate, up, gate_bias, up_bias), down.t())
         else:
-            o, _ = memory.linear_attention(q, k, v, self.decay, state, resets, final_state=False)
-        # The size of a sum over steps says little: each head's output is normed by itself.
-        x = x + self.out(memory.layer_norm(o).flatten(-2))
-        h = self.mlp_norm(x)
-        rows = h.reshape(-1, h.shape[-1])
-        y = memory.checkpointed_mlp(rows.to(qkv.dtype), *zip(*[(w.to(qkv.dtype), b.to(qkv.dtype)) for w, b in (
-            (self.up.weight, self.up.bias), (self.down.weight, self.down.bias))]))
-        return x + y.view(x.shape)
+            y = memory.checkpointed_mlp(rows, (up, down), (up_bias, down_bias))
+        return y.view(h.shape)
 
 
 class MemoryTrunk(nn.Module):
@@ -102,8 +146,8 @@ class MemoryTrunk(nn.Module):
 
 
 class MemoryActorCritic(nn.Module):
-    """States are [2, blocks, E, heads, size, size] float32: the actor's and the
-    critic's."""
+    """States are [2, blocks, E, heads, size, size] float32 (a recurrence's: [2,
+    blocks, E, heads * size]): the actor's and the critic's."""
 
     def __init__(self, actor_obs, critic_obs, actions, cfg: MemoryPPOConfig):
         super().__init__()
@@ -113,7 +157,7 @@ class MemoryActorCritic(nn.Module):
 
     def initial_state(self, envs, device=None):
         c = self.cfg
-        return torch.zeros(2, c.blocks, envs, c.heads, c.head_size, c.head_size, device=device)
+        return torch.zeros(2, c.blocks, envs, *c.state_shape, device=device)
 
     def outputs(self, obs, critic_obs, states, resets):
         """Means and values of one step ([E, ...], states advanced in place) or
@@ -203,7 +247,7 @@ class MemoryPPO(PPO):
                 self.optimizer.zero_grad(set_to_none=False)
                 loss.backward()
                 self.reducer.finish()
-                nn.utils.clip_grad_norm_(self.policy.parameters(), cfg.max_grad_norm)
+                self._clip()
                 self._optimizer_step()
                 stats.append(info)
         return {k: torch.stack([x[k] for x in stats]).mean().item() for k in stats[0]}
@@ -219,12 +263,15 @@ def main():
     parser = argparse.ArgumentParser(description="PPO with a memory policy on the synthetic biped's velocity task.")
     parser.add_argument("--envs", type=int, default=4096)
     parser.add_argument("--iterations", type=int, default=5)
+    parser.add_argument("--memory", choices=("attention", "recurrence"), default="attention")
+    parser.add_argument("--mlp", choices=("elu", "gated"), default="elu")
+    parser.add_argument("--optimizer", choices=("adam", "adamw", "adamw8"), default="adam")
     args = parser.parse_args()
     with tempfile.TemporaryDirectory() as model:
         biped.write_bam(model, seed=0)
         training = dict(command_ranges=[[-0.3, 0.3], [-0.3, 0.3], [-1.0, 1.0]], command_resample_seconds=1.0)
         env = BamEnv(model, num_envs=args.envs, iterations=10, auto_reset=True, reward_enabled=True, training=training)
-        agent = MemoryPPO(env)
+        agent = MemoryPPO(env, MemoryPPOConfig(memory=args.memory, mlp=args.mlp, optimizer=args.optimizer))
         for i in range(args.iterations):
             agent.rollout()
             stats = agent.update()

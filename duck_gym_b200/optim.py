@@ -21,7 +21,9 @@ from __future__ import annotations
 
 import bisect
 import ctypes
+import itertools
 import math
+import operator
 import struct
 from typing import NamedTuple
 
@@ -62,12 +64,43 @@ def state8_zeros(like, signed):
                   torch.zeros(_groups(like), dtype=torch.uint8, device=like.device))
 
 
-def _check_state8(state, like, dtypes, what):
-    codes, exponents = state
-    _require(codes.dtype in dtypes and exponents.dtype is torch.uint8 and codes.is_same_size(like) and exponents.dim() == 1
-             and exponents.numel() == (codes.numel() + GROUP - 1) // GROUP and codes.is_contiguous()
-             and exponents.is_contiguous() and codes.get_device() == exponents.get_device() == like.get_device(),
+# The checks run before every step: maps over methods cost a third of loops.
+def _pointers(ts):
+    return list(map(torch.Tensor.data_ptr, ts))
+
+
+def _numbers(ts):
+    return list(map(torch.Tensor.numel, ts))
+
+
+def _devices(ts):
+    return set(map(torch.Tensor.get_device, ts))
+
+
+def _dtypes(ts, get=operator.attrgetter("dtype")):
+    return set(map(get, ts))
+
+
+def _dense(ts):
+    return all(map(torch.Tensor.is_contiguous, ts))
+
+
+def _alike(ts, others):
+    return all(map(torch.Tensor.is_same_size, ts, others))
+
+
+def _group_counts(numbers):
+    return [(n + GROUP - 1) // GROUP for n in numbers]
+
+
+def _check_states8(states, dtypes, what):
+    """Codes and exponents of moments in 8 bits, and how many values they have."""
+    codes, exponents = [s[0] for s in states], [s[1] for s in states]
+    numbers = _numbers(codes)
+    _require(_dtypes(codes) <= dtypes and _dtypes(exponents) == {torch.uint8} and _numbers(exponents) == _group_counts(numbers)
+             and _dense(codes) and _dense(exponents),
              f"{what}: a moment in 8 bits is dense codes of its tensor's shape and one exponent for 128 of them")
+    return codes, exponents, numbers
 
 
 # ------------------------------------------------------------ plain restatement
@@ -146,63 +179,57 @@ def _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm, 
 
 # ----------------------------------------------------------------- entry points
 def _check_apart(written, read, what):
-    """Spans (first byte, end) of arrays: none that is written overlaps another one."""
-    written.sort()
-    starts = [a for a, _ in written]
-    for (_, end), b in zip(written, starts[1:]):
-        _require(end <= b, f"{what}: a tensor is there twice, or two of them overlap")
-    for a, end in read:
-        i = bisect.bisect_left(starts, end)   # the spans that begin before its end
-        _require(i == 0 or written[i - 1][1] <= a, f"{what}: a gradient overlaps what is written")
+    """Arrays, as (first bytes, bytes): none that is written overlaps another one."""
+    starts, ends = [], []
+    for first, size in written:
+        starts += first
+        ends += map(operator.add, first, size)
+    starts.sort()
+    ends.sort()   # disjoint spans end in the order that they begin in
+    _require(all(map(operator.le, ends, starts[1:])), f"{what}: a tensor is there twice, or two of them overlap")
+    first, size = read
+    before = map(bisect.bisect_left, itertools.repeat(starts), map(operator.add, first, size))   # spans that begin before its end
+    _require(all(not k or ends[k - 1] <= a for k, a in zip(before, first)), f"{what}: a gradient overlaps what is written")
 
 
 def _checked(params, grads, exp_avgs, exp_avg_sqs):
-    """Whether the moments have 8 bits, the tensors' device, and their rows of a
-    table, with dense gradients in the places of others (they are returned too, so
-    that they live until the launch)."""
+    """Whether the moments have 8 bits, the tensors' device, their table, and dense
+    gradients (which have to live until the launch)."""
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     _require(len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) > 0,
              "adamw_step: one gradient and two moments for each of one or more parameters")
-    # This runs before every step: what says the same of a tensor in fewer calls is taken.
-    index = params[0].get_device()
     eight = not torch.is_tensor(exp_avgs[0])
-    dense, rows, written, read = [], [], [], []
-    for place, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
-        dtype = p.dtype
-        kind = _TYPES.get(dtype)
-        _require(kind is not None and p.get_device() == index and p.is_contiguous(),
-                 "adamw_step: parameters are dense float32 or bfloat16 tensors of one device")
-        _require(g.dtype is dtype and g.is_same_size(p) and g.get_device() == index and g.layout is torch.strided,
-                 "adamw_step: a gradient has its parameter's shape, type and device")
-        _require(torch.is_tensor(m) != eight and torch.is_tensor(v) != eight,
-                 "adamw_step: all moments have 32 bits, or all have 8")
-        if not g.is_contiguous():
-            g = g.contiguous()
-        n = p.numel()
-        size = n << (2 - kind)
-        at, gat = p.data_ptr(), g.data_ptr()
-        if eight:
-            _check_state8(m, p, (torch.int8,), "adamw_step")
-            _check_state8(v, p, (torch.uint8,), "adamw_step")
-            mat, vat, meat, veat = m[0].data_ptr(), v[0].data_ptr(), m[1].data_ptr(), v[1].data_ptr()
-            groups = (n + GROUP - 1) // GROUP
-            spans = ((at, at + size), (mat, mat + n), (vat, vat + n), (meat, meat + groups), (veat, veat + groups))
-        else:
-            _require(m.dtype is torch.float32 and v.dtype is torch.float32 and m.is_same_size(p) and v.is_same_size(p)
-                     and m.get_device() == index and v.get_device() == index and m.is_contiguous() and v.is_contiguous(),
-                     "adamw_step: moments are dense float32 tensors of their parameters' shapes")
-            mat, vat, meat, veat = m.data_ptr(), v.data_ptr(), 0, 0
-            spans = ((at, at + size), (mat, mat + 4 * n), (vat, vat + 4 * n))
-        if n:
-            written += spans
-            read.append((gat, gat + size))
-        dense.append(g)
-        rows.append((at, gat, mat, vat, meat, veat, n, kind, place))
-    _check_apart(written, read, "adamw_step")
-    return eight, params[0].device, rows, dense
-
-
-def _table(rows):
-    return b"".join(_TENSOR.pack(*row) for row in rows)
+    _require(all(torch.is_tensor(t) != eight for t in exp_avgs) and all(torch.is_tensor(t) != eight for t in exp_avg_sqs),
+             "adamw_step: all moments have 32 bits, or all have 8")
+    kinds = [_TYPES.get(p.dtype) for p in params]
+    _require(None not in kinds and _dense(params), "adamw_step: parameters are dense float32 or bfloat16 tensors of one device")
+    _require(_alike(grads, params) and [g.dtype for g in grads] == [p.dtype for p in params]
+             and all(g.layout is torch.strided for g in grads), "adamw_step: a gradient has its parameter's shape, type and device")
+    if not _dense(grads):
+        grads = [g.contiguous() for g in grads]
+    numbers = _numbers(params)
+    if eight:
+        (ms, me, _), (vs, ve, _) = (_check_states8(exp_avgs, {torch.int8}, "adamw_step"),
+                                    _check_states8(exp_avg_sqs, {torch.uint8}, "adamw_step"))
+        _require(_alike(ms, params) and _alike(vs, params), "adamw_step: a moment has its parameter's shape")
+        arrays = [*params, *grads, *ms, *vs, *me, *ve]
+        me, ve, size = _pointers(me), _pointers(ve), numbers
+    else:
+        ms, vs, me, ve = exp_avgs, exp_avg_sqs, (0,) * len(params), (0,) * len(params)
+        _require(_dtypes(ms) == _dtypes(vs) == {torch.float32} and _alike(ms, params) and _alike(vs, params) and _dense(ms)
+                 and _dense(vs), "adamw_step: moments are dense float32 tensors of their parameters' shapes")
+        arrays = [*params, *grads, *ms, *vs]
+        size = [4 * n for n in numbers]
+    _require(len(_devices(arrays)) == 1, "adamw_step: one device for parameters, gradients and moments")
+    at, gat, mat, vat = _pointers(params), _pointers(grads), _pointers(ms), _pointers(vs)
+    bytes_ = [n << (2 - kind) for n, kind in zip(numbers, kinds)]
+    written = [(at, bytes_), (mat, size), (vat, size)]
+    if eight:
+        groups = _group_counts(numbers)
+        written += [(me, groups), (ve, groups)]
+    _check_apart(written, (gat, bytes_), "adamw_step")
+    table = b"".join(map(_TENSOR.pack, at, gat, mat, vat, me, ve, numbers, kinds, itertools.count()))
+    return eight, params[0].device, table, grads
 
 
 class _Norm:
@@ -213,34 +240,34 @@ class _Norm:
         self.sums = (torch.empty(SUMS, dtype=torch.float64, device=device) if device.type == "cuda"
                      else torch.zeros((), dtype=torch.float64))
 
-    def add(self, rows, grads):
+    def add(self, table, grads):
         if self.sums.dim() == 0:
             for g in grads:
                 self.sums += g.double().square().sum()
             return
         count = ctypes.c_int()
-        _launch(library().duck_gradient_squares, self.sums.device, _table(rows), len(rows), self.count,
-                self.sums.data_ptr(), ctypes.byref(count))
+        _launch(library().duck_gradient_squares, self.sums.device, table, len(grads), self.count, self.sums.data_ptr(),
+                ctypes.byref(count))
         self.count = count.value
         if self.count == 0:   # only empty gradients: a norm of zero
             self.sums[:1].zero_()
             self.count = 1
 
 
-def _step(params, grads, ms, vs, eight, device, rows, step, lr, betas, eps, weight_decay, max_norm, norm):
+def _step(params, grads, ms, vs, eight, device, table, step, lr, betas, eps, weight_decay, max_norm, norm):
     if device.type != "cuda":
-        return _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm,
-                      None if norm is None else norm.sums)
+        with torch.no_grad():
+            return _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm,
+                          None if norm is None else norm.sums)
     on_device = torch.is_tensor(lr) and lr.is_cuda
     if on_device and lr.dtype != torch.float32:
         lr = lr.float()
     options = _OPTIONS.pack(step.data_ptr(), lr.data_ptr() if on_device else 0, norm.sums.data_ptr() if norm else 0,
                             0.0 if on_device else float(lr), *betas, eps, weight_decay, 0.0 if norm is None else max_norm,
                             norm.count if norm else 0, 8 if eight else 32)
-    _launch(library().duck_adamw_step, device, _table(rows), len(rows), options)
+    _launch(library().duck_adamw_step, device, table, len(grads), options)
     written = [*params, step]
-    for m, v in zip(ms, vs):
-        written += [*m, *v] if eight else [m, v]
+    written += itertools.chain(*ms, *vs) if eight else (*ms, *vs)
     torch.autograd.graph.increment_version(written)   # autograd does not see a kernel's writes
 
 
@@ -256,7 +283,6 @@ def _check_options(step, lr, betas, eps, weight_decay, max_norm, device):
     _require(max_norm is None or max_norm >= 0.0, "adamw_step: a norm of 0 or more")
 
 
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
                max_norm=None):
     """One AdamW step over lists of tensors, in place:
@@ -273,39 +299,36 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999
     bfloat16 parameters and codes are rounded up or down at random, by a hash of t, the
     tensor's place in the list and the value's place in the tensor: what a step adds is
     mostly less than half a place of theirs, and would be lost."""
-    eight, device, rows, grads = _checked(params, grads, exp_avgs, exp_avg_sqs)
+    eight, device, table, grads = _checked(params, grads, exp_avgs, exp_avg_sqs)
     _check_options(step, lr, betas, eps, weight_decay, max_norm, device)
     norm = None
     if max_norm is not None:
         norm = _Norm(device)
-        norm.add(rows, grads)
-    _step(params, grads, exp_avgs, exp_avg_sqs, eight, device, rows, step, lr, betas, eps, weight_decay, max_norm, norm)
+        norm.add(table, grads)
+    _step(params, grads, exp_avgs, exp_avg_sqs, eight, device, table, step, lr, betas, eps, weight_decay, max_norm, norm)
 
 
-@torch.no_grad()
 def state8_values(states):
     """The float32 tensors that moments in 8 bits stand for (on the GPU, parts of one
     buffer)."""
     states = list(states)
     if not states:
         return []
-    for s in states:
-        _check_state8(s, s[0], (torch.int8, torch.uint8), "state8_values")
-        _require(s[0].get_device() == states[0][0].get_device(), "state8_values: states of one device")
-    device = states[0][0].device
+    codes, exponents, numbers = _check_states8(states, {torch.int8, torch.uint8}, "state8_values")
+    _require(len(_devices([*codes, *exponents])) == 1, "state8_values: states of one device")
+    device = codes[0].device
     if device.type != "cuda":
         return [_decode(*s) for s in states]
     # One allocation, each tensor on a 16-byte boundary.
-    sizes = [(codes.numel(), -codes.numel() % 4) for codes, _ in states]
-    flat = torch.empty(sum(map(sum, sizes)), dtype=torch.float32, device=device).split([n for pair in sizes for n in pair])[::2]
-    values = [v if s[0].dim() == 1 else v.view(s[0].shape) for v, s in zip(flat, states)]
-    rows = []
-    for value, (codes, exponents) in zip(flat, states):
-        signed = codes.dtype is torch.int8
-        m, me, v, ve = (codes.data_ptr(), exponents.data_ptr(), 0, 0) if signed else (0, 0, codes.data_ptr(), exponents.data_ptr())
-        rows.append((value.data_ptr(), 0, m, v, me, ve, codes.numel(), 0, 0))
-    _launch(library().duck_moment_values, device, _table(rows), len(rows))
-    return values
+    sizes = [part for n in numbers for part in (n, -n % 4)]
+    values = torch.empty(sum(sizes), dtype=torch.float32, device=device).split(sizes)[::2]
+    signed = [c.dtype is torch.int8 for c in codes]
+    at, es = _pointers(codes), _pointers(exponents)
+    either = lambda ps, which: [p if s == which else 0 for p, s in zip(ps, signed)]
+    table = b"".join(map(_TENSOR.pack, _pointers(values), itertools.repeat(0), either(at, True), either(at, False),
+                         either(es, True), either(es, False), numbers, itertools.repeat(0), itertools.repeat(0)))
+    _launch(library().duck_moment_values, device, table, len(codes))
+    return [v if c.dim() == 1 else v.view(c.shape) for v, c in zip(values, codes)]
 
 
 class AdamW(torch.optim.Optimizer):
@@ -355,17 +378,17 @@ class AdamW(torch.optim.Optimizer):
                 group["step"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
             moments = [self._moments(p, group["bits"]) for p in params]
             ms, vs = [m for m, _ in moments], [v for _, v in moments]
-            eight, device, rows, grads = _checked(params, [p.grad for p in params], ms, vs)
+            eight, device, table, grads = _checked(params, [p.grad for p in params], ms, vs)
             _check_options(group["step"], group["lr"], group["betas"], group["eps"], group["weight_decay"],
                            self.max_grad_norm, device)
             if self.max_grad_norm is not None:
                 _require(not norms or device in norms, "AdamW: one device where gradients are clipped")
                 norms.setdefault(device, None)
                 norms[device] = norms[device] or _Norm(device)
-                norms[device].add(rows, grads)
-            work.append((params, grads, ms, vs, eight, device, rows, group))
-        for params, grads, ms, vs, eight, device, rows, group in work:
-            _step(params, grads, ms, vs, eight, device, rows, group["step"], group["lr"], group["betas"], group["eps"],
+                norms[device].add(table, grads)
+            work.append((params, grads, ms, vs, eight, device, table, group))
+        for params, grads, ms, vs, eight, device, table, group in work:
+            _step(params, grads, ms, vs, eight, device, table, group["step"], group["lr"], group["betas"], group["eps"],
                   group["weight_decay"], self.max_grad_norm, norms.get(device))
         return loss
 

@@ -46,6 +46,8 @@ class PPOConfig:
     learning_rate: float = 3e-4
     desired_kl: float = 0.01
     max_grad_norm: float = 1.0
+    optimizer: str = "adam"      # torch's; "adamw" and "adamw8": optim.AdamW, moments in 32 or 8 bits, clipping in the step
+    weight_decay: float = 0.0    # of the latter two
     initial_std: float = 0.15
     actor_hidden: tuple = (512, 256, 128)
     critic_hidden: tuple = (512, 256, 128)
@@ -288,15 +290,32 @@ class PPO:
         if self.device.type == "cuda":
             self._lr64 = torch.tensor(self.cfg.learning_rate, dtype=torch.float64, device=self.device)
             self._lr = self._lr64.float()
-            self.optimizer = torch.optim.Adam(self.policy.parameters(), lr=self._lr, fused=True, capturable=True)
         else:
             self._lr64 = self._lr = None
-            self.optimizer = torch.optim.Adam(self.policy.parameters(), lr=self.cfg.learning_rate)
             self._host_lr = self.cfg.learning_rate
+        self.optimizer = self._make_optimizer()
         self._graph = None
         self._updates, self._ugraphs, self._flat_grad = 0, None, None
         self.storage = Storage(self.cfg.steps_per_env, env.num_envs, self.obs.shape[1], self.critic_obs.shape[1],
                                env.num_actions, self.device)
+
+    def _make_optimizer(self):
+        cfg, params = self.cfg, self.policy.parameters()
+        if cfg.optimizer == "adam":
+            if self._lr is None:
+                return torch.optim.Adam(params, lr=cfg.learning_rate)
+            return torch.optim.Adam(params, lr=self._lr, fused=True, capturable=True)
+        if cfg.optimizer not in ("adamw", "adamw8"):
+            raise ValueError(f"optimizer: adam, adamw or adamw8, not {cfg.optimizer}")
+        from .optim import AdamW
+
+        return AdamW(params, lr=cfg.learning_rate if self._lr is None else self._lr, weight_decay=cfg.weight_decay,
+                     bits=8 if cfg.optimizer == "adamw8" else 32, max_grad_norm=cfg.max_grad_norm)
+
+    def _clip(self):
+        """Clips the gradients, unless the optimizer does so in its step."""
+        if self.cfg.optimizer == "adam":
+            nn.utils.clip_grad_norm_(self.policy.parameters(), self.cfg.max_grad_norm)
 
     # What a policy with memory does differently (memory_policy.MemoryPPO).
     def _make_policy(self, env):
@@ -404,7 +423,7 @@ class PPO:
                 self.optimizer.zero_grad(set_to_none=False)
                 loss.backward()
                 self.reducer.finish()
-                nn.utils.clip_grad_norm_(self.policy.parameters(), cfg.max_grad_norm)
+                self._clip()
                 self._optimizer_step()
                 stats.append(info)
         return {k: torch.stack([x[k] for x in stats]).mean().item() for k in stats[0]}
@@ -433,7 +452,7 @@ class PPO:
             self._host_lr = kl_schedule_host(self._host_lr, float(self._flat_grad[-1]), self.cfg.desired_kl)
             for group in self.optimizer.param_groups:
                 group["lr"] = self._host_lr
-        nn.utils.clip_grad_norm_(self.policy.parameters(), self.cfg.max_grad_norm)
+        self._clip()
         self.optimizer.step()
 
     def _prepare_flat(self):
