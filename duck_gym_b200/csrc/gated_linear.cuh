@@ -434,8 +434,9 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
 
 // -------------------------------------------------------------------- float32
 // Tiles of 128 rows and 128 columns, 16 steps at a time, 8 by 8 values a thread as
-// pairs; the operands of the next steps are on their way in registers.  The forward
-// pass's columns are 64 of Wg and the same 64 of Wu: a thread has both of a value.
+// pairs; the operands of the next steps are on their way in registers.  Where that
+// leaves multiprocessors without a tile, of 64 by 64 and 4 by 4.  The forward pass's
+// columns are half of Wg's and half the same of Wu's: a thread has both of a value.
 struct ProductArgs {
   const float *x, *wGate, *wUp, *bGate, *bUp;
   float *h, *kept;             // forward: h, and a and u [2, rows, F] or null
@@ -445,7 +446,7 @@ struct ProductArgs {
   int D, F, activation, splits;
   bool wholeX, wholeD, wholeF;   // rows of x, of D and of F values are 16-byte pieces
 };
-constexpr int kProductThreads = 256, kProductTile = 128, kProductSteps = 16, kProductPitch = kProductTile + 4;
+constexpr int kProductThreads = 256, kProductSteps = 16;
 
 // The first `count` of four values.
 __device__ __forceinline__ float4 fetchFour(const float *p, int64_t count, bool whole) {
@@ -467,9 +468,10 @@ __device__ __forceinline__ void addProduct(Two &d, Two a, Two b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
 }
 
-template <Pass PASS> __global__ void __launch_bounds__(kProductThreads, 2) gatedProducts(ProductArgs p) {
+template <Pass PASS, int T> __global__ void __launch_bounds__(kProductThreads, 2) gatedProducts(ProductArgs p) {
   static_assert(PASS != Pass::gradients, "gatedGradients");
-  constexpr int T = kProductTile, K = kProductSteps, P = kProductPitch;
+  constexpr int K = kProductSteps, P = T + 4, R = T / 16, H = R / 2;   // R rows and columns a thread, H in each half of the columns
+  constexpr int kLoads = T / 64, kGroups = T / 4;                       // a thread's, and of four values side by side
   constexpr bool kAlongA = PASS != Pass::weights, kAlongB = PASS == Pass::forward;   // steps are contiguous
   __shared__ __align__(16) float as[2][K][P], bs[2][K][P];
   const int tid = threadIdx.x;
@@ -495,7 +497,7 @@ template <Pass PASS> __global__ void __launch_bounds__(kProductThreads, 2) gated
       const int64_t m = m0 + at / 4, k = (step - (up ? halfSteps : 0)) * K + at % 4 * 4;
       return fetchFour(p.both + (up ? plane : 0) + m * p.F + k, m < p.rows ? p.F - k : 0, p.wholeF);
     } else {
-      const int64_t k = step * K + at / 32, m = m0 + at % 32 * 4;
+      const int64_t k = step * K + at / kGroups, m = m0 + at % kGroups * 4;
       return fetchFour(p.both + (half ? plane : 0) + k * p.F + m, k < p.rows ? p.F - m : 0, p.wholeF);
     }
   };
@@ -507,10 +509,10 @@ template <Pass PASS> __global__ void __launch_bounds__(kProductThreads, 2) gated
       return fetchFour((row < T / 2 ? p.wGate : p.wUp) + int64_t(f) * p.D + k, f < p.F ? p.D - k : 0, p.wholeD);
     } else if constexpr (PASS == Pass::input) {
       const bool up = step >= halfSteps;
-      const int64_t k = (step - (up ? halfSteps : 0)) * K + at / 32, n = n0 + at % 32 * 4;
+      const int64_t k = (step - (up ? halfSteps : 0)) * K + at / kGroups, n = n0 + at % kGroups * 4;
       return fetchFour((up ? p.wUp : p.wGate) + k * p.D + n, k < p.F ? p.D - n : 0, p.wholeD);
     } else {
-      const int64_t k = step * K + at / 32, n = n0 + at % 32 * 4;
+      const int64_t k = step * K + at / kGroups, n = n0 + at % kGroups * 4;
       return fetchFour(p.x + k * p.xStride + n, k < p.rows ? p.D - n : 0, p.wholeX);
     }
   };
@@ -520,66 +522,71 @@ template <Pass PASS> __global__ void __launch_bounds__(kProductThreads, 2) gated
       const int row = at / 4, k = at % 4 * 4;
       tile[k][row] = v.x, tile[k + 1][row] = v.y, tile[k + 2][row] = v.z, tile[k + 3][row] = v.w;
     } else {
-      *reinterpret_cast<float4 *>(&tile[at / 32][at % 32 * 4]) = v;
+      *reinterpret_cast<float4 *>(&tile[at / kGroups][at % kGroups * 4]) = v;
     }
   };
 
   const int ty = tid / 16, tx = tid % 16;
-  Two sum[8][4];
+  Two sum[R][H];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[i][j] = 0;
-  float4 a[2], b[2];
+    for (int j = 0; j < H; ++j) sum[i][j] = 0;
+  float4 a[kLoads], b[kLoads];
   if (first < last) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) put(as[0], kAlongA, i, fetchA(first, i)), put(bs[0], kAlongB, i, fetchB(first, i));
+    for (int i = 0; i < kLoads; ++i) put(as[0], kAlongA, i, fetchA(first, i)), put(bs[0], kAlongB, i, fetchB(first, i));
   }
   __syncthreads();
   for (int64_t step = first; step < last; ++step) {
     const int now = int(step - first) & 1;
     if (step + 1 < last) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) a[i] = fetchA(step + 1, i), b[i] = fetchB(step + 1, i);
+      for (int i = 0; i < kLoads; ++i) a[i] = fetchA(step + 1, i), b[i] = fetchB(step + 1, i);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float4 a0 = *reinterpret_cast<const float4 *>(&as[now][k][ty * 4]);
-      const float4 a1 = *reinterpret_cast<const float4 *>(&as[now][k][64 + ty * 4]);
-      const ulonglong2 b0 = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][tx * 4]);
-      const ulonglong2 b1 = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][64 + tx * 4]);
-      const float rows[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+      float rows[R];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < R; i += 4)
+        *reinterpret_cast<float4 *>(rows + i) = *reinterpret_cast<const float4 *>(&as[now][k][i * 16 + ty * 4]);
+      Two columns[H];
+      if constexpr (H == 4) {
+        *reinterpret_cast<ulonglong2 *>(columns) = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][tx * 4]);
+        *reinterpret_cast<ulonglong2 *>(columns + 2) = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][T / 2 + tx * 4]);
+      } else {
+        columns[0] = *reinterpret_cast<const Two *>(&bs[now][k][tx * 2]);
+        columns[1] = *reinterpret_cast<const Two *>(&bs[now][k][T / 2 + tx * 2]);
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
         const Two r = twoOf(rows[i], rows[i]);
-        addProduct(sum[i][0], r, b0.x);
-        addProduct(sum[i][1], r, b0.y);
-        addProduct(sum[i][2], r, b1.x);
-        addProduct(sum[i][3], r, b1.y);
+#pragma unroll
+        for (int j = 0; j < H; ++j) addProduct(sum[i][j], r, columns[j]);
       }
     }
     if (step + 1 < last) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) put(as[now ^ 1], kAlongA, i, a[i]), put(bs[now ^ 1], kAlongB, i, b[i]);
+      for (int i = 0; i < kLoads; ++i) put(as[now ^ 1], kAlongA, i, a[i]), put(bs[now ^ 1], kAlongB, i, b[i]);
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int64_t m = m0 + (i / 4) * 64 + ty * 4 + i % 4;
     if (m >= (PASS == Pass::weights ? int64_t(p.F) : p.rows)) continue;
-    float v[8];
+    float v[R];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < H; ++j) {
       const float2 two = partsOf(sum[i][j]);
       v[2 * j] = two.x, v[2 * j + 1] = two.y;
     }
     if constexpr (PASS == Pass::forward) {
-      const int f = n0 + tx * 4;
+      const int f = n0 + tx * H;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < H; ++j) {
         if (f + j >= p.F) break;
-        float gate = v[j], up = v[4 + j];
+        float gate = v[j], up = v[H + j];
         if (p.bGate) gate += p.bGate[f + j], up += p.bUp[f + j];
         const int64_t at = m * p.F + f + j;
         if (p.kept) p.kept[at] = gate, p.kept[plane + at] = up;
@@ -588,8 +595,8 @@ template <Pass PASS> __global__ void __launch_bounds__(kProductThreads, 2) gated
     } else {
       float *to = PASS == Pass::input ? p.dx + m * p.D : p.parts + ((int64_t(blockIdx.z) * 2 + half) * p.F + m) * p.D;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int n = n0 + (j / 4) * 64 + tx * 4 + j % 4;
+      for (int j = 0; j < R; ++j) {
+        const int n = n0 + (j / H) * (T / 2) + tx * H + j % H;
         if (n < p.D) to[n] = v[j];
       }
     }
