@@ -82,18 +82,23 @@ struct TileArgs {
   int64_t rows, dhStride;
   int D, F, stride, activation;
   int tiles, columnTiles, rowTiles, splits, steps;   // steps of 64 of a tile's product
-  bool wholeH, wholeDh;      // rows of 16-byte pieces
+  bool wholeH, wholeDh, wholeBias;   // rows of 16-byte pieces: h and dh move by the TMA
 };
 struct TileMaps {
-  CUtensorMap a0, a1, b0, b1;
+  CUtensorMap a0, a1, b0, b1;   // operands
+  CUtensorMap dh, out0, out1;   // gradients: dh, da and du; forward: out0 is h
 };
 
 constexpr int kTileWarps = 16, kTileThreads = 128 + 32 * kTileWarps, kTileRows = 128, kTileSteps = 64, kTileChunk = 16;
-template <int BN> struct TileShared {
-  static constexpr int stages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+template <Pass PASS, int BN> struct TileShared {
+  static constexpr bool dual = PASS == Pass::forward || PASS == Pass::gradients;
+  static constexpr int columns = dual ? BN / 2 : BN;                                      // of the output that a tile has
+  static constexpr int part = columns / 4 < kTileChunk ? kTileChunk : columns / 4;        // and that a warp has
+  static constexpr int stages = PASS == Pass::gradients ? (BN == 256 ? 3 : BN == 128 ? 5 : 6) : (BN == 256 ? 4 : BN == 128 ? 6 : 8);
   static constexpr int a = kTileRows * kTileSteps * 2, b = BN * kTileSteps * 2;
-  static constexpr int staging = 32 * 32, bias = 2 * kTileChunk * 4;   // of a warp
-  static constexpr int bytes = 1024 + stages * (a + b) + kTileWarps * (staging + bias) + 256;
+  static constexpr int staging = dual ? 32 * part * 2 : 32 * 32;                          // of a warp: its rows, or 32 bytes of them
+  static constexpr int incoming = PASS == Pass::gradients ? staging : 0;                  // its rows of dh
+  static constexpr int bytes = 1024 + stages * (a + b) + kTileWarps * (staging + incoming) + 512;
 };
 
 // A warp's 32 rows of 32 bytes: two pieces of 16 bytes, so placed that neither rows
@@ -160,18 +165,18 @@ __device__ __forceinline__ uint4 fourOf(const float *x) {
 
 template <Pass PASS, int BN> __global__ void __launch_bounds__(kTileThreads, 1)
 gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
-  using S = TileShared<BN>;
+  using S = TileShared<PASS, BN>;
   constexpr bool kDual = PASS == Pass::forward || PASS == Pass::gradients;
   constexpr bool kAlongA = PASS != Pass::weights, kAlongB = kDual;
-  constexpr int kColumns = kDual ? BN / 2 : BN;   // of the output that a tile has
+  constexpr int kColumns = S::columns, kPart = S::part, kChunk = kTileChunk;
   extern __shared__ uint8_t raw[];
   uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *tileA = base, *tileB = base + S::stages * S::a;
   uint8_t *staging = tileB + S::stages * S::b;
-  float *biases = reinterpret_cast<float *>(staging + kTileWarps * S::staging);
-  uint64_t *full = reinterpret_cast<uint64_t *>(biases + kTileWarps * S::bias / 4);
-  uint64_t *empty = full + S::stages, *done = empty + S::stages, *taken = done + 2;
-  uint32_t *tensor = reinterpret_cast<uint32_t *>(taken + 2);
+  uint8_t *incoming = staging + kTileWarps * S::staging;
+  uint64_t *full = reinterpret_cast<uint64_t *>(incoming + kTileWarps * S::incoming);
+  uint64_t *empty = full + S::stages, *done = empty + S::stages, *taken = done + 2, *came = taken + 2;
+  uint32_t *tensor = reinterpret_cast<uint32_t *>(came + kTileWarps);
   volatile int *broken = reinterpret_cast<volatile int *>(tensor + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
@@ -179,6 +184,7 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
     *broken = 0;
     for (int i = 0; i < S::stages; ++i) barrierInit(full + i, 1), barrierInit(empty + i, 1);
     for (int i = 0; i < 2; ++i) barrierInit(done + i, 1), barrierInit(taken + i, kTileWarps);
+    for (int i = 0; i < kTileWarps; ++i) barrierInit(came + i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -296,117 +302,197 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
     }
   } else if (warp >= 4) {
     // A warp has a quarter of the tile's rows (that of tensor memory which it reaches) and of its columns.
-    constexpr int kChunk = kTileChunk, kPart = kColumns / 4 < kChunk ? kChunk : kColumns / 4;
+    constexpr int kChunks = kPart / kChunk;
     const int quarter = warp % 4, part = (warp - 4) / 4;
     uint4 *stage = reinterpret_cast<uint4 *>(staging + (warp - 4) * S::staging);
-    float *bias = biases + (warp - 4) * S::bias / 4;
-    int n = 0;
-    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++n) {
-      const Tile at = tileAt(t);
-      const int buffer = n & 1;
-      int first;
-      const int steps = stepsOf(at, first);
-      const int64_t row = at.row + quarter * 32;
-      const int64_t rowsLeft = (PASS == Pass::weights ? int64_t(p.F) : p.rows) - row;
-      const bool mine = lane < rowsLeft;
-      // What the tile needs of memory is asked for before its products are waited for.
-      constexpr int kChunks = kPart / kChunk;
-      uint4 gradients[PASS == Pass::gradients ? kChunks : 1][2];
-      float biasOf[kDual ? kChunks : 1];
-      if constexpr (kDual) {
+    // Accumulators of a tile: zero where it has no steps, NaN where a wait ran out.
+    auto take = [&](float (&x)[kChunk], uint32_t from, bool fine, bool some) {
+      if (fine && some) {
+        tensorLoad16(x, from);
+      } else {
 #pragma unroll
-        for (int k = 0; k < kChunks; ++k) {
-          const int c = part * kPart + k * kChunk, column = at.column + c, columns = c < kColumns ? min(kChunk, p.F - column) : 0;
-          if constexpr (PASS == Pass::gradients) {
-            const bf16 *from = p.dh + (row + lane) * p.dhStride + column;
-            if (p.wholeDh && columns == kChunk) {
+        for (int i = 0; i < kChunk; ++i) x[i] = fine ? 0.f : __int_as_float(0x7fffffff);
+      }
+    };
+    if constexpr (kDual) {
+      // Rows of the warp's part as pieces of 16 bytes, where the TMA's swizzle has them: neither rows of pieces nor columns
+      // of them meet in a bank.
+      constexpr int kPieces = kPart / 8;
+      auto pieceOf = [&](uint4 *base, int piece) { return base + lane * kPieces + (piece ^ (kPieces == 4 ? lane >> 1 & 3 : lane >> 2 & 1)); };
+      uint4 *gradients = reinterpret_cast<uint4 *>(incoming + (warp - 4) * S::incoming);
+      uint64_t *bar = came + (warp - 4);
+      uint32_t parity = 0;
+      bool asked = false, fine = true;
+      auto ours = [&](const Tile &at) {   // the tile has rows and columns for this warp
+        return part * kPart < kColumns && at.row + quarter * 32 < p.rows && at.column + part * kPart < p.F;
+      };
+      auto askGradients = [&](int t) {
+        if (t >= p.tiles) return;
+        const Tile at = tileAt(t);
+        if (!ours(at)) return;
+        barrierExpect(bar, S::incoming);
+        copyBox(gradients, &maps.dh, at.column + part * kPart, at.row + quarter * 32, bar);
+        asked = true;
+      };
+      if (PASS == Pass::gradients && p.wholeDh && lane == 0) askGradients(blockIdx.x);
+      int n = 0;
+      for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++n) {
+        const Tile at = tileAt(t);
+        const bool own = ours(at);
+        const int buffer = n & 1, first = at.column + part * kPart;
+        const int64_t row = at.row + quarter * 32, rowsLeft = p.rows - row;
+        const bool mine = lane < rowsLeft;
+        fine = __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken));
+        if (PASS == Pass::gradients && p.wholeDh && own) {
+          const bool here = __all_sync(0xffffffffu, barrierWait(bar, parity, broken));
+          fine = fine && here;
+          if (here) asked = false, parity ^= 1;
+        }
+        tensorFenceAfter();
+        const uint32_t tensorRow = accumulators + buffer * BN + (uint32_t(quarter * 32) << 16) + part * kPart;
+        uint4 later[kChunks][2];   // du, until da has left
+        if (own) {
+          if (lane == 0) storesRead();   // of the tile before
 #pragma unroll
-              for (int i = 0; i < 2; ++i)
-                gradients[k][i] = mine ? reinterpret_cast<const uint4 *>(from)[i] : make_uint4(0, 0, 0, 0);
+          for (int k = 0; k < kChunks; ++k) {
+            const int column = first + k * kChunk, columns = min(kChunk, p.F - column);
+            if (columns <= 0) break;
+            float a[kChunk], u[kChunk];
+            __syncwarp();   // loads from tensor memory are the whole warp's
+            take(a, tensorRow + k * kChunk, fine, p.steps > 0);
+            take(u, tensorRow + BN / 2 + k * kChunk, fine, p.steps > 0);
+            uint4 dh[2];
+            if constexpr (PASS == Pass::gradients) {
+              if (p.wholeDh) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) dh[i] = *pieceOf(gradients, 2 * k + i);
+              } else {
+                const bf16 *from = p.dh + (row + lane) * p.dhStride + column;
+                uint32_t *w = reinterpret_cast<uint32_t *>(dh);
+#pragma unroll
+                for (int i = 0; i < kChunk; i += 2) {
+                  const uint32_t low = mine && i < columns ? __bfloat16_as_ushort(from[i]) : 0u;
+                  const uint32_t high = mine && i + 1 < columns ? __bfloat16_as_ushort(from[i + 1]) : 0u;
+                  w[i / 2] = high << 16 | low;
+                }
+              }
+            }
+            uint4 bias[2][2];
+            if (p.bGate) {
+              if (p.wholeBias && columns == kChunk) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  bias[0][i] = reinterpret_cast<const uint4 *>(p.bGate + column)[i];
+                  bias[1][i] = reinterpret_cast<const uint4 *>(p.bUp + column)[i];
+                }
+              } else {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                  for (int i = 0; i < kChunk; i += 2) {
+                    const bf16 *from = (b ? p.bUp : p.bGate) + column;
+                    const uint32_t low = i < columns ? __bfloat16_as_ushort(from[i]) : 0u;
+                    const uint32_t high = i + 1 < columns ? __bfloat16_as_ushort(from[i + 1]) : 0u;
+                    reinterpret_cast<uint32_t *>(bias[b])[i / 2] = high << 16 | low;
+                  }
+              }
+            }
+            tensorLoadWait();
+            tensorLoaded(a);
+            tensorLoaded(u);
+            auto half = [](const uint4 (&v)[2], int i) {
+              const uint32_t two = reinterpret_cast<const uint32_t *>(v)[i / 2];
+              return __uint_as_float(i % 2 ? two & 0xffff0000u : two << 16);
+            };
+            if (p.bGate) {
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i) a[i] += half(bias[0], i), u[i] += half(bias[1], i);
+            }
+            withActivation(p.activation, [&](auto kind) {
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i) {
+                const Activated f = activate<kind.value, true>(a[i]);
+                if constexpr (PASS == Pass::forward) {
+                  a[i] = f.y * u[i];
+                } else {
+                  const float d = half(dh, i);
+                  a[i] = d * u[i] * f.slope;
+                  u[i] = d * f.y;
+                }
+              }
+            });
+            if (PASS == Pass::gradients || p.wholeH) {
+              *pieceOf(stage, 2 * k) = eightOf(a);
+              *pieceOf(stage, 2 * k + 1) = eightOf(a + 8);
             } else {
-              bf16 *e = reinterpret_cast<bf16 *>(gradients[k]);
+              storeRows(stage, eightOf(a), eightOf(a + 8), p.h + row * p.F + column, p.F, rowsLeft, columns, false, lane);
+            }
+            if constexpr (PASS == Pass::gradients) {
+              later[k][0] = eightOf(u), later[k][1] = eightOf(u + 8);
+              if (p.biasParts) {
+                if (rowsLeft < 32) {   // (a row that is not there may have become NaN beside an infinite bias)
 #pragma unroll
-              for (int i = 0; i < kChunk; ++i) e[i] = mine && i < columns ? from[i] : __ushort_as_bfloat16(0);
+                  for (int i = 0; i < kChunk; ++i) a[i] = mine ? a[i] : 0.f, u[i] = mine ? u[i] : 0.f;
+                }
+                const float sumA = columnSum(a, lane), sumU = columnSum(u, lane);
+                float *parts = p.biasParts + (int64_t(at.row / kTileRows) * 4 + quarter) * 2 * p.F + column;
+                if (lane < columns) parts[lane] = sumA, parts[p.F + lane] = sumU;
+              }
             }
           }
-          if (p.bGate) {
-            const int i = lane % kChunk;
-            biasOf[k] = i < columns ? toFloat((lane < kChunk ? p.bGate : p.bUp)[column + i]) : 0.f;
+          if (PASS == Pass::gradients || p.wholeH) {
+            fenceForCopies();
+            __syncwarp();
+            if (lane == 0) storeBox(&maps.out0, stage, first, int(row));
+          }
+        } else if (PASS == Pass::gradients && p.biasParts && part * kPart < kColumns && first < p.F) {
+          // No rows: their sums are zero.
+          float *parts = p.biasParts + (int64_t(at.row / kTileRows) * 4 + quarter) * 2 * p.F;
+          for (int column = first + lane; column < min(p.F, first + kPart); column += 32) parts[column] = parts[p.F + column] = 0.f;
+        }
+        tensorFenceBefore();
+        __syncwarp();
+        if (lane == 0) barrierArrive(taken + buffer);
+        if constexpr (PASS == Pass::gradients) {
+          if (p.wholeDh && fine && lane == 0) askGradients(t + gridDim.x);   // every lane has its row of this tile's
+          if (own) {
+            if (lane == 0) storesRead();
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < kChunks; ++k) {
+              *pieceOf(stage, 2 * k) = later[k][0];
+              *pieceOf(stage, 2 * k + 1) = later[k][1];
+            }
+            fenceForCopies();
+            __syncwarp();
+            if (lane == 0) storeBox(&maps.out1, stage, first, int(row));
           }
         }
       }
-      const bool fine = __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken));
-      tensorFenceAfter();
-      const uint32_t tensorRow = accumulators + buffer * BN + (uint32_t(quarter * 32) << 16);
-      // Columns of the accumulators from `column` on; zero where a tile has no steps.
-      auto take = [&](float (&x)[kChunk], int column) {
-        if (fine && steps > 0) {
-          tensorLoad16(x, tensorRow + column);
-        } else {
+      if (lane == 0) {
+        storesDone();
+        int none = 0;
+        if (asked) barrierWait(bar, parity, &none);   // given up: its own copy comes to its end
+      }
+      __syncwarp();
+    } else {
+      int n = 0;
+      for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++n) {
+        const Tile at = tileAt(t);
+        const int buffer = n & 1;
+        int first;
+        const int steps = stepsOf(at, first);
+        const int64_t row = at.row + quarter * 32, rowsLeft = (PASS == Pass::weights ? int64_t(p.F) : p.rows) - row;
+        const bool fine = __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken));
+        tensorFenceAfter();
+        const uint32_t tensorRow = accumulators + buffer * BN + (uint32_t(quarter * 32) << 16) + part * kPart;
 #pragma unroll
-          for (int i = 0; i < kChunk; ++i) x[i] = fine ? 0.f : __int_as_float(0x7fffffff);
-        }
-      };
-#pragma unroll
-      for (int k = 0; k < kChunks; ++k) {
-        const int c = part * kPart + k * kChunk;
-        const int column = at.column + c, columns = c < kColumns ? min(kChunk, (kDual ? p.F : p.D) - column) : 0;
-        if (columns <= 0) break;
-        __syncwarp();   // loads from tensor memory are the whole warp's
-        if constexpr (kDual) {
-          float a[kChunk], u[kChunk];
-          take(a, c);
-          take(u, BN / 2 + c);
-          if (p.bGate) {
-            bias[lane] = biasOf[k];
-            __syncwarp();
-          }
-          tensorLoadWait();
-          tensorLoaded(a);
-          tensorLoaded(u);
-          if (p.bGate) {
-#pragma unroll
-            for (int i = 0; i < kChunk; i += 4) {
-              const float4 g = *reinterpret_cast<const float4 *>(bias + i), b = *reinterpret_cast<const float4 *>(bias + kChunk + i);
-              a[i] += g.x, a[i + 1] += g.y, a[i + 2] += g.z, a[i + 3] += g.w;
-              u[i] += b.x, u[i + 1] += b.y, u[i + 2] += b.z, u[i + 3] += b.w;
-            }
-            __syncwarp();
-          }
-          withActivation(p.activation, [&](auto kind) {
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) {
-              const Activated f = activate<kind.value, true>(a[i]);
-              if constexpr (PASS == Pass::forward) {
-                a[i] = f.y * u[i];
-              } else {
-                const uint32_t two = reinterpret_cast<const uint32_t *>(gradients[k])[i / 2];
-                const float d = __uint_as_float(i % 2 ? two & 0xffff0000u : two << 16);
-                a[i] = d * u[i] * f.slope;
-                u[i] = d * f.y;
-              }
-            }
-          });
-          if constexpr (PASS == Pass::forward) {
-            storeRows(stage, eightOf(a), eightOf(a + 8), p.h + row * p.F + column, p.F, rowsLeft, columns, p.wholeH, lane);
-          } else {
-            bf16 *to = p.both + row * 2 * p.stride + column;
-            const int64_t stride = 2 * int64_t(p.stride);
-            storeRows(stage, eightOf(a), eightOf(a + 8), to, stride, rowsLeft, columns, true, lane);
-            storeRows(stage, eightOf(u), eightOf(u + 8), to + p.stride, stride, rowsLeft, columns, true, lane);
-            if (p.biasParts) {
-              if (!mine) {   // (a row that is not there may have become NaN beside an infinite bias)
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) a[i] = u[i] = 0.f;
-              }
-              const float sumA = columnSum(a, lane), sumU = columnSum(u, lane);
-              float *parts = p.biasParts + (int64_t(at.row / kTileRows) * 4 + quarter) * 2 * p.F + column;
-              if (lane < columns) parts[lane] = sumA, parts[p.F + lane] = sumU;
-            }
-          }
-        } else {
+        for (int k = 0; k < kChunks; ++k) {
+          const int column = at.column + part * kPart + k * kChunk, columns = min(kChunk, p.D - column);
+          if (columns <= 0) break;
           float x[kChunk];
-          take(x, c);
+          __syncwarp();
+          take(x, tensorRow + k * kChunk, fine, steps > 0);
           tensorLoadWait();
           tensorLoaded(x);
           if constexpr (PASS == Pass::input) {
@@ -420,10 +506,10 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
             if (columns > 8) storeRows(stage, fourOf(x + 8), fourOf(x + 12), to + 8, p.D, rowsLeft, columns - 8, true, lane);
           }
         }
+        tensorFenceBefore();
+        __syncwarp();
+        if (lane == 0) barrierArrive(taken + buffer);
       }
-      tensorFenceBefore();
-      __syncwarp();
-      if (lane == 0) barrierArrive(taken + buffer);
     }
   }
   tensorFenceBefore();

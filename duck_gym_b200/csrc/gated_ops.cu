@@ -141,6 +141,7 @@ bool gatedChecked(const duck_gated *a) {
   require(a->rows < (int64_t(1) << 31) - 4096 && a->D <= (1 << 24) && a->F <= (1 << 24), "Too many rows or columns");
   require(a->activation >= DUCK_SILU && a->activation <= DUCK_SIGMOID, "Invalid activation");
   require(a->type == DUCK_FLOAT32 || a->D % 8 == 0, "bfloat16 rows have to be whole 16-byte pieces");
+  require(a->type == DUCK_FLOAT32 || a->rows <= 1 || a->x == nullptr || a->x_stride >= a->D, "bfloat16 rows must not overlap");
   return a->rows > 0;
 }
 
@@ -195,8 +196,8 @@ GatedPlan planGated(const duck_gated &a) {
   return p;
 }
 
-// A map over bfloat16 rows for boxes of 64 values by boxRows rows.
-CUtensorMap mapOf(const void *base, int64_t columns, int64_t rows, int64_t stride, int boxRows) {
+// A map over bfloat16 rows for boxes of boxColumns values (64, 32 or 16: as wide as the swizzle) by boxRows rows.
+CUtensorMap mapOf(const void *base, int64_t columns, int64_t rows, int64_t stride, int boxRows, int boxColumns = 64) {
   using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -210,10 +211,13 @@ CUtensorMap mapOf(const void *base, int64_t columns, int64_t rows, int64_t strid
   }();
   CUtensorMap map;
   const cuuint64_t sizes[2] = {cuuint64_t(columns), cuuint64_t(rows)}, strides[1] = {cuuint64_t(stride) * 2};
-  const cuuint32_t box[2] = {64, cuuint32_t(boxRows)}, steps[2] = {1, 1};
+  const cuuint32_t box[2] = {cuuint32_t(boxColumns), cuuint32_t(boxRows)}, steps[2] = {1, 1};
+  const CUtensorMapSwizzle swizzle = boxColumns == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : boxColumns == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                        : CU_TENSOR_MAP_SWIZZLE_32B;
   auto fill = [&] {
     return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), sizes, strides, box, steps,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult status = fill();
@@ -231,8 +235,9 @@ CUtensorMap mapOf(const void *base, int64_t columns, int64_t rows, int64_t strid
 
 template <Pass PASS, int BN> void launchTiles(const TileMaps &maps, const TileArgs &t, cudaStream_t stream) {
   constexpr auto kernel = gatedTiles<PASS, BN>;
-  allowShared<kernel>(TileShared<BN>::bytes);
-  kernel<<<std::min(t.tiles, 148), kTileThreads, TileShared<BN>::bytes, stream>>>(maps, t);
+  constexpr int bytes = TileShared<PASS, BN>::bytes;
+  allowShared<kernel>(bytes);
+  kernel<<<std::min(t.tiles, 148), kTileThreads, bytes, stream>>>(maps, t);
   check(cudaGetLastError(), "gated linear launch");
 }
 
@@ -247,8 +252,16 @@ template <Pass PASS> void launchProjections(const duck_gated &a, TileArgs t, cud
   const int64_t rowTiles = ceilDiv(a.rows, kTileRows);
   auto run = [&](auto columns) {
     constexpr int BN = columns.value;
-    TileMaps maps;
-    maps.a0 = maps.a1 = mapOf(a.x, a.D, a.rows, a.x_stride, kTileRows);
+    constexpr int part = TileShared<PASS, BN>::part;
+    TileMaps maps{};   // (those that a pass does not use are not read)
+    if (PASS == Pass::gradients) {
+      if (t.wholeDh) maps.dh = mapOf(t.dh, a.F, a.rows, a.rows > 1 ? t.dhStride : t.stride, 32, part);
+      maps.out0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(t.stride), 32, part);
+      maps.out1 = mapOf(t.both + t.stride, a.F, a.rows, 2 * int64_t(t.stride), 32, part);
+    } else if (t.wholeH) {
+      maps.out0 = mapOf(t.h, a.F, a.rows, a.F, 32, part);
+    }
+    maps.a0 = mapOf(a.x, a.D, a.rows, a.rows > 1 ? a.x_stride : a.D, kTileRows);
     maps.b0 = mapOf(a.w_gate, a.D, a.F, a.D, BN / 2);
     maps.b1 = mapOf(a.w_up, a.D, a.F, a.D, BN / 2);
     t.steps = int(ceilDiv(a.D, kTileSteps));
@@ -265,6 +278,7 @@ TileArgs tileArgs(const duck_gated &a) {
   t.bGate = static_cast<const bf16 *>(a.b_gate);
   t.bUp = static_cast<const bf16 *>(a.b_up);
   t.rows = a.rows, t.D = a.D, t.F = a.F, t.activation = a.activation;
+  t.wholeBias = reinterpret_cast<uintptr_t>(a.b_gate) % 16 == 0 && reinterpret_cast<uintptr_t>(a.b_up) % 16 == 0;
   t.splits = 1;
   return t;
 }
@@ -315,7 +329,7 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
   float *parts = plan.partBytes ? reinterpret_cast<float *>(scratch + plan.bothBytes + plan.biasBytes) : nullptr;
   t.dh = static_cast<const bf16 *>(a.dh);
   t.dhStride = a.dh_stride;
-  t.wholeDh = reinterpret_cast<uintptr_t>(a.dh) % 16 == 0 && a.dh_stride % 8 == 0;
+  t.wholeDh = reinterpret_cast<uintptr_t>(a.dh) % 16 == 0 && a.dh_stride % 8 == 0 && a.dh_stride >= a.F;
   t.biasParts = biasParts;
   launchProjections<Pass::gradients>(a, t, stream);
   const int64_t rowTiles = ceilDiv(a.rows, kTileRows);
@@ -323,7 +337,7 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
     t.dx = static_cast<bf16 *>(a.dx);
     t.steps = int(ceilDiv(a.F, kTileSteps));
     withColumns(tileColumns(rowTiles, a.D), [&](auto n) {
-      TileMaps maps;
+      TileMaps maps{};
       maps.a0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
       maps.a1 = mapOf(t.both + plan.stride, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
       maps.b0 = mapOf(a.w_gate, a.D, a.F, a.D, 64);
@@ -342,10 +356,10 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
     t.steps = int(ceilDiv(a.rows, kTileSteps));
     t.rowTiles = int(ceilDiv(a.F, kTileRows));
     withColumns(plan.weightColumns, [&](auto n) {
-      TileMaps maps;
+      TileMaps maps{};
       maps.a0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(plan.stride), 64);
       maps.a1 = mapOf(t.both + plan.stride, a.F, a.rows, 2 * int64_t(plan.stride), 64);
-      maps.b0 = maps.b1 = mapOf(a.x, a.D, a.rows, a.x_stride, 64);
+      maps.b0 = mapOf(a.x, a.D, a.rows, a.rows > 1 ? a.x_stride : a.D, 64);
       t.columnTiles = int(ceilDiv(a.D, n.value));
       const int64_t tiles = int64_t(t.columnTiles) * 2 * t.rowTiles * t.splits;
       require(tiles < (int64_t(1) << 31), "Too many rows and columns");

@@ -61,6 +61,18 @@ __device__ __forceinline__ void copyBox(void *to, const CUtensorMap *map, int x,
       "l"(map), "r"(x), "r"(y), "r"(sharedAddress(bar))
       : "memory");
 }
+// A box from shared memory to the map's array at {x, y}; what lies beyond the array is
+// left out.  The box's memory was written before fenceForCopies().
+__device__ __forceinline__ void storeBox(const CUtensorMap *map, const void *from, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+               "r"(sharedAddress(from))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void fenceForCopies() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Until this thread's stored boxes have been read, or are in memory.
+__device__ __forceinline__ void storesRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void storesDone() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void prefetchMap(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }

@@ -543,10 +543,12 @@ def _gated_workspace(rows, D, F, kind, weights, biases):
 
 def _gated_operand(t, strided):
     """Rows as the kernels take them: dense (`strided`: up to the distance of the
-    rows), for bfloat16 of whole 16-byte pieces on their boundaries."""
+    rows), for bfloat16 of whole 16-byte pieces on their boundaries, and apart."""
     t = _rows_of(t) if strided else t.contiguous()
-    if t.dtype == torch.bfloat16 and (t.data_ptr() % 16 or t.stride(0) % 8):
-        t = t.clone(memory_format=torch.contiguous_format)
+    if t.dtype is torch.bfloat16:
+        stride = t.stride(0)
+        if t.data_ptr() % 16 or stride % 8 or stride < t.shape[1]:
+            t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -555,7 +557,7 @@ def _gated_forward(x, w_gate, w_up, b_gate, b_up, activation, keep):
     F_ = w_gate.shape[0]
     kind = _TYPES[x.dtype]
     h = torch.empty((rows, F_), dtype=x.dtype, device=x.device)
-    kept = _buffer(_gated_workspace(rows, D, F_, kind, False, False)[1], x.device) if keep else None
+    kept = _buffer(_gated_workspace(rows, D, F_, kind, False, False)[1], x.device) if keep and kind == 0 else None
     _launch(library().duck_gated_linear_forward, x.device,
             _GATED.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate), _address(b_up), h.data_ptr(),
                         0, 0, 0, 0, 0, 0, _address(kept), 0, rows, x.stride(0), 0, D, F_, activation, kind))
@@ -570,7 +572,7 @@ class _GatedLinear(torch.autograd.Function):
         h, kept = _gated_forward(x, w_gate, w_up, b_gate, b_up, activation, True)
         ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up, kept)
         ctx.activation = activation
-        return h.view(ctx.shape[:-1] + (h.shape[1],))
+        return h if len(ctx.shape) == 2 else h.view(ctx.shape[:-1] + (h.shape[1],))
 
     @staticmethod
     @_once
@@ -591,7 +593,7 @@ class _GatedLinear(torch.autograd.Function):
                 _GATED.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate), _address(b_up), 0,
                             dh.data_ptr(), _address(dx), _address(dw[0]), _address(dw[1]), _address(db[0]), _address(db[1]),
                             _address(kept), _address(scratch), rows, x.stride(0), dh.stride(0), D, F_, ctx.activation, kind))
-        return dx.view(ctx.shape) if needs[0] else None, *dw, *db, None
+        return dx if dx is None or len(ctx.shape) == 2 else dx.view(ctx.shape), *dw, *db, None
 
 
 @torch.autocast("cpu", enabled=False)
@@ -620,8 +622,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
              and w_gate.numel() > 0, "gated_linear: weights are [F, D] for x [..., D]")
     _require((b_gate is None) == (b_up is None) and all(b is None or b.shape == w_gate.shape[:1] for b in (b_gate, b_up)),
              "gated_linear: biases are [F], both or neither")
-    given = [t for t in (x, w_gate, w_up, b_gate, b_up) if t is not None]
-    _require(all(t.dtype == x.dtype and t.device == x.device for t in given) and x.dtype in _WIDE,
+    dtype, device = x.dtype, x.device
+    _require(dtype in _WIDE and w_gate.dtype is dtype and w_up.dtype is dtype and w_gate.device == device == w_up.device
+             and (b_gate is None or (b_gate.dtype is dtype and b_up.dtype is dtype and b_gate.device == device == b_up.device)),
              "gated_linear: one floating type and device for x, weights and biases")
     if not x.is_cuda:
         return _gated_plain(x, w_gate, w_up, b_gate, b_up, activation)
@@ -636,7 +639,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     shape = x.shape
     x, w_gate, w_up = _gated_operand(x, True), _gated_operand(w_gate, False), _gated_operand(w_up, False)
     h, _ = _gated_forward(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[activation], False)
-    return h.view(shape[:-1] + (h.shape[1],))
+    return h if len(shape) == 2 else h.view(shape[:-1] + (h.shape[1],))
 
 
 # ----------------------------------------------------------- 8-bit checkpoints

@@ -467,7 +467,7 @@ int duck_gated_recurrence_step(const duck_recurrence *args, duck_stream stream);
  * and its gradients.  Element types are those of `type` throughout; h, the
  * weights, their gradients and dx are dense, rows of x and dh have the strides
  * given.  For DUCK_BFLOAT16 the rows of x, the weights and their gradients are
- * whole 16-byte pieces on 16-byte boundaries (D a multiple of 8).  `kept` is what a
+ * whole 16-byte pieces on 16-byte boundaries (D a multiple of 8) and do not overlap.  `kept` is what a
  * forward call leaves for the backward one (DUCK_FLOAT32 only, else NULL).
  * Outputs and workspaces lie on 16-byte boundaries, and no output overlaps an
  * input. */

@@ -376,6 +376,9 @@ def test_linear_strides(D, F, dtype):
     loose = torch.empty(150, F + 3, dtype=dtype, device="cuda")[:, 1:1 + F]
     loose.copy_(dh)
     check_layer(case, "silu", None, loose)
+    window = torch.empty(150 * 8 + D, dtype=dtype, device="cuda").normal_().as_strided((150, D), (8, 1))   # rows that overlap
+    over = [window.cpu(), *case[1:]]
+    check_layer(over, "silu", [window.detach(), *dev()[1:]])
     ones = case[:5] + [torch.ones(150, F, dtype=dtype)]
     check_layer(ones, "silu", None, torch.ones((), dtype=dtype, device="cuda").expand(150, F))
 
