@@ -36,7 +36,7 @@ namespace duckb200 {
 constexpr int kMomentGroup = 128;
 constexpr int kAdamThreads = 256, kAdamRound = kAdamThreads / 32 * kMomentGroup;   // one group for each warp
 constexpr int kAdamRoundsMost = 16;
-constexpr int kNormChunk = 8 * kAdamRound, kValuesChunk = 2 * kAdamRound;
+constexpr int kNormChunk = 8 * kAdamRound;
 constexpr int kNormBlocks = 148 * 4;   // and sums, at most
 
 struct AdamTensor {
@@ -413,36 +413,43 @@ __global__ void __launch_bounds__(kAdamThreads, 4) adamStep(const __grid_constan
 }
 
 // What codes stand for, in float32: param receives the values of m (signed codes)
-// or, where m is null, of v.
-template <int MOST>
+// or, where m is null, of v.  A warp has U groups at once, as many bytes of codes as
+// keep the memory busy (64M values: 57 us with eight, 77 with two), or two of them
+// where the values are few and blocks many.
+template <int MOST, int U>
 __global__ void __launch_bounds__(kAdamThreads) momentValues(const __grid_constant__ AdamTable<MOST> table, int count, int chunks) {
-  constexpr int U = kValuesChunk / kAdamRound;
   const int lane = threadIdx.x % 32;
   for (int chunk = blockIdx.x, index = 0; chunk < chunks; chunk += gridDim.x) {
     index = tensorOf(table, count, chunk, index);
     const AdamTensor &t = table.t[index];
-    const int64_t first = int64_t(chunk - t.first) * kValuesChunk + threadIdx.x / 32 * U * kMomentGroup;
+    const int64_t first = int64_t(chunk - t.first) * U * kAdamRound + threadIdx.x / 32 * U * kMomentGroup;
     float *out = static_cast<float *>(t.param);
     const bool sign = t.m != nullptr;
     const uint8_t *codes = static_cast<const uint8_t *>(sign ? t.m : t.v), *exponents = sign ? t.me : t.ve;
+    auto value = [&](uint32_t code, uint32_t e, int low) {
+      const int c = sign ? int(int8_t(code)) : int(code & 0xff);
+      const float magnitude = e == 255 ? __int_as_float(0x7fffffff) : momentValue(abs(c), low);
+      return c < 0 ? -magnitude : magnitude;
+    };
+    if (t.pieces && first + U * kMomentGroup <= t.n) {   // whole groups, all asked for at once
+      uint32_t code[U], e[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = first + u * kMomentGroup;
-      if (at >= t.n) continue;
-      const int left = int(min(int64_t(kMomentGroup), t.n - at));
-      const uint32_t e = exponents[at / kMomentGroup];
-      const int low = sign ? lowestCode<127>(e) : lowestCode<255>(e);
-      auto value = [&](uint8_t code) {
-        const int c = sign ? int(int8_t(code)) : int(code);
-        const float magnitude = e == 255 ? __int_as_float(0x7fffffff) : momentValue(abs(c), low);
-        return c < 0 ? -magnitude : magnitude;
-      };
-      if (t.pieces && left == kMomentGroup) {
-        const int64_t here = at + 4 * lane;
-        const uchar4 c = *reinterpret_cast<const uchar4 *>(codes + here);
-        *reinterpret_cast<float4 *>(out + here) = make_float4(value(c.x), value(c.y), value(c.z), value(c.w));
-      } else {
-        for (int i = lane; i < left; i += 32) out[at + i] = value(codes[at + i]);
+      for (int u = 0; u < U; ++u) {
+        code[u] = *reinterpret_cast<const uint32_t *>(codes + first + u * kMomentGroup + 4 * lane);
+        e[u] = exponents[first / kMomentGroup + u];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int low = sign ? lowestCode<127>(e[u]) : lowestCode<255>(e[u]);
+        *reinterpret_cast<float4 *>(out + first + u * kMomentGroup + 4 * lane) =
+            make_float4(value(code[u], e[u], low), value(code[u] >> 8, e[u], low), value(code[u] >> 16, e[u], low),
+                        value(code[u] >> 24, e[u], low));
+      }
+    } else {
+      for (int64_t at = first; at < min(t.n, first + U * kMomentGroup); at += kMomentGroup) {
+        const uint32_t e = exponents[at / kMomentGroup];
+        const int low = sign ? lowestCode<127>(e) : lowestCode<255>(e);
+        for (int64_t i = at + lane; i < min(t.n, at + kMomentGroup); i += 32) out[i] = value(codes[i], e, low);
       }
     }
   }

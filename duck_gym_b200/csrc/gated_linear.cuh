@@ -561,11 +561,11 @@ template <Pass PASS, int T> __global__ void __launch_bounds__(kProductThreads, 2
   constexpr bool kAlongA = PASS != Pass::weights, kAlongB = PASS == Pass::forward;   // steps are contiguous
   __shared__ __align__(16) float as[2][K][P], bs[2][K][P];
   const int tid = threadIdx.x;
-  const int64_t row0 = int64_t(blockIdx.y) * T;   // weights: of Wg's and then Wu's tiles
+  const int64_t row0 = int64_t(blockIdx.x) * T;   // weights: of Wg's and then Wu's tiles
   const int rowTiles = (p.F + T - 1) / T;
-  const int half = PASS == Pass::weights && int(blockIdx.y) >= rowTiles;
+  const int half = PASS == Pass::weights && int(blockIdx.x) >= rowTiles;
   const int64_t m0 = PASS == Pass::weights ? row0 - int64_t(half) * rowTiles * T : row0;
-  const int n0 = blockIdx.x * (PASS == Pass::forward ? T / 2 : T);
+  const int n0 = blockIdx.y * (PASS == Pass::forward ? T / 2 : T);
   const int64_t plane = p.rows * p.F;
   const int halfSteps = (p.F + K - 1) / K;   // input: steps of the first product, then those of the second
   const int64_t allSteps = PASS == Pass::forward ? (p.D + K - 1) / K : PASS == Pass::input ? 2 * halfSteps : (p.rows + K - 1) / K;
@@ -700,8 +700,8 @@ struct GradientArgs {
 constexpr int kGradientRows = 64;
 __global__ void __launch_bounds__(256) gatedGradients(GradientArgs p) {
   __shared__ float sums[8][2][32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, f = blockIdx.x * 32 + lane;
-  const int64_t row0 = int64_t(blockIdx.y) * kGradientRows, plane = p.rows * p.F;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, f = blockIdx.y * 32 + lane;
+  const int64_t row0 = int64_t(blockIdx.x) * kGradientRows, plane = p.rows * p.F;
   float sumA = 0.f, sumU = 0.f;
   if (f < p.F)
     withActivation(p.activation, [&](auto kind) {
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(256) gatedGradients(GradientArgs p) {
   float sum = 0.f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) sum += sums[w][warp][lane];
-  p.biasParts[(int64_t(blockIdx.y) * 2 + warp) * p.F + f] = sum;
+  p.biasParts[(int64_t(blockIdx.x) * 2 + warp) * p.F + f] = sum;
 }
 
 // -------------------------------------------------------------- sums of parts

@@ -138,7 +138,7 @@ bool gatedChecked(const duck_gated *a) {
   require(a != nullptr, "Invalid arguments");
   requireType(a->type);
   require(a->rows >= 0 && a->D > 0 && a->F > 0, "Invalid layer sizes");
-  require(a->rows < (int64_t(1) << 31) - 4096 && a->D <= (1 << 24) && a->F <= (1 << 24), "Too many rows or columns");
+  require(a->rows < (int64_t(1) << 31) - 4096 && a->D <= (1 << 20) && a->F <= (1 << 20), "Too many rows or columns");
   require(a->activation >= DUCK_SILU && a->activation <= DUCK_SIGMOID, "Invalid activation");
   require(a->type == DUCK_FLOAT32 || a->D % 8 == 0, "bfloat16 rows have to be whole 16-byte pieces");
   require(a->type == DUCK_FLOAT32 || a->rows <= 1 || a->x == nullptr || a->x_stride >= a->D, "bfloat16 rows must not overlap");
@@ -299,8 +299,7 @@ ProductArgs productArgs(const duck_gated &a) {
 // rows, 61 x 301: the gradient of x 85 us in 40 tiles of 128, 35 in 79 of 64).
 template <Pass PASS> void launchProducts(const ProductArgs &g, int tile, int64_t rows, int64_t columns, int splits, cudaStream_t stream) {
   const int64_t rowTiles = (PASS == Pass::weights ? 2 : 1) * ceilDiv(rows, tile);
-  require(rowTiles < 65536, "Too many rows or columns");
-  const dim3 grid(unsigned(ceilDiv(columns, tile)), unsigned(rowTiles), unsigned(splits));
+  const dim3 grid(unsigned(rowTiles), unsigned(ceilDiv(columns, tile)), unsigned(splits));
   if (tile == 128) gatedProducts<PASS, 128><<<grid, kProductThreads, 0, stream>>>(g);
   else gatedProducts<PASS, 64><<<grid, kProductThreads, 0, stream>>>(g);
   check(cudaGetLastError(), "gated linear launch");
@@ -377,10 +376,9 @@ void gatedBackward32(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
   float *biasParts = a.db_gate ? reinterpret_cast<float *>(scratch + plan.bothBytes) : nullptr;
   float *parts = a.dw_gate ? reinterpret_cast<float *>(scratch + plan.bothBytes + plan.biasBytes) : nullptr;
   const int64_t rowBlocks = ceilDiv(a.rows, kGradientRows);
-  require(rowBlocks < 65536, "Too many rows or columns");
   const GradientArgs e{static_cast<const float *>(a.kept), static_cast<const float *>(a.dh), both, biasParts, a.rows, a.dh_stride,
                        a.F, a.activation};
-  gatedGradients<<<dim3(unsigned(ceilDiv(a.F, 32)), unsigned(rowBlocks)), 256, 0, stream>>>(e);
+  gatedGradients<<<dim3(unsigned(rowBlocks), unsigned(ceilDiv(a.F, 32))), 256, 0, stream>>>(e);
   check(cudaGetLastError(), "gated linear launch");
   g.both = both;
   if (a.dx) {

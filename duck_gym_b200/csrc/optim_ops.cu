@@ -48,6 +48,11 @@ std::vector<Launch> launchesOf(const duck_adamw_tensor *tensors, int count, int 
   }
   return launches;
 }
+int64_t valuesOf(const duck_adamw_tensor *tensors, int count) {
+  int64_t values = 0;
+  for (int i = 0; i < count; ++i) values += tensors[i].n;
+  return values;
+}
 template <class F> void withTable(const Launch &l, F &&f) {
   auto fill = [&](auto table) {
     std::copy(l.tensors.begin(), l.tensors.end(), table.t);
@@ -132,9 +137,8 @@ int duck_adamw_step(const duck_adamw_tensor *tensors, int count, const duck_adam
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     // As many rounds a chunk as leave every block one: a chunk finds its tensor and fills its ring anew.
-    int64_t values = 0;
-    for (int i = 0; i < count; ++i) values += tensors[i].n;
-    const int rounds = int(std::max<int64_t>(1, std::min<int64_t>(kAdamRoundsMost, values / (int64_t(148) * 4 * kAdamRound))));
+    const int rounds = int(std::max<int64_t>(
+        1, std::min<int64_t>(kAdamRoundsMost, valuesOf(tensors, count) / (int64_t(148) * 4 * kAdamRound))));
     std::vector<Launch> launches = launchesOf(tensors, count, rounds * kAdamRound, o.bits == 8);
     if (launches.empty()) launches.push_back({DUCK_FLOAT32, {}, 0});   // the step is counted all the same
     for (size_t i = 0; i < launches.size(); ++i) {
@@ -160,10 +164,13 @@ int duck_moment_values(const duck_adamw_tensor *tensors, int count, duck_stream 
               "Invalid arguments");
     }
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    for (const Launch &l : launchesOf(tensors, count, kValuesChunk, true)) {
+    const int groups = valuesOf(tensors, count) >= int64_t(148) * 8 * 8 * kAdamRound ? 8 : 2;
+    for (const Launch &l : launchesOf(tensors, count, groups * kAdamRound, true)) {
       withTable(l, [&](const auto &table) {
         constexpr int M = sizeof(table.t) / sizeof(AdamTensor);
-        momentValues<M><<<std::min(l.chunks, 148 * 8), kAdamThreads, 0, s>>>(table, int(l.tensors.size()), l.chunks);
+        const int blocks = std::min(l.chunks, 148 * 8);
+        if (groups == 8) momentValues<M, 8><<<blocks, kAdamThreads, 0, s>>>(table, int(l.tensors.size()), l.chunks);
+        else momentValues<M, 2><<<blocks, kAdamThreads, 0, s>>>(table, int(l.tensors.size()), l.chunks);
       });
       check(cudaGetLastError(), "moment values launch");
     }

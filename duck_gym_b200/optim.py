@@ -395,7 +395,8 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """As torch's, but moments keep their types (torch would convert them to the
-        parameters')."""
+        parameters').  One of torch's own Adam or AdamW is taken too: its moments have 32
+        bits, and its count of steps becomes the group's."""
         super().load_state_dict(state_dict)
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         mine = [p for group in self.param_groups for p in group["params"]]
@@ -404,5 +405,10 @@ class AdamW(torch.optim.Optimizer):
                 if torch.is_tensor(value):
                     self.state[p][name] = value.to(p.device, copy=True).contiguous()
         for group in self.param_groups:
-            if torch.is_tensor(group.get("step")):
+            group.setdefault("bits", 32)
+            counts = [int(self.state[p].pop("step")) for p in group["params"] if "step" in self.state[p]]
+            if "step" not in group and counts:
+                _require(len(set(counts)) == 1, "AdamW: the parameters of a group have one count of steps")
+                group["step"] = torch.full((), counts[0], dtype=torch.int64)
+            if "step" in group:
                 group["step"] = group["step"].to(group["params"][0].device, copy=True)

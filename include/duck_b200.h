@@ -464,13 +464,13 @@ int duck_gated_recurrence_step(const duck_recurrence *args, duck_stream stream);
 
 /* Gated linear layer on rows x [rows, D]:
  *   h = act(x w_gate^T + b_gate) (x w_up^T + b_up),  weights [F, D], biases [F]
- * and its gradients.  Element types are those of `type` throughout; h, the
- * weights, their gradients and dx are dense, rows of x and dh have the strides
- * given.  For DUCK_BFLOAT16 the rows of x, the weights and their gradients are
- * whole 16-byte pieces on 16-byte boundaries (D a multiple of 8) and do not overlap.  `kept` is what a
- * forward call leaves for the backward one (DUCK_FLOAT32 only, else NULL).
- * Outputs and workspaces lie on 16-byte boundaries, and no output overlaps an
- * input. */
+ * and its gradients.  rows < 2^31 - 4096, D and F up to 2^20.  Element types are
+ * those of `type` throughout; h, the weights, their gradients and dx are dense,
+ * rows of x and dh have the strides given.  For DUCK_BFLOAT16 the rows of x, the
+ * weights and their gradients are whole 16-byte pieces on 16-byte boundaries (D a
+ * multiple of 8), and rows of x do not overlap.  `kept` is what a forward call
+ * leaves for the backward one (DUCK_FLOAT32 only, else NULL).  Outputs and
+ * workspaces lie on 16-byte boundaries, and no output overlaps an input. */
 enum { DUCK_SILU = 0, DUCK_GELU = 1, DUCK_SIGMOID = 2 };
 typedef struct duck_gated {
   const void *x, *w_gate, *w_up;

@@ -179,6 +179,26 @@ def test_class_goes_on_from_a_state_dict(bits, dtype):
     assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(*runs))
 
 
+@pytest.mark.parametrize("kind", [torch.optim.Adam, torch.optim.AdamW])
+def test_class_goes_on_from_torch(kind):
+    p, g = model(8, [(150,), (3, 4)])
+    results = []
+    for switch in (False, True):
+        params = [torch.nn.Parameter(x.clone()) for x in p]
+        opt = kind(params, lr=1e-2, weight_decay=0.0)
+        for k in range(6):
+            if switch and k == 3:
+                saved, opt = opt.state_dict(), optim.AdamW(params, bits=8)
+                opt.load_state_dict(saved)
+            for x, y in zip(params, g):
+                x.grad = y * (k + 1)
+            opt.step()
+        results.append([x.detach() for x in params])
+    assert int(opt.param_groups[0]["step"]) == 6 and opt.param_groups[0]["bits"] == 32
+    for a, b in zip(*results):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
+
+
 def test_parameters_without_gradients():
     params = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(3))]
     opt = optim.AdamW(params, lr=0.1)
