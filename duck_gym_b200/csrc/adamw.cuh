@@ -26,8 +26,11 @@
 // formula is computed.
 //
 // Bound by memory: 28 bytes a value with 32-bit moments, 16 with 8-bit ones
-// (float32 parameters), and 4 for the norm.  A warp has the 128 values of a
-// group, two groups at once.
+// (float32 parameters), and 4 for the norm.  A warp has the 128 values of a group,
+// and the next three groups' operands on their way through shared memory.  Measured on
+// a B200, cold: 64M values, float32, moments in 8 bits 214 us (5.0 TB/s, issue slots 77 %
+// busy; with the loads in registers, two groups at once, 360); a policy's 0.4M values,
+// moments in 32 bits, 7 us and 3 for the norm.
 #pragma once
 #include "numeric_types.cuh"
 

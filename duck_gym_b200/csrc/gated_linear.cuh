@@ -16,7 +16,13 @@
 //
 // One block a multiprocessor goes through tiles of 128 rows: one thread issues the
 // copies, one the products, sixteen warps take finished accumulators out, while the
-// products of the next tile go to the other half of tensor memory.
+// products of the next tile go to the other half of tensor memory.  Measured on a
+// B200, cold: 16384 rows, 1024 x 4096, forward 181 us (1.52 PFLOP/s, tensor pipe 79 %),
+// da and du 247, dx 209, weights 208 (80 %, of which four rounds for 3.5 of tiles); 24576
+// rows, 256 x 512: 21, 42, 18, 18 and 5 us for the sums, where the accumulators' way out
+// bounds the first two (forward: 10 us of it alone, 10 of products and copies alone, 13
+// together, and 7 for the start and the end; da and du: 18 of 42 for shuffles of the bias
+// sums, dh and stores).
 //
 // float32 (gatedProducts): FMA in pairs; a and u are kept, since they are exact and
 // their products are what the time goes to.

@@ -115,12 +115,12 @@ template <class T, int V, int SLOTS> void launchBackward(const RecurrenceArgs &r
   run<<<recurrenceGrid(channels, V, r.segmentCount), kRecurrenceThreads, bytes, stream>>>(r);
 }
 // Two channels a thread where they can be moved at once (four take twice the registers: a second, partly filled round of
-// blocks).  Four slots where the blocks are less than four a multiprocessor (1000 steps, 256 x 256 channels: forward 108 us,
-// backward 153; eight slots the same), two where there are more and their copies fill the memory's queue.
-constexpr int kFewBlocks = 148 * 4, kFewSlots = 4;
+// blocks).  Four slots where there are fewer than 512 threads a multiprocessor (1000 steps, 256 x 256 channels: forward 108 us,
+// backward 153; eight slots the same, blocks of 32 or 64 threads too), two where there are more and their copies fill the
+// memory's queue.
+constexpr int kFewThreads = 148 * 512, kFewSlots = 4;
 template <class T, class F> void withSlots(const RecurrenceArgs &r, bool two, F &&f) {
-  const int64_t blocks = ceilDiv(int64_t(r.E) * r.N, int64_t(kRecurrenceThreads) * (two ? 2 : 1)) * r.segmentCount;
-  const bool few = blocks < kFewBlocks;
+  const bool few = ceilDiv(int64_t(r.E) * r.N, two ? 2 : 1) * r.segmentCount < kFewThreads;
   auto slots = [&](auto v) {
     if (few) f(v, std::integral_constant<int, kFewSlots>());
     else f(v, std::integral_constant<int, 2>());

@@ -11,7 +11,7 @@
 //
 // A reset replaces the state instead of multiplying it by zero: what an earlier
 // episode left there, infinities and NaN included, does not reach the next one.
-// f and 1 - f both come from t = exp(-|gate|), 1 / (1 + t) and t / (1 + t), so
+// f and 1 - f both come from one exponential t, as 1 / (1 + t) and t / (1 + t), so
 // that neither loses digits where the other is near 1.
 //
 // A thread has V neighbouring channels of one environment and goes along the
@@ -19,7 +19,7 @@
 // pass needs h_{t-1} in float32: the forward pass keeps h at every kKeep-th step
 // only, and the backward pass, which reads gates and values anyway, runs kKeep
 // steps forwards from there in registers before it goes back through them.  So
-// it moves five values an element and 8 / kKeep bytes, and out is not read.
+// it moves five values an element and 4 / kKeep bytes each way, and out is not read.
 //
 // Where channels are few, the steps are split into segments.  A segment maps the
 // state that it begins with to h -> P h + B; a first pass finds P and B of each
@@ -27,7 +27,13 @@
 // to the initial state.  P's sign bit (products of gates have none) says that an
 // episode begins inside, B alone being what is left.
 //
-// Bound by memory, as elementwise passes are.
+// Bound by memory in principle; 23 instructions a value in the forward pass (issue
+// slots 56 % busy) and warps that wait for their copies keep it at 60 % of the copy's
+// rate.  Measured on a B200, cold,
+// bfloat16: 24 steps of 1024 x 256 channels, forward 12 us, backward 15.5 (38 and
+// 65 MB); 1000 steps of 256 x 256, 108 and 153 us (3.6 and 4.3 TB/s, both of them with
+// the kept states); 16384 steps of 1024 channels in 74 segments, 24 us for P and B and
+// 32 for the outputs.  One step of 4096 x 256 channels 4.6 us.
 #pragma once
 #include "numeric_types.cuh"
 
