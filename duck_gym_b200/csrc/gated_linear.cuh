@@ -182,7 +182,8 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
   uint8_t *incoming = staging + kTileWarps * S::staging;
   uint64_t *full = reinterpret_cast<uint64_t *>(incoming + kTileWarps * S::incoming);
   uint64_t *empty = full + S::stages, *done = empty + S::stages, *taken = done + 2, *came = taken + 2;
-  uint32_t *tensor = reinterpret_cast<uint32_t *>(came + kTileWarps);
+  uint64_t *ended = came + kTileWarps;
+  uint32_t *tensor = reinterpret_cast<uint32_t *>(ended + 1);
   volatile int *broken = reinterpret_cast<volatile int *>(tensor + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
@@ -191,6 +192,7 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
     for (int i = 0; i < S::stages; ++i) barrierInit(full + i, 1), barrierInit(empty + i, 1);
     for (int i = 0; i < 2; ++i) barrierInit(done + i, 1), barrierInit(taken + i, kTileWarps);
     for (int i = 0; i < kTileWarps; ++i) barrierInit(came + i, 1);
+    barrierInit(ended, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -304,6 +306,11 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
           if (++stage == S::stages) stage = 0, parity ^= 1;
         }
         if (fine) tensorCommit(done + buffer);
+      }
+      if (!fine) {   // given up: the products that were issued come to their end, too
+        int none = 0;
+        tensorCommit(ended);
+        barrierWait(ended, 0, &none);
       }
     }
   } else if (warp >= 4) {
