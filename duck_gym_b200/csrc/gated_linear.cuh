@@ -84,7 +84,7 @@ struct TileArgs {
   float *biasParts;          // [128-row tiles x 4, 2, F]: sums over 32 rows, or null
   bf16 *dx;                  // input
   bf16 *dwGate, *dwUp;       // weights, where they are not split
-  float *parts;              // [splits, 2, F, D]
+  float *parts;              // weights: [splits, 2, F, D], input: [splits, rows, D]
   int64_t rows, dhStride;
   int D, F, stride, activation;
   int tiles, columnTiles, rowTiles, splits, steps;   // steps of 64 of a tile's product
@@ -215,19 +215,19 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
       at.split = rest / (2 * p.rowTiles);
       at.half = row >= p.rowTiles;
       at.row = (row - at.half * p.rowTiles) * kTileRows;
+    } else if constexpr (PASS == Pass::input) {
+      at.split = rest / p.rowTiles;
+      at.row = (rest - at.split * p.rowTiles) * kTileRows;
     } else {
       at.row = rest * kTileRows;
     }
     return at;
   };
   auto stepsOf = [&](const Tile &at, int &first) {
-    if constexpr (PASS == Pass::weights) {
-      const int each = (p.steps + p.splits - 1) / p.splits;
+    if constexpr (PASS == Pass::weights || PASS == Pass::input) {
+      const int all = PASS == Pass::input ? 2 * p.steps : p.steps, each = (all + p.splits - 1) / p.splits;
       first = at.split * each;
-      return max(0, min(p.steps, first + each) - first);
-    } else if constexpr (PASS == Pass::input) {
-      first = 0;
-      return 2 * p.steps;
+      return max(0, min(all, first + each) - first);
     } else {
       first = 0;
       return p.steps;
@@ -257,8 +257,8 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
             copyBox(b, &maps.b0, x, at.column, bar);
             copyBox(b + S::b / 2, &maps.b1, x, at.column, bar);
           } else if constexpr (PASS == Pass::input) {
-            const bool up = k >= p.steps;
-            const int x = (up ? k - p.steps : k) * kTileSteps;
+            const bool up = first + k >= p.steps;   // du and Wu after da and Wg
+            const int x = (first + k - (up ? p.steps : 0)) * kTileSteps;
             copyBox(a, up ? &maps.a1 : &maps.a0, x, at.row, bar);
 #pragma unroll
             for (int j = 0; j < BN / 64; ++j) copyBox(b + j * 8192, up ? &maps.b1 : &maps.b0, at.column + 64 * j, x, bar);
@@ -508,13 +508,12 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
           take(x, tensorRow + k * kChunk, fine, steps > 0);
           tensorLoadWait();
           tensorLoaded(x);
-          if constexpr (PASS == Pass::input) {
-            storeRows(stage, eightOf(x), eightOf(x + 8), p.dx + row * p.D + column, p.D, rowsLeft, columns, true, lane);
-          } else if (p.splits == 1) {
-            storeRows(stage, eightOf(x), eightOf(x + 8), (at.half ? p.dwUp : p.dwGate) + row * p.D + column, p.D, rowsLeft, columns,
-                      true, lane);
+          if (p.splits == 1) {
+            bf16 *to = PASS == Pass::input ? p.dx : at.half ? p.dwUp : p.dwGate;
+            storeRows(stage, eightOf(x), eightOf(x + 8), to + row * p.D + column, p.D, rowsLeft, columns, true, lane);
           } else {
-            float *to = p.parts + ((int64_t(at.split) * 2 + at.half) * p.F + row) * p.D + column;
+            const int64_t before = PASS == Pass::input ? at.split * p.rows : (int64_t(at.split) * 2 + at.half) * p.F;
+            float *to = p.parts + (before + row) * p.D + column;
             storeRows(stage, fourOf(x), fourOf(x + 4), to, p.D, rowsLeft, columns, true, lane);
             if (columns > 8) storeRows(stage, fourOf(x + 8), fourOf(x + 12), to + 8, p.D, rowsLeft, columns - 8, true, lane);
           }
@@ -536,16 +535,19 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
 // pairs; the operands of the next steps are on their way in registers.  Where that
 // leaves multiprocessors without a tile, of 64 by 64 and 4 by 4.  The forward pass's
 // columns are half of Wg's and half the same of Wu's: a thread has both of a value.
+// A sum of n values of random sign is off by 2^-25 sqrt(n / 2) of itself where each is
+// added to one register; after kProductRun steps it goes to memory, and is added to
+// there, so that long ones are off by no more than 7e-7.
 struct ProductArgs {
   const float *x, *wGate, *wUp, *bGate, *bUp;
   float *h, *kept;             // forward: h, and a and u [2, rows, F] or null
   const float *both;           // [2, rows, F]: da and du
-  float *dx, *parts;           // [splits, 2, F, D]
+  float *dx, *parts;           // weights: [splits, 2, F, D], input: [splits, rows, D] where it is split
   int64_t rows, xStride;
   int D, F, activation, splits;
   bool wholeX, wholeD, wholeF;   // rows of x, of D and of F values are 16-byte pieces
 };
-constexpr int kProductThreads = 256, kProductSteps = 16;
+constexpr int kProductThreads = 256, kProductSteps = 16, kProductRun = 1024 / kProductSteps;
 
 // The first `count` of four values.
 __device__ __forceinline__ float4 fetchFour(const float *p, int64_t count, bool whole) {
@@ -583,8 +585,7 @@ template <Pass PASS, int T> __global__ void __launch_bounds__(kProductThreads, 2
   const int halfSteps = (p.F + K - 1) / K;   // input: steps of the first product, then those of the second
   const int64_t allSteps = PASS == Pass::forward ? (p.D + K - 1) / K : PASS == Pass::input ? 2 * halfSteps : (p.rows + K - 1) / K;
   const int64_t each = (allSteps + p.splits - 1) / p.splits;
-  const int64_t first = PASS == Pass::weights ? blockIdx.z * each : 0;
-  const int64_t last = PASS == Pass::weights ? min(allSteps, first + each) : allSteps;
+  const int64_t first = blockIdx.z * each, last = min(allSteps, first + each);
 
   auto fetchA = [&](int64_t step, int i) {
     const int at = tid + i * kProductThreads;
@@ -637,50 +638,76 @@ template <Pass PASS, int T> __global__ void __launch_bounds__(kProductThreads, 2
     for (int i = 0; i < kLoads; ++i) put(as[0], kAlongA, i, fetchA(first, i)), put(bs[0], kAlongB, i, fetchB(first, i));
   }
   __syncthreads();
-  for (int64_t step = first; step < last; ++step) {
-    const int now = int(step - first) & 1;
-    if (step + 1 < last) {
+  // What the tile's sums go to.
+  auto store = [&](bool add) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) a[i] = fetchA(step + 1, i), b[i] = fetchB(step + 1, i);
-    }
+    for (int i = 0; i < R; ++i) {
+      const int64_t m = m0 + (i / 4) * 64 + ty * 4 + i % 4;
+      if (m >= (PASS == Pass::weights ? int64_t(p.F) : p.rows)) continue;
+      float *to = PASS == Pass::weights ? p.parts + ((int64_t(blockIdx.z) * 2 + half) * p.F + m) * p.D
+                  : p.splits > 1        ? p.parts + (blockIdx.z * p.rows + m) * p.D
+                                        : p.dx + m * p.D;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float rows[R];
-#pragma unroll
-      for (int i = 0; i < R; i += 4)
-        *reinterpret_cast<float4 *>(rows + i) = *reinterpret_cast<const float4 *>(&as[now][k][i * 16 + ty * 4]);
-      Two columns[H];
-      if constexpr (H == 4) {
-        *reinterpret_cast<ulonglong2 *>(columns) = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][tx * 4]);
-        *reinterpret_cast<ulonglong2 *>(columns + 2) = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][T / 2 + tx * 4]);
-      } else {
-        columns[0] = *reinterpret_cast<const Two *>(&bs[now][k][tx * 2]);
-        columns[1] = *reinterpret_cast<const Two *>(&bs[now][k][T / 2 + tx * 2]);
+      for (int j = 0; j < R; ++j) {
+        const int n = n0 + (j / H) * (T / 2) + tx * H + j % H;
+        const float2 two = partsOf(sum[i][j / 2]);
+        const float v = j % 2 ? two.y : two.x;
+        if (n < p.D) to[n] = add ? to[n] + v : v;
       }
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const Two r = twoOf(rows[i], rows[i]);
+      for (int j = 0; j < H; ++j) sum[i][j] = 0;
+    }
+  };
+  int64_t run = first;
+  do {
+    const int64_t end = PASS == Pass::forward ? last : min(last, run + kProductRun);
+    for (int64_t step = run; step < end; ++step) {
+      const int now = int(step - first) & 1;
+      if (step + 1 < last) {
 #pragma unroll
-        for (int j = 0; j < H; ++j) addProduct(sum[i][j], r, columns[j]);
+        for (int i = 0; i < kLoads; ++i) a[i] = fetchA(step + 1, i), b[i] = fetchB(step + 1, i);
       }
-    }
-    if (step + 1 < last) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) put(as[now ^ 1], kAlongA, i, a[i]), put(bs[now ^ 1], kAlongB, i, b[i]);
-    }
-    __syncthreads();
-  }
+      for (int k = 0; k < K; ++k) {
+        float rows[R];
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int64_t m = m0 + (i / 4) * 64 + ty * 4 + i % 4;
-    if (m >= (PASS == Pass::weights ? int64_t(p.F) : p.rows)) continue;
-    float v[R];
+        for (int i = 0; i < R; i += 4)
+          *reinterpret_cast<float4 *>(rows + i) = *reinterpret_cast<const float4 *>(&as[now][k][i * 16 + ty * 4]);
+        Two columns[H];
+        if constexpr (H == 4) {
+          *reinterpret_cast<ulonglong2 *>(columns) = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][tx * 4]);
+          *reinterpret_cast<ulonglong2 *>(columns + 2) = *reinterpret_cast<const ulonglong2 *>(&bs[now][k][T / 2 + tx * 4]);
+        } else {
+          columns[0] = *reinterpret_cast<const Two *>(&bs[now][k][tx * 2]);
+          columns[1] = *reinterpret_cast<const Two *>(&bs[now][k][T / 2 + tx * 2]);
+        }
 #pragma unroll
-    for (int j = 0; j < H; ++j) {
-      const float2 two = partsOf(sum[i][j]);
-      v[2 * j] = two.x, v[2 * j + 1] = two.y;
+        for (int i = 0; i < R; ++i) {
+          const Two r = twoOf(rows[i], rows[i]);
+#pragma unroll
+          for (int j = 0; j < H; ++j) addProduct(sum[i][j], r, columns[j]);
+        }
+      }
+      if (step + 1 < last) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) put(as[now ^ 1], kAlongA, i, a[i]), put(bs[now ^ 1], kAlongB, i, b[i]);
+      }
+      __syncthreads();
     }
-    if constexpr (PASS == Pass::forward) {
+    if (PASS != Pass::forward) store(run > first);
+    run = end;
+  } while (run < last);
+  if constexpr (PASS == Pass::forward) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t m = m0 + (i / 4) * 64 + ty * 4 + i % 4;
+      if (m >= p.rows) continue;
+      float v[R];
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        const float2 two = partsOf(sum[i][j]);
+        v[2 * j] = two.x, v[2 * j + 1] = two.y;
+      }
       const int f = n0 + tx * H;
 #pragma unroll
       for (int j = 0; j < H; ++j) {
@@ -690,13 +717,6 @@ template <Pass PASS, int T> __global__ void __launch_bounds__(kProductThreads, 2
         const int64_t at = m * p.F + f + j;
         if (p.kept) p.kept[at] = gate, p.kept[plane + at] = up;
         withActivation(p.activation, [&](auto kind) { p.h[at] = activate<kind.value, false>(gate).y * up; });
-      }
-    } else {
-      float *to = PASS == Pass::input ? p.dx + m * p.D : p.parts + ((int64_t(blockIdx.z) * 2 + half) * p.F + m) * p.D;
-#pragma unroll
-      for (int j = 0; j < R; ++j) {
-        const int n = n0 + (j / H) * (T / 2) + tx * H + j % H;
-        if (n < p.D) to[n] = v[j];
       }
     }
   }
@@ -741,32 +761,32 @@ __global__ void __launch_bounds__(256) gatedGradients(GradientArgs p) {
 
 // -------------------------------------------------------------- sums of parts
 // out[i] = sum over n of parts[n, i], in float32, to the layer's type; the first
-// `count` values to one array, the next to another.  Bias sums likewise.
+// `cut` of the `count` values to one array, the others to another.  Bias sums likewise.
 template <class T> struct SumArgs {
   const float *parts, *biasParts;
-  T *dwGate, *dwUp, *dbGate, *dbUp;
-  int64_t weights;   // F * D
-  int F, splits, biasCount, weightBlocks;
+  T *first, *second, *dbGate, *dbUp;
+  int64_t cut, count;
+  int F, splits, biasCount, blocks;   // blocks for `parts`
 };
 constexpr int kSumThreads = 256, kSumColumns = 8;
 template <class T> __global__ void __launch_bounds__(kSumThreads) sumParts(SumArgs<T> p) {
-  if (int(blockIdx.x) < p.weightBlocks) {
+  if (int(blockIdx.x) < p.blocks) {
     const int64_t i = (int64_t(blockIdx.x) * kSumThreads + threadIdx.x) * 4;
-    if (i >= 2 * p.weights) return;
-    if (p.weights % 4 == 0) {
+    if (i >= p.count) return;
+    if (p.cut % 4 == 0 && p.count % 4 == 0) {
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
       for (int n = 0; n < p.splits; ++n) {
-        const float4 v = *reinterpret_cast<const float4 *>(p.parts + n * 2 * p.weights + i);
+        const float4 v = *reinterpret_cast<const float4 *>(p.parts + n * p.count + i);
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
       }
-      T *to = i < p.weights ? p.dwGate + i : p.dwUp + (i - p.weights);
+      T *to = i < p.cut ? p.first + i : p.second + (i - p.cut);
       to[0] = fromFloat<T>(sum.x), to[1] = fromFloat<T>(sum.y), to[2] = fromFloat<T>(sum.z), to[3] = fromFloat<T>(sum.w);
     } else {
-      for (int64_t j = i; j < i + 4 && j < 2 * p.weights; ++j) {
+      for (int64_t j = i; j < min(i + 4, p.count); ++j) {
         float sum = 0.f;
-        for (int n = 0; n < p.splits; ++n) sum += p.parts[n * 2 * p.weights + j];
-        (j < p.weights ? p.dwGate[j] : p.dwUp[j - p.weights]) = fromFloat<T>(sum);
+        for (int n = 0; n < p.splits; ++n) sum += p.parts[n * p.count + j];
+        (j < p.cut ? p.first[j] : p.second[j - p.cut]) = fromFloat<T>(sum);
       }
     }
     return;
@@ -775,7 +795,7 @@ template <class T> __global__ void __launch_bounds__(kSumThreads) sumParts(SumAr
   constexpr int kAtOnce = kSumThreads / kSumColumns;
   __shared__ float sums[kAtOnce][kSumColumns];
   const int own = threadIdx.x % kSumColumns, from = threadIdx.x / kSumColumns;
-  const int column = (int(blockIdx.x) - p.weightBlocks) * kSumColumns + own;
+  const int column = (int(blockIdx.x) - p.blocks) * kSumColumns + own;
   float sum = 0.f;
   if (column < 2 * p.F) {
 #pragma unroll 8

@@ -151,9 +151,15 @@ struct GatedPlan {
   int weightColumns;         // of a tile of the weights' gradients
   int splits;                // of the rows, for the weights' gradients
   int weightTile;            // float32: rows and columns of a tile of them
+  int inputColumns, inputSplits;   // of a tile of the gradient of x (float32: rows too), and of F
   int64_t biasCount;
-  int64_t bothBytes, biasBytes, partBytes, keptBytes;
+  int64_t bothBytes, biasBytes, partBytes, inputBytes, keptBytes;   // in this order
 };
+// Where tiles leave multiprocessors idle, the steps of their products are split, so that each part has `least` at least.
+int splitsOf(int64_t tiles, int64_t fit, int64_t steps, int64_t least) {
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(fit / tiles, steps / least));
+  return int(std::max<int64_t>(1, ceilDiv(steps, ceilDiv(std::max<int64_t>(1, steps), splits))));   // none without steps
+}
 int64_t padded(int64_t bytes) { return ceilDiv(bytes, 256) * 256; }
 // Columns of a tile, of which a row of tiles has `columns`: rounds of tiles over the multiprocessors, times a tile's time.  A
 // product of 128 columns takes 0.77 of the time of one of 256: its operands' way out of shared memory bounds it (16384 x 4096
@@ -168,6 +174,11 @@ int tileColumns(int64_t rowTiles, int64_t columns) {
   }
   return best;
 }
+// float32 products in tiles of 128 by 128, or of 64 by 64 where those are less than the multiprocessors or half empty (4999
+// rows, 61 x 301: the gradient of x 85 us in 40 tiles of 128, 35 in 79 of 64).
+int productTile(int64_t rows, int64_t columns) {
+  return columns <= 64 || ceilDiv(rows, 128) * ceilDiv(columns, 128) < 148 ? 64 : 128;
+}
 GatedPlan planGated(const duck_gated &a) {
   GatedPlan p{};
   const bool weights = a.dw_gate != nullptr, biases = a.db_gate != nullptr;
@@ -179,20 +190,23 @@ GatedPlan planGated(const duck_gated &a) {
     // Rows are split so that the tiles fill the GPU once, into parts of 512 rows at least: a part's sums are written and read
     // once more (24576 rows, 256 x 512: 17 us in 18 parts of 256 columns, 20 in 9 of 128).
     p.weightColumns = a.D > 128 ? 256 : a.D > 64 ? 128 : 64;
-    const int64_t tiles = 2 * ceilDiv(a.F, kTileRows) * ceilDiv(a.D, p.weightColumns), steps = ceilDiv(rows, kTileSteps);
-    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(148 / tiles, steps / 8)));
-    p.splits = int(std::max<int64_t>(1, ceilDiv(steps, std::max<int64_t>(1, ceilDiv(steps, p.splits)))));
+    p.splits = splitsOf(2 * ceilDiv(a.F, kTileRows) * ceilDiv(a.D, p.weightColumns), 148, ceilDiv(rows, kTileSteps), 8);
+    // x's gradient of few rows (66 rows, 136 x 3788: three tiles of 120 steps each otherwise).
+    const int64_t rowTiles = ceilDiv(rows, kTileRows);
+    p.inputColumns = tileColumns(rowTiles, a.D);
+    p.inputSplits = splitsOf(rowTiles * ceilDiv(a.D, p.inputColumns), 148, 2 * ceilDiv(a.F, kTileSteps), 8);
   } else {
     p.bothBytes = padded(rows * 2 * a.F * 4);
     p.keptBytes = rows * 2 * a.F * 4;
     p.biasCount = ceilDiv(rows, kGradientRows);
     p.weightTile = a.D <= 64 ? 64 : 128;
-    const int64_t tiles = 2 * ceilDiv(a.F, p.weightTile) * ceilDiv(a.D, p.weightTile), steps = ceilDiv(rows, kProductSteps);
-    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(2 * 148 / tiles, steps / 16)));
-    p.splits = int(std::max<int64_t>(1, ceilDiv(steps, std::max<int64_t>(1, ceilDiv(steps, p.splits)))));
+    p.splits = splitsOf(2 * ceilDiv(a.F, p.weightTile) * ceilDiv(a.D, p.weightTile), 2 * 148, ceilDiv(rows, kProductSteps), 16);
+    p.inputColumns = productTile(rows, a.D);
+    p.inputSplits = splitsOf(ceilDiv(rows, p.inputColumns) * ceilDiv(a.D, p.inputColumns), 2 * 148, 2 * ceilDiv(a.F, kProductSteps), 16);
   }
   if (biases) p.biasBytes = padded(p.biasCount * 2 * a.F * 4);
   if (weights && (a.type == DUCK_FLOAT32 || p.splits > 1)) p.partBytes = padded(int64_t(p.splits) * 2 * a.F * a.D * 4);
+  if (a.dx && p.inputSplits > 1) p.inputBytes = padded(p.inputSplits * rows * a.D * 4);
   return p;
 }
 
@@ -295,8 +309,6 @@ ProductArgs productArgs(const duck_gated &a) {
   g.wholeF = a.F % 4 == 0;
   return g;
 }
-// float32 products in tiles of 128 by 128, or of 64 by 64 where those are less than the multiprocessors or half empty (4999
-// rows, 61 x 301: the gradient of x 85 us in 40 tiles of 128, 35 in 79 of 64).
 template <Pass PASS> void launchProducts(const ProductArgs &g, int tile, int64_t rows, int64_t columns, int splits, cudaStream_t stream) {
   const int64_t rowTiles = (PASS == Pass::weights ? 2 : 1) * ceilDiv(rows, tile);
   const dim3 grid(unsigned(rowTiles), unsigned(ceilDiv(columns, tile)), unsigned(splits));
@@ -304,19 +316,25 @@ template <Pass PASS> void launchProducts(const ProductArgs &g, int tile, int64_t
   else gatedProducts<PASS, 64><<<grid, kProductThreads, 0, stream>>>(g);
   check(cudaGetLastError(), "gated linear launch");
 }
-int productTile(int64_t rows, int64_t columns) {
-  return columns <= 64 || ceilDiv(rows, 128) * ceilDiv(columns, 128) < 148 ? 64 : 128;
-}
-
+// Sums of parts to one or two arrays, and of the biases' parts.
 template <class T>
-void launchSums(const duck_gated &a, const GatedPlan &plan, const float *parts, const float *biasParts, cudaStream_t stream) {
-  SumArgs<T> s{parts, biasParts, static_cast<T *>(a.dw_gate), static_cast<T *>(a.dw_up), static_cast<T *>(a.db_gate),
-               static_cast<T *>(a.db_up), int64_t(a.F) * a.D, a.F, plan.splits, int(plan.biasCount), 0};
-  if (parts) s.weightBlocks = int(ceilDiv(2 * s.weights, kSumThreads * 4));
-  const int64_t blocks = s.weightBlocks + (biasParts ? ceilDiv(2 * int64_t(a.F), kSumColumns) : 0);
-  if (blocks == 0) return;
-  sumParts<T><<<unsigned(blocks), kSumThreads, 0, stream>>>(s);
+void launchSums(const duck_gated &a, const float *parts, int splits, void *first, int64_t cut, void *second, int64_t count,
+                const float *biasParts, int64_t biasCount, cudaStream_t stream) {
+  SumArgs<T> s{parts, biasParts, static_cast<T *>(first), static_cast<T *>(second), static_cast<T *>(a.db_gate),
+               static_cast<T *>(a.db_up), cut, count, a.F, splits, int(biasCount), 0};
+  const int64_t some = parts ? ceilDiv(count, kSumThreads * 4) : 0, all = some + (biasParts ? ceilDiv(2 * int64_t(a.F), kSumColumns) : 0);
+  if (all == 0) return;
+  require(all < (int64_t(1) << 31), "Too many rows and columns");
+  s.blocks = int(some);
+  sumParts<T><<<unsigned(all), kSumThreads, 0, stream>>>(s);
   check(cudaGetLastError(), "gated linear sums launch");
+}
+template <class T>
+void launchSums(const duck_gated &a, const GatedPlan &plan, const float *parts, const float *biasParts, const float *inputParts,
+                cudaStream_t stream) {
+  const int64_t weights = int64_t(a.F) * a.D, input = a.rows * a.D;
+  launchSums<T>(a, parts, plan.splits, a.dw_gate, weights, a.dw_up, 2 * weights, biasParts, plan.biasCount, stream);
+  if (inputParts) launchSums<T>(a, inputParts, plan.inputSplits, a.dx, input, nullptr, input, nullptr, 0, stream);
 }
 
 void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t stream) {
@@ -326,6 +344,7 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
   t.stride = plan.stride;
   float *biasParts = a.db_gate ? reinterpret_cast<float *>(scratch + plan.bothBytes) : nullptr;
   float *parts = plan.partBytes ? reinterpret_cast<float *>(scratch + plan.bothBytes + plan.biasBytes) : nullptr;
+  float *inputParts = plan.inputBytes ? reinterpret_cast<float *>(scratch + plan.bothBytes + plan.biasBytes + plan.partBytes) : nullptr;
   t.dh = static_cast<const bf16 *>(a.dh);
   t.dhStride = a.dh_stride;
   t.wholeDh = reinterpret_cast<uintptr_t>(a.dh) % 16 == 0 && a.dh_stride % 8 == 0 && a.dh_stride >= a.F;
@@ -335,15 +354,19 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
   if (a.dx) {
     t.dx = static_cast<bf16 *>(a.dx);
     t.steps = int(ceilDiv(a.F, kTileSteps));
-    withColumns(tileColumns(rowTiles, a.D), [&](auto n) {
+    t.rowTiles = int(rowTiles);
+    t.splits = plan.inputSplits;
+    t.parts = inputParts;
+    withColumns(plan.inputColumns, [&](auto n) {
       TileMaps maps{};
       maps.a0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
       maps.a1 = mapOf(t.both + plan.stride, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
       maps.b0 = mapOf(a.w_gate, a.D, a.F, a.D, 64);
       maps.b1 = mapOf(a.w_up, a.D, a.F, a.D, 64);
       t.columnTiles = int(ceilDiv(a.D, n.value));
-      require(rowTiles * t.columnTiles < (int64_t(1) << 31), "Too many rows and columns");
-      t.tiles = int(rowTiles * t.columnTiles);
+      const int64_t tiles = rowTiles * t.columnTiles * t.splits;
+      require(tiles < (int64_t(1) << 31), "Too many rows and columns");
+      t.tiles = int(tiles);
       launchTiles<Pass::input, n.value>(maps, t, stream);
     });
   }
@@ -366,7 +389,7 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
       launchTiles<Pass::weights, n.value>(maps, t, stream);
     });
   }
-  launchSums<bf16>(a, plan, a.dw_gate ? parts : nullptr, biasParts, stream);
+  launchSums<bf16>(a, plan, parts, biasParts, inputParts, stream);
 }
 
 void gatedBackward32(const duck_gated &a, const GatedPlan &plan, cudaStream_t stream) {
@@ -375,6 +398,7 @@ void gatedBackward32(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
   float *both = reinterpret_cast<float *>(scratch);
   float *biasParts = a.db_gate ? reinterpret_cast<float *>(scratch + plan.bothBytes) : nullptr;
   float *parts = a.dw_gate ? reinterpret_cast<float *>(scratch + plan.bothBytes + plan.biasBytes) : nullptr;
+  float *inputParts = plan.inputBytes ? reinterpret_cast<float *>(scratch + plan.bothBytes + plan.biasBytes + plan.partBytes) : nullptr;
   const int64_t rowBlocks = ceilDiv(a.rows, kGradientRows);
   const GradientArgs e{static_cast<const float *>(a.kept), static_cast<const float *>(a.dh), both, biasParts, a.rows, a.dh_stride,
                        a.F, a.activation};
@@ -383,14 +407,16 @@ void gatedBackward32(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
   g.both = both;
   if (a.dx) {
     g.dx = static_cast<float *>(a.dx);
-    launchProducts<Pass::input>(g, productTile(a.rows, a.D), a.rows, a.D, 1, stream);
+    g.parts = inputParts;
+    g.splits = plan.inputSplits;
+    launchProducts<Pass::input>(g, plan.inputColumns, a.rows, a.D, plan.inputSplits, stream);
   }
   if (a.dw_gate) {
     g.parts = parts;
     g.splits = plan.splits;
     launchProducts<Pass::weights>(g, plan.weightTile, a.F, a.D, plan.splits, stream);
   }
-  launchSums<float>(a, plan, parts, biasParts, stream);
+  launchSums<float>(a, plan, parts, biasParts, inputParts, stream);
 }
 
 }  // namespace
@@ -403,7 +429,7 @@ int duck_gated_linear_sizes(const duck_gated *args, int64_t *out) {
     out[0] = out[1] = 0;
     if (!gatedChecked(args)) return;
     const GatedPlan plan = planGated(*args);
-    out[0] = plan.bothBytes + plan.biasBytes + plan.partBytes;
+    out[0] = plan.bothBytes + plan.biasBytes + plan.partBytes + plan.inputBytes;
     out[1] = plan.keptBytes;
   });
 }

@@ -530,11 +530,12 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
 
 
 @functools.lru_cache(maxsize=1024)
-def _gated_workspace(rows, D, F, kind, weights, biases):
+def _gated_workspace(rows, D, F, kind, input, weights, biases):
     """Bytes of scratch of a backward call with or without those gradients, and of
     what a forward call keeps for it."""
     out = (ctypes.c_int64 * 2)()
     pointers = [0] * 14
+    pointers[7] = int(input)
     pointers[8] = pointers[9] = int(weights)
     pointers[10] = pointers[11] = int(biases)
     _raise(library().duck_gated_linear_sizes(_GATED.pack(*pointers, rows, 0, 0, D, F, 0, kind), out))
@@ -546,8 +547,10 @@ def _gated_operand(t, strided):
     rows), for bfloat16 of whole 16-byte pieces on their boundaries, and apart."""
     t = _rows_of(t) if strided else t.contiguous()
     if t.dtype is torch.bfloat16:
-        stride = t.stride(0)
-        if t.data_ptr() % 16 or stride % 8 or stride < t.shape[1]:
+        n, stride = t.shape[1], t.stride(0)
+        if n % 8:
+            t = F.pad(t, (0, -n % 8))
+        elif t.data_ptr() % 16 or stride % 8 or stride < n:
             t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -557,7 +560,7 @@ def _gated_forward(x, w_gate, w_up, b_gate, b_up, activation, keep):
     F_ = w_gate.shape[0]
     kind = _TYPES[x.dtype]
     h = torch.empty((rows, F_), dtype=x.dtype, device=x.device)
-    kept = _buffer(_gated_workspace(rows, D, F_, kind, False, False)[1], x.device) if keep and kind == 0 else None
+    kept = _buffer(_gated_workspace(rows, D, F_, kind, False, False, False)[1], x.device) if keep and kind == 0 else None
     _launch(library().duck_gated_linear_forward, x.device,
             _GATED.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate), _address(b_up), h.data_ptr(),
                         0, 0, 0, 0, 0, 0, _address(kept), 0, rows, x.stride(0), 0, D, F_, activation, kind))
@@ -584,16 +587,18 @@ class _GatedLinear(torch.autograd.Function):
         F_ = w_gate.shape[0]
         kind = _TYPES[x.dtype]
         dh = _rows_of(dh)
-        empty = functools.partial(torch.empty, dtype=x.dtype, device=x.device)
+        empty, n = functools.partial(torch.empty, dtype=x.dtype, device=x.device), ctx.shape[-1]
         dx = empty((rows, D)) if needs[0] else None
         dw = (empty((F_, D)), empty((F_, D))) if weights else (None, None)
         db = (empty(F_), empty(F_)) if biases else (None, None)
-        scratch = _buffer(_gated_workspace(rows, D, F_, kind, weights, biases)[0], x.device)
+        scratch = _buffer(_gated_workspace(rows, D, F_, kind, needs[0], weights, biases)[0], x.device)
         _launch(library().duck_gated_linear_backward, x.device,
                 _GATED.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate), _address(b_up), 0,
                             dh.data_ptr(), _address(dx), _address(dw[0]), _address(dw[1]), _address(db[0]), _address(db[1]),
                             _address(kept), _address(scratch), rows, x.stride(0), dh.stride(0), D, F_, ctx.activation, kind))
-        return dx if dx is None or len(ctx.shape) == 2 else dx.view(ctx.shape), *dw, *db, None
+        if n != D:   # rows were padded
+            dx, *dw = (None if t is None else t[:, :n] for t in (dx, *dw))
+        return dx if dx is None or len(ctx.shape) == 2 else dx.reshape(ctx.shape), *dw, *db, None
 
 
 @torch.autocast("cpu", enabled=False)
@@ -629,9 +634,6 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     if not x.is_cuda:
         return _gated_plain(x, w_gate, w_up, b_gate, b_up, activation)
     _check_type(x, "gated_linear")
-    odd = -x.shape[-1] % 8
-    if odd and x.dtype == torch.bfloat16:   # rows of whole 16-byte pieces
-        x, w_gate, w_up = (F.pad(t, (0, odd)) for t in (x, w_gate, w_up))
     if b_gate is not None:
         b_gate, b_up = b_gate.contiguous(), b_up.contiguous()
     if _grad_needed(x, w_gate, w_up, b_gate, b_up):

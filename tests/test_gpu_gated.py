@@ -318,7 +318,7 @@ def check_layer(case, activation, devices=None, dh=None):
 
 
 # Tiles of 128 rows, 64 steps, 32 to 128 features; widths off every boundary; rows that are split for the weights.
-LAYERS = [(1, 1, 1), (1, 64, 64), (2, 8, 5), (16, 256, 512), (127, 61, 33), (128, 64, 128), (129, 72, 130), (300, 61, 301),
+LAYERS = [(1, 1, 1), (1, 64, 64), (2, 8, 5), (3, 16, 8), (40, 8, 24), (16, 256, 512), (127, 61, 33), (128, 64, 128), (129, 72, 130), (300, 61, 301),
           (513, 200, 96), (2000, 96, 264), (2501, 130, 40), (4096, 256, 512), (19000, 128, 128), (1025, 520, 1030), (64, 1024, 2048)]
 
 
