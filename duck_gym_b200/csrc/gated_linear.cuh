@@ -88,7 +88,7 @@ struct TileArgs {
   int64_t rows, dhStride;
   int D, F, stride, activation;
   int tiles, columnTiles, rowTiles, splits, steps;   // steps of 64 of a tile's product
-  bool wholeH, wholeDh, wholeBias;   // rows of 16-byte pieces: h and dh move by the TMA
+  bool wholeH, wholeDh, wholeBias, wholeD;   // rows of 16-byte pieces: h and dh move by the TMA
 };
 struct TileMaps {
   CUtensorMap a0, a1, b0, b1;   // operands
@@ -510,12 +510,12 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
           tensorLoaded(x);
           if (p.splits == 1) {
             bf16 *to = PASS == Pass::input ? p.dx : at.half ? p.dwUp : p.dwGate;
-            storeRows(stage, eightOf(x), eightOf(x + 8), to + row * p.D + column, p.D, rowsLeft, columns, true, lane);
+            storeRows(stage, eightOf(x), eightOf(x + 8), to + row * p.D + column, p.D, rowsLeft, columns, p.wholeD, lane);
           } else {
             const int64_t before = PASS == Pass::input ? at.split * p.rows : (int64_t(at.split) * 2 + at.half) * p.F;
             float *to = p.parts + (before + row) * p.D + column;
-            storeRows(stage, fourOf(x), fourOf(x + 4), to, p.D, rowsLeft, columns, true, lane);
-            if (columns > 8) storeRows(stage, fourOf(x + 8), fourOf(x + 12), to + 8, p.D, rowsLeft, columns - 8, true, lane);
+            storeRows(stage, fourOf(x), fourOf(x + 4), to, p.D, rowsLeft, columns, p.wholeD, lane);
+            if (columns > 8) storeRows(stage, fourOf(x + 8), fourOf(x + 12), to + 8, p.D, rowsLeft, columns - 8, p.wholeD, lane);
           }
         }
         tensorFenceBefore();
@@ -528,6 +528,35 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
   __syncthreads();
   tensorFenceAfter();
   if (warp == 2) tensorFree(accumulators, 2 * BN);
+}
+
+// Rows of x, of Wg and of Wu, one after the other, as rows of whole 16-byte pieces: the
+// TMA takes no others.
+struct PadArgs {
+  const bf16 *x, *wGate, *wUp;
+  bf16 *to;            // [rows + 2 F, stride]
+  int64_t rows, xStride;
+  int D, F, stride;
+};
+constexpr int kPadThreads = 256;
+__global__ void __launch_bounds__(kPadThreads) padRows(PadArgs p) {
+  const int pieces = p.stride / 8;
+  const int64_t all = (p.rows + 2 * int64_t(p.F)) * pieces;
+  for (int64_t i = int64_t(blockIdx.x) * kPadThreads + threadIdx.x; i < all; i += int64_t(gridDim.x) * kPadThreads) {
+    const int64_t row = i / pieces, weight = row - p.rows;
+    const int column = int(i - row * pieces) * 8;
+    const bf16 *from = weight < 0       ? p.x + row * p.xStride
+                       : weight < p.F ? p.wGate + weight * p.D
+                                      : p.wUp + (weight - p.F) * p.D;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const uint32_t low = column + j < p.D ? __bfloat16_as_ushort(from[column + j]) : 0u;
+      const uint32_t high = column + j + 1 < p.D ? __bfloat16_as_ushort(from[column + j + 1]) : 0u;
+      w[j / 2] = high << 16 | low;
+    }
+    *reinterpret_cast<uint4 *>(p.to + row * p.stride + column) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // -------------------------------------------------------------------- float32

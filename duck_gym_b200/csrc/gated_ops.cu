@@ -140,11 +140,12 @@ bool gatedChecked(const duck_gated *a) {
   require(a->rows >= 0 && a->D > 0 && a->F > 0, "Invalid layer sizes");
   require(a->rows < (int64_t(1) << 31) - 4096 && a->D <= (1 << 20) && a->F <= (1 << 20), "Too many rows or columns");
   require(a->activation >= DUCK_SILU && a->activation <= DUCK_SIGMOID, "Invalid activation");
-  require(a->type == DUCK_FLOAT32 || a->D % 8 == 0, "bfloat16 rows have to be whole 16-byte pieces");
-  require(a->type == DUCK_FLOAT32 || a->rows <= 1 || a->x == nullptr || a->x_stride >= a->D, "bfloat16 rows must not overlap");
+  require(a->type == DUCK_FLOAT32 || a->D % 8 || a->rows <= 1 || a->x == nullptr || a->x_stride >= a->D,
+          "bfloat16 rows must not overlap");
   return a->rows > 0;
 }
 
+int64_t wholeColumns(int64_t D) { return ceilDiv(D, 8) * 8; }
 // How a backward call's workspace is laid out.
 struct GatedPlan {
   int stride;                // bfloat16: of da and du
@@ -185,6 +186,7 @@ GatedPlan planGated(const duck_gated &a) {
   const int64_t rows = a.rows;
   if (a.type == DUCK_BFLOAT16) {
     p.stride = int(ceilDiv(a.F, 8) * 8);
+    if (a.D % 8) p.keptBytes = (rows + 2 * int64_t(a.F)) * wholeColumns(a.D) * 2;
     p.bothBytes = padded(rows * 2 * p.stride * 2);
     p.biasCount = ceilDiv(rows, kTileRows) * 4;
     // Rows are split so that the tiles fill the GPU once, into parts of 512 rows at least: a part's sums are written and read
@@ -262,7 +264,7 @@ template <class F> void withColumns(int columns, F &&f) {
 }
 
 // Both projections, side by side.
-template <Pass PASS> void launchProjections(const duck_gated &a, TileArgs t, cudaStream_t stream) {
+template <Pass PASS> void launchProjections(const duck_gated &a, TileArgs t, cudaStream_t stream) {   // a: operandsOf()
   const int64_t rowTiles = ceilDiv(a.rows, kTileRows);
   auto run = [&](auto columns) {
     constexpr int BN = columns.value;
@@ -292,9 +294,20 @@ TileArgs tileArgs(const duck_gated &a) {
   t.bGate = static_cast<const bf16 *>(a.b_gate);
   t.bUp = static_cast<const bf16 *>(a.b_up);
   t.rows = a.rows, t.D = a.D, t.F = a.F, t.activation = a.activation;
+  t.wholeD = a.D % 8 == 0;
   t.wholeBias = reinterpret_cast<uintptr_t>(a.b_gate) % 16 == 0 && reinterpret_cast<uintptr_t>(a.b_up) % 16 == 0;
   t.splits = 1;
   return t;
+}
+// The operands that the tiles read, with D for their rows: the call's own, or the copies that a forward call has padded.
+duck_gated operandsOf(const duck_gated &a) {
+  duck_gated o = a;
+  if (a.D % 8 == 0) return o;
+  const int64_t stride = wholeColumns(a.D);
+  const bf16 *kept = static_cast<const bf16 *>(a.kept);
+  o.x = kept, o.x_stride = stride, o.D = int(stride);
+  o.w_gate = kept + a.rows * stride, o.w_up = kept + (a.rows + a.F) * stride;
+  return o;
 }
 ProductArgs productArgs(const duck_gated &a) {
   ProductArgs g{};
@@ -349,7 +362,8 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
   t.dhStride = a.dh_stride;
   t.wholeDh = reinterpret_cast<uintptr_t>(a.dh) % 16 == 0 && a.dh_stride % 8 == 0 && a.dh_stride >= a.F;
   t.biasParts = biasParts;
-  launchProjections<Pass::gradients>(a, t, stream);
+  const duck_gated o = operandsOf(a);
+  launchProjections<Pass::gradients>(o, t, stream);
   const int64_t rowTiles = ceilDiv(a.rows, kTileRows);
   if (a.dx) {
     t.dx = static_cast<bf16 *>(a.dx);
@@ -361,8 +375,8 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
       TileMaps maps{};
       maps.a0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
       maps.a1 = mapOf(t.both + plan.stride, a.F, a.rows, 2 * int64_t(plan.stride), kTileRows);
-      maps.b0 = mapOf(a.w_gate, a.D, a.F, a.D, 64);
-      maps.b1 = mapOf(a.w_up, a.D, a.F, a.D, 64);
+      maps.b0 = mapOf(o.w_gate, o.D, a.F, o.D, 64);
+      maps.b1 = mapOf(o.w_up, o.D, a.F, o.D, 64);
       t.columnTiles = int(ceilDiv(a.D, n.value));
       const int64_t tiles = rowTiles * t.columnTiles * t.splits;
       require(tiles < (int64_t(1) << 31), "Too many rows and columns");
@@ -381,7 +395,7 @@ void gatedBackward16(const duck_gated &a, const GatedPlan &plan, cudaStream_t st
       TileMaps maps{};
       maps.a0 = mapOf(t.both, a.F, a.rows, 2 * int64_t(plan.stride), 64);
       maps.a1 = mapOf(t.both + plan.stride, a.F, a.rows, 2 * int64_t(plan.stride), 64);
-      maps.b0 = mapOf(a.x, a.D, a.rows, a.rows > 1 ? a.x_stride : a.D, 64);
+      maps.b0 = mapOf(o.x, o.D, a.rows, a.rows > 1 ? o.x_stride : o.D, 64);
       t.columnTiles = int(ceilDiv(a.D, n.value));
       const int64_t tiles = int64_t(t.columnTiles) * 2 * t.rowTiles * t.splits;
       require(tiles < (int64_t(1) << 31), "Too many rows and columns");
@@ -445,7 +459,16 @@ int duck_gated_linear_forward(const duck_gated *args, duck_stream stream) {
       TileArgs t = tileArgs(a);
       t.h = static_cast<bf16 *>(a.h);
       t.wholeH = a.F % 8 == 0;
-      return launchProjections<Pass::forward>(a, t, s);
+      const duck_gated o = operandsOf(a);
+      if (a.D % 8) {
+        require(a.kept, "Invalid arguments");
+        const PadArgs p{static_cast<const bf16 *>(a.x), static_cast<const bf16 *>(a.w_gate), static_cast<const bf16 *>(a.w_up),
+                        static_cast<bf16 *>(a.kept), a.rows, a.x_stride, a.D, a.F, o.D};
+        const int64_t blocks = ceilDiv((a.rows + 2 * int64_t(a.F)) * (o.D / 8), kPadThreads);
+        padRows<<<unsigned(std::min<int64_t>(blocks, 148 * 8)), kPadThreads, 0, s>>>(p);
+        check(cudaGetLastError(), "gated linear launch");
+      }
+      return launchProjections<Pass::forward>(o, t, s);
     }
     ProductArgs g = productArgs(a);
     g.h = static_cast<float *>(a.h);
@@ -469,7 +492,7 @@ int duck_gated_linear_backward(const duck_gated *args, duck_stream stream) {
       return;
     }
     if (!a.dx && !a.dw_gate && !a.db_gate) return;
-    require(a.x && a.w_gate && a.w_up && a.dh && a.scratch && (a.type == DUCK_BFLOAT16 || a.kept), "Invalid arguments");
+    require(a.x && a.w_gate && a.w_up && a.dh && a.scratch && (a.kept || (a.type == DUCK_BFLOAT16 && a.D % 8 == 0)), "Invalid arguments");
     requireAligned({a.dx, a.dw_gate, a.dw_up, a.kept, a.scratch});
     const GatedPlan plan = planGated(a);
     if (a.type == DUCK_BFLOAT16) gatedBackward16(a, plan, s);

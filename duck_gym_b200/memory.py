@@ -544,13 +544,12 @@ def _gated_workspace(rows, D, F, kind, input, weights, biases):
 
 def _gated_operand(t, strided):
     """Rows as the kernels take them: dense (`strided`: up to the distance of the
-    rows), for bfloat16 of whole 16-byte pieces on their boundaries, and apart."""
+    rows); bfloat16 ones of whole 16-byte pieces on their boundaries, and apart (others
+    are padded by the forward call)."""
     t = _rows_of(t) if strided else t.contiguous()
     if t.dtype is torch.bfloat16:
         n, stride = t.shape[1], t.stride(0)
-        if n % 8:
-            t = F.pad(t, (0, -n % 8))
-        elif t.data_ptr() % 16 or stride % 8 or stride < n:
+        if n % 8 == 0 and (t.data_ptr() % 16 or stride % 8 or stride < n):
             t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -560,7 +559,9 @@ def _gated_forward(x, w_gate, w_up, b_gate, b_up, activation, keep):
     F_ = w_gate.shape[0]
     kind = _TYPES[x.dtype]
     h = torch.empty((rows, F_), dtype=x.dtype, device=x.device)
-    kept = _buffer(_gated_workspace(rows, D, F_, kind, False, False, False)[1], x.device) if keep and kind == 0 else None
+    # float32: the projections, for a backward pass; bfloat16: padded operands, for a forward one too.
+    needed = keep if kind == 0 else D % 8
+    kept = _buffer(_gated_workspace(rows, D, F_, kind, False, False, False)[1], x.device) if needed else None
     _launch(library().duck_gated_linear_forward, x.device,
             _GATED.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate), _address(b_up), h.data_ptr(),
                         0, 0, 0, 0, 0, 0, _address(kept), 0, rows, x.stride(0), 0, D, F_, activation, kind))
@@ -587,7 +588,7 @@ class _GatedLinear(torch.autograd.Function):
         F_ = w_gate.shape[0]
         kind = _TYPES[x.dtype]
         dh = _rows_of(dh)
-        empty, n = functools.partial(torch.empty, dtype=x.dtype, device=x.device), ctx.shape[-1]
+        empty = functools.partial(torch.empty, dtype=x.dtype, device=x.device)
         dx = empty((rows, D)) if needs[0] else None
         dw = (empty((F_, D)), empty((F_, D))) if weights else (None, None)
         db = (empty(F_), empty(F_)) if biases else (None, None)
@@ -596,9 +597,7 @@ class _GatedLinear(torch.autograd.Function):
                 _GATED.pack(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate), _address(b_up), 0,
                             dh.data_ptr(), _address(dx), _address(dw[0]), _address(dw[1]), _address(db[0]), _address(db[1]),
                             _address(kept), _address(scratch), rows, x.stride(0), dh.stride(0), D, F_, ctx.activation, kind))
-        if n != D:   # rows were padded
-            dx, *dw = (None if t is None else t[:, :n] for t in (dx, *dw))
-        return dx if dx is None or len(ctx.shape) == 2 else dx.reshape(ctx.shape), *dw, *db, None
+        return dx if dx is None or len(ctx.shape) == 2 else dx.view(ctx.shape), *dw, *db, None
 
 
 @torch.autocast("cpu", enabled=False)

@@ -466,11 +466,12 @@ int duck_gated_recurrence_step(const duck_recurrence *args, duck_stream stream);
  *   h = act(x w_gate^T + b_gate) (x w_up^T + b_up),  weights [F, D], biases [F]
  * and its gradients.  rows < 2^31 - 4096, D and F up to 2^20.  Element types are
  * those of `type` throughout; h, the weights, their gradients and dx are dense,
- * rows of x and dh have the strides given.  For DUCK_BFLOAT16 the rows of x, the
- * weights and their gradients are whole 16-byte pieces on 16-byte boundaries (D a
- * multiple of 8), and rows of x do not overlap.  `kept` is what a forward call
- * leaves for the backward one (DUCK_FLOAT32 only, else NULL).  Outputs and
- * workspaces lie on 16-byte boundaries, and no output overlaps an input. */
+ * rows of x and dh have the strides given.  `kept` is what a
+ * forward call leaves for the backward one; for DUCK_BFLOAT16 it is empty where D is
+ * a multiple of 8 (rows of x and the weights then lie on 16-byte boundaries, and rows
+ * of x do not overlap), else a forward call needs it whether a backward one follows
+ * or not.  Outputs and workspaces lie on 16-byte boundaries, and no output overlaps
+ * an input. */
 enum { DUCK_SILU = 0, DUCK_GELU = 1, DUCK_SIGMOID = 2 };
 typedef struct duck_gated {
   const void *x, *w_gate, *w_up;
@@ -480,7 +481,7 @@ typedef struct duck_gated {
   void *dx;                        /* backward: [rows, D], or NULL */
   void *dw_gate, *dw_up;           /* backward: both, or NULL */
   void *db_gate, *db_up;           /* backward: both, or NULL */
-  void *kept;                      /* forward writes, backward reads: duck_gated_linear_sizes; or NULL */
+  void *kept;                      /* forward writes, backward reads: duck_gated_linear_sizes, which may be 0 */
   void *scratch;                   /* backward: duck_gated_linear_sizes */
   int64_t rows, x_stride, dh_stride;
   int32_t D, F, activation, type;

@@ -534,9 +534,11 @@ def test_linear_refusals_on_the_gpu():
                 scratch=p, rows=16, x_stride=16, dh_stride=24, D=16, F=24, activation=0, type=0)
     pack = lambda **change: memory._GATED.pack(*{**fine, **change}.values())
     for change in (dict(x=0), dict(w_gate=0), dict(h=0), dict(b_gate=p), dict(D=0), dict(F=-1), dict(rows=-1), dict(rows=1 << 31),
-                   dict(activation=3), dict(type=2), dict(type=1, D=12), dict(h=p + 4), dict(type=1, x=p + 2), dict(type=1, x_stride=15)):
+                   dict(activation=3), dict(type=2), dict(type=1, D=12, kept=0), dict(h=p + 4), dict(type=1, x=p + 2),
+                   dict(type=1, x_stride=15), dict(type=1, x_stride=20)):
         assert lib.duck_gated_linear_forward(pack(**change), None) != 0, change
-    for change in (dict(dh=0), dict(scratch=0), dict(kept=0), dict(dw_up=0), dict(db_gate=0), dict(dx=p + 4), dict(type=1, w_up=p + 2)):
+    for change in (dict(dh=0), dict(scratch=0), dict(kept=0), dict(dw_up=0), dict(db_gate=0), dict(dx=p + 4), dict(type=1, w_up=p + 2),
+                   dict(type=1, D=12, kept=0)):
         assert lib.duck_gated_linear_backward(pack(**change), None) != 0, change
     assert lib.duck_gated_linear_forward(None, None) != 0 and lib.duck_gated_linear_backward(None, None) != 0
     assert b"Invalid" in lib.duck_last_error()
