@@ -176,7 +176,7 @@ int tileColumns(int64_t rowTiles, int64_t columns) {
   return best;
 }
 // float32 products in tiles of 128 by 128, or of 64 by 64 where those are less than the multiprocessors or half empty (4999
-// rows, 61 x 301: the gradient of x 85 us in 40 tiles of 128, 35 in 79 of 64).
+// rows, 61 x 301: the gradient of x 85 us in 40 tiles of 128, 35 in 79 of 64, 21 with their steps split three ways).
 int productTile(int64_t rows, int64_t columns) {
   return columns <= 64 || ceilDiv(rows, 128) * ceilDiv(columns, 128) < 148 ? 64 : 128;
 }
@@ -201,10 +201,14 @@ GatedPlan planGated(const duck_gated &a) {
     p.bothBytes = padded(rows * 2 * a.F * 4);
     p.keptBytes = rows * 2 * a.F * 4;
     p.biasCount = ceilDiv(rows, kGradientRows);
-    p.weightTile = a.D <= 64 ? 64 : 128;
-    p.splits = splitsOf(2 * ceilDiv(a.F, p.weightTile) * ceilDiv(a.D, p.weightTile), 2 * 148, ceilDiv(rows, kProductSteps), 16);
+    // Parts of 128 rows at least, or of 128 features.
+    const int64_t large = 2 * ceilDiv(a.F, 128) * ceilDiv(a.D, 128) * std::max<int64_t>(1, rows / 128);
+    p.weightTile = a.D <= 64 || large < 148 ? 64 : 128;
+    p.splits = splitsOf(2 * ceilDiv(a.F, p.weightTile) * ceilDiv(a.D, p.weightTile), 2 * 148,
+                        ceilDiv(rows, productSteps(p.weightTile)), 128 / productSteps(p.weightTile));
     p.inputColumns = productTile(rows, a.D);
-    p.inputSplits = splitsOf(ceilDiv(rows, p.inputColumns) * ceilDiv(a.D, p.inputColumns), 2 * 148, 2 * ceilDiv(a.F, kProductSteps), 16);
+    p.inputSplits = splitsOf(ceilDiv(rows, p.inputColumns) * ceilDiv(a.D, p.inputColumns), 2 * 148,
+                             2 * ceilDiv(a.F, productSteps(p.inputColumns)), 128 / productSteps(p.inputColumns));
   }
   if (biases) p.biasBytes = padded(p.biasCount * 2 * a.F * 4);
   if (weights && (a.type == DUCK_FLOAT32 || p.splits > 1)) p.partBytes = padded(int64_t(p.splits) * 2 * a.F * a.D * 4);
