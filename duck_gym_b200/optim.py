@@ -77,8 +77,11 @@ def _devices(ts):
     return set(map(torch.Tensor.get_device, ts))
 
 
-def _dtypes(ts, get=operator.attrgetter("dtype")):
-    return set(map(get, ts))
+_dtype, _layout = operator.attrgetter("dtype"), operator.attrgetter("layout")
+
+
+def _dtypes(ts):
+    return set(map(_dtype, ts))
 
 
 def _dense(ts):
@@ -199,12 +202,13 @@ def _checked(params, grads, exp_avgs, exp_avg_sqs):
     _require(len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) > 0,
              "adamw_step: one gradient and two moments for each of one or more parameters")
     eight = not torch.is_tensor(exp_avgs[0])
-    _require(all(torch.is_tensor(t) != eight for t in exp_avgs) and all(torch.is_tensor(t) != eight for t in exp_avg_sqs),
-             "adamw_step: all moments have 32 bits, or all have 8")
-    kinds = [_TYPES.get(p.dtype) for p in params]
+    kinds = {*map(type, exp_avgs), *map(type, exp_avg_sqs)}
+    _require(all(issubclass(kind, torch.Tensor) != eight for kind in kinds), "adamw_step: all moments have 32 bits, or all have 8")
+    dtypes = list(map(_dtype, params))
+    kinds = list(map(_TYPES.get, dtypes))
     _require(None not in kinds and _dense(params), "adamw_step: parameters are dense float32 or bfloat16 tensors of one device")
-    _require(_alike(grads, params) and [g.dtype for g in grads] == [p.dtype for p in params]
-             and all(g.layout is torch.strided for g in grads), "adamw_step: a gradient has its parameter's shape, type and device")
+    _require(set(map(_layout, grads)) == {torch.strided} and _alike(grads, params) and list(map(_dtype, grads)) == dtypes,
+             "adamw_step: a gradient has its parameter's shape, type and device")
     if not _dense(grads):
         grads = [g.contiguous() for g in grads]
     numbers = _numbers(params)
