@@ -196,9 +196,8 @@ def _check_apart(written, read, what):
 
 
 def _checked(params, grads, exp_avgs, exp_avg_sqs):
-    """Whether the moments have 8 bits, the tensors' device, their table, and dense
-    gradients (which have to live until the launch)."""
-    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    """Whether the moments of these lists have 8 bits, the tensors' device, their table,
+    and dense gradients (which have to live until the launch)."""
     _require(len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) > 0,
              "adamw_step: one gradient and two moments for each of one or more parameters")
     eight = not torch.is_tensor(exp_avgs[0])
@@ -303,7 +302,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999
     bfloat16 parameters and codes are rounded up or down at random, by a hash of t, the
     tensor's place in the list and the value's place in the tensor: what a step adds is
     mostly less than half a place of theirs, and would be lost."""
-    eight, device, table, grads = _checked(params, grads, exp_avgs, exp_avg_sqs)
+    params, exp_avgs, exp_avg_sqs = list(params), list(exp_avgs), list(exp_avg_sqs)   # they may be iterators
+    eight, device, table, grads = _checked(params, list(grads), exp_avgs, exp_avg_sqs)
     _check_options(step, lr, betas, eps, weight_decay, max_norm, device)
     norm = None
     if max_norm is not None:
