@@ -280,6 +280,8 @@ def _check_options(step, lr, betas, eps, weight_decay, max_norm, device):
     if torch.is_tensor(lr):
         _require(lr.numel() == 1 and lr.is_floating_point() and lr.device in (device, torch.device("cpu")),
                  "adamw_step: the learning rate is a number, or a floating tensor of one value")
+    else:
+        _require(math.isfinite(lr), "adamw_step: the learning rate is not finite")
     _require(len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas) and (eps == 0.0 or 2.0 ** -126 <= eps < 2.0 ** 127)
              and 0.0 <= weight_decay < math.inf,
              "adamw_step: betas in [0, 1), eps 0 or a normal float32 number, weight decay of 0 or more")

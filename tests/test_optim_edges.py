@@ -25,3 +25,11 @@ def test_iterators_are_taken_as_lists_are(bits):
     assert int(a) == int(b) == 1 and not torch.equal(lists[0][0], torch.ones(5))
     flat = lambda x: [t for s in x for t in (flat(s) if isinstance(s, (list, tuple)) else [s])]
     assert all(torch.equal(x, y) for x, y in zip(flat(lists), flat(iterators)))
+
+
+@pytest.mark.parametrize("lr", [float("nan"), float("inf"), -float("inf")])
+def test_a_learning_rate_that_is_not_finite_is_refused(lr):
+    p, step = torch.ones(4), count()
+    with pytest.raises(RuntimeError, match="finite"):
+        optim.adamw_step([p], [torch.ones(4)], [torch.zeros(4)], [torch.zeros(4)], step, lr)
+    assert torch.equal(p, torch.ones(4)) and int(step) == 0
