@@ -337,6 +337,18 @@ def state8_values(states):
     return [v if c.dim() == 1 else v.view(c.shape) for v, c in zip(values, codes)]
 
 
+def _check_loaded(group):
+    """A group of a state dict: one of AdamW below, or of torch's without what would be lost."""
+    if "bits" in group:
+        return
+    _require(group.keys() >= {"lr", "betas", "eps", "weight_decay", "amsgrad"},
+             "AdamW: the state dict is not one of this class, nor of torch's Adam or AdamW")
+    _require(not group["amsgrad"] and not group.get("maximize"), "AdamW: there is no amsgrad and no maximize")
+    _require(group["weight_decay"] == 0 or group.get("decoupled_weight_decay"),
+             "AdamW: the state dict's weight decay is, or may be, added to the gradient; decoupled_weight_decay=True in its "
+             "groups says that it is not")
+
+
 class AdamW(torch.optim.Optimizer):
     """``adamw_step`` as a torch optimizer.
 
@@ -401,8 +413,12 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """As torch's, but moments keep their types (torch would convert them to the
-        parameters').  One of torch's own Adam or AdamW is taken too: its moments have 32
-        bits, and its count of steps becomes the group's."""
+        parameters').  One of torch's own Adam or AdamW is taken too, unless it has maximize,
+        amsgrad or a weight decay that is added to the gradient (Adam's; an older dict does not
+        say whose it is), which raise: its moments have 32 bits, and its count of steps
+        becomes the group's."""
+        for group in state_dict["param_groups"]:
+            _check_loaded(group)
         super().load_state_dict(state_dict)
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         mine = [p for group in self.param_groups for p in group["params"]]

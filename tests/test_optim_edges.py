@@ -33,3 +33,41 @@ def test_a_learning_rate_that_is_not_finite_is_refused(lr):
     with pytest.raises(RuntimeError, match="finite"):
         optim.adamw_step([p], [torch.ones(4)], [torch.zeros(4)], [torch.zeros(4)], step, lr)
     assert torch.equal(p, torch.ones(4)) and int(step) == 0
+
+
+def trained(kind, **options):
+    p = torch.nn.Parameter(torch.ones(3))
+    opt = kind([p], **options)
+    for _ in range(3):
+        p.grad = torch.tensor([1.0, -0.5, 0.1])
+        opt.step()
+    return p, opt
+
+
+@pytest.mark.parametrize("kind,options", [
+    (torch.optim.Adam, dict(maximize=True)), (torch.optim.AdamW, dict(maximize=True)), (torch.optim.Adam, dict(amsgrad=True)),
+    (torch.optim.AdamW, dict(amsgrad=True)), (torch.optim.Adam, dict(weight_decay=0.1)), (torch.optim.RAdam, {}),
+    (torch.optim.SGD, dict(momentum=0.9)), (torch.optim.NAdam, {}), (torch.optim.Adamax, {})])
+def test_a_state_dict_that_cannot_be_gone_on_from_is_refused(kind, options):
+    p, opt = trained(kind, lr=1e-2, **options)
+    mine = optim.AdamW([p], lr=5.0)
+    with pytest.raises(RuntimeError, match="AdamW:"):
+        mine.load_state_dict(opt.state_dict())
+    assert not mine.state and mine.param_groups[0]["lr"] == 5.0   # as it was
+
+
+def test_weight_decay_of_torch_is_taken_where_it_is_decoupled():
+    results = []
+    for switch in (False, True):
+        p, opt = trained(torch.optim.AdamW, lr=1e-2, weight_decay=0.3)
+        if switch:
+            saved, opt = opt.state_dict(), optim.AdamW([p])
+            older = {**saved, "param_groups": [{k: v for k, v in saved["param_groups"][0].items() if k != "decoupled_weight_decay"}]}
+            with pytest.raises(RuntimeError, match="decoupled_weight_decay"):   # Adam's looks the same
+                opt.load_state_dict(older)
+            opt.load_state_dict(saved)
+        for _ in range(3):
+            opt.step()
+        results.append(p.detach())
+    # Three steps of some eight roundings of 2^-24, of a value and of steps of lr.
+    assert bool(((results[0] - results[1]).abs() <= 24 * 2.0 ** -24 * (1 + 1e-2)).all())
