@@ -415,17 +415,19 @@ class AdamW(torch.optim.Optimizer):
         """As torch's, but moments keep their types (torch would convert them to the
         parameters').  One of torch's own Adam or AdamW is taken too, unless it has maximize,
         amsgrad or a weight decay that is added to the gradient (Adam's; an older dict does not
-        say whose it is), which raise: its moments have 32 bits, and its count of steps
-        becomes the group's."""
+        say whose it is), which raise: its moments become float32 whatever they were
+        (bfloat16 parameters' are bfloat16), and its count of steps the group's."""
         for group in state_dict["param_groups"]:
             _check_loaded(group)
+        theirs = {i for group in state_dict["param_groups"] if "bits" not in group for i in group["params"]}
         super().load_state_dict(state_dict)
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         mine = [p for group in self.param_groups for p in group["params"]]
         for i, p in zip(saved, mine):
             for name, value in state_dict["state"].get(i, {}).items():
                 if torch.is_tensor(value):
-                    self.state[p][name] = value.to(p.device, copy=True).contiguous()
+                    dtype = torch.float32 if i in theirs and name != "step" else value.dtype
+                    self.state[p][name] = value.to(p.device, dtype, copy=True).contiguous()
         for group in self.param_groups:
             group.setdefault("bits", 32)
             counts = [int(self.state[p].pop("step")) for p in group["params"] if "step" in self.state[p]]

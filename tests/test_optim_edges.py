@@ -71,3 +71,27 @@ def test_weight_decay_of_torch_is_taken_where_it_is_decoupled():
         results.append(p.detach())
     # Three steps of some eight roundings of 2^-24, of a value and of steps of lr.
     assert bool(((results[0] - results[1]).abs() <= 24 * 2.0 ** -24 * (1 + 1e-2)).all())
+
+
+def test_moments_of_torch_in_bfloat16_become_float32():
+    p = torch.nn.Parameter(torch.ones(300, dtype=torch.bfloat16))
+    opt = torch.optim.AdamW([p], lr=1e-2, weight_decay=0.1)
+    grad = (torch.arange(300) / 100 - 1.5).bfloat16()
+    for _ in range(2):
+        p.grad = grad
+        opt.step()
+    saved = opt.state_dict()
+    m, v, before = (saved["state"][0][k].clone() for k in ("exp_avg", "exp_avg_sq", "step"))
+    was = p.detach().float()
+    mine = optim.AdamW([p])
+    mine.load_state_dict(saved)
+    mine.step()
+    state = mine.state[p]
+    assert m.dtype == torch.bfloat16 and state["exp_avg"].dtype == state["exp_avg_sq"].dtype == torch.float32
+    assert int(before) == 2 and int(mine.param_groups[0]["step"]) == 3
+    g, m, v = grad.double(), m.double(), v.double()
+    m, v = 0.9 * m + 0.1 * g, 0.999 * v + 0.001 * g * g
+    assert torch.allclose(state["exp_avg"].double(), m, rtol=1e-6, atol=1e-7) and torch.allclose(state["exp_avg_sq"].double(), v, rtol=1e-6)
+    want = was * (1 - 1e-3) - 1e-2 * m / (1 - 0.9 ** 3) / ((v / (1 - 0.999 ** 3)).sqrt() + 1e-8)
+    # Up or down by less than a place of bfloat16.
+    assert bool(((p.detach().double() - want).abs() <= 2.0 ** -7 * want.abs()).all())
