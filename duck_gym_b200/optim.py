@@ -167,7 +167,7 @@ def _plain_tensor(place, p, g, m, v, count, clip, beta1, beta2, ahead, widen, sh
         v.copy_(v32)
 
 
-def _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm, total):
+def _plain(params, grads, ms, vs, places, step, lr, betas, eps, weight_decay, max_norm, total):
     step += 1
     count, rate = int(step), float(lr)
     clip = None
@@ -176,7 +176,7 @@ def _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm, 
     scalars = (torch.tensor(x, dtype=torch.float64).float() for x in (
         rate / (1.0 - betas[0] ** count), (1.0 - betas[1] ** count) ** -0.5, 1.0 - rate * weight_decay))
     ahead, widen, shrink = scalars
-    for place, each in enumerate(zip(params, grads, ms, vs)):
+    for place, *each in zip(places, params, grads, ms, vs):
         _plain_tensor(place, *each, count, clip, *betas, ahead, widen, shrink, eps)
 
 
@@ -195,7 +195,7 @@ def _check_apart(written, read, what):
     _require(all(not k or ends[k - 1] <= a for k, a in zip(before, first)), f"{what}: a gradient overlaps what is written")
 
 
-def _checked(params, grads, exp_avgs, exp_avg_sqs):
+def _checked(params, grads, exp_avgs, exp_avg_sqs, places):
     """Whether the moments of these lists have 8 bits, the tensors' device, their table,
     and dense gradients (which have to live until the launch)."""
     _require(len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) > 0,
@@ -231,7 +231,7 @@ def _checked(params, grads, exp_avgs, exp_avg_sqs):
         groups = _group_counts(numbers)
         written += [(me, groups), (ve, groups)]
     _check_apart(written, (gat, bytes_), "adamw_step")
-    table = b"".join(map(_TENSOR.pack, at, gat, mat, vat, me, ve, numbers, kinds, itertools.count()))
+    table = b"".join(map(_TENSOR.pack, at, gat, mat, vat, me, ve, numbers, kinds, places))
     return eight, params[0].device, table, grads
 
 
@@ -257,10 +257,10 @@ class _Norm:
             self.count = 1
 
 
-def _step(params, grads, ms, vs, eight, device, table, step, lr, betas, eps, weight_decay, max_norm, norm):
+def _step(params, grads, ms, vs, places, eight, device, table, step, lr, betas, eps, weight_decay, max_norm, norm):
     if device.type != "cuda":
         with torch.no_grad():
-            return _plain(params, grads, ms, vs, step, lr, betas, eps, weight_decay, max_norm,
+            return _plain(params, grads, ms, vs, places, step, lr, betas, eps, weight_decay, max_norm,
                           None if norm is None else norm.sums)
     on_device = torch.is_tensor(lr) and lr.is_cuda
     if on_device and lr.dtype != torch.float32:
@@ -305,13 +305,14 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas=(0.9, 0.999
     tensor's place in the list and the value's place in the tensor: what a step adds is
     mostly less than half a place of theirs, and would be lost."""
     params, exp_avgs, exp_avg_sqs = list(params), list(exp_avgs), list(exp_avg_sqs)   # they may be iterators
-    eight, device, table, grads = _checked(params, list(grads), exp_avgs, exp_avg_sqs)
+    eight, device, table, grads = _checked(params, list(grads), exp_avgs, exp_avg_sqs, range(len(params)))
     _check_options(step, lr, betas, eps, weight_decay, max_norm, device)
     norm = None
     if max_norm is not None:
         norm = _Norm(device)
         norm.add(table, grads)
-    _step(params, grads, exp_avgs, exp_avg_sqs, eight, device, table, step, lr, betas, eps, weight_decay, max_norm, norm)
+    _step(params, grads, exp_avgs, exp_avg_sqs, range(len(params)), eight, device, table, step, lr, betas, eps, weight_decay,
+          max_norm, norm)
 
 
 def state8_values(states):
@@ -354,9 +355,11 @@ class AdamW(torch.optim.Optimizer):
 
     ``bits`` (32 or 8) of the moments; with ``max_grad_norm`` gradients are clipped by
     the norm of those of all groups, in the step itself (``.grad`` stays as it is).
-    ``lr`` may be a tensor on the device that a schedule writes to.  A group has one
-    count of steps; a parameter without a gradient is left as it is, as torch's is, but
-    its steps are counted."""
+    ``lr`` may be a tensor on the device that a schedule writes to.  A parameter without a
+    gradient is left as it is, and so is its count of steps, as torch's.  The group's
+    ``step`` counts for all parameters that have had a gradient in each of its steps; one
+    that came later, or was left out of one, has a ``step`` in its own state, and a launch
+    for those that share it."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits=32, max_grad_norm=None):
         if bits not in (8, 32):
@@ -366,9 +369,44 @@ class AdamW(torch.optim.Optimizer):
         self.max_grad_norm = max_grad_norm
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits))
 
-    def _moments(self, p, bits):
-        state = self.state[p]
-        if not state:
+    def _counts(self, group):
+        """The group's parameters with gradients: lists of those that have the same steps
+        behind them, each with that count, the parameters' states and their places."""
+        params = [p for p in group["params"] if p.grad is not None]
+        if not params:
+            return []
+        states = [self.state[p] for p in params]
+        if not all("exp_avg" in state for state in states):
+            count = torch.zeros((), dtype=torch.int64, device=params[0].device)
+            if any("exp_avg" in state and "step" not in state for state in map(self._known, group["params"])):
+                for state in states:
+                    if "exp_avg" not in state:
+                        state["step"] = count
+            else:
+                group["step"] = count
+        behind = {}
+        if len(params) < len(group["params"]):
+            going = {state.get("step", group["step"]).data_ptr() for state in states}
+            for p in group["params"]:
+                state = self._known(p)
+                if p.grad is None and "exp_avg" in state:
+                    count = state.get("step", group["step"])
+                    if count.data_ptr() in going:
+                        state["step"] = behind.setdefault(count.data_ptr(), count.clone())
+        if not any("step" in state for state in states):
+            return [(group["step"], params, states, range(len(params)))]
+        lists = {}
+        for place, (p, state) in enumerate(zip(params, states)):
+            count = state.get("step", group["step"])
+            for to, x in zip(lists.setdefault(count.data_ptr(), (count, [], [], []))[1:], (p, state, place)):
+                to.append(x)
+        return list(lists.values())
+
+    def _known(self, p):
+        return self.state[p] if p in self.state else {}
+
+    def _moments(self, p, state, bits):
+        if "exp_avg" not in state:
             if bits == 8:
                 m, v = state8_zeros(p, True), state8_zeros(p, False)
                 state.update(exp_avg=m.codes, exp_avg_exponents=m.exponents, exp_avg_sq=v.codes,
@@ -389,25 +427,21 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         work, norms = [], {}
         for group in self.param_groups:
-            params = [p for p in group["params"] if p.grad is not None]
-            if not params:
-                continue
-            if "step" not in group:
-                group["step"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
-            moments = [self._moments(p, group["bits"]) for p in params]
-            ms, vs = [m for m, _ in moments], [v for _, v in moments]
-            eight, device, table, grads = _checked(params, [p.grad for p in params], ms, vs)
-            _check_options(group["step"], group["lr"], group["betas"], group["eps"], group["weight_decay"],
-                           self.max_grad_norm, device)
-            if self.max_grad_norm is not None:
-                _require(not norms or device in norms, "AdamW: one device where gradients are clipped")
-                norms.setdefault(device, None)
-                norms[device] = norms[device] or _Norm(device)
-                norms[device].add(table, grads)
-            work.append((params, grads, ms, vs, eight, device, table, group))
-        for params, grads, ms, vs, eight, device, table, group in work:
-            _step(params, grads, ms, vs, eight, device, table, group["step"], group["lr"], group["betas"], group["eps"],
-                  group["weight_decay"], self.max_grad_norm, norms.get(device))
+            for count, params, states, places in self._counts(group):
+                moments = [self._moments(p, state, group["bits"]) for p, state in zip(params, states)]
+                ms, vs = [m for m, _ in moments], [v for _, v in moments]
+                eight, device, table, grads = _checked(params, [p.grad for p in params], ms, vs, places)
+                _check_options(count, group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                               self.max_grad_norm, device)
+                if self.max_grad_norm is not None:
+                    _require(not norms or device in norms, "AdamW: one device where gradients are clipped")
+                    norms.setdefault(device, None)
+                    norms[device] = norms[device] or _Norm(device)
+                    norms[device].add(table, grads)
+                work.append(((params, grads, ms, vs, places, eight, device, table, count), group))
+        for tensors, group in work:
+            _step(*tensors, group["lr"], group["betas"], group["eps"], group["weight_decay"], self.max_grad_norm,
+                  norms.get(tensors[0][0].device))
         return loss
 
     @torch.no_grad()
@@ -416,7 +450,8 @@ class AdamW(torch.optim.Optimizer):
         parameters').  One of torch's own Adam or AdamW is taken too, unless it has maximize,
         amsgrad or a weight decay that is added to the gradient (Adam's; an older dict does not
         say whose it is), which raise: its moments become float32 whatever they were
-        (bfloat16 parameters' are bfloat16), and its count of steps the group's."""
+        (bfloat16 parameters' are bfloat16), and the count that most parameters of a group
+        have the group's."""
         for group in state_dict["param_groups"]:
             _check_loaded(group)
         theirs = {i for group in state_dict["param_groups"] if "bits" not in group for i in group["params"]}
@@ -430,9 +465,13 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p][name] = value.to(p.device, dtype, copy=True).contiguous()
         for group in self.param_groups:
             group.setdefault("bits", 32)
-            counts = [int(self.state[p].pop("step")) for p in group["params"] if "step" in self.state[p]]
-            if "step" not in group and counts:
-                _require(len(set(counts)) == 1, "AdamW: the parameters of a group have one count of steps")
-                group["step"] = torch.full((), counts[0], dtype=torch.int64)
-            if "step" in group:
-                group["step"] = group["step"].to(group["params"][0].device, copy=True)
+            own = [(state, int(state.pop("step"))) for state in map(self._known, group["params"]) if "step" in state]
+            values = [n for _, n in own]
+            if "step" not in group and not own:
+                continue
+            most = int(group["step"]) if "step" in group else max(values, key=values.count)
+            counts = {n: torch.full((), n, dtype=torch.int64, device=group["params"][0].device) for n in (most, *values)}
+            group["step"] = counts[most]
+            for state, n in own:
+                if n != most:
+                    state["step"] = counts[n]

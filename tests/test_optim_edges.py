@@ -95,3 +95,79 @@ def test_moments_of_torch_in_bfloat16_become_float32():
     want = was * (1 - 1e-3) - 1e-2 * m / (1 - 0.9 ** 3) / ((v / (1 - 0.999 ** 3)).sqrt() + 1e-8)
     # Up or down by less than a place of bfloat16.
     assert bool(((p.detach().double() - want).abs() <= 2.0 ** -7 * want.abs()).all())
+
+
+# Steps in which each of four parameters has a gradient: always, from the eleventh on, with gaps, and never.
+PATTERN = [lambda k: True, lambda k: k >= 10, lambda k: k % 3 != 1, lambda k: False]
+
+
+def gappy(make, steps, clip=None, switch=None):
+    torch.manual_seed(3)
+    params = [torch.nn.Parameter(torch.randn(40)) for _ in PATTERN]
+    opt = make([dict(params=params[:3]), dict(params=params[3:])])
+    for k in range(steps):
+        for p, has in zip(params, PATTERN):
+            p.grad = torch.randn(40) * (1 + k % 5) if has(k) else None
+        if clip is not None:
+            torch.nn.utils.clip_grad_norm_(params, clip)
+        if switch is not None:
+            opt = switch(k, opt, params)
+        opt.step()
+    return opt, params
+
+
+@pytest.mark.parametrize("clip", [None, 0.5])
+def test_a_parameter_that_comes_late_or_pauses_steps_as_with_torch(clip):
+    opt, params = gappy(lambda groups: optim.AdamW(groups, lr=1e-2, max_grad_norm=clip), 400)
+    _, wants = gappy(lambda groups: torch.optim.AdamW(groups, lr=1e-2), 400, clip)
+    # 400 steps of about lr, each off by some ten roundings of 2^-24 (clipped ones of the norm, too), and the parameter's own.
+    for p, want in zip(params, wants):
+        assert bool(((p - want).abs() <= 400 * (1e-2 * 16 + 4) * 2.0 ** -24).all())
+    steps = [int(opt.state[p].get("step", opt.param_groups[0]["step"])) for p in params[:3]]
+    assert steps == [400, 390, 267] and params[3] not in opt.state and "step" not in opt.param_groups[1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_own_counts_of_steps_pass_through_state_dicts(bits):
+    def switch(k, opt, params):
+        if k in (5, 12, 20):
+            saved, opt = opt.state_dict(), optim.AdamW([dict(params=params[:3]), dict(params=params[3:])], bits=bits)
+            opt.load_state_dict(saved)
+        return opt
+
+    make = lambda groups: optim.AdamW(groups, lr=1e-2, bits=bits)
+    (a, p), (b, q) = gappy(make, 30), gappy(make, 30, switch=switch)
+    assert all(torch.equal(x, y) for x, y in zip(p, q))
+    for x, y in zip(p[:3], q[:3]):
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(a.state[x][name], b.state[y][name])
+        count = lambda opt, z: int(opt.state[z].get("step", opt.param_groups[0]["step"]))
+        assert count(a, x) == count(b, y)
+
+
+def test_different_counts_of_torch_are_gone_on_from():
+    def switch(k, opt, params):
+        if k == 20:
+            saved, opt = opt.state_dict(), optim.AdamW([dict(params=params[:3]), dict(params=params[3:])])
+            opt.load_state_dict(saved)
+        return opt
+
+    make = lambda groups: torch.optim.AdamW(groups, lr=1e-2)
+    (_, p), (opt, q) = gappy(make, 40), gappy(make, 40, switch=switch)
+    for x, y in zip(p, q):
+        assert bool(((x - y).abs() <= 20 * (1e-2 * 16 + 4) * 2.0 ** -24).all())
+    assert [int(opt.state[x].get("step", opt.param_groups[0]["step"])) for x in q[:3]] == [40, 30, 27]
+
+
+def test_a_step_that_was_refused_counts_nothing():
+    p = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(3))]
+    opt = optim.AdamW(p, lr=1e-2)
+    for x in p:
+        x.grad = torch.ones(3)
+    opt.param_groups[0]["eps"] = -1.0
+    with pytest.raises(RuntimeError):
+        opt.step()
+    opt.param_groups[0]["eps"] = 1e-8
+    opt.step()
+    assert int(opt.param_groups[0]["step"]) == 1 and all("step" not in opt.state[x] for x in p)
+    assert torch.allclose(p[0], torch.full((3,), (1 - 1e-4) - 1e-2))
