@@ -350,6 +350,12 @@ def _check_loaded(group):
              "groups says that it is not")
 
 
+def _refuse_capture(device):
+    """Where state is made: a replay would make it anew each time."""
+    _require(device.type != "cuda" or not torch.cuda.is_current_stream_capturing(),
+             "AdamW: a step that makes moments, or a count of steps, is not captured: step once before the capture")
+
+
 class AdamW(torch.optim.Optimizer):
     """``adamw_step`` as a torch optimizer.
 
@@ -359,7 +365,8 @@ class AdamW(torch.optim.Optimizer):
     gradient is left as it is, and so is its count of steps, as torch's.  The group's
     ``step`` counts for all parameters that have had a gradient in each of its steps; one
     that came later, or was left out of one, has a ``step`` in its own state, and a launch
-    for those that share it."""
+    for those that share it.  A step that is captured in a CUDA
+    graph follows one that was not, which made the moments."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits=32, max_grad_norm=None):
         if bits not in (8, 32):
@@ -377,6 +384,7 @@ class AdamW(torch.optim.Optimizer):
             return []
         states = [self.state[p] for p in params]
         if not all("exp_avg" in state for state in states):
+            _refuse_capture(params[0].device)
             count = torch.zeros((), dtype=torch.int64, device=params[0].device)
             if any("exp_avg" in state and "step" not in state for state in map(self._known, group["params"])):
                 for state in states:
@@ -392,6 +400,7 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad is None and "exp_avg" in state:
                     count = state.get("step", group["step"])
                     if count.data_ptr() in going:
+                        _refuse_capture(count.device)
                         state["step"] = behind.setdefault(count.data_ptr(), count.clone())
         if not any("step" in state for state in states):
             return [(group["step"], params, states, range(len(params)))]
