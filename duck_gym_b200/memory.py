@@ -600,14 +600,48 @@ class _GatedLinear(torch.autograd.Function):
         return dx if dx is None or len(ctx.shape) == 2 else dx.view(ctx.shape), *dw, *db, None
 
 
+class _PlainLinear(torch.autograd.Function):
+    """x w^T + b on the CPU, outside autocast regions in the backward pass too."""
+
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(x, w, b):
+        return F.linear(x, w, b)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, w, _ = inputs
+        ctx.save_for_backward(x, w)
+        ctx.save_for_forward(x, w)
+
+    @staticmethod
+    @torch.autocast("cpu", enabled=False)
+    def backward(ctx, dy):
+        x, w = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad
+        return (_PlainLinear.apply(dy, w.t(), None) if need_x else None,
+                _PlainLinear.apply(dy.t(), x.t(), None) if need_w else None, dy.sum(0) if need_b else None)
+
+    @staticmethod
+    @torch.autocast("cpu", enabled=False)
+    def jvp(ctx, dx, dw, db):
+        x, w = ctx.saved_tensors
+        terms = [] if dx is None else [_PlainLinear.apply(dx, w, None)]
+        terms += [] if dw is None else [_PlainLinear.apply(x, dw, None)]
+        terms += [] if db is None else [db.expand(x.shape[0], -1)]
+        return sum(terms[1:], terms[0])
+
+
 @torch.autocast("cpu", enabled=False)
 def _gated_plain(x, w_gate, w_up, b_gate, b_up, activation):
     """In float32 or wider, rounded once."""
     wide = torch.promote_types(x.dtype, torch.float32)
     to = lambda t: None if t is None else t.to(wide)
-    a, u = F.linear(to(x), to(w_gate), to(b_gate)), F.linear(to(x), to(w_up), to(b_up))
+    rows = to(x).reshape(-1, x.shape[-1])
+    a, u = _PlainLinear.apply(rows, to(w_gate), to(b_gate)), _PlainLinear.apply(rows, to(w_up), to(b_up))
     act = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid}[activation]
-    return (act(a) * u).to(x.dtype)
+    return (act(a) * u).to(x.dtype).view(x.shape[:-1] + w_gate.shape[:1])
 
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
