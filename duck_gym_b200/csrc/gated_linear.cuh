@@ -50,9 +50,11 @@ template <int ACT, bool FAST> __device__ __forceinline__ Activated activate(floa
     return {a * below, below + a * density};
   } else {
     float s, rest;
-    if constexpr (FAST) {   // (exp(-a) is held below 2^126; a NaN stays one)
+    // FAST: exp(-a) is held at 2^127, whose reciprocal is flushed to zero, so that s is 0 from a = -87.3 down and no
+    // infinity meets a zero (rest is 0 there, too, where it is 1, but has s as a factor).  A NaN stays one.
+    if constexpr (FAST) {
       float t;
-      asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(t) : "f"(a * -1.4426950408889634f));
+      asm("min.NaN.f32 %0, %1, 0f42FE0000;" : "=f"(t) : "f"(a * -1.4426950408889634f));
       asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t));
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + t));
       rest = t * s;
