@@ -27,7 +27,7 @@
 // to the initial state.  P's sign bit (products of gates have none) says that an
 // episode begins inside, B alone being what is left.
 //
-// Bound by memory in principle; 23 instructions a value in the forward pass (issue
+// Bound by memory in principle; 24 instructions a value in the forward pass (issue
 // slots 56 % busy) and warps that wait for their copies keep it at 60 % of the copy's
 // rate.  Measured on a B200, cold,
 // bfloat16: 24 steps of 1024 x 256 channels, forward 12 us, backward 15.5 (38 and
@@ -99,8 +99,9 @@ struct Gate {
   float f, rest;   // sigmoid(gate) and 1 - sigmoid(gate)
 };
 // For bfloat16, whose gates are known to 2^-9, the exponential and the quotient
-// that the hardware approximates (2^-21), exp(-gate) held below 2^126 (a NaN stays
-// one); for float32 the rounded exponential, of -|gate|, and the hardware's
+// that the hardware approximates (2^-21), exp(-gate) held at 2^126 (a NaN stays one),
+// whose reciprocal is the smallest normal number, and taken off: a gate from -87.3 down
+// leaves nothing of a state, however large; for float32 the rounded exponential, of -|gate|, and the hardware's
 // reciprocal of a number between 1 and 2 after one of Newton's iterations, so that
 // neither f nor 1 - f loses digits where the other is near 1.
 template <class T> __device__ __forceinline__ Gate gateOf(float g) {
@@ -109,7 +110,7 @@ template <class T> __device__ __forceinline__ Gate gateOf(float g) {
     asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(t) : "f"(g * -1.4426950408889634f));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + t));
-    return {r, t * r};
+    return {r - 1.17549435e-38f, t * r};
   } else {
     const float t = expf(-fabsf(g)), d = 1.f + t;
     float r;

@@ -40,3 +40,27 @@ def test_linear_activations_over_the_whole_range(activation, dtype, up):
     for value, want, factor in zip(got, (y * u, 0.25 * u * slope, 0.25 * y), (u, u, torch.ones_like(u))):
         off = (value.detach().cpu().double() - want).abs()
         assert bool((off <= relative * want.abs() + lost * factor.abs() + 2.0 ** -124).all()), (off, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [3, 300])
+def test_recurrence_gates_over_the_whole_range(T, dtype):
+    """What a far gate leaves of a state, or adds of a value, is nothing, however large they are."""
+    gates = torch.tensor([-95.0, -200.0, -1e30, -3e38, float("-inf"), 110.0, 200.0, 3e38, float("inf")]).to(dtype).expand(T, 1, 9)
+    values, state = torch.full((T, 1, 9), 0.5, dtype=dtype), torch.full((1, 9), 1e37)
+    values[..., 5:], state[..., 5:] = 1e37, 0.5
+    leaves = [t.contiguous().cuda().requires_grad_() for t in (gates, values, state)]
+    out, last = memory.gated_recurrence(*leaves)
+    # exp(-95) 1e37 is 0.05 of a half in the first step, which float32's gate keeps; bfloat16's is flushed.
+    want = torch.full((T, 1, 9), 0.5)
+    exact = want.clone()
+    exact[0, 0, 0] = 0.5 + 1e37 * 5.521e-42
+    got = out.detach().float().cpu()
+    assert torch.equal(got[..., 1:], want[..., 1:]) and torch.equal(last.cpu()[..., 1:], want[0, :, 1:])
+    assert bool(((got[..., 0] - 0.5).abs() <= 1.01 * (exact[..., 0] - 0.5)).all())
+    step = state.cuda()
+    assert torch.equal(memory.gated_recurrence_step(gates[0].cuda(), values[0].cuda(), step).float().cpu()[:, 1:], want[0, :, 1:])
+    dg, dv, ds = torch.autograd.grad((out, last), leaves, (torch.full_like(out, 1e30), torch.zeros_like(last)))
+    keep, replace = slice(5, 9), slice(1, 5)
+    assert not bool(dg[..., 1:].any()) and not bool(ds[:, replace].any()) and not bool(dv[..., keep].any())
+    assert torch.equal(dv[..., replace].float(), torch.full_like(dv[..., replace].float(), 1e30).to(dtype).float())
