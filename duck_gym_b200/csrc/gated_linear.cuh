@@ -570,8 +570,10 @@ __global__ void __launch_bounds__(kPadThreads) padRows(PadArgs p) {
 // next steps' way from memory takes longer than their products).  The forward pass's
 // columns are half of Wg's and half the same of Wu's: a thread has both of a value.
 // A sum of n values of random sign is off by 2^-25 sqrt(n / 2) of itself where each is
-// added to one register; after 1024 steps it goes to memory, and is added to
-// there, so that long ones are off by no more than 7e-7.
+// added to one register; after kRunSteps it goes to memory, and is added to
+// there, so that long ones are off by no more than 7e-7.  That is where the outputs
+// are, but for the forward pass, whose sums are not outputs: shared memory (16384
+// rows, 4096 x 1024: 5.20 ms, in one run 4.99).
 struct ProductArgs {
   const float *x, *wGate, *wUp, *bGate, *bUp;
   float *h, *kept;             // forward: h, and a and u [2, rows, F] or null
@@ -583,6 +585,7 @@ struct ProductArgs {
 };
 constexpr int kProductThreads = 256;
 __host__ __device__ constexpr int productSteps(int tile) { return tile == 64 ? 32 : 16; }
+constexpr int kRunSteps = 1024;
 
 // The first `count` of four values.
 __device__ __forceinline__ float4 fetchFour(const float *p, int64_t count, bool whole) {
@@ -604,12 +607,14 @@ __device__ __forceinline__ void addProduct(Two &d, Two a, Two b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
 }
 
-template <Pass PASS, int T> __global__ void __launch_bounds__(kProductThreads, 2) gatedProducts(ProductArgs p) {
+// RUNS: sums may be longer than one run; the forward pass has T T floats of dynamic shared memory then.
+template <Pass PASS, int T, bool RUNS> __global__ void __launch_bounds__(kProductThreads, 2) gatedProducts(ProductArgs p) {
   static_assert(PASS != Pass::gradients, "gatedGradients");
   constexpr int K = productSteps(T), P = T + 4, R = T / 16, H = R / 2;   // R rows and columns a thread, H in each half of the columns
   constexpr int kLoads = T * K / (4 * kProductThreads), kGroups = T / 4, kSteps = K / 4;   // a thread's, and of four values side by side
   constexpr bool kAlongA = PASS != Pass::weights, kAlongB = PASS == Pass::forward;   // steps are contiguous
   __shared__ __align__(16) float as[2][K][P], bs[2][K][P];
+  extern __shared__ __align__(16) Two earlier[];   // forward: sums of the runs before, R H of each thread
   const int tid = threadIdx.x;
   const int64_t row0 = int64_t(blockIdx.x) * T;   // weights: of Wg's and then Wu's tiles
   const int rowTiles = (p.F + T - 1) / T;
@@ -698,7 +703,7 @@ template <Pass PASS, int T> __global__ void __launch_bounds__(kProductThreads, 2
   };
   int64_t run = first;
   do {
-    const int64_t end = PASS == Pass::forward ? last : min(last, run + 1024 / K);
+    const int64_t end = RUNS ? min(last, run + kRunSteps / K) : last;
     for (int64_t step = run; step < end; ++step) {
       const int now = int(step - first) & 1;
       if (step + 1 < last) {
@@ -733,7 +738,20 @@ template <Pass PASS, int T> __global__ void __launch_bounds__(kProductThreads, 2
       }
       __syncthreads();
     }
-    if (PASS != Pass::forward) store(run > first);
+    if constexpr (PASS != Pass::forward) {
+      store(run > first);
+    } else if constexpr (RUNS) {   // (a thread's own sums: no barrier)
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          Two &at = earlier[(i * H + j) * kProductThreads + tid];
+          const float2 now = partsOf(sum[i][j]), before = run > first ? partsOf(at) : make_float2(0.f, 0.f);
+          const Two both = twoOf(before.x + now.x, before.y + now.y);
+          if (end < last) at = both, sum[i][j] = 0;
+          else sum[i][j] = both;
+        }
+    }
     run = end;
   } while (run < last);
   if constexpr (PASS == Pass::forward) {
