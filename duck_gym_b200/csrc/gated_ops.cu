@@ -134,11 +134,18 @@ template <class F> void withLots(const duck_recurrence &a, const RecurrenceArgs 
 }
 
 // ---------------------------------------------------------------- gated linear
+// Products that a tensor core adds up in one accumulator.  It cuts its sums off where float32 rounds them, so that sums of one
+// sign come out too small: 65536 products by 6e-4, a third of a rounding to bfloat16 in the mean square, a million by 6e-3.
+// Longer sums are made of parts, added in float32; those of the projections, whose accumulators go nowhere but into the
+// activation, are refused.
+constexpr int kTensorSum = 1 << 16;
+
 bool gatedChecked(const duck_gated *a) {
   require(a != nullptr, "Invalid arguments");
   requireType(a->type);
   require(a->rows >= 0 && a->D > 0 && a->F > 0, "Invalid layer sizes");
   require(a->rows < (int64_t(1) << 31) - 4096 && a->D <= (1 << 20) && a->F <= (1 << 20), "Too many rows or columns");
+  require(a->type == DUCK_FLOAT32 || a->D <= kTensorSum, "bfloat16 layers have 65536 columns at most");
   require(a->activation >= DUCK_SILU && a->activation <= DUCK_SIGMOID, "Invalid activation");
   require(a->type == DUCK_FLOAT32 || a->D % 8 || a->rows <= 1 || a->x == nullptr || a->x_stride >= a->D,
           "bfloat16 rows must not overlap");
@@ -156,9 +163,10 @@ struct GatedPlan {
   int64_t biasCount;
   int64_t bothBytes, biasBytes, partBytes, inputBytes, keptBytes;   // in this order
 };
-// Where tiles leave multiprocessors idle, the steps of their products are split, so that each part has `least` at least.
-int splitsOf(int64_t tiles, int64_t fit, int64_t steps, int64_t least) {
-  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(fit / tiles, steps / least));
+// Where tiles leave multiprocessors idle, the steps of their products are split, so that each part has `least` at least;
+// and where they are more than `most`.
+int splitsOf(int64_t tiles, int64_t fit, int64_t steps, int64_t least, int64_t most = INT64_MAX) {
+  const int64_t splits = std::max({int64_t(1), std::min<int64_t>(fit / tiles, steps / least), (steps - 1) / most + 1});
   return int(std::max<int64_t>(1, ceilDiv(steps, ceilDiv(std::max<int64_t>(1, steps), splits))));   // none without steps
 }
 int64_t padded(int64_t bytes) { return ceilDiv(bytes, 256) * 256; }
@@ -192,11 +200,12 @@ GatedPlan planGated(const duck_gated &a) {
     // Rows are split so that the tiles fill the GPU once, into parts of 512 rows at least: a part's sums are written and read
     // once more (24576 rows, 256 x 512: 17 us in 18 parts of 256 columns, 20 in 9 of 128).
     p.weightColumns = a.D > 128 ? 256 : a.D > 64 ? 128 : 64;
-    p.splits = splitsOf(2 * ceilDiv(a.F, kTileRows) * ceilDiv(a.D, p.weightColumns), 148, ceilDiv(rows, kTileSteps), 8);
+    constexpr int most = kTensorSum / kTileSteps;
+    p.splits = splitsOf(2 * ceilDiv(a.F, kTileRows) * ceilDiv(a.D, p.weightColumns), 148, ceilDiv(rows, kTileSteps), 8, most);
     // x's gradient of few rows (66 rows, 136 x 3788: three tiles of 120 steps each otherwise).
     const int64_t rowTiles = ceilDiv(rows, kTileRows);
     p.inputColumns = tileColumns(rowTiles, a.D);
-    p.inputSplits = splitsOf(rowTiles * ceilDiv(a.D, p.inputColumns), 148, 2 * ceilDiv(a.F, kTileSteps), 8);
+    p.inputSplits = splitsOf(rowTiles * ceilDiv(a.D, p.inputColumns), 148, 2 * ceilDiv(a.F, kTileSteps), 8, most);
   } else {
     p.bothBytes = padded(rows * 2 * a.F * 4);
     p.keptBytes = rows * 2 * a.F * 4;

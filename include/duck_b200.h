@@ -464,7 +464,7 @@ int duck_gated_recurrence_step(const duck_recurrence *args, duck_stream stream);
 
 /* Gated linear layer on rows x [rows, D]:
  *   h = act(x w_gate^T + b_gate) (x w_up^T + b_up),  weights [F, D], biases [F]
- * and its gradients.  rows < 2^31 - 4096, D and F up to 2^20.  Element types are
+ * and its gradients.  rows < 2^31 - 4096, D and F up to 2^20 (DUCK_BFLOAT16: D up to 2^16).  Element types are
  * those of `type` throughout; h, the weights, their gradients and dx are dense,
  * rows of x and dh have the strides given.  `kept` is what a
  * forward call leaves for the backward one; for DUCK_BFLOAT16 it is empty where D is

@@ -88,3 +88,34 @@ def test_linear_sums_of_many_steps_in_float32(rows, D, F):
     exact = (dh.double() * a * torch.sigmoid(a)).sum(0)
     # Of the projection, and sums of `rows` values.
     assert float((db - exact).norm() / exact.norm()) <= 2e-6 + 4 * (rows ** 0.5 + 8) * 2.0 ** -24
+
+
+def test_linear_long_sums_in_bfloat16():
+    """Tensor cores cut sums off: one of 65536 products of one sign is too small by up to 6e-4, of 524288 by some 2e-3."""
+    # Tiles enough that no split is needed for them: sums over rows, and over features.
+    for rows, D, F in ((1 << 19, 64, 9472), (18944, 64, 1 << 18)):
+        g = torch.Generator("cuda")
+        g.manual_seed(rows)
+        x = torch.rand(rows, D, generator=g, device="cuda").bfloat16().requires_grad_()
+        w = (torch.rand(F, D, generator=g, device="cuda") / D).bfloat16().requires_grad_()
+        none, forty = torch.zeros_like(w).detach(), torch.full((F,), 40.0, dtype=torch.bfloat16, device="cuda")
+        # The gate is open: the gradient of u is dh, that of a zero.
+        h = memory.gated_linear(x, none, w, forty, torch.zeros_like(forty), activation="sigmoid")
+        dh = (0.5 + torch.rand(F, generator=g, device="cuda")).bfloat16()
+        dx, dw = torch.autograd.grad(h, (x, w), dh.expand(rows, F))
+        del h
+        if rows > F:
+            got, want = dw.double(), dh.double()[:, None] * x.detach().double().sum(0)
+        else:
+            got, want = dx[0].double(), dh.double() @ w.detach().double()
+        # The mean of results that are each rounded by 1.7e-3 in the mean square, of 64 at least: 2.2e-4.
+        assert abs(float((got / want - 1).mean())) <= 6e-4 + 2.2e-4
+
+
+def test_linear_refuses_projections_of_long_sums_in_bfloat16():
+    w = torch.zeros(2, (1 << 16) + 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="65536"):
+        memory.gated_linear(w, w, w)
+    fine = w[:, :1 << 16].contiguous()
+    assert memory.gated_linear(fine, fine, fine).shape == (2, 2)
+    assert memory.gated_linear(w.float(), w.float(), w.float()).shape == (2, 2)
