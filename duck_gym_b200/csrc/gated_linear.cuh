@@ -93,6 +93,7 @@ struct TileArgs {
   int D, F, stride, activation;
   int tiles, columnTiles, rowTiles, splits, steps;   // steps of 64 of a tile's product
   bool wholeH, wholeDh, wholeBias, wholeD;   // rows of 16-byte pieces: h and dh move by the TMA
+  uint64_t waitLimit;
 };
 struct TileMaps {
   CUtensorMap a0, a1, b0, b1;   // operands
@@ -192,7 +193,7 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
-    *broken = 0;
+    *broken = p.waitLimit == 0;   // (given up from the start)
     for (int i = 0; i < S::stages; ++i) barrierInit(full + i, 1), barrierInit(empty + i, 1);
     for (int i = 0; i < 2; ++i) barrierInit(done + i, 1), barrierInit(taken + i, kTileWarps);
     for (int i = 0; i < kTileWarps; ++i) barrierInit(came + i, 1);
@@ -250,7 +251,7 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
         int first;
         const int steps = stepsOf(at, first);
         for (int k = 0; k < steps; ++k) {
-          fine = barrierWait(empty + stage, parity ^ 1, broken);
+          fine = barrierWait(empty + stage, parity ^ 1, broken, p.waitLimit);
           if (!fine) break;
           uint64_t *bar = full + stage;
           uint8_t *a = tileA + stage * S::a, *b = tileB + stage * S::b;
@@ -277,11 +278,10 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
           if (++stage == S::stages) stage = 0, parity ^= 1;
         }
       }
-      // Given up: the copies in flight come to their end before the block does.
-      for (int i = 0; !fine && i < issued; ++i) {
+      // The copies come to their end before the block does, whoever gave up.
+      for (int i = 0; i < issued; ++i) {
         if (--stage < 0) stage = S::stages - 1, parity ^= 1;
-        int none = 0;
-        barrierWait(full + stage, parity, &none);
+        barrierSettle(full + stage, parity);
       }
     }
   } else if (warp == 1) {
@@ -294,10 +294,10 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
         const Tile at = tileAt(t);
         int first;
         const int steps = stepsOf(at, first), buffer = n & 1;
-        fine = barrierWait(taken + buffer, (n >> 1 & 1) ^ 1, broken);
+        fine = barrierWait(taken + buffer, (n >> 1 & 1) ^ 1, broken, p.waitLimit);
         tensorFenceAfter();
         for (int k = 0; k < steps && fine; ++k) {
-          fine = barrierWait(full + stage, parity, broken);
+          fine = barrierWait(full + stage, parity, broken, p.waitLimit);
           if (!fine) break;
           tensorFenceAfter();
           const uint64_t a = operandDescriptor<kAlongA>(sharedAddress(tileA + stage * S::a));
@@ -311,11 +311,9 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
         }
         if (fine) tensorCommit(done + buffer);
       }
-      if (!fine) {   // given up: the products that were issued come to their end, too
-        int none = 0;
-        tensorCommit(ended);
-        barrierWait(ended, 0, &none);
-      }
+      // So do the products, before their tensor memory is freed.
+      tensorCommit(ended);
+      barrierSettle(ended, 0);
     }
   } else if (warp >= 4) {
     // A warp has a quarter of the tile's rows (that of tensor memory which it reaches) and of its columns.
@@ -339,7 +337,7 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
       uint4 *gradients = reinterpret_cast<uint4 *>(incoming + (warp - 4) * S::incoming);
       uint64_t *bar = came + (warp - 4);
       uint32_t parity = 0;
-      bool asked = false, fine = true;
+      bool asked = false, fine = p.waitLimit > 0;
       auto ours = [&](const Tile &at) {   // the tile has rows and columns for this warp
         return part * kPart < kColumns && at.row + quarter * 32 < p.rows && at.column + part * kPart < p.F;
       };
@@ -359,11 +357,11 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
         const int buffer = n & 1, first = at.column + part * kPart;
         const int64_t row = at.row + quarter * 32, rowsLeft = p.rows - row;
         const bool mine = lane < rowsLeft;
-        fine = __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken));
-        if (PASS == Pass::gradients && p.wholeDh && own) {
-          const bool here = __all_sync(0xffffffffu, barrierWait(bar, parity, broken));
-          fine = fine && here;
-          if (here) asked = false, parity ^= 1;
+        // (given up once, no tile waits again)
+        fine = fine && __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken, p.waitLimit));
+        if (PASS == Pass::gradients && p.wholeDh && own && fine) {
+          fine = __all_sync(0xffffffffu, barrierWait(bar, parity, broken, p.waitLimit));
+          if (fine) asked = false, parity ^= 1;
         }
         tensorFenceAfter();
         const uint32_t tensorRow = accumulators + buffer * BN + (uint32_t(quarter * 32) << 16) + part * kPart;
@@ -469,7 +467,7 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
         }
         tensorFenceBefore();
         __syncwarp();
-        if (lane == 0) barrierArrive(taken + buffer);
+        if (lane == 0 && fine) barrierArrive(taken + buffer);   // (without it the products do not go on)
         if constexpr (PASS == Pass::gradients) {
           if (p.wholeDh && fine && lane == 0) askGradients(t + gridDim.x);   // every lane has its row of this tile's
           if (own) {
@@ -488,19 +486,19 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
       }
       if (lane == 0) {
         storesDone();
-        int none = 0;
-        if (asked) barrierWait(bar, parity, &none);   // given up: its own copy comes to its end
+        if (asked) barrierSettle(bar, parity);   // given up: its own copy comes to its end
       }
       __syncwarp();
     } else {
       int n = 0;
+      bool fine = p.waitLimit > 0;
       for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++n) {
         const Tile at = tileAt(t);
         const int buffer = n & 1;
         int first;
         const int steps = stepsOf(at, first);
         const int64_t row = at.row + quarter * 32, rowsLeft = (PASS == Pass::weights ? int64_t(p.F) : p.rows) - row;
-        const bool fine = __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken));
+        fine = fine && __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken, p.waitLimit));
         tensorFenceAfter();
         const uint32_t tensorRow = accumulators + buffer * BN + (uint32_t(quarter * 32) << 16) + part * kPart;
 #pragma unroll
@@ -524,7 +522,7 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
         }
         tensorFenceBefore();
         __syncwarp();
-        if (lane == 0) barrierArrive(taken + buffer);
+        if (lane == 0 && fine) barrierArrive(taken + buffer);   // (without it the products do not go on)
       }
     }
   }

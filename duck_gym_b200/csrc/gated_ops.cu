@@ -302,8 +302,10 @@ template <Pass PASS> void launchProjections(const duck_gated &a, TileArgs t, cud
   };
   withColumns(tileColumns(rowTiles, 2 * int64_t(a.F)), run);
 }
+std::atomic<int64_t> waitLimit{int64_t(kWaitLimit)};
 TileArgs tileArgs(const duck_gated &a) {
   TileArgs t{};
+  t.waitLimit = uint64_t(waitLimit.load());
   t.bGate = static_cast<const bf16 *>(a.b_gate);
   t.bUp = static_cast<const bf16 *>(a.b_up);
   t.rows = a.rows, t.D = a.D, t.F = a.F, t.activation = a.activation;
@@ -470,6 +472,13 @@ int duck_gated_linear_sizes(const duck_gated *args, int64_t *out) {
     const GatedPlan plan = planGated(*args);
     out[0] = plan.bothBytes + plan.biasBytes + plan.partBytes + plan.inputBytes;
     out[1] = plan.keptBytes;
+  });
+}
+
+int duck_wait_limit(int64_t nanoseconds) {
+  return guarded([&] {
+    require(nanoseconds >= 0, "A wait's limit is 0 or more");
+    waitLimit = nanoseconds;
   });
 }
 

@@ -2,9 +2,10 @@
 // tiles by the TMA, mbarriers, tensor memory, and products of bfloat16 tiles that
 // are accumulated there in float32.
 //
-// Every wait has a limit of about two seconds.  A thread whose wait runs out says so
-// in `broken`, which ends the others' waits; a kernel then marks its outputs as not
-// computed and ends as it would otherwise.
+// Every wait has a limit.  A thread whose wait runs out says so in `broken`, which
+// ends the others' waits; a kernel then marks its outputs as not computed, waits for
+// the copies and products that it has begun (with kWaitLimit), and ends as it would
+// otherwise.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -37,16 +38,16 @@ __device__ __forceinline__ uint64_t nanoseconds() {
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
   return t;
 }
-constexpr uint64_t kWaitLimit = 2000000000;   // nanoseconds
+constexpr uint64_t kWaitLimit = 2000000000;   // nanoseconds; callers may choose another one
 // Whether the barrier's phase came to its end; false once a wait ran out.
-__device__ __forceinline__ bool barrierWait(uint64_t *bar, uint32_t parity, volatile int *broken) {
+__device__ __forceinline__ bool barrierWait(uint64_t *bar, uint32_t parity, volatile int *broken, uint64_t limit) {
   if (barrierTry(bar, parity)) return true;
   const uint64_t begin = nanoseconds();
   for (;;) {
     for (int i = 0; i < 64; ++i)
       if (barrierTry(bar, parity)) return true;
     if (*broken) return false;
-    if (nanoseconds() - begin > kWaitLimit) {
+    if (nanoseconds() - begin > limit) {
       *broken = 1;
       return false;
     }
@@ -70,6 +71,11 @@ __device__ __forceinline__ void storeBox(const CUtensorMap *map, const void *fro
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 __device__ __forceinline__ void fenceForCopies() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// For what this thread has begun, whether others have given up or not.
+__device__ __forceinline__ void barrierSettle(uint64_t *bar, uint32_t parity) {
+  int none = 0;
+  barrierWait(bar, parity, &none, kWaitLimit);
+}
 // Until this thread's stored boxes have been read, or are in memory.
 __device__ __forceinline__ void storesRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void storesDone() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }

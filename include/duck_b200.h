@@ -494,6 +494,12 @@ int duck_gated_linear_sizes(const duck_gated *args, int64_t *out);
 int duck_gated_linear_forward(const duck_gated *args, duck_stream stream);
 int duck_gated_linear_backward(const duck_gated *args, duck_stream stream);
 
+/* How long a wait inside a kernel of the bfloat16 layer may take (for data on its way
+ * through the multiprocessor, which takes microseconds), in calls from now on: two
+ * seconds unless set.  A block of which a wait runs out writes NaN for what it could
+ * not compute, and ends.  With 0 all blocks give up from the start: for tests. */
+int duck_wait_limit(int64_t nanoseconds);
+
 /* AdamW over many tensors (the Python side is duck_gym_b200/optim.py).  A tensor
  * has n dense values of `type`; its gradient has the same.  Moments are float32
  * [n], or (bits = 8) codes [n], int8 for exp_avg and uint8 for exp_avg_sq, with one

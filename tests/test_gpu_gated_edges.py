@@ -119,3 +119,51 @@ def test_linear_refuses_projections_of_long_sums_in_bfloat16():
     fine = w[:, :1 << 16].contiguous()
     assert memory.gated_linear(fine, fine, fine).shape == (2, 2)
     assert memory.gated_linear(w.float(), w.float(), w.float()).shape == (2, 2)
+
+
+# One tile a block and many, steps that fit in the ring and do not, split sums, padded rows.
+@pytest.mark.parametrize("rows,D,F", [(16, 256, 512), (300, 61, 301), (4096, 1024, 264), (40000, 64, 512)])
+def test_linear_waits_that_run_out(rows, D, F):
+    """A block that gives up ends, with its copies and products, and marks what it could not compute."""
+    from duck_gym_b200.cuda_batch import library
+
+    g = torch.Generator("cuda")
+    g.manual_seed(rows)
+    draw = lambda *s: torch.randn(s, generator=g, device="cuda").bfloat16()
+    leaves = [t.requires_grad_() for t in (draw(rows, D), draw(F, D) / 16, draw(F, D) / 16, draw(F), draw(F))]
+    dh = draw(rows, F)
+    call = lambda: memory.gated_linear(*leaves)
+    grads = lambda h: torch.autograd.grad(h, leaves, dh)
+
+    def limited(f):
+        torch.cuda.synchronize()
+        assert library().duck_wait_limit(0) == 0
+        try:
+            return f()
+        finally:
+            torch.cuda.synchronize()
+            assert library().duck_wait_limit(2 * 10**9) == 0
+
+    def settled(f):
+        """After one that did not; the first call may say so."""
+        try:
+            return f()
+        except RuntimeError:
+            return f()
+
+    h = call()
+    want = [h, *grads(h)]
+    assert all(bool(t.isfinite().all()) for t in want)
+    bad = limited(call)
+    assert bool(bad.isnan().all())
+    h = settled(call)
+    bad = limited(lambda: grads(h))
+    assert all(bool(t.isnan().all()) for t in bad)
+    h = settled(call)
+    assert all(torch.equal(a, b) for a, b in zip([h, *grads(h)], want))
+
+
+def test_a_wait_limit_is_not_negative():
+    from duck_gym_b200.cuda_batch import library
+
+    assert library().duck_wait_limit(-1) != 0 and b"limit" in library().duck_last_error()
