@@ -94,6 +94,7 @@ struct TileArgs {
   int tiles, columnTiles, rowTiles, splits, steps;   // steps of 64 of a tile's product
   bool wholeH, wholeDh, wholeBias, wholeD;   // rows of 16-byte pieces: h and dh move by the TMA
   uint64_t waitLimit;
+  volatile int *ranOut;      // host memory: set where a wait ran out
 };
 struct TileMaps {
   CUtensorMap a0, a1, b0, b1;   // operands
@@ -530,6 +531,7 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
   __syncthreads();
   tensorFenceAfter();
   if (warp == 2) tensorFree(accumulators, 2 * BN);
+  if (threadIdx.x == 0 && *broken) *p.ranOut = 1, __threadfence_system();
 }
 
 // Rows of x, of Wg and of Wu, one after the other, as rows of whole 16-byte pieces: the

@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>
+#include <new>
 
 using namespace duckb200;
 
@@ -303,9 +304,28 @@ template <Pass PASS> void launchProjections(const duck_gated &a, TileArgs t, cud
   withColumns(tileColumns(rowTiles, 2 * int64_t(a.F)), run);
 }
 std::atomic<int64_t> waitLimit{int64_t(kWaitLimit)};
+// A word of host memory that the kernels of every device reach, and set where a wait ran out.
+std::atomic<int> &ranOut() {
+  static std::atomic<int> *const word = [] {
+    // The first call may be a captured one, and this is no work of its stream.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    check(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+    void *memory = nullptr;
+    const cudaError_t status = cudaHostAlloc(&memory, sizeof(std::atomic<int>), cudaHostAllocPortable | cudaHostAllocMapped);
+    check(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+    check(status, "cudaHostAlloc");
+    return new (memory) std::atomic<int>(0);
+  }();
+  return *word;
+}
+void waitsChecked() {
+  if (ranOut().load(std::memory_order_relaxed) && ranOut().exchange(0))
+    throw CudaError("gated linear: a wait of an earlier call's kernel ran out, and results of it are NaN");
+}
 TileArgs tileArgs(const duck_gated &a) {
   TileArgs t{};
   t.waitLimit = uint64_t(waitLimit.load());
+  t.ranOut = reinterpret_cast<volatile int *>(&ranOut());
   t.bGate = static_cast<const bf16 *>(a.b_gate);
   t.bUp = static_cast<const bf16 *>(a.b_up);
   t.rows = a.rows, t.D = a.D, t.F = a.F, t.activation = a.activation;
@@ -482,9 +502,14 @@ int duck_wait_limit(int64_t nanoseconds) {
   });
 }
 
+int duck_wait_status(void) {
+  return guarded([&] { waitsChecked(); });
+}
+
 int duck_gated_linear_forward(const duck_gated *args, duck_stream stream) {
   return guarded([&] {
     if (!gatedChecked(args)) return;
+    if (args->type == DUCK_BFLOAT16) waitsChecked();
     const duck_gated &a = *args;
     require(a.x && a.w_gate && a.w_up && a.h && !a.b_gate == !a.b_up, "Invalid arguments");
     requireAligned({a.h, a.kept});
@@ -515,6 +540,7 @@ int duck_gated_linear_backward(const duck_gated *args, duck_stream stream) {
   return guarded([&] {
     const bool some = gatedChecked(args);
     const duck_gated &a = *args;
+    if (a.type == DUCK_BFLOAT16) waitsChecked();
     require(!a.dw_gate == !a.dw_up && !a.db_gate == !a.db_up && !a.b_gate == !a.b_up, "Invalid arguments");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (!some) {   // no rows: no sums

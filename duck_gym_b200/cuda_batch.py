@@ -88,7 +88,7 @@ def library():
                      "duck_gated_recurrence_step", "duck_gated_linear_sizes", "duck_gated_linear_forward",
                      "duck_gated_linear_backward"):
             getattr(lib, name).argtypes = [P, P]
-        lib.duck_wait_limit.argtypes = [ctypes.c_int64]
+        lib.duck_wait_limit.argtypes, lib.duck_wait_status.argtypes = [ctypes.c_int64], []
         lib.duck_gradient_squares.argtypes = [P, I, I, P, P, P]
         lib.duck_adamw_step.argtypes = [P, I, P, P]
         lib.duck_moment_values.argtypes = [P, I, P]
@@ -118,7 +118,7 @@ def library():
                      "duck_elu_restore", "duck_elu_restore_bounded", "duck_linear_attention_sizes", "duck_linear_attention_forward",
                      "duck_linear_attention_backward", "duck_linear_attention_step", "duck_gated_recurrence_sizes",
                      "duck_gated_recurrence_forward", "duck_gated_recurrence_backward", "duck_gated_recurrence_step",
-                     "duck_gated_linear_sizes", "duck_gated_linear_forward", "duck_gated_linear_backward", "duck_wait_limit", "duck_gradient_squares", "duck_adamw_step", "duck_moment_values"):
+                     "duck_gated_linear_sizes", "duck_gated_linear_forward", "duck_gated_linear_backward", "duck_wait_limit", "duck_wait_status", "duck_gradient_squares", "duck_adamw_step", "duck_moment_values"):
             getattr(lib, name).restype = I
         _lib = lib
     return _lib

@@ -497,8 +497,11 @@ int duck_gated_linear_backward(const duck_gated *args, duck_stream stream);
 /* How long a wait inside a kernel of the bfloat16 layer may take (for data on its way
  * through the multiprocessor, which takes microseconds), in calls from now on: two
  * seconds unless set.  A block of which a wait runs out writes NaN for what it could
- * not compute, and ends.  With 0 all blocks give up from the start: for tests. */
+ * not compute, and ends.  The next call of the bfloat16 layer, or of duck_wait_status,
+ * after that fails with DUCK_ECUDA, once (it does not wait for kernels that still run).
+ * With a limit of 0 all blocks give up from the start: for tests. */
 int duck_wait_limit(int64_t nanoseconds);
+int duck_wait_status(void);
 
 /* AdamW over many tensors (the Python side is duck_gym_b200/optim.py).  A tensor
  * has n dense values of `type`; its gradient has the same.  Moments are float32

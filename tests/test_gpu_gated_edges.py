@@ -167,3 +167,53 @@ def test_a_wait_limit_is_not_negative():
     from duck_gym_b200.cuda_batch import library
 
     assert library().duck_wait_limit(-1) != 0 and b"limit" in library().duck_last_error()
+
+
+def test_linear_says_that_a_wait_ran_out():
+    from duck_gym_b200.cuda_batch import library
+
+    lib, w = library(), torch.ones(8, 16, dtype=torch.bfloat16, device="cuda")
+    leaf = w.clone().requires_grad_()
+    want = memory.gated_linear(leaf, w, w)
+
+    def limited():
+        lib.duck_wait_limit(0)
+        try:
+            with torch.no_grad():
+                return memory.gated_linear(w, w, w)
+        finally:
+            lib.duck_wait_limit(2 * 10**9)
+            torch.cuda.synchronize()
+
+    assert lib.duck_wait_status() == 0
+    for call in (lambda: memory.gated_linear(w, w, w), lambda: torch.autograd.grad(want, leaf, torch.ones_like(want), retain_graph=True)):
+        assert bool(limited().isnan().all())
+        with pytest.raises(RuntimeError, match="ran out"):
+            call()
+        call()   # once
+    limited()
+    # float32 layers do not wait; the status is there without a call, too.
+    memory.gated_linear(w.float(), w.float(), w.float())
+    assert lib.duck_wait_status() != 0 and b"ran out" in lib.duck_last_error() and lib.duck_wait_status() == 0
+    assert torch.equal(memory.gated_linear(w, w, w), want)
+
+
+def test_linear_whose_first_call_is_captured():
+    """What a process needs once is made during a capture, too."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from duck_gym_b200 import memory
+w = torch.ones(8, 16, dtype=torch.bfloat16, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    h = memory.gated_linear(w, w, w)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(h, memory.gated_linear(w, w, w)) and bool((h == 256).all()), h
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
