@@ -38,3 +38,41 @@ def test_a_first_step_is_not_captured(bits):
     for _ in range(5):
         plain.step()
     assert torch.equal(p, params[0])
+
+
+@pytest.mark.parametrize("optimizer", ["adamw", "adamw8"])
+def test_the_ppo_step_from_a_graph_is_the_eager_one_bit_for_bit(tmp_path, optimizer):
+    """The same gradients: the same parameters, moments (codes and exponents), counts and learning rates."""
+    from duck_gym_b200 import biped
+    from duck_gym_b200.bam_env import BamEnv
+    from duck_gym_b200.ppo import PPO, PPOConfig
+
+    biped.write_bam(tmp_path, seed=0)
+    env = BamEnv(tmp_path, num_envs=64, iterations=10, auto_reset=True, reward_enabled=True, seconds=0.1)
+    agent = PPO(env, PPOConfig(steps_per_env=8, optimizer=optimizer, weight_decay=0.01, max_grad_norm=0.5), seed=0)
+    for _ in range(2):   # moments are there, gradients lie in one buffer
+        agent.rollout()
+        agent.update()
+    params = list(agent.policy.parameters())
+    tensors = [*params, agent.optimizer.param_groups[0]["step"], agent._lr64, agent._lr]
+    tensors += [t for p in params for t in agent.optimizer.state[p].values()]
+    kinds = {t.dtype for t in tensors}
+    assert kinds >= ({torch.int8, torch.uint8} if optimizer == "adamw8" else {torch.float32})
+    saved = [t.detach().clone() for t in tensors]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        agent._step_apply()
+    results = []
+    for step in (graph.replay, agent._step_apply):
+        with torch.no_grad():
+            for t, v in zip(tensors, saved):
+                t.copy_(v)
+        g = torch.Generator("cuda")
+        g.manual_seed(7)
+        for k in range(4):
+            agent._flat_grad.normal_(generator=g).mul_(0.01)
+            agent._flat_grad[-1] = [0.05, 0.01, 0.001, 0.01][k]   # the schedule's distance: the rate falls, stays, rises
+            step()
+        results.append([t.detach().clone() for t in tensors])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert not any(torch.equal(a, b) for a, b in zip(results[0][:len(params)], saved))
