@@ -365,8 +365,8 @@ class AdamW(torch.optim.Optimizer):
     gradient is left as it is, and so is its count of steps, as torch's.  The group's
     ``step`` counts for all parameters that have had a gradient in each of its steps; one
     that came later, or was left out of one, has a ``step`` in its own state, and a launch
-    for those that share it.  A step that is captured in a CUDA
-    graph follows one that was not, which made the moments."""
+    for those that share it.  A step that is captured in a CUDA graph follows one that was
+    not, which made the moments."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits=32, max_grad_norm=None):
         if bits not in (8, 32):
@@ -383,14 +383,15 @@ class AdamW(torch.optim.Optimizer):
         if not params:
             return []
         states = [self.state[p] for p in params]
-        if not all("exp_avg" in state for state in states):
+        have = lambda name: map(dict.__contains__, states, itertools.repeat(name))
+        if not all(have("exp_avg")):
             _refuse_capture(params[0].device)
             count = torch.zeros((), dtype=torch.int64, device=params[0].device)
-            if any("exp_avg" in state and "step" not in state for state in map(self._known, group["params"])):
-                for state in states:
-                    if "exp_avg" not in state:
-                        state["step"] = count
-            else:
+            apart = any("exp_avg" in state and "step" not in state for state in map(self._known, group["params"]))
+            for p, state in zip(params, states):
+                if "exp_avg" not in state:
+                    state.update(self._zeros(p, group["bits"]), **(dict(step=count) if apart else {}))
+            if not apart:
                 group["step"] = count
         behind = {}
         if len(params) < len(group["params"]):
@@ -402,7 +403,7 @@ class AdamW(torch.optim.Optimizer):
                     if count.data_ptr() in going:
                         _refuse_capture(count.device)
                         state["step"] = behind.setdefault(count.data_ptr(), count.clone())
-        if not any("step" in state for state in states):
+        if not any(have("step")):
             return [(group["step"], params, states, range(len(params)))]
         lists = {}
         for place, (p, state) in enumerate(zip(params, states)):
@@ -414,19 +415,21 @@ class AdamW(torch.optim.Optimizer):
     def _known(self, p):
         return self.state[p] if p in self.state else {}
 
-    def _moments(self, p, state, bits):
-        if "exp_avg" not in state:
-            if bits == 8:
-                m, v = state8_zeros(p, True), state8_zeros(p, False)
-                state.update(exp_avg=m.codes, exp_avg_exponents=m.exponents, exp_avg_sq=v.codes,
-                             exp_avg_sq_exponents=v.exponents)
-            else:
-                state["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-                state["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+    @staticmethod
+    def _zeros(p, bits):
+        """A parameter's moments before any step."""
         if bits == 8:
-            return (State8(state["exp_avg"], state["exp_avg_exponents"]),
-                    State8(state["exp_avg_sq"], state["exp_avg_sq_exponents"]))
-        return state["exp_avg"], state["exp_avg_sq"]
+            m, v = state8_zeros(p, True), state8_zeros(p, False)
+            return dict(exp_avg=m.codes, exp_avg_exponents=m.exponents, exp_avg_sq=v.codes, exp_avg_sq_exponents=v.exponents)
+        zeros = lambda: torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        return dict(exp_avg=zeros(), exp_avg_sq=zeros())
+
+    @staticmethod
+    def _moments(states, bits):
+        if bits == 8:
+            return ([State8(state["exp_avg"], state["exp_avg_exponents"]) for state in states],
+                    [State8(state["exp_avg_sq"], state["exp_avg_sq_exponents"]) for state in states])
+        return [state["exp_avg"] for state in states], [state["exp_avg_sq"] for state in states]
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -437,8 +440,7 @@ class AdamW(torch.optim.Optimizer):
         work, norms = [], {}
         for group in self.param_groups:
             for count, params, states, places in self._counts(group):
-                moments = [self._moments(p, state, group["bits"]) for p, state in zip(params, states)]
-                ms, vs = [m for m, _ in moments], [v for _, v in moments]
+                ms, vs = self._moments(states, group["bits"])
                 eight, device, table, grads = _checked(params, [p.grad for p in params], ms, vs, places)
                 _check_options(count, group["lr"], group["betas"], group["eps"], group["weight_decay"],
                                self.max_grad_norm, device)
