@@ -12,16 +12,17 @@
 // pass computes them again (a third more products than from stored ones), in
 // float32, and rounds da and du once: a and u as bfloat16 would add two roundings to
 // each, and their two arrays cost as much memory as the layer's output twice.  So
-// forward passes keep x only.
+// forward passes keep x only; and, where the TMA does not take rows as they are, the
+// padded copies of x and the weights that it read.
 //
 // One block a multiprocessor goes through tiles of 128 rows: one thread issues the
 // copies, one the products, sixteen warps take finished accumulators out, while the
 // products of the next tile go to the other half of tensor memory.  Measured on a
-// B200, cold: 16384 rows, 1024 x 4096, forward 181 us (1.52 PFLOP/s, tensor pipe 79 %),
-// da and du 247, dx 209, weights 208 (80 %, of which four rounds for 3.5 of tiles); 24576
-// rows, 256 x 512: 21, 42, 18, 18 and 5 us for the sums, where the accumulators' way out
+// B200, cold: 16384 rows, 1024 x 4096, forward 184 us (1.49 PFLOP/s, tensor pipe 79 %),
+// da and du 251, dx 208, weights 210 (80 %, of which four rounds for 3.5 of tiles); 24576
+// rows, 256 x 512: 21.5, 43, 19, 18 and 5 us for the sums, where the accumulators' way out
 // bounds the first two (forward: 10 us of it alone, 10 of products and copies alone, 13
-// together, and 7 for the start and the end; da and du: 18 of 42 for shuffles of the bias
+// together, and 7 for the start and the end; da and du: 18 of 43 for shuffles of the bias
 // sums, dh and stores).
 //
 // float32 (gatedProducts): FMA in pairs; a and u are kept, since they are exact and

@@ -651,10 +651,12 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
         act(x w_gate^T + b_gate) * (x w_up^T + b_up),   act: "silu", "gelu" (of erf) or "sigmoid"
 
     ``x`` [..., D], weights [F, D] (each up to 2^20; D up to 2^16 for bfloat16 on the
-    GPU), biases [F] or none, all of one type; returns [..., F].  Gradients flow to all of them.  Sums are float32, and so are the two
-    projections; the result is rounded once.  bfloat16 on the GPU: for the backward
-    pass only x is kept; gradients of the projections are rounded to 8 bits on
-    their way to those of x and the weights.  A kernel whose waits run out, which takes
+    GPU), biases [F] or none, all of one type; returns [..., F].  Gradients flow to
+    all of them.  Sums are float32, and so are the two projections; the result is
+    rounded once.  bfloat16 on the GPU: the backward pass needs only x and the weights
+    (where D is no multiple of 8, their padded copies are kept beside them); gradients
+    of the projections are rounded to 8 bits on their way to those of x and the
+    weights.  A kernel whose waits run out, which takes
     a fault, leaves NaN, and the next call that finds it so raises."""
     _require(activation in ACTIVATIONS, f"gated_linear: the activation is one of {', '.join(ACTIVATIONS)}")
     _require(x.dim() > 0 and w_gate.dim() == 2 and w_gate.shape == w_up.shape and w_gate.shape[1] == x.shape[-1]
