@@ -353,7 +353,7 @@ def _check_loaded(group):
 def _refuse_capture(device):
     """Where state is made: a replay would make it anew each time."""
     _require(device.type != "cuda" or not torch.cuda.is_current_stream_capturing(),
-             "AdamW: a step that makes moments, or a count of steps, is not captured: step once before the capture")
+             "AdamW: a step that makes moments, or a count of steps, is not captured: step once, or prepare(), before the capture")
 
 
 class AdamW(torch.optim.Optimizer):
@@ -366,7 +366,7 @@ class AdamW(torch.optim.Optimizer):
     ``step`` counts for all parameters that have had a gradient in each of its steps; one
     that came later, or was left out of one, has a ``step`` in its own state, and a launch
     for those that share it.  A step that is captured in a CUDA graph follows one that was
-    not, which made the moments."""
+    not, which made the moments, or ``prepare()``."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits=32, max_grad_norm=None):
         if bits not in (8, 32):
@@ -430,6 +430,12 @@ class AdamW(torch.optim.Optimizer):
             return ([State8(state["exp_avg"], state["exp_avg_exponents"]) for state in states],
                     [State8(state["exp_avg_sq"], state["exp_avg_sq_exponents"]) for state in states])
         return [state["exp_avg"] for state in states], [state["exp_avg_sq"] for state in states]
+
+    def prepare(self):
+        """Makes the moments and counts that the next step with the present gradients
+        needs, so that it can be captured."""
+        for group in self.param_groups:
+            self._counts(group)
 
     @torch.no_grad()
     def step(self, closure=None):

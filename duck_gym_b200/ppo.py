@@ -475,6 +475,8 @@ class PPO:
             p.grad = view
             offset += p.numel()
         self.reducer.enabled = False
+        if self.cfg.optimizer != "adam":   # a parameter that had no gradient so far has one in the buffer
+            self.optimizer.prepare()
         # One part per side of the gradient all-reduce.
         self._parts = [[self._step_loss, self._step_apply]] if self.world == 1 else [[self._step_loss],
                                                                                       [self._step_apply]]
