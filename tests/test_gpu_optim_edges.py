@@ -118,3 +118,30 @@ def test_a_first_step_is_captured_after_prepare():
     assert int(opt.param_groups[0]["step"]) == 3 and params[1] not in opt.state
     # Three steps of lr, whose gradient is always the same: codes of the moments are an eighth of an octave wide.
     assert bool(((params[0] - 0.97).abs() <= 0.03 * 0.13).all())
+
+
+# (clipped, codes differ where the norms' last bits do)
+@pytest.mark.parametrize("bits,clip", [(32, None), (32, 0.5), (8, None)])
+def test_parameters_that_come_late_or_pause(bits, clip):
+    """Several counts of steps in a group: the same as on the CPU, whose own test is against torch."""
+    from test_optim_edges import PATTERN
+
+    def run(device, steps=40):
+        g = torch.Generator()
+        g.manual_seed(4)
+        params = [torch.nn.Parameter(torch.randn(700, generator=g).to(device)) for _ in PATTERN]
+        opt = optim.AdamW([dict(params=params[:3]), dict(params=params[3:])], lr=1e-2, bits=bits, max_grad_norm=clip)
+        for k in range(steps):
+            for p, has in zip(params, PATTERN):
+                grad = torch.randn(700, generator=g).to(device)
+                p.grad = grad if has(k) else None
+            opt.step()
+        counts = [int(opt.state[p].get("step", opt.param_groups[0]["step"])) for p in params[:3]]
+        return [p.detach().cpu() for p in params], [[t.cpu() for t in opt.state[p].values()] for p in params[:3]], counts
+
+    (a, ms, counts), (b, ns, same) = run("cuda"), run("cpu")
+    assert counts == same == [40, 30, 27]
+    for x, y in zip(a, b):   # 40 steps of about lr, whose roots and quotients are off by 2^-20, and the parameter's own roundings
+        assert bool(((x - y).abs() <= 40 * (1e-2 * 2.0 ** -18 + 2.0 ** -23 * (1 + y.abs()))).all())
+    for x, y in zip(ms, ns):
+        assert bits == 32 or all(torch.equal(s, t) for s, t in zip(x, y))
