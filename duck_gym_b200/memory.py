@@ -656,8 +656,8 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     rounded once.  bfloat16 on the GPU: the backward pass needs only x and the weights
     (where D is no multiple of 8, their padded copies are kept beside them); gradients
     of the projections are rounded to 8 bits on their way to those of x and the
-    weights.  A kernel whose waits run out, which takes
-    a fault, leaves NaN, and the next call that finds it so raises."""
+    weights.  A kernel whose waits run out, which takes a fault, leaves NaN, and the
+    next call that finds it so raises."""
     _require(activation in ACTIVATIONS, f"gated_linear: the activation is one of {', '.join(ACTIVATIONS)}")
     _require(x.dim() > 0 and w_gate.dim() == 2 and w_gate.shape == w_up.shape and w_gate.shape[1] == x.shape[-1]
              and w_gate.numel() > 0, "gated_linear: weights are [F, D] for x [..., D]")
