@@ -18,11 +18,11 @@
 // One block a multiprocessor goes through tiles of 128 rows: one thread issues the
 // copies, one the products, sixteen warps take finished accumulators out, while the
 // products of the next tile go to the other half of tensor memory.  Measured on a
-// B200, cold: 16384 rows, 1024 x 4096, forward 184 us (1.49 PFLOP/s, tensor pipe 79 %),
-// da and du 251, dx 208, weights 210 (80 %, of which four rounds for 3.5 of tiles); 24576
-// rows, 256 x 512: 21.5, 43, 19, 18 and 5 us for the sums, where the accumulators' way out
+// B200, cold: 16384 rows, 1024 x 4096, forward 182 us (1.51 PFLOP/s, tensor pipe 79 %),
+// da and du 251, dx 207, weights 205 (80 %, of which four rounds for 3.5 of tiles); 24576
+// rows, 256 x 512: 21, 41, 19, 18 and 5 us for the sums, where the accumulators' way out
 // bounds the first two (forward: 10 us of it alone, 10 of products and copies alone, 13
-// together, and 7 for the start and the end; da and du: 18 of 43 for shuffles of the bias
+// together, and 7 for the start and the end; da and du: 18 of 41 for shuffles of the bias
 // sums, dh and stores).
 //
 // float32 (gatedProducts): FMA in pairs; a and u are kept, since they are exact and
@@ -360,9 +360,9 @@ gatedTiles(const __grid_constant__ TileMaps maps, TileArgs p) {
         const int64_t row = at.row + quarter * 32, rowsLeft = p.rows - row;
         const bool mine = lane < rowsLeft;
         // (given up once, no tile waits again)
-        fine = fine && __all_sync(0xffffffffu, barrierWait(done + buffer, n >> 1 & 1, broken, p.waitLimit));
+        fine = fine && __all_sync(0xffffffffu, barrierAwait(done + buffer, n >> 1 & 1, broken, p.waitLimit));
         if (PASS == Pass::gradients && p.wholeDh && own && fine) {
-          fine = __all_sync(0xffffffffu, barrierWait(bar, parity, broken, p.waitLimit));
+          fine = __all_sync(0xffffffffu, barrierAwait(bar, parity, broken, p.waitLimit));
           if (fine) asked = false, parity ^= 1;
         }
         tensorFenceAfter();

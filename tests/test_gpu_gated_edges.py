@@ -217,3 +217,29 @@ assert torch.equal(h, memory.gated_linear(w, w, w)) and bool((h == 256).all()), 
 """
     run = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr
+
+
+@pytest.mark.parametrize("rows,D,F", [(16, 256, 512), (6000, 1024, 264)])
+def test_linear_waits_that_may_run_out(rows, D, F):
+    """With limits that are too short, a call's results are right, or the next call says that they are not."""
+    from duck_gym_b200.cuda_batch import library
+
+    lib, g = library(), torch.Generator("cuda")
+    g.manual_seed(rows)
+    x, wg, wu = (torch.randn(s, generator=g, device="cuda").bfloat16() / 4 for s in ((rows, D), (F, D), (F, D)))
+    with torch.no_grad():
+        want = memory.gated_linear(x, wg, wu)
+        torch.cuda.synchronize()
+        try:
+            for k in range(40):
+                assert lib.duck_wait_limit([1, 300, 1000, 3000][k % 4]) == 0
+                h = memory.gated_linear(x, wg, wu)
+                torch.cuda.synchronize()
+                said = lib.duck_wait_status() != 0
+                same = (h == want) | h.isnan()
+                assert bool(same.all()) and said == bool(h.isnan().any())
+        finally:
+            lib.duck_wait_limit(2 * 10**9)
+            torch.cuda.synchronize()
+            lib.duck_wait_status()
+        assert torch.equal(memory.gated_linear(x, wg, wu), want)
